@@ -1,4 +1,5 @@
-"""Builds the sm_100a backend in place: cpp_inference_train_engine_b200/libmm_cuda.so.
+"""Builds the sm_100a backend in place: cpp_inference_train_engine_b200/libmm_cuda.so, from its
+two translation units (the engine and the latent-cache operators).
 
     python -m cpp_inference_train_engine_b200.build
 
@@ -13,7 +14,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SRC = os.path.join(HERE, "csrc", "mm_cuda.cu")
+SRC = [os.path.join(HERE, "csrc", f) for f in ("mm_cuda.cu", "latent.cu")]
 OUT = os.path.join(HERE, "libmm_cuda.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -37,7 +38,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
         return OUT
     cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr",
            "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", "-Xptxas", "-warn-spills",
-           "-I", os.path.join(ROOT, "include"), SRC, "-o", OUT + ".tmp", "-ldl", "-lpthread"]
+           "-t", "2", "-I", os.path.join(ROOT, "include"), *SRC, "-o", OUT + ".tmp", "-ldl", "-lpthread"]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)

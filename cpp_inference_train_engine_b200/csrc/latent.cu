@@ -1,0 +1,302 @@
+// C entries of the shared-prompt decode operators (include/mm_latent.h): argument checks,
+// variant selection and launches. Everything is enqueued on the caller's stream; no entry
+// allocates, waits or throws.
+#include <algorithm>
+#include <atomic>
+#include <cstdio>
+#include <cstring>
+#include <exception>
+#include <string>
+#include <type_traits>
+
+#include "draft_verify.cuh"
+#include "latent_cache.cuh"
+#include "shared_prefix.cuh"
+
+#include "../../include/mm_latent.h"
+
+namespace {
+
+thread_local std::string g_error;
+
+struct Refusal {
+    int code;
+    const char* what;
+};
+
+[[noreturn]] void refuse(int code, const char* what) { throw Refusal{code, what}; }
+void require(bool ok, const char* what) {
+    if (!ok) refuse(MM_INVALID_ARGUMENT, what);
+}
+void check(cudaError_t e, const char* what) {
+    if (e == cudaSuccess) return;
+    g_error = std::string(what) + ": " + cudaGetErrorString(e);
+    throw Refusal{e == cudaErrorMemoryAllocation ? MM_OUT_OF_MEMORY : MM_GPU_ERROR, nullptr};
+}
+
+// Runs f; failures become 1 + ErrorCode with a message.
+template <class F> int guarded(F&& f) {
+    try {
+        f();
+        return MM_OK;
+    } catch (const Refusal& r) {
+        try {
+            if (r.what) g_error = r.what;
+        } catch (...) {
+        }
+        return r.code;
+    } catch (...) {
+        return MM_OUT_OF_MEMORY;
+    }
+}
+
+// Launch with programmatic stream serialization (every kernel enters through MM_PDL_ENTRY or
+// waits itself before it touches memory). The error is taken from the launch itself.
+template <typename... KArgs, typename... Args>
+void launch(cudaStream_t s, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    check(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), "kernel launch");
+}
+
+// cudaFuncSetAttribute(MaxDynamicSharedMemorySize) for a kernel, once per device.
+template <auto Kernel> void set_dynamic_smem(int bytes) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    check(cudaGetDevice(&dev), "cudaGetDevice");
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load() & bit)) return;
+    check(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory attribute");
+    done.fetch_or(bit);
+}
+
+void check_cache(const mm_latent_cache* c) {
+    require(c->rows >= 0 && c->positions >= 0, "latent cache: negative size");
+    require(c->kv >= 1 && c->kv <= 1024 && c->rope_dim >= 0 && c->rope_dim <= 256,
+            "latent cache: kv must be in [1, 1024] and rope_dim in [0, 256]");
+    require(c->kind == MM_F16 || c->kind == MM_BF16 || c->kind == MM_E4M3, "latent cache: unknown kind");
+    const bool empty = c->rows == 0 || c->positions == 0;
+    require(c->latent || empty, "latent cache: null storage");
+    if (c->kind == MM_E4M3) {
+        require(c->rope_kind == MM_F16 || c->rope_kind == MM_BF16, "latent cache: rope must be fp16 or bf16");
+        require(empty || (c->scale && (c->rope || c->rope_dim == 0)), "latent cache: null storage");
+    }
+}
+
+mm::lat::CacheView view(const mm_latent_cache* c) {
+    mm::lat::CacheView v{};
+    if (!c) return v;
+    v.latent = static_cast<const uint8_t*>(c->latent);
+    v.rope = static_cast<const uint8_t*>(c->rope);
+    v.scale = c->scale;
+    v.row_stride = c->row_stride;
+    v.pos_stride = c->pos_stride;
+    v.rope_row_stride = c->rope_row_stride;
+    v.rope_pos_stride = c->rope_pos_stride;
+    v.scale_row_stride = c->scale_row_stride;
+    v.rows = c->rows;
+    v.positions = c->positions;
+    return v;
+}
+
+constexpr long long kMaxBlocks = 2147483647LL;
+
+unsigned blocks(long long n, int per) {
+    const long long b = (n + per - 1) / per;
+    if (b > kMaxBlocks) refuse(MM_UNSUPPORTED, "too many rows for one launch");
+    return static_cast<unsigned>(b);
+}
+
+// Calls f(std::type_identity-like tag) for a 16-bit or 32-bit element type.
+template <typename T> struct Tag {
+    using type = T;
+};
+template <class F> void with_type(int dtype, F&& f) {
+    if (dtype == MM_F16) f(Tag<__half>{});
+    else if (dtype == MM_BF16) f(Tag<__nv_bfloat16>{});
+    else if (dtype == MM_F32) f(Tag<float>{});
+    else refuse(MM_INVALID_ARGUMENT, "unsupported element type");
+}
+template <class F> void with_half(int dtype, F&& f) {
+    if (dtype == MM_F16) f(Tag<__half>{});
+    else if (dtype == MM_BF16) f(Tag<__nv_bfloat16>{});
+    else refuse(MM_INVALID_ARGUMENT, "unsupported element type");
+}
+
+mm::spa::Problem problem(const mm_shared_prefix_desc* d) {
+    require(d != nullptr, "null description");
+    require(d->rows >= 0 && d->tokens >= 1 && d->heads >= 1 && d->groups >= 0, "shared-prefix attention: invalid sizes");
+    require(d->dtype == MM_F16 || d->dtype == MM_BF16, "shared-prefix attention: q must be fp16 or bf16");
+    require(d->prefix || d->suffix, "shared-prefix attention: a prefix or a suffix cache is needed");
+    require(static_cast<long long>(d->rows) * d->tokens <= kMaxBlocks / d->heads,
+            "shared-prefix attention: too many query rows");
+    for (const mm_latent_cache* c : {d->prefix, d->suffix})
+        if (c) {
+            check_cache(c);
+            require(c->kind == d->dtype || (c->kind == MM_E4M3 && c->rope_kind == d->dtype),
+                    "shared-prefix attention: the cache's type must be q's (an e4m3 cache's rope type)");
+        }
+    if (d->prefix && d->suffix)
+        require(d->prefix->kv == d->suffix->kv && d->prefix->rope_dim == d->suffix->rope_dim,
+                "shared-prefix attention: prefix and suffix widths differ");
+    require(d->groups == 0 || (d->prefix && d->prefix->rows >= d->groups), "shared-prefix attention: a prefix row per group");
+    require(!d->suffix || d->suffix->rows >= d->rows, "shared-prefix attention: a suffix row per row");
+    require(d->max_group >= 0 && d->max_prefix >= 0 && d->max_suffix >= 0 &&
+                d->max_prefix <= (d->prefix ? d->prefix->positions : 0) &&
+                d->max_suffix <= (d->suffix ? d->suffix->positions : 0),
+            "shared-prefix attention: max_prefix / max_suffix exceed the cache's positions");
+    if (d->rows > 0) {
+        require(d->q && d->out, "shared-prefix attention: null q or out");
+        require(d->groups == 0 || (d->group_start && d->prefix_len), "shared-prefix attention: null group_start or prefix_len");
+        require(d->max_suffix == 0 || d->suffix_len, "shared-prefix attention: null suffix_len");
+    }
+    const mm_latent_cache* any = d->prefix ? d->prefix : d->suffix;
+    mm::spa::Problem p{};
+    p.q = d->q;
+    p.q_row = d->q_row_stride;
+    p.q_tok = d->q_token_stride;
+    p.q_head = d->q_head_stride;
+    p.B = d->rows;
+    p.T = d->tokens;
+    p.H = d->heads;
+    p.prefix = view(d->prefix);
+    p.suffix = view(d->suffix);
+    p.group_start = d->group_start;
+    p.prefix_len = d->prefix_len;
+    p.suffix_len = d->suffix_len;
+    p.G = d->max_prefix > 0 && d->max_group > 0 ? d->groups : 0;
+    p.max_group = std::min(d->max_group, d->rows);
+    p.max_prefix = d->max_prefix;
+    p.max_suffix = d->max_suffix;
+    p.kv = any->kv;
+    p.rd = any->rope_dim;
+    p.scale = d->scale;
+    p.out = d->out;
+    p.lse = d->lse;
+    return p;
+}
+
+template <typename T, bool Q8P, bool Q8S> void launch_any_width(const mm::spa::Problem& p, cudaStream_t s) {
+    using namespace mm::spa;
+    const int smem = kAnyWarps * (2 * p.kv + p.rd) * 4;  // at most 36 KB
+    launch(s, any_width_kernel<T, Q8P, Q8S>, dim3(blocks(static_cast<long long>(p.B) * p.T * p.H, kAnyWarps)),
+           dim3(32 * kAnyWarps), smem, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mm_latent_last_error(char* buf, size_t cap) {
+    if (buf && cap > 0) {
+        const size_t n = std::min(cap - 1, g_error.size());
+        std::memcpy(buf, g_error.data(), n);
+        buf[n] = 0;
+    }
+    return g_error.size();
+}
+
+int mm_latent_cache_write(const mm_latent_cache* cache, const void* latent, int64_t latent_stride, const void* rope,
+                          int64_t rope_stride, int dtype, const int64_t* slots, int64_t n, void* stream) {
+    return guarded([&] {
+        require(cache != nullptr && n >= 0, "cache write: null cache or negative count");
+        check_cache(cache);
+        require(cache->kind == MM_E4M3, "cache write: the cache must be an e4m3 one");
+        if (n == 0 || cache->rows == 0 || cache->positions == 0) return;
+        require(latent && slots && (rope || cache->rope_dim == 0), "cache write: null input");
+        mm::lat::CacheOut c{static_cast<uint8_t*>(cache->latent), static_cast<uint8_t*>(cache->rope), cache->scale,
+                            cache->row_stride, cache->pos_stride, cache->rope_row_stride, cache->rope_pos_stride,
+                            cache->scale_row_stride, cache->rows, cache->positions};
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        with_type(dtype, [&](auto in) {
+            with_half(cache->rope_kind, [&](auto half) {
+                using T = typename decltype(in)::type;
+                using T16 = typename decltype(half)::type;
+                launch(s, mm::lat::latent_write_kernel<T, T16>, dim3(blocks(n, 8)), dim3(256), 0, c,
+                       static_cast<const T*>(latent), static_cast<long long>(latent_stride), static_cast<const T*>(rope),
+                       static_cast<long long>(rope_stride), reinterpret_cast<const long long*>(slots),
+                       static_cast<long long>(n), cache->kv, cache->rope_dim);
+            });
+        });
+    });
+}
+
+int mm_latent_cache_read(const mm_latent_cache* cache, const int64_t* slots, int64_t n, void* out, int64_t out_stride,
+                         int out_dtype, void* stream) {
+    return guarded([&] {
+        require(cache != nullptr && n >= 0, "cache read: null cache or negative count");
+        check_cache(cache);
+        require(cache->kind == MM_E4M3, "cache read: the cache must be an e4m3 one");
+        if (n == 0) return;
+        require(slots && out, "cache read: null argument");
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        with_type(out_dtype, [&](auto o) {
+            with_half(cache->rope_kind, [&](auto half) {
+                using TO = typename decltype(o)::type;
+                using T16 = typename decltype(half)::type;
+                launch(s, mm::lat::latent_read_kernel<T16, TO>, dim3(blocks(n, 8)), dim3(256), 0, view(cache),
+                       reinterpret_cast<const long long*>(slots), static_cast<long long>(n), static_cast<TO*>(out),
+                       static_cast<long long>(out_stride), cache->kv, cache->rope_dim);
+            });
+        });
+    });
+}
+
+int64_t mm_shared_prefix_attention_workspace(const mm_shared_prefix_desc* desc) {
+    int64_t bytes = 0;
+    const int rc = guarded([&] { problem(desc); });
+    return rc ? -static_cast<int64_t>(rc) : bytes;
+}
+
+int mm_shared_prefix_attention(const mm_shared_prefix_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        const mm::spa::Problem p = problem(desc);
+        if (p.B == 0) return;
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        const bool q8p = desc->prefix && desc->prefix->kind == MM_E4M3;
+        const bool q8s = desc->suffix && desc->suffix->kind == MM_E4M3;
+        with_half(desc->dtype, [&](auto half) {
+            using T = typename decltype(half)::type;
+            if (q8p && q8s) launch_any_width<T, true, true>(p, s);
+            else if (q8p) launch_any_width<T, true, false>(p, s);
+            else if (q8s) launch_any_width<T, false, true>(p, s);
+            else launch_any_width<T, false, false>(p, s);
+        });
+    });
+}
+
+int mm_verify_drafts(const void* target_probs, const void* draft_probs, int dtype, const int32_t* draft_tokens,
+                     const int32_t* draft_len, const float* u_accept, const float* u_sample, int rows, int drafts,
+                     int vocab, int32_t* out_tokens, int32_t* accepted, void* stream) {
+    return guarded([&] {
+        require(rows >= 0 && drafts >= 0 && vocab >= 1, "draft verification: invalid sizes");
+        if (vocab > mm::ver::kMaxVocab) refuse(MM_UNSUPPORTED, "draft verification: vocabulary over 262,144");
+        if (rows == 0) return;
+        require(target_probs && draft_len && u_sample && out_tokens && accepted &&
+                    (drafts == 0 || (draft_tokens && u_accept)),
+                "draft verification: null argument");
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        with_type(dtype, [&](auto t) {
+            using T = typename decltype(t)::type;
+            const T* p = static_cast<const T*>(target_probs);
+            const T* q = drafts > 0 ? static_cast<const T*>(draft_probs) : nullptr;
+            auto fits = [&](const void* x) { return reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0; };
+            if (vocab % 4 == 0 && fits(p) && fits(q))
+                launch(s, mm::ver::verify_drafts_kernel<T, true>, dim3(rows), dim3(mm::ver::kThreads), 0, p, q, draft_tokens,
+                       draft_len, u_accept, u_sample, drafts, vocab, out_tokens, accepted);
+            else
+                launch(s, mm::ver::verify_drafts_kernel<T, false>, dim3(rows), dim3(mm::ver::kThreads), 0, p, q, draft_tokens,
+                       draft_len, u_accept, u_sample, drafts, vocab, out_tokens, accepted);
+        });
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,78 @@
+"""The latent operators' C entries refuse what they can see on the host, without a GPU."""
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import cpp_inference_train_engine_b200 as E
+from cpp_inference_train_engine_b200 import latent
+
+
+def message():
+    buf = ctypes.create_string_buffer(256)
+    latent._lib().mm_latent_last_error(buf, 256)
+    return buf.value.decode()
+
+
+def cache(kind=latent.MM_F16, rows=2, positions=16, kv=128, rope=16, rope_kind=latent.MM_F16):
+    p = 1 << 20  # never read: these calls are refused first
+    return latent._Cache(p, p, p, positions * (kv + rope), kv + rope, positions * rope, rope, positions, rows, positions,
+                         kv, rope, kind, rope_kind)
+
+
+def desc(**over):
+    pre, suf = over.pop("prefix", cache(rows=1)), over.pop("suffix", cache())
+    d = latent._Desc()
+    d.q = d.out = d.group_start = d.prefix_len = d.suffix_len = 1 << 20
+    d.q_row_stride = d.q_token_stride = 8 * 144
+    d.q_head_stride, d.dtype, d.rows, d.tokens, d.heads, d.groups = 144, latent.MM_F16, 2, 1, 8, 1
+    d.max_group, d.max_prefix, d.max_suffix, d.scale = 2, 16, 16, 0.1
+    if pre is not None:
+        d.prefix = ctypes.pointer(pre)
+    if suf is not None:
+        d.suffix = ctypes.pointer(suf)
+    for k, v in over.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("over, what", [
+    (dict(rows=-1), "sizes"), (dict(tokens=0), "sizes"), (dict(heads=0), "sizes"), (dict(groups=-1), "sizes"),
+    (dict(dtype=latent.MM_F32), "fp16 or bf16"), (dict(prefix=None, suffix=None), "is needed"),
+    (dict(prefix=cache(kind=latent.MM_BF16)), "type"), (dict(prefix=cache(latent.MM_E4M3, rope_kind=latent.MM_BF16)), "type"),
+    (dict(prefix=cache(kv=64)), "widths"), (dict(groups=3), "per group"), (dict(suffix=cache(rows=1)), "per row"),
+    (dict(max_prefix=17), "exceed"), (dict(max_suffix=17), "exceed"), (dict(max_prefix=-1), "exceed"),
+    (dict(q=None), "null q"), (dict(out=None), "null q"), (dict(group_start=None), "group_start"),
+    (dict(suffix_len=None), "suffix_len"), (dict(prefix=cache(kv=2000)), "kv must be"), (dict(suffix=cache(kind=7)), "kind"),
+    (dict(tokens=2 ** 20, heads=2 ** 12), "too many"),
+])
+def test_attention_refusals(over, what):
+    d = desc(**over)
+    assert latent._lib().mm_shared_prefix_attention_workspace(ctypes.byref(d)) == -1
+    assert what in message()
+    assert latent._lib().mm_shared_prefix_attention(ctypes.byref(d), None, 0, None) == 1
+    assert what in message()
+
+
+def test_null_arguments_are_refused():
+    L = latent._lib()
+    assert L.mm_shared_prefix_attention(None, None, 0, None) == 1
+    assert L.mm_latent_cache_write(None, None, 0, None, 0, 0, None, 1, None) == 1
+    assert L.mm_latent_cache_read(None, None, 1, None, 0, 0, None) == 1
+    c = cache(latent.MM_E4M3)
+    assert L.mm_latent_cache_write(ctypes.byref(c), None, 0, None, 0, 0, None, 1, None) == 1 and "null" in message()
+    assert L.mm_latent_cache_write(ctypes.byref(c), None, 0, None, 0, 0, None, -1, None) == 1
+    assert L.mm_latent_cache_write(ctypes.byref(c), None, 0, None, 0, 0, None, 0, None) == 0  # nothing to do
+    f16 = cache()
+    assert L.mm_latent_cache_read(ctypes.byref(f16), 1 << 20, 1, 1 << 20, 144, 1, None) == 1 and "e4m3" in message()
+    assert L.mm_verify_drafts(None, None, 0, None, None, None, None, 1, 1, 8, None, None, None) == 1
+    assert L.mm_verify_drafts(None, None, 0, None, None, None, None, 1, 1, 0, None, None, None) == 1
+    assert L.mm_verify_drafts(None, None, 0, None, None, None, None, 1, 1, 2 ** 19, None, None, None) == 3
+    assert L.mm_verify_drafts(None, None, 0, None, None, None, None, 0, 1, 8, None, None, None) == 0
+
+
+def test_cpu_tensors_are_refused():
+    q = torch.zeros(1, 1, 8, 144, dtype=torch.float16)
+    with pytest.raises(E.EngineError, match="CUDA tensor"):
+        latent.shared_prefix_attention(q, None, None, None, None, None, 0.1, kv_rank=128)
