@@ -12,6 +12,7 @@
 #include "draft_verify.cuh"
 #include "latent_cache.cuh"
 #include "shared_prefix.cuh"
+#include "shared_prefix_tc.cuh"
 
 #include "../../include/mm_latent.h"
 
@@ -191,6 +192,121 @@ template <typename T, bool Q8P, bool Q8S> void launch_any_width(const mm::spa::P
            dim3(32 * kAnyWarps), smem, p);
 }
 
+int sm_count() {
+    static std::atomic<int> count{0};
+    int n = count.load();
+    if (!n) {
+        int dev = 0;
+        check(cudaGetDevice(&dev), "cudaGetDevice");
+        check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev), "multiprocessor count");
+        count.store(n);
+    }
+    return n;
+}
+
+// ------------------------------------------------------------------ tensor-core plan
+// The tensor-core form covers the two latent widths of the framework's models when every row
+// can be read in 16-byte pieces.
+bool aligned_cache(const mm_latent_cache* c) {
+    auto ok = [](const void* p, long long a, long long b, int size) {
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a * size % 16 == 0 && b * size % 16 == 0;
+    };
+    if (c->kind == MM_E4M3)
+        return ok(c->latent, c->row_stride, c->pos_stride, 1) && ok(c->rope, c->rope_row_stride, c->rope_pos_stride, 2);
+    return ok(c->latent, c->row_stride, c->pos_stride, 2);
+}
+bool tensor_core_form(const mm_shared_prefix_desc* d, const mm::spa::Problem& p) {
+    if (!((p.kv == 128 && p.rd == 16) || (p.kv == 512 && p.rd == 32))) return false;
+    if (reinterpret_cast<uintptr_t>(p.q) % 16 || p.q_row % 8 || p.q_tok % 8 || p.q_head % 8) return false;
+    return (p.G == 0 || aligned_cache(d->prefix)) && (p.max_suffix == 0 || aligned_cache(d->suffix));
+}
+
+struct Plan {
+    int pre_n = 0, pre_splits = 0, pre_kps = 128;  // queries per block (0: no prefix launch), ranges, keys per range
+    int suf_n = 0, suf_splits = 0, suf_kps = 128;
+    long long pre_blocks = 0, suf_blocks = 0;      // upper bounds of the query blocks
+    bool merge = false;                            // the suffix launch writes the results
+    long long rows = 0;                            // query rows
+    long long pre_part = 0, suf_part = 0;          // partial query rows held by the workspace
+    long long bytes(int kv) const { return (pre_part + suf_part) * (kv + 2) * 4; }
+};
+
+// Key ranges per query block: the waves of (block, range) items over the SMs times an item's
+// tiles, plus what an item costs beside its tiles.
+void pick_splits(long long blocks, int keys, int most, int& splits, int& kps) {
+    const int tiles = (keys + 127) / 128, sms = sm_count();
+    double best = 0;
+    splits = 0;
+    for (int s = 1; s <= std::min(tiles, most); ++s) {
+        const int per = (tiles + s - 1) / s, n = (tiles + per - 1) / per;
+        if (n != s) continue;
+        const double cost = static_cast<double>((blocks * n + sms - 1) / sms) * (per + 2.0) + (n > 1 ? 1.0 + 0.05 * n : 0.0);
+        if (!splits || cost < best) {
+            best = cost;
+            splits = n;
+            kps = per * 128;
+        }
+    }
+}
+
+Plan plan(const mm::spa::Problem& p) {
+    Plan r;
+    const long long th = static_cast<long long>(p.T) * p.H;
+    r.rows = th * p.B;
+    if (p.G > 0) {
+        r.pre_n = p.max_group * th <= 16 ? 16 : 64;
+        r.pre_blocks = std::min((r.rows + r.pre_n - 1) / r.pre_n + p.G, p.G * ((p.max_group * th + r.pre_n - 1) / r.pre_n));
+        pick_splits(r.pre_blocks, p.max_prefix, 64, r.pre_splits, r.pre_kps);
+        r.pre_part = r.rows * r.pre_splits;
+    }
+    if (p.max_suffix > 0) {
+        r.suf_n = th <= 16 ? 16 : 64;
+        r.suf_blocks = p.B * ((th + r.suf_n - 1) / r.suf_n);
+        pick_splits(r.suf_blocks, p.max_suffix, 16, r.suf_splits, r.suf_kps);
+        r.merge = r.suf_splits == 1;
+        if (!r.merge) r.suf_part = r.rows * r.suf_splits;
+    }
+    if (r.pre_blocks * std::max(1, r.pre_splits) > kMaxBlocks || r.suf_blocks * std::max(1, r.suf_splits) > kMaxBlocks)
+        refuse(MM_UNSUPPORTED, "shared-prefix attention: too many query rows");
+    return r;
+}
+
+template <int KV, int R, int N, typename T, bool Q8>
+void launch_tc(const mm::spa::TcArgs& a, long long items, cudaStream_t s) {
+    using namespace mm::spa;
+    set_dynamic_smem<shared_prefix_tc_kernel<KV, R, N, T, Q8>>(TcCfg<KV, R, N, Q8>::kSmem);
+    launch(s, shared_prefix_tc_kernel<KV, R, N, T, Q8>, dim3(static_cast<unsigned>(std::min<long long>(items, sm_count()))),
+           dim3(kTcThreads), TcCfg<KV, R, N, Q8>::kSmem, a);
+}
+template <int KV, int R, typename T>
+void launch_tc_n(const mm::spa::TcArgs& a, int n, bool q8, long long items, cudaStream_t s) {
+    if (n == 16) q8 ? launch_tc<KV, R, 16, T, true>(a, items, s) : launch_tc<KV, R, 16, T, false>(a, items, s);
+    else q8 ? launch_tc<KV, R, 64, T, true>(a, items, s) : launch_tc<KV, R, 64, T, false>(a, items, s);
+}
+
+template <int KV, int R, typename T>
+void run_tc(const mm::spa::Problem& p, const Plan& r, bool q8p, bool q8s, void* workspace, cudaStream_t s) {
+    using namespace mm::spa;
+    float* w = static_cast<float*>(workspace);
+    float* pre_o = w;
+    float* suf_o = pre_o + r.pre_part * KV;
+    float2* pre_ml = reinterpret_cast<float2*>(suf_o + r.suf_part * KV);
+    float2* suf_ml = pre_ml + r.pre_part;
+    if (r.pre_n) {
+        const TcArgs a{p, 0, r.pre_splits, r.pre_kps, pre_o, pre_ml, 0, 0, 128};
+        launch_tc_n<KV, R, T>(a, r.pre_n, q8p, r.pre_blocks * r.pre_splits, s);
+    }
+    if (r.suf_n) {
+        const TcArgs a{p, 1, r.suf_splits, r.suf_kps, r.merge ? pre_o : suf_o, r.merge ? pre_ml : suf_ml, r.merge ? 1 : 0,
+                       r.pre_splits, r.pre_kps};
+        launch_tc_n<KV, R, T>(a, r.suf_n, q8s, r.suf_blocks * r.suf_splits, s);
+    }
+    if (!r.merge)
+        launch(s, shared_prefix_join_kernel<KV, T>, dim3(blocks(r.rows, 8)), dim3(256), 0, p, static_cast<const float*>(pre_o),
+               static_cast<const float2*>(pre_ml), r.pre_kps, static_cast<const float*>(suf_o),
+               static_cast<const float2*>(suf_ml), r.suf_kps);
+}
+
 }  // namespace
 
 extern "C" {
@@ -252,7 +368,10 @@ int mm_latent_cache_read(const mm_latent_cache* cache, const int64_t* slots, int
 
 int64_t mm_shared_prefix_attention_workspace(const mm_shared_prefix_desc* desc) {
     int64_t bytes = 0;
-    const int rc = guarded([&] { problem(desc); });
+    const int rc = guarded([&] {
+        const mm::spa::Problem p = problem(desc);
+        if (p.B > 0 && tensor_core_form(desc, p)) bytes = plan(p).bytes(p.kv);
+    });
     return rc ? -static_cast<int64_t>(rc) : bytes;
 }
 
@@ -263,6 +382,19 @@ int mm_shared_prefix_attention(const mm_shared_prefix_desc* desc, void* workspac
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         const bool q8p = desc->prefix && desc->prefix->kind == MM_E4M3;
         const bool q8s = desc->suffix && desc->suffix->kind == MM_E4M3;
+        if (tensor_core_form(desc, p)) {
+            const Plan r = plan(p);
+            const long long need = r.bytes(p.kv);
+            require(need == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
+                                  workspace_bytes >= static_cast<size_t>(need)),
+                    "shared-prefix attention: workspace too small or not 16-byte aligned");
+            with_half(desc->dtype, [&](auto half) {
+                using T = typename decltype(half)::type;
+                if (p.kv == 128) run_tc<128, 16, T>(p, r, q8p, q8s, workspace, s);
+                else run_tc<512, 32, T>(p, r, q8p, q8s, workspace, s);
+            });
+            return;
+        }
         with_half(desc->dtype, [&](auto half) {
             using T = typename decltype(half)::type;
             if (q8p && q8s) launch_any_width<T, true, true>(p, s);

@@ -1,0 +1,887 @@
+// Shared-prefix latent attention on the 5th-generation tensor cores, for [128 latent | 16 rope]
+// and [512 latent | 32 rope] caches.
+//
+// Keys are the M side of both products, queries the N side:
+//   S^T [128 keys x N queries] = K [128 x (kv + rope)] Q^T,     O^T [kv x N] += V^T [kv x 128] P^T,
+// V being K's first kv columns, so one shared-memory tile of the cache is read by both products
+// (K-major for S^T, MN-major for O^T) and a cache row crosses HBM once per block of N queries.
+// A decode step has few queries per key (8 or 16 heads of a row; a group's rows x heads over its
+// prefix): with queries on M, a 128-row tile would be mostly empty and the [M x kv] fp32
+// accumulator would fill the whole tensor memory at kv = 512; with keys on M every tile is full
+// and O^T takes kv / 128 x N columns (256 of 512 at N = 64).
+//
+// A work item is (block of N query rows, key range): one group's query rows over a range of its
+// prefix, or one row's queries over a range of its suffix. CTAs are persistent (one per SM) and
+// walk the items; barrier phases run on across items. 12 warps (three warpgroups, whose register
+// shares 232 + 168 + 104 add up to the launch's 3 x 168):
+//   warps 4-7  producers: the item's queries, then per 128-key tile the rope columns and kv / 128
+//              pairs of 64-column boxes into rings of swizzled boxes. 16-bit caches go by 16-byte
+//              cp.async; e4m3 codes are loaded four pairs ahead into registers and stored as 16-bit
+//              values (exact). Rows past the range are zero-filled, so whatever the cache holds
+//              there never reaches a product.
+//   warp 8     one thread issues tcgen05.mma (warps 9-11 only fill its warpgroup).
+//   warps 0-3  softmax: thread = key (tensor-memory lane), N query columns. The running maximum
+//              is lazy: a tile whose scores stay below the reference + 8 (base 2) uses the
+//              reference as it is (probabilities up to 2^8 fit fp16, sums are fp32), decided by one
+//              4-warp vote; otherwise the maxima are taken (warp reductions and an exchange) and
+//              O^T and the sums are rescaled. A key's scale (e4m3) multiplies its scores and, for
+//              the second product, its probabilities.
+// Every mbarrier wait is bounded; after a wait that runs out the CTA goes on without waiting (every
+// loop is bounded, every access in bounds) and its results are NaN.
+#pragma once
+#include "shared_prefix.cuh"
+
+namespace mm {
+namespace spa {
+
+// How a launch covers its items and where its partial results go.
+struct TcArgs {
+    Problem p;
+    int suffix;        // 0: prefix items, 1: suffix items
+    int splits, kps;   // key ranges per query block and keys per range (a multiple of 128)
+    // partials of this launch (fp32 O [splits][query rows][kv] unnormalised, (max, sum) in base 2),
+    // or, with merge (suffix, splits = 1): the prefix launch's, which are read, and the final
+    // result is written
+    float* part_o;
+    float2* part_ml;
+    int merge, prefix_splits, prefix_kps;
+};
+
+constexpr int kTcThreads = 384;      // 12 warps: 168 registers each at launch
+constexpr int kTcMaxPlan = 512;   // groups whose item prefix sums fit the shared plan
+constexpr float kNoMax = -1e37f;  // running maximum before any key (finite: its exp2 is 0, never NaN)
+
+template <int KV, int R, int N, bool Q8> struct TcCfg {
+    static constexpr int NP = KV / 128;                    // 128-column pairs of boxes
+    static constexpr int kBox = 128 * 128;                 // 128 keys x 64 columns of 16 bits
+    static constexpr int kPair = 2 * kBox;
+    static constexpr int kRope = 128 * R * 2;
+    static constexpr int kQBox = N * 128;
+    static constexpr int kQ = 2 * NP * kQBox + N * R * 2;  // N query rows
+    static constexpr int kQA = (kQ + 1023) / 1024 * 1024;
+    // P^T: N = 64: one MN-major box [128 keys x 64 queries]; N = 16: two K-major boxes of 64 keys
+    static constexpr int kP = N == 64 ? 128 * 128 : 2 * 16 * 128;
+    // rings: queries, pairs, rope boxes, P buffers, O accumulators (what 227 KB and 512 tensor
+    // memory columns hold)
+    static constexpr int QB = KV == 512 && N == 64 ? 1 : 2;
+    static constexpr int PS = KV == 512 ? (N == 64 ? 4 : 5) : (N == 64 ? 4 : 5);
+    static constexpr int RS = KV == 512 ? (N == 64 ? 1 : 2) : PS;
+    static constexpr int PB = KV == 512 && N == 64 ? 1 : 2;
+    static constexpr int OB = KV == 512 && N == 64 ? 1 : 2;
+    // S of the next tile is issued before this tile's O when the rings hold two tiles
+    static constexpr bool kAhead = PS >= 2 * NP && RS >= 2;
+    // tensor memory columns: two S buffers (e4m3: two more for the rope columns' share, which the
+    // key's scale does not multiply), then the O accumulators
+    static constexpr int kColS = 0, kColR = 2 * N, kColO = Q8 ? 4 * N : 2 * N;
+    static constexpr int kCols = kColO + OB * NP * N;
+    static constexpr int kTmem = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+    static constexpr int kRopeA = (kRope + 1023) / 1024 * 1024;
+    static constexpr int oPair = 0;
+    static constexpr int oQ = oPair + PS * kPair;
+    static constexpr int oRope = oQ + QB * kQA;
+    static constexpr int oP = oRope + RS * kRopeA;
+    static constexpr int oF = oP + PB * kP;  // floats: m[N], corr[N], red[4][N], lim[N]
+    static constexpr int oPlan = oF + 7 * N * 4;
+    static constexpr int oBar = oPlan + (kTcMaxPlan + 1) * 4 + 4;
+    static constexpr int kBars = 2 * QB + 2 * PS + 2 * RS + 4 + 2 * PB + 2 * OB;
+    static constexpr int kSmem = oBar + kBars * 8 + 16 + 1024;  // + alignment of the base
+    static_assert(kSmem <= 227 * 1024 && kCols <= 512, "shared and tensor memory");
+};
+
+// Swizzled byte offset of 16-byte chunk c of row r in a box of 128-, 64- or 32-byte rows.
+__device__ __forceinline__ uint32_t sw128(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+template <int R> __device__ __forceinline__ uint32_t sw_rope(int r, int c) {
+    return R == 32 ? r * 64 + ((c ^ ((r >> 1) & 3)) << 4) : r * 32 + ((c ^ ((r >> 2) & 1)) << 4);
+}
+// Descriptor of a K-major rope box: 64-byte (R = 32) or 32-byte (R = 16) swizzle.
+template <int R> __device__ __forceinline__ uint64_t rope_desc(uint32_t addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr >> 4) & 0x3FFF);
+    d |= static_cast<uint64_t>(1) << 16;
+    d |= static_cast<uint64_t>((8 * R * 2) >> 4) << 32;  // eight rows
+    d |= 1ull << 46;
+    d |= (R == 32 ? 4ull : 6ull) << 61;
+    return d;
+}
+
+__device__ __forceinline__ float warp_max_redux(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+// Barrier of the four softmax warps, with and without an OR of a predicate.
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool soft_any(bool p) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+        "bar.red.or.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r)
+        : "r"(static_cast<uint32_t>(p))
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) {
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(v[i]);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One work item.
+struct Item {
+    int q0, nq;       // query rows [q0, q0 + nq)
+    int row;          // cache row
+    int k0, nk, nt;   // first key, keys, 128-key tiles (0: nothing to attend)
+    int split;
+};
+
+template <int N> struct Walk {
+    const TcArgs& a;
+    const int* plan;  // shared: cumulative query blocks of the groups, or null
+    int items, per;   // query blocks per group (no plan) or per row (suffix)
+    __device__ Walk(const TcArgs& args, const int* pl) : a(args), plan(pl) {
+        const Problem& p = a.p;
+        const int th = p.T * p.H;
+        if (a.suffix) {
+            per = (th + N - 1) / N;
+            items = p.B * per * a.splits;
+        } else {
+            per = (p.max_group * th + N - 1) / N;
+            items = (plan ? plan[p.G] : p.G * per) * a.splits;
+        }
+    }
+    __device__ __forceinline__ Item get(int idx) const {
+        const Problem& p = a.p;
+        const int th = p.T * p.H;
+        Item it;
+        it.split = idx % a.splits;
+        const int blk = idx / a.splits;
+        int len;
+        if (a.suffix) {
+            it.row = blk / per;
+            const int s = (blk - it.row * per) * N;
+            it.q0 = it.row * th + s;
+            it.nq = min(N, th - s);
+            len = suffix_length(p, it.row);
+        } else {
+            int g, s;
+            if (plan) {
+                int lo = 0, hi = p.G;  // the group with plan[g] <= blk < plan[g + 1]
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (plan[mid] <= blk) lo = mid;
+                    else hi = mid;
+                }
+                g = lo;
+                s = (blk - plan[g]) * N;
+            } else {
+                g = blk / per;
+                s = (blk - g * per) * N;
+            }
+            const int b0 = min(max(p.group_start[g], 0), p.B), b1 = min(max(p.group_start[g + 1], b0), p.B);
+            const int total = min(b1 - b0, p.max_group) * th;
+            it.row = g;
+            it.q0 = b0 * th + s;
+            it.nq = max(0, min(N, total - s));
+            len = it.nq > 0 ? prefix_length(p, g) : 0;
+        }
+        it.k0 = it.split * a.kps;
+        it.nk = max(0, min(a.kps, len - it.k0));
+        it.nt = (it.nk + 127) / 128;
+        return it;
+    }
+};
+
+// Cursor over the tiles of a CTA's items that have any.
+template <int N> struct Cursor {
+    const Walk<N>& w;
+    int idx;
+    Item it;
+    int j;
+    __device__ Cursor(const Walk<N>& walk) : w(walk), idx(static_cast<int>(blockIdx.x) - static_cast<int>(gridDim.x)), j(0) {
+        next_item();
+    }
+    __device__ __forceinline__ void next_item() {
+        j = 0;
+        do {
+            idx += gridDim.x;
+            if (idx >= w.items) return;
+            it = w.get(idx);
+        } while (it.nt == 0);
+    }
+    __device__ __forceinline__ bool valid() const { return idx < w.items; }
+    __device__ __forceinline__ void next() {
+        if (++j == it.nt) next_item();
+    }
+};
+
+template <int KV, int R, int N, typename T, bool Q8>
+__global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(const __grid_constant__ TcArgs a) {
+    using C = TcCfg<KV, R, N, Q8>;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ uint8_t tc_smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_smem_raw) + 1023) &
+                                               ~static_cast<uintptr_t>(1023));
+    float* m_s = reinterpret_cast<float*>(smem + C::oF);
+    float* corr_s = m_s + N;
+    float* red_s = corr_s + N;  // [4][N]
+    int* lim_s = reinterpret_cast<int*>(red_s + 4 * N);
+    int* plan_s = reinterpret_cast<int*>(smem + C::oPlan);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::oBar);
+    uint64_t* q_empty = bars;                    // [QB] the item's S products have read Q
+    uint64_t* pair_full = q_empty + C::QB;       // [PS] four producer warps
+    uint64_t* pair_empty = pair_full + C::PS;    // [PS] O products done with the pair
+    uint64_t* rope_full = pair_empty + C::PS;    // [RS] four producer warps (and the item's queries)
+    uint64_t* rope_empty = rope_full + C::RS;    // [RS]
+    uint64_t* s_full = rope_empty + C::RS;       // [2]
+    uint64_t* s_free = s_full + 2;               // [2] four softmax warps
+    uint64_t* p_full = s_free + 2;               // [PB] four softmax warps
+    uint64_t* p_free = p_full + C::PB;           // [PB] the tile's O products are complete
+    uint64_t* o_full = p_free + C::PB;           // [OB]
+    uint64_t* o_free = o_full + C::OB;           // [OB] four softmax warps
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
+    int* bad_s = reinterpret_cast<int*>(tmem_slot + 1);
+    const Problem& p = a.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            for (int i = 0; i < C::QB; ++i) mbar_init(&q_empty[i], 1);
+            for (int i = 0; i < C::PS; ++i) { mbar_init(&pair_full[i], 4); mbar_init(&pair_empty[i], 1); }
+            for (int i = 0; i < C::RS; ++i) { mbar_init(&rope_full[i], 4); mbar_init(&rope_empty[i], 1); }
+            for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); }
+            for (int i = 0; i < C::PB; ++i) { mbar_init(&p_full[i], 4); mbar_init(&p_free[i], 1); }
+            for (int i = 0; i < C::OB; ++i) { mbar_init(&o_full[i], 1); mbar_init(&o_free[i], 4); }
+            *bad_s = 0;
+            fence_mbar_init();
+        }
+        __syncwarp();
+        tmem_alloc(tmem_slot, C::kTmem);
+        tmem_relinquish();
+    }
+    MM_PDL_ENTRY();
+    // plan: cumulative query blocks of the groups
+    const bool planned = !a.suffix && p.G <= kTcMaxPlan;
+    if (planned) {
+        for (int g = tid; g < p.G; g += kTcThreads) {
+            const int b0 = min(max(p.group_start[g], 0), p.B), b1 = min(max(p.group_start[g + 1], b0), p.B);
+            plan_s[g + 1] = (min(b1 - b0, p.max_group) * p.T * p.H + N - 1) / N;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            int base = 0;
+            for (int g0 = 0; g0 < p.G; g0 += 32) {
+                int v = g0 + lane < p.G ? plan_s[g0 + lane + 1] : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(0xffffffffu, v, o);
+                    if (lane >= o) v += u;
+                }
+                if (g0 + lane < p.G) plan_s[g0 + lane + 1] = base + v;
+                base += __shfl_sync(0xffffffffu, v, 31);
+            }
+            if (lane == 0) plan_s[0] = 0;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const Walk<N> walk(a, planned ? plan_s : nullptr);
+    const lat::CacheView& cv = a.suffix ? p.suffix : p.prefix;
+    bool ok = true;
+    // a wait that ran out is recorded once; later waits of this thread are skipped
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok && !mbar_wait_bounded(bar, parity, nullptr)) {
+            ok = false;
+            *reinterpret_cast<volatile int*>(bad_s) = 1;
+        }
+    };
+
+    if (warp >= 4 && warp < 8) {
+        // ------------------------------------------------------------ producers
+        const int pt = tid - 128;  // 0..127
+        uint8_t* sQ = smem + C::oQ;
+        uint8_t* sPair = smem + C::oPair;
+        uint8_t* sRope = smem + C::oRope;
+        const int th = p.T * p.H;
+        auto load_q = [&](const Item& it, int qb) {
+            uint8_t* q = sQ + qb * C::kQA;
+            constexpr int kChunks = (KV + R) / 8;
+            for (int e = pt; e < N * kChunks; e += 128) {
+                const int n = e / kChunks, c = e - n * kChunks;
+                const bool in = n < it.nq;
+                const int r = it.q0 + (in ? n : 0), b = r / th, u = r - b * th, t = u / p.H, h = u - t * p.H;
+                const T* src = static_cast<const T*>(p.q) + b * p.q_row + t * p.q_tok + h * p.q_head + c * 8;
+                uint8_t* dst = c < KV / 8 ? q + (c >> 3) * C::kQBox + sw128(n, c & 7)
+                                          : q + 2 * C::NP * C::kQBox + sw_rope<R>(n, c - KV / 8);
+                cp_async16(dst, src, in);
+            }
+        };
+        auto load_rope = [&](const Item& it, int j, int slot) {
+            constexpr int kChunks = R / 8;
+            uint8_t* d = sRope + slot * C::kRopeA;
+            const uint8_t* base = Q8 ? cv.rope + 2 * (it.row * cv.rope_row_stride)
+                                     : cv.latent + 2 * (it.row * cv.row_stride + KV);
+            const long long ps = Q8 ? cv.rope_pos_stride : cv.pos_stride;
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) {
+                const int e = pt + 128 * i, r = e / kChunks, c = e - r * kChunks;
+                const bool in = j * 128 + r < it.nk;
+                cp_async16(d + sw_rope<R>(r, c), base + 2 * ((it.k0 + (in ? j * 128 + r : 0)) * ps) + c * 16, in);
+            }
+        };
+        auto arrive_full = [&](uint64_t* bar) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        if constexpr (!Q8) {
+            // units in order per tile: rope (the item's queries with its first), pair 0, 1, ...
+            // Each is one cp.async group; a unit is announced once later groups are in flight, or
+            // all at once before the warp would block on a full ring.
+            int issued = 0, told = 0;
+            constexpr int kFlight = C::PS;
+            auto bar_of = [&](int u) {
+                const int t = u / (C::NP + 1), s = u - t * (C::NP + 1);
+                return s == 0 ? &rope_full[t % C::RS] : &pair_full[(t * C::NP + s - 1) % C::PS];
+            };
+            auto tell_to = [&](int n) {
+                if (told >= n) return;
+                fence_proxy_async_smem();
+                __syncwarp();
+                for (; told < n; ++told)
+                    if (lane == 0) mbar_arrive(bar_of(told));
+            };
+            auto room = [&](uint64_t* bar, uint32_t parity) {
+                // uniform over the warp: every lane must take the same path
+                const bool free = __all_sync(0xffffffffu, mbar_try_wait(bar, parity));
+                if (!free) {
+                    cp_async_wait<0>();
+                    tell_to(issued);
+                    wait(bar, parity);
+                }
+            };
+            int qi = -1, tile = 0, pr = 0;
+            for (Cursor<N> c(walk); c.valid(); c.next(), ++tile) {
+                room(&rope_empty[tile % C::RS], ((tile / C::RS) & 1) ^ 1);
+                if (c.j == 0) {
+                    ++qi;
+                    room(&q_empty[qi % C::QB], ((qi / C::QB) & 1) ^ 1);
+                    load_q(c.it, qi % C::QB);
+                }
+                load_rope(c.it, c.j, tile % C::RS);
+                cp_async_commit();
+                ++issued;
+#pragma unroll 1
+                for (int i = 0; i < C::NP; ++i, ++pr) {
+                    const int slot = pr % C::PS;
+                    room(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
+                    uint8_t* d = sPair + slot * C::kPair;
+                    const int cc = pt & 15, r0 = pt >> 4;
+                    const uint8_t* base = cv.latent + 2 * (c.it.row * cv.row_stride + i * 128 + cc * 8);
+                    d += (cc >> 3) * C::kBox;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const int r = r0 + 8 * k;
+                        const bool in = c.j * 128 + r < c.it.nk;
+                        cp_async16(d + sw128(r, cc & 7), base + 2 * ((c.it.k0 + (in ? c.j * 128 + r : 0)) * cv.pos_stride), in);
+                    }
+                    cp_async_commit();
+                    ++issued;
+                    cp_async_wait<kFlight - 1>();
+                    tell_to(issued - (kFlight - 1));
+                }
+            }
+            cp_async_wait<0>();
+            tell_to(issued);
+        } else {
+            // codes four pairs ahead in registers: 8 x 16 bytes of a pair per thread
+            constexpr int D = 4;
+            uint4 v[D][8];
+            const int cc = pt & 7, r0 = pt >> 3;  // 16-byte chunk of the pair's 128 codes, first row
+            auto fetch = [&](uint4 (&x)[8], const Item& it, int j, int i) {
+                const uint8_t* base = cv.latent + it.row * cv.row_stride + i * 128 + cc * 16;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int r = r0 + 16 * k;
+                    x[k] = j * 128 + r < it.nk
+                               ? __ldg(reinterpret_cast<const uint4*>(base + (it.k0 + j * 128 + r) * cv.pos_stride))
+                               : make_uint4(0, 0, 0, 0);
+                }
+            };
+            Cursor<N> lc(walk), sc(walk);
+            int li = 0, si = 0;  // pair of the tile each cursor is at
+            auto step = [&](Cursor<N>& c, int& i) {
+                if (++i == C::NP) {
+                    i = 0;
+                    c.next();
+                }
+            };
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+                if (lc.valid()) {
+                    fetch(v[d], lc.it, lc.j, li);
+                    step(lc, li);
+                }
+            int qi = -1, tile = 0, pr = 0;
+            while (sc.valid()) {
+#pragma unroll
+                for (int d = 0; d < D; ++d) {
+                    if (sc.valid()) {
+                        if (si == 0) {
+                            wait(&rope_empty[tile % C::RS], ((tile / C::RS) & 1) ^ 1);
+                            if (sc.j == 0) {
+                                ++qi;
+                                wait(&q_empty[qi % C::QB], ((qi / C::QB) & 1) ^ 1);
+                                load_q(sc.it, qi % C::QB);
+                            }
+                            load_rope(sc.it, sc.j, tile % C::RS);
+                            cp_async_commit();
+                        }
+                        const int slot = pr % C::PS;
+                        wait(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
+                        uint8_t* dst = sPair + slot * C::kPair + (cc >> 2) * C::kBox;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const int r = r0 + 16 * k;
+                            const uint32_t w[4] = {v[d][k].x, v[d][k].y, v[d][k].z, v[d][k].w};
+                            uint32_t o[8];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                o[2 * e] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] & 0xffff));
+                                o[2 * e + 1] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] >> 16));
+                            }
+                            *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc) & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc + 1) & 7)) = make_uint4(o[4], o[5], o[6], o[7]);
+                        }
+                        if (lc.valid()) {
+                            fetch(v[d], lc.it, lc.j, li);
+                            step(lc, li);
+                        }
+                        if (si == 0) {
+                            cp_async_wait<0>();
+                            arrive_full(&rope_full[tile % C::RS]);
+                        }
+                        arrive_full(&pair_full[slot]);
+                        ++pr;
+                        if (si == C::NP - 1) ++tile;
+                        step(sc, si);
+                    }
+                }
+            }
+            cp_async_wait<0>();
+        }
+    } else if (warp >= 8) {
+        // ------------------------------------------------------------ tensor-core products
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        if (warp == 8 && lane == 0) {
+            const uint32_t id_s = umma_idesc_f16(kBf16, false, false, 128, N);
+            const uint32_t id_o = umma_idesc_f16(kBf16, true, N == 64, 128, N);
+            const uint32_t aPair = smem_u32(smem + C::oPair), aQ = smem_u32(smem + C::oQ), aR = smem_u32(smem + C::oRope),
+                           aP = smem_u32(smem + C::oP);
+            int s_tile = 0, s_pr = 0, s_q = 0;    // S products: tile, pair and item counters
+            int o_tile = 0, o_pr = 0, o_item = 0;  // O products
+            auto issue_s = [&](const Cursor<N>& c) {
+                const uint32_t q = aQ + (s_q % C::QB) * C::kQA;
+                const int sb = s_tile & 1;
+                const uint32_t d = tmem + C::kColS + sb * N;
+                wait(&s_free[sb], ((s_tile >> 1) & 1) ^ 1);
+                const int rs = s_tile % C::RS;
+                wait(&rope_full[rs], (s_tile / C::RS) & 1);
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < R / 16; ++k)
+                    tc_mma_f16(Q8 ? tmem + C::kColR + sb * N : d, rope_desc<R>(aR + rs * C::kRopeA + k * 32),
+                               rope_desc<R>(q + 2 * C::NP * C::kQBox + k * 32), id_s, k ? 1u : 0u);
+                tc_commit(&rope_empty[rs]);
+#pragma unroll 1
+                for (int i = 0; i < C::NP; ++i, ++s_pr) {
+                    const int slot = s_pr % C::PS;
+                    wait(&pair_full[slot], (s_pr / C::PS) & 1);
+                    tc_fence_after();
+                    const uint32_t ka = aPair + slot * C::kPair, qa = q + 2 * i * C::kQBox;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        tc_mma_f16(d, umma_desc_sw128(ka + (k >> 2) * C::kBox + (k & 3) * 32, 16, 1024),
+                                   umma_desc_sw128(qa + (k >> 2) * C::kQBox + (k & 3) * 32, 16, 1024), id_s,
+                                   Q8 ? ((i | k) ? 1u : 0u) : 1u);
+                }
+                tc_commit(&s_full[sb]);
+                if (c.j == c.it.nt - 1) {
+                    tc_commit(&q_empty[s_q % C::QB]);
+                    ++s_q;
+                }
+                ++s_tile;
+            };
+            auto issue_o = [&](const Cursor<N>& c) {
+                const int ob = o_item % C::OB, pb = o_tile % C::PB;
+                if (c.j == 0) wait(&o_free[ob], ((o_item / C::OB) & 1) ^ 1);
+                wait(&p_full[pb], (o_tile / C::PB) & 1);
+                tc_fence_after();
+                const uint32_t pa = aP + pb * C::kP;
+#pragma unroll 1
+                for (int i = 0; i < C::NP; ++i, ++o_pr) {
+                    const int slot = o_pr % C::PS;
+                    const uint32_t va = aPair + slot * C::kPair;
+                    const uint32_t d = tmem + C::kColO + (ob * C::NP + i) * N;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        // V^T MN-major: 16 keys = 2,048 B down a box, the next 64 columns one box on
+                        const uint64_t bd = N == 64 ? umma_desc_sw128(pa + k * 2048, C::kBox, 1024)
+                                                    : umma_desc_sw128(pa + (k >> 2) * 2048 + (k & 3) * 32, 16, 1024);
+                        tc_mma_f16(d, umma_desc_sw128(va + k * 2048, C::kBox, 1024), bd, id_o, (c.j | k) ? 1u : 0u);
+                    }
+                    tc_commit(&pair_empty[slot]);
+                }
+                tc_commit(&p_free[pb]);
+                if (c.j == c.it.nt - 1) {
+                    tc_commit(&o_full[ob]);
+                    ++o_item;
+                }
+                ++o_tile;
+            };
+            Cursor<N> cs(walk), co(walk);
+            if (C::kAhead) {
+                if (cs.valid()) {
+                    issue_s(cs);
+                    cs.next();
+                }
+                for (; co.valid(); co.next()) {
+                    if (cs.valid()) {
+                        issue_s(cs);
+                        cs.next();
+                    }
+                    issue_o(co);
+                }
+            } else {
+                for (; co.valid(); co.next()) {
+                    issue_s(co);
+                    issue_o(co);
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------ softmax and results
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+        const float cs = p.scale * 1.4426950408889634f;
+        const int th = p.T * p.H;
+        const long long rows = static_cast<long long>(p.B) * th;
+        int tile = 0, item = 0;
+        for (int idx = blockIdx.x; idx < walk.items; idx += gridDim.x) {
+            const Item it = walk.get(idx);
+            if (it.nt == 0 && !a.merge) continue;
+            if (it.nq == 0) continue;
+            float l[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) l[n] = 0.f;
+            // keys of the item each query sees; the tokens of a suffix end one position apart
+            const bool causal = a.suffix && p.T > 1;
+            soft_sync();  // the previous item's readers of m_s, lim_s and red_s are done
+            if (tid < N) {
+                m_s[tid] = kNoMax;
+                int lim = it.nk;
+                if (causal) {
+                    const int t = min((it.q0 + tid - it.row * th) / p.H, p.T - 1);
+                    lim = min(it.nk, suffix_length(p, it.row) - (p.T - 1 - t) - it.k0);
+                }
+                lim_s[tid] = lim;
+            }
+            soft_sync();
+            const int lim_min = causal ? it.nk - (p.T - 1) : it.nk;
+            const float* ks_row = Q8 ? cv.scale + it.row * cv.scale_row_stride + it.k0 : nullptr;
+            for (int j = 0; j < it.nt; ++j, ++tile) {
+                const int key = j * 128 + warp * 32 + lane;
+                const float ks = Q8 && key < it.nk ? __ldg(ks_row + key) : 1.f;
+                const int sb = tile & 1;
+                wait(&s_full[sb], (tile >> 1) & 1);
+                tc_fence_after();
+                float z[N];
+                if constexpr (N == 64) {
+                    tmem_ld32_nowait(lane_base + C::kColS + sb * N, z);
+                    tmem_ld32_nowait(lane_base + C::kColS + sb * N + 32, z + 32);
+                    tmem_wait_ld();
+                } else {
+                    tmem_ld16(lane_base + C::kColS + sb * N, z);
+                }
+                if constexpr (Q8) {
+#pragma unroll
+                    for (int n = 0; n < N; n += 16) {
+                        float r[16];
+                        tmem_ld16(lane_base + C::kColR + sb * N + n, r);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) z[n + e] = fmaf(z[n + e], ks, r[e]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_free[sb]);
+                if ((j + 1) * 128 > lim_min) {  // the last tile(s): keys past a query's limit
+#pragma unroll
+                    for (int n = 0; n < N; ++n) z[n] = key < lim_s[n] ? z[n] * cs : -INFINITY;
+                } else {
+#pragma unroll
+                    for (int n = 0; n < N; ++n) z[n] *= cs;
+                }
+                bool over = false;
+#pragma unroll
+                for (int n = 0; n < N; n += 4) {
+                    const float4 m = *reinterpret_cast<const float4*>(m_s + n);
+                    over |= z[n] > m.x + 8.f;
+                    over |= z[n + 1] > m.y + 8.f;
+                    over |= z[n + 2] > m.z + 8.f;
+                    over |= z[n + 3] > m.w + 8.f;
+                }
+                if (soft_any(over)) {
+                    float mine[(N + 31) / 32];
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        const float v = warp_max_redux(z[n]);
+                        if (lane == (n & 31)) mine[n >> 5] = v;
+                    }
+#pragma unroll
+                    for (int k = 0; k < (N + 31) / 32; ++k)
+                        if (lane + 32 * k < N) red_s[warp * N + lane + 32 * k] = mine[k];
+                    soft_sync();
+                    if (tid < N) {
+                        const float mt = fmaxf(fmaxf(red_s[tid], red_s[N + tid]), fmaxf(red_s[2 * N + tid], red_s[3 * N + tid]));
+                        const float mo = m_s[tid], mn = mt > mo + 8.f ? mt : mo;
+                        corr_s[tid] = fast_exp2(mo - mn);
+                        m_s[tid] = mn;
+                    }
+                    soft_sync();
+#pragma unroll
+                    for (int n = 0; n < N; ++n) l[n] *= corr_s[n];
+                    if (j > 0) {
+                        // the previous tile's products have landed: rescale the accumulator
+                        const int pt = tile - 1;
+                        wait(&p_free[pt % C::PB], (pt / C::PB) & 1);
+                        tc_fence_after();
+                        const uint32_t o = lane_base + C::kColO + (item % C::OB) * C::NP * N;
+#pragma unroll 1
+                        for (int i = 0; i < C::NP; ++i)
+#pragma unroll 1
+                            for (int c = 0; c < N; c += 16) {
+                                float v[16];
+                                tmem_ld16(o + i * N + c, v);
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) v[e] *= corr_s[c + e];
+                                tmem_st16(o + i * N + c, v);
+                            }
+                        tmem_wait_st();
+                    }
+                }
+                const int pb = tile % C::PB;
+                wait(&p_free[pb], ((tile / C::PB) & 1) ^ 1);
+                uint8_t* P = smem + C::oP + pb * C::kP;
+                const int kr = warp * 32 + lane;  // key row of the tile
+#pragma unroll
+                for (int n0 = 0; n0 < N; n0 += 8) {
+                    float e[8];
+#pragma unroll
+                    for (int q = 0; q < 8; q += 4) {
+                        const float4 m = *reinterpret_cast<const float4*>(m_s + n0 + q);
+                        e[q] = fast_exp2(z[n0 + q] - m.x);
+                        e[q + 1] = fast_exp2(z[n0 + q + 1] - m.y);
+                        e[q + 2] = fast_exp2(z[n0 + q + 2] - m.z);
+                        e[q + 3] = fast_exp2(z[n0 + q + 3] - m.w);
+                    }
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        l[n0 + q] += e[q];
+                        if (Q8) e[q] *= ks;
+                    }
+                    if constexpr (N == 64) {
+                        *reinterpret_cast<uint4*>(P + sw128(kr, n0 >> 3)) =
+                            make_uint4(lat::pack2<T>(e[0], e[1]), lat::pack2<T>(e[2], e[3]), lat::pack2<T>(e[4], e[5]),
+                                       lat::pack2<T>(e[6], e[7]));
+                    } else {
+                        // K-major: query row n, key kr of the 64-key box kr / 64
+#pragma unroll
+                        for (int q = 0; q < 8; ++q)
+                            *reinterpret_cast<T*>(P + (kr >> 6) * 2048 + sw128(n0 + q, (kr & 63) >> 3) + (kr & 7) * 2) =
+                                lat::from_f32<T>(e[q]);
+                    }
+                }
+                tc_fence_before();
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[pb]);
+            }
+            // the sums over the tile's 128 keys: halve the columns while folding the lanes
+            int own = 0;  // first column this lane ends up with
+            {
+                int w = N;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    if (w > 1) {
+                        w >>= 1;
+                        const bool up = lane & o;
+#pragma unroll
+                        for (int i = 0; i < N / 2; ++i)
+                            if (i < w) {
+                                const float send = up ? l[i] : l[i + w];
+                                const float got = __shfl_xor_sync(0xffffffffu, send, o);
+                                l[i] = (up ? l[i + w] : l[i]) + got;
+                            }
+                        if (up) own += w;
+                    } else {
+                        l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+                    }
+                }
+            }
+            if constexpr (N == 64) {
+                red_s[warp * N + own] = l[0];
+                red_s[warp * N + own + 1] = l[1];
+            } else if ((lane & 1) == 0) {
+                red_s[warp * N + own] = l[0];
+            }
+            soft_sync();
+            if (tid < N) {
+                float t = (red_s[tid] + red_s[N + tid]) + (red_s[2 * N + tid] + red_s[3 * N + tid]);
+                corr_s[tid] = *reinterpret_cast<volatile int*>(bad_s) ? __int_as_float(0x7fc00000) : t;  // the sum
+            }
+            soft_sync();
+            const int ob = item % C::OB;
+            if (it.nt > 0) {
+                wait(&o_full[ob], (item / C::OB) & 1);
+                tc_fence_after();
+            }
+            const uint32_t o = lane_base + C::kColO + ob * C::NP * N;
+            const int d0 = warp * 32 + lane;
+            if (!a.merge) {
+                const long long at = it.split * rows + it.q0;
+                if (tid < it.nq) a.part_ml[at + tid] = make_float2(m_s[tid], corr_s[tid]);
+#pragma unroll 1
+                for (int i = 0; i < C::NP; ++i)
+#pragma unroll 1
+                    for (int c = 0; c < it.nq; c += 16) {
+                        float v[16];
+                        tmem_ld16(o + i * N + c, v);
+                        float* dst = a.part_o + (at + c) * KV + i * 128 + d0;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (c + e < it.nq) dst[static_cast<long long>(e) * KV] = v[e];
+                    }
+            } else {
+                // join the prefix partials of the row's group, then the result itself
+                const int g = p.G > 0 ? group_of(p, it.row) : -1;
+                const int plen = prefix_length(p, g);
+                const int np = (plen + a.prefix_kps - 1) / a.prefix_kps;
+                if (tid < it.nq) {
+                    // factor of each part relative to the joint maximum
+                    float M = corr_s[tid] > 0.f || corr_s[tid] != corr_s[tid] ? m_s[tid] : kNoMax;
+                    for (int s = 0; s < np; ++s) M = fmaxf(M, __ldcg(&a.part_ml[s * rows + it.q0 + tid]).x);
+                    float L = corr_s[tid] * fast_exp2(m_s[tid] - M);
+                    for (int s = 0; s < np; ++s) {
+                        const float2 ml = __ldcg(&a.part_ml[s * rows + it.q0 + tid]);
+                        L += ml.y * fast_exp2(ml.x - M);
+                    }
+                    red_s[tid] = M;
+                    red_s[N + tid] = L == 0.f ? 0.f : 1.f / L;
+                    if (p.lse) p.lse[it.q0 + tid] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+                }
+                soft_sync();
+#pragma unroll 1
+                for (int i = 0; i < C::NP; ++i)
+#pragma unroll 1
+                    for (int c = 0; c < it.nq; c += 16) {
+                        float v[16];
+                        if (it.nt > 0) tmem_ld16(o + i * N + c, v);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) v[e] = it.nt > 0 ? v[e] * fast_exp2(m_s[c + e] - red_s[c + e]) : 0.f;
+                        for (int s = 0; s < np; ++s) {
+                            const long long at = s * rows + it.q0 + c;
+                            const float* src = a.part_o + at * KV + i * 128 + d0;
+                            float x[16];
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                x[e] = c + e < it.nq ? __ldcg(src + static_cast<long long>(e) * KV) : 0.f;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (c + e < it.nq) v[e] += x[e] * fast_exp2(__ldcg(&a.part_ml[at + e]).x - red_s[c + e]);
+                        }
+                        T* dst = static_cast<T*>(p.out) + static_cast<long long>(it.q0 + c) * KV + i * 128 + d0;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (c + e < it.nq) dst[static_cast<long long>(e) * KV] = lat::from_f32<T>(v[e] * red_s[N + c + e]);
+                    }
+            }
+            if (it.nt > 0) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&o_free[ob]);
+                ++item;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::kTmem);
+    }
+}
+
+// Joins the partials of a query row: its group's prefix ranges and its suffix ranges. One warp
+// per query row, V columns per lane and pass; grid-stride.
+template <int KV, typename T>
+__global__ void __launch_bounds__(256) shared_prefix_join_kernel(const Problem p, const float* __restrict__ pre_o,
+                                                                 const float2* __restrict__ pre_ml, int pre_kps,
+                                                                 const float* __restrict__ suf_o,
+                                                                 const float2* __restrict__ suf_ml, int suf_kps) {
+    MM_PDL_ENTRY();
+    const int th = p.T * p.H, lane = threadIdx.x & 31;
+    const long long rows = static_cast<long long>(p.B) * th;
+    const long long r = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+    if (r >= rows) return;
+    const int b = static_cast<int>(r / th);
+    const int g = p.G > 0 ? group_of(p, b) : -1;
+    const int np = (prefix_length(p, g) + pre_kps - 1) / pre_kps;
+    const int ns = (suffix_length(p, b) + suf_kps - 1) / suf_kps;
+    auto ml = [&](int s) { return s < np ? __ldcg(&pre_ml[s * rows + r]) : __ldcg(&suf_ml[(s - np) * rows + r]); };
+    float M = kNoMax;
+    for (int s = lane; s < np + ns; s += 32) M = fmaxf(M, ml(s).x);
+    M = warp_max(M);
+    float L = 0.f;
+    for (int s = lane; s < np + ns; s += 32) {
+        const float2 v = ml(s);
+        L += v.y * fast_exp2(v.x - M);
+    }
+    L = warp_sum(L);
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    constexpr int C = KV / 128;  // float4s per lane
+    float4 acc[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < np + ns; ++s) {
+        const float f = fast_exp2(ml(s).x - M);
+        const float4* o = reinterpret_cast<const float4*>((s < np ? pre_o + (s * rows + r) * KV : suf_o + ((s - np) * rows + r) * KV)) + lane;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const float4 v = __ldcg(o + 32 * c);
+            acc[c].x += f * v.x;
+            acc[c].y += f * v.y;
+            acc[c].z += f * v.z;
+            acc[c].w += f * v.w;
+        }
+    }
+    uint2* out = reinterpret_cast<uint2*>(static_cast<T*>(p.out) + r * KV) + lane;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+        out[32 * c] = make_uint2(lat::pack2<T>(acc[c].x * inv, acc[c].y * inv), lat::pack2<T>(acc[c].z * inv, acc[c].w * inv));
+    if (p.lse && lane == 0) p.lse[r] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+}
+
+}  // namespace spa
+}  // namespace mm
