@@ -273,10 +273,10 @@ Plan plan(const mm::spa::Problem& p) {
 
 template <int KV, int R, int N, typename T, bool Q8>
 void launch_tc(const mm::spa::TcArgs& a, long long items, cudaStream_t s) {
-    using namespace mm::spa;
-    set_dynamic_smem<shared_prefix_tc_kernel<KV, R, N, T, Q8>>(TcCfg<KV, R, N, Q8>::kSmem);
-    launch(s, shared_prefix_tc_kernel<KV, R, N, T, Q8>, dim3(static_cast<unsigned>(std::min<long long>(items, sm_count()))),
-           dim3(kTcThreads), TcCfg<KV, R, N, Q8>::kSmem, a);
+    using C = mm::spa::TcCfg<KV, R, N, Q8>;
+    set_dynamic_smem<mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8>>(C::kSmem);
+    launch(s, mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8>,
+           dim3(static_cast<unsigned>(std::min<long long>(items, sm_count() * C::kCtas))), dim3(C::kThreads), C::kSmem, a);
 }
 template <int KV, int R, typename T>
 void launch_tc_n(const mm::spa::TcArgs& a, int n, bool q8, long long items, cudaStream_t s) {
@@ -292,13 +292,24 @@ void run_tc(const mm::spa::Problem& p, const Plan& r, bool q8p, bool q8s, void* 
     float* suf_o = pre_o + r.pre_part * KV;
     float2* pre_ml = reinterpret_cast<float2*>(suf_o + r.suf_part * KV);
     float2* suf_ml = pre_ml + r.pre_part;
+    TcArgs a{};
+    a.p = p;
     if (r.pre_n) {
-        const TcArgs a{p, 0, r.pre_splits, r.pre_kps, pre_o, pre_ml, 0, 0, 128};
+        a.splits = r.pre_splits;
+        a.kps = r.pre_kps;
+        a.part_o = pre_o;
+        a.part_ml = pre_ml;
         launch_tc_n<KV, R, T>(a, r.pre_n, q8p, r.pre_blocks * r.pre_splits, s);
     }
     if (r.suf_n) {
-        const TcArgs a{p, 1, r.suf_splits, r.suf_kps, r.merge ? pre_o : suf_o, r.merge ? pre_ml : suf_ml, r.merge ? 1 : 0,
-                       r.pre_splits, r.pre_kps};
+        a.suffix = 1;
+        a.splits = r.suf_splits;
+        a.kps = r.suf_kps;
+        a.merge = r.merge ? 1 : 0;
+        a.part_o = r.merge ? pre_o : suf_o;
+        a.part_ml = r.merge ? pre_ml : suf_ml;
+        a.prefix_kps = r.pre_kps;
+        a.overlap = r.pre_n ? 1 : 0;
         launch_tc_n<KV, R, T>(a, r.suf_n, q8s, r.suf_blocks * r.suf_splits, s);
     }
     if (!r.merge)

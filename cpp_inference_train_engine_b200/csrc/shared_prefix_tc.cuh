@@ -2,7 +2,7 @@
 // and [512 latent | 32 rope] caches.
 //
 // Keys are the M side of both products, queries the N side:
-//   S^T [128 keys x N queries] = K [128 x (kv + rope)] Q^T,     O^T [kv x N] += V^T [kv x 128] P^T,
+//   S^T [128 keys x N queries] = K [128 x (kv + rope)] Q^T,     O^T [kv x N] += V^T [kv x keys] P^T,
 // V being K's first kv columns, so one shared-memory tile of the cache is read by both products
 // (K-major for S^T, MN-major for O^T) and a cache row crosses HBM once per block of N queries.
 // A decode step has few queries per key (8 or 16 heads of a row; a group's rows x heads over its
@@ -11,21 +11,22 @@
 // and O^T takes kv / 128 x N columns (256 of 512 at N = 64).
 //
 // A work item is (block of N query rows, key range): one group's query rows over a range of its
-// prefix, or one row's queries over a range of its suffix. CTAs are persistent (one per SM) and
-// walk the items; barrier phases run on across items. 12 warps (three warpgroups, whose register
-// shares 232 + 168 + 104 add up to the launch's 3 x 168):
-//   warps 4-7  producers: the item's queries, then per 128-key tile the rope columns and kv / 128
-//              pairs of 64-column boxes into rings of swizzled boxes. 16-bit caches go by 16-byte
-//              cp.async; e4m3 codes are loaded four pairs ahead into registers and stored as 16-bit
+// prefix, or one row's queries over a range of its suffix. CTAs are persistent and walk the items
+// (tables of 32 at a time in shared memory, so no role waits for an item's lengths); barrier
+// phases run on across items. Warps:
+//   softmax    4 (N = 16) or 8 (N = 64, each four take 32 of the queries): thread = key
+//              (tensor-memory lane). The running maximum is lazy: a tile whose scores stay below
+//              the reference + 8 (base 2) uses the reference as it is (probabilities up to 2^8 fit
+//              fp16, sums are fp32), decided by one 4-warp vote; otherwise the column maxima are
+//              taken and O^T and the sums are rescaled. A key's scale (e4m3) multiplies its latent
+//              scores and, for the second product, its probabilities.
+//   producers  4: the item's queries, then per tile of KT keys the rope columns and kv / 128 pairs
+//              of 64-column boxes into rings of swizzled boxes. 16-bit caches go by 16-byte
+//              cp.async; e4m3 codes are loaded D pairs ahead into registers and stored as 16-bit
 //              values (exact). Rows past the range are zero-filled, so whatever the cache holds
 //              there never reaches a product.
-//   warp 8     one thread issues tcgen05.mma (warps 9-11 only fill its warpgroup).
-//   warps 0-3  softmax: thread = key (tensor-memory lane), N query columns. The running maximum
-//              is lazy: a tile whose scores stay below the reference + 8 (base 2) uses the
-//              reference as it is (probabilities up to 2^8 fit fp16, sums are fp32), decided by one
-//              4-warp vote; otherwise the maxima are taken (warp reductions and an exchange) and
-//              O^T and the sums are rescaled. A key's scale (e4m3) multiplies its scores and, for
-//              the second product, its probabilities.
+//   one more   one thread issues tcgen05.mma. With KT = 64 the S^T product still has M = 128: its
+//              upper half reads whatever follows the box in shared memory and is never looked at.
 // Every mbarrier wait is bounded; after a wait that runs out the CTA goes on without waiting (every
 // loop is bounded, every access in bounds) and its results are NaN.
 #pragma once
@@ -44,28 +45,41 @@ struct TcArgs {
     // result is written
     float* part_o;
     float2* part_ml;
-    int merge, prefix_splits, prefix_kps;
+    int merge, prefix_kps;
+    int overlap;       // the launch before this one is the call's own prefix launch: run beside it
 };
 
-constexpr int kTcThreads = 384;      // 12 warps: 168 registers each at launch
 constexpr int kTcMaxPlan = 512;   // groups whose item prefix sums fit the shared plan
+constexpr int kTcTable = 32;      // items per shared table
 constexpr float kNoMax = -1e37f;  // running maximum before any key (finite: its exp2 is 0, never NaN)
+
+// One work item.
+struct Item {
+    int q0, nq;       // query rows [q0, q0 + nq)
+    int row;          // cache row
+    int k0, nk, nt;   // first key, keys, tiles (0: nothing to attend)
+    int split;
+    int np;           // merge: the prefix ranges to join
+};
 
 template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int NP = KV / 128;                    // 128-column pairs of boxes
-    static constexpr int kBox = 128 * 128;                 // 128 keys x 64 columns of 16 bits
+    static constexpr int KT = N == 64 ? 128 : 64;          // keys per tile
+    static constexpr int kBox = KT * 128;                  // KT keys x 64 columns of 16 bits
     static constexpr int kPair = 2 * kBox;
-    static constexpr int kRope = 128 * R * 2;
+    static constexpr int kRope = KT * R * 2;
+    static constexpr int kRopeA = (kRope + 1023) / 1024 * 1024;
     static constexpr int kQBox = N * 128;
     static constexpr int kQ = 2 * NP * kQBox + N * R * 2;  // N query rows
     static constexpr int kQA = (kQ + 1023) / 1024 * 1024;
-    // P^T: N = 64: one MN-major box [128 keys x 64 queries]; N = 16: two K-major boxes of 64 keys
-    static constexpr int kP = N == 64 ? 128 * 128 : 2 * 16 * 128;
-    // rings: queries, pairs, rope boxes, P buffers, O accumulators (what 227 KB and 512 tensor
-    // memory columns hold)
+    // P^T: N = 64: one MN-major box [128 keys x 64 queries]; N = 16: K-major boxes of 64 keys
+    static constexpr int kP = N == 64 ? 128 * 128 : KT / 64 * 16 * 128;
+    // CTAs per SM, and rings: queries, pairs, rope boxes, P buffers, O accumulators (what 227 KB
+    // and 512 tensor memory columns hold)
+    static constexpr int kCtas = KV == 128 && N == 16 ? 2 : 1;
     static constexpr int QB = KV == 512 && N == 64 ? 1 : 2;
-    static constexpr int PS = KV == 512 ? (N == 64 ? 4 : 5) : (N == 64 ? 4 : 5);
-    static constexpr int RS = KV == 512 ? (N == 64 ? 1 : 2) : PS;
+    static constexpr int PS = KV == 512 ? (N == 64 ? 4 : 10) : (N == 64 ? 4 : 5);
+    static constexpr int RS = KV == 512 ? (N == 64 ? 1 : 3) : PS;
     static constexpr int PB = KV == 512 && N == 64 ? 1 : 2;
     static constexpr int OB = KV == 512 && N == 64 ? 1 : 2;
     // S of the next tile is issued before this tile's O when the rings hold two tiles
@@ -75,17 +89,23 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int kColS = 0, kColR = 2 * N, kColO = Q8 ? 4 * N : 2 * N;
     static constexpr int kCols = kColO + OB * NP * N;
     static constexpr int kTmem = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
-    static constexpr int kRopeA = (kRope + 1023) / 1024 * 1024;
+    // warps: softmax groups of four, four producers, the MMA warp (N = 64: its whole warpgroup, so
+    // that registers can move between the roles)
+    static constexpr int SG = N == 64 ? 2 : 1, NC = N / SG, SW = 4 * SG;
+    static constexpr int kThreads = 32 * (SW + 4 + (N == 64 ? 4 : 1));
+    // e4m3 pairs ahead in registers (KT / 16 16-byte loads per pair and thread)
+    static constexpr int VPT = KT / 16, D = KV == 512 && N == 16 ? 8 : KV == 128 && N == 16 ? 3 : 4;
     static constexpr int oPair = 0;
     static constexpr int oQ = oPair + PS * kPair;
     static constexpr int oRope = oQ + QB * kQA;
     static constexpr int oP = oRope + RS * kRopeA;
-    static constexpr int oF = oP + PB * kP;  // floats: m[N], corr[N], red[4][N], lim[N]
+    static constexpr int oTab = oP + PB * kP;
+    static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N]
     static constexpr int oPlan = oF + 7 * N * 4;
     static constexpr int oBar = oPlan + (kTcMaxPlan + 1) * 4 + 4;
-    static constexpr int kBars = 2 * QB + 2 * PS + 2 * RS + 4 + 2 * PB + 2 * OB;
+    static constexpr int kBars = QB + 2 * PS + 2 * RS + 4 + 2 * PB + 2 * OB;
     static constexpr int kSmem = oBar + kBars * 8 + 16 + 1024;  // + alignment of the base
-    static_assert(kSmem <= 227 * 1024 && kCols <= 512, "shared and tensor memory");
+    static_assert(kCtas * (kSmem + 1024) <= 228 * 1024 && kCols * kCtas <= 512, "shared and tensor memory");
 };
 
 // Swizzled byte offset of 16-byte chunk c of row r in a box of 128-, 64- or 32-byte rows.
@@ -104,20 +124,26 @@ template <int R> __device__ __forceinline__ uint64_t rope_desc(uint32_t addr) {
     return d;
 }
 
-__device__ __forceinline__ float warp_max_redux(float v) {
-    float r;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-    return r;
+// One lane of the warp (the same one every time). Inside a branch on it the compiler knows that a
+// single thread runs and keeps tcgen05.mma's descriptors in uniform registers; under lane == 0 it
+// goes through the possible lanes for every instruction (about 95 cycles each, measured here).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
 }
-// Barrier of the four softmax warps, with and without an OR of a predicate.
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ bool soft_any(bool p) {
+
+// Barrier of the four warps of a softmax group, with and without an OR of a predicate.
+__device__ __forceinline__ void soft_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory"); }
+__device__ __forceinline__ bool soft_any(int group, bool p) {
     uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
-        "bar.red.or.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        "bar.red.or.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(r)
-        : "r"(static_cast<uint32_t>(p))
+        : "r"(static_cast<uint32_t>(p)), "r"(group + 1)
         : "memory");
     return r != 0;
 }
@@ -134,101 +160,106 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) 
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// One work item.
-struct Item {
-    int q0, nq;       // query rows [q0, q0 + nq)
-    int row;          // cache row
-    int k0, nk, nt;   // first key, keys, 128-key tiles (0: nothing to attend)
-    int split;
-};
-
-template <int N> struct Walk {
-    const TcArgs& a;
-    const int* plan;  // shared: cumulative query blocks of the groups, or null
-    int items, per;   // query blocks per group (no plan) or per row (suffix)
-    __device__ Walk(const TcArgs& args, const int* pl) : a(args), plan(pl) {
-        const Problem& p = a.p;
-        const int th = p.T * p.H;
-        if (a.suffix) {
-            per = (th + N - 1) / N;
-            items = p.B * per * a.splits;
-        } else {
-            per = (p.max_group * th + N - 1) / N;
-            items = (plan ? plan[p.G] : p.G * per) * a.splits;
-        }
-    }
-    __device__ __forceinline__ Item get(int idx) const {
-        const Problem& p = a.p;
-        const int th = p.T * p.H;
-        Item it;
-        it.split = idx % a.splits;
-        const int blk = idx / a.splits;
-        int len;
-        if (a.suffix) {
-            it.row = blk / per;
-            const int s = (blk - it.row * per) * N;
-            it.q0 = it.row * th + s;
-            it.nq = min(N, th - s);
-            len = suffix_length(p, it.row);
-        } else {
-            int g, s;
-            if (plan) {
-                int lo = 0, hi = p.G;  // the group with plan[g] <= blk < plan[g + 1]
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (plan[mid] <= blk) lo = mid;
-                    else hi = mid;
+// Column reductions over the 32 lanes: each step folds half of the remaining columns into the
+// other half's lane (62 shuffles for 64 values). Returns the first column the lane ends up with;
+// its results are v[0] (and v[1] for 64 columns; 16 columns: both lanes of a pair hold it).
+template <int NC, class Op> __device__ __forceinline__ int fold_columns(float (&v)[NC], int lane, Op op) {
+    int own = 0, w = NC;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        if (w > 1) {
+            w >>= 1;
+            const bool up = lane & o;
+#pragma unroll
+            for (int i = 0; i < NC / 2; ++i)
+                if (i < w) {
+                    const float got = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + w], o);
+                    v[i] = op(up ? v[i + w] : v[i], got);
                 }
-                g = lo;
-                s = (blk - plan[g]) * N;
-            } else {
-                g = blk / per;
-                s = (blk - g * per) * N;
-            }
-            const int b0 = min(max(p.group_start[g], 0), p.B), b1 = min(max(p.group_start[g + 1], b0), p.B);
-            const int total = min(b1 - b0, p.max_group) * th;
-            it.row = g;
-            it.q0 = b0 * th + s;
-            it.nq = max(0, min(N, total - s));
-            len = it.nq > 0 ? prefix_length(p, g) : 0;
+            if (up) own += w;
+        } else {
+            v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
         }
-        it.k0 = it.split * a.kps;
-        it.nk = max(0, min(a.kps, len - it.k0));
-        it.nt = (it.nk + 127) / 128;
-        return it;
     }
-};
+    return own;
+}
 
-// Cursor over the tiles of a CTA's items that have any.
-template <int N> struct Cursor {
-    const Walk<N>& w;
-    int idx;
+// Item idx of the launch. plan (shared, prefix launches): cumulative query blocks of the
+// groups, or null when there are more groups than it holds.
+template <int N, int KT>
+__device__ __forceinline__ Item get_item(const TcArgs& a, const int* plan, int per, int idx) {
+    const Problem& p = a.p;
+    const int th = p.T * p.H;
     Item it;
-    int j;
-    __device__ Cursor(const Walk<N>& walk) : w(walk), idx(static_cast<int>(blockIdx.x) - static_cast<int>(gridDim.x)), j(0) {
-        next_item();
+    it.split = idx % a.splits;
+    const int blk = idx / a.splits;
+    int len;
+    it.np = 0;
+    if (a.suffix) {
+        it.row = blk / per;
+        const int s = (blk - it.row * per) * N;
+        it.q0 = it.row * th + s;
+        it.nq = min(N, th - s);
+        len = suffix_length(p, it.row);
+        if (a.merge) it.np = (prefix_length(p, p.G > 0 ? group_of(p, it.row) : -1) + a.prefix_kps - 1) / a.prefix_kps;
+    } else {
+        int g, s;
+        if (plan) {
+            int lo = 0, hi = p.G;  // the group with plan[g] <= blk < plan[g + 1]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (plan[mid] <= blk) lo = mid;
+                else hi = mid;
+            }
+            g = lo;
+            s = (blk - plan[g]) * N;
+        } else {
+            g = blk / per;
+            s = (blk - g * per) * N;
+        }
+        const int b0 = min(max(p.group_start[g], 0), p.B), b1 = min(max(p.group_start[g + 1], b0), p.B);
+        const int total = min(b1 - b0, p.max_group) * th;
+        it.row = g;
+        it.q0 = b0 * th + s;
+        it.nq = max(0, min(N, total - s));
+        len = it.nq > 0 ? prefix_length(p, g) : 0;
     }
+    it.k0 = it.split * a.kps;
+    it.nk = max(0, min(a.kps, len - it.k0));
+    it.nt = (it.nk + KT - 1) / KT;
+    return it;
+}
+
+// Cursor over the tiles of a table's items that have any.
+struct Cursor {
+    const Item* tab;
+    int n, at, j, nt;
+    __device__ __forceinline__ Cursor(const Item* t, int count) : tab(t), n(count), at(-1), j(0), nt(0) { next_item(); }
     __device__ __forceinline__ void next_item() {
         j = 0;
         do {
-            idx += gridDim.x;
-            if (idx >= w.items) return;
-            it = w.get(idx);
-        } while (it.nt == 0);
+            if (++at >= n) return;
+            nt = tab[at].nt;
+        } while (nt == 0);
     }
-    __device__ __forceinline__ bool valid() const { return idx < w.items; }
+    __device__ __forceinline__ bool valid() const { return at < n; }
+    __device__ __forceinline__ bool last() const { return j == nt - 1; }
+    __device__ __forceinline__ const Item& item() const { return tab[at]; }
     __device__ __forceinline__ void next() {
-        if (++j == it.nt) next_item();
+        if (++j == nt) next_item();
     }
 };
 
 template <int KV, int R, int N, typename T, bool Q8>
-__global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(const __grid_constant__ TcArgs a) {
+__global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N, Q8>::kCtas)
+    shared_prefix_tc_kernel(const __grid_constant__ TcArgs a) {
     using C = TcCfg<KV, R, N, Q8>;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    constexpr int NC = C::NC, KT = C::KT;
     extern __shared__ uint8_t tc_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
+    Item* table = reinterpret_cast<Item*>(smem + C::oTab);
     float* m_s = reinterpret_cast<float*>(smem + C::oF);
     float* corr_s = m_s + N;
     float* red_s = corr_s + N;  // [4][N]
@@ -241,24 +272,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(const _
     uint64_t* rope_full = pair_empty + C::PS;    // [RS] four producer warps (and the item's queries)
     uint64_t* rope_empty = rope_full + C::RS;    // [RS]
     uint64_t* s_full = rope_empty + C::RS;       // [2]
-    uint64_t* s_free = s_full + 2;               // [2] four softmax warps
-    uint64_t* p_full = s_free + 2;               // [PB] four softmax warps
+    uint64_t* s_free = s_full + 2;               // [2] the softmax warps
+    uint64_t* p_full = s_free + 2;               // [PB] the softmax warps
     uint64_t* p_free = p_full + C::PB;           // [PB] the tile's O products are complete
     uint64_t* o_full = p_free + C::PB;           // [OB]
-    uint64_t* o_free = o_full + C::OB;           // [OB] four softmax warps
+    uint64_t* o_free = o_full + C::OB;           // [OB] the softmax warps
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
     int* bad_s = reinterpret_cast<int*>(tmem_slot + 1);
     const Problem& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int th = p.T * p.H;
+    constexpr int kMmaWarp = C::SW + 4;
 
-    if (warp == 8) {
+    if (warp == kMmaWarp) {
         if (lane == 0) {
             for (int i = 0; i < C::QB; ++i) mbar_init(&q_empty[i], 1);
             for (int i = 0; i < C::PS; ++i) { mbar_init(&pair_full[i], 4); mbar_init(&pair_empty[i], 1); }
             for (int i = 0; i < C::RS; ++i) { mbar_init(&rope_full[i], 4); mbar_init(&rope_empty[i], 1); }
-            for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); }
-            for (int i = 0; i < C::PB; ++i) { mbar_init(&p_full[i], 4); mbar_init(&p_free[i], 1); }
-            for (int i = 0; i < C::OB; ++i) { mbar_init(&o_full[i], 1); mbar_init(&o_free[i], 4); }
+            for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_free[i], C::SW); }
+            for (int i = 0; i < C::PB; ++i) { mbar_init(&p_full[i], C::SW); mbar_init(&p_free[i], 1); }
+            for (int i = 0; i < C::OB; ++i) { mbar_init(&o_full[i], 1); mbar_init(&o_free[i], C::SW); }
             *bad_s = 0;
             fence_mbar_init();
         }
@@ -266,35 +299,51 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(const _
         tmem_alloc(tmem_slot, C::kTmem);
         tmem_relinquish();
     }
-    MM_PDL_ENTRY();
-    // plan: cumulative query blocks of the groups
-    const bool planned = !a.suffix && p.G <= kTcMaxPlan;
-    if (planned) {
-        for (int g = tid; g < p.G; g += kTcThreads) {
-            const int b0 = min(max(p.group_start[g], 0), p.B), b1 = min(max(p.group_start[g + 1], b0), p.B);
-            plan_s[g + 1] = (min(b1 - b0, p.max_group) * p.T * p.H + N - 1) / N;
-        }
-        __syncthreads();
-        if (warp == 0) {
-            int base = 0;
-            for (int g0 = 0; g0 < p.G; g0 += 32) {
-                int v = g0 + lane < p.G ? plan_s[g0 + lane + 1] : 0;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int u = __shfl_up_sync(0xffffffffu, v, o);
-                    if (lane >= o) v += u;
-                }
-                if (g0 + lane < p.G) plan_s[g0 + lane + 1] = base + v;
-                base += __shfl_sync(0xffffffffu, v, 31);
+    // Beside its own prefix launch a suffix launch starts at once: that launch lets its dependents
+    // begin only after it has itself waited for everything before it. Its partials are waited for
+    // where they are read.
+    if (!a.overlap) pdl_wait();
+    pdl_launch_dependents();
+    int per, items;
+    const int* plan = nullptr;
+    if (a.suffix) {
+        per = (th + N - 1) / N;
+        items = p.B * per * a.splits;
+    } else {
+        per = (p.max_group * th + N - 1) / N;
+        if (p.G <= kTcMaxPlan) {
+            // cumulative query blocks of the groups
+            plan = plan_s;
+            for (int g = tid; g < p.G; g += C::kThreads) {
+                const int b0 = min(max(p.group_start[g], 0), p.B), b1 = min(max(p.group_start[g + 1], b0), p.B);
+                plan_s[g + 1] = (min(b1 - b0, p.max_group) * th + N - 1) / N;
             }
-            if (lane == 0) plan_s[0] = 0;
+            __syncthreads();
+            if (warp == 0) {
+                int base = 0;
+                for (int g0 = 0; g0 < p.G; g0 += 32) {
+                    int v = g0 + lane < p.G ? plan_s[g0 + lane + 1] : 0;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int u = __shfl_up_sync(0xffffffffu, v, o);
+                        if (lane >= o) v += u;
+                    }
+                    if (g0 + lane < p.G) plan_s[g0 + lane + 1] = base + v;
+                    base += __shfl_sync(0xffffffffu, v, 31);
+                }
+                if (lane == 0) plan_s[0] = 0;
+            }
+            __syncthreads();
+            items = plan_s[p.G] * a.splits;
+        } else {
+            items = p.G * per * a.splits;
         }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const Walk<N> walk(a, planned ? plan_s : nullptr);
+    const int mine = blockIdx.x < items ? (items - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
     const lat::CacheView& cv = a.suffix ? p.suffix : p.prefix;
     bool ok = true;
     // a wait that ran out is recorded once; later waits of this thread are skipped
@@ -304,51 +353,59 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(const _
             *reinterpret_cast<volatile int*>(bad_s) = 1;
         }
     };
+    // The next table of this CTA's items; every thread of the CTA comes here for each table.
+    auto next_table = [&](int base) {
+        if (base > 0) __syncthreads();
+        if (tid < kTcTable && base + tid < mine)
+            table[tid] = get_item<N, KT>(a, plan, per, blockIdx.x + (base + tid) * gridDim.x);
+        __syncthreads();
+        return min(kTcTable, mine - base);
+    };
 
-    if (warp >= 4 && warp < 8) {
+    if (warp >= C::SW && warp < kMmaWarp) {
         // ------------------------------------------------------------ producers
-        const int pt = tid - 128;  // 0..127
+        if constexpr (Q8 && N == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        const int pt = tid - 32 * C::SW;  // 0..127
         uint8_t* sQ = smem + C::oQ;
         uint8_t* sPair = smem + C::oPair;
         uint8_t* sRope = smem + C::oRope;
-        const int th = p.T * p.H;
+        // eight lanes per query row and 64-column box
         auto load_q = [&](const Item& it, int qb) {
             uint8_t* q = sQ + qb * C::kQA;
-            constexpr int kChunks = (KV + R) / 8;
-            for (int e = pt; e < N * kChunks; e += 128) {
-                const int n = e / kChunks, c = e - n * kChunks;
+            const int c = pt & 7;
+#pragma unroll 1
+            for (int n = pt >> 3; n < N; n += 16) {
                 const bool in = n < it.nq;
                 const int r = it.q0 + (in ? n : 0), b = r / th, u = r - b * th, t = u / p.H, h = u - t * p.H;
                 const T* src = static_cast<const T*>(p.q) + b * p.q_row + t * p.q_tok + h * p.q_head + c * 8;
-                uint8_t* dst = c < KV / 8 ? q + (c >> 3) * C::kQBox + sw128(n, c & 7)
-                                          : q + 2 * C::NP * C::kQBox + sw_rope<R>(n, c - KV / 8);
-                cp_async16(dst, src, in);
+                uint8_t* dst = q + sw128(n, c);
+#pragma unroll
+                for (int x = 0; x < 2 * C::NP; ++x) cp_async16(dst + x * C::kQBox, src + x * 64, in);
+                if (c < R / 8) cp_async16(q + 2 * C::NP * C::kQBox + sw_rope<R>(n, c), src + KV, in);
             }
         };
         auto load_rope = [&](const Item& it, int j, int slot) {
-            constexpr int kChunks = R / 8;
+            constexpr int kChunks = R / 8, kRows = 128 / kChunks;
+            const int c = pt % kChunks, r0 = pt / kChunks, left = it.nk - j * KT;
             uint8_t* d = sRope + slot * C::kRopeA;
-            const uint8_t* base = Q8 ? cv.rope + 2 * (it.row * cv.rope_row_stride)
-                                     : cv.latent + 2 * (it.row * cv.row_stride + KV);
-            const long long ps = Q8 ? cv.rope_pos_stride : cv.pos_stride;
+            const long long ps = 2 * (Q8 ? cv.rope_pos_stride : cv.pos_stride);
+            const uint8_t* src = (Q8 ? cv.rope + 2 * (it.row * cv.rope_row_stride)
+                                     : cv.latent + 2 * (it.row * cv.row_stride + KV)) + (it.k0 + j * KT) * ps + c * 16;
 #pragma unroll
-            for (int i = 0; i < kChunks; ++i) {
-                const int e = pt + 128 * i, r = e / kChunks, c = e - r * kChunks;
-                const bool in = j * 128 + r < it.nk;
-                cp_async16(d + sw_rope<R>(r, c), base + 2 * ((it.k0 + (in ? j * 128 + r : 0)) * ps) + c * 16, in);
-            }
+            for (int r = r0; r < KT; r += kRows) cp_async16(d + sw_rope<R>(r, c), src + (r < left ? r : 0) * ps, r < left);
         };
         auto arrive_full = [&](uint64_t* bar) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
+        int qi = -1, tile = 0, pr = 0;
         if constexpr (!Q8) {
             // units in order per tile: rope (the item's queries with its first), pair 0, 1, ...
             // Each is one cp.async group; a unit is announced once later groups are in flight, or
             // all at once before the warp would block on a full ring.
             int issued = 0, told = 0;
-            constexpr int kFlight = C::PS;
+            constexpr int kFlight = C::PS < 6 ? C::PS : 6;
             auto bar_of = [&](int u) {
                 const int t = u / (C::NP + 1), s = u - t * (C::NP + 1);
                 return s == 0 ? &rope_full[t % C::RS] : &pair_full[(t * C::NP + s - 1) % C::PS];
@@ -369,464 +426,503 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_prefix_tc_kernel(const _
                     wait(bar, parity);
                 }
             };
-            int qi = -1, tile = 0, pr = 0;
-            for (Cursor<N> c(walk); c.valid(); c.next(), ++tile) {
-                room(&rope_empty[tile % C::RS], ((tile / C::RS) & 1) ^ 1);
-                if (c.j == 0) {
-                    ++qi;
-                    room(&q_empty[qi % C::QB], ((qi / C::QB) & 1) ^ 1);
-                    load_q(c.it, qi % C::QB);
-                }
-                load_rope(c.it, c.j, tile % C::RS);
-                cp_async_commit();
-                ++issued;
-#pragma unroll 1
-                for (int i = 0; i < C::NP; ++i, ++pr) {
-                    const int slot = pr % C::PS;
-                    room(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
-                    uint8_t* d = sPair + slot * C::kPair;
-                    const int cc = pt & 15, r0 = pt >> 4;
-                    const uint8_t* base = cv.latent + 2 * (c.it.row * cv.row_stride + i * 128 + cc * 8);
-                    d += (cc >> 3) * C::kBox;
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const int r = r0 + 8 * k;
-                        const bool in = c.j * 128 + r < c.it.nk;
-                        cp_async16(d + sw128(r, cc & 7), base + 2 * ((c.it.k0 + (in ? c.j * 128 + r : 0)) * cv.pos_stride), in);
+            const int cc = pt & 15, r0 = pt >> 4;  // 16-byte chunk of the pair's row, first row
+            const long long ps = 2 * cv.pos_stride;
+            for (int base = 0; base < mine; base += kTcTable) {
+                const int count = next_table(base);
+                for (Cursor c(table, count); c.valid(); c.next(), ++tile) {
+                    const Item& it = c.item();
+                    room(&rope_empty[tile % C::RS], ((tile / C::RS) & 1) ^ 1);
+                    if (c.j == 0) {
+                        ++qi;
+                        room(&q_empty[qi % C::QB], ((qi / C::QB) & 1) ^ 1);
+                        load_q(it, qi % C::QB);
                     }
+                    load_rope(it, c.j, tile % C::RS);
                     cp_async_commit();
                     ++issued;
-                    cp_async_wait<kFlight - 1>();
-                    tell_to(issued - (kFlight - 1));
-                }
-            }
-            cp_async_wait<0>();
-            tell_to(issued);
-        } else {
-            // codes four pairs ahead in registers: 8 x 16 bytes of a pair per thread
-            constexpr int D = 4;
-            uint4 v[D][8];
-            const int cc = pt & 7, r0 = pt >> 3;  // 16-byte chunk of the pair's 128 codes, first row
-            auto fetch = [&](uint4 (&x)[8], const Item& it, int j, int i) {
-                const uint8_t* base = cv.latent + it.row * cv.row_stride + i * 128 + cc * 16;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int r = r0 + 16 * k;
-                    x[k] = j * 128 + r < it.nk
-                               ? __ldg(reinterpret_cast<const uint4*>(base + (it.k0 + j * 128 + r) * cv.pos_stride))
-                               : make_uint4(0, 0, 0, 0);
-                }
-            };
-            Cursor<N> lc(walk), sc(walk);
-            int li = 0, si = 0;  // pair of the tile each cursor is at
-            auto step = [&](Cursor<N>& c, int& i) {
-                if (++i == C::NP) {
-                    i = 0;
-                    c.next();
-                }
-            };
-#pragma unroll
-            for (int d = 0; d < D; ++d)
-                if (lc.valid()) {
-                    fetch(v[d], lc.it, lc.j, li);
-                    step(lc, li);
-                }
-            int qi = -1, tile = 0, pr = 0;
-            while (sc.valid()) {
-#pragma unroll
-                for (int d = 0; d < D; ++d) {
-                    if (sc.valid()) {
-                        if (si == 0) {
-                            wait(&rope_empty[tile % C::RS], ((tile / C::RS) & 1) ^ 1);
-                            if (sc.j == 0) {
-                                ++qi;
-                                wait(&q_empty[qi % C::QB], ((qi / C::QB) & 1) ^ 1);
-                                load_q(sc.it, qi % C::QB);
-                            }
-                            load_rope(sc.it, sc.j, tile % C::RS);
-                            cp_async_commit();
-                        }
+                    const int left = it.nk - c.j * KT;
+                    const uint8_t* src = cv.latent + 2 * (it.row * cv.row_stride) + (it.k0 + c.j * KT) * ps + cc * 16;
+#pragma unroll 1
+                    for (int i = 0; i < C::NP; ++i, ++pr, src += 256) {
                         const int slot = pr % C::PS;
-                        wait(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
-                        uint8_t* dst = sPair + slot * C::kPair + (cc >> 2) * C::kBox;
+                        room(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
+                        uint8_t* d = sPair + slot * C::kPair + (cc >> 3) * C::kBox + sw128(r0, cc & 7);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const int r = r0 + 16 * k;
-                            const uint32_t w[4] = {v[d][k].x, v[d][k].y, v[d][k].z, v[d][k].w};
-                            uint32_t o[8];
+                        for (int k = 0; k < KT / 8; ++k) {  // rows 8 apart: the same swizzle phase
+                            const int r = r0 + 8 * k;
+                            cp_async16(d + k * 1024, src + (r < left ? r : 0) * ps, r < left);
+                        }
+                        cp_async_commit();
+                        ++issued;
+                        cp_async_wait<kFlight - 1>();
+                        tell_to(issued - (kFlight - 1));
+                    }
+                }
+                cp_async_wait<0>();
+                tell_to(issued);
+            }
+        } else {
+            // codes D pairs ahead in registers: VPT x 16 bytes of a pair per thread
+            constexpr int D = C::D;
+            uint4 v[D][C::VPT];
+            const int cc = pt & 7, r0 = pt >> 3;  // 16-byte chunk of the pair's 128 codes, first row
+            auto fetch = [&](uint4 (&x)[C::VPT], const Item& it, int j, int i) {
+                const int left = it.nk - j * KT - r0;
+                const uint8_t* src = cv.latent + it.row * cv.row_stride + (it.k0 + j * KT + r0) * cv.pos_stride + i * 128 + cc * 16;
+                const long long step = 16 * cv.pos_stride;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                o[2 * e] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] & 0xffff));
-                                o[2 * e + 1] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] >> 16));
+                for (int k = 0; k < C::VPT; ++k)
+                    x[k] = 16 * k < left ? __ldg(reinterpret_cast<const uint4*>(src + k * step)) : make_uint4(0, 0, 0, 0);
+            };
+            for (int base = 0; base < mine; base += kTcTable) {
+                const int count = next_table(base);
+                Cursor lc(table, count), sc(table, count);
+                int li = 0, si = 0;  // pair of the tile each cursor is at
+                auto step = [&](Cursor& c, int& i) {
+                    if (++i == C::NP) {
+                        i = 0;
+                        c.next();
+                    }
+                };
+#pragma unroll
+                for (int d = 0; d < D; ++d)
+                    if (lc.valid()) {
+                        fetch(v[d], lc.item(), lc.j, li);
+                        step(lc, li);
+                    }
+                while (sc.valid()) {
+#pragma unroll
+                    for (int d = 0; d < D; ++d) {
+                        if (sc.valid()) {
+                            if (si == 0) {
+                                wait(&rope_empty[tile % C::RS], ((tile / C::RS) & 1) ^ 1);
+                                if (sc.j == 0) {
+                                    ++qi;
+                                    wait(&q_empty[qi % C::QB], ((qi / C::QB) & 1) ^ 1);
+                                    load_q(sc.item(), qi % C::QB);
+                                }
+                                load_rope(sc.item(), sc.j, tile % C::RS);
+                                cp_async_commit();
                             }
-                            *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc) & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
-                            *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc + 1) & 7)) = make_uint4(o[4], o[5], o[6], o[7]);
+                            const int slot = pr % C::PS;
+                            wait(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
+                            uint8_t* dst = sPair + slot * C::kPair + (cc >> 2) * C::kBox;
+#pragma unroll
+                            for (int k = 0; k < C::VPT; ++k) {
+                                const int r = r0 + 16 * k;
+                                const uint32_t w[4] = {v[d][k].x, v[d][k].y, v[d][k].z, v[d][k].w};
+                                uint32_t o[8];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    o[2 * e] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] & 0xffff));
+                                    o[2 * e + 1] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] >> 16));
+                                }
+                                *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc) & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+                                *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc + 1) & 7)) =
+                                    make_uint4(o[4], o[5], o[6], o[7]);
+                            }
+                            if (lc.valid()) {
+                                fetch(v[d], lc.item(), lc.j, li);
+                                step(lc, li);
+                            }
+                            if (si == 0) {
+                                cp_async_wait<0>();
+                                arrive_full(&rope_full[tile % C::RS]);
+                            }
+                            arrive_full(&pair_full[slot]);
+                            ++pr;
+                            if (si == C::NP - 1) ++tile;
+                            step(sc, si);
                         }
-                        if (lc.valid()) {
-                            fetch(v[d], lc.it, lc.j, li);
-                            step(lc, li);
-                        }
-                        if (si == 0) {
-                            cp_async_wait<0>();
-                            arrive_full(&rope_full[tile % C::RS]);
-                        }
-                        arrive_full(&pair_full[slot]);
-                        ++pr;
-                        if (si == C::NP - 1) ++tile;
-                        step(sc, si);
                     }
                 }
             }
             cp_async_wait<0>();
         }
-    } else if (warp >= 8) {
+    } else if (warp >= kMmaWarp) {
         // ------------------------------------------------------------ tensor-core products
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        if (warp == 8 && lane == 0) {
-            const uint32_t id_s = umma_idesc_f16(kBf16, false, false, 128, N);
-            const uint32_t id_o = umma_idesc_f16(kBf16, true, N == 64, 128, N);
-            const uint32_t aPair = smem_u32(smem + C::oPair), aQ = smem_u32(smem + C::oQ), aR = smem_u32(smem + C::oRope),
-                           aP = smem_u32(smem + C::oP);
-            int s_tile = 0, s_pr = 0, s_q = 0;    // S products: tile, pair and item counters
-            int o_tile = 0, o_pr = 0, o_item = 0;  // O products
-            auto issue_s = [&](const Cursor<N>& c) {
-                const uint32_t q = aQ + (s_q % C::QB) * C::kQA;
-                const int sb = s_tile & 1;
-                const uint32_t d = tmem + C::kColS + sb * N;
-                wait(&s_free[sb], ((s_tile >> 1) & 1) ^ 1);
-                const int rs = s_tile % C::RS;
-                wait(&rope_full[rs], (s_tile / C::RS) & 1);
-                tc_fence_after();
+        if constexpr (Q8 && N == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        const uint32_t id_s = umma_idesc_f16(kBf16, false, false, 128, N);
+        const uint32_t id_o = umma_idesc_f16(kBf16, true, N == 64, 128, N);
+        const uint32_t aPair = smem_u32(smem + C::oPair), aQ = smem_u32(smem + C::oQ), aR = smem_u32(smem + C::oRope),
+                       aP = smem_u32(smem + C::oP);
+        // descriptors advance by address / 16 (shared memory ends below 2^18, so no field overflows)
+        const uint64_t kd = umma_desc_sw128(aPair, 16, 1024), vd = umma_desc_sw128(aPair, C::kBox, 1024);
+        int s_tile = 0, s_pr = 0, s_q = 0;     // S products: tile, pair and item counters
+        int o_tile = 0, o_pr = 0, o_item = 0;  // O products
+        auto issue_s = [&](const Cursor& c) {
+            const uint32_t q = aQ + (s_q % C::QB) * C::kQA;
+            const uint64_t qd = umma_desc_sw128(q, 16, 1024);
+            const int sb = s_tile & 1;
+            const uint32_t d = tmem + C::kColS + sb * N;
+            wait(&s_free[sb], ((s_tile >> 1) & 1) ^ 1);
+            const int rs = s_tile % C::RS;
+            wait(&rope_full[rs], (s_tile / C::RS) & 1);
+            tc_fence_after();
+            {
+                const uint64_t ka = rope_desc<R>(aR + rs * C::kRopeA), qa = rope_desc<R>(q + 2 * C::NP * C::kQBox);
+                const uint32_t dr = Q8 ? tmem + C::kColR + sb * N : d;
 #pragma unroll
-                for (int k = 0; k < R / 16; ++k)
-                    tc_mma_f16(Q8 ? tmem + C::kColR + sb * N : d, rope_desc<R>(aR + rs * C::kRopeA + k * 32),
-                               rope_desc<R>(q + 2 * C::NP * C::kQBox + k * 32), id_s, k ? 1u : 0u);
-                tc_commit(&rope_empty[rs]);
+                for (int k = 0; k < R / 16; ++k) tc_mma_f16(dr, ka + k * 2, qa + k * 2, id_s, k ? 1u : 0u);
+            }
+            tc_commit(&rope_empty[rs]);
 #pragma unroll 1
-                for (int i = 0; i < C::NP; ++i, ++s_pr) {
-                    const int slot = s_pr % C::PS;
-                    wait(&pair_full[slot], (s_pr / C::PS) & 1);
-                    tc_fence_after();
-                    const uint32_t ka = aPair + slot * C::kPair, qa = q + 2 * i * C::kQBox;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        tc_mma_f16(d, umma_desc_sw128(ka + (k >> 2) * C::kBox + (k & 3) * 32, 16, 1024),
-                                   umma_desc_sw128(qa + (k >> 2) * C::kQBox + (k & 3) * 32, 16, 1024), id_s,
-                                   Q8 ? ((i | k) ? 1u : 0u) : 1u);
-                }
-                tc_commit(&s_full[sb]);
-                if (c.j == c.it.nt - 1) {
-                    tc_commit(&q_empty[s_q % C::QB]);
-                    ++s_q;
-                }
-                ++s_tile;
-            };
-            auto issue_o = [&](const Cursor<N>& c) {
-                const int ob = o_item % C::OB, pb = o_tile % C::PB;
-                if (c.j == 0) wait(&o_free[ob], ((o_item / C::OB) & 1) ^ 1);
-                wait(&p_full[pb], (o_tile / C::PB) & 1);
+            for (int i = 0; i < C::NP; ++i, ++s_pr) {
+                const int slot = s_pr % C::PS;
+                wait(&pair_full[slot], (s_pr / C::PS) & 1);
                 tc_fence_after();
-                const uint32_t pa = aP + pb * C::kP;
-#pragma unroll 1
-                for (int i = 0; i < C::NP; ++i, ++o_pr) {
-                    const int slot = o_pr % C::PS;
-                    const uint32_t va = aPair + slot * C::kPair;
-                    const uint32_t d = tmem + C::kColO + (ob * C::NP + i) * N;
+                const uint64_t ka = kd + static_cast<uint32_t>(slot * (C::kPair >> 4));
+                const uint64_t qa = qd + static_cast<uint32_t>(i * (2 * C::kQBox >> 4));
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        // V^T MN-major: 16 keys = 2,048 B down a box, the next 64 columns one box on
-                        const uint64_t bd = N == 64 ? umma_desc_sw128(pa + k * 2048, C::kBox, 1024)
-                                                    : umma_desc_sw128(pa + (k >> 2) * 2048 + (k & 3) * 32, 16, 1024);
-                        tc_mma_f16(d, umma_desc_sw128(va + k * 2048, C::kBox, 1024), bd, id_o, (c.j | k) ? 1u : 0u);
-                    }
-                    tc_commit(&pair_empty[slot]);
-                }
-                tc_commit(&p_free[pb]);
-                if (c.j == c.it.nt - 1) {
-                    tc_commit(&o_full[ob]);
-                    ++o_item;
-                }
-                ++o_tile;
-            };
-            Cursor<N> cs(walk), co(walk);
-            if (C::kAhead) {
-                if (cs.valid()) {
-                    issue_s(cs);
-                    cs.next();
-                }
-                for (; co.valid(); co.next()) {
+                for (int k = 0; k < 8; ++k)
+                    tc_mma_f16(d, ka + ((k >> 2) * C::kBox + (k & 3) * 32) / 16, qa + ((k >> 2) * C::kQBox + (k & 3) * 32) / 16,
+                               id_s, Q8 ? ((i | k) ? 1u : 0u) : 1u);
+            }
+            tc_commit(&s_full[sb]);
+            if (c.last()) {
+                tc_commit(&q_empty[s_q % C::QB]);
+                ++s_q;
+            }
+            ++s_tile;
+        };
+        auto issue_o = [&](const Cursor& c) {
+            const int ob = o_item % C::OB, pb = o_tile % C::PB;
+            if (c.j == 0) wait(&o_free[ob], ((o_item / C::OB) & 1) ^ 1);
+            wait(&p_full[pb], (o_tile / C::PB) & 1);
+            tc_fence_after();
+            const uint64_t pa = umma_desc_sw128(aP + pb * C::kP, N == 64 ? C::kBox : 16, 1024);
+#pragma unroll 1
+            for (int i = 0; i < C::NP; ++i, ++o_pr) {
+                const int slot = o_pr % C::PS;
+                const uint64_t va = vd + static_cast<uint32_t>(slot * (C::kPair >> 4));
+                const uint32_t d = tmem + C::kColO + (ob * C::NP + i) * N;
+#pragma unroll
+                for (int k = 0; k < KT / 16; ++k)
+                    // V^T MN-major: 16 keys = 2,048 B down a box, the next 64 columns one box on
+                    tc_mma_f16(d, va + k * 128, pa + (N == 64 ? k * 128 : ((k >> 2) * 2048 + (k & 3) * 32) / 16), id_o,
+                               (c.j | k) ? 1u : 0u);
+                tc_commit(&pair_empty[slot]);
+            }
+            tc_commit(&p_free[pb]);
+            if (c.last()) {
+                tc_commit(&o_full[ob]);
+                ++o_item;
+            }
+            ++o_tile;
+        };
+        for (int base = 0; base < mine; base += kTcTable) {
+            const int count = next_table(base);
+            if (warp == kMmaWarp && elect_one()) {
+                Cursor cs(table, count), co(table, count);
+                if (C::kAhead) {
                     if (cs.valid()) {
                         issue_s(cs);
                         cs.next();
                     }
-                    issue_o(co);
-                }
-            } else {
-                for (; co.valid(); co.next()) {
-                    issue_s(co);
-                    issue_o(co);
+                    for (; co.valid(); co.next()) {
+                        if (cs.valid()) {
+                            issue_s(cs);
+                            cs.next();
+                        }
+                        issue_o(co);
+                    }
+                } else {
+                    for (; co.valid(); co.next()) {
+                        issue_s(co);
+                        issue_o(co);
+                    }
                 }
             }
+            __syncwarp();
         }
-        __syncwarp();
     } else {
         // ------------------------------------------------------------ softmax and results
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-        const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+        const int group = warp >> 2, gw = warp & 3, gt = tid & 127;  // gt: key of the tile, TMEM lane
+        const int c0 = group * NC;                                   // first query column of the group
+        const bool live = gw * 32 < KT;                              // the warp's lanes hold keys
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>(gw * 32) << 16);
         const float cs = p.scale * 1.4426950408889634f;
-        const int th = p.T * p.H;
         const long long rows = static_cast<long long>(p.B) * th;
+        const float* m_c = m_s + c0;
         int tile = 0, item = 0;
-        for (int idx = blockIdx.x; idx < walk.items; idx += gridDim.x) {
-            const Item it = walk.get(idx);
-            if (it.nt == 0 && !a.merge) continue;
-            if (it.nq == 0) continue;
-            float l[N];
+        bool waited = !a.overlap;
+        for (int base = 0; base < mine; base += kTcTable) {
+            const int count = next_table(base);
+            for (int e0 = 0; e0 < count; ++e0) {
+                const Item it = table[e0];
+                if (it.nt == 0 && !a.merge) continue;
+                float l[NC];
 #pragma unroll
-            for (int n = 0; n < N; ++n) l[n] = 0.f;
-            // keys of the item each query sees; the tokens of a suffix end one position apart
-            const bool causal = a.suffix && p.T > 1;
-            soft_sync();  // the previous item's readers of m_s, lim_s and red_s are done
-            if (tid < N) {
-                m_s[tid] = kNoMax;
-                int lim = it.nk;
-                if (causal) {
-                    const int t = min((it.q0 + tid - it.row * th) / p.H, p.T - 1);
-                    lim = min(it.nk, suffix_length(p, it.row) - (p.T - 1 - t) - it.k0);
+                for (int n = 0; n < NC; ++n) l[n] = 0.f;
+                // keys of the item each query sees; the tokens of a suffix end one position apart
+                const bool causal = a.suffix && p.T > 1;
+                soft_sync(group);  // the previous item's readers of m_s, lim_s and red_s are done
+                if (gt < NC) {
+                    m_s[c0 + gt] = kNoMax;
+                    if (causal) {
+                        const int t = min((it.q0 + c0 + gt - it.row * th) / p.H, p.T - 1);
+                        lim_s[c0 + gt] = min(it.nk, suffix_length(p, it.row) - (p.T - 1 - t) - it.k0);
+                    }
                 }
-                lim_s[tid] = lim;
-            }
-            soft_sync();
-            const int lim_min = causal ? it.nk - (p.T - 1) : it.nk;
-            const float* ks_row = Q8 ? cv.scale + it.row * cv.scale_row_stride + it.k0 : nullptr;
-            for (int j = 0; j < it.nt; ++j, ++tile) {
-                const int key = j * 128 + warp * 32 + lane;
-                const float ks = Q8 && key < it.nk ? __ldg(ks_row + key) : 1.f;
-                const int sb = tile & 1;
-                wait(&s_full[sb], (tile >> 1) & 1);
-                tc_fence_after();
-                float z[N];
-                if constexpr (N == 64) {
-                    tmem_ld32_nowait(lane_base + C::kColS + sb * N, z);
-                    tmem_ld32_nowait(lane_base + C::kColS + sb * N + 32, z + 32);
-                    tmem_wait_ld();
+                soft_sync(group);
+                const int lim_min = causal ? it.nk - (p.T - 1) : it.nk;
+                const float* ks_row = Q8 ? cv.scale + it.row * cv.scale_row_stride + it.k0 : nullptr;
+                float ks_next = 1.f;
+                if (Q8 && live && gt < it.nk) ks_next = __ldg(ks_row + gt);
+                for (int j = 0; j < it.nt; ++j, ++tile) {
+                    const int key = j * KT + gt;
+                    const float ks = ks_next;
+                    if (Q8) ks_next = live && key + KT < it.nk ? __ldg(ks_row + key + KT) : 1.f;
+                    const int sb = tile & 1;
+                    wait(&s_full[sb], (tile >> 1) & 1);
+                    tc_fence_after();
+                    float z[NC];
+                    if (live) {
+                        if constexpr (NC == 32) {
+                            tmem_ld32_nowait(lane_base + C::kColS + sb * N + c0, z);
+                            tmem_wait_ld();
+                        } else {
+                            tmem_ld16(lane_base + C::kColS + sb * N, z);
+                        }
+                        if constexpr (Q8) {
+#pragma unroll
+                            for (int n = 0; n < NC; n += 16) {
+                                float r[16];
+                                tmem_ld16(lane_base + C::kColR + sb * N + c0 + n, r);
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) z[n + e] = fmaf(z[n + e], ks, r[e]);
+                            }
+                        }
+                        tc_fence_before();
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_free[sb]);
+                    bool over = false;
+                    if (live) {
+                        if ((j + 1) * KT > lim_min) {  // the last tile(s): keys past a query's limit
+                            if (causal) {
+#pragma unroll
+                                for (int n = 0; n < NC; ++n) z[n] = key < lim_s[c0 + n] ? z[n] * cs : -INFINITY;
+                            } else {
+#pragma unroll
+                                for (int n = 0; n < NC; ++n) z[n] = key < it.nk ? z[n] * cs : -INFINITY;
+                            }
+                        } else {
+#pragma unroll
+                            for (int n = 0; n < NC; ++n) z[n] *= cs;
+                        }
+#pragma unroll
+                        for (int n = 0; n < NC; n += 4) {
+                            const float4 m = *reinterpret_cast<const float4*>(m_c + n);
+                            over |= z[n] > m.x + 8.f;
+                            over |= z[n + 1] > m.y + 8.f;
+                            over |= z[n + 2] > m.z + 8.f;
+                            over |= z[n + 3] > m.w + 8.f;
+                        }
+                    }
+                    if (soft_any(group, over)) {
+                        if (live) {
+                            float x[NC];
+#pragma unroll
+                            for (int n = 0; n < NC; ++n) x[n] = z[n];
+                            const int own = fold_columns(x, lane, [](float u, float w) { return fmaxf(u, w); });
+                            if (NC == 32 || (lane & 1) == 0) red_s[gw * N + c0 + own] = x[0];
+                        }
+                        soft_sync(group);
+                        if (gt < NC) {
+                            const int n = c0 + gt;
+                            float mt = fmaxf(red_s[n], red_s[N + n]);
+                            if (KT == 128) mt = fmaxf(mt, fmaxf(red_s[2 * N + n], red_s[3 * N + n]));
+                            const float mo = m_s[n], mn = mt > mo + 8.f ? mt : mo;
+                            corr_s[n] = fast_exp2(mo - mn);
+                            m_s[n] = mn;
+                        }
+                        soft_sync(group);
+#pragma unroll
+                        for (int n = 0; n < NC; ++n) l[n] *= corr_s[c0 + n];
+                        if (j > 0) {
+                            // the previous tile's products have landed: rescale the accumulator
+                            const int pt = tile - 1;
+                            wait(&p_free[pt % C::PB], (pt / C::PB) & 1);
+                            tc_fence_after();
+                            const uint32_t o = lane_base + C::kColO + (item % C::OB) * C::NP * N + c0;
+#pragma unroll 1
+                            for (int i = 0; i < C::NP; ++i)
+#pragma unroll 1
+                                for (int c = 0; c < NC; c += 16) {
+                                    float v[16];
+                                    tmem_ld16(o + i * N + c, v);
+#pragma unroll
+                                    for (int e = 0; e < 16; ++e) v[e] *= corr_s[c0 + c + e];
+                                    tmem_st16(o + i * N + c, v);
+                                }
+                            tmem_wait_st();
+                        }
+                    }
+                    const int pb = tile % C::PB;
+                    wait(&p_free[pb], ((tile / C::PB) & 1) ^ 1);
+                    if (live) {
+                        uint8_t* P = smem + C::oP + pb * C::kP;
+#pragma unroll
+                        for (int n0 = 0; n0 < NC; n0 += 8) {
+                            float e[8];
+#pragma unroll
+                            for (int q = 0; q < 8; q += 4) {
+                                const float4 m = *reinterpret_cast<const float4*>(m_c + n0 + q);
+                                e[q] = fast_exp2(z[n0 + q] - m.x);
+                                e[q + 1] = fast_exp2(z[n0 + q + 1] - m.y);
+                                e[q + 2] = fast_exp2(z[n0 + q + 2] - m.z);
+                                e[q + 3] = fast_exp2(z[n0 + q + 3] - m.w);
+                            }
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) {
+                                l[n0 + q] += e[q];
+                                if (Q8) e[q] *= ks;
+                            }
+                            if constexpr (N == 64) {
+                                *reinterpret_cast<uint4*>(P + sw128(gt, (c0 + n0) >> 3)) =
+                                    make_uint4(lat::pack2<T>(e[0], e[1]), lat::pack2<T>(e[2], e[3]),
+                                               lat::pack2<T>(e[4], e[5]), lat::pack2<T>(e[6], e[7]));
+                            } else {
+                                // K-major: query row n, key gt of the 64-key box gt / 64
+#pragma unroll
+                                for (int q = 0; q < 8; ++q)
+                                    *reinterpret_cast<T*>(P + (gt >> 6) * 2048 + sw128(n0 + q, (gt & 63) >> 3) + (gt & 7) * 2) =
+                                        lat::from_f32<T>(e[q]);
+                            }
+                        }
+                        fence_proxy_async_smem();
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[pb]);
+                }
+                const int ob = item % C::OB;
+                const uint32_t o = lane_base + C::kColO + ob * C::NP * N + c0;
+                const int nq = min(it.nq - c0, NC);  // the group's queries (none: <= 0)
+                const long long at = (a.merge ? 0 : it.split * rows) + it.q0 + c0;
+                // the prefix's share of the results: asked for before the sums are folded
+                if (!waited) {
+                    pdl_wait();
+                    waited = true;
+                }
+                float2 ml0 = make_float2(kNoMax, 0.f);
+                float x0[16];
+                if (a.merge && it.np > 0) {
+                    if (gt < nq) ml0 = __ldcg(&a.part_ml[at + gt]);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x0[e] = e < nq ? __ldcg(a.part_o + (at + e) * KV + gt) : 0.f;
+                }
+                // the sums over the tile's keys
+                if (live) {
+                    const int own = fold_columns(l, lane, [](float u, float w) { return u + w; });
+                    if (NC == 32 || (lane & 1) == 0) red_s[gw * N + c0 + own] = l[0];
+                }
+                soft_sync(group);
+                float m_own = kNoMax, l_own = 0.f;  // of query c0 + gt
+                if (gt < NC) {
+                    const int n = c0 + gt;
+                    l_own = red_s[n] + red_s[N + n];
+                    if (KT == 128) l_own += red_s[2 * N + n] + red_s[3 * N + n];
+                    if (*reinterpret_cast<volatile int*>(bad_s)) l_own = __int_as_float(0x7fc00000);
+                    m_own = m_s[n];
+                }
+                if (!a.merge) {
+                    if (gt < nq) a.part_ml[at + gt] = make_float2(m_own, l_own);
+                    wait(&o_full[ob], (item / C::OB) & 1);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int i = 0; i < C::NP; ++i)
+#pragma unroll 1
+                        for (int c = 0; c < nq; c += 16) {
+                            float v[16];
+                            tmem_ld16(o + i * N + c, v);
+                            float* dst = a.part_o + (at + c) * KV + i * 128 + gt;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (c + e < nq) dst[static_cast<long long>(e) * KV] = v[e];
+                        }
                 } else {
-                    tmem_ld16(lane_base + C::kColS + sb * N, z);
-                }
-                if constexpr (Q8) {
-#pragma unroll
-                    for (int n = 0; n < N; n += 16) {
-                        float r[16];
-                        tmem_ld16(lane_base + C::kColR + sb * N + n, r);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) z[n + e] = fmaf(z[n + e], ks, r[e]);
+                    // joint maximum and sum with the prefix's ranges; each part's factor, the division
+                    // by the sum included
+                    if (gt < nq) {
+                        float M = l_own == 0.f ? kNoMax : m_own;
+                        if (it.np > 0) M = fmaxf(M, ml0.x);
+                        for (int s = 1; s < it.np; ++s) M = fmaxf(M, __ldcg(&a.part_ml[s * rows + at + gt]).x);
+                        const float f = fast_exp2(m_own - M);
+                        float L = l_own * f + ml0.y * fast_exp2(ml0.x - M);
+                        for (int s = 1; s < it.np; ++s) {
+                            const float2 ml = __ldcg(&a.part_ml[s * rows + at + gt]);
+                            L += ml.y * fast_exp2(ml.x - M);
+                        }
+                        const float inv = L == 0.f ? 0.f : 1.f / L;
+                        m_s[c0 + gt] = M;
+                        lim_s[c0 + gt] = __float_as_int(inv);
+                        corr_s[c0 + gt] = f * inv;
+                        red_s[N + c0 + gt] = fast_exp2(ml0.x - M) * inv;
+                        if (p.lse) p.lse[at + gt] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
                     }
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s_free[sb]);
-                if ((j + 1) * 128 > lim_min) {  // the last tile(s): keys past a query's limit
-#pragma unroll
-                    for (int n = 0; n < N; ++n) z[n] = key < lim_s[n] ? z[n] * cs : -INFINITY;
-                } else {
-#pragma unroll
-                    for (int n = 0; n < N; ++n) z[n] *= cs;
-                }
-                bool over = false;
-#pragma unroll
-                for (int n = 0; n < N; n += 4) {
-                    const float4 m = *reinterpret_cast<const float4*>(m_s + n);
-                    over |= z[n] > m.x + 8.f;
-                    over |= z[n + 1] > m.y + 8.f;
-                    over |= z[n + 2] > m.z + 8.f;
-                    over |= z[n + 3] > m.w + 8.f;
-                }
-                if (soft_any(over)) {
-                    float mine[(N + 31) / 32];
-#pragma unroll
-                    for (int n = 0; n < N; ++n) {
-                        const float v = warp_max_redux(z[n]);
-                        if (lane == (n & 31)) mine[n >> 5] = v;
-                    }
-#pragma unroll
-                    for (int k = 0; k < (N + 31) / 32; ++k)
-                        if (lane + 32 * k < N) red_s[warp * N + lane + 32 * k] = mine[k];
-                    soft_sync();
-                    if (tid < N) {
-                        const float mt = fmaxf(fmaxf(red_s[tid], red_s[N + tid]), fmaxf(red_s[2 * N + tid], red_s[3 * N + tid]));
-                        const float mo = m_s[tid], mn = mt > mo + 8.f ? mt : mo;
-                        corr_s[tid] = fast_exp2(mo - mn);
-                        m_s[tid] = mn;
-                    }
-                    soft_sync();
-#pragma unroll
-                    for (int n = 0; n < N; ++n) l[n] *= corr_s[n];
-                    if (j > 0) {
-                        // the previous tile's products have landed: rescale the accumulator
-                        const int pt = tile - 1;
-                        wait(&p_free[pt % C::PB], (pt / C::PB) & 1);
+                    if (it.nt > 0) {
+                        wait(&o_full[ob], (item / C::OB) & 1);
                         tc_fence_after();
-                        const uint32_t o = lane_base + C::kColO + (item % C::OB) * C::NP * N;
+                    }
+                    soft_sync(group);
 #pragma unroll 1
-                        for (int i = 0; i < C::NP; ++i)
+                    for (int i = 0; i < C::NP; ++i)
 #pragma unroll 1
-                            for (int c = 0; c < N; c += 16) {
-                                float v[16];
+                        for (int c = 0; c < nq; c += 16) {
+                            float v[16];
+                            if (it.nt > 0) {
                                 tmem_ld16(o + i * N + c, v);
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) v[e] *= corr_s[c + e];
-                                tmem_st16(o + i * N + c, v);
+                                for (int e = 0; e < 16; ++e) v[e] *= corr_s[c0 + c + e];
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) v[e] = 0.f;
                             }
-                        tmem_wait_st();
-                    }
-                }
-                const int pb = tile % C::PB;
-                wait(&p_free[pb], ((tile / C::PB) & 1) ^ 1);
-                uint8_t* P = smem + C::oP + pb * C::kP;
-                const int kr = warp * 32 + lane;  // key row of the tile
+                            if (it.np > 0) {
+                                if (i | c) {
 #pragma unroll
-                for (int n0 = 0; n0 < N; n0 += 8) {
-                    float e[8];
+                                    for (int e = 0; e < 16; ++e)
+                                        x0[e] = c + e < nq ? __ldcg(a.part_o + (at + c + e) * KV + i * 128 + gt) : 0.f;
+                                }
 #pragma unroll
-                    for (int q = 0; q < 8; q += 4) {
-                        const float4 m = *reinterpret_cast<const float4*>(m_s + n0 + q);
-                        e[q] = fast_exp2(z[n0 + q] - m.x);
-                        e[q + 1] = fast_exp2(z[n0 + q + 1] - m.y);
-                        e[q + 2] = fast_exp2(z[n0 + q + 2] - m.z);
-                        e[q + 3] = fast_exp2(z[n0 + q + 3] - m.w);
-                    }
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        l[n0 + q] += e[q];
-                        if (Q8) e[q] *= ks;
-                    }
-                    if constexpr (N == 64) {
-                        *reinterpret_cast<uint4*>(P + sw128(kr, n0 >> 3)) =
-                            make_uint4(lat::pack2<T>(e[0], e[1]), lat::pack2<T>(e[2], e[3]), lat::pack2<T>(e[4], e[5]),
-                                       lat::pack2<T>(e[6], e[7]));
-                    } else {
-                        // K-major: query row n, key kr of the 64-key box kr / 64
-#pragma unroll
-                        for (int q = 0; q < 8; ++q)
-                            *reinterpret_cast<T*>(P + (kr >> 6) * 2048 + sw128(n0 + q, (kr & 63) >> 3) + (kr & 7) * 2) =
-                                lat::from_f32<T>(e[q]);
-                    }
-                }
-                tc_fence_before();
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[pb]);
-            }
-            // the sums over the tile's 128 keys: halve the columns while folding the lanes
-            int own = 0;  // first column this lane ends up with
-            {
-                int w = N;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    if (w > 1) {
-                        w >>= 1;
-                        const bool up = lane & o;
-#pragma unroll
-                        for (int i = 0; i < N / 2; ++i)
-                            if (i < w) {
-                                const float send = up ? l[i] : l[i + w];
-                                const float got = __shfl_xor_sync(0xffffffffu, send, o);
-                                l[i] = (up ? l[i + w] : l[i]) + got;
+                                for (int e = 0; e < 16; ++e)
+                                    if (c + e < nq) v[e] = fmaf(x0[e], red_s[N + c0 + c + e], v[e]);
                             }
-                        if (up) own += w;
-                    } else {
-                        l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
-                    }
-                }
-            }
-            if constexpr (N == 64) {
-                red_s[warp * N + own] = l[0];
-                red_s[warp * N + own + 1] = l[1];
-            } else if ((lane & 1) == 0) {
-                red_s[warp * N + own] = l[0];
-            }
-            soft_sync();
-            if (tid < N) {
-                float t = (red_s[tid] + red_s[N + tid]) + (red_s[2 * N + tid] + red_s[3 * N + tid]);
-                corr_s[tid] = *reinterpret_cast<volatile int*>(bad_s) ? __int_as_float(0x7fc00000) : t;  // the sum
-            }
-            soft_sync();
-            const int ob = item % C::OB;
-            if (it.nt > 0) {
-                wait(&o_full[ob], (item / C::OB) & 1);
-                tc_fence_after();
-            }
-            const uint32_t o = lane_base + C::kColO + ob * C::NP * N;
-            const int d0 = warp * 32 + lane;
-            if (!a.merge) {
-                const long long at = it.split * rows + it.q0;
-                if (tid < it.nq) a.part_ml[at + tid] = make_float2(m_s[tid], corr_s[tid]);
-#pragma unroll 1
-                for (int i = 0; i < C::NP; ++i)
-#pragma unroll 1
-                    for (int c = 0; c < it.nq; c += 16) {
-                        float v[16];
-                        tmem_ld16(o + i * N + c, v);
-                        float* dst = a.part_o + (at + c) * KV + i * 128 + d0;
+                            for (int s = 1; s < it.np; ++s) {
+                                const long long as = s * rows + at + c;
+                                float x[16];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if (c + e < it.nq) dst[static_cast<long long>(e) * KV] = v[e];
-                    }
-            } else {
-                // join the prefix partials of the row's group, then the result itself
-                const int g = p.G > 0 ? group_of(p, it.row) : -1;
-                const int plen = prefix_length(p, g);
-                const int np = (plen + a.prefix_kps - 1) / a.prefix_kps;
-                if (tid < it.nq) {
-                    // factor of each part relative to the joint maximum
-                    float M = corr_s[tid] > 0.f || corr_s[tid] != corr_s[tid] ? m_s[tid] : kNoMax;
-                    for (int s = 0; s < np; ++s) M = fmaxf(M, __ldcg(&a.part_ml[s * rows + it.q0 + tid]).x);
-                    float L = corr_s[tid] * fast_exp2(m_s[tid] - M);
-                    for (int s = 0; s < np; ++s) {
-                        const float2 ml = __ldcg(&a.part_ml[s * rows + it.q0 + tid]);
-                        L += ml.y * fast_exp2(ml.x - M);
-                    }
-                    red_s[tid] = M;
-                    red_s[N + tid] = L == 0.f ? 0.f : 1.f / L;
-                    if (p.lse) p.lse[it.q0 + tid] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-                }
-                soft_sync();
-#pragma unroll 1
-                for (int i = 0; i < C::NP; ++i)
-#pragma unroll 1
-                    for (int c = 0; c < it.nq; c += 16) {
-                        float v[16];
-                        if (it.nt > 0) tmem_ld16(o + i * N + c, v);
+                                for (int e = 0; e < 16; ++e)
+                                    x[e] = c + e < nq ? __ldcg(a.part_o + (as + e) * KV + i * 128 + gt) : 0.f;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) v[e] = it.nt > 0 ? v[e] * fast_exp2(m_s[c + e] - red_s[c + e]) : 0.f;
-                        for (int s = 0; s < np; ++s) {
-                            const long long at = s * rows + it.q0 + c;
-                            const float* src = a.part_o + at * KV + i * 128 + d0;
-                            float x[16];
+                                for (int e = 0; e < 16; ++e)
+                                    if (c + e < nq)
+                                        v[e] += x[e] * (fast_exp2(__ldcg(&a.part_ml[as + e]).x - m_s[c0 + c + e]) *
+                                                        __int_as_float(lim_s[c0 + c + e]));
+                            }
+                            T* dst = static_cast<T*>(p.out) + (at + c) * KV + i * 128 + gt;
 #pragma unroll
                             for (int e = 0; e < 16; ++e)
-                                x[e] = c + e < it.nq ? __ldcg(src + static_cast<long long>(e) * KV) : 0.f;
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                if (c + e < it.nq) v[e] += x[e] * fast_exp2(__ldcg(&a.part_ml[at + e]).x - red_s[c + e]);
+                                if (c + e < nq) dst[static_cast<long long>(e) * KV] = lat::from_f32<T>(v[e]);
                         }
-                        T* dst = static_cast<T*>(p.out) + static_cast<long long>(it.q0 + c) * KV + i * 128 + d0;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if (c + e < it.nq) dst[static_cast<long long>(e) * KV] = lat::from_f32<T>(v[e] * red_s[N + c + e]);
-                    }
-            }
-            if (it.nt > 0) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&o_free[ob]);
-                ++item;
+                }
+                if (it.nt > 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&o_free[ob]);
+                    ++item;
+                }
             }
         }
+        // this launch must not end before the one it ran beside
+        if (!waited) pdl_wait();
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, C::kTmem);
     }
