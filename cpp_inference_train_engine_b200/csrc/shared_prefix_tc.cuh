@@ -135,6 +135,14 @@ __device__ __forceinline__ bool elect_one() {
     return r != 0;
 }
 
+// The barrier counts this thread once its cp.async copies so far have landed. What crosses to
+// the asynchronous proxy (copies, converted codes, probabilities) is fenced by the one thread
+// that issues the products, after its wait: a proxy fence in the loading threads would wait for
+// every load they have in flight (measured: 1.7 instead of over 5 TB/s).
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 // Barrier of the four warps of a softmax group, with and without an OR of a predicate.
 __device__ __forceinline__ void soft_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory"); }
 __device__ __forceinline__ bool soft_any(int group, bool p) {
@@ -267,9 +275,9 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     int* plan_s = reinterpret_cast<int*>(smem + C::oPlan);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::oBar);
     uint64_t* q_empty = bars;                    // [QB] the item's S products have read Q
-    uint64_t* pair_full = q_empty + C::QB;       // [PS] four producer warps
+    uint64_t* pair_full = q_empty + C::QB;       // [PS] the producer threads (e4m3: warps)
     uint64_t* pair_empty = pair_full + C::PS;    // [PS] O products done with the pair
-    uint64_t* rope_full = pair_empty + C::PS;    // [RS] four producer warps (and the item's queries)
+    uint64_t* rope_full = pair_empty + C::PS;    // [RS] the producer threads (the item's queries included)
     uint64_t* rope_empty = rope_full + C::RS;    // [RS]
     uint64_t* s_full = rope_empty + C::RS;       // [2]
     uint64_t* s_free = s_full + 2;               // [2] the softmax warps
@@ -287,8 +295,8 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     if (warp == kMmaWarp) {
         if (lane == 0) {
             for (int i = 0; i < C::QB; ++i) mbar_init(&q_empty[i], 1);
-            for (int i = 0; i < C::PS; ++i) { mbar_init(&pair_full[i], 4); mbar_init(&pair_empty[i], 1); }
-            for (int i = 0; i < C::RS; ++i) { mbar_init(&rope_full[i], 4); mbar_init(&rope_empty[i], 1); }
+            for (int i = 0; i < C::PS; ++i) { mbar_init(&pair_full[i], Q8 ? 4 : 128); mbar_init(&pair_empty[i], 1); }
+            for (int i = 0; i < C::RS; ++i) { mbar_init(&rope_full[i], 128); mbar_init(&rope_empty[i], 1); }
             for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_free[i], C::SW); }
             for (int i = 0; i < C::PB; ++i) { mbar_init(&p_full[i], C::SW); mbar_init(&p_free[i], 1); }
             for (int i = 0; i < C::OB; ++i) { mbar_init(&o_full[i], 1); mbar_init(&o_free[i], C::SW); }
@@ -394,73 +402,37 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
 #pragma unroll
             for (int r = r0; r < KT; r += kRows) cp_async16(d + sw_rope<R>(r, c), src + (r < left ? r : 0) * ps, r < left);
         };
-        auto arrive_full = [&](uint64_t* bar) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
-        };
         int qi = -1, tile = 0, pr = 0;
         if constexpr (!Q8) {
-            // units in order per tile: rope (the item's queries with its first), pair 0, 1, ...
-            // Each is one cp.async group; a unit is announced once later groups are in flight, or
-            // all at once before the warp would block on a full ring.
-            int issued = 0, told = 0;
-            constexpr int kFlight = C::PS < 6 ? C::PS : 6;
-            auto bar_of = [&](int u) {
-                const int t = u / (C::NP + 1), s = u - t * (C::NP + 1);
-                return s == 0 ? &rope_full[t % C::RS] : &pair_full[(t * C::NP + s - 1) % C::PS];
-            };
-            auto tell_to = [&](int n) {
-                if (told >= n) return;
-                fence_proxy_async_smem();
-                __syncwarp();
-                for (; told < n; ++told)
-                    if (lane == 0) mbar_arrive(bar_of(told));
-            };
-            auto room = [&](uint64_t* bar, uint32_t parity) {
-                // uniform over the warp: every lane must take the same path
-                const bool free = __all_sync(0xffffffffu, mbar_try_wait(bar, parity));
-                if (!free) {
-                    cp_async_wait<0>();
-                    tell_to(issued);
-                    wait(bar, parity);
-                }
-            };
             const int cc = pt & 15, r0 = pt >> 4;  // 16-byte chunk of the pair's row, first row
             const long long ps = 2 * cv.pos_stride;
             for (int base = 0; base < mine; base += kTcTable) {
                 const int count = next_table(base);
                 for (Cursor c(table, count); c.valid(); c.next(), ++tile) {
                     const Item& it = c.item();
-                    room(&rope_empty[tile % C::RS], ((tile / C::RS) & 1) ^ 1);
+                    wait(&rope_empty[tile % C::RS], ((tile / C::RS) & 1) ^ 1);
                     if (c.j == 0) {
                         ++qi;
-                        room(&q_empty[qi % C::QB], ((qi / C::QB) & 1) ^ 1);
+                        wait(&q_empty[qi % C::QB], ((qi / C::QB) & 1) ^ 1);
                         load_q(it, qi % C::QB);
                     }
                     load_rope(it, c.j, tile % C::RS);
-                    cp_async_commit();
-                    ++issued;
+                    cp_async_arrive(&rope_full[tile % C::RS]);
                     const int left = it.nk - c.j * KT;
                     const uint8_t* src = cv.latent + 2 * (it.row * cv.row_stride) + (it.k0 + c.j * KT) * ps + cc * 16;
 #pragma unroll 1
                     for (int i = 0; i < C::NP; ++i, ++pr, src += 256) {
                         const int slot = pr % C::PS;
-                        room(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
+                        wait(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
                         uint8_t* d = sPair + slot * C::kPair + (cc >> 3) * C::kBox + sw128(r0, cc & 7);
 #pragma unroll
                         for (int k = 0; k < KT / 8; ++k) {  // rows 8 apart: the same swizzle phase
                             const int r = r0 + 8 * k;
                             cp_async16(d + k * 1024, src + (r < left ? r : 0) * ps, r < left);
                         }
-                        cp_async_commit();
-                        ++issued;
-                        cp_async_wait<kFlight - 1>();
-                        tell_to(issued - (kFlight - 1));
+                        cp_async_arrive(&pair_full[slot]);
                     }
                 }
-                cp_async_wait<0>();
-                tell_to(issued);
             }
         } else {
             // codes D pairs ahead in registers: VPT x 16 bytes of a pair per thread
@@ -503,7 +475,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                                     load_q(sc.item(), qi % C::QB);
                                 }
                                 load_rope(sc.item(), sc.j, tile % C::RS);
-                                cp_async_commit();
+                                cp_async_arrive(&rope_full[tile % C::RS]);
                             }
                             const int slot = pr % C::PS;
                             wait(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
@@ -526,11 +498,8 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                                 fetch(v[d], lc.item(), lc.j, li);
                                 step(lc, li);
                             }
-                            if (si == 0) {
-                                cp_async_wait<0>();
-                                arrive_full(&rope_full[tile % C::RS]);
-                            }
-                            arrive_full(&pair_full[slot]);
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&pair_full[slot]);
                             ++pr;
                             if (si == C::NP - 1) ++tile;
                             step(sc, si);
@@ -538,8 +507,8 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     }
                 }
             }
-            cp_async_wait<0>();
         }
+        cp_async_wait<0>();
     } else if (warp >= kMmaWarp) {
         // ------------------------------------------------------------ tensor-core products
         if constexpr (Q8 && N == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
@@ -559,6 +528,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             wait(&s_free[sb], ((s_tile >> 1) & 1) ^ 1);
             const int rs = s_tile % C::RS;
             wait(&rope_full[rs], (s_tile / C::RS) & 1);
+            fence_proxy_async_smem();
             tc_fence_after();
             {
                 const uint64_t ka = rope_desc<R>(aR + rs * C::kRopeA), qa = rope_desc<R>(q + 2 * C::NP * C::kQBox);
@@ -571,7 +541,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             for (int i = 0; i < C::NP; ++i, ++s_pr) {
                 const int slot = s_pr % C::PS;
                 wait(&pair_full[slot], (s_pr / C::PS) & 1);
-                tc_fence_after();
+                fence_proxy_async_smem();
                 const uint64_t ka = kd + static_cast<uint32_t>(slot * (C::kPair >> 4));
                 const uint64_t qa = qd + static_cast<uint32_t>(i * (2 * C::kQBox >> 4));
 #pragma unroll
@@ -590,6 +560,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             const int ob = o_item % C::OB, pb = o_tile % C::PB;
             if (c.j == 0) wait(&o_free[ob], ((o_item / C::OB) & 1) ^ 1);
             wait(&p_full[pb], (o_tile / C::PB) & 1);
+            fence_proxy_async_smem();
             tc_fence_after();
             const uint64_t pa = umma_desc_sw128(aP + pb * C::kP, N == 64 ? C::kBox : 16, 1024);
 #pragma unroll 1
@@ -792,7 +763,6 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                                         lat::from_f32<T>(e[q]);
                             }
                         }
-                        fence_proxy_async_smem();
                     }
                     tc_fence_before();
                     __syncwarp();
