@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 #include <exception>
 #include <string>
@@ -225,7 +226,7 @@ struct Plan {
     int pre_n = 0, pre_splits = 0, pre_kps = 128;  // queries per block (0: no prefix launch), ranges, keys per range
     int suf_n = 0, suf_splits = 0, suf_kps = 128;
     long long pre_blocks = 0, suf_blocks = 0;      // upper bounds of the query blocks
-    bool merge = false;                            // the suffix launch writes the results
+    bool join = false;                             // a join launch: not every row is one suffix range
     long long rows = 0;                            // query rows
     long long pre_part = 0, suf_part = 0;          // partial query rows held by the workspace
     long long bytes(int kv) const { return (pre_part + suf_part) * (kv + 2) * 4; }
@@ -257,15 +258,17 @@ Plan plan(const mm::spa::Problem& p) {
         r.pre_n = p.max_group * th <= 16 ? 16 : 64;
         r.pre_blocks = std::min((r.rows + r.pre_n - 1) / r.pre_n + p.G, p.G * ((p.max_group * th + r.pre_n - 1) / r.pre_n));
         pick_splits(r.pre_blocks, p.max_prefix, 64, r.pre_splits, r.pre_kps);
+        if (const char* e = std::getenv("MM_SPA_PRE")) { r.pre_kps = std::atoi(e); r.pre_splits = (p.max_prefix + r.pre_kps - 1) / r.pre_kps; }
         r.pre_part = r.rows * r.pre_splits;
     }
     if (p.max_suffix > 0) {
         r.suf_n = th <= 16 ? 16 : 64;
         r.suf_blocks = p.B * ((th + r.suf_n - 1) / r.suf_n);
         pick_splits(r.suf_blocks, p.max_suffix, 16, r.suf_splits, r.suf_kps);
-        r.merge = r.suf_splits == 1;
-        if (!r.merge) r.suf_part = r.rows * r.suf_splits;
+        if (const char* e = std::getenv("MM_SPA_SUF")) { r.suf_kps = std::atoi(e); r.suf_splits = (p.max_suffix + r.suf_kps - 1) / r.suf_kps; }
     }
+    r.join = !r.suf_n || r.suf_splits > 1 || r.pre_splits > mm::spa::kMaxJoin;
+    if (r.join) r.suf_part = r.rows * r.suf_splits;
     if (r.pre_blocks * std::max(1, r.pre_splits) > kMaxBlocks || r.suf_blocks * std::max(1, r.suf_splits) > kMaxBlocks)
         refuse(MM_UNSUPPORTED, "shared-prefix attention: too many query rows");
     return r;
@@ -305,17 +308,18 @@ void run_tc(const mm::spa::Problem& p, const Plan& r, bool q8p, bool q8s, void* 
         a.suffix = 1;
         a.splits = r.suf_splits;
         a.kps = r.suf_kps;
-        a.merge = r.merge ? 1 : 0;
-        a.part_o = r.merge ? pre_o : suf_o;
-        a.part_ml = r.merge ? pre_ml : suf_ml;
+        a.part_o = suf_o;
+        a.part_ml = suf_ml;
+        a.pre_o = pre_o;
+        a.pre_ml = pre_ml;
         a.prefix_kps = r.pre_kps;
         a.overlap = r.pre_n ? 1 : 0;
         launch_tc_n<KV, R, T>(a, r.suf_n, q8s, r.suf_blocks * r.suf_splits, s);
     }
-    if (!r.merge)
+    if (r.join)
         launch(s, shared_prefix_join_kernel<KV, T>, dim3(blocks(r.rows, 8)), dim3(256), 0, p, static_cast<const float*>(pre_o),
                static_cast<const float2*>(pre_ml), r.pre_kps, static_cast<const float*>(suf_o),
-               static_cast<const float2*>(suf_ml), r.suf_kps);
+               static_cast<const float2*>(suf_ml), r.suf_kps, r.suf_n ? 1 : 0);
 }
 
 }  // namespace

@@ -15,18 +15,21 @@
 // (tables of 32 at a time in shared memory, so no role waits for an item's lengths); barrier
 // phases run on across items. Warps:
 //   softmax    4 (N = 16) or 8 (N = 64, each four take 32 of the queries): thread = key
-//              (tensor-memory lane). The running maximum is lazy: a tile whose scores stay below
-//              the reference + 8 (base 2) uses the reference as it is (probabilities up to 2^8 fit
-//              fp16, sums are fp32), decided by one 4-warp vote; otherwise the column maxima are
-//              taken and O^T and the sums are rescaled. A key's scale (e4m3) multiplies its latent
+//              (tensor-memory lane). The running maximum is lazy: the first tile's maximum is the
+//              reference, and a later tile whose scores stay below the reference + 8 (base 2) uses
+//              it as it is (probabilities up to 2^8 fit fp16, sums are fp32), decided by one 4-warp
+//              vote; otherwise the column maxima are taken and O^T and the sums are rescaled. A key's scale (e4m3) multiplies its latent
 //              scores and, for the second product, its probabilities.
-//   producers  4: the item's queries, then per tile of KT keys the rope columns and kv / 128 pairs
+//   producers  2 to 8: the item's queries, then per tile of KT keys the rope columns and kv / 128 pairs
 //              of 64-column boxes into rings of swizzled boxes. 16-bit caches go by 16-byte
-//              cp.async; e4m3 codes are loaded D pairs ahead into registers and stored as 16-bit
+//              cp.async; e4m3 codes are loaded D tiles ahead into registers and stored as 16-bit
 //              values (exact). Rows past the range are zero-filled, so whatever the cache holds
 //              there never reaches a product.
-//   one more   one thread issues tcgen05.mma. With KT = 64 the S^T product still has M = 128: its
-//              upper half reads whatever follows the box in shared memory and is never looked at.
+//   fence      one thread passes each landed box on to the asynchronous proxy: a proxy fence costs
+//              about 100 ns, and in the loading threads it would wait for every load they have in
+//              flight (measured: 1.7 instead of over 5 TB/s).
+//   MMA        one thread issues tcgen05.mma. With KT = 64 the S^T product has M = 64, whose row r
+//              is tensor-memory lane 32 (r / 16) + r % 16.
 // Every mbarrier wait is bounded; after a wait that runs out the CTA goes on without waiting (every
 // loop is bounded, every access in bounds) and its results are NaN.
 #pragma once
@@ -40,17 +43,20 @@ struct TcArgs {
     Problem p;
     int suffix;        // 0: prefix items, 1: suffix items
     int splits, kps;   // key ranges per query block and keys per range (a multiple of 128)
-    // partials of this launch (fp32 O [splits][query rows][kv] unnormalised, (max, sum) in base 2),
-    // or, with merge (suffix, splits = 1): the prefix launch's, which are read, and the final
-    // result is written
+    // partials of this launch: fp32 O [splits][query rows][kv] unnormalised, (max, sum) in base 2
     float* part_o;
     float2* part_ml;
-    int merge, prefix_kps;
+    // a suffix launch writes the results of the rows whose suffix is one range (or empty) itself and
+    // joins the prefix launch's partials (at most kMaxJoin ranges of prefix_kps keys) to them
+    const float* pre_o;
+    const float2* pre_ml;
+    int prefix_kps;
     int overlap;       // the launch before this one is the call's own prefix launch: run beside it
 };
 
-constexpr int kTcMaxPlan = 512;   // groups whose item prefix sums fit the shared plan
+constexpr int kTcMaxPlan = 512;   // groups or rows whose item prefix sums fit the shared plan
 constexpr int kTcTable = 32;      // items per shared table
+constexpr int kMaxJoin = 4;       // prefix ranges a suffix launch joins itself
 constexpr float kNoMax = -1e37f;  // running maximum before any key (finite: its exp2 is 0, never NaN)
 
 // One work item.
@@ -59,12 +65,12 @@ struct Item {
     int row;          // cache row
     int k0, nk, nt;   // first key, keys, tiles (0: nothing to attend)
     int split;
-    int np;           // merge: the prefix ranges to join
+    int np;           // the prefix ranges to join to the result, -1: this item writes partials
 };
 
 template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int NP = KV / 128;                    // 128-column pairs of boxes
-    static constexpr int KT = N == 64 ? 128 : 64;          // keys per tile
+    static constexpr int KT = KV == 512 && N == 16 ? 64 : 128;  // keys per tile
     static constexpr int kBox = KT * 128;                  // KT keys x 64 columns of 16 bits
     static constexpr int kPair = 2 * kBox;
     static constexpr int kRope = KT * R * 2;
@@ -78,32 +84,34 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     // and 512 tensor memory columns hold)
     static constexpr int kCtas = KV == 128 && N == 16 ? 2 : 1;
     static constexpr int QB = KV == 512 && N == 64 ? 1 : 2;
-    static constexpr int PS = KV == 512 ? (N == 64 ? 4 : 10) : (N == 64 ? 4 : 5);
+    static constexpr int PS = KV == 512 ? (N == 64 ? 4 : 10) : (N == 64 ? 4 : 2);
     static constexpr int RS = KV == 512 ? (N == 64 ? 1 : 3) : PS;
     static constexpr int PB = KV == 512 && N == 64 ? 1 : 2;
     static constexpr int OB = KV == 512 && N == 64 ? 1 : 2;
-    // S of the next tile is issued before this tile's O when the rings hold two tiles
-    static constexpr bool kAhead = PS >= 2 * NP && RS >= 2;
+    // order of the products: 0 tile by tile (the ring holds one), 1 S one tile ahead and pair by pair
+    // as it lands, 2 S or O, whichever can go
+    static constexpr int kOrder = PS < 2 * NP ? 0 : KV == 128 || Q8 ? 2 : 1;
     // tensor memory columns: two S buffers (e4m3: two more for the rope columns' share, which the
     // key's scale does not multiply), then the O accumulators
     static constexpr int kColS = 0, kColR = 2 * N, kColO = Q8 ? 4 * N : 2 * N;
     static constexpr int kCols = kColO + OB * NP * N;
     static constexpr int kTmem = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
-    // warps: softmax groups of four, four producers, the MMA warp (N = 64: its whole warpgroup, so
-    // that registers can move between the roles)
+    // warps: softmax groups of four, producers, the MMA warp and the fence warp (N = 64: a whole
+    // warpgroup for these two, so that registers can move between the roles)
     static constexpr int SG = N == 64 ? 2 : 1, NC = N / SG, SW = 4 * SG;
-    static constexpr int kThreads = 32 * (SW + 4 + (N == 64 ? 4 : 1));
-    // e4m3 pairs ahead in registers (KT / 16 16-byte loads per pair and thread)
-    static constexpr int VPT = KT / 16, D = KV == 512 && N == 16 ? 8 : KV == 128 && N == 16 ? 3 : 4;
+    static constexpr int PW = N == 64 ? 4 : KV == 512 ? (Q8 ? 8 : 4) : 2, PT = 32 * PW;
+    static constexpr int kThreads = 32 * (SW + PW + (N == 64 ? 4 : 2));
+    // e4m3: 16-byte loads per pair and thread, tiles ahead in registers
+    static constexpr int VPT = KT * 8 / PT, D = KV == 512 ? (N == 16 ? 2 : 1) : (N == 16 ? 1 : 3);
     static constexpr int oPair = 0;
     static constexpr int oQ = oPair + PS * kPair;
     static constexpr int oRope = oQ + QB * kQA;
     static constexpr int oP = oRope + RS * kRopeA;
     static constexpr int oTab = oP + PB * kP;
-    static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N]
-    static constexpr int oPlan = oF + 7 * N * 4;
+    static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N], up[N]
+    static constexpr int oPlan = oF + 8 * N * 4;
     static constexpr int oBar = oPlan + (kTcMaxPlan + 1) * 4 + 4;
-    static constexpr int kBars = QB + 2 * PS + 2 * RS + 4 + 2 * PB + 2 * OB;
+    static constexpr int kBars = QB + 3 * PS + 3 * RS + 4 + 2 * PB + 2 * OB;
     static constexpr int kSmem = oBar + kBars * 8 + 16 + 1024;  // + alignment of the base
     static_assert(kCtas * (kSmem + 1024) <= 228 * 1024 && kCols * kCtas <= 512, "shared and tensor memory");
 };
@@ -135,10 +143,19 @@ __device__ __forceinline__ bool elect_one() {
     return r != 0;
 }
 
-// The barrier counts this thread once its cp.async copies so far have landed. What crosses to
-// the asynchronous proxy (copies, converted codes, probabilities) is fenced by the one thread
-// that issues the products, after its wait: a proxy fence in the loading threads would wait for
-// every load they have in flight (measured: 1.7 instead of over 5 TB/s).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+// The barrier counts this thread once its cp.async copies so far have landed.
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -192,49 +209,72 @@ template <int NC, class Op> __device__ __forceinline__ int fold_columns(float (&
     return own;
 }
 
-// Item idx of the launch. plan (shared, prefix launches): cumulative query blocks of the
-// groups, or null when there are more groups than it holds.
-template <int N, int KT>
-__device__ __forceinline__ Item get_item(const TcArgs& a, const int* plan, int per, int idx) {
+// The prefix ranges a suffix launch joins to row b's result, -1 when the row is left to the join
+// kernel (several suffix ranges, or more than kMaxJoin prefix ranges).
+__device__ __forceinline__ int direct_join(const Problem& p, int b, int suffix_kps, int prefix_kps) {
+    if (suffix_length(p, b) > suffix_kps) return -1;
+    const int np = (prefix_length(p, p.G > 0 ? group_of(p, b) : -1) + prefix_kps - 1) / prefix_kps;
+    return np <= kMaxJoin ? np : -1;
+}
+
+// A launch's items come from units: groups (prefix) or rows (suffix). Unit u holds `blocks` blocks of
+// N query rows from q0 on and attends over `len` keys in `ranges` key ranges (a suffix row of a
+// direct result keeps one, however empty).
+struct Unit {
+    int q0, nq, len, blocks, ranges, np;
+};
+template <int N> __device__ __forceinline__ Unit get_unit(const TcArgs& a, int u) {
     const Problem& p = a.p;
     const int th = p.T * p.H;
-    Item it;
-    it.split = idx % a.splits;
-    const int blk = idx / a.splits;
-    int len;
-    it.np = 0;
+    Unit r;
+    r.np = -1;
     if (a.suffix) {
-        it.row = blk / per;
-        const int s = (blk - it.row * per) * N;
-        it.q0 = it.row * th + s;
-        it.nq = min(N, th - s);
-        len = suffix_length(p, it.row);
-        if (a.merge) it.np = (prefix_length(p, p.G > 0 ? group_of(p, it.row) : -1) + a.prefix_kps - 1) / a.prefix_kps;
+        r.q0 = u * th;
+        r.nq = th;
+        r.len = suffix_length(p, u);
+        r.np = direct_join(p, u, a.kps, a.prefix_kps);
     } else {
-        int g, s;
-        if (plan) {
-            int lo = 0, hi = p.G;  // the group with plan[g] <= blk < plan[g + 1]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (plan[mid] <= blk) lo = mid;
-                else hi = mid;
-            }
-            g = lo;
-            s = (blk - plan[g]) * N;
-        } else {
-            g = blk / per;
-            s = (blk - g * per) * N;
-        }
-        const int b0 = min(max(p.group_start[g], 0), p.B), b1 = min(max(p.group_start[g + 1], b0), p.B);
-        const int total = min(b1 - b0, p.max_group) * th;
-        it.row = g;
-        it.q0 = b0 * th + s;
-        it.nq = max(0, min(N, total - s));
-        len = it.nq > 0 ? prefix_length(p, g) : 0;
+        const int b0 = min(max(p.group_start[u], 0), p.B), b1 = min(max(p.group_start[u + 1], b0), p.B);
+        r.q0 = b0 * th;
+        r.nq = min(b1 - b0, p.max_group) * th;
+        r.len = r.nq > 0 ? prefix_length(p, u) : 0;
     }
+    r.blocks = (r.nq + N - 1) / N;
+    r.ranges = max((r.len + a.kps - 1) / a.kps, r.np >= 0 ? 1 : 0);
+    return r;
+}
+
+// Item idx of the launch. With a plan (shared: cumulative items of the units) the items are
+// dense, so that they spread evenly over the CTAs whatever the lengths; without one (more units
+// than it holds) every unit has `per` blocks of a.splits ranges, some of them empty.
+template <int N, int KT>
+__device__ __forceinline__ Item get_item(const TcArgs& a, const int* plan, int units, int per, int idx) {
+    int u, local;
+    if (plan) {
+        int lo = 0, hi = units;  // the unit with plan[u] <= idx < plan[u + 1]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (plan[mid] <= idx) lo = mid;
+            else hi = mid;
+        }
+        u = lo;
+        local = idx - plan[u];
+    } else {
+        u = idx / (per * a.splits);
+        local = idx - u * per * a.splits;
+    }
+    const Unit r = get_unit<N>(a, u);
+    const int ranges = plan ? r.ranges : a.splits;
+    const int block = local / ranges;
+    Item it;
+    it.split = local - block * ranges;
+    it.row = u;
+    it.q0 = r.q0 + block * N;
+    it.nq = max(0, min(N, r.nq - block * N));
     it.k0 = it.split * a.kps;
-    it.nk = max(0, min(a.kps, len - it.k0));
+    it.nk = it.nq > 0 ? max(0, min(a.kps, r.len - it.k0)) : 0;
     it.nt = (it.nk + KT - 1) / KT;
+    it.np = it.split == 0 ? r.np : -1;
     return it;
 }
 
@@ -272,12 +312,15 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     float* corr_s = m_s + N;
     float* red_s = corr_s + N;  // [4][N]
     int* lim_s = reinterpret_cast<int*>(red_s + 4 * N);
+    float* up_s = red_s + 5 * N;
     int* plan_s = reinterpret_cast<int*>(smem + C::oPlan);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::oBar);
     uint64_t* q_empty = bars;                    // [QB] the item's S products have read Q
-    uint64_t* pair_full = q_empty + C::QB;       // [PS] the producer threads (e4m3: warps)
+    uint64_t* pair_in = q_empty + C::QB;         // [PS] the producer threads (e4m3: warps)
+    uint64_t* pair_full = pair_in + C::PS;       // [PS] the fence warp
     uint64_t* pair_empty = pair_full + C::PS;    // [PS] O products done with the pair
-    uint64_t* rope_full = pair_empty + C::PS;    // [RS] the producer threads (the item's queries included)
+    uint64_t* rope_in = pair_empty + C::PS;      // [RS] the producer threads (the item's queries included)
+    uint64_t* rope_full = rope_in + C::RS;       // [RS] the fence warp
     uint64_t* rope_empty = rope_full + C::RS;    // [RS]
     uint64_t* s_full = rope_empty + C::RS;       // [2]
     uint64_t* s_free = s_full + 2;               // [2] the softmax warps
@@ -290,13 +333,21 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     const Problem& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int th = p.T * p.H;
-    constexpr int kMmaWarp = C::SW + 4;
+    constexpr int kMmaWarp = C::SW + C::PW, kFenceWarp = kMmaWarp + 1;
 
     if (warp == kMmaWarp) {
         if (lane == 0) {
             for (int i = 0; i < C::QB; ++i) mbar_init(&q_empty[i], 1);
-            for (int i = 0; i < C::PS; ++i) { mbar_init(&pair_full[i], Q8 ? 4 : 128); mbar_init(&pair_empty[i], 1); }
-            for (int i = 0; i < C::RS; ++i) { mbar_init(&rope_full[i], 128); mbar_init(&rope_empty[i], 1); }
+            for (int i = 0; i < C::PS; ++i) {
+                mbar_init(&pair_in[i], Q8 ? C::PW : C::PT);
+                mbar_init(&pair_full[i], 1);
+                mbar_init(&pair_empty[i], 1);
+            }
+            for (int i = 0; i < C::RS; ++i) {
+                mbar_init(&rope_in[i], C::PT);
+                mbar_init(&rope_full[i], 1);
+                mbar_init(&rope_empty[i], 1);
+            }
             for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_free[i], C::SW); }
             for (int i = 0; i < C::PB; ++i) { mbar_init(&p_full[i], C::SW); mbar_init(&p_free[i], 1); }
             for (int i = 0; i < C::OB; ++i) { mbar_init(&o_full[i], 1); mbar_init(&o_free[i], C::SW); }
@@ -312,40 +363,34 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     // where they are read.
     if (!a.overlap) pdl_wait();
     pdl_launch_dependents();
-    int per, items;
+    const int units = a.suffix ? p.B : p.G;
+    const int per = ((a.suffix ? th : p.max_group * th) + N - 1) / N;
     const int* plan = nullptr;
-    if (a.suffix) {
-        per = (th + N - 1) / N;
-        items = p.B * per * a.splits;
-    } else {
-        per = (p.max_group * th + N - 1) / N;
-        if (p.G <= kTcMaxPlan) {
-            // cumulative query blocks of the groups
-            plan = plan_s;
-            for (int g = tid; g < p.G; g += C::kThreads) {
-                const int b0 = min(max(p.group_start[g], 0), p.B), b1 = min(max(p.group_start[g + 1], b0), p.B);
-                plan_s[g + 1] = (min(b1 - b0, p.max_group) * th + N - 1) / N;
-            }
-            __syncthreads();
-            if (warp == 0) {
-                int base = 0;
-                for (int g0 = 0; g0 < p.G; g0 += 32) {
-                    int v = g0 + lane < p.G ? plan_s[g0 + lane + 1] : 0;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const int u = __shfl_up_sync(0xffffffffu, v, o);
-                        if (lane >= o) v += u;
-                    }
-                    if (g0 + lane < p.G) plan_s[g0 + lane + 1] = base + v;
-                    base += __shfl_sync(0xffffffffu, v, 31);
-                }
-                if (lane == 0) plan_s[0] = 0;
-            }
-            __syncthreads();
-            items = plan_s[p.G] * a.splits;
-        } else {
-            items = p.G * per * a.splits;
+    int items = units * per * a.splits;
+    if (units <= kTcMaxPlan && (a.splits > 1 || !a.suffix)) {
+        // cumulative items of the units (a suffix launch with one range per row has none to skip)
+        plan = plan_s;
+        for (int u = tid; u < units; u += C::kThreads) {
+            const Unit r = get_unit<N>(a, u);
+            plan_s[u + 1] = r.blocks * r.ranges;
         }
+        __syncthreads();
+        if (warp == 0) {
+            int base = 0;
+            for (int u0 = 0; u0 < units; u0 += 32) {
+                int v = u0 + lane < units ? plan_s[u0 + lane + 1] : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int w = __shfl_up_sync(0xffffffffu, v, o);
+                    if (lane >= o) v += w;
+                }
+                if (u0 + lane < units) plan_s[u0 + lane + 1] = base + v;
+                base += __shfl_sync(0xffffffffu, v, 31);
+            }
+            if (lane == 0) plan_s[0] = 0;
+        }
+        __syncthreads();
+        items = plan_s[units];
     }
     tc_fence_before();
     __syncthreads();
@@ -365,7 +410,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     auto next_table = [&](int base) {
         if (base > 0) __syncthreads();
         if (tid < kTcTable && base + tid < mine)
-            table[tid] = get_item<N, KT>(a, plan, per, blockIdx.x + (base + tid) * gridDim.x);
+            table[tid] = get_item<N, KT>(a, plan, units, per, blockIdx.x + (base + tid) * gridDim.x);
         __syncthreads();
         return min(kTcTable, mine - base);
     };
@@ -373,7 +418,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     if (warp >= C::SW && warp < kMmaWarp) {
         // ------------------------------------------------------------ producers
         if constexpr (Q8 && N == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-        const int pt = tid - 32 * C::SW;  // 0..127
+        const int pt = tid - 32 * C::SW;  // 0..PT - 1
         uint8_t* sQ = smem + C::oQ;
         uint8_t* sPair = smem + C::oPair;
         uint8_t* sRope = smem + C::oRope;
@@ -382,7 +427,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             uint8_t* q = sQ + qb * C::kQA;
             const int c = pt & 7;
 #pragma unroll 1
-            for (int n = pt >> 3; n < N; n += 16) {
+            for (int n = pt >> 3; n < N; n += C::PT / 8) {
                 const bool in = n < it.nq;
                 const int r = it.q0 + (in ? n : 0), b = r / th, u = r - b * th, t = u / p.H, h = u - t * p.H;
                 const T* src = static_cast<const T*>(p.q) + b * p.q_row + t * p.q_tok + h * p.q_head + c * 8;
@@ -393,7 +438,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             }
         };
         auto load_rope = [&](const Item& it, int j, int slot) {
-            constexpr int kChunks = R / 8, kRows = 128 / kChunks;
+            constexpr int kChunks = R / 8, kRows = C::PT / kChunks;
             const int c = pt % kChunks, r0 = pt / kChunks, left = it.nk - j * KT;
             uint8_t* d = sRope + slot * C::kRopeA;
             const long long ps = 2 * (Q8 ? cv.rope_pos_stride : cv.pos_stride);
@@ -417,92 +462,93 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                         load_q(it, qi % C::QB);
                     }
                     load_rope(it, c.j, tile % C::RS);
-                    cp_async_arrive(&rope_full[tile % C::RS]);
+                    cp_async_arrive(&rope_in[tile % C::RS]);
                     const int left = it.nk - c.j * KT;
                     const uint8_t* src = cv.latent + 2 * (it.row * cv.row_stride) + (it.k0 + c.j * KT) * ps + cc * 16;
 #pragma unroll 1
                     for (int i = 0; i < C::NP; ++i, ++pr, src += 256) {
                         const int slot = pr % C::PS;
                         wait(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
-                        uint8_t* d = sPair + slot * C::kPair + (cc >> 3) * C::kBox + sw128(r0, cc & 7);
+                        uint8_t* d = sPair + slot * C::kPair + (cc >> 3) * C::kBox;
 #pragma unroll
-                        for (int k = 0; k < KT / 8; ++k) {  // rows 8 apart: the same swizzle phase
-                            const int r = r0 + 8 * k;
-                            cp_async16(d + k * 1024, src + (r < left ? r : 0) * ps, r < left);
+                        for (int k = 0; k < KT * 16 / C::PT; ++k) {
+                            const int r = r0 + C::PT / 16 * k;
+                            cp_async16(d + sw128(r, cc & 7), src + (r < left ? r : 0) * ps, r < left);
                         }
-                        cp_async_arrive(&pair_full[slot]);
+                        cp_async_arrive(&pair_in[slot]);
                     }
                 }
             }
         } else {
-            // codes D pairs ahead in registers: VPT x 16 bytes of a pair per thread
-            constexpr int D = C::D;
-            uint4 v[D][C::VPT];
-            const int cc = pt & 7, r0 = pt >> 3;  // 16-byte chunk of the pair's 128 codes, first row
-            auto fetch = [&](uint4 (&x)[C::VPT], const Item& it, int j, int i) {
-                const int left = it.nk - j * KT - r0;
-                const uint8_t* src = cv.latent + it.row * cv.row_stride + (it.k0 + j * KT + r0) * cv.pos_stride + i * 128 + cc * 16;
-                const long long step = 16 * cv.pos_stride;
+            // codes D tiles ahead in registers: each pair is asked for again for a later tile as soon
+            // as it has been converted
+            constexpr int D = C::D, kRows = C::PT / 8;
+            uint4 v[D][C::NP][C::VPT];
+            const int cc = pt & 7, r0 = pt >> 3;  // 16-byte chunk of a pair's 128 codes, first row
+            const long long rstep = kRows * cv.pos_stride;
+            const uint8_t* src = nullptr;
+            int left = 0;
+            auto at_tile = [&](const Cursor& c) {
+                const Item& it = c.item();
+                left = it.nk - c.j * KT - r0;
+                src = cv.latent + it.row * cv.row_stride + (it.k0 + c.j * KT + r0) * cv.pos_stride + cc * 16;
+            };
+            auto fetch = [&](uint4 (&x)[C::VPT], int i) {
 #pragma unroll
                 for (int k = 0; k < C::VPT; ++k)
-                    x[k] = 16 * k < left ? __ldg(reinterpret_cast<const uint4*>(src + k * step)) : make_uint4(0, 0, 0, 0);
+                    x[k] = kRows * k < left ? __ldg(reinterpret_cast<const uint4*>(src + k * rstep + i * 128)) : make_uint4(0, 0, 0, 0);
             };
             for (int base = 0; base < mine; base += kTcTable) {
                 const int count = next_table(base);
                 Cursor lc(table, count), sc(table, count);
-                int li = 0, si = 0;  // pair of the tile each cursor is at
-                auto step = [&](Cursor& c, int& i) {
-                    if (++i == C::NP) {
-                        i = 0;
-                        c.next();
-                    }
-                };
 #pragma unroll
                 for (int d = 0; d < D; ++d)
                     if (lc.valid()) {
-                        fetch(v[d], lc.item(), lc.j, li);
-                        step(lc, li);
+                        at_tile(lc);
+#pragma unroll
+                        for (int i = 0; i < C::NP; ++i) fetch(v[d][i], i);
+                        lc.next();
                     }
                 while (sc.valid()) {
 #pragma unroll
                     for (int d = 0; d < D; ++d) {
                         if (sc.valid()) {
-                            if (si == 0) {
-                                wait(&rope_empty[tile % C::RS], ((tile / C::RS) & 1) ^ 1);
-                                if (sc.j == 0) {
-                                    ++qi;
-                                    wait(&q_empty[qi % C::QB], ((qi / C::QB) & 1) ^ 1);
-                                    load_q(sc.item(), qi % C::QB);
-                                }
-                                load_rope(sc.item(), sc.j, tile % C::RS);
-                                cp_async_arrive(&rope_full[tile % C::RS]);
+                            wait(&rope_empty[tile % C::RS], ((tile / C::RS) & 1) ^ 1);
+                            if (sc.j == 0) {
+                                ++qi;
+                                wait(&q_empty[qi % C::QB], ((qi / C::QB) & 1) ^ 1);
+                                load_q(sc.item(), qi % C::QB);
                             }
-                            const int slot = pr % C::PS;
-                            wait(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
-                            uint8_t* dst = sPair + slot * C::kPair + (cc >> 2) * C::kBox;
+                            load_rope(sc.item(), sc.j, tile % C::RS);
+                            cp_async_arrive(&rope_in[tile % C::RS]);
+                            const bool more = lc.valid();
+                            if (more) at_tile(lc);
 #pragma unroll
-                            for (int k = 0; k < C::VPT; ++k) {
-                                const int r = r0 + 16 * k;
-                                const uint32_t w[4] = {v[d][k].x, v[d][k].y, v[d][k].z, v[d][k].w};
-                                uint32_t o[8];
+                            for (int i = 0; i < C::NP; ++i, ++pr) {
+                                const int slot = pr % C::PS;
+                                wait(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
+                                uint8_t* dst = sPair + slot * C::kPair + (cc >> 2) * C::kBox;
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    o[2 * e] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] & 0xffff));
-                                    o[2 * e + 1] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] >> 16));
+                                for (int k = 0; k < C::VPT; ++k) {
+                                    const int r = r0 + kRows * k;
+                                    const uint32_t w[4] = {v[d][i][k].x, v[d][i][k].y, v[d][i][k].z, v[d][i][k].w};
+                                    uint32_t o[8];
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        o[2 * e] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] & 0xffff));
+                                        o[2 * e + 1] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] >> 16));
+                                    }
+                                    *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc) & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+                                    *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc + 1) & 7)) =
+                                        make_uint4(o[4], o[5], o[6], o[7]);
                                 }
-                                *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc) & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
-                                *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc + 1) & 7)) =
-                                    make_uint4(o[4], o[5], o[6], o[7]);
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(&pair_in[slot]);
+                                if (more) fetch(v[d][i], i);
                             }
-                            if (lc.valid()) {
-                                fetch(v[d], lc.item(), lc.j, li);
-                                step(lc, li);
-                            }
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&pair_full[slot]);
-                            ++pr;
-                            if (si == C::NP - 1) ++tile;
-                            step(sc, si);
+                            if (more) lc.next();
+                            sc.next();
+                            ++tile;
                         }
                     }
                 }
@@ -512,7 +558,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     } else if (warp >= kMmaWarp) {
         // ------------------------------------------------------------ tensor-core products
         if constexpr (Q8 && N == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        const uint32_t id_s = umma_idesc_f16(kBf16, false, false, 128, N);
+        const uint32_t id_s = umma_idesc_f16(kBf16, false, false, KT, N);
         const uint32_t id_o = umma_idesc_f16(kBf16, true, N == 64, 128, N);
         const uint32_t aPair = smem_u32(smem + C::oPair), aQ = smem_u32(smem + C::oQ), aR = smem_u32(smem + C::oRope),
                        aP = smem_u32(smem + C::oP);
@@ -520,15 +566,19 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         const uint64_t kd = umma_desc_sw128(aPair, 16, 1024), vd = umma_desc_sw128(aPair, C::kBox, 1024);
         int s_tile = 0, s_pr = 0, s_q = 0;     // S products: tile, pair and item counters
         int o_tile = 0, o_pr = 0, o_item = 0;  // O products
-        auto issue_s = [&](const Cursor& c) {
+        auto s_ready = [&] {
+            bool r = mbar_test(&s_free[s_tile & 1], ((s_tile >> 1) & 1) ^ 1) &&
+                     mbar_test(&rope_full[s_tile % C::RS], (s_tile / C::RS) & 1);
+            for (int i = 0; i < C::NP && r; ++i) r = mbar_test(&pair_full[(s_pr + i) % C::PS], ((s_pr + i) / C::PS) & 1);
+            return r;
+        };
+        auto issue_s = [&](Cursor& c) {
             const uint32_t q = aQ + (s_q % C::QB) * C::kQA;
             const uint64_t qd = umma_desc_sw128(q, 16, 1024);
-            const int sb = s_tile & 1;
+            const int sb = s_tile & 1, rs = s_tile % C::RS;
             const uint32_t d = tmem + C::kColS + sb * N;
             wait(&s_free[sb], ((s_tile >> 1) & 1) ^ 1);
-            const int rs = s_tile % C::RS;
             wait(&rope_full[rs], (s_tile / C::RS) & 1);
-            fence_proxy_async_smem();
             tc_fence_after();
             {
                 const uint64_t ka = rope_desc<R>(aR + rs * C::kRopeA), qa = rope_desc<R>(q + 2 * C::NP * C::kQBox);
@@ -538,10 +588,9 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             }
             tc_commit(&rope_empty[rs]);
 #pragma unroll 1
-            for (int i = 0; i < C::NP; ++i, ++s_pr) {
+            for (int i = 0; i < C::NP; ++i, ++s_pr) {  // pair by pair as the boxes land
                 const int slot = s_pr % C::PS;
                 wait(&pair_full[slot], (s_pr / C::PS) & 1);
-                fence_proxy_async_smem();
                 const uint64_t ka = kd + static_cast<uint32_t>(slot * (C::kPair >> 4));
                 const uint64_t qa = qd + static_cast<uint32_t>(i * (2 * C::kQBox >> 4));
 #pragma unroll
@@ -555,12 +604,12 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 ++s_q;
             }
             ++s_tile;
+            c.next();
         };
-        auto issue_o = [&](const Cursor& c) {
+        auto issue_o = [&](Cursor& c) {
             const int ob = o_item % C::OB, pb = o_tile % C::PB;
             if (c.j == 0) wait(&o_free[ob], ((o_item / C::OB) & 1) ^ 1);
             wait(&p_full[pb], (o_tile / C::PB) & 1);
-            fence_proxy_async_smem();
             tc_fence_after();
             const uint64_t pa = umma_desc_sw128(aP + pb * C::kP, N == 64 ? C::kBox : 16, 1024);
 #pragma unroll 1
@@ -581,26 +630,52 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 ++o_item;
             }
             ++o_tile;
+            c.next();
         };
+        int f_tile = 0, f_pr = 0;
         for (int base = 0; base < mine; base += kTcTable) {
             const int count = next_table(base);
+            if (warp == kFenceWarp && lane == 0) {
+                // what has been written in the generic proxy (copies, converted codes) becomes
+                // readable by the products
+                for (Cursor c(table, count); c.valid(); c.next(), ++f_tile) {
+                    wait(&rope_in[f_tile % C::RS], (f_tile / C::RS) & 1);
+                    fence_proxy_async_smem();
+                    mbar_arrive(&rope_full[f_tile % C::RS]);
+                    for (int i = 0; i < C::NP; ++i, ++f_pr) {
+                        wait(&pair_in[f_pr % C::PS], (f_pr / C::PS) & 1);
+                        fence_proxy_async_smem();
+                        mbar_arrive(&pair_full[f_pr % C::PS]);
+                    }
+                }
+            }
             if (warp == kMmaWarp && elect_one()) {
                 Cursor cs(table, count), co(table, count);
-                if (C::kAhead) {
-                    if (cs.valid()) {
-                        issue_s(cs);
-                        cs.next();
-                    }
-                    for (; co.valid(); co.next()) {
-                        if (cs.valid()) {
+                if (C::kOrder == 2) {
+                    // the next tile's S when its boxes are there, this tile's O when its probabilities are:
+                    // neither waits behind the other
+                    int polls = 0;
+                    while (co.valid()) {
+                        const bool late = !ok || polls > (1 << 24);  // gave up: go on in order, waits and all
+                        if (cs.valid() && s_tile - o_tile < 2 && (s_ready() || (late && s_tile == o_tile))) {
                             issue_s(cs);
-                            cs.next();
+                            polls = 0;
+                        } else if (s_tile > o_tile && (late || mbar_test(&p_full[o_tile % C::PB], (o_tile / C::PB) & 1))) {
+                            issue_o(co);
+                            polls = 0;
+                        } else {
+                            ++polls;
                         }
+                    }
+                } else if (C::kOrder == 1) {
+                    if (cs.valid()) issue_s(cs);
+                    while (co.valid()) {
+                        if (cs.valid()) issue_s(cs);
                         issue_o(co);
                     }
                 } else {
-                    for (; co.valid(); co.next()) {
-                        issue_s(co);
+                    while (co.valid()) {
+                        issue_s(cs);
                         issue_o(co);
                     }
                 }
@@ -609,9 +684,11 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         }
     } else {
         // ------------------------------------------------------------ softmax and results
-        const int group = warp >> 2, gw = warp & 3, gt = tid & 127;  // gt: key of the tile, TMEM lane
+        const int group = warp >> 2, gw = warp & 3, gt = tid & 127;  // gt: tensor-memory lane
         const int c0 = group * NC;                                   // first query column of the group
-        const bool live = gw * 32 < KT;                              // the warp's lanes hold keys
+        // the key this lane's scores belong to (64-key tiles: the lower half of each warp)
+        const int kt = KT == 128 ? gt : gw * 16 + lane;
+        const bool live = KT == 128 || lane < 16;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(gw * 32) << 16);
         const float cs = p.scale * 1.4426950408889634f;
         const long long rows = static_cast<long long>(p.B) * th;
@@ -622,15 +699,34 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             const int count = next_table(base);
             for (int e0 = 0; e0 < count; ++e0) {
                 const Item it = table[e0];
-                if (it.nt == 0 && !a.merge) continue;
+                const bool direct = it.np >= 0;
+                if (it.nt == 0 && !direct) continue;
+                const int nq = min(it.nq - c0, NC);  // the group's queries (none: <= 0)
                 float l[NC];
 #pragma unroll
                 for (int n = 0; n < NC; ++n) l[n] = 0.f;
+                const long long at = it.q0 + c0;  // first query row; partials of this launch: + split * rows
+                // The prefix's share of a direct result: unit u = (16-column block, prefix range) of the
+                // partials, 16 queries of this thread's dimension. Unit 0 is asked for before the tiles:
+                // a load issued behind a full ring of cache tiles waits its turn (2 to 4 us).
+                const bool joins = it.np > 0 && nq > 0;
+                const int cb = (nq + 15) / 16;
+                float x0[16];
+                float2 ml0 = make_float2(kNoMax, 0.f);
+                auto ask = [&](int u, float (&x)[16]) {
+                    const int s = u % it.np, k = u / it.np, i = k / cb, c = (k - i * cb) * 16;
+                    const float* src = a.pre_o + (s * rows + at + c) * KV + i * 128 + gt;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = c + e < nq ? __ldcg(src + static_cast<long long>(e) * KV) : 0.f;
+                    if (u == 0 && gt < nq) ml0 = __ldcg(&a.pre_ml[at + gt]);
+                };
+                const bool asked = N == 16 && joins && waited;
+                if (asked) ask(0, x0);
                 // keys of the item each query sees; the tokens of a suffix end one position apart
                 const bool causal = a.suffix && p.T > 1;
                 soft_sync(group);  // the previous item's readers of m_s, lim_s and red_s are done
                 if (gt < NC) {
-                    m_s[c0 + gt] = kNoMax;
+                    m_s[c0 + gt] = 0.f;
                     if (causal) {
                         const int t = min((it.q0 + c0 + gt - it.row * th) / p.H, p.T - 1);
                         lim_s[c0 + gt] = min(it.nk, suffix_length(p, it.row) - (p.T - 1 - t) - it.k0);
@@ -640,79 +736,84 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 const int lim_min = causal ? it.nk - (p.T - 1) : it.nk;
                 const float* ks_row = Q8 ? cv.scale + it.row * cv.scale_row_stride + it.k0 : nullptr;
                 float ks_next = 1.f;
-                if (Q8 && live && gt < it.nk) ks_next = __ldg(ks_row + gt);
+                if (Q8 && live && kt < it.nk) ks_next = __ldg(ks_row + kt);
                 for (int j = 0; j < it.nt; ++j, ++tile) {
-                    const int key = j * KT + gt;
+                    const int key = j * KT + kt;
                     const float ks = ks_next;
                     if (Q8) ks_next = live && key + KT < it.nk ? __ldg(ks_row + key + KT) : 1.f;
                     const int sb = tile & 1;
                     wait(&s_full[sb], (tile >> 1) & 1);
                     tc_fence_after();
                     float z[NC];
-                    if (live) {
-                        if constexpr (NC == 32) {
-                            tmem_ld32_nowait(lane_base + C::kColS + sb * N + c0, z);
-                            tmem_wait_ld();
-                        } else {
-                            tmem_ld16(lane_base + C::kColS + sb * N, z);
-                        }
-                        if constexpr (Q8) {
-#pragma unroll
-                            for (int n = 0; n < NC; n += 16) {
-                                float r[16];
-                                tmem_ld16(lane_base + C::kColR + sb * N + c0 + n, r);
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) z[n + e] = fmaf(z[n + e], ks, r[e]);
-                            }
-                        }
-                        tc_fence_before();
+                    if constexpr (NC == 32) {
+                        tmem_ld32_nowait(lane_base + C::kColS + sb * N + c0, z);
+                        tmem_wait_ld();
+                    } else {
+                        tmem_ld16(lane_base + C::kColS + sb * N, z);
                     }
+                    if constexpr (Q8) {
+#pragma unroll
+                        for (int n = 0; n < NC; n += 16) {
+                            float r[16];
+                            tmem_ld16(lane_base + C::kColR + sb * N + c0 + n, r);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) z[n + e] = fmaf(z[n + e], ks, r[e]);
+                        }
+                    }
+                    tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s_free[sb]);
-                    bool over = false;
-                    if (live) {
-                        if ((j + 1) * KT > lim_min) {  // the last tile(s): keys past a query's limit
-                            if (causal) {
+                    // scores relative to the column's reference, base 2; the first tile's reference is 0
+                    bool over = j == 0;
+                    float top = -INFINITY;
 #pragma unroll
-                                for (int n = 0; n < NC; ++n) z[n] = key < lim_s[c0 + n] ? z[n] * cs : -INFINITY;
-                            } else {
+                    for (int n = 0; n < NC; n += 4) {
+                        const float4 m = *reinterpret_cast<const float4*>(m_c + n);
+                        z[n] = fmaf(z[n], cs, -m.x);
+                        z[n + 1] = fmaf(z[n + 1], cs, -m.y);
+                        z[n + 2] = fmaf(z[n + 2], cs, -m.z);
+                        z[n + 3] = fmaf(z[n + 3], cs, -m.w);
+                    }
+                    if ((j + 1) * KT > lim_min) {  // the last tile(s): keys past a query's limit
+                        if (causal) {
 #pragma unroll
-                                for (int n = 0; n < NC; ++n) z[n] = key < it.nk ? z[n] * cs : -INFINITY;
-                            }
-                        } else {
+                            for (int n = 0; n < NC; ++n)
+                                if (key >= lim_s[c0 + n]) z[n] = -INFINITY;
+                        } else if (key >= it.nk) {
 #pragma unroll
-                            for (int n = 0; n < NC; ++n) z[n] *= cs;
-                        }
-#pragma unroll
-                        for (int n = 0; n < NC; n += 4) {
-                            const float4 m = *reinterpret_cast<const float4*>(m_c + n);
-                            over |= z[n] > m.x + 8.f;
-                            over |= z[n + 1] > m.y + 8.f;
-                            over |= z[n + 2] > m.z + 8.f;
-                            over |= z[n + 3] > m.w + 8.f;
+                            for (int n = 0; n < NC; ++n) z[n] = -INFINITY;
                         }
                     }
-                    if (soft_any(group, over)) {
-                        if (live) {
-                            float x[NC];
+                    if (KT == 64 && !live) {
 #pragma unroll
-                            for (int n = 0; n < NC; ++n) x[n] = z[n];
-                            const int own = fold_columns(x, lane, [](float u, float w) { return fmaxf(u, w); });
-                            if (NC == 32 || (lane & 1) == 0) red_s[gw * N + c0 + own] = x[0];
-                        }
+                        for (int n = 0; n < NC; ++n) z[n] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) top = fmaxf(top, z[n]);
+                    over |= top > 8.f;
+                    if (soft_any(group, over)) {
+                        float x[NC];
+#pragma unroll
+                        for (int n = 0; n < NC; ++n) x[n] = z[n];
+                        const int own = fold_columns(x, lane, [](float u, float w) { return fmaxf(u, w); });
+                        if (NC == 32 || (lane & 1) == 0) red_s[gw * N + c0 + own] = x[0];
                         soft_sync(group);
                         if (gt < NC) {
+                            // every column that sees a key of the item sees one in its first tile: there
+                            // the reference becomes the tile's maximum, later it moves only by more than 8
                             const int n = c0 + gt;
-                            float mt = fmaxf(red_s[n], red_s[N + n]);
-                            if (KT == 128) mt = fmaxf(mt, fmaxf(red_s[2 * N + n], red_s[3 * N + n]));
-                            const float mo = m_s[n], mn = mt > mo + 8.f ? mt : mo;
-                            corr_s[n] = fast_exp2(mo - mn);
-                            m_s[n] = mn;
+                            float up = fmaxf(fmaxf(red_s[n], red_s[N + n]), fmaxf(red_s[2 * N + n], red_s[3 * N + n]));
+                            if (j == 0 ? up == -INFINITY : !(up > 8.f)) up = 0.f;
+                            corr_s[n] = fast_exp2(-up);
+                            up_s[n] = up;
+                            m_s[n] += up;
                         }
                         soft_sync(group);
 #pragma unroll
-                        for (int n = 0; n < NC; ++n) l[n] *= corr_s[c0 + n];
+                        for (int n = 0; n < NC; ++n) z[n] -= up_s[c0 + n];
                         if (j > 0) {
+#pragma unroll
+                            for (int n = 0; n < NC; ++n) l[n] *= corr_s[c0 + n];
                             // the previous tile's products have landed: rescale the accumulator
                             const int pt = tile - 1;
                             wait(&p_free[pt % C::PB], (pt / C::PB) & 1);
@@ -737,17 +838,11 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                         uint8_t* P = smem + C::oP + pb * C::kP;
 #pragma unroll
                         for (int n0 = 0; n0 < NC; n0 += 8) {
+                            if (n0 >= nq) break;  // columns past the block's queries feed results nobody reads
                             float e[8];
 #pragma unroll
-                            for (int q = 0; q < 8; q += 4) {
-                                const float4 m = *reinterpret_cast<const float4*>(m_c + n0 + q);
-                                e[q] = fast_exp2(z[n0 + q] - m.x);
-                                e[q + 1] = fast_exp2(z[n0 + q + 1] - m.y);
-                                e[q + 2] = fast_exp2(z[n0 + q + 2] - m.z);
-                                e[q + 3] = fast_exp2(z[n0 + q + 3] - m.w);
-                            }
-#pragma unroll
                             for (int q = 0; q < 8; ++q) {
+                                e[q] = fast_exp2(z[n0 + q]);
                                 l[n0 + q] += e[q];
                                 if (Q8) e[q] *= ks;
                             }
@@ -756,13 +851,14 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                                     make_uint4(lat::pack2<T>(e[0], e[1]), lat::pack2<T>(e[2], e[3]),
                                                lat::pack2<T>(e[4], e[5]), lat::pack2<T>(e[6], e[7]));
                             } else {
-                                // K-major: query row n, key gt of the 64-key box gt / 64
+                                // K-major: query row n, key kt of the 64-key box kt / 64
 #pragma unroll
                                 for (int q = 0; q < 8; ++q)
-                                    *reinterpret_cast<T*>(P + (gt >> 6) * 2048 + sw128(n0 + q, (gt & 63) >> 3) + (gt & 7) * 2) =
+                                    *reinterpret_cast<T*>(P + (kt >> 6) * 2048 + sw128(n0 + q, (kt & 63) >> 3) + (kt & 7) * 2) =
                                         lat::from_f32<T>(e[q]);
                             }
                         }
+                        fence_proxy_async_smem();
                     }
                     tc_fence_before();
                     __syncwarp();
@@ -770,36 +866,25 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 }
                 const int ob = item % C::OB;
                 const uint32_t o = lane_base + C::kColO + ob * C::NP * N + c0;
-                const int nq = min(it.nq - c0, NC);  // the group's queries (none: <= 0)
-                const long long at = (a.merge ? 0 : it.split * rows) + it.q0 + c0;
-                // the prefix's share of the results: asked for before the sums are folded
-                if (!waited) {
+                if (joins && !waited) {
                     pdl_wait();
                     waited = true;
                 }
-                float2 ml0 = make_float2(kNoMax, 0.f);
-                float x0[16];
-                if (a.merge && it.np > 0) {
-                    if (gt < nq) ml0 = __ldcg(&a.part_ml[at + gt]);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x0[e] = e < nq ? __ldcg(a.part_o + (at + e) * KV + gt) : 0.f;
-                }
+                if (joins && !asked) ask(0, x0);
                 // the sums over the tile's keys
-                if (live) {
-                    const int own = fold_columns(l, lane, [](float u, float w) { return u + w; });
-                    if (NC == 32 || (lane & 1) == 0) red_s[gw * N + c0 + own] = l[0];
-                }
+                const int own = fold_columns(l, lane, [](float u, float w) { return u + w; });
+                if (NC == 32 || (lane & 1) == 0) red_s[gw * N + c0 + own] = l[0];
                 soft_sync(group);
                 float m_own = kNoMax, l_own = 0.f;  // of query c0 + gt
                 if (gt < NC) {
                     const int n = c0 + gt;
-                    l_own = red_s[n] + red_s[N + n];
-                    if (KT == 128) l_own += red_s[2 * N + n] + red_s[3 * N + n];
+                    l_own = (red_s[n] + red_s[N + n]) + (red_s[2 * N + n] + red_s[3 * N + n]);
                     if (*reinterpret_cast<volatile int*>(bad_s)) l_own = __int_as_float(0x7fc00000);
-                    m_own = m_s[n];
+                    m_own = l_own == 0.f ? kNoMax : m_s[n];
                 }
-                if (!a.merge) {
-                    if (gt < nq) a.part_ml[at + gt] = make_float2(m_own, l_own);
+                if (!direct) {
+                    const long long as = it.split * rows + at;
+                    if (gt < nq) a.part_ml[as + gt] = make_float2(m_own, l_own);
                     wait(&o_full[ob], (item / C::OB) & 1);
                     tc_fence_after();
 #pragma unroll 1
@@ -808,29 +893,30 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                         for (int c = 0; c < nq; c += 16) {
                             float v[16];
                             tmem_ld16(o + i * N + c, v);
-                            float* dst = a.part_o + (at + c) * KV + i * 128 + gt;
+                            float* dst = a.part_o + (as + c) * KV + i * 128 + gt;
 #pragma unroll
                             for (int e = 0; e < 16; ++e)
                                 if (c + e < nq) dst[static_cast<long long>(e) * KV] = v[e];
                         }
                 } else {
-                    // joint maximum and sum with the prefix's ranges; each part's factor, the division
-                    // by the sum included
+                    // joint maximum and sum with the prefix's ranges (at most kMaxJoin); each part's factor,
+                    // the division by the sum included
                     if (gt < nq) {
-                        float M = l_own == 0.f ? kNoMax : m_own;
-                        if (it.np > 0) M = fmaxf(M, ml0.x);
-                        for (int s = 1; s < it.np; ++s) M = fmaxf(M, __ldcg(&a.part_ml[s * rows + at + gt]).x);
-                        const float f = fast_exp2(m_own - M);
-                        float L = l_own * f + ml0.y * fast_exp2(ml0.x - M);
-                        for (int s = 1; s < it.np; ++s) {
-                            const float2 ml = __ldcg(&a.part_ml[s * rows + at + gt]);
-                            L += ml.y * fast_exp2(ml.x - M);
+                        float2 ml[kMaxJoin];
+                        float M = m_own;
+#pragma unroll
+                        for (int s = 0; s < kMaxJoin; ++s) {
+                            ml[s] = s == 0 ? ml0 : s < it.np ? __ldcg(&a.pre_ml[s * rows + at + gt]) : make_float2(kNoMax, 0.f);
+                            M = fmaxf(M, ml[s].x);
                         }
+                        const float f = fast_exp2(m_own - M);
+                        float L = l_own * f;
+#pragma unroll
+                        for (int s = 0; s < kMaxJoin; ++s) L += ml[s].y * fast_exp2(ml[s].x - M);
                         const float inv = L == 0.f ? 0.f : 1.f / L;
-                        m_s[c0 + gt] = M;
-                        lim_s[c0 + gt] = __float_as_int(inv);
                         corr_s[c0 + gt] = f * inv;
-                        red_s[N + c0 + gt] = fast_exp2(ml0.x - M) * inv;
+#pragma unroll
+                        for (int s = 0; s < kMaxJoin; ++s) red_s[s * N + c0 + gt] = fast_exp2(ml[s].x - M) * inv;
                         if (p.lse) p.lse[at + gt] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
                     }
                     if (it.nt > 0) {
@@ -838,6 +924,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                         tc_fence_after();
                     }
                     soft_sync(group);
+                    int u = 0;
 #pragma unroll 1
                     for (int i = 0; i < C::NP; ++i)
 #pragma unroll 1
@@ -851,27 +938,15 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
 #pragma unroll
                                 for (int e = 0; e < 16; ++e) v[e] = 0.f;
                             }
-                            if (it.np > 0) {
-                                if (i | c) {
-#pragma unroll
-                                    for (int e = 0; e < 16; ++e)
-                                        x0[e] = c + e < nq ? __ldcg(a.part_o + (at + c + e) * KV + i * 128 + gt) : 0.f;
-                                }
+#pragma unroll 1
+                            for (int s = 0; s < it.np; ++s, ++u) {
+                                float xn[16];
+                                if (u + 1 < it.np * cb * C::NP) ask(u + 1, xn);
 #pragma unroll
                                 for (int e = 0; e < 16; ++e)
-                                    if (c + e < nq) v[e] = fmaf(x0[e], red_s[N + c0 + c + e], v[e]);
-                            }
-                            for (int s = 1; s < it.np; ++s) {
-                                const long long as = s * rows + at + c;
-                                float x[16];
+                                    if (c + e < nq) v[e] = fmaf(x0[e], red_s[s * N + c0 + c + e], v[e]);
 #pragma unroll
-                                for (int e = 0; e < 16; ++e)
-                                    x[e] = c + e < nq ? __ldcg(a.part_o + (as + e) * KV + i * 128 + gt) : 0.f;
-#pragma unroll
-                                for (int e = 0; e < 16; ++e)
-                                    if (c + e < nq)
-                                        v[e] += x[e] * (fast_exp2(__ldcg(&a.part_ml[as + e]).x - m_s[c0 + c + e]) *
-                                                        __int_as_float(lim_s[c0 + c + e]));
+                                for (int e = 0; e < 16; ++e) x0[e] = xn[e];
                             }
                             T* dst = static_cast<T*>(p.out) + (at + c) * KV + i * 128 + gt;
 #pragma unroll
@@ -899,18 +974,20 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
 }
 
 // Joins the partials of a query row: its group's prefix ranges and its suffix ranges. One warp
-// per query row, V columns per lane and pass; grid-stride.
+// per query row, kv / 32 columns per lane.
 template <int KV, typename T>
 __global__ void __launch_bounds__(256) shared_prefix_join_kernel(const Problem p, const float* __restrict__ pre_o,
                                                                  const float2* __restrict__ pre_ml, int pre_kps,
                                                                  const float* __restrict__ suf_o,
-                                                                 const float2* __restrict__ suf_ml, int suf_kps) {
+                                                                 const float2* __restrict__ suf_ml, int suf_kps,
+                                                                 int direct) {
     MM_PDL_ENTRY();
     const int th = p.T * p.H, lane = threadIdx.x & 31;
     const long long rows = static_cast<long long>(p.B) * th;
     const long long r = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
     if (r >= rows) return;
     const int b = static_cast<int>(r / th);
+    if (direct && direct_join(p, b, suf_kps, pre_kps) >= 0) return;  // the suffix launch wrote it
     const int g = p.G > 0 ? group_of(p, b) : -1;
     const int np = (prefix_length(p, g) + pre_kps - 1) / pre_kps;
     const int ns = (suffix_length(p, b) + suf_kps - 1) / suf_kps;
