@@ -267,7 +267,7 @@ Plan plan(const mm::spa::Problem& p) {
         pick_splits(r.suf_blocks, p.max_suffix, 16, r.suf_splits, r.suf_kps);
         if (const char* e = std::getenv("MM_SPA_SUF")) { r.suf_kps = std::atoi(e); r.suf_splits = (p.max_suffix + r.suf_kps - 1) / r.suf_kps; }
     }
-    r.join = !r.suf_n || r.suf_splits > 1 || r.pre_splits > mm::spa::kMaxJoin;
+    r.join = r.suf_n != 16 || r.suf_splits > 1 || r.pre_splits > mm::spa::kMaxJoin;
     if (r.join) r.suf_part = r.rows * r.suf_splits;
     if (r.pre_blocks * std::max(1, r.pre_splits) > kMaxBlocks || r.suf_blocks * std::max(1, r.suf_splits) > kMaxBlocks)
         refuse(MM_UNSUPPORTED, "shared-prefix attention: too many query rows");
@@ -319,7 +319,7 @@ void run_tc(const mm::spa::Problem& p, const Plan& r, bool q8p, bool q8s, void* 
     if (r.join)
         launch(s, shared_prefix_join_kernel<KV, T>, dim3(blocks(r.rows, 8)), dim3(256), 0, p, static_cast<const float*>(pre_o),
                static_cast<const float2*>(pre_ml), r.pre_kps, static_cast<const float*>(suf_o),
-               static_cast<const float2*>(suf_ml), r.suf_kps, r.suf_n ? 1 : 0);
+               static_cast<const float2*>(suf_ml), r.suf_kps, r.suf_n == 16 ? 1 : 0);
 }
 
 }  // namespace

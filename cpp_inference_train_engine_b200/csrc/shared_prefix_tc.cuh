@@ -48,6 +48,7 @@ struct TcArgs {
     float2* part_ml;
     // a suffix launch writes the results of the rows whose suffix is one range (or empty) itself and
     // joins the prefix launch's partials (at most kMaxJoin ranges of prefix_kps keys) to them
+    // (16-query blocks only: with 64 the registers are needed for the tiles)
     const float* pre_o;
     const float2* pre_ml;
     int prefix_kps;
@@ -232,7 +233,7 @@ template <int N> __device__ __forceinline__ Unit get_unit(const TcArgs& a, int u
         r.q0 = u * th;
         r.nq = th;
         r.len = suffix_length(p, u);
-        r.np = direct_join(p, u, a.kps, a.prefix_kps);
+        if (N == 16) r.np = direct_join(p, u, a.kps, a.prefix_kps);
     } else {
         const int b0 = min(max(p.group_start[u], 0), p.B), b1 = min(max(p.group_start[u + 1], b0), p.B);
         r.q0 = b0 * th;
@@ -699,7 +700,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             const int count = next_table(base);
             for (int e0 = 0; e0 < count; ++e0) {
                 const Item it = table[e0];
-                const bool direct = it.np >= 0;
+                const bool direct = N == 16 && it.np >= 0;
                 if (it.nt == 0 && !direct) continue;
                 const int nq = min(it.nq - c0, NC);  // the group's queries (none: <= 0)
                 float l[NC];
@@ -709,7 +710,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 // The prefix's share of a direct result: unit u = (16-column block, prefix range) of the
                 // partials, 16 queries of this thread's dimension. Unit 0 is asked for before the tiles:
                 // a load issued behind a full ring of cache tiles waits its turn (2 to 4 us).
-                const bool joins = it.np > 0 && nq > 0;
+                const bool joins = direct && it.np > 0 && nq > 0;
                 const int cb = (nq + 15) / 16;
                 float x0[16];
                 float2 ml0 = make_float2(kNoMax, 0.f);
@@ -720,7 +721,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     for (int e = 0; e < 16; ++e) x[e] = c + e < nq ? __ldcg(src + static_cast<long long>(e) * KV) : 0.f;
                     if (u == 0 && gt < nq) ml0 = __ldcg(&a.pre_ml[at + gt]);
                 };
-                const bool asked = N == 16 && joins && waited;
+                const bool asked = joins && waited;
                 if (asked) ask(0, x0);
                 // keys of the item each query sees; the tokens of a suffix end one position apart
                 const bool causal = a.suffix && p.T > 1;
