@@ -25,7 +25,7 @@
 //              cp.async; e4m3 codes are loaded D tiles ahead into registers and stored as 16-bit
 //              values (exact). Rows past the range are zero-filled, so whatever the cache holds
 //              there never reaches a product.
-//   fence      one thread passes each landed box on to the asynchronous proxy: a proxy fence costs
+//   fence      one thread passes each landed tile on to the asynchronous proxy: a proxy fence costs
 //              about 100 ns, and in the loading threads it would wait for every load they have in
 //              flight (measured: 1.7 instead of over 5 TB/s).
 //   MMA        one thread issues tcgen05.mma. With KT = 64 the S^T product has M = 64, whose row r
@@ -71,7 +71,7 @@ struct Item {
 
 template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int NP = KV / 128;                    // 128-column pairs of boxes
-    static constexpr int KT = KV == 512 && N == 16 ? 64 : 128;  // keys per tile
+    static constexpr int KT = KV == 512 ? 64 : 128;        // keys per tile
     static constexpr int kBox = KT * 128;                  // KT keys x 64 columns of 16 bits
     static constexpr int kPair = 2 * kBox;
     static constexpr int kRope = KT * R * 2;
@@ -79,19 +79,17 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int kQBox = N * 128;
     static constexpr int kQ = 2 * NP * kQBox + N * R * 2;  // N query rows
     static constexpr int kQA = (kQ + 1023) / 1024 * 1024;
-    // P^T: N = 64: one MN-major box [128 keys x 64 queries]; N = 16: K-major boxes of 64 keys
-    static constexpr int kP = N == 64 ? 128 * 128 : KT / 64 * 16 * 128;
+    // P^T: N = 64: one MN-major box [KT keys x 64 queries]; N = 16: K-major boxes of 64 keys
+    static constexpr int kP = N == 64 ? KT * 128 : KT / 64 * 16 * 128;
     // CTAs per SM, and rings: queries, pairs, rope boxes, P buffers, O accumulators (what 227 KB
     // and 512 tensor memory columns hold)
     static constexpr int kCtas = KV == 128 && N == 16 ? 2 : 1;
     static constexpr int QB = KV == 512 && N == 64 ? 1 : 2;
-    static constexpr int PS = KV == 512 ? (N == 64 ? 4 : 10) : (N == 64 ? 4 : 2);
-    static constexpr int RS = KV == 512 ? (N == 64 ? 1 : 3) : PS;
-    static constexpr int PB = KV == 512 && N == 64 ? 1 : 2;
+    static constexpr int PS = KV == 512 ? (N == 64 ? 8 : 10) : (N == 64 ? 4 : 2);
+    static constexpr int RS = KV == 512 ? (N == 64 ? 2 : 3) : PS;
+    static constexpr int PB = 2;
+    static constexpr int TS = 4;  // tiles announced: more than the pair ring ever holds
     static constexpr int OB = KV == 512 && N == 64 ? 1 : 2;
-    // order of the products: 0 tile by tile (the ring holds one), 1 S one tile ahead and pair by pair
-    // as it lands, 2 S or O, whichever can go
-    static constexpr int kOrder = PS < 2 * NP ? 0 : KV == 128 || Q8 ? 2 : 1;
     // tensor memory columns: two S buffers (e4m3: two more for the rope columns' share, which the
     // key's scale does not multiply), then the O accumulators
     static constexpr int kColS = 0, kColR = 2 * N, kColO = Q8 ? 4 * N : 2 * N;
@@ -112,7 +110,7 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N], up[N]
     static constexpr int oPlan = oF + 8 * N * 4;
     static constexpr int oBar = oPlan + (kTcMaxPlan + 1) * 4 + 4;
-    static constexpr int kBars = QB + 3 * PS + 3 * RS + 4 + 2 * PB + 2 * OB;
+    static constexpr int kBars = QB + 2 * PS + 2 * RS + TS + 4 + 2 * PB + 2 * OB;
     static constexpr int kSmem = oBar + kBars * 8 + 16 + 1024;  // + alignment of the base
     static_assert(kCtas * (kSmem + 1024) <= 228 * 1024 && kCols * kCtas <= 512, "shared and tensor memory");
 };
@@ -279,6 +277,18 @@ __device__ __forceinline__ Item get_item(const TcArgs& a, const int* plan, int u
     return it;
 }
 
+// Position in a ring of S barriers: the slot and its phase parity.
+template <int S> struct Ring {
+    int i = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++i == S) {
+            i = 0;
+            phase ^= 1;
+        }
+    }
+};
+
 // Cursor over the tiles of a table's items that have any.
 struct Cursor {
     const Item* tab;
@@ -318,12 +328,11 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::oBar);
     uint64_t* q_empty = bars;                    // [QB] the item's S products have read Q
     uint64_t* pair_in = q_empty + C::QB;         // [PS] the producer threads (e4m3: warps)
-    uint64_t* pair_full = pair_in + C::PS;       // [PS] the fence warp
-    uint64_t* pair_empty = pair_full + C::PS;    // [PS] O products done with the pair
+    uint64_t* pair_empty = pair_in + C::PS;      // [PS] O products done with the pair
     uint64_t* rope_in = pair_empty + C::PS;      // [RS] the producer threads (the item's queries included)
-    uint64_t* rope_full = rope_in + C::RS;       // [RS] the fence warp
-    uint64_t* rope_empty = rope_full + C::RS;    // [RS]
-    uint64_t* s_full = rope_empty + C::RS;       // [2]
+    uint64_t* rope_empty = rope_in + C::RS;      // [RS]
+    uint64_t* tile_full = rope_empty + C::RS;    // [TS] the fence warp: the tile's boxes can be read
+    uint64_t* s_full = tile_full + C::TS;        // [2]
     uint64_t* s_free = s_full + 2;               // [2] the softmax warps
     uint64_t* p_full = s_free + 2;               // [PB] the softmax warps
     uint64_t* p_free = p_full + C::PB;           // [PB] the tile's O products are complete
@@ -341,14 +350,13 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             for (int i = 0; i < C::QB; ++i) mbar_init(&q_empty[i], 1);
             for (int i = 0; i < C::PS; ++i) {
                 mbar_init(&pair_in[i], Q8 ? C::PW : C::PT);
-                mbar_init(&pair_full[i], 1);
                 mbar_init(&pair_empty[i], 1);
             }
             for (int i = 0; i < C::RS; ++i) {
                 mbar_init(&rope_in[i], C::PT);
-                mbar_init(&rope_full[i], 1);
                 mbar_init(&rope_empty[i], 1);
             }
+            for (int i = 0; i < C::TS; ++i) mbar_init(&tile_full[i], 1);
             for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_free[i], C::SW); }
             for (int i = 0; i < C::PB; ++i) { mbar_init(&p_full[i], C::SW); mbar_init(&p_free[i], 1); }
             for (int i = 0; i < C::OB; ++i) { mbar_init(&o_full[i], 1); mbar_init(&o_free[i], C::SW); }
@@ -448,28 +456,30 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
 #pragma unroll
             for (int r = r0; r < KT; r += kRows) cp_async16(d + sw_rope<R>(r, c), src + (r < left ? r : 0) * ps, r < left);
         };
-        int qi = -1, tile = 0, pr = 0;
+        Ring<C::QB> rq;
+        Ring<C::RS> rr;
+        Ring<C::PS> rp;
         if constexpr (!Q8) {
             const int cc = pt & 15, r0 = pt >> 4;  // 16-byte chunk of the pair's row, first row
             const long long ps = 2 * cv.pos_stride;
             for (int base = 0; base < mine; base += kTcTable) {
                 const int count = next_table(base);
-                for (Cursor c(table, count); c.valid(); c.next(), ++tile) {
+                for (Cursor c(table, count); c.valid(); c.next(), rr.next()) {
                     const Item& it = c.item();
-                    wait(&rope_empty[tile % C::RS], ((tile / C::RS) & 1) ^ 1);
+                    wait(&rope_empty[rr.i], rr.phase ^ 1);
                     if (c.j == 0) {
-                        ++qi;
-                        wait(&q_empty[qi % C::QB], ((qi / C::QB) & 1) ^ 1);
-                        load_q(it, qi % C::QB);
+                        wait(&q_empty[rq.i], rq.phase ^ 1);
+                        load_q(it, rq.i);
+                        rq.next();
                     }
-                    load_rope(it, c.j, tile % C::RS);
-                    cp_async_arrive(&rope_in[tile % C::RS]);
+                    load_rope(it, c.j, rr.i);
+                    cp_async_arrive(&rope_in[rr.i]);
                     const int left = it.nk - c.j * KT;
                     const uint8_t* src = cv.latent + 2 * (it.row * cv.row_stride) + (it.k0 + c.j * KT) * ps + cc * 16;
 #pragma unroll 1
-                    for (int i = 0; i < C::NP; ++i, ++pr, src += 256) {
-                        const int slot = pr % C::PS;
-                        wait(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
+                    for (int i = 0; i < C::NP; ++i, rp.next(), src += 256) {
+                        const int slot = rp.i;
+                        wait(&pair_empty[slot], rp.phase ^ 1);
                         uint8_t* d = sPair + slot * C::kPair + (cc >> 3) * C::kBox;
 #pragma unroll
                         for (int k = 0; k < KT * 16 / C::PT; ++k) {
@@ -514,20 +524,21 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
 #pragma unroll
                     for (int d = 0; d < D; ++d) {
                         if (sc.valid()) {
-                            wait(&rope_empty[tile % C::RS], ((tile / C::RS) & 1) ^ 1);
+                            wait(&rope_empty[rr.i], rr.phase ^ 1);
                             if (sc.j == 0) {
-                                ++qi;
-                                wait(&q_empty[qi % C::QB], ((qi / C::QB) & 1) ^ 1);
-                                load_q(sc.item(), qi % C::QB);
+                                wait(&q_empty[rq.i], rq.phase ^ 1);
+                                load_q(sc.item(), rq.i);
+                                rq.next();
                             }
-                            load_rope(sc.item(), sc.j, tile % C::RS);
-                            cp_async_arrive(&rope_in[tile % C::RS]);
+                            load_rope(sc.item(), sc.j, rr.i);
+                            cp_async_arrive(&rope_in[rr.i]);
+                            rr.next();
                             const bool more = lc.valid();
                             if (more) at_tile(lc);
 #pragma unroll
-                            for (int i = 0; i < C::NP; ++i, ++pr) {
-                                const int slot = pr % C::PS;
-                                wait(&pair_empty[slot], ((pr / C::PS) & 1) ^ 1);
+                            for (int i = 0; i < C::NP; ++i, rp.next()) {
+                                const int slot = rp.i;
+                                wait(&pair_empty[slot], rp.phase ^ 1);
                                 uint8_t* dst = sPair + slot * C::kPair + (cc >> 2) * C::kBox;
 #pragma unroll
                                 for (int k = 0; k < C::VPT; ++k) {
@@ -549,7 +560,6 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                             }
                             if (more) lc.next();
                             sc.next();
-                            ++tile;
                         }
                     }
                 }
@@ -565,119 +575,111 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                        aP = smem_u32(smem + C::oP);
         // descriptors advance by address / 16 (shared memory ends below 2^18, so no field overflows)
         const uint64_t kd = umma_desc_sw128(aPair, 16, 1024), vd = umma_desc_sw128(aPair, C::kBox, 1024);
-        int s_tile = 0, s_pr = 0, s_q = 0;     // S products: tile, pair and item counters
-        int o_tile = 0, o_pr = 0, o_item = 0;  // O products
-        auto s_ready = [&] {
-            bool r = mbar_test(&s_free[s_tile & 1], ((s_tile >> 1) & 1) ^ 1) &&
-                     mbar_test(&rope_full[s_tile % C::RS], (s_tile / C::RS) & 1);
-            for (int i = 0; i < C::NP && r; ++i) r = mbar_test(&pair_full[(s_pr + i) % C::PS], ((s_pr + i) / C::PS) & 1);
-            return r;
-        };
+        // positions of the S side and of the O side, and how many tiles S is ahead. This thread's
+        // instructions are on the path of every tile: positions are kept instead of computed, and a
+        // tile's boxes are waited for as one.
+        Ring<C::PS> sp, op;
+        Ring<C::RS> sr;
+        Ring<C::TS> st;
+        Ring<C::QB> sq;
+        Ring<2> ss;
+        Ring<C::PB> pb;
+        Ring<C::OB> ob;
+        int ahead = 0;
         auto issue_s = [&](Cursor& c) {
-            const uint32_t q = aQ + (s_q % C::QB) * C::kQA;
-            const uint64_t qd = umma_desc_sw128(q, 16, 1024);
-            const int sb = s_tile & 1, rs = s_tile % C::RS;
-            const uint32_t d = tmem + C::kColS + sb * N;
-            wait(&s_free[sb], ((s_tile >> 1) & 1) ^ 1);
-            wait(&rope_full[rs], (s_tile / C::RS) & 1);
+            const uint32_t q = aQ + sq.i * C::kQA, d = tmem + C::kColS + ss.i * N;
             tc_fence_after();
             {
-                const uint64_t ka = rope_desc<R>(aR + rs * C::kRopeA), qa = rope_desc<R>(q + 2 * C::NP * C::kQBox);
-                const uint32_t dr = Q8 ? tmem + C::kColR + sb * N : d;
+                const uint64_t ka = rope_desc<R>(aR + sr.i * C::kRopeA), qa = rope_desc<R>(q + 2 * C::NP * C::kQBox);
+                const uint32_t dr = Q8 ? tmem + C::kColR + ss.i * N : d;
 #pragma unroll
                 for (int k = 0; k < R / 16; ++k) tc_mma_f16(dr, ka + k * 2, qa + k * 2, id_s, k ? 1u : 0u);
             }
-            tc_commit(&rope_empty[rs]);
-#pragma unroll 1
-            for (int i = 0; i < C::NP; ++i, ++s_pr) {  // pair by pair as the boxes land
-                const int slot = s_pr % C::PS;
-                wait(&pair_full[slot], (s_pr / C::PS) & 1);
-                const uint64_t ka = kd + static_cast<uint32_t>(slot * (C::kPair >> 4));
-                const uint64_t qa = qd + static_cast<uint32_t>(i * (2 * C::kQBox >> 4));
+            tc_commit(&rope_empty[sr.i]);
+            sr.next();
+            const uint64_t qd = umma_desc_sw128(q, 16, 1024);
+#pragma unroll
+            for (int i = 0; i < C::NP; ++i) {
+                const uint64_t ka = kd + static_cast<uint32_t>(sp.i * (C::kPair >> 4));
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    tc_mma_f16(d, ka + ((k >> 2) * C::kBox + (k & 3) * 32) / 16, qa + ((k >> 2) * C::kQBox + (k & 3) * 32) / 16,
-                               id_s, Q8 ? ((i | k) ? 1u : 0u) : 1u);
+                    tc_mma_f16(d, ka + ((k >> 2) * C::kBox + (k & 3) * 32) / 16,
+                               qd + (2 * i * C::kQBox + (k >> 2) * C::kQBox + (k & 3) * 32) / 16, id_s,
+                               Q8 && i == 0 && k == 0 ? 0u : 1u);
+                sp.next();
             }
-            tc_commit(&s_full[sb]);
+            tc_commit(&s_full[ss.i]);
+            ss.next();
+            st.next();
             if (c.last()) {
-                tc_commit(&q_empty[s_q % C::QB]);
-                ++s_q;
+                tc_commit(&q_empty[sq.i]);
+                sq.next();
             }
-            ++s_tile;
+            ++ahead;
             c.next();
         };
         auto issue_o = [&](Cursor& c) {
-            const int ob = o_item % C::OB, pb = o_tile % C::PB;
-            if (c.j == 0) wait(&o_free[ob], ((o_item / C::OB) & 1) ^ 1);
-            wait(&p_full[pb], (o_tile / C::PB) & 1);
+            if (c.j == 0) wait(&o_free[ob.i], ob.phase ^ 1);
             tc_fence_after();
-            const uint64_t pa = umma_desc_sw128(aP + pb * C::kP, N == 64 ? C::kBox : 16, 1024);
-#pragma unroll 1
-            for (int i = 0; i < C::NP; ++i, ++o_pr) {
-                const int slot = o_pr % C::PS;
-                const uint64_t va = vd + static_cast<uint32_t>(slot * (C::kPair >> 4));
-                const uint32_t d = tmem + C::kColO + (ob * C::NP + i) * N;
+            const uint64_t pa = umma_desc_sw128(aP + pb.i * C::kP, N == 64 ? C::kBox : 16, 1024);
+            const uint32_t d = tmem + C::kColO + ob.i * C::NP * N;
+            const uint32_t first = c.j ? 1u : 0u;
+#pragma unroll
+            for (int i = 0; i < C::NP; ++i) {
+                const uint64_t va = vd + static_cast<uint32_t>(op.i * (C::kPair >> 4));
 #pragma unroll
                 for (int k = 0; k < KT / 16; ++k)
                     // V^T MN-major: 16 keys = 2,048 B down a box, the next 64 columns one box on
-                    tc_mma_f16(d, va + k * 128, pa + (N == 64 ? k * 128 : ((k >> 2) * 2048 + (k & 3) * 32) / 16), id_o,
-                               (c.j | k) ? 1u : 0u);
-                tc_commit(&pair_empty[slot]);
+                    tc_mma_f16(d + i * N, va + k * 128, pa + (N == 64 ? k * 128 : ((k >> 2) * 2048 + (k & 3) * 32) / 16), id_o,
+                               k ? 1u : first);
+                tc_commit(&pair_empty[op.i]);
+                op.next();
             }
-            tc_commit(&p_free[pb]);
+            tc_commit(&p_free[pb.i]);
+            pb.next();
             if (c.last()) {
-                tc_commit(&o_full[ob]);
-                ++o_item;
+                tc_commit(&o_full[ob.i]);
+                ob.next();
             }
-            ++o_tile;
+            --ahead;
             c.next();
         };
-        int f_tile = 0, f_pr = 0;
+        Ring<C::RS> fr;
+        Ring<C::PS> fp;
+        Ring<C::TS> ft;
         for (int base = 0; base < mine; base += kTcTable) {
             const int count = next_table(base);
             if (warp == kFenceWarp && lane == 0) {
                 // what has been written in the generic proxy (copies, converted codes) becomes
                 // readable by the products
-                for (Cursor c(table, count); c.valid(); c.next(), ++f_tile) {
-                    wait(&rope_in[f_tile % C::RS], (f_tile / C::RS) & 1);
-                    fence_proxy_async_smem();
-                    mbar_arrive(&rope_full[f_tile % C::RS]);
-                    for (int i = 0; i < C::NP; ++i, ++f_pr) {
-                        wait(&pair_in[f_pr % C::PS], (f_pr / C::PS) & 1);
-                        fence_proxy_async_smem();
-                        mbar_arrive(&pair_full[f_pr % C::PS]);
+                for (Cursor c(table, count); c.valid(); c.next(), fr.next()) {
+                    wait(&rope_in[fr.i], fr.phase);
+                    for (int i = 0; i < C::NP; ++i, fp.next()) {
+                        wait(&pair_in[fp.i], fp.phase);
                     }
+                    fence_proxy_async_smem();
+                    mbar_arrive(&tile_full[ft.i]);
+                    ft.next();
                 }
             }
             if (warp == kMmaWarp && elect_one()) {
                 Cursor cs(table, count), co(table, count);
-                if (C::kOrder == 2) {
-                    // the next tile's S when its boxes are there, this tile's O when its probabilities are:
-                    // neither waits behind the other
-                    int polls = 0;
-                    while (co.valid()) {
-                        const bool late = !ok || polls > (1 << 24);  // gave up: go on in order, waits and all
-                        if (cs.valid() && s_tile - o_tile < 2 && (s_ready() || (late && s_tile == o_tile))) {
-                            issue_s(cs);
-                            polls = 0;
-                        } else if (s_tile > o_tile && (late || mbar_test(&p_full[o_tile % C::PB], (o_tile / C::PB) & 1))) {
-                            issue_o(co);
-                            polls = 0;
-                        } else {
-                            ++polls;
-                        }
-                    }
-                } else if (C::kOrder == 1) {
-                    if (cs.valid()) issue_s(cs);
-                    while (co.valid()) {
-                        if (cs.valid()) issue_s(cs);
+                // a tile's O when its probabilities are there, else the next tile's S when its boxes are:
+                // neither waits behind the other
+                int polls = 0;
+                while (co.valid()) {
+                    if (ahead > 0 && mbar_test(&p_full[pb.i], pb.phase)) {
                         issue_o(co);
-                    }
-                } else {
-                    while (co.valid()) {
+                        polls = 0;
+                    } else if (ahead < 2 && cs.valid() && mbar_test(&tile_full[st.i], st.phase) &&
+                               mbar_test(&s_free[ss.i], ss.phase ^ 1)) {
                         issue_s(cs);
-                        issue_o(co);
+                        polls = 0;
+                    } else if (!ok || ++polls > (1 << 24)) {  // gave up: go on in order without waiting
+                        ok = false;
+                        *reinterpret_cast<volatile int*>(bad_s) = 1;
+                        if (ahead == 0) issue_s(cs);
+                        else issue_o(co);
                     }
                 }
             }
@@ -848,7 +850,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                                 if (Q8) e[q] *= ks;
                             }
                             if constexpr (N == 64) {
-                                *reinterpret_cast<uint4*>(P + sw128(gt, (c0 + n0) >> 3)) =
+                                *reinterpret_cast<uint4*>(P + sw128(kt, (c0 + n0) >> 3)) =
                                     make_uint4(lat::pack2<T>(e[0], e[1]), lat::pack2<T>(e[2], e[3]),
                                                lat::pack2<T>(e[4], e[5]), lat::pack2<T>(e[6], e[7]));
                             } else {
