@@ -21,7 +21,7 @@
 //              vote; otherwise the column maxima are taken and O^T and the sums are rescaled. A key's scale (e4m3) multiplies its latent
 //              scores and, for the second product, its probabilities.
 //   producers  2 to 8: the item's queries, then per tile of KT keys the rope columns and kv / 128 pairs
-//              of 64-column boxes into rings of swizzled boxes. 16-bit caches go by 16-byte
+//              of 64-column boxes (each pair its own warps) into rings of swizzled boxes. 16-bit caches go by 16-byte
 //              cp.async; e4m3 codes are loaded D tiles ahead into registers and stored as 16-bit
 //              values (exact). Rows past the range are zero-filled, so whatever the cache holds
 //              there never reaches a product.
@@ -100,8 +100,10 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int SG = N == 64 ? 2 : 1, NC = N / SG, SW = 4 * SG;
     static constexpr int PW = N == 64 ? 4 : KV == 512 ? (Q8 ? 8 : 4) : 2, PT = 32 * PW;
     static constexpr int kThreads = 32 * (SW + PW + (N == 64 ? 4 : 2));
-    // e4m3: 16-byte loads per pair and thread, tiles ahead in registers
-    static constexpr int VPT = KT * 8 / PT, D = KV == 512 ? (N == 16 ? 2 : 1) : (N == 16 ? 1 : 3);
+    // producer warps per pair of a tile
+    static constexpr int WPP = PW / NP;
+    // e4m3: 16-byte loads per tile and thread, tiles ahead in registers
+    static constexpr int VPT = KT * 8 / (32 * WPP), D = KV == 512 ? (N == 16 ? 2 : 1) : (N == 16 ? 1 : 3);
     static constexpr int oPair = 0;
     static constexpr int oQ = oPair + PS * kPair;
     static constexpr int oRope = oQ + QB * kQA;
@@ -110,7 +112,8 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N], up[N]
     static constexpr int oPlan = oF + 8 * N * 4;
     static constexpr int oBar = oPlan + (kTcMaxPlan + 1) * 4 + 4;
-    static constexpr int kBars = QB + 2 * PS + 2 * RS + TS + 4 + 2 * PB + 2 * OB;
+    static constexpr int kBars = QB + PS + 2 * TS + 4 + 2 * PB + 2 * OB;
+    static_assert(RS * NP >= PS && TS * NP >= PS, "the rope ring and the tile barriers outlast the pair ring");
     static constexpr int kSmem = oBar + kBars * 8 + 16 + 1024;  // + alignment of the base
     static_assert(kCtas * (kSmem + 1024) <= 228 * 1024 && kCols * kCtas <= 512, "shared and tensor memory");
 };
@@ -287,6 +290,12 @@ template <int S> struct Ring {
             phase ^= 1;
         }
     }
+    __device__ __forceinline__ void skip(int n) {
+        if ((i += n) >= S) {
+            i -= S;
+            phase ^= 1;
+        }
+    }
 };
 
 // Cursor over the tiles of a table's items that have any.
@@ -327,11 +336,9 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     int* plan_s = reinterpret_cast<int*>(smem + C::oPlan);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::oBar);
     uint64_t* q_empty = bars;                    // [QB] the item's S products have read Q
-    uint64_t* pair_in = q_empty + C::QB;         // [PS] the producer threads (e4m3: warps)
-    uint64_t* pair_empty = pair_in + C::PS;      // [PS] O products done with the pair
-    uint64_t* rope_in = pair_empty + C::PS;      // [RS] the producer threads (the item's queries included)
-    uint64_t* rope_empty = rope_in + C::RS;      // [RS]
-    uint64_t* tile_full = rope_empty + C::RS;    // [TS] the fence warp: the tile's boxes can be read
+    uint64_t* pair_empty = q_empty + C::QB;      // [PS] O products done with the pair
+    uint64_t* tile_in = pair_empty + C::PS;      // [TS] the producer threads
+    uint64_t* tile_full = tile_in + C::TS;       // [TS] the fence warp: the tile's boxes can be read
     uint64_t* s_full = tile_full + C::TS;        // [2]
     uint64_t* s_free = s_full + 2;               // [2] the softmax warps
     uint64_t* p_full = s_free + 2;               // [PB] the softmax warps
@@ -348,15 +355,8 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     if (warp == kMmaWarp) {
         if (lane == 0) {
             for (int i = 0; i < C::QB; ++i) mbar_init(&q_empty[i], 1);
-            for (int i = 0; i < C::PS; ++i) {
-                mbar_init(&pair_in[i], Q8 ? C::PW : C::PT);
-                mbar_init(&pair_empty[i], 1);
-            }
-            for (int i = 0; i < C::RS; ++i) {
-                mbar_init(&rope_in[i], C::PT);
-                mbar_init(&rope_empty[i], 1);
-            }
-            for (int i = 0; i < C::TS; ++i) mbar_init(&tile_full[i], 1);
+            for (int i = 0; i < C::PS; ++i) mbar_init(&pair_empty[i], 1);
+            for (int i = 0; i < C::TS; ++i) { mbar_init(&tile_in[i], C::PT + (Q8 ? C::PW : 0)); mbar_init(&tile_full[i], 1); }
             for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_free[i], C::SW); }
             for (int i = 0; i < C::PB; ++i) { mbar_init(&p_full[i], C::SW); mbar_init(&p_free[i], 1); }
             for (int i = 0; i < C::OB; ++i) { mbar_init(&o_full[i], 1); mbar_init(&o_free[i], C::SW); }
@@ -456,58 +456,70 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
 #pragma unroll
             for (int r = r0; r < KT; r += kRows) cp_async16(d + sw_rope<R>(r, c), src + (r < left ? r : 0) * ps, r < left);
         };
+        // WPP warps per pair of a tile, so that the pairs' waits and copies run side by side; a tile
+        // (and the item's queries with its first) is announced by one arrival per thread (e4m3: and warp). The rope
+        // ring holds at least the tiles of the pair ring: its boxes are free when the pair's are.
+        const int pw = warp - C::SW, own = pw / C::WPP, sub = pw % C::WPP;
         Ring<C::QB> rq;
         Ring<C::RS> rr;
+        Ring<C::TS> rt;
         Ring<C::PS> rp;
+        rp.i = own;
+        auto begin_tile = [&](const Item& it, int j) {
+            wait(&pair_empty[rp.i], rp.phase ^ 1);
+            if (j == 0) {
+                wait(&q_empty[rq.i], rq.phase ^ 1);
+                load_q(it, rq.i);
+                rq.next();
+            }
+            load_rope(it, j, rr.i);
+            rr.next();
+        };
+        auto end_tile = [&] {
+            cp_async_arrive(&tile_in[rt.i]);
+            if (Q8) {  // the warp's converted codes
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&tile_in[rt.i]);
+            }
+            rt.next();
+            rp.skip(C::NP);
+        };
         if constexpr (!Q8) {
-            const int cc = pt & 15, r0 = pt >> 4;  // 16-byte chunk of the pair's row, first row
+            const int cc = lane & 15, r0 = (lane >> 4) + 2 * sub;  // 16-byte chunk of the pair's row, first row
             const long long ps = 2 * cv.pos_stride;
             for (int base = 0; base < mine; base += kTcTable) {
                 const int count = next_table(base);
-                for (Cursor c(table, count); c.valid(); c.next(), rr.next()) {
+                for (Cursor c(table, count); c.valid(); c.next()) {
                     const Item& it = c.item();
-                    wait(&rope_empty[rr.i], rr.phase ^ 1);
-                    if (c.j == 0) {
-                        wait(&q_empty[rq.i], rq.phase ^ 1);
-                        load_q(it, rq.i);
-                        rq.next();
-                    }
-                    load_rope(it, c.j, rr.i);
-                    cp_async_arrive(&rope_in[rr.i]);
+                    begin_tile(it, c.j);
                     const int left = it.nk - c.j * KT;
-                    const uint8_t* src = cv.latent + 2 * (it.row * cv.row_stride) + (it.k0 + c.j * KT) * ps + cc * 16;
-#pragma unroll 1
-                    for (int i = 0; i < C::NP; ++i, rp.next(), src += 256) {
-                        const int slot = rp.i;
-                        wait(&pair_empty[slot], rp.phase ^ 1);
-                        uint8_t* d = sPair + slot * C::kPair + (cc >> 3) * C::kBox;
-#pragma unroll
-                        for (int k = 0; k < KT * 16 / C::PT; ++k) {
-                            const int r = r0 + C::PT / 16 * k;
-                            cp_async16(d + sw128(r, cc & 7), src + (r < left ? r : 0) * ps, r < left);
-                        }
-                        cp_async_arrive(&pair_in[slot]);
+                    const uint8_t* first = cv.latent + 2 * (it.row * cv.row_stride) + (it.k0 + c.j * KT) * ps + own * 256 + cc * 16;
+                    const uint8_t* src = first + r0 * ps;
+                    uint8_t* d = sPair + rp.i * C::kPair + (cc >> 3) * C::kBox;
+#pragma unroll 16
+                    for (int r = r0; r < KT; r += 2 * C::WPP) {
+                        const bool in = r < left;
+                        cp_async16(d + sw128(r, cc & 7), in ? src : first, in);
+                        src += 2 * C::WPP * ps;
                     }
+                    end_tile();
                 }
             }
         } else {
-            // codes D tiles ahead in registers: each pair is asked for again for a later tile as soon
-            // as it has been converted
-            constexpr int D = C::D, kRows = C::PT / 8;
-            uint4 v[D][C::NP][C::VPT];
-            const int cc = pt & 7, r0 = pt >> 3;  // 16-byte chunk of a pair's 128 codes, first row
+            // codes D tiles ahead in registers, asked for again as soon as they have been converted
+            constexpr int D = C::D, kRows = 4 * C::WPP;
+            uint4 v[D][C::VPT];
+            const int cc = lane & 7, r0 = (lane >> 3) + 4 * sub;  // 16-byte chunk of the pair's 128 codes, first row
             const long long rstep = kRows * cv.pos_stride;
-            const uint8_t* src = nullptr;
-            int left = 0;
-            auto at_tile = [&](const Cursor& c) {
+            auto fetch = [&](uint4 (&x)[C::VPT], const Cursor& c) {
                 const Item& it = c.item();
-                left = it.nk - c.j * KT - r0;
-                src = cv.latent + it.row * cv.row_stride + (it.k0 + c.j * KT + r0) * cv.pos_stride + cc * 16;
-            };
-            auto fetch = [&](uint4 (&x)[C::VPT], int i) {
+                const int left = it.nk - c.j * KT - r0;
+                const uint8_t* src = cv.latent + it.row * cv.row_stride + (it.k0 + c.j * KT + r0) * cv.pos_stride + own * 128 + cc * 16;
 #pragma unroll
-                for (int k = 0; k < C::VPT; ++k)
-                    x[k] = kRows * k < left ? __ldg(reinterpret_cast<const uint4*>(src + k * rstep + i * 128)) : make_uint4(0, 0, 0, 0);
+                for (int k = 0; k < C::VPT; ++k) {
+                    x[k] = kRows * k < left ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+                    src += rstep;
+                }
             };
             for (int base = 0; base < mine; base += kTcTable) {
                 const int count = next_table(base);
@@ -515,50 +527,33 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
 #pragma unroll
                 for (int d = 0; d < D; ++d)
                     if (lc.valid()) {
-                        at_tile(lc);
-#pragma unroll
-                        for (int i = 0; i < C::NP; ++i) fetch(v[d][i], i);
+                        fetch(v[d], lc);
                         lc.next();
                     }
                 while (sc.valid()) {
 #pragma unroll
                     for (int d = 0; d < D; ++d) {
                         if (sc.valid()) {
-                            wait(&rope_empty[rr.i], rr.phase ^ 1);
-                            if (sc.j == 0) {
-                                wait(&q_empty[rq.i], rq.phase ^ 1);
-                                load_q(sc.item(), rq.i);
-                                rq.next();
-                            }
-                            load_rope(sc.item(), sc.j, rr.i);
-                            cp_async_arrive(&rope_in[rr.i]);
-                            rr.next();
-                            const bool more = lc.valid();
-                            if (more) at_tile(lc);
+                            begin_tile(sc.item(), sc.j);
+                            uint8_t* dst = sPair + rp.i * C::kPair + (cc >> 2) * C::kBox;
 #pragma unroll
-                            for (int i = 0; i < C::NP; ++i, rp.next()) {
-                                const int slot = rp.i;
-                                wait(&pair_empty[slot], rp.phase ^ 1);
-                                uint8_t* dst = sPair + slot * C::kPair + (cc >> 2) * C::kBox;
+                            for (int k = 0; k < C::VPT; ++k) {
+                                const int r = r0 + kRows * k;
+                                const uint32_t w[4] = {v[d][k].x, v[d][k].y, v[d][k].z, v[d][k].w};
+                                uint32_t o[8];
 #pragma unroll
-                                for (int k = 0; k < C::VPT; ++k) {
-                                    const int r = r0 + kRows * k;
-                                    const uint32_t w[4] = {v[d][i][k].x, v[d][i][k].y, v[d][i][k].z, v[d][i][k].w};
-                                    uint32_t o[8];
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) {
-                                        o[2 * e] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] & 0xffff));
-                                        o[2 * e + 1] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] >> 16));
-                                    }
-                                    *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc) & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
-                                    *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc + 1) & 7)) =
-                                        make_uint4(o[4], o[5], o[6], o[7]);
+                                for (int e = 0; e < 4; ++e) {
+                                    o[2 * e] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] & 0xffff));
+                                    o[2 * e + 1] = lat::e4m3x2_to<T>(static_cast<uint16_t>(w[e] >> 16));
                                 }
-                                __syncwarp();
-                                if (lane == 0) mbar_arrive(&pair_in[slot]);
-                                if (more) fetch(v[d][i], i);
+                                *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc) & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+                                *reinterpret_cast<uint4*>(dst + sw128(r, (2 * cc + 1) & 7)) = make_uint4(o[4], o[5], o[6], o[7]);
                             }
-                            if (more) lc.next();
+                            end_tile();
+                            if (lc.valid()) {
+                                fetch(v[d], lc);
+                                lc.next();
+                            }
                             sc.next();
                         }
                     }
@@ -595,7 +590,6 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
 #pragma unroll
                 for (int k = 0; k < R / 16; ++k) tc_mma_f16(dr, ka + k * 2, qa + k * 2, id_s, k ? 1u : 0u);
             }
-            tc_commit(&rope_empty[sr.i]);
             sr.next();
             const uint64_t qd = umma_desc_sw128(q, 16, 1024);
 #pragma unroll
@@ -644,22 +638,16 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             --ahead;
             c.next();
         };
-        Ring<C::RS> fr;
-        Ring<C::PS> fp;
         Ring<C::TS> ft;
         for (int base = 0; base < mine; base += kTcTable) {
             const int count = next_table(base);
             if (warp == kFenceWarp && lane == 0) {
                 // what has been written in the generic proxy (copies, converted codes) becomes
                 // readable by the products
-                for (Cursor c(table, count); c.valid(); c.next(), fr.next()) {
-                    wait(&rope_in[fr.i], fr.phase);
-                    for (int i = 0; i < C::NP; ++i, fp.next()) {
-                        wait(&pair_in[fp.i], fp.phase);
-                    }
+                for (Cursor c(table, count); c.valid(); c.next(), ft.next()) {
+                    wait(&tile_in[ft.i], ft.phase);
                     fence_proxy_async_smem();
                     mbar_arrive(&tile_full[ft.i]);
-                    ft.next();
                 }
             }
             if (warp == kMmaWarp && elect_one()) {
