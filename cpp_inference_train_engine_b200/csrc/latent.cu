@@ -133,34 +133,53 @@ template <class F> void with_half(int dtype, F&& f) {
     else refuse(MM_INVALID_ARGUMENT, "unsupported element type");
 }
 
-mm::spa::Problem problem(const mm_shared_prefix_desc* d) {
+static_assert(sizeof(mm_latent_cache) == 88 && sizeof(mm_shared_prefix_desc) == 112, "the Python binding packs these field by field");
+
+// Whether the rows of an e4m3 cache can be accessed 16 bytes at a time.
+bool aligned_e4m3(const mm_latent_cache* c) {
+    auto ok = [](const void* p, long long a, long long b, int size) {
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a * size % 16 == 0 && b * size % 16 == 0;
+    };
+    return ok(c->latent, c->row_stride, c->pos_stride, 1) && ok(c->rope, c->rope_row_stride, c->rope_pos_stride, 2);
+}
+
+// The vector forms of cache write and read: the models' widths, 16-byte aligned rows.
+template <class F> bool with_width(const mm_latent_cache* c, bool aligned, F&& f) {
+    if (!aligned || !aligned_e4m3(c)) return false;
+    if (c->kv == 128 && c->rope_dim == 16) f(std::integral_constant<int, 128>{}, std::integral_constant<int, 16>{});
+    else if (c->kv == 512 && c->rope_dim == 32) f(std::integral_constant<int, 512>{}, std::integral_constant<int, 32>{});
+    else return false;
+    return true;
+}
+
+mm::spa::Problem problem(const mm_shared_prefix_desc* d, const mm_latent_cache* prefix, const mm_latent_cache* suffix) {
     require(d != nullptr, "null description");
     require(d->rows >= 0 && d->tokens >= 1 && d->heads >= 1 && d->groups >= 0, "shared-prefix attention: invalid sizes");
     require(d->dtype == MM_F16 || d->dtype == MM_BF16, "shared-prefix attention: q must be fp16 or bf16");
-    require(d->prefix || d->suffix, "shared-prefix attention: a prefix or a suffix cache is needed");
+    require(prefix || suffix, "shared-prefix attention: a prefix or a suffix cache is needed");
     require(static_cast<long long>(d->rows) * d->tokens <= kMaxBlocks / d->heads,
             "shared-prefix attention: too many query rows");
-    for (const mm_latent_cache* c : {d->prefix, d->suffix})
+    for (const mm_latent_cache* c : {prefix, suffix})
         if (c) {
             check_cache(c);
             require(c->kind == d->dtype || (c->kind == MM_E4M3 && c->rope_kind == d->dtype),
                     "shared-prefix attention: the cache's type must be q's (an e4m3 cache's rope type)");
         }
-    if (d->prefix && d->suffix)
-        require(d->prefix->kv == d->suffix->kv && d->prefix->rope_dim == d->suffix->rope_dim,
+    if (prefix && suffix)
+        require(prefix->kv == suffix->kv && prefix->rope_dim == suffix->rope_dim,
                 "shared-prefix attention: prefix and suffix widths differ");
-    require(d->groups == 0 || (d->prefix && d->prefix->rows >= d->groups), "shared-prefix attention: a prefix row per group");
-    require(!d->suffix || d->suffix->rows >= d->rows, "shared-prefix attention: a suffix row per row");
+    require(d->groups == 0 || (prefix && prefix->rows >= d->groups), "shared-prefix attention: a prefix row per group");
+    require(!suffix || suffix->rows >= d->rows, "shared-prefix attention: a suffix row per row");
     require(d->max_group >= 0 && d->max_prefix >= 0 && d->max_suffix >= 0 &&
-                d->max_prefix <= (d->prefix ? d->prefix->positions : 0) &&
-                d->max_suffix <= (d->suffix ? d->suffix->positions : 0),
+                d->max_prefix <= (prefix ? prefix->positions : 0) &&
+                d->max_suffix <= (suffix ? suffix->positions : 0),
             "shared-prefix attention: max_prefix / max_suffix exceed the cache's positions");
     if (d->rows > 0) {
         require(d->q && d->out, "shared-prefix attention: null q or out");
         require(d->groups == 0 || (d->group_start && d->prefix_len), "shared-prefix attention: null group_start or prefix_len");
         require(d->max_suffix == 0 || d->suffix_len, "shared-prefix attention: null suffix_len");
     }
-    const mm_latent_cache* any = d->prefix ? d->prefix : d->suffix;
+    const mm_latent_cache* any = prefix ? prefix : suffix;
     mm::spa::Problem p{};
     p.q = d->q;
     p.q_row = d->q_row_stride;
@@ -169,8 +188,8 @@ mm::spa::Problem problem(const mm_shared_prefix_desc* d) {
     p.B = d->rows;
     p.T = d->tokens;
     p.H = d->heads;
-    p.prefix = view(d->prefix);
-    p.suffix = view(d->suffix);
+    p.prefix = view(prefix);
+    p.suffix = view(suffix);
     p.group_start = d->group_start;
     p.prefix_len = d->prefix_len;
     p.suffix_len = d->suffix_len;
@@ -209,17 +228,13 @@ int sm_count() {
 // The tensor-core form covers the two latent widths of the framework's models when every row
 // can be read in 16-byte pieces.
 bool aligned_cache(const mm_latent_cache* c) {
-    auto ok = [](const void* p, long long a, long long b, int size) {
-        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a * size % 16 == 0 && b * size % 16 == 0;
-    };
-    if (c->kind == MM_E4M3)
-        return ok(c->latent, c->row_stride, c->pos_stride, 1) && ok(c->rope, c->rope_row_stride, c->rope_pos_stride, 2);
-    return ok(c->latent, c->row_stride, c->pos_stride, 2);
+    if (c->kind == MM_E4M3) return aligned_e4m3(c);
+    return reinterpret_cast<uintptr_t>(c->latent) % 16 == 0 && c->row_stride % 8 == 0 && c->pos_stride % 8 == 0;
 }
-bool tensor_core_form(const mm_shared_prefix_desc* d, const mm::spa::Problem& p) {
+bool tensor_core_form(const mm::spa::Problem& p, const mm_latent_cache* prefix, const mm_latent_cache* suffix) {
     if (!((p.kv == 128 && p.rd == 16) || (p.kv == 512 && p.rd == 32))) return false;
     if (reinterpret_cast<uintptr_t>(p.q) % 16 || p.q_row % 8 || p.q_tok % 8 || p.q_head % 8) return false;
-    return (p.G == 0 || aligned_cache(d->prefix)) && (p.max_suffix == 0 || aligned_cache(d->suffix));
+    return (p.G == 0 || aligned_cache(prefix)) && (p.max_suffix == 0 || aligned_cache(suffix));
 }
 
 struct Plan {
@@ -351,6 +366,19 @@ int mm_latent_cache_write(const mm_latent_cache* cache, const void* latent, int6
             with_half(cache->rope_kind, [&](auto half) {
                 using T = typename decltype(in)::type;
                 using T16 = typename decltype(half)::type;
+                const long long e = 16 / sizeof(T);
+                const bool aligned = reinterpret_cast<uintptr_t>(latent) % 16 == 0 && latent_stride % e == 0 &&
+                                     reinterpret_cast<uintptr_t>(rope) % 16 == 0 && rope_stride % e == 0;
+                if (with_width(cache, aligned, [&](auto kv, auto rd) {
+                        // positions per block: 8 warps x U x (32 lanes / (kv / 16))
+                        constexpr int kKv = decltype(kv)::value, kRd = decltype(rd)::value, kU = 1;
+                        launch(s, mm::lat::latent_write_vec_kernel<T, T16, kKv, kRd, kU>,
+                               dim3(blocks(n, 8 * kU * (512 / kKv))), dim3(256), 0, c, static_cast<const T*>(latent),
+                               static_cast<long long>(latent_stride), static_cast<const T*>(rope),
+                               static_cast<long long>(rope_stride), reinterpret_cast<const long long*>(slots),
+                               static_cast<long long>(n));
+                    }))
+                    return;
                 launch(s, mm::lat::latent_write_kernel<T, T16>, dim3(blocks(n, 8)), dim3(256), 0, c,
                        static_cast<const T*>(latent), static_cast<long long>(latent_stride), static_cast<const T*>(rope),
                        static_cast<long long>(rope_stride), reinterpret_cast<const long long*>(slots),
@@ -373,6 +401,15 @@ int mm_latent_cache_read(const mm_latent_cache* cache, const int64_t* slots, int
             with_half(cache->rope_kind, [&](auto half) {
                 using TO = typename decltype(o)::type;
                 using T16 = typename decltype(half)::type;
+                const bool aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_stride * sizeof(TO) % 16 == 0;
+                if (with_width(cache, aligned, [&](auto kv, auto rd) {
+                        constexpr int kKv = decltype(kv)::value, kRd = decltype(rd)::value, kU = 2;
+                        launch(s, mm::lat::latent_read_vec_kernel<T16, TO, kKv, kRd, kU>,
+                               dim3(blocks(n, 8 * kU * (512 / kKv))), dim3(256), 0, view(cache),
+                               reinterpret_cast<const long long*>(slots), static_cast<long long>(n), static_cast<TO*>(out),
+                               static_cast<long long>(out_stride));
+                    }))
+                    return;
                 launch(s, mm::lat::latent_read_kernel<T16, TO>, dim3(blocks(n, 8)), dim3(256), 0, view(cache),
                        reinterpret_cast<const long long*>(slots), static_cast<long long>(n), static_cast<TO*>(out),
                        static_cast<long long>(out_stride), cache->kv, cache->rope_dim);
@@ -381,23 +418,25 @@ int mm_latent_cache_read(const mm_latent_cache* cache, const int64_t* slots, int
     });
 }
 
-int64_t mm_shared_prefix_attention_workspace(const mm_shared_prefix_desc* desc) {
+int64_t mm_shared_prefix_attention_workspace(const mm_shared_prefix_desc* desc, const mm_latent_cache* prefix,
+                                             const mm_latent_cache* suffix) {
     int64_t bytes = 0;
     const int rc = guarded([&] {
-        const mm::spa::Problem p = problem(desc);
-        if (p.B > 0 && tensor_core_form(desc, p)) bytes = plan(p).bytes(p.kv);
+        const mm::spa::Problem p = problem(desc, prefix, suffix);
+        if (p.B > 0 && tensor_core_form(p, prefix, suffix)) bytes = plan(p).bytes(p.kv);
     });
     return rc ? -static_cast<int64_t>(rc) : bytes;
 }
 
-int mm_shared_prefix_attention(const mm_shared_prefix_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
+int mm_shared_prefix_attention(const mm_shared_prefix_desc* desc, const mm_latent_cache* prefix, const mm_latent_cache* suffix,
+                               void* workspace, size_t workspace_bytes, void* stream) {
     return guarded([&] {
-        const mm::spa::Problem p = problem(desc);
+        const mm::spa::Problem p = problem(desc, prefix, suffix);
         if (p.B == 0) return;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        const bool q8p = desc->prefix && desc->prefix->kind == MM_E4M3;
-        const bool q8s = desc->suffix && desc->suffix->kind == MM_E4M3;
-        if (tensor_core_form(desc, p)) {
+        const bool q8p = prefix && prefix->kind == MM_E4M3;
+        const bool q8s = suffix && suffix->kind == MM_E4M3;
+        if (tensor_core_form(p, prefix, suffix)) {
             const Plan r = plan(p);
             const long long need = r.bytes(p.kv);
             require(need == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&

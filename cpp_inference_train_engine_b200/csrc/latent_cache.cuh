@@ -67,8 +67,8 @@ struct CacheOut {
 };
 
 // ------------------------------------------------------------------ write
-// One warp per position: the row maximum in one pass held in registers (up to 1024 latent
-// values, 32 per lane), the scale, then the codes. Any width, stride and alignment.
+// Any width, stride and alignment: one warp per position, the row maximum and then the codes in
+// 32-value steps. The widths of the framework's models run on latent_write_vec_kernel.
 template <typename T, typename T16>
 __global__ void latent_write_kernel(CacheOut c, const T* __restrict__ latent, long long latent_stride,
                                     const T* __restrict__ rope, long long rope_stride, const long long* __restrict__ slots,
@@ -92,7 +92,186 @@ __global__ void latent_write_kernel(CacheOut c, const T* __restrict__ latent, lo
     for (int k = lane; k < rd; k += 32) rdst[k] = from_f32<T16>(to_f32(rope[i * rope_stride + k]));
 }
 
+// 16 consecutive values of a row as fp32.
+template <typename T> __device__ __forceinline__ void load16(const T* __restrict__ p, float (&v)[16]) {
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 16 / kPer; ++i) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) v[i * kPer + e] = to_f32(t[e]);
+    }
+}
+template <typename T> __device__ __forceinline__ void store16(T* __restrict__ p, const float (&v)[16]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            reinterpret_cast<uint4*>(p)[i] =
+                make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
+                           pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
+    }
+}
+// Eight values of one type to eight of a 16-bit one.
+template <typename T, typename T16> __device__ __forceinline__ uint4 rope8(const T* __restrict__ p) {
+    float v[8];
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8 / kPer; ++i) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) v[i * kPer + e] = to_f32(t[e]);
+    }
+    return make_uint4(pack2<T16>(v[0], v[1]), pack2<T16>(v[2], v[3]), pack2<T16>(v[4], v[5]), pack2<T16>(v[6], v[7]));
+}
+
+// The e4m3 codes of v[i] / s (IEEE quotients), 16 of them. The product with the reciprocal is
+// within 2 ulp of the quotient, and rounding is monotonic: where the products with a reciprocal
+// 2^-21 lower and higher round to the same code, so does the quotient. A lane in which they differ
+// anywhere (a quotient that close to the middle of two codes) divides.
+__device__ __forceinline__ uint4 e4m3_quotients(const float (&v)[16], float s) {
+    const float inv = __frcp_rn(s), below = inv * (1.f - 4.76837158e-7f), above = inv * (1.f + 4.76837158e-7f);
+    auto codes4 = [](float a, float b, float c, float d) {
+        return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3)) |
+               (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16);
+    };
+    uint32_t w[4], differ = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        w[e] = codes4(v[4 * e] * below, v[4 * e + 1] * below, v[4 * e + 2] * below, v[4 * e + 3] * below);
+        differ |= w[e] ^ codes4(v[4 * e] * above, v[4 * e + 1] * above, v[4 * e + 2] * above, v[4 * e + 3] * above);
+    }
+    if (differ) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[e] = codes4(__fdiv_rn(v[4 * e], s), __fdiv_rn(v[4 * e + 1], s), __fdiv_rn(v[4 * e + 2], s), __fdiv_rn(v[4 * e + 3], s));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Slot -> (row, position); 32-bit division where the cache has fewer than 2^31 positions.
+__device__ __forceinline__ void split_slot(long long slot, long long total, int positions, long long& row, long long& pos) {
+    if (total <= 0x7fffffffLL) {
+        const uint32_t r = static_cast<uint32_t>(slot) / static_cast<uint32_t>(positions);
+        row = r;
+        pos = static_cast<uint32_t>(slot) - r * static_cast<uint32_t>(positions);
+    } else {
+        row = slot / positions;
+        pos = slot - row * positions;
+    }
+}
+
+// KV = 128 or 512, 16-byte accesses: a lane takes 16 values of a position (KV / 16 lanes each, U
+// positions per lane group, all loads first), the maximum is a shuffle reduction over the lane
+// group. Bound by the bytes in and out: at 196,608 x (512 + 32) fp16 values, 330 MB.
+template <typename T, typename T16, int KV, int R, int U>
+__global__ void __launch_bounds__(256) latent_write_vec_kernel(CacheOut c, const T* __restrict__ latent,
+                                                               long long latent_stride, const T* __restrict__ rope,
+                                                               long long rope_stride, const long long* __restrict__ slots,
+                                                               long long n) {
+    MM_PDL_ENTRY();
+    constexpr int L = KV / 16, P = 32 / L;  // lanes per position, positions side by side in a warp
+    const int lane = threadIdx.x & 31, sub = lane % L;
+    const long long first = ((static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * U) * P + lane / L;
+    const long long total = static_cast<long long>(c.rows) * c.positions;
+    long long slot[U];
+    float v[U][16];
+    uint4 rv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long i = first + u * P;
+        slot[u] = i < n ? slots[i] : -1;
+        if (i < n) {
+            load16(latent + i * latent_stride + sub * 16, v[u]);
+            if (sub < R / 8) rv[u] = rope8<T, T16>(rope + i * rope_stride + sub * 8);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[u][e] = 0.f;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float mx = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, fabsf(v[u][e]));
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float s = fmaxf(__fdiv_rn(mx, kE4m3Max), kScaleFloor);
+        const uint4 codes = e4m3_quotients(v[u], s);
+        if (slot[u] < 0 || slot[u] >= total) continue;
+        long long row, pos;
+        split_slot(slot[u], total, c.positions, row, pos);
+        *reinterpret_cast<uint4*>(c.latent + row * c.row_stride + pos * c.pos_stride + sub * 16) = codes;
+        if (sub < R / 8)
+            *reinterpret_cast<uint4*>(c.rope + 2 * (row * c.rope_row_stride + pos * c.rope_pos_stride) + sub * 16) = rv[u];
+        if (sub == 0) c.scale[row * c.scale_row_stride + pos] = s;
+    }
+}
+
 // ------------------------------------------------------------------ read
+// KV = 128 or 512, 16-byte accesses: 16 codes of a position per lane, U positions per lane
+// group with all loads first. Bound by the bytes in and out.
+template <typename T16, typename TO, int KV, int R, int U>
+__global__ void __launch_bounds__(256) latent_read_vec_kernel(CacheView c, const long long* __restrict__ slots, long long n,
+                                                              TO* __restrict__ out, long long out_stride) {
+    MM_PDL_ENTRY();
+    constexpr int L = KV / 16, P = 32 / L;
+    const int lane = threadIdx.x & 31, sub = lane % L;
+    const long long first = ((static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * U) * P + lane / L;
+    const long long total = static_cast<long long>(c.rows) * c.positions;
+    uint4 code[U], rv[U];
+    float s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long i = first + u * P, slot = i < n ? slots[i] : -1;
+        code[u] = rv[u] = make_uint4(0, 0, 0, 0);
+        s[u] = 0.f;
+        if (slot >= 0 && slot < total) {
+            long long row, pos;
+            split_slot(slot, total, c.positions, row, pos);
+            code[u] = __ldg(reinterpret_cast<const uint4*>(c.latent + row * c.row_stride + pos * c.pos_stride + sub * 16));
+            s[u] = __ldg(c.scale + row * c.scale_row_stride + pos);
+            if (sub < R / 8)
+                rv[u] = __ldg(reinterpret_cast<const uint4*>(c.rope + 2 * (row * c.rope_row_stride + pos * c.rope_pos_stride) + sub * 16));
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long i = first + u * P;
+        if (i >= n) return;
+        TO* o = out + i * out_stride;
+        float v[16];
+        const uint32_t w[4] = {code[u].x, code[u].y, code[u].z, code[u].w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(
+                static_cast<__nv_fp8x2_storage_t>(w[e >> 1] >> (16 * (e & 1))), __NV_E4M3)));
+            v[2 * e] = f.x * s[u];
+            v[2 * e + 1] = f.y * s[u];
+        }
+        store16(o + sub * 16, v);
+        if (sub < R / 8) {
+            const T16* t = reinterpret_cast<const T16*>(&rv[u]);
+            float q[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[e] = to_f32(t[e]);
+            if constexpr (sizeof(TO) == 4) {
+                reinterpret_cast<float4*>(o + KV + sub * 8)[0] = make_float4(q[0], q[1], q[2], q[3]);
+                reinterpret_cast<float4*>(o + KV + sub * 8)[1] = make_float4(q[4], q[5], q[6], q[7]);
+            } else {
+                *reinterpret_cast<uint4*>(o + KV + sub * 8) =
+                    make_uint4(pack2<TO>(q[0], q[1]), pack2<TO>(q[2], q[3]), pack2<TO>(q[4], q[5]), pack2<TO>(q[6], q[7]));
+            }
+        }
+    }
+}
+
+// Any width, stride and alignment: one warp per position.
 template <typename T16, typename TO>
 __global__ void latent_read_kernel(CacheView c, const long long* __restrict__ slots, long long n, TO* __restrict__ out,
                                    long long out_stride, int kv, int rd) {

@@ -88,8 +88,6 @@ typedef struct mm_shared_prefix_desc {
     const void* q;
     int64_t q_row_stride, q_token_stride, q_head_stride;
     int32_t dtype, rows, tokens, heads;
-    const mm_latent_cache* prefix;
-    const mm_latent_cache* suffix;
     const int32_t* group_start;
     const int32_t* prefix_len;
     const int32_t* suffix_len;
@@ -101,8 +99,11 @@ typedef struct mm_shared_prefix_desc {
 } mm_shared_prefix_desc;
 
 /* Bytes of workspace the call needs (0 possible), or -(1 + ErrorCode). */
-int64_t mm_shared_prefix_attention_workspace(const mm_shared_prefix_desc* desc);
-int mm_shared_prefix_attention(const mm_shared_prefix_desc* desc, void* workspace,
+int64_t mm_shared_prefix_attention_workspace(const mm_shared_prefix_desc* desc,
+                                             const mm_latent_cache* prefix,
+                                             const mm_latent_cache* suffix);
+int mm_shared_prefix_attention(const mm_shared_prefix_desc* desc, const mm_latent_cache* prefix,
+                               const mm_latent_cache* suffix, void* workspace,
                                size_t workspace_bytes, void* stream);
 
 /* Verification of drafted tokens (speculative sampling) from given random numbers. For row b,

@@ -17,24 +17,17 @@ def message():
 
 def cache(kind=latent.MM_F16, rows=2, positions=16, kv=128, rope=16, rope_kind=latent.MM_F16):
     p = 1 << 20  # never read: these calls are refused first
-    return latent._Cache(p, p, p, positions * (kv + rope), kv + rope, positions * rope, rope, positions, rows, positions,
-                         kv, rope, kind, rope_kind)
+    return latent._CACHE.pack(p, p, p, positions * (kv + rope), kv + rope, positions * rope, rope, positions, rows,
+                              positions, kv, rope, kind, rope_kind)
 
 
 def desc(**over):
+    d = dict(q=1 << 20, q_row_stride=8 * 144, q_token_stride=8 * 144, q_head_stride=144, dtype=latent.MM_F16, rows=2,
+             tokens=1, heads=8, group_start=1 << 20, prefix_len=1 << 20, suffix_len=1 << 20, groups=1, max_group=2,
+             max_prefix=16, max_suffix=16, scale=0.1, reserved=0, out=1 << 20, lse=0)
     pre, suf = over.pop("prefix", cache(rows=1)), over.pop("suffix", cache())
-    d = latent._Desc()
-    d.q = d.out = d.group_start = d.prefix_len = d.suffix_len = 1 << 20
-    d.q_row_stride = d.q_token_stride = 8 * 144
-    d.q_head_stride, d.dtype, d.rows, d.tokens, d.heads, d.groups = 144, latent.MM_F16, 2, 1, 8, 1
-    d.max_group, d.max_prefix, d.max_suffix, d.scale = 2, 16, 16, 0.1
-    if pre is not None:
-        d.prefix = ctypes.pointer(pre)
-    if suf is not None:
-        d.suffix = ctypes.pointer(suf)
-    for k, v in over.items():
-        setattr(d, k, v)
-    return d
+    d.update({k: v or 0 for k, v in over.items()})
+    return latent._DESC.pack(*d.values()), pre, suf
 
 
 @pytest.mark.parametrize("over, what", [
@@ -49,23 +42,23 @@ def desc(**over):
 ])
 def test_attention_refusals(over, what):
     d = desc(**over)
-    assert latent._lib().mm_shared_prefix_attention_workspace(ctypes.byref(d)) == -1
+    assert latent._lib().mm_shared_prefix_attention_workspace(*d) == -1
     assert what in message()
-    assert latent._lib().mm_shared_prefix_attention(ctypes.byref(d), None, 0, None) == 1
+    assert latent._lib().mm_shared_prefix_attention(*d, None, 0, None) == 1
     assert what in message()
 
 
 def test_null_arguments_are_refused():
     L = latent._lib()
-    assert L.mm_shared_prefix_attention(None, None, 0, None) == 1
+    assert L.mm_shared_prefix_attention(None, None, None, None, 0, None) == 1
     assert L.mm_latent_cache_write(None, None, 0, None, 0, 0, None, 1, None) == 1
     assert L.mm_latent_cache_read(None, None, 1, None, 0, 0, None) == 1
     c = cache(latent.MM_E4M3)
-    assert L.mm_latent_cache_write(ctypes.byref(c), None, 0, None, 0, 0, None, 1, None) == 1 and "null" in message()
-    assert L.mm_latent_cache_write(ctypes.byref(c), None, 0, None, 0, 0, None, -1, None) == 1
-    assert L.mm_latent_cache_write(ctypes.byref(c), None, 0, None, 0, 0, None, 0, None) == 0  # nothing to do
+    assert L.mm_latent_cache_write(c, None, 0, None, 0, 0, None, 1, None) == 1 and "null" in message()
+    assert L.mm_latent_cache_write(c, None, 0, None, 0, 0, None, -1, None) == 1
+    assert L.mm_latent_cache_write(c, None, 0, None, 0, 0, None, 0, None) == 0  # nothing to do
     f16 = cache()
-    assert L.mm_latent_cache_read(ctypes.byref(f16), 1 << 20, 1, 1 << 20, 144, 1, None) == 1 and "e4m3" in message()
+    assert L.mm_latent_cache_read(f16, 1 << 20, 1, 1 << 20, 144, 1, None) == 1 and "e4m3" in message()
     assert L.mm_verify_drafts(None, None, 0, None, None, None, None, 1, 1, 8, None, None, None) == 1
     assert L.mm_verify_drafts(None, None, 0, None, None, None, None, 1, 1, 0, None, None, None) == 1
     assert L.mm_verify_drafts(None, None, 0, None, None, None, None, 1, 1, 2 ** 19, None, None, None) == 3
