@@ -1,6 +1,8 @@
 // C entries of the shared-prompt decode operators (include/mm_latent.h): argument checks,
 // variant selection and launches. Everything is enqueued on the caller's stream; no entry
 // allocates, waits or throws.
+#include <cudaTypedefs.h>
+
 #include <algorithm>
 #include <atomic>
 #include <cstdio>
@@ -289,12 +291,45 @@ Plan plan(const mm::spa::Problem& p) {
     return r;
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> fn{nullptr};
+    PFN_cuTensorMapEncodeTiled_v12000 f = fn.load();
+    if (!f) {
+        cudaDriverEntryPointQueryResult found;
+        void* p = nullptr;
+        check(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found), "cuTensorMapEncodeTiled");
+        if (found != cudaDriverEntryPointSuccess || !p) refuse(MM_GPU_ERROR, "cuTensorMapEncodeTiled unavailable");
+        f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+        fn.store(f);
+    }
+    return f;
+}
+
+// Boxes of `box` columns x `keys` positions of one cache row. False where the encoder does not take
+// the cache's strides; the kernel then copies row by row.
+bool cache_map(CUtensorMap* map, const mm::lat::CacheView& c, int width, int dtype, int box, int keys, CUtensorMapSwizzle swizzle) {
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(c.positions), static_cast<cuuint64_t>(c.rows)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(c.pos_stride) * 2, static_cast<cuuint64_t>(c.row_stride) * 2};
+    const cuuint32_t boxes[3] = {static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(keys), 1}, steps[3] = {1, 1, 1};
+    return tensor_map_encoder()(map, dtype == MM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                                const_cast<uint8_t*>(c.latent), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int KV, int R, int N, typename T, bool Q8>
-void launch_tc(const mm::spa::TcArgs& a, long long items, cudaStream_t s) {
+void launch_tc(mm::spa::TcArgs a, long long items, cudaStream_t s) {
     using C = mm::spa::TcCfg<KV, R, N, Q8>;
+    CUtensorMap pair{}, rope{};
+    if (!Q8 && std::min(a.kps, a.suffix ? a.p.max_suffix : a.p.max_prefix) >= C::KT) {
+        const mm::lat::CacheView& c = a.suffix ? a.p.suffix : a.p.prefix;
+        const int dtype = std::is_same<T, __nv_bfloat16>::value ? MM_BF16 : MM_F16;
+        a.tma = cache_map(&pair, c, KV + R, dtype, 64, C::KT, CU_TENSOR_MAP_SWIZZLE_128B) &&
+                cache_map(&rope, c, KV + R, dtype, R, C::KT, R == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
+    }
     set_dynamic_smem<mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8>>(C::kSmem);
     launch(s, mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8>,
-           dim3(static_cast<unsigned>(std::min<long long>(items, sm_count() * C::kCtas))), dim3(C::kThreads), C::kSmem, a);
+           dim3(static_cast<unsigned>(std::min<long long>(items, sm_count() * C::kCtas))), dim3(C::kThreads), C::kSmem, a,
+           pair, rope);
 }
 template <int KV, int R, typename T>
 void launch_tc_n(const mm::spa::TcArgs& a, int n, bool q8, long long items, cudaStream_t s) {

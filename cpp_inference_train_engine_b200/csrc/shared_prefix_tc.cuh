@@ -21,13 +21,14 @@
 //              vote; otherwise the column maxima are taken and O^T and the sums are rescaled. A key's scale (e4m3) multiplies its latent
 //              scores and, for the second product, its probabilities.
 //   producers  2 to 8: the item's queries, then per tile of KT keys the rope columns and kv / 128 pairs
-//              of 64-column boxes (each pair its own warps) into rings of swizzled boxes. 16-bit caches go by 16-byte
-//              cp.async; e4m3 codes are loaded D tiles ahead into registers and stored as 16-bit
+//              of 64-column boxes (each pair its own warps) into rings of swizzled boxes. Whole tiles of a
+//              16-bit cache come by TMA, a range's last tile by 16-byte cp.async; e4m3 codes are loaded D tiles ahead into registers and stored as 16-bit
 //              values (exact). Rows past the range are zero-filled, so whatever the cache holds
 //              there never reaches a product.
 //   fence      one thread passes each landed tile on to the asynchronous proxy: a proxy fence costs
 //              about 100 ns, and in the loading threads it would wait for every load they have in
 //              flight (measured: 1.7 instead of over 5 TB/s).
+//   results    4 (N = 16): an item's O^T and sums, joined with the prefix's share, to memory.
 //   MMA        one thread issues tcgen05.mma. With KT = 64 the S^T product has M = 64, whose row r
 //              is tensor-memory lane 32 (r / 16) + r % 16.
 // Every mbarrier wait is bounded; after a wait that runs out the CTA goes on without waiting (every
@@ -53,6 +54,7 @@ struct TcArgs {
     const float2* pre_ml;
     int prefix_kps;
     int overlap;       // the launch before this one is the call's own prefix launch: run beside it
+    int tma;           // the tensor maps are valid: whole tiles of a 16-bit cache come by TMA
 };
 
 constexpr int kTcMaxPlan = 512;   // groups or rows whose item prefix sums fit the shared plan
@@ -98,21 +100,24 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     // warps: softmax groups of four, producers, the MMA warp and the fence warp (N = 64: a whole
     // warpgroup for these two, so that registers can move between the roles)
     static constexpr int SG = N == 64 ? 2 : 1, NC = N / SG, SW = 4 * SG;
-    static constexpr int PW = N == 64 ? 4 : KV == 512 ? (Q8 ? 8 : 4) : 2, PT = 32 * PW;
-    static constexpr int kThreads = 32 * (SW + PW + (N == 64 ? 4 : 2));
+    static constexpr int PW = N == 64 || KV == 512 ? 4 : 2, PT = 32 * PW;
+    // N = 16: four warps of their own write the results, while the softmax goes on with the next item
+    // (N = 64: the softmax warps write them, the registers are needed there)
+    static constexpr int EW = N == 16 ? 4 : 0;
+    static constexpr int kThreads = 32 * (SW + PW + (N == 64 ? 4 : 2) + EW);
     // producer warps per pair of a tile
     static constexpr int WPP = PW / NP;
     // e4m3: 16-byte loads per tile and thread, tiles ahead in registers
-    static constexpr int VPT = KT * 8 / (32 * WPP), D = KV == 512 ? (N == 16 ? 2 : 1) : (N == 16 ? 1 : 3);
+    static constexpr int VPT = KT * 8 / (32 * WPP), D = KV == 128 && N == 64 ? 3 : 1;
     static constexpr int oPair = 0;
     static constexpr int oQ = oPair + PS * kPair;
     static constexpr int oRope = oQ + QB * kQA;
     static constexpr int oP = oRope + RS * kRopeA;
     static constexpr int oTab = oP + PB * kP;
-    static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N], up[N]
-    static constexpr int oPlan = oF + 8 * N * 4;
+    static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N], up[N], mail[2][5][N], factor[5][N]
+    static constexpr int oPlan = oF + (8 + (EW ? 15 : 0)) * N * 4;
     static constexpr int oBar = oPlan + (kTcMaxPlan + 1) * 4 + 4;
-    static constexpr int kBars = QB + PS + 2 * TS + 4 + 2 * PB + 2 * OB;
+    static constexpr int kBars = QB + PS + 2 * TS + 4 + 2 * PB + 2 * OB + 4;
     static_assert(RS * NP >= PS && TS * NP >= PS, "the rope ring and the tile barriers outlast the pair ring");
     static constexpr int kSmem = oBar + kBars * 8 + 16 + 1024;  // + alignment of the base
     static_assert(kCtas * (kSmem + 1024) <= 228 * 1024 && kCols * kCtas <= 512, "shared and tensor memory");
@@ -143,6 +148,14 @@ __device__ __forceinline__ bool elect_one() {
         "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(r));
     return r != 0;
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
 }
 
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
@@ -320,7 +333,8 @@ struct Cursor {
 
 template <int KV, int R, int N, typename T, bool Q8>
 __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N, Q8>::kCtas)
-    shared_prefix_tc_kernel(const __grid_constant__ TcArgs a) {
+    shared_prefix_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap map_pair,
+                            const __grid_constant__ CUtensorMap map_rope) {
     using C = TcCfg<KV, R, N, Q8>;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     constexpr int NC = C::NC, KT = C::KT;
@@ -333,6 +347,8 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     float* red_s = corr_s + N;  // [4][N]
     int* lim_s = reinterpret_cast<int*>(red_s + 4 * N);
     float* up_s = red_s + 5 * N;
+    float* mail_s = up_s + N;        // [2][5][N] an item's sums (one row per softmax warp) and maxima
+    float* fac_s = mail_s + 10 * N;  // [5][N]
     int* plan_s = reinterpret_cast<int*>(smem + C::oPlan);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::oBar);
     uint64_t* q_empty = bars;                    // [QB] the item's S products have read Q
@@ -344,22 +360,25 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     uint64_t* p_full = s_free + 2;               // [PB] the softmax warps
     uint64_t* p_free = p_full + C::PB;           // [PB] the tile's O products are complete
     uint64_t* o_full = p_free + C::PB;           // [OB]
-    uint64_t* o_free = o_full + C::OB;           // [OB] the softmax warps
+    uint64_t* o_free = o_full + C::OB;           // [OB] the warps that write the results
+    uint64_t* e_full = o_free + C::OB;           // [2] the softmax warps: an item's sums and maxima
+    uint64_t* e_free = e_full + 2;               // [2] the result warps
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
     int* bad_s = reinterpret_cast<int*>(tmem_slot + 1);
     const Problem& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int th = p.T * p.H;
-    constexpr int kMmaWarp = C::SW + C::PW, kFenceWarp = kMmaWarp + 1;
+    constexpr int kMmaWarp = C::SW + C::PW, kFenceWarp = kMmaWarp + 1, kResultWarp = kMmaWarp + (C::EW ? 2 : 4);
 
     if (warp == kMmaWarp) {
         if (lane == 0) {
             for (int i = 0; i < C::QB; ++i) mbar_init(&q_empty[i], 1);
             for (int i = 0; i < C::PS; ++i) mbar_init(&pair_empty[i], 1);
-            for (int i = 0; i < C::TS; ++i) { mbar_init(&tile_in[i], C::PT + (Q8 ? C::PW : 0)); mbar_init(&tile_full[i], 1); }
+            for (int i = 0; i < C::TS; ++i) { mbar_init(&tile_in[i], C::PT + (Q8 ? C::PW : C::NP)); mbar_init(&tile_full[i], 1); }
             for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_free[i], C::SW); }
             for (int i = 0; i < C::PB; ++i) { mbar_init(&p_full[i], C::SW); mbar_init(&p_free[i], 1); }
-            for (int i = 0; i < C::OB; ++i) { mbar_init(&o_full[i], 1); mbar_init(&o_free[i], C::SW); }
+            for (int i = 0; i < C::OB; ++i) { mbar_init(&o_full[i], 1); mbar_init(&o_free[i], C::EW ? C::EW : C::SW); }
+            for (int i = 0; i < 2; ++i) { mbar_init(&e_full[i], C::SW); mbar_init(&e_free[i], 4); }
             *bad_s = 0;
             fence_mbar_init();
         }
@@ -435,11 +454,18 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         auto load_q = [&](const Item& it, int qb) {
             uint8_t* q = sQ + qb * C::kQA;
             const int c = pt & 7;
+            // query rows one q_head apart (contiguous q, or one token per row with rows in line): no divisions
+            const bool line = p.q_tok == p.H * p.q_head && p.q_row == th * p.q_head;
 #pragma unroll 1
             for (int n = pt >> 3; n < N; n += C::PT / 8) {
                 const bool in = n < it.nq;
-                const int r = it.q0 + (in ? n : 0), b = r / th, u = r - b * th, t = u / p.H, h = u - t * p.H;
-                const T* src = static_cast<const T*>(p.q) + b * p.q_row + t * p.q_tok + h * p.q_head + c * 8;
+                const int r = it.q0 + (in ? n : 0);
+                long long off = r * p.q_head;
+                if (!line) {
+                    const int b = r / th, u = r - b * th, t = u / p.H;
+                    off = b * p.q_row + t * p.q_tok + (u - t * p.H) * p.q_head;
+                }
+                const T* src = static_cast<const T*>(p.q) + off + c * 8;
                 uint8_t* dst = q + sw128(n, c);
 #pragma unroll
                 for (int x = 0; x < 2 * C::NP; ++x) cp_async16(dst + x * C::kQBox, src + x * 64, in);
@@ -472,10 +498,9 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 load_q(it, rq.i);
                 rq.next();
             }
-            load_rope(it, j, rr.i);
-            rr.next();
         };
         auto end_tile = [&] {
+            rr.next();
             cp_async_arrive(&tile_in[rt.i]);
             if (Q8) {  // the warp's converted codes
                 __syncwarp();
@@ -493,6 +518,27 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     const Item& it = c.item();
                     begin_tile(it, c.j);
                     const int left = it.nk - c.j * KT;
+                    // a whole tile: one thread per pair asks for its two boxes (and the first for the rope
+                    // columns); a range's last tile is copied row by row, zeros past the range
+                    const bool tma = a.tma && left >= KT;
+                    if (sub == 0 && lane == 0) {
+                        if (tma) {
+                            uint64_t* bar = &tile_in[rt.i];
+                            mbar_arrive_expect_tx(bar, C::kPair + (own == 0 ? C::kRope : 0));
+                            uint8_t* box = sPair + rp.i * C::kPair;
+                            const int pos = it.k0 + c.j * KT;
+                            tma_load_3d(box, &map_pair, bar, own * 128, pos, it.row);
+                            tma_load_3d(box + C::kBox, &map_pair, bar, own * 128 + 64, pos, it.row);
+                            if (own == 0) tma_load_3d(sRope + rr.i * C::kRopeA, &map_rope, bar, KV, pos, it.row);
+                        } else {
+                            mbar_arrive(&tile_in[rt.i]);
+                        }
+                    }
+                    if (tma) {
+                        end_tile();
+                        continue;
+                    }
+                    load_rope(it, c.j, rr.i);
                     const uint8_t* first = cv.latent + 2 * (it.row * cv.row_stride) + (it.k0 + c.j * KT) * ps + own * 256 + cc * 16;
                     const uint8_t* src = first + r0 * ps;
                     uint8_t* d = sPair + rp.i * C::kPair + (cc >> 3) * C::kBox;
@@ -535,6 +581,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     for (int d = 0; d < D; ++d) {
                         if (sc.valid()) {
                             begin_tile(sc.item(), sc.j);
+                            load_rope(sc.item(), sc.j, rr.i);
                             uint8_t* dst = sPair + rp.i * C::kPair + (cc >> 2) * C::kBox;
 #pragma unroll
                             for (int k = 0; k < C::VPT; ++k) {
@@ -561,7 +608,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             }
         }
         cp_async_wait<0>();
-    } else if (warp >= kMmaWarp) {
+    } else if (warp >= kMmaWarp && warp < kResultWarp) {
         // ------------------------------------------------------------ tensor-core products
         if constexpr (Q8 && N == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         const uint32_t id_s = umma_idesc_f16(kBf16, false, false, KT, N);
@@ -673,8 +720,8 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             }
             __syncwarp();
         }
-    } else {
-        // ------------------------------------------------------------ softmax and results
+    } else if (warp < C::SW) {
+        // ------------------------------------------------------------ softmax (N = 64: and results)
         const int group = warp >> 2, gw = warp & 3, gt = tid & 127;  // gt: tensor-memory lane
         const int c0 = group * NC;                                   // first query column of the group
         // the key this lane's scores belong to (64-key tiles: the lower half of each warp)
@@ -685,34 +732,16 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         const long long rows = static_cast<long long>(p.B) * th;
         const float* m_c = m_s + c0;
         int tile = 0, item = 0;
-        bool waited = !a.overlap;
+        Ring<2> eb;
         for (int base = 0; base < mine; base += kTcTable) {
             const int count = next_table(base);
             for (int e0 = 0; e0 < count; ++e0) {
                 const Item it = table[e0];
-                const bool direct = N == 16 && it.np >= 0;
-                if (it.nt == 0 && !direct) continue;
+                if (it.nt == 0 && (N != 16 || it.np < 0)) continue;
                 const int nq = min(it.nq - c0, NC);  // the group's queries (none: <= 0)
                 float l[NC];
 #pragma unroll
                 for (int n = 0; n < NC; ++n) l[n] = 0.f;
-                const long long at = it.q0 + c0;  // first query row; partials of this launch: + split * rows
-                // The prefix's share of a direct result: unit u = (16-column block, prefix range) of the
-                // partials, 16 queries of this thread's dimension. Unit 0 is asked for before the tiles:
-                // a load issued behind a full ring of cache tiles waits its turn (2 to 4 us).
-                const bool joins = direct && it.np > 0 && nq > 0;
-                const int cb = (nq + 15) / 16;
-                float x0[16];
-                float2 ml0 = make_float2(kNoMax, 0.f);
-                auto ask = [&](int u, float (&x)[16]) {
-                    const int s = u % it.np, k = u / it.np, i = k / cb, c = (k - i * cb) * 16;
-                    const float* src = a.pre_o + (s * rows + at + c) * KV + i * 128 + gt;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = c + e < nq ? __ldcg(src + static_cast<long long>(e) * KV) : 0.f;
-                    if (u == 0 && gt < nq) ml0 = __ldcg(&a.pre_ml[at + gt]);
-                };
-                const bool asked = joins && waited;
-                if (asked) ask(0, x0);
                 // keys of the item each query sees; the tokens of a suffix end one position apart
                 const bool causal = a.suffix && p.T > 1;
                 soft_sync(group);  // the previous item's readers of m_s, lim_s and red_s are done
@@ -855,29 +884,31 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&p_full[pb]);
                 }
-                const int ob = item % C::OB;
-                const uint32_t o = lane_base + C::kColO + ob * C::NP * N + c0;
-                if (joins && !waited) {
-                    pdl_wait();
-                    waited = true;
-                }
-                if (joins && !asked) ask(0, x0);
-                // the sums over the tile's keys
+                // the sums over the item's keys
                 const int own = fold_columns(l, lane, [](float u, float w) { return u + w; });
-                if (NC == 32 || (lane & 1) == 0) red_s[gw * N + c0 + own] = l[0];
-                soft_sync(group);
-                float m_own = kNoMax, l_own = 0.f;  // of query c0 + gt
-                if (gt < NC) {
-                    const int n = c0 + gt;
-                    l_own = (red_s[n] + red_s[N + n]) + (red_s[2 * N + n] + red_s[3 * N + n]);
-                    if (*reinterpret_cast<volatile int*>(bad_s)) l_own = __int_as_float(0x7fc00000);
-                    m_own = l_own == 0.f ? kNoMax : m_s[n];
-                }
-                if (!direct) {
-                    const long long as = it.split * rows + at;
-                    if (gt < nq) a.part_ml[as + gt] = make_float2(m_own, l_own);
+                if constexpr (C::EW > 0) {
+                    float* mail = mail_s + eb.i * 5 * N;
+                    wait(&e_free[eb.i], eb.phase ^ 1);
+                    if ((lane & 1) == 0) mail[gw * N + own] = l[0];
+                    if (gt < N) mail[4 * N + gt] = m_s[gt];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&e_full[eb.i]);
+                    eb.next();
+                    if (it.nt > 0) ++item;
+                } else {
+                    const long long as = it.split * rows + it.q0 + c0;
+                    const int ob = item % C::OB;
+                    red_s[gw * N + c0 + own] = l[0];
+                    soft_sync(group);
+                    if (gt < nq) {
+                        const int n = c0 + gt;
+                        float l_own = (red_s[n] + red_s[N + n]) + (red_s[2 * N + n] + red_s[3 * N + n]);
+                        if (*reinterpret_cast<volatile int*>(bad_s)) l_own = __int_as_float(0x7fc00000);
+                        a.part_ml[as + gt] = make_float2(l_own == 0.f ? kNoMax : m_s[n], l_own);
+                    }
                     wait(&o_full[ob], (item / C::OB) & 1);
                     tc_fence_after();
+                    const uint32_t o = lane_base + C::kColO + ob * C::NP * N + c0;
 #pragma unroll 1
                     for (int i = 0; i < C::NP; ++i)
 #pragma unroll 1
@@ -889,63 +920,6 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                             for (int e = 0; e < 16; ++e)
                                 if (c + e < nq) dst[static_cast<long long>(e) * KV] = v[e];
                         }
-                } else {
-                    // joint maximum and sum with the prefix's ranges (at most kMaxJoin); each part's factor,
-                    // the division by the sum included
-                    if (gt < nq) {
-                        float2 ml[kMaxJoin];
-                        float M = m_own;
-#pragma unroll
-                        for (int s = 0; s < kMaxJoin; ++s) {
-                            ml[s] = s == 0 ? ml0 : s < it.np ? __ldcg(&a.pre_ml[s * rows + at + gt]) : make_float2(kNoMax, 0.f);
-                            M = fmaxf(M, ml[s].x);
-                        }
-                        const float f = fast_exp2(m_own - M);
-                        float L = l_own * f;
-#pragma unroll
-                        for (int s = 0; s < kMaxJoin; ++s) L += ml[s].y * fast_exp2(ml[s].x - M);
-                        const float inv = L == 0.f ? 0.f : 1.f / L;
-                        corr_s[c0 + gt] = f * inv;
-#pragma unroll
-                        for (int s = 0; s < kMaxJoin; ++s) red_s[s * N + c0 + gt] = fast_exp2(ml[s].x - M) * inv;
-                        if (p.lse) p.lse[at + gt] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-                    }
-                    if (it.nt > 0) {
-                        wait(&o_full[ob], (item / C::OB) & 1);
-                        tc_fence_after();
-                    }
-                    soft_sync(group);
-                    int u = 0;
-#pragma unroll 1
-                    for (int i = 0; i < C::NP; ++i)
-#pragma unroll 1
-                        for (int c = 0; c < nq; c += 16) {
-                            float v[16];
-                            if (it.nt > 0) {
-                                tmem_ld16(o + i * N + c, v);
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) v[e] *= corr_s[c0 + c + e];
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) v[e] = 0.f;
-                            }
-#pragma unroll 1
-                            for (int s = 0; s < it.np; ++s, ++u) {
-                                float xn[16];
-                                if (u + 1 < it.np * cb * C::NP) ask(u + 1, xn);
-#pragma unroll
-                                for (int e = 0; e < 16; ++e)
-                                    if (c + e < nq) v[e] = fmaf(x0[e], red_s[s * N + c0 + c + e], v[e]);
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) x0[e] = xn[e];
-                            }
-                            T* dst = static_cast<T*>(p.out) + (at + c) * KV + i * 128 + gt;
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                if (c + e < nq) dst[static_cast<long long>(e) * KV] = lat::from_f32<T>(v[e]);
-                        }
-                }
-                if (it.nt > 0) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&o_free[ob]);
@@ -953,9 +927,119 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 }
             }
         }
+    } else if constexpr (C::EW > 0) {
+        // ------------------------------------------------------------ results (N = 16)
+        // thread = latent dimension (tensor-memory lane) of a 128-column pair, 16 query columns
+        const int quad = warp & 3, dim = quad * 32 + lane;
+        const int n = tid - 32 * kResultWarp;  // < N: the query whose factors this thread works out
+        const long long rows = static_cast<long long>(p.B) * th;
+        Ring<C::OB> ob;
+        Ring<2> eb;
+        bool waited = !a.overlap;
+        for (int base = 0; base < mine; base += kTcTable) {
+            const int count = next_table(base);
+            for (int e0 = 0; e0 < count; ++e0) {
+                const Item it = table[e0];
+                const bool direct = it.np >= 0;
+                if (it.nt == 0 && !direct) continue;
+                const long long at = it.q0;  // first query row; partials of this launch: + split * rows
+                // The prefix's share of a direct result: unit u = (pair, prefix range) of the partials. The
+                // first is asked for before the item's tiles are done: a load issued behind a full ring
+                // of cache tiles waits its turn (2 to 4 us).
+                const bool joins = it.np > 0;
+                float x0[16];
+                float2 ml[kMaxJoin];
+                auto ask = [&](int u, float (&x)[16]) {
+                    const int s = u % it.np, i = u / it.np;
+                    const float* src = a.pre_o + (s * rows + at) * KV + i * 128 + dim;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = e < it.nq ? __ldcg(src + static_cast<long long>(e) * KV) : 0.f;
+                };
+                if (joins) {
+                    if (!waited) {
+                        pdl_wait();
+                        waited = true;
+                    }
+                    ask(0, x0);
+                }
+#pragma unroll
+                for (int s = 0; s < kMaxJoin; ++s)
+                    ml[s] = s < it.np && n < it.nq ? __ldcg(&a.pre_ml[s * rows + at + n]) : make_float2(kNoMax, 0.f);
+                wait(&e_full[eb.i], eb.phase);
+                const float* mail = mail_s + eb.i * 5 * N;
+                if (n < it.nq) {
+                    float l_own = (mail[n] + mail[N + n]) + (mail[2 * N + n] + mail[3 * N + n]);
+                    if (*reinterpret_cast<volatile int*>(bad_s)) l_own = __int_as_float(0x7fc00000);
+                    const float m_own = l_own == 0.f ? kNoMax : mail[4 * N + n];
+                    if (!direct) {
+                        a.part_ml[it.split * rows + at + n] = make_float2(m_own, l_own);
+                    } else {
+                        // joint maximum and sum with the prefix's ranges (at most kMaxJoin); each part's
+                        // factor, the division by the sum included
+                        float M = m_own;
+#pragma unroll
+                        for (int s = 0; s < kMaxJoin; ++s) M = fmaxf(M, ml[s].x);
+                        const float f = fast_exp2(m_own - M);
+                        float L = l_own * f;
+#pragma unroll
+                        for (int s = 0; s < kMaxJoin; ++s) L += ml[s].y * fast_exp2(ml[s].x - M);
+                        const float inv = L == 0.f ? 0.f : 1.f / L;
+                        fac_s[n] = f * inv;
+#pragma unroll
+                        for (int s = 0; s < kMaxJoin; ++s) fac_s[(1 + s) * N + n] = fast_exp2(ml[s].x - M) * inv;
+                        if (p.lse) p.lse[at + n] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+                    }
+                }
+                soft_sync(2);
+                if (lane == 0) mbar_arrive(&e_free[eb.i]);
+                eb.next();
+                if (it.nt > 0) {
+                    wait(&o_full[ob.i], ob.phase);
+                    tc_fence_after();
+                }
+                const uint32_t o = tmem + (static_cast<uint32_t>(quad * 32) << 16) + C::kColO + ob.i * C::NP * N;
+                int u = 0;
+#pragma unroll 1
+                for (int i = 0; i < C::NP; ++i) {
+                    float v[16];
+                    if (it.nt > 0) tmem_ld16(o + i * N, v);
+                    if (!direct) {
+                        float* dst = a.part_o + (it.split * rows + at) * KV + i * 128 + dim;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (e < it.nq) dst[static_cast<long long>(e) * KV] = v[e];
+                        continue;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] = it.nt > 0 ? v[e] * fac_s[e] : 0.f;
+#pragma unroll 1
+                    for (int s = 0; s < it.np; ++s, ++u) {
+                        float xn[16];
+                        if (u + 1 < it.np * C::NP) ask(u + 1, xn);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (e < it.nq) v[e] = fmaf(x0[e], fac_s[(1 + s) * N + e], v[e]);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x0[e] = xn[e];
+                    }
+                    T* dst = static_cast<T*>(p.out) + at * KV + i * 128 + dim;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (e < it.nq) dst[static_cast<long long>(e) * KV] = lat::from_f32<T>(v[e]);
+                }
+                soft_sync(2);  // fac_s may be written again
+                if (it.nt > 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&o_free[ob.i]);
+                    ob.next();
+                }
+            }
+        }
         // this launch must not end before the one it ran beside
         if (!waited) pdl_wait();
     }
+    if (C::EW == 0 && a.overlap) pdl_wait();  // nor with 64-query blocks
     tc_fence_before();
     __syncthreads();
     if (warp == kMmaWarp) {
