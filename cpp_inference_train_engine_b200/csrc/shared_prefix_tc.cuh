@@ -21,11 +21,11 @@
 //              vote; otherwise the column maxima are taken and O^T and the sums are rescaled. A key's scale (e4m3) multiplies its latent
 //              scores and, for the second product, its probabilities.
 //   producers  2 to 8: the item's queries, then per tile of KT keys the rope columns and kv / 128 pairs
-//              of 64-column boxes (each pair its own warps) into rings of swizzled boxes. Whole tiles of a
-//              16-bit cache come by TMA, a range's last tile by 16-byte cp.async; e4m3 codes are loaded D tiles ahead into registers and stored as 16-bit
-//              values (exact). Rows past the range are zero-filled, so whatever the cache holds
-//              there never reaches a product.
-//   fence      one thread passes each landed tile on to the asynchronous proxy: a proxy fence costs
+//              of 64-column boxes (each pair its own warps) into rings of swizzled boxes. 16-bit caches come
+//              by TMA (where the encoder does not take the strides: by 16-byte cp.async); e4m3 codes are loaded D tiles ahead into registers and stored as 16-bit
+//              values (exact). Rows past the range are zeros in shared memory, so whatever the
+//              cache holds there never reaches a product.
+//   fence      one warp passes each landed tile on to the asynchronous proxy: a proxy fence costs
 //              about 100 ns, and in the loading threads it would wait for every load they have in
 //              flight (measured: 1.7 instead of over 5 TB/s).
 //   results    4 (N = 16): an item's O^T and sums, joined with the prefix's share, to memory.
@@ -54,7 +54,7 @@ struct TcArgs {
     const float2* pre_ml;
     int prefix_kps;
     int overlap;       // the launch before this one is the call's own prefix launch: run beside it
-    int tma;           // the tensor maps are valid: whole tiles of a 16-bit cache come by TMA
+    int tma;           // the tensor maps are valid: a 16-bit cache comes by TMA
 };
 
 constexpr int kTcMaxPlan = 512;   // groups or rows whose item prefix sums fit the shared plan
@@ -518,26 +518,26 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     const Item& it = c.item();
                     begin_tile(it, c.j);
                     const int left = it.nk - c.j * KT;
-                    // a whole tile: one thread per pair asks for its two boxes (and the first for the rope
-                    // columns); a range's last tile is copied row by row, zeros past the range
-                    const bool tma = a.tma && left >= KT;
-                    if (sub == 0 && lane == 0) {
-                        if (tma) {
-                            uint64_t* bar = &tile_in[rt.i];
-                            mbar_arrive_expect_tx(bar, C::kPair + (own == 0 ? C::kRope : 0));
-                            uint8_t* box = sPair + rp.i * C::kPair;
-                            const int pos = it.k0 + c.j * KT;
-                            tma_load_3d(box, &map_pair, bar, own * 128, pos, it.row);
-                            tma_load_3d(box + C::kBox, &map_pair, bar, own * 128 + 64, pos, it.row);
-                            if (own == 0) tma_load_3d(sRope + rr.i * C::kRopeA, &map_rope, bar, KV, pos, it.row);
-                        } else {
-                            mbar_arrive(&tile_in[rt.i]);
+                    if (a.tma) {
+                        // blocks of 32 positions that the range reaches: lane 2 b and 2 b + 1 ask for block
+                        // b's two boxes of the warp's pair, lane 8 + b of the first pair for its rope columns
+                        const int nb = min((left + 31) >> 5, KT / 32), pos = it.k0 + c.j * KT;
+                        uint64_t* bar = &tile_in[rt.i];
+                        if (sub == 0) {
+                            if (lane == 0) mbar_arrive_expect_tx(bar, nb * (2 * 4096 + (own == 0 ? 64 * R : 0)));
+                            __syncwarp();
+                            const int blk = lane >> 1, half = lane & 1;
+                            if (lane < 8 && blk < nb)
+                                tma_load_3d(sPair + rp.i * C::kPair + half * C::kBox + blk * 4096, &map_pair, bar,
+                                            own * 128 + half * 64, pos + blk * 32, it.row);
+                            if (own == 0 && lane >= 8 && lane - 8 < nb)
+                                tma_load_3d(sRope + rr.i * C::kRopeA + (lane - 8) * 64 * R, &map_rope, bar, KV,
+                                            pos + (lane - 8) * 32, it.row);
                         }
-                    }
-                    if (tma) {
                         end_tile();
                         continue;
                     }
+                    if (sub == 0 && lane == 0) mbar_arrive(&tile_in[rt.i]);
                     load_rope(it, c.j, rr.i);
                     const uint8_t* first = cv.latent + 2 * (it.row * cv.row_stride) + (it.k0 + c.j * KT) * ps + own * 256 + cc * 16;
                     const uint8_t* src = first + r0 * ps;
@@ -686,15 +686,34 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             c.next();
         };
         Ring<C::TS> ft;
+        Ring<C::PS> fp;
+        Ring<C::RS> fr;
         for (int base = 0; base < mine; base += kTcTable) {
             const int count = next_table(base);
-            if (warp == kFenceWarp && lane == 0) {
-                // what has been written in the generic proxy (copies, converted codes) becomes
-                // readable by the products
+            if (warp == kFenceWarp) {
+                // what has been written in the generic proxy (copies, converted codes) becomes readable by
+                // the products. TMA brings whole blocks of positions, whatever lies past the range: those
+                // rows are cleared first (a probability of zero times a NaN would be one).
                 for (Cursor c(table, count); c.valid(); c.next(), ft.next()) {
                     wait(&tile_in[ft.i], ft.phase);
+                    const int left = c.item().nk - c.j * KT;
+                    if (!Q8 && a.tma && left < KT) {
+                        const uint4 zero = make_uint4(0, 0, 0, 0);
+                        Ring<C::PS> z = fp;
+#pragma unroll 1
+                        for (int i = 0; i < 2 * C::NP; ++i) {
+                            uint8_t* box = smem + C::oPair + z.i * C::kPair + (i & 1) * C::kBox;
+                            for (int e = left * 8 + lane; e < KT * 8; e += 32) reinterpret_cast<uint4*>(box)[e] = zero;
+                            if (i & 1) z.next();
+                        }
+                        uint8_t* box = smem + C::oRope + fr.i * C::kRopeA;
+                        for (int e = left * (R / 8) + lane; e < KT * (R / 8); e += 32) reinterpret_cast<uint4*>(box)[e] = zero;
+                    }
+                    fp.skip(C::NP);
+                    fr.next();
                     fence_proxy_async_smem();
-                    mbar_arrive(&tile_full[ft.i]);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&tile_full[ft.i]);
                 }
             }
             if (warp == kMmaWarp && elect_one()) {
