@@ -319,17 +319,18 @@ bool cache_map(CUtensorMap* map, const mm::lat::CacheView& c, int width, int dty
 template <int KV, int R, int N, typename T, bool Q8>
 void launch_tc(mm::spa::TcArgs a, long long items, cudaStream_t s) {
     using C = mm::spa::TcCfg<KV, R, N, Q8>;
-    CUtensorMap pair{}, rope{};
+    CUtensorMap tile{}, block{}, rope{};
     if (!Q8) {
         const mm::lat::CacheView& c = a.suffix ? a.p.suffix : a.p.prefix;
         const int dtype = std::is_same<T, __nv_bfloat16>::value ? MM_BF16 : MM_F16;
-        a.tma = cache_map(&pair, c, KV + R, dtype, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B) &&
+        a.tma = cache_map(&tile, c, KV + R, dtype, 64, C::KT, CU_TENSOR_MAP_SWIZZLE_128B) &&
+                cache_map(&block, c, KV + R, dtype, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B) &&
                 cache_map(&rope, c, KV + R, dtype, R, 32, R == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
     }
     set_dynamic_smem<mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8>>(C::kSmem);
     launch(s, mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8>,
            dim3(static_cast<unsigned>(std::min<long long>(items, sm_count() * C::kCtas))), dim3(C::kThreads), C::kSmem, a,
-           pair, rope);
+           tile, block, rope);
 }
 template <int KV, int R, typename T>
 void launch_tc_n(const mm::spa::TcArgs& a, int n, bool q8, long long items, cudaStream_t s) {

@@ -23,8 +23,8 @@
 //   producers  2 to 8: the item's queries, then per tile of KT keys the rope columns and kv / 128 pairs
 //              of 64-column boxes (each pair its own warps) into rings of swizzled boxes. 16-bit caches come
 //              by TMA (where the encoder does not take the strides: by 16-byte cp.async); e4m3 codes are loaded D tiles ahead into registers and stored as 16-bit
-//              values (exact). Rows past the range are zeros in shared memory, so whatever the
-//              cache holds there never reaches a product.
+//              values (exact). What the cache holds past the range is masked in
+//              S and never read by an O product.
 //   fence      one warp passes each landed tile on to the asynchronous proxy: a proxy fence costs
 //              about 100 ns, and in the loading threads it would wait for every load they have in
 //              flight (measured: 1.7 instead of over 5 TB/s).
@@ -333,8 +333,8 @@ struct Cursor {
 
 template <int KV, int R, int N, typename T, bool Q8>
 __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N, Q8>::kCtas)
-    shared_prefix_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap map_pair,
-                            const __grid_constant__ CUtensorMap map_rope) {
+    shared_prefix_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap map_tile,
+                            const __grid_constant__ CUtensorMap map_block, const __grid_constant__ CUtensorMap map_rope) {
     using C = TcCfg<KV, R, N, Q8>;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     constexpr int NC = C::NC, KT = C::KT;
@@ -492,12 +492,12 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         Ring<C::PS> rp;
         rp.i = own;
         auto begin_tile = [&](const Item& it, int j) {
-            wait(&pair_empty[rp.i], rp.phase ^ 1);
             if (j == 0) {
                 wait(&q_empty[rq.i], rq.phase ^ 1);
                 load_q(it, rq.i);
                 rq.next();
             }
+            wait(&pair_empty[rp.i], rp.phase ^ 1);
         };
         auto end_tile = [&] {
             rr.next();
@@ -519,21 +519,30 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     begin_tile(it, c.j);
                     const int left = it.nk - c.j * KT;
                     if (a.tma) {
-                        // blocks of 32 positions that the range reaches: lane 2 b and 2 b + 1 ask for block
-                        // b's two boxes of the warp's pair, lane 8 + b of the first pair for its rope columns
-                        const int nb = min((left + 31) >> 5, KT / 32), pos = it.k0 + c.j * KT;
-                        uint64_t* bar = &tile_in[rt.i];
-                        if (sub == 0) {
-                            if (lane == 0) mbar_arrive_expect_tx(bar, nb * (2 * 4096 + (own == 0 ? 64 * R : 0)));
-                            __syncwarp();
-                            const int blk = lane >> 1, half = lane & 1;
-                            if (lane < 8 && blk < nb)
-                                tma_load_3d(sPair + rp.i * C::kPair + half * C::kBox + blk * 4096, &map_pair, bar,
-                                            own * 128 + half * 64, pos + blk * 32, it.row);
-                            if (own == 0 && lane >= 8 && lane - 8 < nb)
-                                tma_load_3d(sRope + rr.i * C::kRopeA + (lane - 8) * 64 * R, &map_rope, bar, KV,
-                                            pos + (lane - 8) * 32, it.row);
+                        // one thread per pair asks for its two boxes, a range's last tile in the blocks of 32
+                        // positions that the range reaches, and the first pair's for the rope columns
+                        if (sub == 0 && elect_one()) {
+                            const int nb = min((left + 31) >> 5, KT / 32), pos = it.k0 + c.j * KT;
+                            uint64_t* bar = &tile_in[rt.i];
+                            mbar_arrive_expect_tx(bar, nb * (2 * 4096 + (own == 0 ? 64 * R : 0)));
+                            uint8_t* box = sPair + rp.i * C::kPair;
+                            if (left >= KT) {
+                                tma_load_3d(box, &map_tile, bar, own * 128, pos, it.row);
+                                tma_load_3d(box + C::kBox, &map_tile, bar, own * 128 + 64, pos, it.row);
+                            } else {
+#pragma unroll 1
+                                for (int k = 0; k < nb; ++k) {
+                                    tma_load_3d(box + k * 4096, &map_block, bar, own * 128, pos + 32 * k, it.row);
+                                    tma_load_3d(box + C::kBox + k * 4096, &map_block, bar, own * 128 + 64, pos + 32 * k, it.row);
+                                }
+                            }
+                            if (own == 0) {
+#pragma unroll 1
+                                for (int k = 0; k < nb; ++k)
+                                    tma_load_3d(sRope + rr.i * C::kRopeA + k * 64 * R, &map_rope, bar, KV, pos + 32 * k, it.row);
+                            }
                         }
+                        __syncwarp();
                         end_tile();
                         continue;
                     }
@@ -665,14 +674,17 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             const uint64_t pa = umma_desc_sw128(aP + pb.i * C::kP, N == 64 ? C::kBox : 16, 1024);
             const uint32_t d = tmem + C::kColO + ob.i * C::NP * N;
             const uint32_t first = c.j ? 1u : 0u;
+            const int left = c.item().nk - c.j * KT;
 #pragma unroll
             for (int i = 0; i < C::NP; ++i) {
                 const uint64_t va = vd + static_cast<uint32_t>(op.i * (C::kPair >> 4));
 #pragma unroll
-                for (int k = 0; k < KT / 16; ++k)
+                for (int k = 0; k < KT / 16; ++k) {
+                    if (16 * k >= left) break;  // keys past the range
                     // V^T MN-major: 16 keys = 2,048 B down a box, the next 64 columns one box on
                     tc_mma_f16(d + i * N, va + k * 128, pa + (N == 64 ? k * 128 : ((k >> 2) * 2048 + (k & 3) * 32) / 16), id_o,
                                k ? 1u : first);
+                }
                 tc_commit(&pair_empty[op.i]);
                 op.next();
             }
@@ -687,30 +699,29 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         };
         Ring<C::TS> ft;
         Ring<C::PS> fp;
-        Ring<C::RS> fr;
         for (int base = 0; base < mine; base += kTcTable) {
             const int count = next_table(base);
             if (warp == kFenceWarp) {
                 // what has been written in the generic proxy (copies, converted codes) becomes readable by
-                // the products. TMA brings whole blocks of positions, whatever lies past the range: those
-                // rows are cleared first (a probability of zero times a NaN would be one).
+                // the products. TMA brings whole blocks of positions, whatever lies past the range: the rows
+                // that the O products still read are cleared first (a probability of zero times a NaN
+                // would be one).
                 for (Cursor c(table, count); c.valid(); c.next(), ft.next()) {
                     wait(&tile_in[ft.i], ft.phase);
                     const int left = c.item().nk - c.j * KT;
-                    if (!Q8 && a.tma && left < KT) {
+                    if (!Q8 && a.tma && left < KT && (left & 15)) {
+                        // the O products read whole steps of 16 keys: rows [left, next multiple of 16)
+                        const int rows = 16 - (left & 15);
                         const uint4 zero = make_uint4(0, 0, 0, 0);
                         Ring<C::PS> z = fp;
 #pragma unroll 1
                         for (int i = 0; i < 2 * C::NP; ++i) {
-                            uint8_t* box = smem + C::oPair + z.i * C::kPair + (i & 1) * C::kBox;
-                            for (int e = left * 8 + lane; e < KT * 8; e += 32) reinterpret_cast<uint4*>(box)[e] = zero;
+                            uint4* box = reinterpret_cast<uint4*>(smem + C::oPair + z.i * C::kPair + (i & 1) * C::kBox) + left * 8;
+                            for (int e = lane; e < rows * 8; e += 32) box[e] = zero;
                             if (i & 1) z.next();
                         }
-                        uint8_t* box = smem + C::oRope + fr.i * C::kRopeA;
-                        for (int e = left * (R / 8) + lane; e < KT * (R / 8); e += 32) reinterpret_cast<uint4*>(box)[e] = zero;
                     }
                     fp.skip(C::NP);
-                    fr.next();
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&tile_full[ft.i]);
