@@ -1,5 +1,6 @@
 """Builds the sm_100a backend in place: cpp_inference_train_engine_b200/libmm_cuda.so, from its
-two translation units (the engine and the latent-cache operators).
+two translation units (the engine and the latent-cache operators), and _latent_torch.so, the
+binding of the latter to torch tensors.
 
     python -m cpp_inference_train_engine_b200.build
 
@@ -16,6 +17,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SRC = [os.path.join(HERE, "csrc", f) for f in ("mm_cuda.cu", "latent.cu")]
 OUT = os.path.join(HERE, "libmm_cuda.so")
+TORCH_SRC = os.path.join(HERE, "csrc", "latent_torch.cpp")
+TORCH_OUT = os.path.join(HERE, "_latent_torch.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -27,10 +30,26 @@ def sources():
 
 
 def up_to_date() -> bool:
-    if not os.path.exists(OUT):
+    if not os.path.exists(OUT) or not os.path.exists(TORCH_OUT):
         return False
-    t = os.path.getmtime(OUT)
+    t = min(os.path.getmtime(OUT), os.path.getmtime(TORCH_OUT))
     return all(os.path.getmtime(s) <= t for s in sources())
+
+
+def torch_command():
+    """g++ on the torch binding, against the installed torch's headers and libraries and the
+    library beside it."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(NVCC), "..", "include")
+    includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                sysconfig.get_paths()["include"], cuda]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            *[f"-isystem{i}" for i in includes], TORCH_SRC, "-o", TORCH_OUT + ".tmp", f"-L{HERE}", "-l:libmm_cuda.so",
+            f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
+            "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = True) -> str:
@@ -39,15 +58,16 @@ def build(force: bool = False, verbose: bool = True) -> str:
     cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr",
            "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", "-Xptxas", "-warn-spills",
            "-t", "2", "-I", os.path.join(ROOT, "include"), *SRC, "-o", OUT + ".tmp", "-ldl", "-lpthread"]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        sys.stderr.write(r.stdout + r.stderr)
-        raise RuntimeError("nvcc failed")
-    if verbose and r.stderr.strip():
-        sys.stderr.write(r.stderr)
-    os.replace(OUT + ".tmp", OUT)
+    for out, c in ((OUT, cmd), (TORCH_OUT, torch_command())):
+        if verbose:
+            print(" ".join(c), flush=True)
+        r = subprocess.run(c, capture_output=True, text=True)
+        if r.returncode != 0:
+            sys.stderr.write(r.stdout + r.stderr)
+            raise RuntimeError(f"{c[0]} failed")
+        if verbose and r.stderr.strip():
+            sys.stderr.write(r.stderr)
+        os.replace(out + ".tmp", out)
     return OUT
 
 
