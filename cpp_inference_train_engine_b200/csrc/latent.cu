@@ -6,7 +6,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdio>
-#include <cstdlib>
 #include <cstring>
 #include <exception>
 #include <string>
@@ -275,14 +274,12 @@ Plan plan(const mm::spa::Problem& p) {
         r.pre_n = p.max_group * th <= 16 ? 16 : 64;
         r.pre_blocks = std::min((r.rows + r.pre_n - 1) / r.pre_n + p.G, p.G * ((p.max_group * th + r.pre_n - 1) / r.pre_n));
         pick_splits(r.pre_blocks, p.max_prefix, 64, r.pre_splits, r.pre_kps);
-        if (const char* e = std::getenv("MM_SPA_PRE")) { r.pre_kps = std::atoi(e); r.pre_splits = (p.max_prefix + r.pre_kps - 1) / r.pre_kps; }
         r.pre_part = r.rows * r.pre_splits;
     }
     if (p.max_suffix > 0) {
         r.suf_n = th <= 16 ? 16 : 64;
         r.suf_blocks = p.B * ((th + r.suf_n - 1) / r.suf_n);
         pick_splits(r.suf_blocks, p.max_suffix, 16, r.suf_splits, r.suf_kps);
-        if (const char* e = std::getenv("MM_SPA_SUF")) { r.suf_kps = std::atoi(e); r.suf_splits = (p.max_suffix + r.suf_kps - 1) / r.suf_kps; }
     }
     r.join = r.suf_n != 16 || r.suf_splits > 1 || r.pre_splits > mm::spa::kMaxJoin;
     if (r.join) r.suf_part = r.rows * r.suf_splits;

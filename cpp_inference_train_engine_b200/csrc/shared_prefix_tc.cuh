@@ -34,6 +34,8 @@
 // Every mbarrier wait is bounded; after a wait that runs out the CTA goes on without waiting (every
 // loop is bounded, every access in bounds) and its results are NaN.
 #pragma once
+#include <type_traits>
+
 #include "shared_prefix.cuh"
 
 namespace mm {
@@ -57,7 +59,7 @@ struct TcArgs {
     int tma;           // the tensor maps are valid: a 16-bit cache comes by TMA
 };
 
-constexpr int kTcMaxPlan = 512;   // groups or rows whose item prefix sums fit the shared plan
+constexpr int kTcMaxPlan = 512;   // entries of the shared plan (the items of runs of groups or rows)
 constexpr int kTcTable = 32;      // items per shared table
 constexpr int kMaxJoin = 4;       // prefix ranges a suffix launch joins itself
 constexpr float kNoMax = -1e37f;  // running maximum before any key (finite: its exp2 is 0, never NaN)
@@ -259,27 +261,37 @@ template <int N> __device__ __forceinline__ Unit get_unit(const TcArgs& a, int u
     return r;
 }
 
-// Item idx of the launch. With a plan (shared: cumulative items of the units) the items are
-// dense, so that they spread evenly over the CTAs whatever the lengths; without one (more units
-// than it holds) every unit has `per` blocks of a.splits ranges, some of them empty.
+template <int N> __device__ __forceinline__ int unit_items(const TcArgs& a, int u) {
+    const Unit r = get_unit<N>(a, u);
+    return r.blocks * r.ranges;
+}
+
+// Item idx of the launch. With a plan (shared: cumulative items of runs of `step` units) the items are
+// dense, so that they spread evenly over the CTAs whatever the lengths; without one (a suffix launch
+// of one range per row, where there is none to skip) every unit has `per` blocks.
 template <int N, int KT>
-__device__ __forceinline__ Item get_item(const TcArgs& a, const int* plan, int units, int per, int idx) {
+__device__ __forceinline__ Item get_item(const TcArgs& a, const int* plan, int units, int step, int per, int idx) {
     int u, local;
     if (plan) {
-        int lo = 0, hi = units;  // the unit with plan[u] <= idx < plan[u + 1]
+        int lo = 0, hi = (units + step - 1) / step;  // the run with plan[lo] <= idx < plan[lo + 1]
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (plan[mid] <= idx) lo = mid;
             else hi = mid;
         }
-        u = lo;
-        local = idx - plan[u];
+        u = lo * step;
+        local = idx - plan[lo];
+        if (step > 1) {
+            const int last = min(units, u + step) - 1;
+#pragma unroll 1
+            for (int n; u < last && local >= (n = unit_items<N>(a, u)); ++u) local -= n;
+        }
     } else {
-        u = idx / (per * a.splits);
-        local = idx - u * per * a.splits;
+        u = idx / per;
+        local = idx - u * per;
     }
     const Unit r = get_unit<N>(a, u);
-    const int ranges = plan ? r.ranges : a.splits;
+    const int ranges = plan ? r.ranges : 1;
     const int block = local / ranges;
     Item it;
     it.split = local - block * ranges;
@@ -394,31 +406,34 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     const int units = a.suffix ? p.B : p.G;
     const int per = ((a.suffix ? th : p.max_group * th) + N - 1) / N;
     const int* plan = nullptr;
-    int items = units * per * a.splits;
-    if (units <= kTcMaxPlan && (a.splits > 1 || !a.suffix)) {
-        // cumulative items of the units (a suffix launch with one range per row has none to skip)
+    int items = units * per;
+    const int step = (units + kTcMaxPlan - 1) / kTcMaxPlan;
+    if (a.splits > 1 || !a.suffix) {
         plan = plan_s;
-        for (int u = tid; u < units; u += C::kThreads) {
-            const Unit r = get_unit<N>(a, u);
-            plan_s[u + 1] = r.blocks * r.ranges;
+        const int runs = (units + step - 1) / step;
+        for (int i = tid; i < runs; i += C::kThreads) {
+            int n = unit_items<N>(a, i * step);
+#pragma unroll 1
+            for (int u = i * step + 1; u < min(units, (i + 1) * step); ++u) n += unit_items<N>(a, u);
+            plan_s[i + 1] = n;
         }
         __syncthreads();
         if (warp == 0) {
             int base = 0;
-            for (int u0 = 0; u0 < units; u0 += 32) {
-                int v = u0 + lane < units ? plan_s[u0 + lane + 1] : 0;
+            for (int u0 = 0; u0 < runs; u0 += 32) {
+                int v = u0 + lane < runs ? plan_s[u0 + lane + 1] : 0;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const int w = __shfl_up_sync(0xffffffffu, v, o);
                     if (lane >= o) v += w;
                 }
-                if (u0 + lane < units) plan_s[u0 + lane + 1] = base + v;
+                if (u0 + lane < runs) plan_s[u0 + lane + 1] = base + v;
                 base += __shfl_sync(0xffffffffu, v, 31);
             }
             if (lane == 0) plan_s[0] = 0;
         }
         __syncthreads();
-        items = plan_s[units];
+        items = plan_s[runs];
     }
     tc_fence_before();
     __syncthreads();
@@ -434,11 +449,14 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             *reinterpret_cast<volatile int*>(bad_s) = 1;
         }
     };
-    // The next table of this CTA's items; every thread of the CTA comes here for each table.
-    auto next_table = [&](int base) {
+    // The next table of this CTA's items; every thread of the CTA comes here for each table. The first
+    // softmax warp builds it (only its branch holds the code and the registers for it).
+    auto next_table = [&](int base, auto builds) {
         if (base > 0) __syncthreads();
-        if (tid < kTcTable && base + tid < mine)
-            table[tid] = get_item<N, KT>(a, plan, units, per, blockIdx.x + (base + tid) * gridDim.x);
+        if constexpr (decltype(builds)::value) {
+            if (tid < kTcTable && base + tid < mine)
+                table[tid] = get_item<N, KT>(a, plan, units, step, per, blockIdx.x + (base + tid) * gridDim.x);
+        }
         __syncthreads();
         return min(kTcTable, mine - base);
     };
@@ -513,7 +531,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             const int cc = lane & 15, r0 = (lane >> 4) + 2 * sub;  // 16-byte chunk of the pair's row, first row
             const long long ps = 2 * cv.pos_stride;
             for (int base = 0; base < mine; base += kTcTable) {
-                const int count = next_table(base);
+                const int count = next_table(base, std::false_type());
                 for (Cursor c(table, count); c.valid(); c.next()) {
                     const Item& it = c.item();
                     begin_tile(it, c.j);
@@ -577,7 +595,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 }
             };
             for (int base = 0; base < mine; base += kTcTable) {
-                const int count = next_table(base);
+                const int count = next_table(base, std::false_type());
                 Cursor lc(table, count), sc(table, count);
 #pragma unroll
                 for (int d = 0; d < D; ++d)
@@ -700,7 +718,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         Ring<C::TS> ft;
         Ring<C::PS> fp;
         for (int base = 0; base < mine; base += kTcTable) {
-            const int count = next_table(base);
+            const int count = next_table(base, std::false_type());
             if (warp == kFenceWarp) {
                 // what has been written in the generic proxy (copies, converted codes) becomes readable by
                 // the products. TMA brings whole blocks of positions, whatever lies past the range: the rows
@@ -764,7 +782,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         int tile = 0, item = 0;
         Ring<2> eb;
         for (int base = 0; base < mine; base += kTcTable) {
-            const int count = next_table(base);
+            const int count = next_table(base, std::true_type());
             for (int e0 = 0; e0 < count; ++e0) {
                 const Item it = table[e0];
                 if (it.nt == 0 && (N != 16 || it.np < 0)) continue;
@@ -967,7 +985,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         Ring<2> eb;
         bool waited = !a.overlap;
         for (int base = 0; base < mine; base += kTcTable) {
-            const int count = next_table(base);
+            const int count = next_table(base, std::false_type());
             for (int e0 = 0; e0 < count; ++e0) {
                 const Item it = table[e0];
                 const bool direct = it.np >= 0;

@@ -564,3 +564,49 @@ def test_refusals():
     bad("u_accept", latent.verify_drafts, p, xt, sl, ua[:1], us)
     bad("262,144", latent.verify_drafts, torch.zeros(1, 1, 262145, device="cuda"), xt[:1, :0].contiguous(), sl[:1],
         ua[:1, :0].contiguous(), us[:1])
+
+
+@pytest.mark.parametrize("width", WIDTHS[:2], ids=str)
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_attention_reads_every_code(width, dtype):
+    """All 254 finite e4m3 codes as latent values, and a NaN that stays with the queries that see it."""
+    torch, latent = mods()
+    kv, rope, H = width
+    dtype = getattr(torch, dtype)
+    codes = [c for c in range(256) if c & 0x7F != 0x7F]
+    raw = torch.tensor([codes[i % 254] for i in range(2 * kv)], dtype=torch.uint8, device="cuda").view(2, 1, kv)
+    lat = raw.view(torch.float8_e4m3fn)
+    rk = torch.zeros(2, 1, rope, dtype=dtype, device="cuda")
+    for scale in (1.0, 2.0 ** -7):
+        cache = (lat, rk, torch.full((2, 1), scale, device="cuda"))
+        q = torch.zeros(2, 1, H, kv + rope, dtype=dtype, device="cuda")
+        one = torch.ones(2, dtype=torch.int32, device="cuda")
+        out = latent.shared_prefix_attention(q, None, cache, None, None, one, 1.0, kv_rank=kv)
+        # one key: its probability is 1, so the output is the value itself, exactly
+        assert torch.equal(out.float(), (lat.float() * scale).view(2, 1, 1, kv).expand(2, 1, H, kv).to(dtype).float())
+    bad = raw.clone()
+    bad[1, 0, 5] = 0x7F
+    out = latent.shared_prefix_attention(q, None, (bad.view(torch.float8_e4m3fn), rk, cache[2]), None, None, one, 1.0,
+                                         kv_rank=kv)
+    assert torch.isfinite(out[0]).all() and torch.isnan(out[1, 0, :, 5]).all()
+
+
+@pytest.mark.parametrize("width", WIDTHS[:2], ids=str)
+@pytest.mark.parametrize("prefix", [40, 1100])
+def test_attention_thousands_of_groups(width, prefix):
+    """More groups than the work list has entries, most of them of one row or none, with no bound on
+    their sizes given; short prefixes (one range each) and long ones (several)."""
+    torch, latent = mods()
+    kv, rope, H = width
+    g = torch.Generator(device="cuda").manual_seed(16)
+    groups = [(i * 7919) % 5 % 3 for i in range(1300)]
+    groups[700] = 41
+    starts = [sum(groups[:i]) for i in range(len(groups) + 1)]
+    plen = [0 if i % 3 == 0 else 1 + i % 33 for i in range(len(groups))]
+    for i in (0, 511, 512, 513, 700, 1299):
+        plen[i] = prefix
+    slen = [i % 4 for i in range(starts[-1])]
+    pre = make_cache(torch, g, plen, prefix, kv, rope, torch.float16, False)
+    suf = make_cache(torch, g, slen, 4, kv, rope, torch.float16, False)
+    q = torch.randn(starts[-1], 1, H, kv + rope, generator=g, device="cuda").half()
+    check_attention(torch, latent, q, pre, suf, starts, plen, slen, kv, 0.1)
