@@ -90,3 +90,19 @@ def test_cpu_tensors_are_refused():
     q = torch.zeros(1, 1, 8, 144, dtype=torch.float16)
     with pytest.raises(E.EngineError, match="CUDA tensor"):
         latent.shared_prefix_attention(q, None, None, None, None, None, 0.1, kv_rank=128)
+
+
+@pytest.mark.parametrize("kwargs,message", [
+    (dict(cache_bits=4), "cache_bits"), (dict(drafts=-1), "drafts"), (dict(new_tokens=0), "new_tokens"),
+    (dict(new_tokens=64), "context"), (dict(prompts=[]), "prompts"), (dict(prompts=[[1], []]), "prompts"),
+    (dict(rows=[1, 2]), "rows"), (dict(rows=0), "rows"),
+])
+def test_group_decoder_refuses_bad_arguments(kwargs, message):
+    import numpy as np
+
+    from cpp_inference_train_engine_b200 import TINY, EngineError
+    from cpp_inference_train_engine_b200.group_decode import GroupDecoder
+    args = dict(prompts=[[1, 2]], rows=1, new_tokens=4, drafts=0)
+    args.update(kwargs)
+    with pytest.raises(EngineError, match=message):
+        GroupDecoder(TINY, np.zeros(1, np.float32), **args)
