@@ -403,11 +403,12 @@ int mm_latent_cache_write(const mm_latent_cache* cache, const void* latent, int6
                 const bool aligned = reinterpret_cast<uintptr_t>(latent) % 16 == 0 && latent_stride % e == 0 &&
                                      reinterpret_cast<uintptr_t>(rope) % 16 == 0 && rope_stride % e == 0;
                 if (with_width(cache, aligned, [&](auto kv, auto rd) {
-                        // positions per block: 8 warps x U x (32 lanes / (kv / 16))
-                        constexpr int kKv = decltype(kv)::value, kRd = decltype(rd)::value, kU = 1;
-                        launch(s, mm::lat::latent_write_vec_kernel<T, T16, kKv, kRd, kU>,
-                               dim3(blocks(n, 8 * kU * (512 / kKv))), dim3(256), 0, c, static_cast<const T*>(latent),
-                               static_cast<long long>(latent_stride), static_cast<const T*>(rope),
+                        // 8 warps of 512 / kv positions each; at most the CTAs that are resident together
+                        constexpr int kKv = decltype(kv)::value, kRd = decltype(rd)::value;
+                        const unsigned ctas = std::min(blocks(n, 8 * (512 / kKv)),
+                                                       static_cast<unsigned>(sm_count() * mm::lat::kWriteCtas<T>));
+                        launch(s, mm::lat::latent_write_vec_kernel<T, T16, kKv, kRd>, dim3(ctas), dim3(256), 0, c,
+                               static_cast<const T*>(latent), static_cast<long long>(latent_stride), static_cast<const T*>(rope),
                                static_cast<long long>(rope_stride), reinterpret_cast<const long long*>(slots),
                                static_cast<long long>(n));
                     }))

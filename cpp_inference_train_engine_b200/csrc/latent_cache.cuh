@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace mm {
@@ -92,17 +94,6 @@ __global__ void latent_write_kernel(CacheOut c, const T* __restrict__ latent, lo
     for (int k = lane; k < rd; k += 32) rdst[k] = from_f32<T16>(to_f32(rope[i * rope_stride + k]));
 }
 
-// 16 consecutive values of a row as fp32.
-template <typename T> __device__ __forceinline__ void load16(const T* __restrict__ p, float (&v)[16]) {
-    constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 16 / kPer; ++i) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        const T* t = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) v[i * kPer + e] = to_f32(t[e]);
-    }
-}
 template <typename T> __device__ __forceinline__ void store16(T* __restrict__ p, const float (&v)[16]) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -117,24 +108,24 @@ template <typename T> __device__ __forceinline__ void store16(T* __restrict__ p,
     }
 }
 // Eight values of one type to eight of a 16-bit one.
-template <typename T, typename T16> __device__ __forceinline__ uint4 rope8(const T* __restrict__ p) {
-    float v[8];
-    constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 8 / kPer; ++i) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        const T* t = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) v[i * kPer + e] = to_f32(t[e]);
+template <typename T, typename T16> __device__ __forceinline__ uint4 rope8(const uint4 (&r)[sizeof(T) / 2]) {
+    if constexpr (std::is_same<T, T16>::value) {
+        return r[0];
+    } else {
+        const T* t = reinterpret_cast<const T*>(r);
+        return make_uint4(pack2<T16>(to_f32(t[0]), to_f32(t[1])), pack2<T16>(to_f32(t[2]), to_f32(t[3])),
+                          pack2<T16>(to_f32(t[4]), to_f32(t[5])), pack2<T16>(to_f32(t[6]), to_f32(t[7])));
     }
-    return make_uint4(pack2<T16>(v[0], v[1]), pack2<T16>(v[2], v[3]), pack2<T16>(v[4], v[5]), pack2<T16>(v[6], v[7]));
 }
 
 // The e4m3 codes of v[i] / s (IEEE quotients), 16 of them. The product with the reciprocal is
 // within 2 ulp of the quotient, and rounding is monotonic: where the products with a reciprocal
 // 2^-21 lower and higher round to the same code, so does the quotient. A lane in which they differ
 // anywhere (a quotient that close to the middle of two codes) divides.
-__device__ __forceinline__ uint4 e4m3_quotients(const float (&v)[16], float s) {
+template <typename T> __device__ __forceinline__ uint4 e4m3_quotients(const uint4 (&x)[sizeof(T)], float s) {
+    float v[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = to_f32(reinterpret_cast<const T*>(x)[e]);
     const float inv = __frcp_rn(s), below = inv * (1.f - 4.76837158e-7f), above = inv * (1.f + 4.76837158e-7f);
     auto codes4 = [](float a, float b, float c, float d) {
         return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3)) |
@@ -166,49 +157,86 @@ __device__ __forceinline__ void split_slot(long long slot, long long total, int 
     }
 }
 
-// KV = 128 or 512, 16-byte accesses: a lane takes 16 values of a position (KV / 16 lanes each, U
-// positions per lane group, all loads first), the maximum is a shuffle reduction over the lane
-// group. Bound by the bytes in and out: at 196,608 x (512 + 32) fp16 values, 330 MB.
-template <typename T, typename T16, int KV, int R, int U>
-__global__ void __launch_bounds__(256) latent_write_vec_kernel(CacheOut c, const T* __restrict__ latent,
-                                                               long long latent_stride, const T* __restrict__ rope,
-                                                               long long rope_stride, const long long* __restrict__ slots,
-                                                               long long n) {
+// The largest magnitude of 16 values held as uint4s of T (NaN is passed over).
+template <typename T> __device__ __forceinline__ float amax16(const uint4 (&x)[sizeof(T)]) {
+    float mx = 0.f;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 f = *reinterpret_cast<const float4*>(&x[i]);
+            mx = fmaxf(fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
+        }
+    } else {
+        using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+        const T2* t = reinterpret_cast<const T2*>(x);
+        T2 m = __habs2(t[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = __hmax2(m, __habs2(t[i]));
+        const T* e = reinterpret_cast<const T*>(&m);
+        mx = fmaxf(fmaxf(mx, to_f32(e[0])), to_f32(e[1]));
+    }
+    return mx;
+}
+
+// A lane's share of a position to write, as it was loaded.
+template <typename T> struct WriteRow {
+    uint4 x[sizeof(T)], r[sizeof(T) / 2];
+    long long slot;
+};
+
+// KV = 128 or 512, 16-byte accesses: a lane takes 16 values of a position (KV / 16 lanes each), the
+// maximum is a shuffle reduction over the lane group. The CTAs that fit walk the positions with the
+// next ones already loaded, as they are (14 registers for 16-bit rows). Bound by the bytes in and out,
+// with the scattered rows of the cache short of the copy rate: 196,608 x (512 + 32) fp16 values to
+// random slots, 330 MB in 67.7 us (4.9 TB/s; a CTA per eight positions 79.9; two positions ahead, or five
+// and six CTAs an SM, 77 to 97: spills or fewer CTAs); 50,001 fp32 rows 24.9 us (5.5 TB/s).
+template <typename T> constexpr int kWriteCtas = sizeof(T) == 4 ? 3 : 4;  // CTAs per SM
+template <typename T, typename T16, int KV, int R>
+__global__ void __launch_bounds__(256, kWriteCtas<T>) latent_write_vec_kernel(
+    CacheOut c, const T* __restrict__ latent, long long latent_stride, const T* __restrict__ rope, long long rope_stride,
+    const long long* __restrict__ slots, long long n) {
     MM_PDL_ENTRY();
     constexpr int L = KV / 16, P = 32 / L;  // lanes per position, positions side by side in a warp
     const int lane = threadIdx.x & 31, sub = lane % L;
-    const long long first = ((static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * U) * P + lane / L;
-    const long long total = static_cast<long long>(c.rows) * c.positions;
-    long long slot[U];
-    float v[U][16];
-    uint4 rv[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const long long i = first + u * P;
-        slot[u] = i < n ? slots[i] : -1;
+    const long long step = static_cast<long long>(gridDim.x) * 8 * P, total = static_cast<long long>(c.rows) * c.positions;
+    auto fetch = [&](long long i) {
+        WriteRow<T> w;
+        w.slot = -1;
         if (i < n) {
-            load16(latent + i * latent_stride + sub * 16, v[u]);
-            if (sub < R / 8) rv[u] = rope8<T, T16>(rope + i * rope_stride + sub * 8);
+            w.slot = slots[i];
+            const uint4* x = reinterpret_cast<const uint4*>(latent + i * latent_stride + sub * 16);
+#pragma unroll
+            for (int e = 0; e < static_cast<int>(sizeof(T)); ++e) w.x[e] = __ldcs(x + e);
+            if (sub < R / 8) {
+                const uint4* r = reinterpret_cast<const uint4*>(rope + i * rope_stride + sub * 8);
+#pragma unroll
+                for (int e = 0; e < static_cast<int>(sizeof(T)) / 2; ++e) w.r[e] = __ldcs(r + e);
+            }
         } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[u][e] = 0.f;
+            for (int e = 0; e < static_cast<int>(sizeof(T)); ++e) w.x[e] = make_uint4(0, 0, 0, 0);
         }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        float mx = 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, fabsf(v[u][e]));
+        return w;
+    };
+    // whole warps walk together (the reduction's shuffles); lane groups past n hold nothing
+    long long i0 = (static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * P;
+    const int mine = lane / L;
+    WriteRow<T> next = fetch(i0 + mine);
+    for (; i0 < n; i0 += step) {
+        const WriteRow<T> w = next;
+        next = fetch(i0 + mine + step);
+        float mx = amax16<T>(w.x);
 #pragma unroll
         for (int o = L / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         const float s = fmaxf(__fdiv_rn(mx, kE4m3Max), kScaleFloor);
-        const uint4 codes = e4m3_quotients(v[u], s);
-        if (slot[u] < 0 || slot[u] >= total) continue;
+        const uint4 codes = e4m3_quotients<T>(w.x, s);
+        if (w.slot < 0 || w.slot >= total) continue;
         long long row, pos;
-        split_slot(slot[u], total, c.positions, row, pos);
+        split_slot(w.slot, total, c.positions, row, pos);
         *reinterpret_cast<uint4*>(c.latent + row * c.row_stride + pos * c.pos_stride + sub * 16) = codes;
         if (sub < R / 8)
-            *reinterpret_cast<uint4*>(c.rope + 2 * (row * c.rope_row_stride + pos * c.rope_pos_stride) + sub * 16) = rv[u];
+            *reinterpret_cast<uint4*>(c.rope + 2 * (row * c.rope_row_stride + pos * c.rope_pos_stride) + sub * 16) =
+                rope8<T, T16>(w.r);
         if (sub == 0) c.scale[row * c.scale_row_stride + pos] = s;
     }
 }
