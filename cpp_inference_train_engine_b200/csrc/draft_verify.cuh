@@ -6,8 +6,6 @@
 namespace mm {
 namespace ver {
 
-constexpr int kThreads = 1024;
-constexpr int kWarps = kThreads / 32;
 constexpr int kChunk = 512;                       // vocabulary entries one warp sums at a time
 constexpr int kMaxVocab = 262144;
 constexpr int kMaxChunks = kMaxVocab / kChunk;
@@ -17,6 +15,17 @@ using i64 = long long;
 // floor(2^38 clamp(r, 0, 1)); NaN gives 0. Scaling by a power of two is exact.
 __device__ __forceinline__ i64 weight(float r) {
     return __float2ll_rz(fminf(fmaxf(r, 0.f), 1.f) * 274877906944.f);
+}
+
+// Adds floor(2^38 clamp(r, 0, 1)) = 2^16 hi + lo to two 32-bit sums: hi = floor(x), x = 2^22 r, and lo the
+// next 16 bits. Adding 2^23 towards zero leaves the floor in the low mantissa bits (x < 2^23), the
+// difference of x and its floor is exact, and the sums count kWeightBias too much per value.
+constexpr uint32_t kWeightBias = 0x4B000000u;  // the bits of 2^23
+__device__ __forceinline__ void add_weight(float r, uint32_t& hi, uint32_t& lo) {
+    const float x = __saturatef(r) * 4194304.f;  // NaN: 0
+    const float h = __fadd_rz(x, 8388608.f);
+    hi += __float_as_uint(h);
+    lo += __float_as_uint(__fmaf_rz(x - (h - 8388608.f), 65536.f, 8388608.f));
 }
 
 __device__ __forceinline__ i64 warp_sum_i64(i64 v) {
@@ -50,12 +59,40 @@ __device__ __forceinline__ void load4(const T* __restrict__ row, int x, int voca
     }
 }
 
+// A lane's 8 entries of the 256 from entry x0 on: entry i, and all of them (zeros past the
+// vocabulary). ALIGNED: two vector loads; else the warp's lanes load neighbours.
+template <bool ALIGNED> __device__ __forceinline__ int entry_of(int x0, int lane, int i) {
+    return ALIGNED ? x0 + (i >> 2) * 128 + lane * 4 + (i & 3) : x0 + i * 32 + lane;
+}
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void load_entries(const T* __restrict__ row, int x0, int lane, int vocab, float (&v)[8]) {
+    if constexpr (ALIGNED) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float f[4];
+            load4<T, true>(row, x0 + k * 128 + lane * 4, vocab, f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * k + i] = f[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int at = x0 + i * 32 + lane;
+            v[i] = at < vocab ? lat::to_f32(row[at]) : 0.f;
+        }
+    }
+}
+
 // One block per row. Acceptance is one gather per draft; then one pass over one row of p (and
 // q) sums the weights of 512-entry chunks, warp 0 finds the chunk that holds the draw from the
 // chunk sums, and the chunk alone is read again to find the entry. Bound by the p (and q)
-// row's bytes at large batches and by that chain's latency at small ones.
-template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) verify_drafts_kernel(
+// row's bytes at large batches and by that chain's latency at small ones. 32 registers keep every
+// warp slot taken. THREADS: 1024 spreads a row over more warps, 512 runs four rows beside each other on
+// an SM, whose chains overlap (fp32 probabilities of 32,768 tokens; 64 rows: 8.3 us with 1024, 10.1 with
+// 512; 1,024 rows: 48.2 and 44.1, 5.5 TB/s; 600 bf16 rows: 28.2 and 29.2): 512 from five rows per
+// SM on (at four and a few more its second wave is nearly empty).
+template <typename T, bool ALIGNED, int THREADS>
+__global__ void __launch_bounds__(THREADS, 2048 / THREADS) verify_drafts_kernel(
     const T* __restrict__ target, const T* __restrict__ draft, const int* __restrict__ tokens,
     const int* __restrict__ lens, const float* __restrict__ u_accept, const float* __restrict__ u_sample, int K, int V,
     int* __restrict__ out_tokens, int* __restrict__ accepted) {
@@ -118,15 +155,30 @@ __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(
     };
 
     for (int pass = 0; pass < 2; ++pass) {
-        for (int c = warp; c < chunks; c += kWarps) {
-            i64 s = 0;
+        for (int c = warp; c < chunks; c += THREADS / 32) {
+            // 8 entries a lane at a time, all loads first; any order: the sums are exact
+            uint32_t hi = 0, lo = 0;
+#pragma unroll 1
+            for (int x0 = c * kChunk; x0 < (c + 1) * kChunk; x0 += 256) {
+                float pv[8];
+                load_entries<T, ALIGNED>(p, x0, lane, V, pv);
+                if (residual && q) {
+                    float qv[8];
+                    load_entries<T, ALIGNED>(q, x0, lane, V, qv);
 #pragma unroll
-            for (int k = 0; k < kChunk / 128; ++k) {
-                i64 w[4];
-                weights4(c * kChunk + k * 128 + lane * 4, w);
-                s += (w[0] + w[1]) + (w[2] + w[3]);
+                    for (int i = 0; i < 8; ++i) pv[i] -= qv[i];
+                } else if (residual && hole >= x0 && hole < x0 + 256) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (entry_of<ALIGNED>(x0, lane, i) == hole) pv[i] -= 1.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) add_weight(pv[i], hi, lo);
             }
-            s = warp_sum_i64(s);
+            // at most 2^31 and 2^25 in a chunk
+            hi = __reduce_add_sync(0xffffffffu, hi - kChunk / 32 * kWeightBias);
+            lo = __reduce_add_sync(0xffffffffu, lo - kChunk / 32 * kWeightBias);
+            const i64 s = (static_cast<i64>(hi) << 16) + lo;
             if (lane == 0) sums[c] = s;
         }
         __syncthreads();

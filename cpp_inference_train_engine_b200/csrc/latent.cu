@@ -509,12 +509,15 @@ int mm_verify_drafts(const void* target_probs, const void* draft_probs, int dtyp
             const T* p = static_cast<const T*>(target_probs);
             const T* q = drafts > 0 ? static_cast<const T*>(draft_probs) : nullptr;
             auto fits = [&](const void* x) { return reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0; };
-            if (vocab % 4 == 0 && fits(p) && fits(q))
-                launch(s, mm::ver::verify_drafts_kernel<T, true>, dim3(rows), dim3(mm::ver::kThreads), 0, p, q, draft_tokens,
-                       draft_len, u_accept, u_sample, drafts, vocab, out_tokens, accepted);
+            auto run = [&](auto kernel, int threads) {
+                launch(s, kernel, dim3(rows), dim3(threads), 0, p, q, draft_tokens, draft_len, u_accept, u_sample, drafts, vocab,
+                       out_tokens, accepted);
+            };
+            const bool aligned = vocab % 4 == 0 && fits(p) && fits(q);
+            if (rows >= 5 * sm_count())
+                aligned ? run(mm::ver::verify_drafts_kernel<T, true, 512>, 512) : run(mm::ver::verify_drafts_kernel<T, false, 512>, 512);
             else
-                launch(s, mm::ver::verify_drafts_kernel<T, false>, dim3(rows), dim3(mm::ver::kThreads), 0, p, q, draft_tokens,
-                       draft_len, u_accept, u_sample, drafts, vocab, out_tokens, accepted);
+                aligned ? run(mm::ver::verify_drafts_kernel<T, true, 1024>, 1024) : run(mm::ver::verify_drafts_kernel<T, false, 1024>, 1024);
         });
     });
 }

@@ -610,3 +610,24 @@ def test_attention_thousands_of_groups(width, prefix):
     suf = make_cache(torch, g, slen, 4, kv, rope, torch.float16, False)
     q = torch.randn(starts[-1], 1, H, kv + rope, generator=g, device="cuda").half()
     check_attention(torch, latent, q, pre, suf, starts, plen, slen, kv, 0.1)
+
+
+@pytest.mark.parametrize("vocab", [1024, 1027])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_verify_many_rows(vocab, dtype):
+    """A batch of several blocks per multiprocessor gives each row what it gets in a small batch."""
+    torch, latent = mods()
+    dtype = getattr(torch, dtype)
+    g = torch.Generator(device="cuda").manual_seed(21)
+    B, K = 900, 3
+    p = torch.softmax(2 * torch.randn(B, K + 1, vocab, generator=g, device="cuda"), -1).to(dtype)
+    q = torch.softmax(2 * torch.randn(B, K, vocab, generator=g, device="cuda"), -1).to(dtype)
+    x = torch.randint(0, vocab, (B, K), generator=g, device="cuda", dtype=torch.int32)
+    n = torch.randint(0, K + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    ua, us = torch.rand(B, K, generator=g, device="cuda"), torch.rand(B, generator=g, device="cuda")
+    for d in (q, None):
+        tokens, accepted = latent.verify_drafts(p, x, n, ua, us, draft_probs=d)
+        for b in range(0, B, 90):
+            r = slice(b, b + 90)
+            t, a = latent.verify_drafts(p[r], x[r], n[r], ua[r], us[r], draft_probs=None if d is None else d[r])
+            assert torch.equal(t, tokens[r]) and torch.equal(a, accepted[r])
