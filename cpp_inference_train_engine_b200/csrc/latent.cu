@@ -245,7 +245,9 @@ struct Plan {
     bool join = false;                             // a join launch: not every row is one suffix range
     long long rows = 0;                            // query rows
     long long pre_part = 0, suf_part = 0;          // partial query rows held by the workspace
-    long long bytes(int kv) const { return (pre_part + suf_part) * (kv + 2) * 4; }
+    bool span = false;                             // suffix rows in even shares of their tiles (TcArgs::pieces)
+    long long pieces = 0;                          // rows whose parts the workspace lists
+    long long bytes(int kv) const { return (pre_part + suf_part) * (kv + 2) * 4 + pieces * 8; }
 };
 
 // Key ranges per query block: the waves of (block, range) items over the SMs times an item's
@@ -280,9 +282,19 @@ Plan plan(const mm::spa::Problem& p) {
         r.suf_n = th <= 16 ? 16 : 64;
         r.suf_blocks = p.B * ((th + r.suf_n - 1) / r.suf_n);
         pick_splits(r.suf_blocks, p.max_suffix, 16, r.suf_splits, r.suf_kps);
+        // Rows long enough to be worth cutting, one range each: the launch may divide them by their lengths
+        using C = mm::spa::TcCfg<512, 32, 16, false>;
+        const long long ctas = sm_count() * C::kCtas, tiles = (p.max_suffix + C::KT - 1) / C::KT, weight = p.B * (tiles + 1);
+        r.span = p.kv == 512 && r.suf_n == 16 && r.suf_splits == 1 && tiles >= 8 && r.pre_splits <= mm::spa::kMaxJoin &&
+                 weight + ctas * mm::spa::kMinSpan <= kMaxBlocks;
+        if (r.span) {
+            r.suf_blocks = std::min(ctas, weight);
+            r.suf_part = 2 * r.suf_blocks * 16;
+            r.pieces = p.B;
+        }
     }
-    r.join = r.suf_n != 16 || r.suf_splits > 1 || r.pre_splits > mm::spa::kMaxJoin;
-    if (r.join) r.suf_part = r.rows * r.suf_splits;
+    r.join = r.span || r.suf_n != 16 || r.suf_splits > 1 || r.pre_splits > mm::spa::kMaxJoin;
+    if (r.join && !r.span) r.suf_part = r.rows * r.suf_splits;
     if (r.pre_blocks * std::max(1, r.pre_splits) > kMaxBlocks || r.suf_blocks * std::max(1, r.suf_splits) > kMaxBlocks)
         refuse(MM_UNSUPPORTED, "shared-prefix attention: too many query rows");
     return r;
@@ -343,6 +355,7 @@ void run_tc(const mm::spa::Problem& p, const Plan& r, bool q8p, bool q8s, void* 
     float* suf_o = pre_o + r.pre_part * KV;
     float2* pre_ml = reinterpret_cast<float2*>(suf_o + r.suf_part * KV);
     float2* suf_ml = pre_ml + r.pre_part;
+    int2* pieces = r.span ? reinterpret_cast<int2*>(suf_ml + r.suf_part) : nullptr;
     TcArgs a{};
     a.p = p;
     if (r.pre_n) {
@@ -362,12 +375,14 @@ void run_tc(const mm::spa::Problem& p, const Plan& r, bool q8p, bool q8s, void* 
         a.pre_ml = pre_ml;
         a.prefix_kps = r.pre_kps;
         a.overlap = r.pre_n ? 1 : 0;
+        a.pieces = pieces;
         launch_tc_n<KV, R, T>(a, r.suf_n, q8s, r.suf_blocks * r.suf_splits, s);
     }
     if (r.join)
-        launch(s, shared_prefix_join_kernel<KV, T>, dim3(blocks(r.rows, 8)), dim3(256), 0, p, static_cast<const float*>(pre_o),
-               static_cast<const float2*>(pre_ml), r.pre_kps, static_cast<const float*>(suf_o),
-               static_cast<const float2*>(suf_ml), r.suf_kps, r.suf_n == 16 ? 1 : 0);
+        launch(s, r.span ? shared_prefix_join_kernel<KV, T, true> : shared_prefix_join_kernel<KV, T, false>, dim3(blocks(r.rows, 8)),
+               dim3(256), 0, p, static_cast<const float*>(pre_o), static_cast<const float2*>(pre_ml), r.pre_kps,
+               static_cast<const float*>(suf_o), static_cast<const float2*>(suf_ml), r.suf_kps, r.suf_n == 16 ? 1 : 0,
+               static_cast<const int2*>(pieces));
 }
 
 }  // namespace

@@ -18,13 +18,14 @@
 //              (tensor-memory lane). The running maximum is lazy: the first tile's maximum is the
 //              reference, and a later tile whose scores stay below the reference + 8 (base 2) uses
 //              it as it is (probabilities up to 2^8 fit fp16, sums are fp32), decided by one 4-warp
-//              vote; otherwise the column maxima are taken and O^T and the sums are rescaled. A key's scale (e4m3) multiplies its latent
-//              scores and, for the second product, its probabilities.
+//              vote; otherwise the column maxima are taken and O^T and the sums are rescaled. A key's
+//              scale (e4m3) multiplies its latent scores and, for the second product, its
+//              probabilities.
 //   producers  2 to 8: the item's queries, then per tile of KT keys the rope columns and kv / 128 pairs
 //              of 64-column boxes (each pair its own warps) into rings of swizzled boxes. 16-bit caches come
-//              by TMA (where the encoder does not take the strides: by 16-byte cp.async); e4m3 codes are loaded D tiles ahead into registers and stored as 16-bit
-//              values (exact). What the cache holds past the range is masked in
-//              S and never read by an O product.
+//              by TMA (where the encoder does not take the strides: by 16-byte cp.async); e4m3 codes
+//              are loaded D tiles ahead into registers and stored as 16-bit values (exact). What the
+//              cache holds past the range is masked in S and never read by an O product.
 //   fence      one warp passes each landed tile on to the asynchronous proxy: a proxy fence costs
 //              about 100 ns, and in the loading threads it would wait for every load they have in
 //              flight (measured: 1.7 instead of over 5 TB/s).
@@ -33,6 +34,13 @@
 //              is tensor-memory lane 32 (r / 16) + r % 16.
 // Every mbarrier wait is bounded; after a wait that runs out the CTA goes on without waiting (every
 // loop is bounded, every access in bounds) and its results are NaN.
+//
+// Measured on one B200. Cache loads: 296 rows of 1,024 positions, 512 + 32 wide, fp16, 66 us (5.0 TB/s of
+// the 6.5 a copy reaches); one SM's ring holds ten pairs of boxes (160 KB). e4m3 rows are bound by their
+// conversion instead (1.9 us a tile of 64). Products: 2,048 query rows over one prompt of 8,192, 80 us
+// (445 TFLOP/s): an N = 64 product takes 48 cycles where the pipe's rate would allow 32, its S product has
+// M = 64, and two tiles fill the ring. (128 queries would run at the full rate, but their fp32 O^T fills the
+// tensor memory at 512 columns.)
 #pragma once
 #include <type_traits>
 
@@ -56,11 +64,16 @@ struct TcArgs {
     const float2* pre_ml;
     int prefix_kps;
     int overlap;       // the launch before this one is the call's own prefix launch: run beside it
+    // a suffix launch of 16-query blocks, 512 wide, may divide the tiles of all its rows evenly over the
+    // CTAs; a row cut where a CTA's share ends is left to the join kernel. Per row the first CTA and the number of
+    // its parts (0: whole, the launch wrote its result); null: key ranges
+    int2* pieces;
     int tma;           // the tensor maps are valid: a 16-bit cache comes by TMA
 };
 
 constexpr int kTcMaxPlan = 512;   // entries of the shared plan (the items of runs of groups or rows)
 constexpr int kTcTable = 32;      // items per shared table
+constexpr int kMinSpan = 4;       // tiles of a CTA's share at least
 constexpr int kMaxJoin = 4;       // prefix ranges a suffix launch joins itself
 constexpr float kNoMax = -1e37f;  // running maximum before any key (finite: its exp2 is 0, never NaN)
 
@@ -69,7 +82,7 @@ struct Item {
     int q0, nq;       // query rows [q0, q0 + nq)
     int row;          // cache row
     int k0, nk, nt;   // first key, keys, tiles (0: nothing to attend)
-    int split;
+    int split;        // key range (span: the CTA's slot of partials)
     int np;           // the prefix ranges to join to the result, -1: this item writes partials
 };
 
@@ -118,7 +131,7 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int oTab = oP + PB * kP;
     static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N], up[N], mail[2][5][N], factor[5][N]
     static constexpr int oPlan = oF + (8 + (EW ? 15 : 0)) * N * 4;
-    static constexpr int oBar = oPlan + (kTcMaxPlan + 1) * 4 + 4;
+    static constexpr int oBar = oPlan + (kTcMaxPlan + 1) * 4 + 12;
     static constexpr int kBars = QB + PS + 2 * TS + 4 + 2 * PB + 2 * OB + 4;
     static_assert(RS * NP >= PS && TS * NP >= PS, "the rope ring and the tile barriers outlast the pair ring");
     static constexpr int kSmem = oBar + kBars * 8 + 16 + 1024;  // + alignment of the base
@@ -305,6 +318,51 @@ __device__ __forceinline__ Item get_item(const TcArgs& a, const int* plan, int u
     return it;
 }
 
+// Even shares of a suffix launch's work: a row weighs its tiles and one more (its queries and results),
+// CTA c has the weights [c span, (c + 1) span) of the rows in line. What a share holds of a row is one
+// item; a cut row's first part is its CTA's last item (slot 2 c + 1), a later part its CTA's first (slot 2 c).
+template <int KT> __device__ __forceinline__ int row_weight(const Problem& p, int u) {
+    return (suffix_length(p, u) + KT - 1) / KT + 1;
+}
+// The row that holds weight w; before: the weight of the rows ahead of it.
+template <int KT>
+__device__ __forceinline__ int row_at(const Problem& p, const int* plan, int units, int step, int w, int& before) {
+    int lo = 0, hi = (units + step - 1) / step;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (plan[mid] <= w) lo = mid;
+        else hi = mid;
+    }
+    int u = lo * step;
+    before = plan[lo];
+    const int last = min(units, u + step) - 1;
+    for (int n; u < last && before + (n = row_weight<KT>(p, u)) <= w; ++u) before += n;
+    return u;
+}
+template <int KT>
+__device__ __forceinline__ Item span_item(const TcArgs& a, const int* plan, int step, int span, int u) {
+    const Problem& p = a.p;
+    int before = plan[u / step];
+    for (int v = u / step * step; v < u; ++v) before += row_weight<KT>(p, v);
+    const int th = p.T * p.H, len = suffix_length(p, u), nt = (len + KT - 1) / KT;
+    const int w0 = static_cast<int>(blockIdx.x) * span, from = min(max(w0 - before, 0), nt), to = min(w0 + span - before, nt);
+    const bool whole = before >= w0 && to == nt;
+    if (whole || (to == nt && from < nt)) {  // the share that ends the row notes its parts
+        const int first = before / span;
+        a.pieces[u] = make_int2(first, whole ? 0 : static_cast<int>(blockIdx.x) - first + 1);
+    }
+    Item it;
+    it.row = u;
+    it.q0 = u * th;
+    it.nq = th;
+    it.k0 = from * KT;
+    it.nt = to - from;
+    it.nk = min(len - it.k0, it.nt * KT);
+    it.split = 2 * static_cast<int>(blockIdx.x) + (from == 0 ? 1 : 0);
+    it.np = whole ? (prefix_length(p, p.G > 0 ? group_of(p, u) : -1) + a.prefix_kps - 1) / a.prefix_kps : -1;
+    return it;
+}
+
 // Position in a ring of S barriers: the slot and its phase parity.
 template <int S> struct Ring {
     int i = 0;
@@ -405,16 +463,23 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     pdl_launch_dependents();
     const int units = a.suffix ? p.B : p.G;
     const int per = ((a.suffix ? th : p.max_group * th) + N - 1) / N;
+    constexpr bool kShares = KV == 512 && N == 16;  // (128 wide: the registers of two CTAs per SM are needed)
     const int* plan = nullptr;
     int items = units * per;
     const int step = (units + kTcMaxPlan - 1) / kTcMaxPlan;
-    if (a.splits > 1 || !a.suffix) {
+    bool spans = kShares && a.pieces;
+    if (spans || a.splits > 1 || !a.suffix) {
         plan = plan_s;
         const int runs = (units + step - 1) / step;
         for (int i = tid; i < runs; i += C::kThreads) {
-            int n = unit_items<N>(a, i * step);
+            int n = 0;
+            if (kShares && spans) {
+                for (int u = i * step; u < min(units, (i + 1) * step); ++u) n += row_weight<KT>(p, u);
+            } else {
+                n = unit_items<N>(a, i * step);
 #pragma unroll 1
-            for (int u = i * step + 1; u < min(units, (i + 1) * step); ++u) n += unit_items<N>(a, u);
+                for (int u = i * step + 1; u < min(units, (i + 1) * step); ++u) n += unit_items<N>(a, u);
+            }
             plan_s[i + 1] = n;
         }
         __syncthreads();
@@ -435,11 +500,41 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         __syncthreads();
         items = plan_s[runs];
     }
+    // Shares, or the rows one by one in turn, which needs no join and serves rows of like lengths: by the
+    // fullest CTA's rows against the mean. 512 + 32 wide, 136 ragged rows of up to 1,536 (2.1): 70.4 us in
+    // turn, 65.0 in shares, as e4m3 86 and 72; 300 rows of 700 (1.5): 79.5 in turn, 89.8 in shares.
+    int span = 0;
+    if (kShares && spans) {
+        int* bins = reinterpret_cast<int*>(table);  // free until the first table
+        const int grid = static_cast<int>(gridDim.x);
+        int most = 0;
+        if (grid <= kTcTable * 8) {
+            for (int i = tid; i < grid; i += C::kThreads) bins[i] = 0;
+            __syncthreads();
+            for (int u = tid; u < units; u += C::kThreads) atomicAdd(&bins[u % grid], row_weight<KT>(p, u));
+            __syncthreads();
+            for (int i = lane; i < grid; i += 32) most = max(most, bins[i]);
+            most = __reduce_max_sync(0xffffffffu, most);
+        }
+        span = max((items + grid - 1) / grid, kMinSpan);
+        if (most > 0 && 4 * most < 7 * span) {
+            spans = false;
+            plan = nullptr;
+            items = units;
+        } else if (tid < 2) {
+            // the first row of the share and the row after its last
+            const int w = min((static_cast<int>(blockIdx.x) + tid) * span, items) - tid;
+            int before, u = units;
+            if (w >= 0 && w < items) u = row_at<KT>(p, plan, units, step, w, before) + tid;
+            plan_s[kTcMaxPlan + 1 + tid] = u;
+        }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int mine = blockIdx.x < items ? (items - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+    const int mine = kShares && spans ? max(plan_s[kTcMaxPlan + 2] - plan_s[kTcMaxPlan + 1], 0)
+                           : blockIdx.x < items ? (items - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
     const lat::CacheView& cv = a.suffix ? p.suffix : p.prefix;
     bool ok = true;
     // a wait that ran out is recorded once; later waits of this thread are skipped
@@ -454,8 +549,15 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     auto next_table = [&](int base, auto builds) {
         if (base > 0) __syncthreads();
         if constexpr (decltype(builds)::value) {
-            if (tid < kTcTable && base + tid < mine)
-                table[tid] = get_item<N, KT>(a, plan, units, step, per, blockIdx.x + (base + tid) * gridDim.x);
+            if (tid < kTcTable && base + tid < mine) {
+                if (kShares && spans) {
+                    table[tid] = span_item<KT>(a, plan, step, span, plan_s[kTcMaxPlan + 1] + base + tid);
+                } else {
+                    const Item it = get_item<N, KT>(a, plan, units, step, per, blockIdx.x + (base + tid) * gridDim.x);
+                    table[tid] = it;
+                    if (kShares && a.pieces) a.pieces[it.row] = make_int2(0, 0);
+                }
+            }
         }
         __syncthreads();
         return min(kTcTable, mine - base);
@@ -990,7 +1092,8 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 const Item it = table[e0];
                 const bool direct = it.np >= 0;
                 if (it.nt == 0 && !direct) continue;
-                const long long at = it.q0;  // first query row; partials of this launch: + split * rows
+                const long long at = it.q0;  // first query row
+                const long long part = kShares && spans ? it.split * static_cast<long long>(N) : it.split * rows + at;
                 // The prefix's share of a direct result: unit u = (pair, prefix range) of the partials. The
                 // first is asked for before the item's tiles are done: a load issued behind a full ring
                 // of cache tiles waits its turn (2 to 4 us).
@@ -1020,7 +1123,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     if (*reinterpret_cast<volatile int*>(bad_s)) l_own = __int_as_float(0x7fc00000);
                     const float m_own = l_own == 0.f ? kNoMax : mail[4 * N + n];
                     if (!direct) {
-                        a.part_ml[it.split * rows + at + n] = make_float2(m_own, l_own);
+                        a.part_ml[part + n] = make_float2(m_own, l_own);
                     } else {
                         // joint maximum and sum with the prefix's ranges (at most kMaxJoin); each part's
                         // factor, the division by the sum included
@@ -1052,7 +1155,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     float v[16];
                     if (it.nt > 0) tmem_ld16(o + i * N, v);
                     if (!direct) {
-                        float* dst = a.part_o + (it.split * rows + at) * KV + i * 128 + dim;
+                        float* dst = a.part_o + part * KV + i * 128 + dim;
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
                             if (e < it.nq) dst[static_cast<long long>(e) * KV] = v[e];
@@ -1098,23 +1201,35 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
 
 // Joins the partials of a query row: its group's prefix ranges and its suffix ranges. One warp
 // per query row, kv / 32 columns per lane.
-template <int KV, typename T>
+template <int KV, typename T, bool PIECES>
 __global__ void __launch_bounds__(256) shared_prefix_join_kernel(const Problem p, const float* __restrict__ pre_o,
                                                                  const float2* __restrict__ pre_ml, int pre_kps,
                                                                  const float* __restrict__ suf_o,
                                                                  const float2* __restrict__ suf_ml, int suf_kps,
-                                                                 int direct) {
+                                                                 int direct, const int2* __restrict__ pieces) {
     MM_PDL_ENTRY();
     const int th = p.T * p.H, lane = threadIdx.x & 31;
     const long long rows = static_cast<long long>(p.B) * th;
     const long long r = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
     if (r >= rows) return;
     const int b = static_cast<int>(r / th);
-    if (direct && direct_join(p, b, suf_kps, pre_kps) >= 0) return;  // the suffix launch wrote it
+    int first = 0, ns;
+    if constexpr (PIECES) {  // the parts of a row cut between CTAs
+        const int2 v = __ldcg(&pieces[b]);
+        if (v.y == 0) return;  // the suffix launch wrote it
+        first = v.x;
+        ns = v.y;
+    } else {
+        if (direct && direct_join(p, b, suf_kps, pre_kps) >= 0) return;  // the suffix launch wrote it
+        ns = (suffix_length(p, b) + suf_kps - 1) / suf_kps;
+    }
     const int g = p.G > 0 ? group_of(p, b) : -1;
     const int np = (prefix_length(p, g) + pre_kps - 1) / pre_kps;
-    const int ns = (suffix_length(p, b) + suf_kps - 1) / suf_kps;
-    auto ml = [&](int s) { return s < np ? __ldcg(&pre_ml[s * rows + r]) : __ldcg(&suf_ml[(s - np) * rows + r]); };
+    auto suf_at = [&](int s) {  // the query row of suffix part s among the partials
+        if constexpr (PIECES) return (2LL * (first + s) + (s == 0)) * 16 + (r - static_cast<long long>(b) * th);
+        else return s * rows + r;
+    };
+    auto ml = [&](int s) { return s < np ? __ldcg(&pre_ml[s * rows + r]) : __ldcg(&suf_ml[suf_at(s - np)]); };
     float M = kNoMax;
     for (int s = lane; s < np + ns; s += 32) M = fmaxf(M, ml(s).x);
     M = warp_max(M);
@@ -1132,7 +1247,7 @@ __global__ void __launch_bounds__(256) shared_prefix_join_kernel(const Problem p
 #pragma unroll 4
     for (int s = 0; s < np + ns; ++s) {
         const float f = fast_exp2(ml(s).x - M);
-        const float4* o = reinterpret_cast<const float4*>((s < np ? pre_o + (s * rows + r) * KV : suf_o + ((s - np) * rows + r) * KV)) + lane;
+        const float4* o = reinterpret_cast<const float4*>((s < np ? pre_o + (s * rows + r) * KV : suf_o + suf_at(s - np) * KV)) + lane;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const float4 v = __ldcg(o + 32 * c);

@@ -631,3 +631,27 @@ def test_verify_many_rows(vocab, dtype):
             r = slice(b, b + 90)
             t, a = latent.verify_drafts(p[r], x[r], n[r], ua[r], us[r], draft_probs=None if d is None else d[r])
             assert torch.equal(t, tokens[r]) and torch.equal(a, accepted[r])
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16", "fp8/fp16", "mixed"])
+@pytest.mark.parametrize("shape", ["ragged", "one long", "alike", "many"])
+def test_attention_rows_divided_by_their_lengths(kind, shape):
+    """Suffixes of very different lengths over as many rows as there are CTAs, with short prefixes: rows
+    are cut where a CTA's share ends."""
+    torch, latent = mods()
+    kv, rope, H = 512, 32, 5
+    dtype = torch.bfloat16 if "bf16" in kind else torch.float16
+    g = torch.Generator(device="cuda").manual_seed(23)
+    T = 2 if shape == "ragged" else 1
+    B = 700 if shape == "many" else 141
+    slen = {"ragged": [(b * 211) % 601 for b in range(B)], "one long": [b % 3 for b in range(B - 1)] + [1500],
+            "alike": [520 + b % 3 for b in range(B)], "many": [0 if b % 5 else (b * 37) % 700 for b in range(B)]}[shape]
+    groups = [B // 3, 0, B - B // 3 - 4]  # the last rows have no prefix
+    starts = [0, groups[0], groups[0], groups[0] + groups[2]]
+    plen = [130, 5, 0 if shape == "many" else 64]
+    pre = make_cache(torch, g, plen, 131, kv, rope, dtype, "fp8" in kind or kind == "mixed")
+    suf = make_cache(torch, g, slen, max(slen), kv, rope, dtype, "fp8" in kind)
+    q = torch.randn(B, T, H, kv + rope, generator=g, device="cuda").to(dtype)
+    a = check_attention(torch, latent, q, pre, suf, starts, plen, slen, kv, 0.08)
+    b = check_attention(torch, latent, q, pre, suf, starts, plen, slen, kv, 0.08)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
