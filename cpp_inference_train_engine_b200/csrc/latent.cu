@@ -81,6 +81,9 @@ template <auto Kernel> void set_dynamic_smem(int bytes) {
     done.fetch_or(bit);
 }
 
+// Whether p is a multiple of n bytes.
+bool multiple(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
 void check_cache(const mm_latent_cache* c) {
     require(c->rows >= 0 && c->positions >= 0, "latent cache: negative size");
     require(c->kv >= 1 && c->kv <= 1024 && c->rope_dim >= 0 && c->rope_dim <= 256,
@@ -92,6 +95,8 @@ void check_cache(const mm_latent_cache* c) {
         require(c->rope_kind == MM_F16 || c->rope_kind == MM_BF16, "latent cache: rope must be fp16 or bf16");
         require(empty || (c->scale && (c->rope || c->rope_dim == 0)), "latent cache: null storage");
     }
+    require(multiple(c->latent, c->kind == MM_E4M3 ? 1 : 2) && (c->kind != MM_E4M3 || (multiple(c->rope, 2) && multiple(c->scale, 4))),
+            "latent cache: storage not aligned to its elements");
 }
 
 mm::lat::CacheView view(const mm_latent_cache* c) {
@@ -134,7 +139,7 @@ template <class F> void with_half(int dtype, F&& f) {
     else refuse(MM_INVALID_ARGUMENT, "unsupported element type");
 }
 
-static_assert(sizeof(mm_latent_cache) == 88 && sizeof(mm_shared_prefix_desc) == 112, "the Python binding packs these field by field");
+static_assert(sizeof(mm_latent_cache) == 88 && sizeof(mm_shared_prefix_desc) == 112, "callers without this header pack these field by field");
 
 // Whether the rows of an e4m3 cache can be accessed 16 bytes at a time.
 bool aligned_e4m3(const mm_latent_cache* c) {
@@ -177,6 +182,8 @@ mm::spa::Problem problem(const mm_shared_prefix_desc* d, const mm_latent_cache* 
             "shared-prefix attention: max_prefix / max_suffix exceed the cache's positions");
     if (d->rows > 0) {
         require(d->q && d->out, "shared-prefix attention: null q or out");
+        require(multiple(d->q, 2) && multiple(d->out, 2) && multiple(d->lse, 4),
+                "shared-prefix attention: q, out or lse not aligned to its elements");
         require(d->groups == 0 || (d->group_start && d->prefix_len), "shared-prefix attention: null group_start or prefix_len");
         require(d->max_suffix == 0 || d->suffix_len, "shared-prefix attention: null suffix_len");
     }
@@ -227,14 +234,14 @@ int sm_count() {
 
 // ------------------------------------------------------------------ tensor-core plan
 // The tensor-core form covers the two latent widths of the framework's models when every row
-// can be read in 16-byte pieces.
+// can be read in 16-byte pieces and the results written in 8-byte ones (the join kernel).
 bool aligned_cache(const mm_latent_cache* c) {
     if (c->kind == MM_E4M3) return aligned_e4m3(c);
     return reinterpret_cast<uintptr_t>(c->latent) % 16 == 0 && c->row_stride % 8 == 0 && c->pos_stride % 8 == 0;
 }
 bool tensor_core_form(const mm::spa::Problem& p, const mm_latent_cache* prefix, const mm_latent_cache* suffix) {
     if (!((p.kv == 128 && p.rd == 16) || (p.kv == 512 && p.rd == 32))) return false;
-    if (reinterpret_cast<uintptr_t>(p.q) % 16 || p.q_row % 8 || p.q_tok % 8 || p.q_head % 8) return false;
+    if (!multiple(p.q, 16) || p.q_row % 8 || p.q_tok % 8 || p.q_head % 8 || !multiple(p.out, 8)) return false;
     return (p.G == 0 || aligned_cache(prefix)) && (p.max_suffix == 0 || aligned_cache(suffix));
 }
 
@@ -416,6 +423,7 @@ int mm_latent_cache_write(const mm_latent_cache* cache, const void* latent, int6
             with_half(cache->rope_kind, [&](auto half) {
                 using T = typename decltype(in)::type;
                 using T16 = typename decltype(half)::type;
+                require(multiple(latent, sizeof(T)) && multiple(rope, sizeof(T)), "cache write: input not aligned to its elements");
                 const long long e = 16 / sizeof(T);
                 const bool aligned = reinterpret_cast<uintptr_t>(latent) % 16 == 0 && latent_stride % e == 0 &&
                                      reinterpret_cast<uintptr_t>(rope) % 16 == 0 && rope_stride % e == 0;
@@ -452,6 +460,7 @@ int mm_latent_cache_read(const mm_latent_cache* cache, const int64_t* slots, int
             with_half(cache->rope_kind, [&](auto half) {
                 using TO = typename decltype(o)::type;
                 using T16 = typename decltype(half)::type;
+                require(multiple(out, sizeof(TO)), "cache read: out not aligned to its elements");
                 const bool aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_stride * sizeof(TO) % 16 == 0;
                 if (with_width(cache, aligned, [&](auto kv, auto rd) {
                         constexpr int kKv = decltype(kv)::value, kRd = decltype(rd)::value, kU = 2;
@@ -525,6 +534,7 @@ int mm_verify_drafts(const void* target_probs, const void* draft_probs, int dtyp
             using T = typename decltype(t)::type;
             const T* p = static_cast<const T*>(target_probs);
             const T* q = drafts > 0 ? static_cast<const T*>(draft_probs) : nullptr;
+            require(multiple(p, sizeof(T)) && multiple(q, sizeof(T)), "draft verification: probabilities not aligned to their elements");
             auto fits = [&](const void* x) { return reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0; };
             auto run = [&](auto kernel, int threads) {
                 launch(s, kernel, dim3(rows), dim3(threads), 0, p, q, draft_tokens, draft_len, u_accept, u_sample, drafts, vocab,

@@ -83,7 +83,9 @@ int mm_latent_cache_read(const mm_latent_cache* cache, const int64_t* slots, int
  * q: dtype MM_F16 / MM_BF16 with element strides, last dimension contiguous; 16-bit caches
  * have the same dtype, e4m3 caches the same rope_kind. out [rows][tokens][heads][kv] of dtype
  * and lse [rows][tokens][heads] fp32 (may be NULL) are contiguous. prefix may be NULL (with
- * groups = 0), and so may suffix. */
+ * groups = 0), and so may suffix. Pointers are aligned to their elements; the tensor-core form
+ * (128 + 16 and 512 + 32 wide) also needs q and cache rows of 16-byte multiples at 16-byte
+ * addresses and out at an 8-byte one, other calls take a slower form of the same results. */
 typedef struct mm_shared_prefix_desc {
     const void* q;
     int64_t q_row_stride, q_token_stride, q_head_stride;
