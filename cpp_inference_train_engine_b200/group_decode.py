@@ -53,6 +53,9 @@ class GroupDecoder:
         rows = [rows] * len(prompts) if isinstance(rows, int) else list(rows)
         if len(rows) != len(prompts) or min(rows) < 1:
             raise EngineError(1, "rows: one positive number per group")
+        prompts = [list(map(int, p)) for p in prompts]
+        if any(not 0 <= t < cfg.vocab_size for p in prompts for t in p):
+            raise EngineError(1, "a prompt's token is outside the vocabulary")
         self.cfg, self.drafts, self.new_tokens, self.bits = cfg, drafts, new_tokens, cache_bits
         self.device = device
         flat = torch.from_numpy(np.ascontiguousarray(params, np.float32)).to(device)
@@ -83,7 +86,7 @@ class GroupDecoder:
         self.history = torch.full((B, self.max_prompt + self.capacity + 1), -1, dtype=torch.int32, device=device)
         padded = torch.zeros(G, self.max_prompt, dtype=torch.int32, device=device)
         for i, p in enumerate(prompts):
-            tokens = i32(list(map(int, p)))
+            tokens = i32(p)
             padded[i, self.max_prompt - len(p):] = tokens  # aligned at the end: the positions before the first are negative
             self.history[self.row_group == i, :len(p)] = tokens
         self.count = torch.zeros(B, dtype=torch.int64, device=device)  # generated tokens per row
@@ -128,7 +131,8 @@ class GroupDecoder:
         stores[layer] at `slots`, attends with attend(layer, q) and returns the final hidden rows."""
         c = self.cfg
         n, T = tokens.shape
-        x = self.embedding[tokens.long()].float()
+        # what only the device knows is kept inside the table instead of checked
+        x = self.embedding[tokens.long().clamp(0, c.vocab_size - 1)].float()
         for l, w in enumerate(self.layers):
             h = _rmsnorm(x, w["attn_norm"], c.norm_epsilon).half()
             cq = _rmsnorm(h @ w["w_dq"], w["q_norm"], c.norm_epsilon).half()

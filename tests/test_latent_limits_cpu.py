@@ -48,3 +48,13 @@ def test_inputs_inside_an_element_are_refused(dtype, off):
     assert L.mm_latent_cache_read(c, P, 1, P + off, 144, dtype, None) == 1 and "aligned" in message()
     assert L.mm_verify_drafts(P + off, None, dtype, P, P, P, P, 1, 1, 8, P, P, None) == 1 and "aligned" in message()
     assert L.mm_verify_drafts(P, P + off, dtype, P, P, P, P, 1, 1, 8, P, P, None) == 1 and "aligned" in message()
+
+
+@pytest.mark.parametrize("prompts", [[[1, 264]], [[1], [-1, 3]], [[1, 2 ** 40]]])
+def test_group_decoder_refuses_tokens_outside_the_vocabulary(prompts):
+    import numpy as np
+
+    from cpp_inference_train_engine_b200 import TINY, EngineError
+    from cpp_inference_train_engine_b200.group_decode import GroupDecoder
+    with pytest.raises(EngineError, match="vocabulary"):
+        GroupDecoder(TINY, np.zeros(TINY.parameter_count(), np.float32), prompts, 1, 4, device="cpu")
