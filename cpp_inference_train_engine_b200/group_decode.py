@@ -56,9 +56,12 @@ class GroupDecoder:
         prompts = [list(map(int, p)) for p in prompts]
         if any(not 0 <= t < cfg.vocab_size for p in prompts for t in p):
             raise EngineError(1, "a prompt's token is outside the vocabulary")
+        params = np.ascontiguousarray(params, np.float32).reshape(-1)
+        if params.size != cfg.parameter_count():
+            raise EngineError(1, f"the model has {cfg.parameter_count()} parameters, got {params.size}")
         self.cfg, self.drafts, self.new_tokens, self.bits = cfg, drafts, new_tokens, cache_bits
         self.device = device
-        flat = torch.from_numpy(np.ascontiguousarray(params, np.float32)).to(device)
+        flat = torch.from_numpy(params).to(device)
         tensors, at = [], 0
         for _, (r, c), _ in cfg.parameter_shapes():
             tensors.append(flat[at:at + r * c].view(r, c))

@@ -58,3 +58,13 @@ def test_group_decoder_refuses_tokens_outside_the_vocabulary(prompts):
     from cpp_inference_train_engine_b200.group_decode import GroupDecoder
     with pytest.raises(EngineError, match="vocabulary"):
         GroupDecoder(TINY, np.zeros(TINY.parameter_count(), np.float32), prompts, 1, 4, device="cpu")
+
+
+@pytest.mark.parametrize("by", [-1, 1])
+def test_group_decoder_refuses_parameters_of_another_model(by):
+    import numpy as np
+
+    from cpp_inference_train_engine_b200 import TINY, EngineError
+    from cpp_inference_train_engine_b200.group_decode import GroupDecoder
+    with pytest.raises(EngineError, match="parameters"):
+        GroupDecoder(TINY, np.zeros(TINY.parameter_count() + by, np.float32), [[1]], 1, 4, device="cpu")
