@@ -1,6 +1,6 @@
 // C entries of the shared-prompt decode operators (include/mm_latent.h): argument checks,
 // variant selection and launches. Everything is enqueued on the caller's stream; no entry
-// allocates, waits or throws.
+// allocates or throws, and none but mm_latent_status waits.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -405,6 +405,20 @@ size_t mm_latent_last_error(char* buf, size_t cap) {
         buf[n] = 0;
     }
     return g_error.size();
+}
+
+int mm_latent_status(void* stream) {
+    return guarded([&] {
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        int bits = 0;
+        const int none = 0;
+        check(cudaMemcpyFromSymbolAsync(&bits, mm::spa::latent_status, sizeof bits, 0, cudaMemcpyDeviceToHost, s), "status");
+        check(cudaStreamSynchronize(s), "status");
+        if (!bits) return;
+        check(cudaMemcpyToSymbolAsync(mm::spa::latent_status, &none, sizeof none, 0, cudaMemcpyHostToDevice, s), "status");
+        check(cudaStreamSynchronize(s), "status");
+        refuse(MM_GPU_ERROR, "shared-prefix attention: a kernel gave up on a wait; its results are NaN");
+    });
 }
 
 int mm_latent_cache_write(const mm_latent_cache* cache, const void* latent, int64_t latent_stride, const void* rope,

@@ -32,8 +32,10 @@
 //   results    4 (N = 16): an item's O^T and sums, joined with the prefix's share, to memory.
 //   MMA        one thread issues tcgen05.mma. With KT = 64 the S^T product has M = 64, whose row r
 //              is tensor-memory lane 32 (r / 16) + r % 16.
-// Every mbarrier wait is bounded; after a wait that runs out the CTA goes on without waiting (every
-// loop is bounded, every access in bounds) and its results are NaN.
+// Every mbarrier wait is bounded. After a wait that runs out the CTA asks for no more tiles and products and
+// goes on without waiting (every loop is bounded, every access in bounds): its results are NaN, the wait is
+// noted in latent_status, and the CTA ends once the copies and products that it had in flight have (waited for
+// with a limit of their own).
 //
 // Measured on one B200. Cache loads: 296 rows of 1,024 positions, 512 + 32 wide, fp16, 66 us (5.0 TB/s of
 // the 6.5 a copy reaches); one SM's ring holds ten pairs of boxes (160 KB). e4m3 rows are bound by their
@@ -48,6 +50,19 @@
 
 namespace mm {
 namespace spa {
+
+__device__ int latent_status;  // DeviceError bits since they were last read (mm_latent_status)
+
+// A CTA that gave up on a wait notes it and stays until the tiles that it asked for have landed (the phases
+// of their barriers that are open; a phase that nothing is in lasts its limit, some 20 ms): its shared memory
+// is another CTA's after that. Out of line: the code is never run and costs the tile loops registers.
+__device__ __noinline__ void end_after_timeout(uint64_t* tile_in, int n) {
+    raise_error(&latent_status, kErrWaitTimeout);
+    for (int i = 0; i < n; ++i) {
+        const uint32_t open = mbar_try_wait(&tile_in[i], 0) ? 1 : 0;
+        for (int k = 0; k < 1 << 16 && !mbar_try_wait(&tile_in[i], open); ++k) __nanosleep(256);
+    }
+}
 
 // How a launch covers its items and where its partial results go.
 struct TcArgs {
@@ -132,7 +147,7 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N], up[N], mail[2][5][N], factor[5][N]
     static constexpr int oPlan = oF + (8 + (EW ? 15 : 0)) * N * 4;
     static constexpr int oBar = oPlan + (kTcMaxPlan + 1) * 4 + 12;
-    static constexpr int kBars = QB + PS + 2 * TS + 4 + 2 * PB + 2 * OB + 4;
+    static constexpr int kBars = QB + PS + 2 * TS + 4 + 2 * PB + 2 * OB + 4 + 1;
     static_assert(RS * NP >= PS && TS * NP >= PS, "the rope ring and the tile barriers outlast the pair ring");
     static constexpr int kSmem = oBar + kBars * 8 + 16 + 1024;  // + alignment of the base
     static_assert(kCtas * (kSmem + 1024) <= 228 * 1024 && kCols * kCtas <= 512, "shared and tensor memory");
@@ -433,6 +448,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     uint64_t* o_free = o_full + C::OB;           // [OB] the warps that write the results
     uint64_t* e_full = o_free + C::OB;           // [2] the softmax warps: an item's sums and maxima
     uint64_t* e_free = e_full + 2;               // [2] the result warps
+    uint64_t* ended = e_free + 2;                // after a wait that ran out: the products in flight are complete
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
     int* bad_s = reinterpret_cast<int*>(tmem_slot + 1);
     const Problem& p = a.p;
@@ -449,6 +465,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             for (int i = 0; i < C::PB; ++i) { mbar_init(&p_full[i], C::SW); mbar_init(&p_free[i], 1); }
             for (int i = 0; i < C::OB; ++i) { mbar_init(&o_full[i], 1); mbar_init(&o_free[i], C::EW ? C::EW : C::SW); }
             for (int i = 0; i < 2; ++i) { mbar_init(&e_full[i], C::SW); mbar_init(&e_free[i], 4); }
+            mbar_init(ended, 1);
             *bad_s = 0;
             fence_mbar_init();
         }
@@ -641,7 +658,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     if (a.tma) {
                         // one thread per pair asks for its two boxes, a range's last tile in the blocks of 32
                         // positions that the range reaches, and the first pair's for the rope columns
-                        if (sub == 0 && elect_one()) {
+                        if (sub == 0 && elect_one() && ok) {
                             const int nb = min((left + 31) >> 5, KT / 32), pos = it.k0 + c.j * KT;
                             uint64_t* bar = &tile_in[rt.i];
                             mbar_arrive_expect_tx(bar, nb * (2 * 4096 + (own == 0 ? 64 * R : 0)));
@@ -662,7 +679,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                                     tma_load_3d(sRope + rr.i * C::kRopeA + k * 64 * R, &map_rope, bar, KV, pos + 32 * k, it.row);
                             }
                         }
-                        __syncwarp();
+                        if (__any_sync(0xffffffffu, !ok)) break;
                         end_tile();
                         continue;
                     }
@@ -852,7 +869,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 // a tile's O when its probabilities are there, else the next tile's S when its boxes are:
                 // neither waits behind the other
                 int polls = 0;
-                while (co.valid()) {
+                while (ok && co.valid()) {
                     if (ahead > 0 && mbar_test(&p_full[pb.i], pb.phase)) {
                         issue_o(co);
                         polls = 0;
@@ -860,12 +877,14 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                                mbar_test(&s_free[ss.i], ss.phase ^ 1)) {
                         issue_s(cs);
                         polls = 0;
-                    } else if (!ok || ++polls > (1 << 24)) {  // gave up: go on in order without waiting
+                    } else if (++polls > (1 << 24)) {
                         ok = false;
                         *reinterpret_cast<volatile int*>(bad_s) = 1;
-                        if (ahead == 0) issue_s(cs);
-                        else issue_o(co);
                     }
+                }
+                if (!ok) {  // the products in flight end before the CTA does
+                    tc_commit(ended);
+                    mbar_wait_bounded(ended, 0, nullptr);
                 }
             }
             __syncwarp();
@@ -1193,6 +1212,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     if (C::EW == 0 && a.overlap) pdl_wait();  // nor with 64-query blocks
     tc_fence_before();
     __syncthreads();
+    if (tid == 0 && *reinterpret_cast<volatile int*>(bad_s)) end_after_timeout(tile_in, C::TS);
     if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, C::kTmem);

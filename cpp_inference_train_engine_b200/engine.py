@@ -84,6 +84,8 @@ def lib():
                                                      ctypes.c_float]),
         "mm_cuda_create": (ctypes.c_int, [ctypes.POINTER(ModelDesc), ctypes.c_int, ctypes.c_int,
                                           ctypes.POINTER(AdamWDesc), ctypes.POINTER(_vp)]),
+        "mm_latent_status": (ctypes.c_int, [_vp]),
+        "mm_latent_last_error": (ctypes.c_size_t, [ctypes.c_char_p, ctypes.c_size_t]),
         "mm_cuda_destroy": (None, [_vp]),
         "mm_cuda_last_error": (ctypes.c_size_t, [_vp, ctypes.c_char_p, ctypes.c_size_t]),
         "mm_cuda_upload_params": (ctypes.c_int, [_vp, _f32p, _f32p, _f32p, ctypes.c_uint64]),

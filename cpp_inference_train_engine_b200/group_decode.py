@@ -241,6 +241,7 @@ class GroupDecoder:
             steps += 1
             kept += int((accepted * (number > 0)).sum())
             proposed += int(number.sum())
+        latent.check_status(self.device)
         history, count, start = self.history.cpu(), self.count.cpu(), self.row_prompt.cpu()
         out = [history[b, start[b]:start[b] + count[b]].tolist() for b in range(B)]
         return out, {"steps": steps, "tokens": int(count.sum()), "proposed": proposed, "accepted": kept}

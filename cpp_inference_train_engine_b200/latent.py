@@ -16,13 +16,15 @@ The reference decodes one request at a time over its own fp32 cache
 (src/infer/inference.cpp:47-174, 469-579). A 16-bit cache is a plain tensor ``[rows,
 positions, kv + rope]`` (the layout of the context's own cache), an 8-bit one a
 :class:`LatentCache`. Calls enqueue on the current stream of the tensors' device and do not
-wait; outputs and scratch come from torch's allocator. Failures raise :class:`EngineError`.
+wait; outputs and scratch come from torch's allocator. Failures raise :class:`EngineError`
+(what only the device knows: ``check_status``).
 
 The checks, allocations and C calls are in csrc/latent_torch.cpp (a small call's time is its
 host path); this module names the arguments and documents them.
 """
 from __future__ import annotations
 
+import ctypes
 import importlib.machinery
 import importlib.util
 import os
@@ -49,6 +51,17 @@ def _load():
 _ext = _load()
 _attention, _write, _read, _verify = (_ext.shared_prefix_attention, _ext.cache_write, _ext.cache_read,
                                       _ext.verify_drafts)
+
+
+def check_status(device=None) -> None:
+    """Waits for the current stream and raises EngineError when a kernel of these operators gave up on
+    a wait on `device` since the last check (the results it concerns are NaN)."""
+    with torch.cuda.device(device):
+        rc = lib().mm_latent_status(torch.cuda.current_stream().cuda_stream)
+    if rc:
+        text = ctypes.create_string_buffer(512)
+        lib().mm_latent_last_error(text, len(text))
+        raise EngineError(rc, text.value.decode())
 
 
 class LatentCache(NamedTuple):

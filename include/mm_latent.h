@@ -8,7 +8,7 @@
  * Conventions:
  *   - every call validates what the host can see, enqueues its kernels on `stream` (a
  *     cudaStream_t of the current device; NULL = the legacy default stream) and returns
- *     without waiting. Nothing is allocated and no context is involved; scratch is the
+ *     without waiting (mm_latent_status alone waits). Nothing is allocated and no context is involved; scratch is the
  *     caller's `workspace` and may be reused by the next call on the same stream;
  *   - returns 0 or 1 + ErrorCode as include/mm_cuda.h; mm_latent_last_error() gives the
  *     calling thread's last message. No C++ exception leaves an entry;
@@ -16,7 +16,9 @@
  *     on the host; kernels clamp or skip out-of-range values, so no access leaves a buffer;
  *   - results do not depend on scheduling (no floating-point atomics): equal inputs give equal
  *     bits;
- *   - memory past a length may hold anything, NaN included: it never reaches a result.
+ *   - memory past a length may hold anything, NaN included: it never reaches a result;
+ *   - the attention kernel's waits are bounded. One that runs out (a defect or a fault of the
+ *     machine, never the input) makes the results it concerns NaN, and mm_latent_status says so.
  */
 #ifndef MM_LATENT_H
 #define MM_LATENT_H
@@ -54,6 +56,10 @@ typedef struct mm_latent_cache {
 /* Copies the calling thread's last message (NUL-terminated, truncated to cap); returns its
  * length. */
 size_t mm_latent_last_error(char* buf, size_t cap);
+
+/* Waits for `stream` and reports whether a kernel of this library on the current device gave up on
+ * a wait since the last report: 0, or MM_GPU_ERROR (results of a call in between are then NaN). */
+int mm_latent_status(void* stream);
 
 /* Quantises n new positions into an MM_E4M3 cache. latent [n][kv] and rope [n][rope_dim] of
  * `dtype` (row strides in elements); position i goes to slots[i] = row * positions + position;

@@ -68,3 +68,11 @@ def test_group_decoder_refuses_parameters_of_another_model(by):
     from cpp_inference_train_engine_b200.group_decode import GroupDecoder
     with pytest.raises(EngineError, match="parameters"):
         GroupDecoder(TINY, np.zeros(TINY.parameter_count() + by, np.float32), [[1]], 1, 4, device="cpu")
+
+
+def test_status_of_the_waits_is_reported():
+    """mm_latent_status tells the host of waits that ran out; without a device it fails loudly."""
+    import cpp_inference_train_engine_b200 as E
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is present")
+    assert E.lib().mm_latent_status(None) == 5 and "status" in message()
