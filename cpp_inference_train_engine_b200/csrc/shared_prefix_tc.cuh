@@ -16,11 +16,15 @@
 // phases run on across items. Warps:
 //   softmax    4 (N = 16) or 8 (N = 64, each four take 32 of the queries): thread = key
 //              (tensor-memory lane). The running maximum is lazy: the first tile's maximum is the
-//              reference, and a later tile whose scores stay below the reference + 8 (base 2) uses
-//              it as it is (probabilities up to 2^8 fit fp16, sums are fp32), decided by one 4-warp
-//              vote; otherwise the column maxima are taken and O^T and the sums are rescaled. A key's
-//              scale (e4m3) multiplies its latent scores and, for the second product, its
-//              probabilities.
+//              reference, and a later tile whose weights stay below 2^8 times the largest of the first
+//              uses it as it is, decided by one 4-warp vote; otherwise the column maxima are taken and
+//              O^T and the sums are rescaled. A key's scale (e4m3) multiplies its latent scores and,
+//              for the second product, its probabilities.
+//              The second product takes the weights (probability, times the scale) as 16-bit values, each
+//              rounded once, as the tensor cores' operand has to be; sums and statistics are fp32. So that
+//              fp16 loses no weight to its range, the maximum is taken over the weights (score + log2 scale)
+//              and stands at 2^6: small weights are in the normal range down to 2^-20 of the largest, large
+//              ones reach 2^15.
 //   producers  2 or 4: the item's queries, then per tile of KT keys the rope columns and kv / 128 pairs
 //              of 64-column boxes (each pair its own warps) into rings of swizzled boxes. 16-bit caches come
 //              by TMA (where the encoder does not take the strides: by 16-byte cp.async); e4m3 codes
@@ -90,6 +94,7 @@ constexpr int kTcMaxPlan = 512;   // entries of the shared plan (the items of ru
 constexpr int kTcTable = 32;      // items per shared table
 constexpr int kMinSpan = 4;       // tiles of a CTA's share at least
 constexpr int kMaxJoin = 4;       // prefix ranges a suffix launch joins itself
+constexpr float kGrowth = 8.f;    // log2 of what a weight may grow over its reference
 constexpr float kNoMax = -1e37f;  // running maximum before any key (finite: its exp2 is 0, never NaN)
 
 // One work item.
@@ -152,6 +157,12 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int kSmem = oBar + kBars * 8 + 16 + 1024;  // + alignment of the base
     static_assert(kCtas * (kSmem + 1024) <= 228 * 1024 && kCols * kCtas <= 512, "shared and tensor memory");
 };
+
+// floor(log2 |s|) of an e4m3 key's scale, kept within what the weights' range needs: below 2^-40 a value is
+// less than fp16 (and its share of a bf16 row) can show, above 2^100 probabilities would leave fp32.
+__device__ __forceinline__ float scale_exponent(float s) {
+    return static_cast<float>(min(max(static_cast<int>((__float_as_uint(s) >> 23) & 255) - 127, -40), 100));
+}
 
 // Swizzled byte offset of 16-byte chunk c of row r in a box of 128-, 64- or 32-byte rows.
 __device__ __forceinline__ uint32_t sw128(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
@@ -900,6 +911,8 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         const float cs = p.scale * 1.4426950408889634f;
         const long long rows = static_cast<long long>(p.B) * th;
         const float* m_c = m_s + c0;
+        // log2 of the largest weight when its reference is taken
+        constexpr float kLift = kBf16 ? 0.f : 6.f;
         int tile = 0, item = 0;
         Ring<2> eb;
         for (int base = 0; base < mine; base += kTcTable) {
@@ -979,20 +992,21 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     }
 #pragma unroll
                     for (int n = 0; n < NC; ++n) top = fmaxf(top, z[n]);
-                    over |= top > 8.f;
+                    if (Q8) top += scale_exponent(ks);
+                    over |= top > kLift + kGrowth;
                     if (soft_any(group, over)) {
                         float x[NC];
 #pragma unroll
-                        for (int n = 0; n < NC; ++n) x[n] = z[n];
+                        for (int n = 0; n < NC; ++n) x[n] = Q8 ? z[n] + scale_exponent(ks) : z[n];
                         const int own = fold_columns(x, lane, [](float u, float w) { return fmaxf(u, w); });
                         if (NC == 32 || (lane & 1) == 0) red_s[gw * N + c0 + own] = x[0];
                         soft_sync(group);
                         if (gt < NC) {
                             // every column that sees a key of the item sees one in its first tile: there
-                            // the reference becomes the tile's maximum, later it moves only by more than 8
+                            // the reference becomes the tile's maximum, later it moves only by more than the growth
                             const int n = c0 + gt;
                             float up = fmaxf(fmaxf(red_s[n], red_s[N + n]), fmaxf(red_s[2 * N + n], red_s[3 * N + n]));
-                            if (j == 0 ? up == -INFINITY : !(up > 8.f)) up = 0.f;
+                            up = (j == 0 ? up == -INFINITY : !(up > kLift + kGrowth)) ? 0.f : up - kLift;
                             corr_s[n] = fast_exp2(-up);
                             up_s[n] = up;
                             m_s[n] += up;

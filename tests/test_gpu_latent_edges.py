@@ -13,12 +13,69 @@ FORMS = [(128, 16, 8, 1), (512, 32, 5, 3), (128, 16, 8, 9), (512, 32, 16, 5), (4
 TENSOR_CORE = FORMS[:4]
 
 
+def stored(torch, x, kv, dtype, fp8):
+    """Rows x as a cache: (what the call takes, its values in 64 bits, one unit per position): 16-bit values
+    have the unit 1, codes their scale."""
+    if not fp8:
+        c = x.to(dtype)
+        return c, c.double(), torch.ones(x.shape[:2], dtype=torch.float64, device="cuda")
+    s = (x[..., :kv].float().abs().amax(-1) / 448).clamp_min(2.0 ** -100)
+    codes = (x[..., :kv].float() / s[..., None]).to(torch.float8_e4m3fn)
+    rk = x[..., kv:].to(dtype)
+    return (codes, rk, s), torch.cat([codes.float().double() * s.double()[..., None], rk.double()], -1), s.double()
+
+
 def run(torch, latent, q, pre, suf, starts, plen, slen, kv, scale):
     i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
     return latent.shared_prefix_attention(
         q, pre, suf, i32(starts) if pre is not None else None, i32(plen) if pre is not None else None,
         i32(slen) if suf is not None else None, scale, kv_rank=kv, return_lse=True)
 
+
+def bound(torch, q, pre, suf, starts, plen, slen, kv, scale, fp8):
+    """(out, lse, tolerance of out, tolerance of lse) of the definition. The tolerance of a result counts
+    - two roundings of weights and results to 16 bits, relative 2^-11 (fp16) or 2^-8 (bf16) each,
+    - the scores' fp32 sums of W products in steps of 16, 2^-23 of their magnitude each, as a change of the
+      weights (twice: above and below the line),
+    - fp16 weights below its normal range: they are held relative to the largest weight of a part, which is
+      stored as 2^6 or more, so each is off by at most 2^-25 / 2^6 of that one,
+    - an fp16 result below the normal range: 2^-25."""
+    values = lambda c: None if c is None else c[1]  # noqa: E731
+    want, lse, size, mag = reference(torch, q, values(pre), values(suf), starts, plen, slen, scale, kv)
+    half = q.dtype == torch.float16
+    u = 2.0 ** -11 if half else 2.0 ** -8
+    es = (q.shape[-1] / 16 + 2) * 2.0 ** -23 * mag
+    tol = size * (2 * u + 2 * es[..., None]) + 1e-30
+    if half:
+        # weights are probabilities times the positions' units
+        top = torch.zeros_like(lse)
+        for (_, v, unit), lens, row in ((pre, plen, False), (suf, slen, True)):
+            for b in range(q.shape[0]):
+                g = b if row else max([i for i in range(len(starts) - 1) if starts[i] <= b < starts[i + 1]], default=-1)
+                if g < 0 or lens[g] <= 0:
+                    continue
+                k = v[g, :lens[g]]
+                p = torch.exp(torch.einsum("thw,kw->thk", q[b].double(), k) * scale - lse[b][..., None]).clamp_max(1)
+                top[b] = torch.maximum(top[b], torch.nan_to_num((p * unit[g, :lens[g]]).amax(-1)))
+        keys = max(plen, default=0) + max(slen, default=0)
+        code = 448.0 if fp8 else max([c[1][..., :kv].abs().amax().item() for c in (pre, suf)])
+        tol = tol + keys * code * top[..., None] * 2.0 ** -31 + 2.0 ** -25
+    keys = max(plen, default=0) + max(slen, default=0)
+    return want, lse, tol, es + keys * 2.0 ** -24 + 2.0 ** -20 * (1 + lse.abs())
+
+
+def agree(torch, got, want, where=None):
+    out, lse = got
+    wo, wl, to, tl = want
+    where = torch.ones_like(wl, dtype=torch.bool) if where is None else where
+    err = (out.double() - wo).abs() / to
+    # a result past the type's largest value is its infinity
+    most = torch.finfo(out.dtype).max
+    past = torch.isinf(out) & (out.double().sign() == wo.sign()) & (wo.abs() + to >= most)
+    err = torch.where(past, 0.0, err)[where]
+    assert torch.all(err <= 1), float(torch.nan_to_num(err, nan=1e9).max())
+    el = (lse.double() - wl)[where].abs()
+    assert torch.all(el <= tl[where]), float((el / tl[where]).max())
 
 def test_no_wait_ran_out():
     """The device's note of waits that ran out stays empty over calls of every form, and can be read on
@@ -34,3 +91,55 @@ def test_no_wait_ran_out():
             latent.check_status()
     with torch.cuda.stream(torch.cuda.Stream()):
         latent.check_status("cuda")
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("dtype,rms", [("float16", 1.0), ("float16", 1e-2), ("float16", 1e-3), ("float16", 1e-5),
+                                       ("float16", 3e4), ("float16", "mixed"), ("bfloat16", 1e-20), ("bfloat16", 1e-3),
+                                       ("bfloat16", 1e10), ("bfloat16", "mixed")])
+def test_8_bit_values_of_any_size(form, dtype, rms):
+    """An e4m3 cache's values are codes times any scale: small ones, large ones, and both side by side."""
+    torch, latent = mods()
+    kv, rope, H, T = form
+    dtype = getattr(torch, dtype)
+    g = torch.Generator(device="cuda").manual_seed(31)
+    starts, plen, slen = [0, 2, 3], [700, 130], [40, 300, 9]
+    if rms == "mixed":
+        size = lambda *s: 10.0 ** (-5 * torch.rand(*s, 1, generator=g, device="cuda"))  # noqa: E731
+    else:
+        size = lambda *s: torch.full((*s, 1), rms, device="cuda")  # noqa: E731
+
+    def cache(lens):
+        s = (len(lens), max(lens))
+        x = torch.randn(*s, kv + rope, generator=g, device="cuda")
+        x[..., :kv] = (x[..., :kv] + 0.25) * size(*s)  # a mean that the average does not lose
+        return stored(torch, x, kv, dtype, True)
+
+    pre, suf = cache(plen), cache(slen)
+    q = torch.randn(3, T, H, kv + rope, generator=g, device="cuda")
+    q[..., :kv] *= min(1.0 if rms == "mixed" else 1 / rms, 10.0)
+    q = q.to(dtype)
+    args = (starts, plen, slen, kv, 0.08)
+    agree(torch, run(torch, latent, q, pre[0], suf[0], *args), bound(torch, q, pre, suf, *args, True))
+
+
+@pytest.mark.parametrize("form", TENSOR_CORE, ids=str)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("nats", [8, 15])
+def test_many_weak_keys_beside_a_dominant_one(form, fp8, nats):
+    """One position without a value takes nearly all of the weight: the result is what thousands of others,
+    each of little weight, add up to."""
+    torch, latent = mods()
+    kv, rope, H, T = form
+    g = torch.Generator(device="cuda").manual_seed(32)
+    n, scale = 9000, 0.125
+    x = 0.01 * (1 + 0.3 * torch.randn(1, n, kv + rope, generator=g, device="cuda"))
+    x[..., kv:] = 0
+    x[0, 5, :kv] = 0
+    x[0, 5, kv] = nats / scale
+    pre = stored(torch, x, kv, torch.float16, fp8)
+    suf = stored(torch, x[:, :20].expand(2, 20, kv + rope).contiguous(), kv, torch.float16, fp8)
+    q = torch.zeros(2, T, H, kv + rope, device="cuda").half()
+    q[..., kv] = 1
+    args = ([0, 2], [n], [0, 20], kv, scale)
+    agree(torch, run(torch, latent, q, pre[0], suf[0], *args), bound(torch, q, pre, suf, *args, fp8))
