@@ -334,7 +334,7 @@ bool cache_map(CUtensorMap* map, const mm::lat::CacheView& c, int width, int dty
                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int KV, int R, int N, typename T, bool Q8>
+template <int KV, int R, int N, typename T, bool Q8, bool CAUSAL>
 void launch_tc(mm::spa::TcArgs a, long long items, cudaStream_t s) {
     using C = mm::spa::TcCfg<KV, R, N, Q8>;
     CUtensorMap tile{}, block{}, rope{};
@@ -345,15 +345,23 @@ void launch_tc(mm::spa::TcArgs a, long long items, cudaStream_t s) {
                 cache_map(&block, c, KV + R, dtype, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B) &&
                 cache_map(&rope, c, KV + R, dtype, R, 32, R == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
     }
-    set_dynamic_smem<mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8>>(C::kSmem);
-    launch(s, mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8>,
+    set_dynamic_smem<mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8, CAUSAL>>(C::kSmem);
+    launch(s, mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8, CAUSAL>,
            dim3(static_cast<unsigned>(std::min<long long>(items, sm_count() * C::kCtas))), dim3(C::kThreads), C::kSmem, a,
            tile, block, rope);
 }
 template <int KV, int R, typename T>
 void launch_tc_n(const mm::spa::TcArgs& a, int n, bool q8, long long items, cudaStream_t s) {
-    if (n == 16) q8 ? launch_tc<KV, R, 16, T, true>(a, items, s) : launch_tc<KV, R, 16, T, false>(a, items, s);
-    else q8 ? launch_tc<KV, R, 64, T, true>(a, items, s) : launch_tc<KV, R, 64, T, false>(a, items, s);
+    auto go = [&](auto size, auto codes) {
+        constexpr int N = decltype(size)::value;
+        constexpr bool Q8 = decltype(codes)::value;
+        if (a.suffix && a.p.T > 1) launch_tc<KV, R, N, T, Q8, true>(a, items, s);
+        else launch_tc<KV, R, N, T, Q8, false>(a, items, s);
+    };
+    using N16 = std::integral_constant<int, 16>;
+    using N64 = std::integral_constant<int, 64>;
+    if (n == 16) q8 ? go(N16{}, std::true_type{}) : go(N16{}, std::false_type{});
+    else q8 ? go(N64{}, std::true_type{}) : go(N64{}, std::false_type{});
 }
 
 template <int KV, int R, typename T>

@@ -32,7 +32,8 @@
 //              cache holds past the range is masked in S and never read by an O product.
 //   fence      one warp passes each landed tile on to the asynchronous proxy: a proxy fence costs
 //              about 100 ns, and in the loading threads it would wait for every load they have in
-//              flight (measured: 1.7 instead of over 5 TB/s).
+//              flight (measured: 1.7 instead of over 5 TB/s). It also takes a NaN or an infinity out of the
+//              value rows that some tokens of a block see and others do not (drop_bad_rows).
 //   results    4 (N = 16): an item's O^T and sums, joined with the prefix's share, to memory.
 //   MMA        one thread issues tcgen05.mma. With KT = 64 the S^T product has M = 64, whose row r
 //              is tensor-memory lane 32 (r / 16) + r % 16.
@@ -273,6 +274,9 @@ __device__ __forceinline__ int direct_join(const Problem& p, int b, int suffix_k
     return np <= kMaxJoin ? np : -1;
 }
 
+// Keys of a row's suffix of `len` that its query row u (< T * H) sees.
+__device__ __forceinline__ int seen_by(const Problem& p, int len, int u) { return max(len - (p.T - 1 - u / p.H), 0); }
+
 // A launch's items come from units: groups (prefix) or rows (suffix). Unit u holds `blocks` blocks of
 // N query rows from q0 on and attends over `len` keys in `ranges` key ranges (a suffix row of a
 // direct result keeps one, however empty).
@@ -308,7 +312,7 @@ template <int N> __device__ __forceinline__ int unit_items(const TcArgs& a, int 
 // Item idx of the launch. With a plan (shared: cumulative items of runs of `step` units) the items are
 // dense, so that they spread evenly over the CTAs whatever the lengths; without one (a suffix launch
 // of one range per row, where there is none to skip) every unit has `per` blocks.
-template <int N, int KT>
+template <int N, int KT, bool CAUSAL>
 __device__ __forceinline__ Item get_item(const TcArgs& a, const int* plan, int units, int step, int per, int idx) {
     int u, local;
     if (plan) {
@@ -338,7 +342,10 @@ __device__ __forceinline__ Item get_item(const TcArgs& a, const int* plan, int u
     it.q0 = r.q0 + block * N;
     it.nq = max(0, min(N, r.nq - block * N));
     it.k0 = it.split * a.kps;
-    it.nk = it.nq > 0 ? max(0, min(a.kps, r.len - it.k0)) : 0;
+    // a block ends at the last key that its last query sees (16-query blocks hold a row's last token)
+    int len = r.len;
+    if (N == 64 && CAUSAL && it.nq > 0) len = seen_by(a.p, len, block * N + it.nq - 1);
+    it.nk = it.nq > 0 ? max(0, min(a.kps, len - it.k0)) : 0;
     it.nt = (it.nk + KT - 1) / KT;
     it.np = it.split == 0 ? r.np : -1;
     return it;
@@ -427,7 +434,35 @@ struct Cursor {
     }
 };
 
-template <int KV, int R, int N, typename T, bool Q8>
+// Value rows [from, to) of a landed tile are seen by some of the block's queries and masked for others, and a
+// probability of zero times a NaN or an infinity is a NaN: a row that holds one becomes zeros, with a NaN in
+// its rope columns, which only the scores read. So the queries that see it get NaN, and no other.
+template <class C, int R, bool kBf16>
+__device__ __noinline__ void drop_bad_rows(uint8_t* pairs, int first_pair, uint8_t* rope, int from, int to, int lane) {
+    constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
+    auto chunk = [&](int r, int e) {  // 16-byte chunk e of row r
+        int pair = first_pair + (e >> 4);
+        if (pair >= C::PS) pair -= C::PS;
+        return reinterpret_cast<uint4*>(pairs + pair * C::kPair + ((e >> 3) & 1) * C::kBox + sw128(r, e & 7));
+    };
+    for (int r = from; r < to; ++r) {
+        bool bad = false;
+        for (int e = lane; e < 16 * C::NP; e += 32) {
+            const uint4 v = *chunk(r, e);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bad |= (w[i] & kExp) == kExp || (w[i] >> 16 & kExp) == kExp;
+        }
+        if (!__any_sync(0xffffffffu, bad)) continue;
+        for (int e = lane; e < 16 * C::NP; e += 32) *chunk(r, e) = make_uint4(0, 0, 0, 0);
+        if (lane < R / 8) *reinterpret_cast<uint4*>(rope + sw_rope<R>(r, lane)) = make_uint4(~0u, ~0u, ~0u, ~0u);
+    }
+}
+
+// CAUSAL: a suffix launch of more than one token a row, whose last positions are masked for some of them. A
+// kernel of its own, because the other launches pay for code that they do not run (2,048 rows, 128 + 16 wide:
+// 62.6 us, in one kernel with it 64.0).
+template <int KV, int R, int N, typename T, bool Q8, bool CAUSAL>
 __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N, Q8>::kCtas)
     shared_prefix_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap map_tile,
                             const __grid_constant__ CUtensorMap map_block, const __grid_constant__ CUtensorMap map_rope) {
@@ -581,7 +616,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 if (kShares && spans) {
                     table[tid] = span_item<KT>(a, plan, step, span, plan_s[kTcMaxPlan + 1] + base + tid);
                 } else {
-                    const Item it = get_item<N, KT>(a, plan, units, step, per, blockIdx.x + (base + tid) * gridDim.x);
+                    const Item it = get_item<N, KT, CAUSAL>(a, plan, units, step, per, blockIdx.x + (base + tid) * gridDim.x);
                     table[tid] = it;
                     if (kShares && a.pieces) a.pieces[it.row] = make_int2(0, 0);
                 }
@@ -847,6 +882,8 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         };
         Ring<C::TS> ft;
         Ring<C::PS> fp;
+        Ring<C::RS> fr;
+        int shown = 0;  // keys of the item that all of its queries see
         for (int base = 0; base < mine; base += kTcTable) {
             const int count = next_table(base, std::false_type());
             if (warp == kFenceWarp) {
@@ -855,6 +892,10 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 // that the O products still read are cleared first (a probability of zero times a NaN
                 // would be one).
                 for (Cursor c(table, count); c.valid(); c.next(), ft.next()) {
+                    if (CAUSAL && c.j == 0) {
+                        const Item& it = c.item();
+                        shown = seen_by(p, suffix_length(p, it.row), it.q0 - it.row * th) - it.k0;
+                    }
                     wait(&tile_in[ft.i], ft.phase);
                     const int left = c.item().nk - c.j * KT;
                     if (!Q8 && a.tma && left < KT && (left & 15)) {
@@ -868,6 +909,13 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                             for (int e = lane; e < rows * 8; e += 32) box[e] = zero;
                             if (i & 1) z.next();
                         }
+                    }
+                    if constexpr (CAUSAL) {
+                        const int from = shown - c.j * KT, to = min(left, KT);
+                        __syncwarp();
+                        if (from < to)
+                            drop_bad_rows<C, R, kBf16>(smem + C::oPair, fp.i, smem + C::oRope + fr.i * C::kRopeA, max(from, 0), to, lane);
+                        fr.next();
                     }
                     fp.skip(C::NP);
                     fence_proxy_async_smem();
@@ -925,23 +973,25 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
 #pragma unroll
                 for (int n = 0; n < NC; ++n) l[n] = 0.f;
                 // keys of the item each query sees; the tokens of a suffix end one position apart
-                const bool causal = a.suffix && p.T > 1;
                 soft_sync(group);  // the previous item's readers of m_s, lim_s and red_s are done
                 if (gt < NC) {
                     m_s[c0 + gt] = 0.f;
-                    if (causal) {
+                    if (CAUSAL) {
                         const int t = min((it.q0 + c0 + gt - it.row * th) / p.H, p.T - 1);
                         lim_s[c0 + gt] = min(it.nk, suffix_length(p, it.row) - (p.T - 1 - t) - it.k0);
                     }
                 }
                 soft_sync(group);
-                const int lim_min = causal ? it.nk - (p.T - 1) : it.nk;
+                const int u0 = it.q0 - it.row * th;  // the tokens of the block end at most this far apart
+                const int lim_min = CAUSAL ? it.nk - ((u0 + it.nq - 1) / p.H - u0 / p.H) : it.nk;
                 const float* ks_row = Q8 ? cv.scale + it.row * cv.scale_row_stride + it.k0 : nullptr;
                 float ks_next = 1.f;
                 if (Q8 && live && kt < it.nk) ks_next = __ldg(ks_row + kt);
                 for (int j = 0; j < it.nt; ++j, ++tile) {
                     const int key = j * KT + kt;
-                    const float ks = ks_next;
+                    // an infinite scale is no number either (it would be one for scores of one sign)
+                    const float ks = !Q8 || fabsf(ks_next) <= 3.402823466e38f ? ks_next : __int_as_float(0x7fc00000);
+                    const float kw = ks == ks ? ks : 1.f;  // a masked probability of zero stays zero
                     if (Q8) ks_next = live && key + KT < it.nk ? __ldg(ks_row + key + KT) : 1.f;
                     const int sb = tile & 1;
                     wait(&s_full[sb], (tile >> 1) & 1);
@@ -977,7 +1027,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                         z[n + 3] = fmaf(z[n + 3], cs, -m.w);
                     }
                     if ((j + 1) * KT > lim_min) {  // the last tile(s): keys past a query's limit
-                        if (causal) {
+                        if (CAUSAL) {
 #pragma unroll
                             for (int n = 0; n < NC; ++n)
                                 if (key >= lim_s[c0 + n]) z[n] = -INFINITY;
@@ -1047,7 +1097,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                             for (int q = 0; q < 8; ++q) {
                                 e[q] = fast_exp2(z[n0 + q]);
                                 l[n0 + q] += e[q];
-                                if (Q8) e[q] *= ks;
+                                if (Q8) e[q] *= kw;
                             }
                             if constexpr (N == 64) {
                                 *reinterpret_cast<uint4*>(P + sw128(kt, (c0 + n0) >> 3)) =
@@ -1255,7 +1305,12 @@ __global__ void __launch_bounds__(256) shared_prefix_join_kernel(const Problem p
         ns = v.y;
     } else {
         if (direct && direct_join(p, b, suf_kps, pre_kps) >= 0) return;  // the suffix launch wrote it
-        ns = (suffix_length(p, b) + suf_kps - 1) / suf_kps;
+        int len = suffix_length(p, b);
+        if (!direct) {  // blocks of 64 queries end where their last one does
+            const int u = static_cast<int>(r - static_cast<long long>(b) * th);
+            len = seen_by(p, len, min((u / 64 + 1) * 64, th) - 1);
+        }
+        ns = (len + suf_kps - 1) / suf_kps;
     }
     const int g = p.G > 0 ? group_of(p, b) : -1;
     const int np = (prefix_length(p, g) + pre_kps - 1) / pre_kps;

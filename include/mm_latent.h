@@ -83,6 +83,8 @@ int mm_latent_cache_read(const mm_latent_cache* cache, const int64_t* slots, int
  * [0, suffix_len[b] - (tokens - 1 - t)). With K the concatenation of both,
  *   s = scale * q . K_j,  out = sum_j softmax(s)_j K_j[0, kv),  lse = ln sum_j e^s
  * and a query that sees no position gets out = 0, lse = -infinity.
+ * A latent NaN or infinity, or a scale that is one, makes the results of the queries that see its
+ * position not finite, and no other's.
  * Lengths are clamped to [0, max_prefix] and [0, max_suffix]; max_* are host-side bounds
  * (<= the caches' positions) that size the launch, as is max_group (rows of the largest group;
  * larger groups leave their further rows without the prefix).

@@ -143,3 +143,92 @@ def test_many_weak_keys_beside_a_dominant_one(form, fp8, nats):
     q[..., kv] = 1
     args = ([0, 2], [n], [0, 20], kv, scale)
     agree(torch, run(torch, latent, q, pre[0], suf[0], *args), bound(torch, q, pre, suf, *args, fp8))
+
+
+BAD = {False: ["latent nan", "latent inf", "latent -inf", "rope nan"],
+       True: ["latent nan", "rope nan", "scale nan", "scale inf"]}
+
+
+@pytest.mark.parametrize("form", [f for f in FORMS if f[3] > 1] + [(128, 16, 3, 4), (512, 32, 1, 9), (128, 16, 64, 2)], ids=str)
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("bad", [(k, b) for k in BAD for b in BAD[k]], ids=str)
+def test_a_bad_position_reaches_the_tokens_that_see_it_alone(form, dtype, bad):
+    """A later token's own position holds a NaN or an infinity: the tokens before it do not notice."""
+    torch, latent = mods()
+    kv, rope, H, T = form
+    fp8, what = bad
+    dtype = getattr(torch, dtype)
+    g = torch.Generator(device="cuda").manual_seed(34)
+    # last positions inside a tile, across tiles of 64 and 128 and across key ranges, and nothing but them
+    slen = [50, 66, 130, 129, 385, 700, T, 258, 257, 50]
+    back = [(3 * b) % T for b in range(len(slen))]
+    back[0], back[1], back[-1] = 0, T - 1, None  # how many positions from the last; the last row is sound
+    starts, plen = [0, 7], [90]
+    pre = make_cache(torch, g, plen, 90, kv, rope, dtype, fp8)
+    suf = make_cache(torch, g, slen, max(slen), kv, rope, dtype, fp8)
+    q = torch.randn(len(slen), T, H, kv + rope, generator=g, device="cuda").to(dtype)
+    clean = (suf[0] if not fp8 else None, suf[1].clone(), None)
+    raw = suf[0] if not fp8 else tuple(t.clone() for t in suf[0])
+    raw = raw.clone() if not fp8 else raw
+    sees = torch.zeros(len(slen), T, dtype=torch.bool, device="cuda")
+    for b, d in enumerate(back):
+        if d is None:
+            continue
+        j = slen[b] - 1 - d
+        sees[b, T - 1 - d:] = True
+        value = {"nan": NAN, "inf": float("inf"), "-inf": float("-inf")}[what.split()[1]]
+        if what.startswith("scale"):
+            raw[2][b, j] = value
+        elif what.startswith("rope"):
+            (raw[1][b, j] if fp8 else raw[b, j, kv:])[rope // 2] = value
+        elif fp8:
+            raw[0].view(torch.uint8)[b, j, kv // 3] = 0x7F
+        else:
+            raw[b, j, kv // 3] = value
+    out, lse = run(torch, latent, q, pre[0], raw, starts, plen, slen, kv, 0.11)
+    want, wl, size, mag = reference(torch, q, pre[1], clean[1], starts, plen, slen, 0.11, kv)
+    u = 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -8
+    es = (q.shape[-1] / 16 + 2) * 2.0 ** -23 * mag
+    ok = ~sees[..., None].expand(-1, -1, H)
+    # fp16 weights: at most 2^-25 of 2^6 off each, for at most 800 values of up to 6
+    tol = size * (3 * u + 2 * es[..., None]) + 800 * 6 * 2.0 ** -31 + 1e-7
+    assert torch.isfinite(out[ok]).all() and torch.isfinite(lse[ok]).all()
+    assert torch.all(((out.double() - want).abs() <= tol)[ok])
+    assert torch.all(((lse.double() - wl).abs() <= es + 800 * 2.0 ** -24 + 2.0 ** -20 * (1 + wl.abs()))[ok])
+    # who sees it has a NaN in its result
+    assert torch.isnan(out[~ok]).any(-1).all()
+
+
+@pytest.mark.parametrize("form", [(128, 16, 8), (512, 32, 16), (512, 32, 5), (128, 16, 1), (40, 6, 2)], ids=str)
+@pytest.mark.parametrize("kind", ["fp16", "bf16", "fp8/fp16"])
+@pytest.mark.parametrize("tokens", [70, 333])
+def test_every_position_of_a_prompt_is_a_query(form, kind, tokens):
+    """The prompt form: rows of different lengths whose positions are their own query tokens, aligned at the
+    end (a short row's first tokens see nothing), one of them with a NaN inside."""
+    torch, latent = mods()
+    kv, rope, H = form
+    dtype = torch.bfloat16 if "bf16" in kind else torch.float16
+    fp8 = "fp8" in kind
+    g = torch.Generator(device="cuda").manual_seed(35)
+    slen = [tokens, 1, tokens // 2 + 3, 0, tokens]
+    suf = make_cache(torch, g, slen, tokens, kv, rope, dtype, fp8)
+    q = torch.randn(len(slen), tokens, H, kv + rope, generator=g, device="cuda").to(dtype)
+    at = tokens // 2 + 2  # the last row's bad position
+    values = suf[1].clone()
+    if fp8:
+        suf[0][0].view(torch.uint8)[4, at, 3] = 0x7F
+    else:
+        suf[0][4, at, 3] = NAN
+        values[4, at, 3] = 0
+    out, lse = run(torch, latent, q, None, suf[0], [0], [], slen, kv, 0.11)
+    want, wl, size, mag = reference(torch, q, None, values, [0], [], slen, 0.11, kv)
+    u = 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -8
+    es = (q.shape[-1] / 16 + 2) * 2.0 ** -23 * mag
+    tol = size * (3 * u + 2 * es[..., None]) + tokens * 6 * 2.0 ** -31 + 1e-7
+    ok = torch.ones_like(wl, dtype=torch.bool)
+    ok[4, at:] = False
+    seen = torch.isfinite(wl)
+    assert torch.all(out[~seen] == 0) and torch.all(lse[~seen] == float("-inf"))
+    assert torch.all(((out.double() - want).abs() <= tol)[ok])
+    assert torch.all(((lse.double() - wl).abs() <= es + tokens * 2.0 ** -24 + 2.0 ** -20 * (1 + wl.abs()))[ok & seen])
+    assert torch.isnan(out[~ok]).all()
