@@ -18,7 +18,9 @@
 //              (tensor-memory lane). The running maximum is lazy: the first tile's maximum is the
 //              reference, and a later tile whose weights stay below 2^8 times the largest of the first
 //              uses it as it is, decided by one 4-warp vote; otherwise the column maxima are taken and
-//              O^T and the sums are rescaled. A key's scale (e4m3) multiplies its latent scores and,
+//              O^T and the sums are rescaled. Behind a reference of large magnitude (keys that are masked
+//              by the lowest score) every tile looks at its maxima again, from its scores as they are.
+//              A key's scale (e4m3) multiplies its latent scores and,
 //              for the second product, its probabilities.
 //              The second product takes the weights (probability, times the scale) as 16-bit values, each
 //              rounded once, as the tensor cores' operand has to be; sums and statistics are fp32. So that
@@ -96,7 +98,8 @@ constexpr int kTcTable = 32;      // items per shared table
 constexpr int kMinSpan = 4;       // tiles of a CTA's share at least
 constexpr int kMaxJoin = 4;       // prefix ranges a suffix launch joins itself
 constexpr float kGrowth = 8.f;    // log2 of what a weight may grow over its reference
-constexpr float kNoMax = -1e37f;  // running maximum before any key (finite: its exp2 is 0, never NaN)
+constexpr float kNear = 512.f;    // references up to here are subtracted with the scale's product
+constexpr float kNoMax = -3.402823466e38f;  // running maximum before any key (finite: its exp2 is 0, never NaN)
 
 // One work item.
 struct Item {
@@ -150,8 +153,8 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int oRope = oQ + QB * kQA;
     static constexpr int oP = oRope + RS * kRopeA;
     static constexpr int oTab = oP + PB * kP;
-    static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N], up[N], mail[2][5][N], factor[5][N]
-    static constexpr int oPlan = oF + (8 + (EW ? 15 : 0)) * N * 4;
+    static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N], up[N], base[N], mail[2][5][N], factor[5][N]
+    static constexpr int oPlan = oF + (9 + (EW ? 15 : 0)) * N * 4;
     static constexpr int oBar = oPlan + (kTcMaxPlan + 1) * 4 + 12;
     static constexpr int kBars = QB + PS + 2 * TS + 4 + 2 * PB + 2 * OB + 4 + 1;
     static_assert(RS * NP >= PS && TS * NP >= PS, "the rope ring and the tile barriers outlast the pair ring");
@@ -478,7 +481,8 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     float* red_s = corr_s + N;  // [4][N]
     int* lim_s = reinterpret_cast<int*>(red_s + 4 * N);
     float* up_s = red_s + 5 * N;
-    float* mail_s = up_s + N;        // [2][5][N] an item's sums (one row per softmax warp) and maxima
+    float* base_s = up_s + N;        // the part of m that a tile's scores start from
+    float* mail_s = base_s + N;      // [2][5][N] an item's sums (one row per softmax warp) and maxima
     float* fac_s = mail_s + 10 * N;  // [5][N]
     int* plan_s = reinterpret_cast<int*>(smem + C::oPlan);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::oBar);
@@ -958,7 +962,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(gw * 32) << 16);
         const float cs = p.scale * 1.4426950408889634f;
         const long long rows = static_cast<long long>(p.B) * th;
-        const float* m_c = m_s + c0;
+        const float* base_c = base_s + c0;
         // log2 of the largest weight when its reference is taken
         constexpr float kLift = kBf16 ? 0.f : 6.f;
         int tile = 0, item = 0;
@@ -975,7 +979,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 // keys of the item each query sees; the tokens of a suffix end one position apart
                 soft_sync(group);  // the previous item's readers of m_s, lim_s and red_s are done
                 if (gt < NC) {
-                    m_s[c0 + gt] = 0.f;
+                    m_s[c0 + gt] = base_s[c0 + gt] = 0.f;
                     if (CAUSAL) {
                         const int t = min((it.q0 + c0 + gt - it.row * th) / p.H, p.T - 1);
                         lim_s[c0 + gt] = min(it.nk, suffix_length(p, it.row) - (p.T - 1 - t) - it.k0);
@@ -985,6 +989,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 const int u0 = it.q0 - it.row * th;  // the tokens of the block end at most this far apart
                 const int lim_min = CAUSAL ? it.nk - ((u0 + it.nq - 1) / p.H - u0 / p.H) : it.nk;
                 const float* ks_row = Q8 ? cv.scale + it.row * cv.scale_row_stride + it.k0 : nullptr;
+                bool far = false;  // a column's reference is not its base
                 float ks_next = 1.f;
                 if (Q8 && live && kt < it.nk) ks_next = __ldg(ks_row + kt);
                 for (int j = 0; j < it.nt; ++j, ++tile) {
@@ -1016,11 +1021,11 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s_free[sb]);
                     // scores relative to the column's reference, base 2; the first tile's reference is 0
-                    bool over = j == 0;
+                    bool over = j == 0 || far;
                     float top = -INFINITY;
 #pragma unroll
                     for (int n = 0; n < NC; n += 4) {
-                        const float4 m = *reinterpret_cast<const float4*>(m_c + n);
+                        const float4 m = *reinterpret_cast<const float4*>(base_c + n);
                         z[n] = fmaf(z[n], cs, -m.x);
                         z[n + 1] = fmaf(z[n + 1], cs, -m.y);
                         z[n + 2] = fmaf(z[n + 2], cs, -m.z);
@@ -1053,15 +1058,22 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                         soft_sync(group);
                         if (gt < NC) {
                             // every column that sees a key of the item sees one in its first tile: there
-                            // the reference becomes the tile's maximum, later it moves only by more than the growth
+                            // the reference becomes the tile's maximum, later it moves only by more than the
+                            // growth. A column whose keys so far score -infinity keeps kNoMax.
                             const int n = c0 + gt;
-                            float up = fmaxf(fmaxf(red_s[n], red_s[N + n]), fmaxf(red_s[2 * N + n], red_s[3 * N + n]));
-                            up = (j == 0 ? up == -INFINITY : !(up > kLift + kGrowth)) ? 0.f : up - kLift;
-                            corr_s[n] = fast_exp2(-up);
-                            up_s[n] = up;
-                            m_s[n] += up;
+                            const float top_n = fmaxf(fmaxf(red_s[n], red_s[N + n]), fmaxf(red_s[2 * N + n], red_s[3 * N + n]));
+                            const float old = m_s[n], from = base_s[n];
+                            float m = old;
+                            if (j == 0 ? top_n > -INFINITY : (from - old) + top_n > kLift + kGrowth) m = from + (top_n - kLift);
+                            else if (j == 0 && !(CAUSAL && lim_s[n] <= 0)) m = kNoMax;
+                            corr_s[n] = fast_exp2(old - m);
+                            up_s[n] = m - from;
+                            m_s[n] = m;
+                            // scores relative to a large reference (keys masked by the lowest value, say) would
+                            // lose the digits of what comes after it: from there on every tile starts from 0
+                            base_s[n] = fabsf(m) <= kNear ? m : 0.f;
                         }
-                        soft_sync(group);
+                        far = soft_any(group, gt < NC && !(fabsf(m_s[c0 + (gt & (NC - 1))]) <= kNear));
 #pragma unroll
                         for (int n = 0; n < NC; ++n) z[n] -= up_s[c0 + n];
                         if (j > 0) {

@@ -49,7 +49,10 @@ def bound(torch, q, pre, suf, starts, plen, slen, kv, scale, fp8):
     if half:
         # weights are probabilities times the positions' units
         top = torch.zeros_like(lse)
-        for (_, v, unit), lens, row in ((pre, plen, False), (suf, slen, True)):
+        for cache, lens, row in ((pre, plen, False), (suf, slen, True)):
+            if cache is None:
+                continue
+            _, v, unit = cache
             for b in range(q.shape[0]):
                 g = b if row else max([i for i in range(len(starts) - 1) if starts[i] <= b < starts[i + 1]], default=-1)
                 if g < 0 or lens[g] <= 0:
@@ -58,7 +61,7 @@ def bound(torch, q, pre, suf, starts, plen, slen, kv, scale, fp8):
                 p = torch.exp(torch.einsum("thw,kw->thk", q[b].double(), k) * scale - lse[b][..., None]).clamp_max(1)
                 top[b] = torch.maximum(top[b], torch.nan_to_num((p * unit[g, :lens[g]]).amax(-1)))
         keys = max(plen, default=0) + max(slen, default=0)
-        code = 448.0 if fp8 else max([c[1][..., :kv].abs().amax().item() for c in (pre, suf)])
+        code = 448.0 if fp8 else max(c[1][..., :kv].abs().amax().item() for c in (pre, suf) if c is not None)
         tol = tol + keys * code * top[..., None] * 2.0 ** -31 + 2.0 ** -25
     keys = max(plen, default=0) + max(slen, default=0)
     return want, lse, tol, es + keys * 2.0 ** -24 + 2.0 ** -20 * (1 + lse.abs())
@@ -143,6 +146,78 @@ def test_many_weak_keys_beside_a_dominant_one(form, fp8, nats):
     q[..., kv] = 1
     args = ([0, 2], [n], [0, 20], kv, scale)
     agree(torch, run(torch, latent, q, pre[0], suf[0], *args), bound(torch, q, pre, suf, *args, fp8))
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("low", ["lowest", "-inf"])
+def test_positions_masked_by_their_rope_key(form, dtype, fp8, low):
+    """Keys whose scores are the type's lowest value or minus infinity weigh nothing beside others, wherever
+    they lie; where all are lowest they weigh the same, where all are -infinity the sum is zero."""
+    torch, latent = mods()
+    kv, rope, H, T = form
+    dtype = getattr(torch, dtype)
+    g = torch.Generator(device="cuda").manual_seed(33)
+    bottom = float("-inf") if low == "-inf" else torch.finfo(dtype).min
+    x = torch.randn(1, 700, kv + rope, generator=g, device="cuda")
+    y = torch.randn(4, 300, kv + rope, generator=g, device="cuda")
+    x[..., kv], y[..., kv] = 0, 0
+    masked = torch.zeros(700, dtype=torch.bool, device="cuda")
+    masked[:300] = True      # the first tiles
+    masked[400:450] = True
+    q = torch.randn(4, T, H, kv + rope, generator=g, device="cuda").to(dtype)
+    q[..., kv] = 1.0
+    plen, slen, starts = [700], [300, 40, 0, 300], [0, 3]
+    kept = stored(torch, x[:, ~masked], kv, dtype, fp8)
+    x[0, masked, kv] = bottom
+    y[0, :290, kv] = bottom  # a row of one suffix range, masked but for its end
+    y[3, :, kv] = bottom     # a row without a prefix, masked altogether
+    pre, suf = stored(torch, x, kv, dtype, fp8), stored(torch, y, kv, dtype, fp8)
+    got = run(torch, latent, q, pre[0], suf[0], starts, plen, slen, kv, 0.1)
+    # row 0 keeps its last positions, of which its tokens see all but the last T - 1 - t
+    want = bound(torch, q, kept, tuple(t for t in stored(torch, y[:, 290:], kv, dtype, fp8)), starts,
+                 [int((~masked).sum())], [10, 0, 0, 0], kv, 0.1, fp8)
+    rows = torch.zeros(4, T, H, dtype=torch.bool, device="cuda")
+    rows[0] = True
+    agree(torch, got, want, rows)
+    want = bound(torch, q, kept, stored(torch, y[:, :40], kv, dtype, fp8), starts, [int((~masked).sum())], [0, 40, 0, 0], kv, 0.1, fp8)
+    rows[0], rows[1:3] = False, True
+    agree(torch, got, want, rows)
+    if low == "-inf":
+        assert torch.all(got[0][3] == 0) and torch.all(got[1][3] == float("-inf"))
+    else:
+        # the differences of such scores are below what fp32 (and the product's sums) resolve, or above what a
+        # weight can hold: a mean of the values, whatever the weights
+        assert torch.isfinite(got[0][3]).all() and torch.isfinite(got[1][3]).all()
+        top = suf[1][3, :, :kv].abs().amax()
+        assert torch.all(got[0][3].double().abs() <= top * (1 + 2.0 ** -6)) and torch.any(got[0][3] != 0)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("low", ["lowest", "-inf"])
+@pytest.mark.parametrize("level", [-400.0, 900.0])
+def test_scores_far_from_zero_beside_masked_ones(form, dtype, low, level):
+    """All scores that count lie far below or above zero, after key tiles that are masked altogether, in rows
+    that are not divided (there are more of them than multiprocessors)."""
+    torch, latent = mods()
+    kv, rope, H, T = form
+    dtype = getattr(torch, dtype)
+    g = torch.Generator(device="cuda").manual_seed(37)
+    B, n = 400, 600
+    x = 0.5 * torch.randn(B, n, kv + rope, generator=g, device="cuda")
+    x[..., kv], x[..., kv + 1] = 0, level
+    x[:, :290, kv] = float("-inf") if low == "-inf" else torch.finfo(dtype).min
+    suf = stored(torch, x, kv, dtype, False)
+    q = torch.randn(B, T, H, kv + rope, generator=g, device="cuda").to(dtype)
+    q[..., kv], q[..., kv + 1] = 1.0, 1.0
+    slen = [n - b % 3 for b in range(B)]
+    out, lse = run(torch, latent, q, None, suf[0], [0], [], slen, kv, 1.0)
+    rows = [0, 1, 2, B - 1]
+    kept = stored(torch, x[rows, 290:], kv, dtype, False)
+    agree(torch, (out[rows], lse[rows]),
+          bound(torch, q[rows], None, kept, [0], [], [slen[b] - 290 for b in rows], kv, 1.0, False))
 
 
 BAD = {False: ["latent nan", "latent inf", "latent -inf", "rope nan"],
