@@ -237,7 +237,10 @@ int sm_count() {
 // can be read in 16-byte pieces and the results written in 8-byte ones (the join kernel).
 bool aligned_cache(const mm_latent_cache* c) {
     if (c->kind == MM_E4M3) return aligned_e4m3(c);
-    return reinterpret_cast<uintptr_t>(c->latent) % 16 == 0 && c->row_stride % 8 == 0 && c->pos_stride % 8 == 0;
+    // 16-bit caches come by tensor maps: strides of up to 40 bits in bytes, rows that may be one and the same
+    constexpr int64_t kMost = 1LL << 39;
+    return multiple(c->latent, 16) && c->row_stride % 8 == 0 && c->pos_stride % 8 == 0 && c->pos_stride > 0 && c->pos_stride < kMost &&
+           c->row_stride >= 0 && c->row_stride < kMost;
 }
 bool tensor_core_form(const mm::spa::Problem& p, const mm_latent_cache* prefix, const mm_latent_cache* suffix) {
     if (!((p.kv == 128 && p.rd == 16) || (p.kv == 512 && p.rd == 32))) return false;
@@ -323,40 +326,48 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     return f;
 }
 
+// The tensor maps of a 16-bit cache: whole tiles, blocks of 32 positions, and their rope columns.
+struct Maps {
+    CUtensorMap tile{}, block{}, rope{};
+};
+
 // Boxes of `box` columns x `keys` positions of one cache row. False where the encoder does not take
-// the cache's strides; the kernel then copies row by row.
-bool cache_map(CUtensorMap* map, const mm::lat::CacheView& c, int width, int dtype, int box, int keys, CUtensorMapSwizzle swizzle) {
-    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(c.positions), static_cast<cuuint64_t>(c.rows)};
-    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(c.pos_stride) * 2, static_cast<cuuint64_t>(c.row_stride) * 2};
+// the cache's strides.
+bool cache_map(CUtensorMap* map, const mm_latent_cache* c, int box, int keys, CUtensorMapSwizzle swizzle) {
+    const bool rows = c->rows > 1 && c->row_stride > 0;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(c->kv + c->rope_dim), static_cast<cuuint64_t>(c->positions),
+                                static_cast<cuuint64_t>(rows ? c->rows : 1)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(c->pos_stride) * 2,
+                                   static_cast<cuuint64_t>(rows ? c->row_stride : c->pos_stride) * 2};
     const cuuint32_t boxes[3] = {static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(keys), 1}, steps[3] = {1, 1, 1};
-    return tensor_map_encoder()(map, dtype == MM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                                const_cast<uint8_t*>(c.latent), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+    return tensor_map_encoder()(map, c->kind == MM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                                c->latent, dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool cache_maps(Maps& m, const mm_latent_cache* c) {
+    if (c->kind == MM_E4M3) return true;  // read without maps
+    const int keys = c->kv == 512 ? mm::spa::TcCfg<512, 32, 16, false>::KT : mm::spa::TcCfg<128, 16, 16, false>::KT;
+    return cache_map(&m.tile, c, 64, keys, CU_TENSOR_MAP_SWIZZLE_128B) && cache_map(&m.block, c, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           cache_map(&m.rope, c, c->rope_dim, 32, c->rope_dim == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
 }
 
 template <int KV, int R, int N, typename T, bool Q8, bool CAUSAL>
-void launch_tc(mm::spa::TcArgs a, long long items, cudaStream_t s) {
+void launch_tc(mm::spa::TcArgs a, const Maps& m, long long items, cudaStream_t s) {
     using C = mm::spa::TcCfg<KV, R, N, Q8>;
-    CUtensorMap tile{}, block{}, rope{};
-    if (!Q8) {
-        const mm::lat::CacheView& c = a.suffix ? a.p.suffix : a.p.prefix;
-        const int dtype = std::is_same<T, __nv_bfloat16>::value ? MM_BF16 : MM_F16;
-        a.tma = cache_map(&tile, c, KV + R, dtype, 64, C::KT, CU_TENSOR_MAP_SWIZZLE_128B) &&
-                cache_map(&block, c, KV + R, dtype, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B) &&
-                cache_map(&rope, c, KV + R, dtype, R, 32, R == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
-    }
+    const mm::lat::CacheView& c = a.suffix ? a.p.suffix : a.p.prefix;
+    a.map_rows = c.rows > 1 && c.row_stride > 0 ? 1 : 0;
     set_dynamic_smem<mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8, CAUSAL>>(C::kSmem);
     launch(s, mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8, CAUSAL>,
            dim3(static_cast<unsigned>(std::min<long long>(items, sm_count() * C::kCtas))), dim3(C::kThreads), C::kSmem, a,
-           tile, block, rope);
+           m.tile, m.block, m.rope);
 }
 template <int KV, int R, typename T>
-void launch_tc_n(const mm::spa::TcArgs& a, int n, bool q8, long long items, cudaStream_t s) {
+void launch_tc_n(const mm::spa::TcArgs& a, const Maps& m, int n, bool q8, long long items, cudaStream_t s) {
     auto go = [&](auto size, auto codes) {
         constexpr int N = decltype(size)::value;
         constexpr bool Q8 = decltype(codes)::value;
-        if (a.suffix && a.p.T > 1) launch_tc<KV, R, N, T, Q8, true>(a, items, s);
-        else launch_tc<KV, R, N, T, Q8, false>(a, items, s);
+        if (a.suffix && a.p.T > 1) launch_tc<KV, R, N, T, Q8, true>(a, m, items, s);
+        else launch_tc<KV, R, N, T, Q8, false>(a, m, items, s);
     };
     using N16 = std::integral_constant<int, 16>;
     using N64 = std::integral_constant<int, 64>;
@@ -365,7 +376,8 @@ void launch_tc_n(const mm::spa::TcArgs& a, int n, bool q8, long long items, cuda
 }
 
 template <int KV, int R, typename T>
-void run_tc(const mm::spa::Problem& p, const Plan& r, bool q8p, bool q8s, void* workspace, cudaStream_t s) {
+void run_tc(const mm::spa::Problem& p, const Plan& r, const Maps& pre, const Maps& suf, bool q8p, bool q8s, void* workspace,
+            cudaStream_t s) {
     using namespace mm::spa;
     float* w = static_cast<float*>(workspace);
     float* pre_o = w;
@@ -380,7 +392,7 @@ void run_tc(const mm::spa::Problem& p, const Plan& r, bool q8p, bool q8s, void* 
         a.kps = r.pre_kps;
         a.part_o = pre_o;
         a.part_ml = pre_ml;
-        launch_tc_n<KV, R, T>(a, r.pre_n, q8p, r.pre_blocks * r.pre_splits, s);
+        launch_tc_n<KV, R, T>(a, pre, r.pre_n, q8p, r.pre_blocks * r.pre_splits, s);
     }
     if (r.suf_n) {
         a.suffix = 1;
@@ -393,7 +405,7 @@ void run_tc(const mm::spa::Problem& p, const Plan& r, bool q8p, bool q8s, void* 
         a.prefix_kps = r.pre_kps;
         a.overlap = r.pre_n ? 1 : 0;
         a.pieces = pieces;
-        launch_tc_n<KV, R, T>(a, r.suf_n, q8s, r.suf_blocks * r.suf_splits, s);
+        launch_tc_n<KV, R, T>(a, suf, r.suf_n, q8s, r.suf_blocks * r.suf_splits, s);
     }
     if (r.join)
         launch(s, r.span ? shared_prefix_join_kernel<KV, T, true> : shared_prefix_join_kernel<KV, T, false>, dim3(blocks(r.rows, 8)),
@@ -518,7 +530,8 @@ int mm_shared_prefix_attention(const mm_shared_prefix_desc* desc, const mm_laten
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         const bool q8p = prefix && prefix->kind == MM_E4M3;
         const bool q8s = suffix && suffix->kind == MM_E4M3;
-        if (tensor_core_form(p, prefix, suffix)) {
+        Maps pre, suf;
+        if (tensor_core_form(p, prefix, suffix) && (p.G == 0 || cache_maps(pre, prefix)) && (p.max_suffix == 0 || cache_maps(suf, suffix))) {
             const Plan r = plan(p);
             const long long need = r.bytes(p.kv);
             require(need == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
@@ -526,8 +539,8 @@ int mm_shared_prefix_attention(const mm_shared_prefix_desc* desc, const mm_laten
                     "shared-prefix attention: workspace too small or not 16-byte aligned");
             with_half(desc->dtype, [&](auto half) {
                 using T = typename decltype(half)::type;
-                if (p.kv == 128) run_tc<128, 16, T>(p, r, q8p, q8s, workspace, s);
-                else run_tc<512, 32, T>(p, r, q8p, q8s, workspace, s);
+                if (p.kv == 128) run_tc<128, 16, T>(p, r, pre, suf, q8p, q8s, workspace, s);
+                else run_tc<512, 32, T>(p, r, pre, suf, q8p, q8s, workspace, s);
             });
             return;
         }

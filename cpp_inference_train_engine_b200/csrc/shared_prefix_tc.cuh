@@ -29,9 +29,8 @@
 //              ones reach 2^15.
 //   producers  2 or 4: the item's queries, then per tile of KT keys the rope columns and kv / 128 pairs
 //              of 64-column boxes (each pair its own warps) into rings of swizzled boxes. 16-bit caches come
-//              by TMA (where the encoder does not take the strides: by 16-byte cp.async); e4m3 codes
-//              are loaded D tiles ahead into registers and stored as 16-bit values (exact). What the
-//              cache holds past the range is masked in S and never read by an O product.
+//              by TMA; e4m3 codes are loaded D tiles ahead into registers and stored as 16-bit values
+//              (exact). What the cache holds past the range is masked in S and never read by an O product.
 //   fence      one warp passes each landed tile on to the asynchronous proxy: a proxy fence costs
 //              about 100 ns, and in the loading threads it would wait for every load they have in
 //              flight (measured: 1.7 instead of over 5 TB/s). It also takes a NaN or an infinity out of the
@@ -90,7 +89,7 @@ struct TcArgs {
     // CTAs; a row cut where a CTA's share ends is left to the join kernel. Per row the first CTA and the number of
     // its parts (0: whole, the launch wrote its result); null: key ranges
     int2* pieces;
-    int tma;           // the tensor maps are valid: a 16-bit cache comes by TMA
+    int map_rows;      // 0: the cache's rows are one and the same (a row stride of zero), and so is the tensor maps'
 };
 
 constexpr int kTcMaxPlan = 512;   // entries of the shared plan (the items of runs of groups or rows)
@@ -129,7 +128,7 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int PS = KV == 512 ? (N == 64 ? 8 : 10) : (N == 64 ? 4 : 2);
     static constexpr int RS = KV == 512 ? (N == 64 ? 2 : 3) : PS;
     static constexpr int PB = 2;
-    static constexpr int TS = 4;  // tiles announced: more than the pair ring ever holds
+    static constexpr int TS = 4;  // tiles announced: no fewer than the pair ring holds
     static constexpr int OB = KV == 512 && N == 64 ? 1 : 2;
     // tensor memory columns: two S buffers (e4m3: two more for the rope columns' share, which the
     // key's scale does not multiply), then the O accumulators
@@ -663,9 +662,8 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             constexpr int kChunks = R / 8, kRows = C::PT / kChunks;
             const int c = pt % kChunks, r0 = pt / kChunks, left = it.nk - j * KT;
             uint8_t* d = sRope + slot * C::kRopeA;
-            const long long ps = 2 * (Q8 ? cv.rope_pos_stride : cv.pos_stride);
-            const uint8_t* src = (Q8 ? cv.rope + 2 * (it.row * cv.rope_row_stride)
-                                     : cv.latent + 2 * (it.row * cv.row_stride + KV)) + (it.k0 + j * KT) * ps + c * 16;
+            const long long ps = 2 * cv.rope_pos_stride;
+            const uint8_t* src = cv.rope + 2 * (it.row * cv.rope_row_stride) + (it.k0 + j * KT) * ps + c * 16;
 #pragma unroll
             for (int r = r0; r < KT; r += kRows) cp_async16(d + sw_rope<R>(r, c), src + (r < left ? r : 0) * ps, r < left);
         };
@@ -697,53 +695,36 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             rp.skip(C::NP);
         };
         if constexpr (!Q8) {
-            const int cc = lane & 15, r0 = (lane >> 4) + 2 * sub;  // 16-byte chunk of the pair's row, first row
-            const long long ps = 2 * cv.pos_stride;
             for (int base = 0; base < mine; base += kTcTable) {
                 const int count = next_table(base, std::false_type());
                 for (Cursor c(table, count); c.valid(); c.next()) {
                     const Item& it = c.item();
                     begin_tile(it, c.j);
                     const int left = it.nk - c.j * KT;
-                    if (a.tma) {
-                        // one thread per pair asks for its two boxes, a range's last tile in the blocks of 32
-                        // positions that the range reaches, and the first pair's for the rope columns
-                        if (sub == 0 && elect_one() && ok) {
-                            const int nb = min((left + 31) >> 5, KT / 32), pos = it.k0 + c.j * KT;
-                            uint64_t* bar = &tile_in[rt.i];
-                            mbar_arrive_expect_tx(bar, nb * (2 * 4096 + (own == 0 ? 64 * R : 0)));
-                            uint8_t* box = sPair + rp.i * C::kPair;
-                            if (left >= KT) {
-                                tma_load_3d(box, &map_tile, bar, own * 128, pos, it.row);
-                                tma_load_3d(box + C::kBox, &map_tile, bar, own * 128 + 64, pos, it.row);
-                            } else {
+                    // one thread per pair asks for its two boxes, a range's last tile in the blocks of 32
+                    // positions that the range reaches, and the first pair's for the rope columns
+                    if (sub == 0 && elect_one() && ok) {
+                        const int nb = min((left + 31) >> 5, KT / 32), pos = it.k0 + c.j * KT, row = it.row * a.map_rows;
+                        uint64_t* bar = &tile_in[rt.i];
+                        mbar_arrive_expect_tx(bar, nb * (2 * 4096 + (own == 0 ? 64 * R : 0)));
+                        uint8_t* box = sPair + rp.i * C::kPair;
+                        if (left >= KT) {
+                            tma_load_3d(box, &map_tile, bar, own * 128, pos, row);
+                            tma_load_3d(box + C::kBox, &map_tile, bar, own * 128 + 64, pos, row);
+                        } else {
 #pragma unroll 1
-                                for (int k = 0; k < nb; ++k) {
-                                    tma_load_3d(box + k * 4096, &map_block, bar, own * 128, pos + 32 * k, it.row);
-                                    tma_load_3d(box + C::kBox + k * 4096, &map_block, bar, own * 128 + 64, pos + 32 * k, it.row);
-                                }
-                            }
-                            if (own == 0) {
-#pragma unroll 1
-                                for (int k = 0; k < nb; ++k)
-                                    tma_load_3d(sRope + rr.i * C::kRopeA + k * 64 * R, &map_rope, bar, KV, pos + 32 * k, it.row);
+                            for (int k = 0; k < nb; ++k) {
+                                tma_load_3d(box + k * 4096, &map_block, bar, own * 128, pos + 32 * k, row);
+                                tma_load_3d(box + C::kBox + k * 4096, &map_block, bar, own * 128 + 64, pos + 32 * k, row);
                             }
                         }
-                        if (__any_sync(0xffffffffu, !ok)) break;
-                        end_tile();
-                        continue;
+                        if (own == 0) {
+#pragma unroll 1
+                            for (int k = 0; k < nb; ++k)
+                                tma_load_3d(sRope + rr.i * C::kRopeA + k * 64 * R, &map_rope, bar, KV, pos + 32 * k, row);
+                        }
                     }
-                    if (sub == 0 && lane == 0) mbar_arrive(&tile_in[rt.i]);
-                    load_rope(it, c.j, rr.i);
-                    const uint8_t* first = cv.latent + 2 * (it.row * cv.row_stride) + (it.k0 + c.j * KT) * ps + own * 256 + cc * 16;
-                    const uint8_t* src = first + r0 * ps;
-                    uint8_t* d = sPair + rp.i * C::kPair + (cc >> 3) * C::kBox;
-#pragma unroll 16
-                    for (int r = r0; r < KT; r += 2 * C::WPP) {
-                        const bool in = r < left;
-                        cp_async16(d + sw128(r, cc & 7), in ? src : first, in);
-                        src += 2 * C::WPP * ps;
-                    }
+                    if (__any_sync(0xffffffffu, !ok)) break;
                     end_tile();
                 }
             }
@@ -902,7 +883,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     }
                     wait(&tile_in[ft.i], ft.phase);
                     const int left = c.item().nk - c.j * KT;
-                    if (!Q8 && a.tma && left < KT && (left & 15)) {
+                    if (!Q8 && left < KT && (left & 15)) {
                         // the O products read whole steps of 16 keys: rows [left, next multiple of 16)
                         const int rows = 16 - (left & 15);
                         const uint4 zero = make_uint4(0, 0, 0, 0);

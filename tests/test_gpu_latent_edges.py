@@ -307,3 +307,25 @@ def test_every_position_of_a_prompt_is_a_query(form, kind, tokens):
     assert torch.all(((out.double() - want).abs() <= tol)[ok])
     assert torch.all(((lse.double() - wl).abs() <= es + tokens * 2.0 ** -24 + 2.0 ** -20 * (1 + wl.abs()))[ok & seen])
     assert torch.isnan(out[~ok]).all()
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("fp8", [False, True])
+def test_caches_whose_rows_share_their_storage(form, fp8):
+    """Groups that share one stored prompt, and rows one suffix: strides of zero. And a cache of one row."""
+    torch, latent = mods()
+    kv, rope, H, T = form
+    g = torch.Generator(device="cuda").manual_seed(38)
+
+    def shared(n, positions):
+        c, v, unit = stored(torch, torch.randn(1, positions, kv + rope, generator=g, device="cuda"), kv, torch.float16, fp8)
+        e = lambda t: t.expand(n, *t.shape[1:])  # noqa: E731
+        return (tuple(map(e, c)) if fp8 else e(c)), e(v), e(unit)
+
+    pre, suf = shared(2, 300), shared(5, 210)
+    q = torch.randn(5, T, H, kv + rope, generator=g, device="cuda").half()
+    args = ([0, 3, 5], [300, 141], [210, 9, 0, 64, 130], kv, 0.1)
+    agree(torch, run(torch, latent, q, pre[0], suf[0], *args), bound(torch, q, pre, suf, *args, fp8))
+    pre, suf = shared(1, 130), shared(1, 90)
+    args = ([0, 1], [130], [90], kv, 0.1)
+    agree(torch, run(torch, latent, q[:1], pre[0], suf[0], *args), bound(torch, q[:1], pre, suf, *args, fp8))

@@ -76,3 +76,12 @@ def test_status_of_the_waits_is_reported():
     if torch.cuda.is_available():
         pytest.skip("a GPU is present")
     assert E.lib().mm_latent_status(None) == 5 and "status" in message()
+
+
+@pytest.mark.parametrize("field,value", [(3, 2 ** 39), (3, -2304), (4, 0), (4, -144), (4, 2 ** 39)])
+def test_strides_that_no_tensor_map_takes_use_the_other_form(field, value):
+    """Row strides (field 3) and position strides (field 4) of 16-bit caches outside a tensor map's range."""
+    import struct
+    raw = bytearray(cache())
+    struct.pack_into("=q", raw, 8 * field, value)
+    assert entries().mm_shared_prefix_attention_workspace(*desc(suffix=bytes(raw))) == 0
