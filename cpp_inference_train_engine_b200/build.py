@@ -1,6 +1,7 @@
 """Builds the sm_100a backend in place: cpp_inference_train_engine_b200/libmm_cuda.so, from its
-two translation units (the engine and the latent-cache operators), and _latent_torch.so, the
-binding of the latter to torch tensors.
+two translation units (the engine and the latent-cache operators), and after it _latent_torch.so,
+the binding of the latter to torch tensors, where a torch with CUDA can be imported (the library
+needs none).
 
     python -m cpp_inference_train_engine_b200.build
 
@@ -29,19 +30,21 @@ def sources():
         os.path.join(ROOT, "include", f) for f in os.listdir(os.path.join(ROOT, "include"))]
 
 
-def up_to_date() -> bool:
-    if not os.path.exists(OUT) or not os.path.exists(TORCH_OUT):
+def up_to_date(out: str) -> bool:
+    if not os.path.exists(out):
         return False
-    t = min(os.path.getmtime(OUT), os.path.getmtime(TORCH_OUT))
+    t = os.path.getmtime(out)
     return all(os.path.getmtime(s) <= t for s in sources())
 
 
 def torch_command():
     """g++ on the torch binding, against the installed torch's headers and libraries and the
-    library beside it."""
+    library beside it. ImportError where there is no torch with CUDA."""
     import sysconfig
 
     import torch
+    if not torch.version.cuda:
+        raise ImportError("the installed torch has no CUDA")
     root = os.path.dirname(torch.__file__)
     cuda = os.path.join(os.path.dirname(NVCC), "..", "include")
     includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
@@ -52,22 +55,31 @@ def torch_command():
             "-Wl,-rpath,$ORIGIN"]
 
 
+def _run(command, out: str, verbose: bool) -> None:
+    """A compiler that writes out + ".tmp", put in place when it succeeds."""
+    if verbose:
+        print(" ".join(command), flush=True)
+    r = subprocess.run(command, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError(f"{command[0]} failed")
+    if verbose and r.stderr.strip():
+        sys.stderr.write(r.stderr)
+    os.replace(out + ".tmp", out)
+
+
 def build(force: bool = False, verbose: bool = True) -> str:
-    if not force and up_to_date():
-        return OUT
-    cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr",
-           "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", "-Xptxas", "-warn-spills",
-           "-t", "2", "-I", os.path.join(ROOT, "include"), *SRC, "-o", OUT + ".tmp", "-ldl", "-lpthread"]
-    for out, c in ((OUT, cmd), (TORCH_OUT, torch_command())):
-        if verbose:
-            print(" ".join(c), flush=True)
-        r = subprocess.run(c, capture_output=True, text=True)
-        if r.returncode != 0:
-            sys.stderr.write(r.stdout + r.stderr)
-            raise RuntimeError(f"{c[0]} failed")
-        if verbose and r.stderr.strip():
-            sys.stderr.write(r.stderr)
-        os.replace(out + ".tmp", out)
+    if force or not up_to_date(OUT):
+        _run([NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr",
+              "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", "-Xptxas", "-warn-spills",
+              "-t", "2", "-I", os.path.join(ROOT, "include"), *SRC, "-o", OUT + ".tmp", "-ldl", "-lpthread"], OUT, verbose)
+    if force or not up_to_date(TORCH_OUT):
+        try:
+            command = torch_command()
+        except ImportError as e:
+            sys.stderr.write(f"{os.path.basename(TORCH_OUT)} (latent.py) was not built, it needs a torch with CUDA: {e}\n")
+        else:
+            _run(command, TORCH_OUT, verbose)
     return OUT
 
 
