@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/Dtype.h>
 
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -57,9 +58,15 @@ void call(int rc) {
     throw Refusal{rc, text};
 }
 
+// The calls go past autograd: a result would silently be a constant of its inputs.
+const at::Tensor& no_gradient(const at::Tensor& t) {
+    if (t.requires_grad() && at::GradMode::is_enabled())
+        bad("no gradient flows through these operators: detach the tensors that require one, or call under torch.no_grad()");
+    return t;
+}
 const at::Tensor& tensor(PyObject* o, const char* what) {
     if (!THPVariable_Check(o)) bad(std::string(what) + " must be a tensor");
-    return THPVariable_Unpack(o);
+    return no_gradient(THPVariable_Unpack(o));
 }
 const at::Tensor& cuda_tensor(PyObject* o, const char* what) {
     const at::Tensor& t = tensor(o, what);
@@ -109,7 +116,7 @@ mm_latent_cache cache(PyObject* o, c10::Device d, int64_t kv) {
     mm_latent_cache c{};
     if (THPVariable_Check(o)) {
         if (kv < 0) bad("an 8-bit cache (LatentCache) is needed");
-        const at::Tensor& t = THPVariable_Unpack(o);
+        const at::Tensor& t = no_gradient(THPVariable_Unpack(o));
         const int kind = kind_of(t.scalar_type());
         if (t.dim() != 3 || !half(kind) || !last_adjacent(t))
             bad("a 16-bit cache is fp16 or bf16 [rows, positions, kv + rope] with adjacent values");

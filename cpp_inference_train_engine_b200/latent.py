@@ -16,7 +16,8 @@ The reference decodes one request at a time over its own fp32 cache
 (src/infer/inference.cpp:47-174, 469-579). A 16-bit cache is a plain tensor ``[rows,
 positions, kv + rope]`` (the layout of the context's own cache), an 8-bit one a
 :class:`LatentCache`. Calls enqueue on the current stream of the tensors' device and do not
-wait; outputs and scratch come from torch's allocator. Failures raise :class:`EngineError`
+wait; outputs and scratch come from torch's allocator. No gradient flows through them: a tensor
+that requires one is refused while gradients are recorded. Failures raise :class:`EngineError`
 (what only the device knows: ``check_status``).
 
 The checks, allocations and C calls are in csrc/latent_torch.cpp (a small call's time is its

@@ -329,3 +329,27 @@ def test_caches_whose_rows_share_their_storage(form, fp8):
     pre, suf = shared(1, 130), shared(1, 90)
     args = ([0, 1], [130], [90], kv, 0.1)
     agree(torch, run(torch, latent, q[:1], pre[0], suf[0], *args), bound(torch, q[:1], pre, suf, *args, fp8))
+
+
+def test_no_argument_may_require_a_gradient():
+    torch, latent = mods()
+    from cpp_inference_train_engine_b200 import EngineError
+    half = dict(dtype=torch.float16, device="cuda")
+    q, pre, suf = torch.zeros(2, 1, 8, 144, **half), torch.zeros(1, 16, 144, **half), torch.zeros(2, 16, 144, **half)
+    for t in (q, pre, suf):
+        t.requires_grad_()
+        with pytest.raises(EngineError, match="gradient"):
+            run(torch, latent, q, pre, suf, [0, 2], [4], [1, 2], 128, 0.1)
+        with torch.no_grad():
+            run(torch, latent, q, pre, suf, [0, 2], [4], [1, 2], 128, 0.1)
+        t.requires_grad_(False)
+    c = latent.alloc_cache(2, 16, 128, 16)
+    x, r, s = torch.zeros(3, 128, **half), torch.zeros(3, 16, **half), torch.arange(3, device="cuda")
+    for t in (x, r, c.rope, c.scale):
+        t.requires_grad_()
+        with pytest.raises(EngineError, match="gradient"):
+            latent.cache_write(c, x, r, s)
+        t.requires_grad_(False)
+    c.scale.requires_grad_()
+    with pytest.raises(EngineError, match="gradient"):
+        latent.cache_read(c, s)

@@ -85,3 +85,20 @@ def test_strides_that_no_tensor_map_takes_use_the_other_form(field, value):
     raw = bytearray(cache())
     struct.pack_into("=q", raw, 8 * field, value)
     assert entries().mm_shared_prefix_attention_workspace(*desc(suffix=bytes(raw))) == 0
+
+
+def test_tensors_that_require_a_gradient_are_refused():
+    """No gradient flows through the operators; without recording, or detached, the tensors are taken (and
+    refused here for not being on a GPU)."""
+    from cpp_inference_train_engine_b200 import EngineError, latent
+    q = torch.zeros(1, 1, 8, 144, dtype=torch.float16, requires_grad=True)
+    p = torch.ones(1, 2, 8, requires_grad=True)
+    ints, one = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1)
+    calls = [lambda: latent.shared_prefix_attention(q, None, None, None, None, None, 0.1, kv_rank=128),
+             lambda: latent.cache_write(None, q[0, 0, :, :128], q[0, 0, :, 128:], torch.zeros(8, dtype=torch.int64)),
+             lambda: latent.verify_drafts(p, ints, ints[0], one[None], one)]
+    for call in calls:
+        with pytest.raises(EngineError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(EngineError, match="CUDA tensor"):
+            call()
