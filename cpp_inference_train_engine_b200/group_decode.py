@@ -211,9 +211,11 @@ class GroupDecoder:
         return torch.nn.functional.one_hot(logits.argmax(-1), logits.shape[-1]).float()
 
     def generate(self, temperature: float = 0.0, seed: int = 0):
-        """Completes every row: (tokens as one list per row, statistics). A completion ends with
-        the end-of-sequence token or after `new_tokens`."""
+        """Completes every row from its prompt: (tokens as one list per row, statistics). A completion
+        ends with the end-of-sequence token or after `new_tokens`."""
         c, B = self.cfg, self.row_group.numel()
+        self.count.zero_()
+        self.history.masked_fill_(torch.arange(self.history.shape[1], device=self.device) >= self.row_prompt[:, None], -1)
         g = torch.Generator(device=self.device).manual_seed(seed)
         uniform = lambda *shape: torch.rand(*shape, generator=g, device=self.device)  # noqa: E731
 
