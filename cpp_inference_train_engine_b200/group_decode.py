@@ -212,7 +212,8 @@ class GroupDecoder:
 
     def generate(self, temperature: float = 0.0, seed: int = 0):
         """Completes every row from its prompt: (tokens as one list per row, statistics). A completion
-        ends with the end-of-sequence token or after `new_tokens`."""
+        ends with the end-of-sequence token or after `new_tokens`. Raises EngineError when a row's
+        logits leave no token to pick (a NaN)."""
         c, B = self.cfg, self.row_group.numel()
         self.count.zero_()
         self.history.masked_fill_(torch.arange(self.history.shape[1], device=self.device) >= self.row_prompt[:, None], -1)
@@ -229,11 +230,18 @@ class GroupDecoder:
         self._append(first, torch.ones_like(self.count))
         open_rows = (first[:, 0] != c.eos_id) & (self.count < self.new_tokens)
         steps = kept = proposed = 0
-        while bool(open_rows.any()):
+        failed = (first[:, 0] < 0).any()
+        while True:
+            go_on, no_token = torch.stack([open_rows.any(), failed]).tolist()
+            if no_token:
+                raise EngineError(6, "no token has a probability (the logits hold a NaN)")
+            if not go_on:
+                break
             last = self.history.gather(1, (self.row_prompt + self.count - 1)[:, None])
             tokens, number = self._propose() if self.drafts else (none, zero)
             number = torch.where(open_rows, number, 0).int()
             picked, accepted = accept(self.step_logits(torch.cat([last, tokens], 1)), tokens.contiguous(), number)
+            failed = (open_rows & (picked.gather(1, accepted.long()[:, None])[:, 0] < 0)).any()
             # nothing after an end-of-sequence token, nothing for the rows that are done
             take = accepted.long() + 1
             stop = (picked == c.eos_id) & (torch.arange(picked.shape[1], device=self.device)[None] < take[:, None])
