@@ -173,6 +173,9 @@ class GroupDecoder:
         completions' first count - 1 tokens)."""
         B, T = tokens.shape
         done = (self.count - 1).clamp_min(0)
+        # a generating row has room for its last token and `drafts` more; only for others is the count waited for
+        if T > self.drafts + 1 and int(done.max()) + T > self.capacity:
+            raise EngineError(1, "a row's completion has no room for that many tokens")
         at = done[:, None] + torch.arange(T, device=self.device)
         slots = torch.where(at < self.capacity, torch.arange(B, device=self.device)[:, None] * self.capacity + at, -1)
         suffix_len = (done + T).clamp_max(self.capacity).int()

@@ -29,3 +29,17 @@ def test_logits_without_a_token_are_an_error():
             with pytest.raises(E.EngineError, match="no token") as e:
                 d.generate(temperature)
             assert e.value.name == "numerical_error"
+
+
+def test_more_tokens_than_a_completion_has_room_for_are_refused():
+    import torch
+    d = make("tiny", 8, new=5, drafts=2)[3]
+    rows = d.row_group.numel()
+    tokens = torch.ones(rows, 8, dtype=torch.int32, device="cuda")
+    with pytest.raises(E.EngineError, match="room"):
+        d.step_logits(tokens)
+    assert torch.isfinite(d.step_logits(tokens[:, :7])).all()
+    d._append(tokens[:, :4], torch.full_like(d.count, 4))
+    with pytest.raises(E.EngineError, match="room"):
+        d.step_logits(tokens[:, :5])
+    assert torch.isfinite(d.step_logits(tokens[:, :4])).all()
