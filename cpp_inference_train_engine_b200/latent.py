@@ -85,7 +85,8 @@ def alloc_cache(rows: int, positions: int, kv: int, rope: int, dtype=torch.float
 def cache_write(cache: LatentCache, latent: torch.Tensor, rope: torch.Tensor, slots: torch.Tensor) -> None:
     """Quantises new positions into an 8-bit cache in place: latent [n, kv] and rope [n, rope] of
     one type (fp32, fp16 or bf16), position i into slots[i] = row * positions + position; slots
-    outside the cache are skipped (free rows of a step pass -1)."""
+    outside the cache are skipped (free rows of a step pass -1), the others must be distinct (a
+    position given twice ends as a mix of both)."""
     _write(cache, latent, rope, slots)
 
 

@@ -15,7 +15,7 @@
  *   - what only the device holds (lengths, group bounds, slots, draft tokens) is not checked
  *     on the host; kernels clamp or skip out-of-range values, so no access leaves a buffer;
  *   - results do not depend on scheduling (no floating-point atomics): equal inputs give equal
- *     bits;
+ *     bits (a slot written twice by one call excepted);
  *   - memory past a length may hold anything, NaN included: it never reaches a result;
  *   - the attention kernel's waits are bounded. One that runs out (a defect or a fault of the
  *     machine, never the input) makes the results it concerns NaN, and mm_latent_status says so.
@@ -63,7 +63,8 @@ int mm_latent_status(void* stream);
 
 /* Quantises n new positions into an MM_E4M3 cache. latent [n][kv] and rope [n][rope_dim] of
  * `dtype` (row strides in elements); position i goes to slots[i] = row * positions + position;
- * slots outside [0, rows * positions) are skipped (two equal slots: either may win).
+ * slots outside [0, rows * positions) are skipped. The others are distinct: a position given twice
+ * in one call may end with the codes, scale and rope key of different inputs (nothing else changes).
  *   scale = max(max_c |x_c| / 448, 2^-100), code = e4m3(x / scale) round to nearest even,
  * both in IEEE fp32. A NaN reads back as NaN; an infinity makes its position read back NaN. */
 int mm_latent_cache_write(const mm_latent_cache* cache, const void* latent, int64_t latent_stride,
