@@ -211,7 +211,8 @@ class GroupDecoder:
     def _probabilities(self, logits, temperature):
         if temperature > 0:
             return torch.softmax(logits / temperature, -1)
-        return torch.nn.functional.one_hot(logits.argmax(-1), logits.shape[-1]).float()
+        best = torch.nn.functional.one_hot(logits.argmax(-1), logits.shape[-1]).float()
+        return best.masked_fill_(logits.isnan().any(-1, keepdim=True), 0)  # argmax would pick the NaN
 
     def generate(self, temperature: float = 0.0, seed: int = 0):
         """Completes every row from its prompt: (tokens as one list per row, statistics). A completion

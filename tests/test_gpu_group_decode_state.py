@@ -34,6 +34,18 @@ def test_logits_without_a_token_are_an_error():
             assert e.value.name == "numerical_error"
 
 
+@pytest.mark.parametrize("where", ["prompt", "step"])
+def test_greedy_logits_with_a_nan_are_an_error(where):
+    import torch
+    d = make("tiny", 8)[3]
+    if where == "prompt":
+        d.prompt_logits[1, 7] = float("nan")
+    else:
+        d.final_norm = torch.full_like(d.final_norm, float("nan"))
+    with pytest.raises(E.EngineError, match="no token"):
+        d.generate(0.0)
+
+
 def test_more_tokens_than_a_completion_has_room_for_are_refused():
     import torch
     d = make("tiny", 8, new=5, drafts=2)[3]
