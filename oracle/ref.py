@@ -28,6 +28,10 @@ _u64p = ctypes.POINTER(ctypes.c_uint64)
 _libs = {}
 
 
+class NotBuilt(RuntimeError):
+    """The reference's sources were not there to build the oracle from (tests that need it are skipped)."""
+
+
 def available(backend: str = "cpu") -> bool:
     return os.path.exists(CUDA_LIB_PATH if backend == "cuda" else LIB_PATH)
 
@@ -37,7 +41,7 @@ def lib(backend: str = "cpu"):
     if L is None:
         path = CUDA_LIB_PATH if backend == "cuda" else LIB_PATH
         if not os.path.exists(path):
-            raise RuntimeError(f"reference oracle not built: {path} (run make -C oracle)")
+            raise NotBuilt(f"reference oracle not built: {path} (run make -C oracle)")
         L = ctypes.CDLL(path)
         L.ref_last_error.restype = ctypes.c_char_p
         L.ref_session_create.restype = ctypes.c_void_p
