@@ -210,6 +210,11 @@ PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const c10::cuda::CUDAGuard guard(d);
         call(mm_latent_cache_write(&c, latent.data_ptr(), latent.stride(0), rope.data_ptr(), rope.stride(0), kind, s, n,
                                    stream_of(d)));
+        // written in place: what autograd has kept of these tensors is no longer theirs
+        for (int i = 0; i < 3; ++i) {
+            const at::Tensor& t = THPVariable_Unpack(PyTuple_GET_ITEM(a[0], i));
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+        }
         Py_RETURN_NONE;
     });
 }

@@ -353,3 +353,19 @@ def test_no_argument_may_require_a_gradient():
     c.scale.requires_grad_()
     with pytest.raises(EngineError, match="gradient"):
         latent.cache_read(c, s)
+
+
+def test_a_write_counts_as_one():
+    """autograd notices that a tensor which it keeps was written."""
+    torch, latent = mods()
+    c = latent.alloc_cache(2, 16, 128, 16)
+    w = torch.ones_like(c.scale, requires_grad=True)
+    loss = (c.scale * w).sum()  # keeps the scales for w's gradient
+    x, r, s = torch.ones(3, 128, device="cuda"), torch.ones(3, 16, device="cuda"), torch.arange(3, device="cuda")
+    before = [t._version for t in c]
+    latent.cache_write(c, x, r, s)
+    assert all(t._version > v for t, v in zip(c, before))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        latent.cache_write(latent.alloc_cache(2, 16, 128, 16), x, r, s)
