@@ -88,9 +88,13 @@ __device__ __forceinline__ void load_entries(const T* __restrict__ row, int x0, 
 // chunk sums, and the chunk alone is read again to find the entry. Bound by the p (and q)
 // row's bytes at large batches and by that chain's latency at small ones. 32 registers keep every
 // warp slot taken. THREADS: 1024 spreads a row over more warps, 512 runs four rows beside each other on
-// an SM, whose chains overlap (fp32 probabilities of 32,768 tokens; 64 rows: 8.3 us with 1024, 10.1 with
-// 512; 1,024 rows: 48.2 and 44.1, 5.5 TB/s; 600 bf16 rows: 28.2 and 29.2): 512 from five rows per
-// SM on (at four and a few more its second wave is nearly empty).
+// an SM, whose chains overlap: 512 where the rows do not fit at once with 1024, two to an SM. Both, in us
+// (1024 / 512), probabilities read from memory, with draft probabilities:
+//   rows                      64           148          296          370          592          600          1024
+//   16,384 tokens, fp32    8.0 / 9.6    8.8 / 10.0  11.0 / 11.9  15.6 / 13.1  19.0 / 16.0  20.2 / 19.0  31.0 / 26.0
+//   32,768 tokens, fp32   11.1 / 14.9  12.6 / 15.6  16.8 / 18.9  23.3 / 21.1  29.8 / 28.1  31.0 / 31.9  47.6 / 43.5
+//   32,768 tokens, bf16   11.9 / 17.4  12.2 / 17.6  14.2 / 19.1  21.6 / 22.1  26.6 / 23.2  27.9 / 28.9  44.3 / 40.1
+// (at 600 the second wave of 512 is nearly empty). 1,024 fp32 rows of 32,768 run at 5.5 TB/s.
 template <typename T, bool ALIGNED, int THREADS>
 __global__ void __launch_bounds__(THREADS, 2048 / THREADS) verify_drafts_kernel(
     const T* __restrict__ target, const T* __restrict__ draft, const int* __restrict__ tokens,

@@ -576,7 +576,7 @@ int mm_verify_drafts(const void* target_probs, const void* draft_probs, int dtyp
                        out_tokens, accepted);
             };
             const bool aligned = vocab % 4 == 0 && fits(p) && fits(q);
-            if (rows >= 5 * sm_count())
+            if (rows > 2 * sm_count())
                 aligned ? run(mm::ver::verify_drafts_kernel<T, true, 512>, 512) : run(mm::ver::verify_drafts_kernel<T, false, 512>, 512);
             else
                 aligned ? run(mm::ver::verify_drafts_kernel<T, true, 1024>, 1024) : run(mm::ver::verify_drafts_kernel<T, false, 1024>, 1024);
