@@ -567,8 +567,14 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         items = plan_s[runs];
     }
     // Shares, or the rows one by one in turn, which needs no join and serves rows of like lengths: by the
-    // fullest CTA's rows against the mean. 512 + 32 wide, 136 ragged rows of up to 1,536 (2.1): 70.4 us in
-    // turn, 65.0 in shares, as e4m3 86 and 72; 300 rows of 700 (1.5): 79.5 in turn, 89.8 in shares.
+    // fullest CTA's rows against the mean, shares from 1.25 on. 512 + 32 wide, us in turn / in shares, fp16
+    // and e4m3:
+    //   136 rows of about 1,000, spread (fullest over mean 1.06, 1.25, 1.44, 1.75, 2.06)
+    //     38.4 / 44.6, 41.8 / 43.8, 44.6 / 43.6, 51.4 / 44.6, 56.1 / 44.0
+    //     41.9 / 46.1, 47.6 / 46.4, 51.5 / 47.0, 60.9 / 47.7, 69.3 / 47.4
+    //   250, 600, 340, 300, 170 rows of 700 (1.14, 1.22, 1.29, 1.44, 1.71)
+    //     49.2 / 50.8, 105.4 / 98.4, 68.0 / 63.5, 65.6 / 58.5, 47.0 / 40.1
+    //     57.4 / 57.6, 121.5 / 114.3, 79.3 / 72.0, 76.0 / 65.8, 52.4 / 41.8
     int span = 0;
     if (kShares && spans) {
         int* bins = reinterpret_cast<int*>(table);  // free until the first table
@@ -583,7 +589,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
             most = __reduce_max_sync(0xffffffffu, most);
         }
         span = max((items + grid - 1) / grid, kMinSpan);
-        if (most > 0 && 4 * most < 7 * span) {
+        if (most > 0 && 4 * most < 5 * span) {
             spans = false;
             plan = nullptr;
             items = units;
