@@ -355,6 +355,7 @@ template <int KV, int R, int N, typename T, bool Q8, bool CAUSAL>
 void launch_tc(mm::spa::TcArgs a, const Maps& m, long long items, cudaStream_t s) {
     using C = mm::spa::TcCfg<KV, R, N, Q8>;
     const mm::lat::CacheView& c = a.suffix ? a.p.suffix : a.p.prefix;
+    a.apart = std::min(a.p.T - 1, (N + a.p.H - 2) / a.p.H);
     a.map_rows = c.rows > 1 && c.row_stride > 0 ? 1 : 0;
     set_dynamic_smem<mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8, CAUSAL>>(C::kSmem);
     launch(s, mm::spa::shared_prefix_tc_kernel<KV, R, N, T, Q8, CAUSAL>,
@@ -366,7 +367,7 @@ void launch_tc_n(const mm::spa::TcArgs& a, const Maps& m, int n, bool q8, long l
     auto go = [&](auto size, auto codes) {
         constexpr int N = decltype(size)::value;
         constexpr bool Q8 = decltype(codes)::value;
-        if (a.suffix && a.p.T > 1) launch_tc<KV, R, N, T, Q8, true>(a, m, items, s);
+        if (a.p.T > 1) launch_tc<KV, R, N, T, Q8, true>(a, m, items, s);
         else launch_tc<KV, R, N, T, Q8, false>(a, m, items, s);
     };
     using N16 = std::integral_constant<int, 16>;

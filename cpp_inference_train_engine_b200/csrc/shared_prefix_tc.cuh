@@ -89,6 +89,7 @@ struct TcArgs {
     // CTAs; a row cut where a CTA's share ends is left to the join kernel. Per row the first CTA and the number of
     // its parts (0: whole, the launch wrote its result); null: key ranges
     int2* pieces;
+    int apart;         // the limits of a suffix block's tokens end at most this far apart
     int map_rows;      // 0: the cache's rows are one and the same (a row stride of zero), and so is the tensor maps'
 };
 
@@ -152,8 +153,8 @@ template <int KV, int R, int N, bool Q8> struct TcCfg {
     static constexpr int oRope = oQ + QB * kQA;
     static constexpr int oP = oRope + RS * kRopeA;
     static constexpr int oTab = oP + PB * kP;
-    static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N], up[N], base[N], mail[2][5][N], factor[5][N]
-    static constexpr int oPlan = oF + (9 + (EW ? 15 : 0)) * N * 4;
+    static constexpr int oF = oTab + kTcTable * 32;  // floats: m[N], corr[N], red[4][N], lim[N], up[N], base[N], mail[2][5][N], factor[5][N], limit[2] + 2
+    static constexpr int oPlan = oF + (9 + (EW ? 15 : 0)) * N * 4 + 16;
     static constexpr int oBar = oPlan + (kTcMaxPlan + 1) * 4 + 12;
     static constexpr int kBars = QB + PS + 2 * TS + 4 + 2 * PB + 2 * OB + 4 + 1;
     static_assert(RS * NP >= PS && TS * NP >= PS, "the rope ring and the tile barriers outlast the pair ring");
@@ -244,13 +245,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) 
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Column reductions over the 32 lanes: each step folds half of the remaining columns into the
-// other half's lane (62 shuffles for 64 values). Returns the first column the lane ends up with;
-// its results are v[0] (and v[1] for 64 columns; 16 columns: both lanes of a pair hold it).
-template <int NC, class Op> __device__ __forceinline__ int fold_columns(float (&v)[NC], int lane, Op op) {
+// Column reductions over the 32 lanes (those that differ in the bits up to FIRST): each step folds half of
+// the remaining columns into the other half's lane (31 shuffles for 32 values). Returns the column the lane
+// ends up with; its result is v[0] (16 columns: both lanes of a pair hold it).
+template <int FIRST = 16, int NC, class Op> __device__ __forceinline__ int fold_columns(float (&v)[NC], int lane, Op op) {
     int own = 0, w = NC;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = FIRST; o > 0; o >>= 1) {
         if (w > 1) {
             w >>= 1;
             const bool up = lane & o;
@@ -346,7 +347,7 @@ __device__ __forceinline__ Item get_item(const TcArgs& a, const int* plan, int u
     it.k0 = it.split * a.kps;
     // a block ends at the last key that its last query sees (16-query blocks hold a row's last token)
     int len = r.len;
-    if (N == 64 && CAUSAL && it.nq > 0) len = seen_by(a.p, len, block * N + it.nq - 1);
+    if (N == 64 && CAUSAL && a.suffix && it.nq > 0) len = seen_by(a.p, len, block * N + it.nq - 1);
     it.nk = it.nq > 0 ? max(0, min(a.kps, len - it.k0)) : 0;
     it.nt = (it.nk + KT - 1) / KT;
     it.np = it.split == 0 ? r.np : -1;
@@ -439,31 +440,33 @@ struct Cursor {
 // Value rows [from, to) of a landed tile are seen by some of the block's queries and masked for others, and a
 // probability of zero times a NaN or an infinity is a NaN: a row that holds one becomes zeros, with a NaN in
 // its rope columns, which only the scores read. So the queries that see it get NaN, and no other.
+template <bool kBf16> __device__ __forceinline__ bool bad_chunk(const uint4& v) {  // 16-bit values of it
+    constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
+    auto odd = [](uint32_t w) { return (w & kExp) == kExp || (w >> 16 & kExp) == kExp; };
+    return odd(v.x) || odd(v.y) || odd(v.z) || odd(v.w);
+}
+// 16-byte chunk e of value row r; the tile's pairs begin at first_pair of the ring.
+template <class C> __device__ __forceinline__ uint4* value_chunk(uint8_t* pairs, int first_pair, int r, int e) {
+    int pair = first_pair + (e >> 4);
+    if (pair >= C::PS) pair -= C::PS;
+    return reinterpret_cast<uint4*>(pairs + pair * C::kPair + ((e >> 3) & 1) * C::kBox + sw128(r, e & 7));
+}
 template <class C, int R, bool kBf16>
 __device__ __noinline__ void drop_bad_rows(uint8_t* pairs, int first_pair, uint8_t* rope, int from, int to, int lane) {
-    constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
-    auto chunk = [&](int r, int e) {  // 16-byte chunk e of row r
-        int pair = first_pair + (e >> 4);
-        if (pair >= C::PS) pair -= C::PS;
-        return reinterpret_cast<uint4*>(pairs + pair * C::kPair + ((e >> 3) & 1) * C::kBox + sw128(r, e & 7));
-    };
     for (int r = from; r < to; ++r) {
         bool bad = false;
-        for (int e = lane; e < 16 * C::NP; e += 32) {
-            const uint4 v = *chunk(r, e);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) bad |= (w[i] & kExp) == kExp || (w[i] >> 16 & kExp) == kExp;
-        }
+        for (int e = lane; e < 16 * C::NP; e += 32) bad |= bad_chunk<kBf16>(*value_chunk<C>(pairs, first_pair, r, e));
         if (!__any_sync(0xffffffffu, bad)) continue;
-        for (int e = lane; e < 16 * C::NP; e += 32) *chunk(r, e) = make_uint4(0, 0, 0, 0);
+        for (int e = lane; e < 16 * C::NP; e += 32) *value_chunk<C>(pairs, first_pair, r, e) = make_uint4(0, 0, 0, 0);
         if (lane < R / 8) *reinterpret_cast<uint4*>(rope + sw_rope<R>(r, lane)) = make_uint4(~0u, ~0u, ~0u, ~0u);
     }
 }
 
-// CAUSAL: a suffix launch of more than one token a row, whose last positions are masked for some of them. A
-// kernel of its own, because the other launches pay for code that they do not run (2,048 rows, 128 + 16 wide:
-// 62.6 us, in one kernel with it 64.0).
+// CAUSAL: a call of more than one token a row, whose last positions are masked for some of them in the suffix
+// launch. A kernel of its own, because the others pay for code that they do not run (2,048 rows, 128 + 16 wide:
+// 64.0 us in one kernel with it, 59.4 apart). Both launches of a call use the same one: a suffix launch
+// begins beside its prefix launch only where they are one kernel (143 rows of 4 tokens, e4m3: 22.7 us with
+// two kernels, 15.5).
 template <int KV, int R, int N, typename T, bool Q8, bool CAUSAL>
 __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N, Q8>::kCtas)
     shared_prefix_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap map_tile,
@@ -483,6 +486,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     float* base_s = up_s + N;        // the part of m that a tile's scores start from
     float* mail_s = base_s + N;      // [2][5][N] an item's sums (one row per softmax warp) and maxima
     float* fac_s = mail_s + 10 * N;  // [5][N]
+    float* over_s = reinterpret_cast<float*>(smem + C::oPlan - 16);  // [2] scores above it make a group look at its maxima
     int* plan_s = reinterpret_cast<int*>(smem + C::oPlan);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::oBar);
     uint64_t* q_empty = bars;                    // [QB] the item's S products have read Q
@@ -610,6 +614,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
     const lat::CacheView& cv = a.suffix ? p.suffix : p.prefix;
     bool ok = true;
     // a wait that ran out is recorded once; later waits of this thread are skipped
+    const bool causal = CAUSAL && a.suffix;  // the last positions are masked for some tokens
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (ok && !mbar_wait_bounded(bar, parity, nullptr)) {
             ok = false;
@@ -874,7 +879,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
         Ring<C::TS> ft;
         Ring<C::PS> fp;
         Ring<C::RS> fr;
-        int shown = 0;  // keys of the item that all of its queries see
+        int shown = 0x7fffffff;  // keys of the item that all of its queries see
         for (int base = 0; base < mine; base += kTcTable) {
             const int count = next_table(base, std::false_type());
             if (warp == kFenceWarp) {
@@ -883,7 +888,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 // that the O products still read are cleared first (a probability of zero times a NaN
                 // would be one).
                 for (Cursor c(table, count); c.valid(); c.next(), ft.next()) {
-                    if (CAUSAL && c.j == 0) {
+                    if (causal && c.j == 0) {
                         const Item& it = c.item();
                         shown = seen_by(p, suffix_length(p, it.row), it.q0 - it.row * th) - it.k0;
                     }
@@ -902,10 +907,13 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                         }
                     }
                     if constexpr (CAUSAL) {
-                        const int from = shown - c.j * KT, to = min(left, KT);
+                        const int to = min(left, KT), from = min(max(shown - c.j * KT, 0), to), chunks = (to - from) * 16 * C::NP;
+                        bool bad = false;
                         __syncwarp();
-                        if (from < to)
-                            drop_bad_rows<C, R, kBf16>(smem + C::oPair, fp.i, smem + C::oRope + fr.i * C::kRopeA, max(from, 0), to, lane);
+                        for (int e = lane; e < chunks; e += 32)
+                            bad |= bad_chunk<kBf16>(*value_chunk<C>(smem + C::oPair, fp.i, from + e / (16 * C::NP), e % (16 * C::NP)));
+                        if (__any_sync(0xffffffffu, bad))
+                            drop_bad_rows<C, R, kBf16>(smem + C::oPair, fp.i, smem + C::oRope + fr.i * C::kRopeA, from, to, lane);
                         fr.next();
                     }
                     fp.skip(C::NP);
@@ -965,18 +973,17 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                 for (int n = 0; n < NC; ++n) l[n] = 0.f;
                 // keys of the item each query sees; the tokens of a suffix end one position apart
                 soft_sync(group);  // the previous item's readers of m_s, lim_s and red_s are done
+                if (gt == 0) over_s[group] = kLift + kGrowth;
                 if (gt < NC) {
                     m_s[c0 + gt] = base_s[c0 + gt] = 0.f;
-                    if (CAUSAL) {
+                    if (causal) {
                         const int t = min((it.q0 + c0 + gt - it.row * th) / p.H, p.T - 1);
                         lim_s[c0 + gt] = min(it.nk, suffix_length(p, it.row) - (p.T - 1 - t) - it.k0);
                     }
                 }
                 soft_sync(group);
-                const int u0 = it.q0 - it.row * th;  // the tokens of the block end at most this far apart
-                const int lim_min = CAUSAL ? it.nk - ((u0 + it.nq - 1) / p.H - u0 / p.H) : it.nk;
+                const int lim_min = causal ? it.nk - a.apart : it.nk;
                 const float* ks_row = Q8 ? cv.scale + it.row * cv.scale_row_stride + it.k0 : nullptr;
-                bool far = false;  // a column's reference is not its base
                 float ks_next = 1.f;
                 if (Q8 && live && kt < it.nk) ks_next = __ldg(ks_row + kt);
                 for (int j = 0; j < it.nt; ++j, ++tile) {
@@ -1008,7 +1015,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s_free[sb]);
                     // scores relative to the column's reference, base 2; the first tile's reference is 0
-                    bool over = j == 0 || far;
+                    bool over = j == 0;
                     float top = -INFINITY;
 #pragma unroll
                     for (int n = 0; n < NC; n += 4) {
@@ -1019,7 +1026,7 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                         z[n + 3] = fmaf(z[n + 3], cs, -m.w);
                     }
                     if ((j + 1) * KT > lim_min) {  // the last tile(s): keys past a query's limit
-                        if (CAUSAL) {
+                        if (causal) {
 #pragma unroll
                             for (int n = 0; n < NC; ++n)
                                 if (key >= lim_s[c0 + n]) z[n] = -INFINITY;
@@ -1035,13 +1042,32 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
 #pragma unroll
                     for (int n = 0; n < NC; ++n) top = fmaxf(top, z[n]);
                     if (Q8) top += scale_exponent(ks);
-                    over |= top > kLift + kGrowth;
+                    over |= top > over_s[group];
                     if (soft_any(group, over)) {
-                        float x[NC];
+                        auto larger = [](float u, float w) { return fmaxf(u, w); };
+                        int own;
+                        float most;
+                        if constexpr (Q8) {
+                            // the first step here: its lanes have exponents of their own, and values with
+                            // them beside the scores would not fit the registers
+                            float x[NC / 2];
+                            const bool up = lane & 16;
+                            const float te = scale_exponent(ks), to = __shfl_xor_sync(0xffffffffu, te, 16);
 #pragma unroll
-                        for (int n = 0; n < NC; ++n) x[n] = Q8 ? z[n] + scale_exponent(ks) : z[n];
-                        const int own = fold_columns(x, lane, [](float u, float w) { return fmaxf(u, w); });
-                        if (NC == 32 || (lane & 1) == 0) red_s[gw * N + c0 + own] = x[0];
+                            for (int n = 0; n < NC / 2; ++n) {
+                                const float got = __shfl_xor_sync(0xffffffffu, up ? z[n] : z[n + NC / 2], 16);
+                                x[n] = fmaxf((up ? z[n + NC / 2] : z[n]) + te, got + to);
+                            }
+                            own = (up ? NC / 2 : 0) + fold_columns<8>(x, lane, larger);
+                            most = x[0];
+                        } else {
+                            float x[NC];
+#pragma unroll
+                            for (int n = 0; n < NC; ++n) x[n] = z[n];
+                            own = fold_columns(x, lane, larger);
+                            most = x[0];
+                        }
+                        if (NC == 32 || (lane & 1) == 0) red_s[gw * N + c0 + own] = most;
                         soft_sync(group);
                         if (gt < NC) {
                             // every column that sees a key of the item sees one in its first tile: there
@@ -1052,15 +1078,17 @@ __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N,
                             const float old = m_s[n], from = base_s[n];
                             float m = old;
                             if (j == 0 ? top_n > -INFINITY : (from - old) + top_n > kLift + kGrowth) m = from + (top_n - kLift);
-                            else if (j == 0 && !(CAUSAL && lim_s[n] <= 0)) m = kNoMax;
+                            else if (j == 0 && !(causal && lim_s[n] <= 0)) m = kNoMax;
                             corr_s[n] = fast_exp2(old - m);
                             up_s[n] = m - from;
                             m_s[n] = m;
                             // scores relative to a large reference (keys masked by the lowest value, say) would
                             // lose the digits of what comes after it: from there on every tile starts from 0
-                            base_s[n] = fabsf(m) <= kNear ? m : 0.f;
+                            const bool near = fabsf(m) <= kNear;
+                            base_s[n] = near ? m : 0.f;
+                            if (!near) over_s[group] = -INFINITY;
                         }
-                        far = soft_any(group, gt < NC && !(fabsf(m_s[c0 + (gt & (NC - 1))]) <= kNear));
+                        soft_sync(group);
 #pragma unroll
                         for (int n = 0; n < NC; ++n) z[n] -= up_s[c0 + n];
                         if (j > 0) {
@@ -1292,10 +1320,10 @@ __global__ void __launch_bounds__(256) shared_prefix_join_kernel(const Problem p
                                                                  int direct, const int2* __restrict__ pieces) {
     MM_PDL_ENTRY();
     const int th = p.T * p.H, lane = threadIdx.x & 31;
-    const long long rows = static_cast<long long>(p.B) * th;
+    const long long rows = static_cast<long long>(p.B) * th;  // below 2^31
     const long long r = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
     if (r >= rows) return;
-    const int b = static_cast<int>(r / th);
+    const int b = static_cast<int>(r) / th, u = static_cast<int>(r) - b * th;
     int first = 0, ns;
     if constexpr (PIECES) {  // the parts of a row cut between CTAs
         const int2 v = __ldcg(&pieces[b]);
@@ -1306,7 +1334,6 @@ __global__ void __launch_bounds__(256) shared_prefix_join_kernel(const Problem p
         if (direct && direct_join(p, b, suf_kps, pre_kps) >= 0) return;  // the suffix launch wrote it
         int len = suffix_length(p, b);
         if (!direct) {  // blocks of 64 queries end where their last one does
-            const int u = static_cast<int>(r - static_cast<long long>(b) * th);
             len = seen_by(p, len, min((u / 64 + 1) * 64, th) - 1);
         }
         ns = (len + suf_kps - 1) / suf_kps;
@@ -1314,7 +1341,7 @@ __global__ void __launch_bounds__(256) shared_prefix_join_kernel(const Problem p
     const int g = p.G > 0 ? group_of(p, b) : -1;
     const int np = (prefix_length(p, g) + pre_kps - 1) / pre_kps;
     auto suf_at = [&](int s) {  // the query row of suffix part s among the partials
-        if constexpr (PIECES) return (2LL * (first + s) + (s == 0)) * 16 + (r - static_cast<long long>(b) * th);
+        if constexpr (PIECES) return (2LL * (first + s) + (s == 0)) * 16 + u;
         else return s * rows + r;
     };
     auto ml = [&](int s) { return s < np ? __ldcg(&pre_ml[s * rows + r]) : __ldcg(&suf_ml[suf_at(s - np)]); };
