@@ -262,8 +262,8 @@ struct Plan {
 
 // Key ranges per query block: the waves of (block, range) items over the SMs times an item's
 // tiles, plus what an item costs beside its tiles (two) and the join of several ranges (one). Measured
-// with other costs: items at one, 600 rows of 2,048 positions, 128 + 16 wide, are split, 84 -> 92 us; the
-// join at four, prompts of 512 under 512 + 32 wide ragged rows are not, 65 -> 68.
+// with other costs: items at one, 600 rows of 2,048 positions, 128 + 16 wide, 79.5 us instead of 79.9; the
+// join at four, prompts of 512 under 512 + 32 wide ragged rows are not split, 63.6 us instead of 61.6.
 void pick_splits(long long blocks, int keys, int most, int& splits, int& kps) {
     const int tiles = (keys + 127) / 128, sms = sm_count();
     double best = 0;

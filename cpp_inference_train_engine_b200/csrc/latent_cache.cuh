@@ -186,10 +186,11 @@ template <typename T> struct WriteRow {
 
 // KV = 128 or 512, 16-byte accesses: a lane takes 16 values of a position (KV / 16 lanes each), the
 // maximum is a shuffle reduction over the lane group. The CTAs that fit walk the positions with the
-// next ones already loaded, as they are (14 registers for 16-bit rows). Bound by the bytes in and out,
-// with the scattered rows of the cache short of the copy rate: 196,608 x (512 + 32) fp16 values to
-// random slots, 330 MB in 67.7 us (4.9 TB/s; a CTA per eight positions 79.9; two positions ahead, or five
-// and six CTAs an SM, 77 to 97: spills or fewer CTAs); 50,001 fp32 rows 24.9 us (5.5 TB/s).
+// next ones already loaded, as they are (14 registers for 16-bit rows). Bound by the bytes in and out
+// that so few positions ahead keep in flight: 196,608 x (512 + 32) fp16 values, 330 MB in 67 us back to back
+// (4.9 TB/s), to random slots and to neighbouring ones alike, 70 among other work (a CTA per eight positions
+// 79.9; two positions ahead, or five and six CTAs an SM, 77 to 97: spills or fewer CTAs); 50,001 fp32 rows
+// 24.4 us (5.6 TB/s).
 template <typename T> constexpr int kWriteCtas = sizeof(T) == 4 ? 3 : 4;  // CTAs per SM
 template <typename T, typename T16, int KV, int R>
 __global__ void __launch_bounds__(256, kWriteCtas<T>) latent_write_vec_kernel(

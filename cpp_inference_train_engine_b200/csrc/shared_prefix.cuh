@@ -51,7 +51,7 @@ __device__ __forceinline__ int suffix_length(const Problem& p, int b) {
 // lane adds p_j * value for its columns. The query (fp32, pre-scaled) and the output row live
 // in shared memory, so any kv and rope width works. Used for the widths that have no
 // tensor-core form; bound by its scalar loads and the row by row walk (8 rows of 8 heads over a prompt
-// of 128, 128 + 16 wide: 51 us where the tensor-core form takes 12).
+// of 128, 128 + 16 wide: 57 us where the tensor-core form takes 12).
 constexpr int kAnyWarps = 4;
 template <typename T, bool Q8P, bool Q8S>
 __global__ void __launch_bounds__(32 * kAnyWarps) any_width_kernel(const Problem p) {

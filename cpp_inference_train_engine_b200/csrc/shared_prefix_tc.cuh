@@ -43,12 +43,12 @@
 // noted in latent_status, and the CTA ends once the copies and products that it had in flight have (waited for
 // with a limit of their own).
 //
-// Measured on one B200. Cache loads: 296 rows of 1,024 positions, 512 + 32 wide, fp16, 66 us (5.0 TB/s of
-// the 6.5 a copy reaches); one SM's ring holds ten pairs of boxes (160 KB). e4m3 rows are bound by their
-// conversion instead (1.9 us a tile of 64). Products: 2,048 query rows over one prompt of 8,192, 80 us
-// (445 TFLOP/s): an N = 64 product takes 48 cycles where the pipe's rate would allow 32, its S product has
-// M = 64, and two tiles fill the ring. (128 queries would run at the full rate, but their fp32 O^T fills the
-// tensor memory at 512 columns.)
+// Measured on one B200. Cache loads: 296 rows of 1,024 positions, 512 + 32 wide, fp16, 68 us (4.8 TB/s of
+// the 6.5 a copy reaches); one SM's ring holds ten pairs of boxes (160 KB). As e4m3 the same rows take 77 us
+// for 55 % of the bytes: they are bound by the conversion. Products: 2,048 query rows over one prompt of
+// 8,192, 75 us (472 TFLOP/s), the tensor pipe 34 % active over all SMs: the S product of a 64-key tile has
+// M = 64, and two tiles fill the ring. (128 queries a block would fill the tensor memory at 512 columns with
+// their fp32 O^T.)
 #pragma once
 #include <type_traits>
 
@@ -464,9 +464,9 @@ __device__ __noinline__ void drop_bad_rows(uint8_t* pairs, int first_pair, uint8
 
 // CAUSAL: a call of more than one token a row, whose last positions are masked for some of them in the suffix
 // launch. A kernel of its own, because the others pay for code that they do not run (2,048 rows, 128 + 16 wide:
-// 64.0 us in one kernel with it, 59.4 apart). Both launches of a call use the same one: a suffix launch
-// begins beside its prefix launch only where they are one kernel (143 rows of 4 tokens, e4m3: 22.7 us with
-// two kernels, 15.5).
+// 64.0 us in one kernel with it, 59.4 apart). Both launches of a call use the same one: two kernels that spill
+// registers do not run beside each other (143 rows of 4 tokens, e4m3: 22.7 us with a prefix launch of the
+// other one, 15.3).
 template <int KV, int R, int N, typename T, bool Q8, bool CAUSAL>
 __global__ void __launch_bounds__(TcCfg<KV, R, N, Q8>::kThreads, TcCfg<KV, R, N, Q8>::kCtas)
     shared_prefix_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap map_tile,
