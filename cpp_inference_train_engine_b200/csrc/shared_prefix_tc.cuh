@@ -452,7 +452,7 @@ template <class C> __device__ __forceinline__ uint4* value_chunk(uint8_t* pairs,
     return reinterpret_cast<uint4*>(pairs + pair * C::kPair + ((e >> 3) & 1) * C::kBox + sw128(r, e & 7));
 }
 template <class C, int R, bool kBf16>
-__device__ __noinline__ void drop_bad_rows(uint8_t* pairs, int first_pair, uint8_t* rope, int from, int to, int lane) {
+__device__ __forceinline__ void drop_bad_rows(uint8_t* pairs, int first_pair, uint8_t* rope, int from, int to, int lane) {
     for (int r = from; r < to; ++r) {
         bool bad = false;
         for (int e = lane; e < 16 * C::NP; e += 32) bad |= bad_chunk<kBf16>(*value_chunk<C>(pairs, first_pair, r, e));
