@@ -1,7 +1,7 @@
 """Builds the sm_100a backend in place: cpp_inference_train_engine_b200/libmm_cuda.so, from its
-two translation units (the engine and the latent-cache operators), and after it _latent_torch.so,
-the binding of the latter to torch tensors, where a torch with CUDA can be imported (the library
-needs none).
+three translation units (the engine, the latent-cache operators and those of paged caches), and after it
+_latent_torch.so, the binding of the operators to torch tensors, where a torch with CUDA can be imported
+(the library needs none).
 
     python -m cpp_inference_train_engine_b200.build
 
@@ -16,9 +16,9 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SRC = [os.path.join(HERE, "csrc", f) for f in ("mm_cuda.cu", "latent.cu")]
+SRC = [os.path.join(HERE, "csrc", f) for f in ("mm_cuda.cu", "latent.cu", "paged.cu")]
 OUT = os.path.join(HERE, "libmm_cuda.so")
-TORCH_SRC = os.path.join(HERE, "csrc", "latent_torch.cpp")
+TORCH_SRC = [os.path.join(HERE, "csrc", f) for f in ("latent_torch.cpp", "paged_torch.cpp")]
 TORCH_OUT = os.path.join(HERE, "_latent_torch.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -50,7 +50,7 @@ def torch_command():
     includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                 sysconfig.get_paths()["include"], cuda]
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
-            *[f"-isystem{i}" for i in includes], TORCH_SRC, "-o", TORCH_OUT + ".tmp", f"-L{HERE}", "-l:libmm_cuda.so",
+            *[f"-isystem{i}" for i in includes], *TORCH_SRC, "-o", TORCH_OUT + ".tmp", f"-L{HERE}", "-l:libmm_cuda.so",
             f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
             "-Wl,-rpath,$ORIGIN"]
 
@@ -72,7 +72,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
     if force or not up_to_date(OUT):
         _run([NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr",
               "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", "-Xptxas", "-warn-spills",
-              "-t", "2", "-I", os.path.join(ROOT, "include"), *SRC, "-o", OUT + ".tmp", "-ldl", "-lpthread"], OUT, verbose)
+              "-t", "3", "-I", os.path.join(ROOT, "include"), *SRC, "-o", OUT + ".tmp", "-ldl", "-lpthread"], OUT, verbose)
     if force or not up_to_date(TORCH_OUT):
         try:
             command = torch_command()

@@ -1,0 +1,212 @@
+// C entries of the paged-cache and beam-search operators (include/mm_paged.h): argument checks,
+// variant selection and launches. Everything is enqueued on the caller's stream; no entry
+// allocates or throws, and none but mm_paged_status waits.
+#include <algorithm>
+#include <cmath>
+
+#include "beam_select.cuh"
+#include "entries.cuh"
+#include "paged_attention.cuh"
+#include "paged_cache.cuh"
+
+#include "../../include/mm_paged.h"
+
+using namespace mm::entry;
+
+namespace {
+
+static_assert(sizeof(mm_paged_cache) == 112 && sizeof(mm_paged_attention_desc) == 80, "callers without this header pack these field by field");
+
+mm::paged::Table table_of(const mm_paged_cache* c) {
+    return {c->table, c->table_stride, c->table_rows, c->table_columns};
+}
+
+void check_paged(const mm_paged_cache* c) {
+    require(c != nullptr, "paged cache: null description");
+    check_cache(&c->pool);
+    require(c->pool.positions >= 1, "paged cache: a page holds one position or more");
+    require(c->table_rows >= 0 && c->table_columns >= 0, "paged cache: negative size");
+    require(static_cast<long long>(c->table_columns) * c->pool.positions <= INT32_MAX, "paged cache: a row's positions exceed 32 bits");
+    require((c->table && multiple(c->table, 4)) || c->table_rows == 0 || c->table_columns == 0, "paged cache: null or misaligned table");
+}
+
+mm::lat::CacheOut out_view(const mm_latent_cache* c) {
+    return {static_cast<uint8_t*>(c->latent), static_cast<uint8_t*>(c->rope), c->scale, c->row_stride, c->pos_stride,
+            c->rope_row_stride, c->rope_pos_stride, c->scale_row_stride, c->rows, c->positions};
+}
+
+mm::paged::Attention problem(const mm_paged_attention_desc* d, const mm_paged_cache* c) {
+    require(d != nullptr, "null description");
+    check_paged(c);
+    require(d->rows >= 0 && d->heads >= 1 && d->rows <= kMaxBlocks / d->heads, "paged attention: invalid sizes");
+    require(d->dtype == MM_F16 || d->dtype == MM_BF16, "paged attention: q must be fp16 or bf16");
+    const int kind = c->pool.kind == MM_E4M3 ? c->pool.rope_kind : c->pool.kind;
+    require(kind == d->dtype, "paged attention: the cache's type must be q's (an e4m3 cache's rope type)");
+    require(d->rows <= c->table_rows, "paged attention: a table row per row");
+    require(d->window >= 0 && d->sinks >= 0, "paged attention: negative window or sinks");
+    require(d->max_length >= 0 && d->max_length <= static_cast<long long>(c->table_columns) * c->pool.positions,
+            "paged attention: max_length exceeds the table");
+    if (d->rows > 0) {
+        require(d->q && d->out, "paged attention: null q or out");
+        require(multiple(d->q, 2) && multiple(d->out, 2) && multiple(d->lse, 4) && multiple(d->lengths, 4),
+                "paged attention: q, out, lse or lengths not aligned to its elements");
+        require(d->lengths || d->max_length == 0, "paged attention: null lengths");
+    }
+    mm::paged::Attention p{};
+    p.q = d->q;
+    p.q_row = d->q_row_stride;
+    p.q_head = d->q_head_stride;
+    p.B = d->rows;
+    p.H = d->heads;
+    p.pool = view(&c->pool);
+    p.table = table_of(c);
+    p.lengths = d->lengths;
+    p.max_length = d->max_length;
+    p.window = d->window;
+    p.sinks = d->window > 0 ? d->sinks : 0;
+    p.kv = c->pool.kv;
+    p.rd = c->pool.rope_dim;
+    p.scale = d->scale;
+    p.out = d->out;
+    p.lse = d->lse;
+    return p;
+}
+
+template <typename T, bool Q8> void launch_any_width(const mm::paged::Attention& p, cudaStream_t s) {
+    using namespace mm::paged;
+    const int smem = kAnyWarps * (2 * p.kv + p.rd) * 4;  // at most 36 KB
+    launch(s, any_width_kernel<T, Q8>, dim3(blocks(static_cast<long long>(p.B) * p.H, kAnyWarps)), dim3(32 * kAnyWarps), smem, p);
+}
+
+void check_select(int batch, int beams, int vocab, int count) {
+    require(batch >= 0 && beams >= 1 && vocab >= 1 && count >= 1, "beam selection: invalid sizes");
+    if (beams > mm::beam::kMaxBeams || count > mm::beam::kMaxBeams) refuse(MM_UNSUPPORTED, "beam selection: more than 32 beams");
+    if (vocab > mm::beam::kMaxVocab) refuse(MM_UNSUPPORTED, "beam selection: vocabulary over 1,048,576");
+}
+
+}  // namespace
+
+extern "C" {
+
+int mm_paged_status(void* stream) {
+    return guarded([&] {
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        int bits = 0;
+        const int none = 0;
+        check(cudaMemcpyFromSymbolAsync(&bits, mm::paged::paged_status, sizeof bits, 0, cudaMemcpyDeviceToHost, s), "status");
+        check(cudaStreamSynchronize(s), "status");
+        if (!bits) return;
+        check(cudaMemcpyToSymbolAsync(mm::paged::paged_status, &none, sizeof none, 0, cudaMemcpyHostToDevice, s), "status");
+        check(cudaStreamSynchronize(s), "status");
+        refuse(MM_GPU_ERROR, "paged attention: a kernel gave up on a wait; its results are NaN");
+    });
+}
+
+int mm_paged_append(const mm_paged_cache* cache, const void* values, int64_t values_stride, int dtype, const int32_t* rows,
+                    const int32_t* positions, int64_t n, double theta, const float* norm, float eps, void* stream) {
+    return guarded([&] {
+        check_paged(cache);
+        require(n >= 0 && (rows || n <= INT32_MAX), "paged append: invalid count");
+        require(cache->pool.rope_dim % 2 == 0, "paged append: rope_dim must be even");
+        require(theta > 0 && std::isfinite(theta) && (!norm || eps >= 0), "paged append: theta must be positive and eps not negative");
+        if (n == 0 || cache->pool.rows == 0 || cache->table_rows == 0 || cache->table_columns == 0) return;
+        require(values && positions, "paged append: null input");
+        require(multiple(positions, 4) && multiple(rows, 4) && multiple(norm, 4), "paged append: input not aligned to its elements");
+        mm::paged::Rotation rot;
+        for (int j = 0; j < cache->pool.rope_dim / 2; ++j)
+            rot.f[j] = std::pow(theta, -2.0 * j / cache->pool.rope_dim) / 6.283185307179586476925;
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        const bool q8 = cache->pool.kind == MM_E4M3;
+        with_type(dtype, [&](auto in) {
+            with_half(q8 ? cache->pool.rope_kind : cache->pool.kind, [&](auto half) {
+                using T = typename decltype(in)::type;
+                using T16 = typename decltype(half)::type;
+                require(multiple(values, sizeof(T)), "paged append: input not aligned to its elements");
+                launch(s, q8 ? mm::paged::append_kernel<T, T16, true> : mm::paged::append_kernel<T, T16, false>, dim3(blocks(n, 8)),
+                       dim3(256), 0, out_view(&cache->pool), table_of(cache), static_cast<const T*>(values),
+                       static_cast<long long>(values_stride), rows, positions, static_cast<long long>(n), cache->pool.kv,
+                       cache->pool.rope_dim, norm, eps, rot);
+            });
+        });
+    });
+}
+
+int64_t mm_paged_attention_workspace(const mm_paged_attention_desc* desc, const mm_paged_cache* cache) {
+    int64_t bytes = 0;
+    const int rc = guarded([&] { problem(desc, cache); });
+    return rc ? -static_cast<int64_t>(rc) : bytes;
+}
+
+int mm_paged_attention(const mm_paged_attention_desc* desc, const mm_paged_cache* cache, void*, size_t, void* stream) {
+    return guarded([&] {
+        const mm::paged::Attention p = problem(desc, cache);
+        if (p.B == 0) return;
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        with_half(desc->dtype, [&](auto half) {
+            using T = typename decltype(half)::type;
+            if (cache->pool.kind == MM_E4M3) launch_any_width<T, true>(p, s);
+            else launch_any_width<T, false>(p, s);
+        });
+    });
+}
+
+int64_t mm_beam_select_workspace(int batch, int beams, int vocab, int count) {
+    const int rc = guarded([&] { check_select(batch, beams, vocab, count); });
+    return rc ? -static_cast<int64_t>(rc) : 0;
+}
+
+int mm_beam_select(const void* logits, int64_t batch_stride, int64_t beam_stride, int dtype, const float* scores,
+                   const uint8_t* finished, int eos, int batch, int beams, int vocab, int count, float* out_scores,
+                   int32_t* out_parents, int32_t* out_tokens, void*, size_t, void* stream) {
+    return guarded([&] {
+        check_select(batch, beams, vocab, count);
+        require(!finished || (eos >= 0 && eos < vocab), "beam selection: eos must be in the vocabulary");
+        if (batch == 0) return;
+        require(logits && scores && out_scores && out_parents && out_tokens, "beam selection: null argument");
+        require(multiple(scores, 4) && multiple(out_scores, 4) && multiple(out_parents, 4) && multiple(out_tokens, 4),
+                "beam selection: argument not aligned to its elements");
+        mm::beam::Select a{logits, batch_stride, beam_stride, scores, finished, eos, batch, beams, vocab, count,
+                           out_scores, out_parents, out_tokens};
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        with_type(dtype, [&](auto t) {
+            using T = typename decltype(t)::type;
+            require(multiple(logits, sizeof(T)), "beam selection: logits not aligned to their elements");
+            launch(s, mm::beam::select_kernel<T>, dim3(batch), dim3(256), 0, a);
+        });
+    });
+}
+
+int mm_beam_reorder(const mm_paged_cache* cache, int layers, const int64_t layer_strides[3], const int32_t* spare,
+                    const int32_t* lengths, const int32_t* parents, int32_t* out_table, int32_t* out_spare,
+                    int32_t* out_lengths, void* stream) {
+    return guarded([&] {
+        check_paged(cache);
+        require(layers >= 0 && layer_strides, "beam reorder: invalid layers");
+        const mm_latent_cache& c = cache->pool;
+        const int rows = cache->table_rows;
+        if (rows == 0) return;
+        require(cache->table_columns >= 1, "beam reorder: a table of no pages");
+        require(spare && lengths && parents && out_table && out_spare && out_lengths, "beam reorder: null argument");
+        for (const int32_t* x : {spare, lengths, parents, const_cast<const int32_t*>(out_table), const_cast<const int32_t*>(out_spare),
+                                 const_cast<const int32_t*>(out_lengths)})
+            require(multiple(x, 4), "beam reorder: argument not aligned to its elements");
+        const bool q8 = c.kind == MM_E4M3;
+        mm::paged::Reorder a{table_of(cache), spare, lengths, parents, out_table, out_spare, out_lengths, c.positions,
+                             c.rows, layers, {}};
+        auto plane = [](void* data, int64_t layer, int64_t page, int64_t position, int n, int size) {
+            return mm::paged::Plane{static_cast<uint8_t*>(data), static_cast<long long>(layer * size),
+                                    static_cast<long long>(page * size), static_cast<long long>(position * size), n * size};
+        };
+        if (q8) {
+            a.plane[0] = plane(c.latent, layer_strides[0], c.row_stride, c.pos_stride, c.kv, 1);
+            a.plane[1] = plane(c.rope, layer_strides[1], c.rope_row_stride, c.rope_pos_stride, c.rope_dim, 2);
+            a.plane[2] = plane(c.scale, layer_strides[2], c.scale_row_stride, 1, 1, 4);
+        } else {
+            a.plane[0] = plane(c.latent, layer_strides[0], c.row_stride, c.pos_stride, c.kv + c.rope_dim, 2);
+        }
+        launch(static_cast<cudaStream_t>(stream), mm::paged::reorder_kernel<uint8_t>,
+               dim3(static_cast<unsigned>(rows), static_cast<unsigned>(std::min(std::max(layers, 1), 64))), dim3(256), 0, a);
+    });
+}
+
+}  // extern "C"

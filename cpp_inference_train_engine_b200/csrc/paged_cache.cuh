@@ -1,0 +1,163 @@
+// A latent cache in pages: appending positions through a page table (normalised, rotated, in 8 or 16
+// bits) and page tables that follow a beam search's parents.
+#pragma once
+#include "latent_cache.cuh"
+
+namespace mm {
+namespace paged {
+
+struct Table {
+    const int* entry;
+    long long stride;
+    int rows, columns;
+};
+
+// The pool's page of position t of table row r, or -1 (a position or a page that is not there); at: the entry.
+__device__ __forceinline__ int page_of(const Table& t, int pages, int page, int row, int position, int& at) {
+    if (row < 0 || row >= t.rows || position < 0) return -1;
+    const int column = position / page;
+    if (column >= t.columns) return -1;
+    at = position - column * page;
+    const int p = __ldg(t.entry + row * t.stride + column);
+    return p >= 0 && p < pages ? p : -1;
+}
+
+// Pair j's angle at `position` in turns: f = theta^(-2 j / width) / (2 pi) in fp64, whose product with any
+// 31-bit position is off by less than 2^-22 turns of the exact one only through f itself (2^31 * 2^-54);
+// the fraction goes on in fp32 (2^-25 turns, below a 16-bit key's rounding).
+__device__ __forceinline__ void rotation(double f, int position, float& sin_t, float& cos_t) {
+    const double turns = f * position;
+    sincospif(2.f * static_cast<float>(turns - rint(turns)), &sin_t, &cos_t);
+}
+
+constexpr int kMaxPairs = 128;  // of a rope key of 256
+struct Rotation {
+    double f[kMaxPairs];
+};
+
+// ------------------------------------------------------------------ append
+// Any width, stride and alignment: one warp per token. The widths of the framework's models run on
+// append_vec_kernel.
+template <typename T, typename T16, bool Q8>
+__global__ void __launch_bounds__(256) append_kernel(lat::CacheOut c, Table table, const T* __restrict__ values,
+                                                     long long stride, const int* __restrict__ rows,
+                                                     const int* __restrict__ positions, long long n, int kv, int rd,
+                                                     const float* __restrict__ norm, float eps,
+                                                     const __grid_constant__ Rotation rot) {
+    MM_PDL_ENTRY();
+    const long long i = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+    const int lane = threadIdx.x & 31;
+    if (i >= n) return;
+    const int position = positions[i];
+    int at = 0;
+    const long long p = page_of(table, c.rows, c.positions, rows ? rows[i] : static_cast<int>(i), position, at);
+    if (p < 0) return;
+    const T* x = values + i * stride;
+    float inv = 1.f;
+    if (norm) {
+        float sum = 0.f;
+        for (int k = lane; k < kv; k += 32) {
+            const float v = lat::to_f32(x[k]);
+            sum = fmaf(v, v, sum);
+        }
+        inv = rsqrtf(warp_sum(sum) / kv + eps);
+    }
+    auto value = [&](int k) { return norm ? lat::to_f32(x[k]) * inv * norm[k] : lat::to_f32(x[k]); };
+    T16* key;
+    if constexpr (Q8) {
+        float mx = 0.f;
+        for (int k = lane; k < kv; k += 32) mx = fmaxf(mx, fabsf(value(k)));
+        const float s = fmaxf(__fdiv_rn(warp_max(mx), lat::kE4m3Max), lat::kScaleFloor);
+        uint8_t* dst = c.latent + p * c.row_stride + at * c.pos_stride;
+        for (int k = lane; k < kv; k += 32) dst[k] = __nv_cvt_float_to_fp8(__fdiv_rn(value(k), s), __NV_SATFINITE, __NV_E4M3);
+        if (lane == 0) c.scale[p * c.scale_row_stride + at] = s;
+        key = reinterpret_cast<T16*>(c.rope) + p * c.rope_row_stride + at * c.rope_pos_stride;
+    } else {
+        T16* dst = reinterpret_cast<T16*>(c.latent) + p * c.row_stride + at * c.pos_stride;
+        for (int k = lane; k < kv; k += 32) dst[k] = lat::from_f32<T16>(value(k));
+        key = dst + kv;
+    }
+    for (int j = lane; j < rd / 2; j += 32) {
+        float sn, cs;
+        rotation(rot.f[j], position, sn, cs);
+        const float a = lat::to_f32(x[kv + 2 * j]), b = lat::to_f32(x[kv + 2 * j + 1]);
+        key[2 * j] = lat::from_f32<T16>(a * cs - b * sn);
+        key[2 * j + 1] = lat::from_f32<T16>(a * sn + b * cs);
+    }
+}
+
+// ------------------------------------------------------------------ reorder
+// One array of the pool (latent, rope keys or scales) as bytes.
+struct Plane {
+    uint8_t* data;
+    long long layer, page, position;  // strides in bytes
+    int bytes;                        // of a position
+};
+struct Reorder {
+    Table table;
+    const int* spare;
+    const int* lengths;
+    const int* parents;
+    int* out_table;
+    int* out_spare;
+    int* out_lengths;
+    int page, pages, layers;
+    Plane plane[3];
+};
+
+struct Move {
+    int parent, full, part;  // the parent's full pages and the positions of its last one
+    int from, to;            // pages of the copy; part == 0: none
+};
+__device__ __forceinline__ int length_of(const Reorder& a, int row) {
+    return static_cast<int>(min(max(static_cast<long long>(a.lengths[row]), 0LL), static_cast<long long>(a.table.columns) * a.page));
+}
+__device__ __forceinline__ Move move_of(const Reorder& a, int row) {
+    Move m;
+    m.parent = a.parents[row];
+    if (m.parent < 0 || m.parent >= a.table.rows) m.parent = row;
+    const int n = length_of(a, m.parent);
+    m.full = n / a.page;
+    m.part = m.parent == row ? 0 : n - m.full * a.page;
+    m.from = m.to = -1;
+    if (m.part > 0) {
+        m.from = a.table.entry[m.parent * a.table.stride + m.full];
+        m.to = a.spare[row];
+    }
+    return m;
+}
+
+// Block (row, layer group): copies the row's tail in the layers blockIdx.y, blockIdx.y + gridDim.y, ...;
+// the first group's block writes the row's table entries. VEC bytes an access.
+template <typename V>
+__global__ void __launch_bounds__(256) reorder_kernel(const Reorder a) {
+    MM_PDL_ENTRY();
+    const int row = blockIdx.x, tid = threadIdx.x;
+    const Move m = move_of(a, row);
+    if (blockIdx.y == 0) {
+        const int own = m.part > 0 ? min(length_of(a, row) / a.page, a.table.columns - 1) : 0;
+        for (int j = tid; j < a.table.columns; j += blockDim.x)
+            a.out_table[static_cast<long long>(row) * a.table.columns + j] =
+                m.part > 0 && j == m.full ? m.to : a.table.entry[(j < m.full ? m.parent : row) * a.table.stride + j];
+        if (tid == 0) {
+            a.out_spare[row] = m.part > 0 ? a.table.entry[row * a.table.stride + own] : a.spare[row];
+            a.out_lengths[row] = length_of(a, m.parent);
+        }
+    }
+    if (m.part == 0 || m.from < 0 || m.from >= a.pages || m.to < 0 || m.to >= a.pages || m.from == m.to) return;
+    for (int l = blockIdx.y; l < a.layers; l += gridDim.y)
+        for (int q = 0; q < 3; ++q) {
+            const Plane& p = a.plane[q];
+            const int per = p.bytes / static_cast<int>(sizeof(V));
+            const uint8_t* src = p.data + l * p.layer + m.from * p.page;
+            uint8_t* dst = p.data + l * p.layer + m.to * p.page;
+            for (int e = tid; e < m.part * per; e += blockDim.x) {
+                const int t = e / per;
+                const long long off = t * p.position + (e - t * per) * static_cast<long long>(sizeof(V));
+                *reinterpret_cast<V*>(dst + off) = *reinterpret_cast<const V*>(src + off);
+            }
+        }
+}
+
+}  // namespace paged
+}  // namespace mm
