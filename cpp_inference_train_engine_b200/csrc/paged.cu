@@ -7,6 +7,7 @@
 #include "beam_select.cuh"
 #include "entries.cuh"
 #include "paged_attention.cuh"
+#include "paged_attention_mma.cuh"
 #include "paged_cache.cuh"
 
 #include "../../include/mm_paged.h"
@@ -78,6 +79,100 @@ template <typename T, bool Q8> void launch_any_width(const mm::paged::Attention&
     launch(s, any_width_kernel<T, Q8>, dim3(blocks(static_cast<long long>(p.B) * p.H, kAnyWarps)), dim3(32 * kAnyWarps), smem, p);
 }
 
+// ------------------------------------------------------------------ tensor-core form of attention
+// The models' two widths, pages of whole boxes of 16 positions, and what tensor maps and the kernel's 8-byte
+// loads of q take.
+bool mma_form(const mm::paged::Attention& p, const mm_latent_cache& c) {
+    if (!((p.kv == 128 && p.rd == 16) || (p.kv == 512 && p.rd == 32)) || c.positions % 16 || c.rows == 0 || p.max_length == 0) return false;
+    if (!multiple(p.q, 8) || p.q_row % 4 || p.q_head % 4 || !multiple(p.out, 8)) return false;
+    constexpr int64_t kMost = 1LL << 39;  // strides of up to 40 bits in bytes
+    auto strides = [&](const void* base, int64_t page, int64_t position, int size) {
+        return multiple(base, 16) && position > 0 && position < kMost && position * size % 16 == 0 &&
+               (c.rows == 1 || (page > 0 && page < kMost && page * size % 16 == 0));
+    };
+    if (c.kind != MM_E4M3) return strides(c.latent, c.row_stride, c.pos_stride, 2);
+    return strides(c.latent, c.row_stride, c.pos_stride, 1) && strides(c.rope, c.rope_row_stride, c.rope_pos_stride, 2) &&
+           strides(c.scale, c.scale_row_stride, 4, 4);
+}
+
+// Boxes of `width` columns x `box` positions of a page of one of the pool's arrays (its scales: of `box`
+// positions). False where the encoder does not take the strides.
+bool pool_map(CUtensorMap* map, CUtensorMapDataType type, int size, const mm_latent_cache& c, const void* base, int columns,
+              int64_t page_stride, int64_t position_stride, int width, int box, CUtensorMapSwizzle swizzle) {
+    if (c.rows == 1) page_stride = std::max<int64_t>(page_stride, 16 * position_stride);  // any: there is one
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(c.positions), static_cast<cuuint64_t>(c.rows)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(position_stride) * size, static_cast<cuuint64_t>(page_stride) * size};
+    const cuuint32_t boxes[3] = {static_cast<cuuint32_t>(width), static_cast<cuuint32_t>(box), 1}, steps[3] = {1, 1, 1};
+    return tensor_map_encoder()(map, type, 3, const_cast<void*>(base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool scale_map(CUtensorMap* map, const mm_latent_cache& c, int box) {
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(c.positions), static_cast<cuuint64_t>(c.rows)};
+    const cuuint64_t stride = static_cast<cuuint64_t>(c.rows == 1 ? std::max<int64_t>(c.scale_row_stride, 16) & ~3LL : c.scale_row_stride) * 4;
+    const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(box), 1}, steps[2] = {1, 1};
+    return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, c.scale, dims, &stride, boxes, steps,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+struct PoolMaps {
+    CUtensorMap latent{}, rope{}, scale{};
+};
+bool pool_maps(PoolMaps& m, const mm_latent_cache& c, int box) {
+    const CUtensorMapSwizzle by_rope = c.rope_dim == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+    const CUtensorMapDataType half = (c.kind == MM_E4M3 ? c.rope_kind : c.kind) == MM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if (c.kind == MM_E4M3)
+        return pool_map(&m.latent, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c, c.latent, c.kv, c.row_stride, c.pos_stride, 128, box,
+                        CU_TENSOR_MAP_SWIZZLE_128B) &&
+               pool_map(&m.rope, half, 2, c, c.rope, c.rope_dim, c.rope_row_stride, c.rope_pos_stride, c.rope_dim, box, by_rope) &&
+               scale_map(&m.scale, c, box);
+    return pool_map(&m.latent, half, 2, c, c.latent, c.kv + c.rope_dim, c.row_stride, c.pos_stride, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           pool_map(&m.rope, half, 2, c, c.latent, c.kv + c.rope_dim, c.row_stride, c.pos_stride, c.rope_dim, box, by_rope);
+}
+
+struct MmaPlan {
+    int blocks = 0, grid = 0, entries = 0;
+    bool shares = false;
+    int64_t units = 0;
+    int64_t bytes(int kv) const { return shares ? int64_t(2) * grid * 16 * (kv * 4 + 8) + int64_t(entries) * 16 : 0; }
+};
+MmaPlan mma_plan(const mm::paged::Attention& p) {
+    using namespace mm::paged;
+    MmaPlan r;
+    r.blocks = (p.H + 15) / 16;
+    r.units = static_cast<int64_t>(p.B) * r.blocks;
+    const int64_t all = (static_cast<int64_t>(p.max_length) + kTile - 1) / kTile;
+    const int64_t tiles = p.window > 0 ? std::min(all, (static_cast<int64_t>(p.window) + p.sinks) / kTile + 3) : all;
+    const int64_t ctas = 2 * sm_count();
+    // rows of few tiles are not worth cutting
+    r.shares = tiles > kMinShare;
+    r.grid = static_cast<int>(std::min(ctas, r.shares ? (r.units * (tiles + kRowCost) + kMinShare - 1) / kMinShare : r.units));
+    r.entries = static_cast<int>(std::min<int64_t>(r.units, r.grid));
+    return r;
+}
+
+template <int KV, int R, typename T, bool Q8>
+void run_mma(const mm::paged::Attention& p, const MmaPlan& r, const PoolMaps& maps, void* workspace, cudaStream_t s) {
+    using namespace mm::paged;
+    using C = MmaCfg<KV, R, Q8>;
+    MmaArgs a{};
+    a.p = p;
+    a.box = p.pool.positions % 32 == 0 ? 32 : 16;
+    a.blocks = r.blocks;
+    a.shares = r.shares;
+    a.by_unit = r.units <= r.grid;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(2) * r.grid * 16 * KV);
+    a.cut = reinterpret_cast<int4*>(a.part_ml + int64_t(2) * r.grid * 16);
+    set_dynamic_smem<paged_mma_kernel<KV, R, T, Q8>>(C::kSmem);
+    launch(s, paged_mma_kernel<KV, R, T, Q8>, dim3(r.grid), dim3(kMmaThreads), C::kSmem, a, maps.latent, maps.rope, maps.scale);
+    if (r.shares) {
+        // some two blocks of the join per SM
+        const int y = std::min(std::max(2 * sm_count() / r.entries, 1), 16 * KV / 128);
+        launch(s, paged_join_kernel<KV, T>, dim3(r.entries, y), dim3(256), 0, a);
+    }
+}
+
 void check_select(int batch, int beams, int vocab, int count) {
     require(batch >= 0 && beams >= 1 && vocab >= 1 && count >= 1, "beam selection: invalid sizes");
     if (beams > mm::beam::kMaxBeams || count > mm::beam::kMaxBeams) refuse(MM_UNSUPPORTED, "beam selection: more than 32 beams");
@@ -133,18 +228,36 @@ int mm_paged_append(const mm_paged_cache* cache, const void* values, int64_t val
 
 int64_t mm_paged_attention_workspace(const mm_paged_attention_desc* desc, const mm_paged_cache* cache) {
     int64_t bytes = 0;
-    const int rc = guarded([&] { problem(desc, cache); });
+    const int rc = guarded([&] {
+        const mm::paged::Attention p = problem(desc, cache);
+        if (p.B > 0 && mma_form(p, cache->pool)) bytes = mma_plan(p).bytes(p.kv);
+    });
     return rc ? -static_cast<int64_t>(rc) : bytes;
 }
 
-int mm_paged_attention(const mm_paged_attention_desc* desc, const mm_paged_cache* cache, void*, size_t, void* stream) {
+int mm_paged_attention(const mm_paged_attention_desc* desc, const mm_paged_cache* cache, void* workspace, size_t workspace_bytes,
+                       void* stream) {
     return guarded([&] {
         const mm::paged::Attention p = problem(desc, cache);
         if (p.B == 0) return;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
+        const bool q8 = cache->pool.kind == MM_E4M3;
+        PoolMaps maps;
+        if (mma_form(p, cache->pool) && pool_maps(maps, cache->pool, cache->pool.positions % 32 == 0 ? 32 : 16)) {
+            const MmaPlan r = mma_plan(p);
+            const int64_t need = r.bytes(p.kv);
+            require(need == 0 || (workspace && multiple(workspace, 16) && workspace_bytes >= static_cast<size_t>(need)),
+                    "paged attention: workspace too small or not 16-byte aligned");
+            with_half(desc->dtype, [&](auto half) {
+                using T = typename decltype(half)::type;
+                if (p.kv == 128) q8 ? run_mma<128, 16, T, true>(p, r, maps, workspace, s) : run_mma<128, 16, T, false>(p, r, maps, workspace, s);
+                else q8 ? run_mma<512, 32, T, true>(p, r, maps, workspace, s) : run_mma<512, 32, T, false>(p, r, maps, workspace, s);
+            });
+            return;
+        }
         with_half(desc->dtype, [&](auto half) {
             using T = typename decltype(half)::type;
-            if (cache->pool.kind == MM_E4M3) launch_any_width<T, true>(p, s);
+            if (q8) launch_any_width<T, true>(p, s);
             else launch_any_width<T, false>(p, s);
         });
     });
