@@ -36,6 +36,14 @@ mm::lat::CacheOut out_view(const mm_latent_cache* c) {
             c->rope_row_stride, c->rope_pos_stride, c->scale_row_stride, c->rows, c->positions};
 }
 
+// The vector form of append: the models' widths, 16-byte aligned rows.
+template <typename T> bool append_vector_form(const mm_latent_cache& c, const void* values, int64_t stride, const float* norm) {
+    if (!((c.kv == 128 && c.rope_dim == 16) || (c.kv == 512 && c.rope_dim == 32))) return false;
+    if (!multiple(values, 16) || stride * static_cast<int64_t>(sizeof(T)) % 16 || !multiple(norm, 16)) return false;
+    if (c.kind == MM_E4M3) return aligned_e4m3(&c);
+    return multiple(c.latent, 16) && c.row_stride % 8 == 0 && c.pos_stride % 8 == 0;
+}
+
 mm::paged::Attention problem(const mm_paged_attention_desc* d, const mm_paged_cache* c) {
     require(d != nullptr, "null description");
     check_paged(c);
@@ -179,6 +187,15 @@ void check_select(int batch, int beams, int vocab, int count) {
     if (vocab > mm::beam::kMaxVocab) refuse(MM_UNSUPPORTED, "beam selection: vocabulary over 1,048,576");
 }
 
+// Parts of a beam's tokens, a warp each: as many as fill the multiprocessors with 32 warps, of 512 tokens or more.
+int select_parts(int batch, int beams, int vocab) {
+    const int64_t rows = static_cast<int64_t>(batch) * beams, most = std::min((vocab + 511) / 512, mm::beam::kMaxParts);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 32 * sm_count() / std::max<int64_t>(rows, 1))));
+}
+int64_t select_bytes(int batch, int beams, int vocab, int count) {
+    return batch == 0 ? 0 : static_cast<int64_t>(batch) * beams * select_parts(batch, beams, vocab) * (8 + 8LL * count);
+}
+
 }  // namespace
 
 extern "C" {
@@ -217,6 +234,23 @@ int mm_paged_append(const mm_paged_cache* cache, const void* values, int64_t val
                 using T = typename decltype(in)::type;
                 using T16 = typename decltype(half)::type;
                 require(multiple(values, sizeof(T)), "paged append: input not aligned to its elements");
+                if (append_vector_form<T>(cache->pool, values, values_stride, norm)) {
+                    auto run = [&](auto kv, auto rd, auto codes) {
+                        constexpr int kKv = decltype(kv)::value, kRd = decltype(rd)::value;
+                        const unsigned ctas = std::min(blocks(n, 8 * (512 / kKv)),
+                                                       static_cast<unsigned>(sm_count() * mm::paged::kAppendCtas<T>));
+                        launch(s, mm::paged::append_vec_kernel<T, T16, kKv, kRd, decltype(codes)::value>, dim3(ctas), dim3(256), 0,
+                               out_view(&cache->pool), table_of(cache), static_cast<const T*>(values),
+                               static_cast<long long>(values_stride), rows, positions, static_cast<long long>(n), norm, eps, rot);
+                    };
+                    using Narrow = std::integral_constant<int, 128>;
+                    using Wide = std::integral_constant<int, 512>;
+                    using R16 = std::integral_constant<int, 16>;
+                    using R32 = std::integral_constant<int, 32>;
+                    if (cache->pool.kv == 128) q8 ? run(Narrow{}, R16{}, std::true_type{}) : run(Narrow{}, R16{}, std::false_type{});
+                    else q8 ? run(Wide{}, R32{}, std::true_type{}) : run(Wide{}, R32{}, std::false_type{});
+                    return;
+                }
                 launch(s, q8 ? mm::paged::append_kernel<T, T16, true> : mm::paged::append_kernel<T, T16, false>, dim3(blocks(n, 8)),
                        dim3(256), 0, out_view(&cache->pool), table_of(cache), static_cast<const T*>(values),
                        static_cast<long long>(values_stride), rows, positions, static_cast<long long>(n), cache->pool.kv,
@@ -264,13 +298,17 @@ int mm_paged_attention(const mm_paged_attention_desc* desc, const mm_paged_cache
 }
 
 int64_t mm_beam_select_workspace(int batch, int beams, int vocab, int count) {
-    const int rc = guarded([&] { check_select(batch, beams, vocab, count); });
-    return rc ? -static_cast<int64_t>(rc) : 0;
+    int64_t bytes = 0;
+    const int rc = guarded([&] {
+        check_select(batch, beams, vocab, count);
+        bytes = select_bytes(batch, beams, vocab, count);
+    });
+    return rc ? -static_cast<int64_t>(rc) : bytes;
 }
 
 int mm_beam_select(const void* logits, int64_t batch_stride, int64_t beam_stride, int dtype, const float* scores,
                    const uint8_t* finished, int eos, int batch, int beams, int vocab, int count, float* out_scores,
-                   int32_t* out_parents, int32_t* out_tokens, void*, size_t, void* stream) {
+                   int32_t* out_parents, int32_t* out_tokens, void* workspace, size_t workspace_bytes, void* stream) {
     return guarded([&] {
         check_select(batch, beams, vocab, count);
         require(!finished || (eos >= 0 && eos < vocab), "beam selection: eos must be in the vocabulary");
@@ -278,13 +316,22 @@ int mm_beam_select(const void* logits, int64_t batch_stride, int64_t beam_stride
         require(logits && scores && out_scores && out_parents && out_tokens, "beam selection: null argument");
         require(multiple(scores, 4) && multiple(out_scores, 4) && multiple(out_parents, 4) && multiple(out_tokens, 4),
                 "beam selection: argument not aligned to its elements");
-        mm::beam::Select a{logits, batch_stride, beam_stride, scores, finished, eos, batch, beams, vocab, count,
-                           out_scores, out_parents, out_tokens};
+        with_type(dtype, [&](auto t) {
+            require(multiple(logits, sizeof(typename decltype(t)::type)), "beam selection: logits not aligned to their elements");
+        });
+        require(workspace && multiple(workspace, 16) && workspace_bytes >= static_cast<size_t>(select_bytes(batch, beams, vocab, count)),
+                "beam selection: workspace too small or not 16-byte aligned");
+        const int parts = select_parts(batch, beams, vocab);
+        const int64_t lists = static_cast<int64_t>(batch) * beams * parts;
+        float2* sums = static_cast<float2*>(workspace);
+        float* best = reinterpret_cast<float*>(sums + lists);
+        mm::beam::Select a{logits, batch_stride, beam_stride, scores, finished, eos, batch, beams, vocab, count, parts,
+                           out_scores, out_parents, out_tokens, best, reinterpret_cast<int*>(best + lists * count), sums};
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         with_type(dtype, [&](auto t) {
             using T = typename decltype(t)::type;
-            require(multiple(logits, sizeof(T)), "beam selection: logits not aligned to their elements");
-            launch(s, mm::beam::select_kernel<T>, dim3(batch), dim3(256), 0, a);
+            launch(s, mm::beam::select_parts_kernel<T>, dim3(blocks(lists, 4)), dim3(128), 0, a);
+            launch(s, mm::beam::select_join_kernel, dim3(batch), dim3(32 * beams), 0, a);
         });
     });
 }
@@ -307,17 +354,21 @@ int mm_beam_reorder(const mm_paged_cache* cache, int layers, const int64_t layer
         mm::paged::Reorder a{table_of(cache), spare, lengths, parents, out_table, out_spare, out_lengths, c.positions,
                              c.rows, layers, {}};
         auto plane = [](void* data, int64_t layer, int64_t page, int64_t position, int n, int size) {
-            return mm::paged::Plane{static_cast<uint8_t*>(data), static_cast<long long>(layer * size),
-                                    static_cast<long long>(page * size), static_cast<long long>(position * size), n * size};
+            mm::paged::Plane r{static_cast<uint8_t*>(data), static_cast<long long>(layer * size),
+                               static_cast<long long>(page * size), static_cast<long long>(position * size), n * size, 1};
+            // positions in line are copied as one row, whose end need not be a whole access of 16 bytes
+            for (int v : {4, 16})
+                if (multiple(data, v) && r.layer % v == 0 && r.page % v == 0 && r.position % v == 0 && r.bytes % v == 0) r.vec = v;
+            return r;
         };
         if (q8) {
             a.plane[0] = plane(c.latent, layer_strides[0], c.row_stride, c.pos_stride, c.kv, 1);
-            a.plane[1] = plane(c.rope, layer_strides[1], c.rope_row_stride, c.rope_pos_stride, c.rope_dim, 2);
+            if (c.rope_dim > 0) a.plane[1] = plane(c.rope, layer_strides[1], c.rope_row_stride, c.rope_pos_stride, c.rope_dim, 2);
             a.plane[2] = plane(c.scale, layer_strides[2], c.scale_row_stride, 1, 1, 4);
         } else {
             a.plane[0] = plane(c.latent, layer_strides[0], c.row_stride, c.pos_stride, c.kv + c.rope_dim, 2);
         }
-        launch(static_cast<cudaStream_t>(stream), mm::paged::reorder_kernel<uint8_t>,
+        launch(static_cast<cudaStream_t>(stream), mm::paged::reorder_kernel,
                dim3(static_cast<unsigned>(rows), static_cast<unsigned>(std::min(std::max(layers, 1), 64))), dim3(256), 0, a);
     });
 }

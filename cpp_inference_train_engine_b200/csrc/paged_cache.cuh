@@ -86,12 +86,106 @@ __global__ void __launch_bounds__(256) append_kernel(lat::CacheOut c, Table tabl
     }
 }
 
+// KV = 128 or 512, 16-byte accesses: KV / 16 lanes take a token, 16 latent values and (the first R / 2 of them)
+// one pair of the key each; sums and maxima are shuffle reductions over the lane group. The CTAs that fit walk
+// the tokens, the next one already loaded. Bound by the bytes in and out.
+template <typename T> struct AppendRow {
+    uint4 x[sizeof(T)];
+    T key[2];
+    int position, row;
+};
+template <typename T> constexpr int kAppendCtas = sizeof(T) == 4 ? 2 : 3;  // CTAs per SM
+template <typename T, typename T16, int KV, int R, bool Q8>
+__global__ void __launch_bounds__(256, kAppendCtas<T>) append_vec_kernel(
+    lat::CacheOut c, Table table, const T* __restrict__ values, long long stride, const int* __restrict__ rows,
+    const int* __restrict__ positions, long long n, const float* __restrict__ norm, float eps, const __grid_constant__ Rotation rot) {
+    constexpr int L = KV / 16, P = 32 / L;  // lanes per token, tokens side by side in a warp
+    const int lane = threadIdx.x & 31, sub = lane % L;
+    const double f = sub < R / 2 ? rot.f[sub] : 0.0;
+    MM_PDL_ENTRY();
+    float w[16];
+    if (norm) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<float4*>(w + 4 * e) = __ldg(reinterpret_cast<const float4*>(norm + sub * 16) + e);
+    }
+    auto fetch = [&](long long i) {
+        AppendRow<T> v;
+        v.position = -1;
+        v.row = 0;
+        if (i < n) {
+            v.position = __ldg(positions + i);
+            v.row = rows ? __ldg(rows + i) : static_cast<int>(i);
+            const T* x = values + i * stride;
+#pragma unroll
+            for (int e = 0; e < static_cast<int>(sizeof(T)); ++e) v.x[e] = __ldcs(reinterpret_cast<const uint4*>(x + sub * 16) + e);
+            if (sub < R / 2) {
+                v.key[0] = __ldcs(x + KV + 2 * sub);
+                v.key[1] = __ldcs(x + KV + 2 * sub + 1);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < static_cast<int>(sizeof(T)); ++e) v.x[e] = make_uint4(0, 0, 0, 0);
+        }
+        return v;
+    };
+    const long long step = static_cast<long long>(gridDim.x) * 8 * P;
+    long long i0 = (static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * P;
+    const int mine = lane / L;
+    AppendRow<T> next = fetch(i0 + mine);
+    for (; i0 < n; i0 += step) {  // whole warps walk together (the reductions' shuffles)
+        const AppendRow<T> r = next;
+        int at = 0;
+        const long long p = page_of(table, c.rows, c.positions, r.row, r.position, at);
+        next = fetch(i0 + mine + step);
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = lat::to_f32(reinterpret_cast<const T*>(r.x)[e]);
+        if (norm) {
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum = fmaf(v[e], v[e], sum);
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const float inv = rsqrtf(sum * (1.f / KV) + eps);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = v[e] * inv * w[e];
+        }
+        float s = 0.f;
+        if constexpr (Q8) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s = fmaxf(s, fabsf(v[e]));
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
+            s = fmaxf(__fdiv_rn(s, lat::kE4m3Max), lat::kScaleFloor);
+        }
+        if (p < 0) continue;
+        T16* key;
+        if constexpr (Q8) {
+            *reinterpret_cast<uint4*>(c.latent + p * c.row_stride + at * c.pos_stride + sub * 16) =
+                lat::e4m3_quotients<float>(*reinterpret_cast<const uint4(*)[4]>(v), s);
+            if (sub == 0) c.scale[p * c.scale_row_stride + at] = s;
+            key = reinterpret_cast<T16*>(c.rope) + p * c.rope_row_stride + at * c.rope_pos_stride;
+        } else {
+            T16* dst = reinterpret_cast<T16*>(c.latent) + p * c.row_stride + at * c.pos_stride;
+            lat::store16(dst + sub * 16, v);
+            key = dst + KV;
+        }
+        if (sub < R / 2) {
+            float sn, cs;
+            rotation(f, r.position, sn, cs);
+            const float a = lat::to_f32(r.key[0]), b = lat::to_f32(r.key[1]);
+            *reinterpret_cast<uint32_t*>(key + 2 * sub) = lat::pack2<T16>(a * cs - b * sn, a * sn + b * cs);
+        }
+    }
+}
+
 // ------------------------------------------------------------------ reorder
 // One array of the pool (latent, rope keys or scales) as bytes.
 struct Plane {
     uint8_t* data;
     long long layer, page, position;  // strides in bytes
     int bytes;                        // of a position
+    int vec;                          // bytes an access may take: 16, 4 or 1
 };
 struct Reorder {
     Table table;
@@ -127,10 +221,35 @@ __device__ __forceinline__ Move move_of(const Reorder& a, int row) {
     return m;
 }
 
-// Block (row, layer group): copies the row's tail in the layers blockIdx.y, blockIdx.y + gridDim.y, ...;
-// the first group's block writes the row's table entries. VEC bytes an access.
+// `n` elements of type V per position, `positions` of them; all loads of a step ahead of its stores.
 template <typename V>
-__global__ void __launch_bounds__(256) reorder_kernel(const Reorder a) {
+__device__ __forceinline__ void copy_tail(const Plane& p, const uint8_t* src, uint8_t* dst, int positions) {
+    constexpr int U = 4;
+    int rows = positions, n = p.bytes / static_cast<int>(sizeof(V));
+    if (p.position == p.bytes) {  // positions in line: one row
+        n *= rows;
+        rows = 1;
+    }
+    const int width = rows == 1 ? 256 : 32, lanes = threadIdx.x % width;  // threads along a row
+    for (int r = threadIdx.x / width; r < rows; r += 256 / width) {
+        const V* s = reinterpret_cast<const V*>(src + r * p.position);
+        V* d = reinterpret_cast<V*>(dst + r * p.position);
+        for (int e = lanes; e < n; e += U * width) {
+            V v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (e + u * width < n) v[u] = __ldcs(s + e + u * width);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (e + u * width < n) d[e + u * width] = v[u];
+        }
+    }
+}
+
+// Block (row, layer group): copies the row's tail in the layers blockIdx.y, blockIdx.y + gridDim.y, ...;
+// the first group's block writes the row's table entries. Bound by the bytes read and written, and for few rows
+// by the chain parent, its length, its page, the copy.
+static __global__ void __launch_bounds__(256) reorder_kernel(const __grid_constant__ Reorder a) {
     MM_PDL_ENTRY();
     const int row = blockIdx.x, tid = threadIdx.x;
     const Move m = move_of(a, row);
@@ -146,16 +265,15 @@ __global__ void __launch_bounds__(256) reorder_kernel(const Reorder a) {
     }
     if (m.part == 0 || m.from < 0 || m.from >= a.pages || m.to < 0 || m.to >= a.pages || m.from == m.to) return;
     for (int l = blockIdx.y; l < a.layers; l += gridDim.y)
+#pragma unroll
         for (int q = 0; q < 3; ++q) {
             const Plane& p = a.plane[q];
-            const int per = p.bytes / static_cast<int>(sizeof(V));
+            if (!p.data) continue;
             const uint8_t* src = p.data + l * p.layer + m.from * p.page;
             uint8_t* dst = p.data + l * p.layer + m.to * p.page;
-            for (int e = tid; e < m.part * per; e += blockDim.x) {
-                const int t = e / per;
-                const long long off = t * p.position + (e - t * per) * static_cast<long long>(sizeof(V));
-                *reinterpret_cast<V*>(dst + off) = *reinterpret_cast<const V*>(src + off);
-            }
+            if (p.vec == 16) copy_tail<uint4>(p, src, dst, m.part);
+            else if (p.vec == 4) copy_tail<uint32_t>(p, src, dst, m.part);
+            else copy_tail<uint8_t>(p, src, dst, m.part);
         }
 }
 
