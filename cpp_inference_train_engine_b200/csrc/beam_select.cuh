@@ -1,9 +1,10 @@
 // Beam search's selection over beams and vocabulary (mm_beam_select).
 //
-// One pass over the logits: a warp takes a part of a beam's tokens and keeps their maximum, the sum of
-// exponentials below it, and the best `count` of them (rank r in lane r); a second kernel joins the parts of a
-// beam and then the beams. A token enters the list by a vote against its last entry, which after the first few
-// hundred tokens almost never happens, so the pass is bound by its loads.
+// One pass over the logits: a block takes a part of a beam's tokens, each of its warps a quarter, and keeps
+// their maximum, the sum of exponentials below it and the best `count` of them (rank r in lane r); a second kernel
+// joins the parts of a beam and then the beams. The pass itself keeps one maximum per lane and step: of the 32
+// lanes' maxima over a stretch of steps the count-th largest bounds the list from below, so that only the few (lane,
+// step) pairs that reach it are looked at again, from the cache.
 #pragma once
 #include "latent_cache.cuh"
 
@@ -12,7 +13,8 @@ namespace beam {
 
 constexpr int kMaxBeams = 32;
 constexpr int kMaxVocab = 1 << 20;  // flat candidates k * vocab + v stay below 2^25
-constexpr int kMaxParts = 64;       // of a beam's tokens
+constexpr float kLowest = -3.402823466e38f;
+constexpr int kMaxParts = 32;       // of a beam's tokens
 
 struct Select {
     const void* logits;
@@ -29,127 +31,180 @@ struct Select {
     float2* sum;
 };
 
-// The best `count` candidates so far, rank r in lane r; lanes behind the last hold (-infinity, kNobody).
+// Candidates in order: by value, then by the lower index. Nobody: (-infinity, kNobody).
 constexpr int kNobody = 0x7fffffff;
-template <typename V> struct Best {
-    V value;
+struct Pair {
+    float value;
     int at;
-    V last;     // of rank count - 1
-    int last_at;
-    __device__ __forceinline__ Best() : value(-INFINITY), at(kNobody), last(-INFINITY), last_at(kNobody) {}
-    __device__ __forceinline__ bool enters(V v, int i) const { return (v > last || (v == last && i < last_at)) && v > -INFINITY; }
-    // Offers every lane's candidate.
-    __device__ __forceinline__ void offer(V v, int i, int count) {
-        const int lane = threadIdx.x & 31;
-        unsigned todo = __ballot_sync(0xffffffffu, enters(v, i));
-        while (todo) {
-            const int from = __ffs(todo) - 1;
-            const V cv = __shfl_sync(0xffffffffu, v, from);
-            const int ci = __shfl_sync(0xffffffffu, i, from);
-            const int rank = __popc(__ballot_sync(0xffffffffu, value > cv || (value == cv && at < ci)));
-            const V uv = __shfl_up_sync(0xffffffffu, value, 1);
-            const int ui = __shfl_up_sync(0xffffffffu, at, 1);
-            if (lane >= rank) {
-                value = lane == rank ? cv : uv;
-                at = lane == rank ? ci : ui;
-            }
-            if (lane >= count) {
-                value = -INFINITY;
-                at = kNobody;
-            }
-            last = __shfl_sync(0xffffffffu, value, count - 1);
-            last_at = __shfl_sync(0xffffffffu, at, count - 1);
-            todo &= todo - 1;
-            todo &= __ballot_sync(0xffffffffu, enters(v, i));
-        }
+};
+__device__ __forceinline__ bool ahead(Pair a, Pair b) { return a.value > b.value || (a.value == b.value && a.at < b.at); }
+__device__ __forceinline__ Pair from_lane(Pair p, int lane_xor) {
+    return {__shfl_xor_sync(0xffffffffu, p.value, lane_xor), __shfl_xor_sync(0xffffffffu, p.at, lane_xor)};
+}
+// One step of a bitonic network over the lanes; `down`: the better of the two goes to the lower lane.
+__device__ __forceinline__ void exchange(Pair& p, int o, bool down) {
+    const Pair q = from_lane(p, o);
+    const bool lower = (threadIdx.x & o) == 0;
+    if (ahead(q, p) == (lower == down)) p = q;
+}
+// The best 32 candidates so far, rank r in lane r.
+struct Best {
+    Pair p{-INFINITY, kNobody};
+    // Joins 32 more, one a lane, in any order.
+    __device__ __forceinline__ void join(Pair q) {
+#pragma unroll
+        for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+            for (int o = size >> 1; o > 0; o >>= 1) exchange(q, o, (threadIdx.x & size) == 0 || size == 32);
+        join_sorted(q);
+    }
+    // The same, from the best to the last.
+    __device__ __forceinline__ void join_sorted(Pair q) {
+        // the better of rank r and rank 31 - r are the best 32, rising and falling once
+        q = from_lane(q, 31);
+        if (ahead(q, p)) p = q;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) exchange(p, o, true);
+    }
+    __device__ __forceinline__ Pair rank(int r) const {
+        return {__shfl_sync(0xffffffffu, p.value, r), __shfl_sync(0xffffffffu, p.at, r)};
     }
 };
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
 
-// Warp: part `part` of beam row `row`. E values of 16 bytes a load; a row's first and last tokens that are
-// not in a whole aligned load are taken one a lane.
+// Block (part, beam row). E values of 16 bytes a load; a row's first and last tokens that are not in a whole
+// aligned load are taken one a lane.
 template <typename T>
 __global__ void __launch_bounds__(128) select_parts_kernel(const Select a) {
     MM_PDL_ENTRY();
-    constexpr int E = 16 / sizeof(T), U = 4;  // values per load, loads per step
-    const int lane = threadIdx.x & 31;
-    const long long w = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (w >= static_cast<long long>(a.batch) * a.beams * a.parts) return;
-    const int row = static_cast<int>(w / a.parts), part = static_cast<int>(w - static_cast<long long>(row) * a.parts);
+    constexpr int E = 16 / sizeof(T), U = 4, kSteps = 4;  // values per load, loads per step, steps per stretch
+    __shared__ Pair wait_s[4][64];
+    __shared__ float2 sum_s[4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
     if (!finite(__ldg(a.scores + row)) || (a.finished && a.finished[row])) return;  // the join does not read it either
     const int b = row / a.beams;
     const T* x = static_cast<const T*>(a.logits) + b * a.batch_stride + (row - b * a.beams) * a.beam_stride;
     // whole loads begin at token `head`, which is where the address is a multiple of 16
     const int head = min(a.vocab, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
     const int loads = (a.vocab - head) / E;
-    const int per = (loads + a.parts - 1) / a.parts, l0 = min(part * per, loads), l1 = min(l0 + per, loads);
-    Best<float> best;
-    float m = -INFINITY, s = 0.f;
-    auto add = [&](const float* v, int n, float top) {  // n values of this lane into its sum
-        if (top > m) {
-            s *= m == -INFINITY ? 0.f : fast_exp2((m - top) * 1.4426950408889634f);
-            m = top;
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        for (int e = 0; e < n; ++e) s += fast_exp2((v[e] - ref) * 1.4426950408889634f);
+    const int per = (loads + 4 * a.parts - 1) / (4 * a.parts), l0 = min((part * 4 + warp) * per, loads), l1 = min(l0 + per, loads);
+    // Candidates wait in shared memory until there are 32 (or no more): joining the list costs a sort. What is
+    // behind the list's last entry does not wait.
+    Pair* wait = wait_s[warp];
+    int waiting = 0;
+    Best best;
+    Pair last{-INFINITY, kNobody};
+    auto join = [&] {
+        __syncwarp();
+        best.join(lane < waiting ? wait[lane] : Pair{-INFINITY, kNobody});
+        const Pair l = best.rank(a.count - 1);
+        if (l.at != kNobody) last = l;  // (a list that is not full keeps its floor)
+        const Pair rest = wait[32 + lane];
+        __syncwarp();
+        wait[lane] = rest;
+        waiting = max(waiting - 32, 0);
     };
-    for (int i0 = l0; i0 < l1; i0 += 32 * U) {
-        uint4 raw[U];
+    auto offer = [&](float v, int i) {
+        const bool in = v > -INFINITY && ahead({v, i}, last);
+        const unsigned who = __ballot_sync(0xffffffffu, in);
+        if (in) wait[waiting + __popc(who & ((1u << lane) - 1))] = {v, i};
+        waiting += __popc(who);
+        if (waiting >= 32) join();
+    };
+    constexpr float kLog2e = 1.4426950408889634f;
+    float m = kLowest, s = 0.f;  // (a finite maximum of nothing: differences from it are no NaN)
+    uint4 raw[U];
+    auto fetch = [&](int i0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * 32 + lane;
-            if (i < l1) raw[u] = __ldcs(reinterpret_cast<const uint4*>(x + head) + i);
+            if (i < l1) raw[u] = __ldg(reinterpret_cast<const uint4*>(x + head) + i);
+        }
+    };
+    fetch(l0);
+    for (int base = l0; base < l1; base += 32 * U * kSteps) {
+        float tops[kSteps], most = -INFINITY;
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+            const int i0 = base + st * 32 * U;
+            tops[st] = -INFINITY;
+            if (i0 >= l1) continue;
+            float v[U][E];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    v[u][e] = i0 + u * 32 + lane < l1 ? lat::to_f32(reinterpret_cast<const T*>(&raw[u])[e]) : -INFINITY;
+                    tops[st] = fmaxf(tops[st], v[u][e]);
+                }
+            fetch(i0 + 32 * U);
+            const float mn = fmaxf(m, tops[st]);
+            s *= fast_exp2((m - mn) * kLog2e);
+            m = mn;
+            float sums[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                sums[u] = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) sums[u] += fast_exp2((v[u][e] - m) * kLog2e);
+            }
+            s += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            most = fmaxf(most, tops[st]);
+        }
+        // `count` of the lanes' largest are `count` candidates: nothing below the least of them enters
+        {
+            Best all;
+            all.join({most, lane});
+            const float floor = all.rank(a.count - 1).value;
+            if (floor > last.value) last = {floor, kNobody};
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * 32 + lane;
-            if (i0 + u * 32 >= l1) break;
-            float v[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = i < l1 ? lat::to_f32(reinterpret_cast<const T*>(&raw[u])[e]) : -INFINITY;
-            float top = v[0];
-#pragma unroll
-            for (int e = 1; e < E; ++e) top = fmaxf(top, v[e]);
-            if (top > m) {
-                s *= m == -INFINITY ? 0.f : fast_exp2((m - top) * 1.4426950408889634f);
-                m = top;
+        for (int st = 0; st < kSteps; ++st)
+            for (unsigned who = __ballot_sync(0xffffffffu, tops[st] >= last.value && tops[st] > -INFINITY); who; who &= who - 1) {
+                const int i = base + st * 32 * U + lane / E * 32 + __ffs(who) - 1, t = head + i * E + lane % E;
+                offer(lane < U * E && i < l1 ? lat::to_f32(x[t]) : -INFINITY, t);
             }
-            const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int e = 0; e < E; ++e) s += fast_exp2((v[e] - ref) * 1.4426950408889634f);
-            if (__any_sync(0xffffffffu, top >= best.last && top > -INFINITY)) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) best.offer(v[e], head + i * E + e, a.count);
-            }
-        }
     }
-    if (part == 0) {  // the ends, at most 2 (E - 1) <= 14 tokens
+    if (part == 0 && warp == 0) {  // the ends, at most 2 (E - 1) <= 14 tokens
         const int tail = head + loads * E;
         const int t = lane < head ? lane : tail + lane - head;
         const float v = t < a.vocab ? lat::to_f32(x[t]) : -INFINITY;
-        add(&v, 1, v);
-        best.offer(v, t, a.count);
+        const float mn = fmaxf(m, v);
+        s = s * fast_exp2((m - mn) * kLog2e) + fast_exp2((v - mn) * kLog2e);
+        m = mn;
+        offer(v, t);
     }
-    // the lanes' sums below one maximum (a NaN or +infinity anywhere makes the sum a NaN)
-    const float top = warp_max(m);
-    s *= m == -INFINITY ? 0.f : fast_exp2((m - top) * 1.4426950408889634f);
-    s = warp_sum(m == -INFINITY && s == 0.f ? 0.f : s);
+    join();
+    // the lanes' sums below one maximum (a NaN or +infinity anywhere makes the sum a NaN), then the warps'
+    auto scaled = [&](float2 v, float top) { return v.y * fast_exp2((v.x - top) * kLog2e); };
+    float top = warp_max(m);
+    s = warp_sum(scaled({m, s}, top));
+    if (lane == 0) sum_s[warp] = make_float2(top, s);
+    wait[lane] = best.p;
+    __syncthreads();
+    if (warp) return;
+    for (int w = 1; w < 4; ++w) best.join_sorted(wait_s[w][lane]);
+    const long long o = static_cast<long long>(blockIdx.x) * a.count + lane;
     if (lane < a.count) {
-        a.best[w * a.count + lane] = best.value;
-        a.token[w * a.count + lane] = best.at;
+        a.best[o] = best.p.value;
+        a.token[o] = best.p.at;
     }
-    if (lane == 0) a.sum[w] = make_float2(top, s);
+    if (lane == 0) {
+        top = fmaxf(fmaxf(sum_s[0].x, sum_s[1].x), fmaxf(sum_s[2].x, sum_s[3].x));
+        a.sum[blockIdx.x] = make_float2(top, (scaled(sum_s[0], top) + scaled(sum_s[1], top)) + (scaled(sum_s[2], top) + scaled(sum_s[3], top)));
+    }
 }
 
-// Block per batch entry, a warp per beam: its log-sum-exp and its best tokens' scores; then the first warp
-// takes the best of the beams' lists.
+// Block per batch entry, a warp per beam: its log-sum-exp and the best of its parts' lists; then the rank of
+// every beam's candidates among all of them, counted by a thread each.
 static __global__ void __launch_bounds__(1024) select_join_kernel(const Select a) {
     MM_PDL_ENTRY();
     __shared__ double score_s[kMaxBeams * kMaxBeams];
     __shared__ int at_s[kMaxBeams * kMaxBeams];
     const int b = blockIdx.x, k = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = b * a.beams + k;
+    const int row = b * a.beams + k, n = a.parts * a.count;
     const float score = __ldg(a.scores + row);
     double cand = -INFINITY;
     int at = kNobody;
@@ -161,48 +216,47 @@ static __global__ void __launch_bounds__(1024) select_join_kernel(const Select a
             }
         } else {
             const long long p0 = static_cast<long long>(row) * a.parts;
-            float top = -INFINITY;
-            for (int p = lane; p < a.parts; p += 32) top = fmaxf(top, a.sum[p0 + p].x);
-            top = warp_max(top);
-            double s = 0;
-            for (int p = lane; p < a.parts; p += 32) {
-                const float2 v = a.sum[p0 + p];
-                s += v.x == -INFINITY ? static_cast<double>(v.y) : static_cast<double>(v.y) * exp(static_cast<double>(v.x) - top);
+            auto entry = [&](int i) { return i < n ? Pair{a.best[p0 * a.count + i], a.token[p0 * a.count + i]} : Pair{-INFINITY, kNobody}; };
+            Pair next = entry(lane);
+            const float2 sum = lane < a.parts ? a.sum[p0 + lane] : make_float2(kLowest, 0.f);
+            const float top = warp_max(sum.x);
+            const double s = static_cast<double>(sum.y) * exp(static_cast<double>(sum.x) - top);
+            const double lse = top + log(warp_sum(s));
+            Best best;
+#pragma unroll 1
+            for (int i = 32; i < n + 32; i += 32) {
+                const Pair q = next;
+                next = entry(i + lane);
+                best.join(q);
             }
-            s = warp_sum(s);
-            const double lse = top + log(s);
-            Best<float> best;
-            const int n = a.parts * a.count;
-            for (int i = lane; i < (n + 31) / 32 * 32; i += 32) {
-                const float v = i < n ? a.best[p0 * a.count + i] : -INFINITY;
-                best.offer(v, i < n ? a.token[p0 * a.count + i] : kNobody, a.count);
-            }
-            // not a number where the log-sum-exp is not finite
-            if (best.at != kNobody && fabs(lse) < INFINITY) {
-                cand = score + (static_cast<double>(best.value) - lse);
-                at = k * a.vocab + best.at;
-            }
+            // a log-sum-exp that is not finite makes no candidate; what fp32 cannot hold is no score
+            cand = score + (static_cast<double>(best.p.value) - lse);
+            if (best.p.at != kNobody && fabs(lse) < INFINITY && static_cast<float>(cand) > -INFINITY) at = k * a.vocab + best.p.at;
         }
-    }
-    if (!(static_cast<float>(cand) > -INFINITY)) {  // what fp32 cannot hold is no score
-        cand = -INFINITY;
-        at = kNobody;
     }
     if (lane < a.count) {
         score_s[k * a.count + lane] = cand;
         at_s[k * a.count + lane] = at;
     }
-    __syncthreads();
-    if (k) return;
-    Best<double> best;
-    const int n = a.beams * a.count;
-    for (int i = lane; i < (n + 31) / 32 * 32; i += 32) best.offer(i < n ? score_s[i] : -INFINITY, i < n ? at_s[i] : kNobody, a.count);
-    if (lane < a.count) {
-        const bool none = best.at == kNobody;
-        const long long o = static_cast<long long>(b) * a.count + lane;
-        a.out_scores[o] = static_cast<float>(best.value);
-        a.out_parents[o] = none ? min(lane, a.beams - 1) : best.at / a.vocab;
-        a.out_tokens[o] = none ? -1 : best.at % a.vocab;
+    const int all = a.beams * a.count, i = threadIdx.x;
+    const long long o = static_cast<long long>(b) * a.count;
+    const int candidates = __syncthreads_count(lane < a.count && at != kNobody);
+    if (i < all && at_s[i] != kNobody) {
+        const double c = score_s[i];
+        const int t = at_s[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < all; ++j) rank += at_s[j] != kNobody && (score_s[j] > c || (score_s[j] == c && at_s[j] < t));
+        if (rank < a.count) {
+            a.out_scores[o + rank] = static_cast<float>(c);
+            a.out_parents[o + rank] = t / a.vocab;
+            a.out_tokens[o + rank] = t % a.vocab;
+        }
+    }
+    if (i >= candidates && i < a.count) {  // left over
+        a.out_scores[o + i] = -INFINITY;
+        a.out_parents[o + i] = min(i, a.beams - 1);
+        a.out_tokens[o + i] = -1;
     }
 }
 

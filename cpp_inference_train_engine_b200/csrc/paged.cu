@@ -187,10 +187,11 @@ void check_select(int batch, int beams, int vocab, int count) {
     if (vocab > mm::beam::kMaxVocab) refuse(MM_UNSUPPORTED, "beam selection: vocabulary over 1,048,576");
 }
 
-// Parts of a beam's tokens, a warp each: as many as fill the multiprocessors with 32 warps, of 512 tokens or more.
+// Parts of a beam's tokens, a block of four warps each: as many as fill the multiprocessors with 32 warps, of
+// 2,048 tokens or more.
 int select_parts(int batch, int beams, int vocab) {
-    const int64_t rows = static_cast<int64_t>(batch) * beams, most = std::min((vocab + 511) / 512, mm::beam::kMaxParts);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 32 * sm_count() / std::max<int64_t>(rows, 1))));
+    const int64_t rows = static_cast<int64_t>(batch) * beams, most = std::min((vocab + 2047) / 2048, mm::beam::kMaxParts);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 8 * sm_count() / std::max<int64_t>(rows, 1))));
 }
 int64_t select_bytes(int batch, int beams, int vocab, int count) {
     return batch == 0 ? 0 : static_cast<int64_t>(batch) * beams * select_parts(batch, beams, vocab) * (8 + 8LL * count);
@@ -330,7 +331,7 @@ int mm_beam_select(const void* logits, int64_t batch_stride, int64_t beam_stride
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         with_type(dtype, [&](auto t) {
             using T = typename decltype(t)::type;
-            launch(s, mm::beam::select_parts_kernel<T>, dim3(blocks(lists, 4)), dim3(128), 0, a);
+            launch(s, mm::beam::select_parts_kernel<T>, dim3(blocks(lists, 1)), dim3(128), 0, a);
             launch(s, mm::beam::select_join_kernel, dim3(batch), dim3(32 * beams), 0, a);
         });
     });

@@ -94,7 +94,7 @@ template <typename T> struct AppendRow {
     T key[2];
     int position, row;
 };
-template <typename T> constexpr int kAppendCtas = sizeof(T) == 4 ? 2 : 3;  // CTAs per SM
+template <typename T> constexpr int kAppendCtas = sizeof(T) == 4 ? 3 : 4;  // CTAs per SM
 template <typename T, typename T16, int KV, int R, bool Q8>
 __global__ void __launch_bounds__(256, kAppendCtas<T>) append_vec_kernel(
     lat::CacheOut c, Table table, const T* __restrict__ values, long long stride, const int* __restrict__ rows,
@@ -161,8 +161,14 @@ __global__ void __launch_bounds__(256, kAppendCtas<T>) append_vec_kernel(
         if (p < 0) continue;
         T16* key;
         if constexpr (Q8) {
-            *reinterpret_cast<uint4*>(c.latent + p * c.row_stride + at * c.pos_stride + sub * 16) =
-                lat::e4m3_quotients<float>(*reinterpret_cast<const uint4(*)[4]>(v), s);
+            // by the reciprocal: within 2 ulp of the quotient, as the normalised values are of theirs
+            const float inv = __frcp_rn(s);
+            uint32_t q[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                q[e] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(v[4 * e] * inv, v[4 * e + 1] * inv), __NV_SATFINITE, __NV_E4M3)) |
+                       (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(v[4 * e + 2] * inv, v[4 * e + 3] * inv), __NV_SATFINITE, __NV_E4M3)) << 16);
+            *reinterpret_cast<uint4*>(c.latent + p * c.row_stride + at * c.pos_stride + sub * 16) = make_uint4(q[0], q[1], q[2], q[3]);
             if (sub == 0) c.scale[p * c.scale_row_stride + at] = s;
             key = reinterpret_cast<T16*>(c.rope) + p * c.rope_row_stride + at * c.rope_pos_stride;
         } else {
