@@ -19,7 +19,10 @@ namespace {
 static_assert(sizeof(mm_paged_cache) == 112 && sizeof(mm_paged_attention_desc) == 80, "callers without this header pack these field by field");
 
 mm::paged::Table table_of(const mm_paged_cache* c) {
-    return {c->table, c->table_stride, c->table_rows, c->table_columns};
+    const int page = c->pool.positions;
+    int shift = 0;
+    while (1LL << shift < page) ++shift;
+    return {c->table, c->table_stride, c->table_rows, c->table_columns, 1LL << shift == page ? shift : -1};
 }
 
 void check_paged(const mm_paged_cache* c) {

@@ -10,12 +10,13 @@ struct Table {
     const int* entry;
     long long stride;
     int rows, columns;
+    int shift;  // log2 of the page size, -1 where it is no power of two
 };
 
 // The pool's page of position t of table row r, or -1 (a position or a page that is not there); at: the entry.
 __device__ __forceinline__ int page_of(const Table& t, int pages, int page, int row, int position, int& at) {
     if (row < 0 || row >= t.rows || position < 0) return -1;
-    const int column = position / page;
+    const int column = t.shift >= 0 ? position >> t.shift : position / page;
     if (column >= t.columns) return -1;
     at = position - column * page;
     const int p = __ldg(t.entry + row * t.stride + column);
@@ -23,11 +24,12 @@ __device__ __forceinline__ int page_of(const Table& t, int pages, int page, int 
 }
 
 // Pair j's angle at `position` in turns: f = theta^(-2 j / width) / (2 pi) in fp64, whose product with any
-// 31-bit position is off by less than 2^-22 turns of the exact one only through f itself (2^31 * 2^-54);
-// the fraction goes on in fp32 (2^-25 turns, below a 16-bit key's rounding).
+// 31-bit position is off by 2^31 * 2^-53 turns at most; the fraction, within half a turn, goes on in fp32, where
+// the fast sine and cosine are off by 2^-21, far below a 16-bit key's rounding. (sincospif: 40 instructions more
+// a token, 63 us instead of 55 for 131,072 tokens.)
 __device__ __forceinline__ void rotation(double f, int position, float& sin_t, float& cos_t) {
     const double turns = f * position;
-    sincospif(2.f * static_cast<float>(turns - rint(turns)), &sin_t, &cos_t);
+    __sincosf(6.283185307f * static_cast<float>(turns - rint(turns)), &sin_t, &cos_t);
 }
 
 constexpr int kMaxPairs = 128;  // of a rope key of 256
@@ -140,15 +142,17 @@ __global__ void __launch_bounds__(256, kAppendCtas<T>) append_vec_kernel(
         float v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = lat::to_f32(reinterpret_cast<const T*>(r.x)[e]);
+        float inv = 1.f;  // what the values below are still to be multiplied by
         if (norm) {
             float sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sum = fmaf(v[e], v[e], sum);
+            for (int e = 0; e < 16; ++e) {
+                sum = fmaf(v[e], v[e], sum);
+                v[e] *= w[e];
+            }
 #pragma unroll
             for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const float inv = rsqrtf(sum * (1.f / KV) + eps);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = v[e] * inv * w[e];
+            inv = rsqrtf(sum * (1.f / KV) + eps);
         }
         float s = 0.f;
         if constexpr (Q8) {
@@ -156,23 +160,27 @@ __global__ void __launch_bounds__(256, kAppendCtas<T>) append_vec_kernel(
             for (int e = 0; e < 16; ++e) s = fmaxf(s, fabsf(v[e]));
 #pragma unroll
             for (int o = L / 2; o > 0; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
-            s = fmaxf(__fdiv_rn(s, lat::kE4m3Max), lat::kScaleFloor);
+            s = fmaxf(__fdiv_rn(s * inv, lat::kE4m3Max), lat::kScaleFloor);
         }
         if (p < 0) continue;
         T16* key;
         if constexpr (Q8) {
             // by the reciprocal: within 2 ulp of the quotient, as the normalised values are of theirs
-            const float inv = __frcp_rn(s);
+            const float f8 = inv * __frcp_rn(s);
             uint32_t q[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                q[e] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(v[4 * e] * inv, v[4 * e + 1] * inv), __NV_SATFINITE, __NV_E4M3)) |
-                       (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(v[4 * e + 2] * inv, v[4 * e + 3] * inv), __NV_SATFINITE, __NV_E4M3)) << 16);
+                q[e] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(v[4 * e] * f8, v[4 * e + 1] * f8), __NV_SATFINITE, __NV_E4M3)) |
+                       (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(v[4 * e + 2] * f8, v[4 * e + 3] * f8), __NV_SATFINITE, __NV_E4M3)) << 16);
             *reinterpret_cast<uint4*>(c.latent + p * c.row_stride + at * c.pos_stride + sub * 16) = make_uint4(q[0], q[1], q[2], q[3]);
             if (sub == 0) c.scale[p * c.scale_row_stride + at] = s;
             key = reinterpret_cast<T16*>(c.rope) + p * c.rope_row_stride + at * c.rope_pos_stride;
         } else {
             T16* dst = reinterpret_cast<T16*>(c.latent) + p * c.row_stride + at * c.pos_stride;
+            if (norm) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] *= inv;
+            }
             lat::store16(dst + sub * 16, v);
             key = dst + KV;
         }
