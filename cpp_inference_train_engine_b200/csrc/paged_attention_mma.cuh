@@ -10,7 +10,8 @@
 //              its O [16 x 128] stay in registers, and it alone reads (and clears) those columns. 512 wide: the
 //              four take a tile together and add their shares of S through shared memory; 128 wide: each has
 //              tiles of its own (every fourth) and the four results are joined at the row's end.
-//   loads      1, which walks the same runs ahead of them: page numbers 32 boxes at a time, a box a lane.
+//   loads      1, which walks the CTA's runs ahead of them and queues what they need to know of each: a box a
+//              lane, its page number asked for a step ahead.
 // Positions that a row does not see are masked in S and cleared in the tile (a probability of zero times a NaN
 // would be one). Two CTAs an SM, each with a ring of its own; the row's sums and maxima are fp32, the weights of
 // the second product are rounded to 16 bits once, as its operand has to be.
@@ -40,6 +41,7 @@ constexpr int kTile = 32;       // positions
 constexpr int kRowCost = 2;     // tiles that a row's queries and results cost
 constexpr int kMinShare = 6;    // tiles of a CTA at least
 constexpr int kMmaThreads = 160;
+constexpr int kQueue = 4;       // runs queued for the warps of the products
 constexpr float kNone = -3.402823466e38f;  // maximum of nothing (finite: its exp2 is 0, never NaN)
 
 template <int KV, int R, bool Q8> struct MmaCfg {
@@ -57,18 +59,22 @@ template <int KV, int R, bool Q8> struct MmaCfg {
     static constexpr int kShare = KV == 512 ? 4 * 16 * kTile * 4 : 4 * 16 * 128 * 4;
     static constexpr int oShare = SLOTS * kSlot;
     static constexpr int oStat = oShare + kShare;           // [4][16] maxima and sums (128 wide)
-    static constexpr int oBar = oStat + 4 * 16 * 8;
-    static constexpr int oMeta = oBar + 2 * SLOTS * 8;
-    static constexpr int oPlan = (oMeta + SLOTS * 4 + 15) / 16 * 16;
-    static constexpr int kSmem = oPlan + 64 + 1024;         // + alignment of the base
-    static_assert(oBar % 8 == 0 && oStat % 8 == 0 && oShare % 1024 == 0 && kSlot % 1024 == 0, "alignment");
+    static constexpr int oTops = oStat;                     // [4][16] maxima, sums (512 wide)
+    static constexpr int oHand = oStat + 4 * 16 * 8;        // [4][32] weights, 8 positions from each warp (512 wide)
+    static constexpr int oRuns = oHand + (KV == 512 ? 1024 : 0);
+    static constexpr int oPlan = oRuns + kQueue * 32;
+    static constexpr int oBar = oPlan + 48;
+    static constexpr int oMeta = oBar + (2 * SLOTS + 2 * kQueue) * 8;
+    static constexpr int kSmem = oMeta + SLOTS * 4 + 1024;  // + alignment of the base
+    static_assert(oBar % 8 == 0 && oRuns % 16 == 0 && oStat % 8 == 0 && oShare % 1024 == 0 && kSlot % 1024 == 0, "alignment");
     static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
-// What a CTA does next: tiles [from, to) of a unit (16 heads of a row). Tile i stands at position 32 i below
+// What a CTA does next: tiles [from, to) of 16 heads of a row, from h0 on. Tile i stands at position 32 i below
 // `sinks` tiles, behind them `skip` tiles further.
-struct Run {
-    int row, block, unit, len, n, sinks, skip, from, to, part;  // part: slot of partial results, -1: the whole unit
+struct alignas(16) Run {
+    int row, h0, len, sinks, skip, from, to;
+    int part;  // slot of partial results, -1: the whole row
     __device__ __forceinline__ int position(int i) const { return kTile * (i < sinks ? i : i + skip); }
 };
 
@@ -76,19 +82,19 @@ struct Run {
 __device__ __forceinline__ int row_tiles(const Attention& p, int len, int& sink_tiles, int& skip) {
     const int start = window_start(p, len), all = (len + kTile - 1) / kTile;
     sink_tiles = (min(p.sinks, start) + kTile - 1) / kTile;
-    const int first = max(start / kTile, sink_tiles);
-    skip = first - sink_tiles;
+    skip = max(start / kTile, sink_tiles) - sink_tiles;
     return all - skip;
 }
 
-// The runs of a CTA, the same in every warp.
+// The runs of a CTA. With even shares, the CTA's are the tiles of weight [w0, w1) of all rows in line, where a
+// row's tiles are followed by kRowCost more.
 struct Runs {
     const MmaArgs& a;
-    long long w0, w1, span, before;  // the share, and the weight ahead of row `row`
+    int w0, w1, span, before;  // the share, and the weight ahead of row `row`
     int row, block, len;
-    __device__ __forceinline__ Runs(const MmaArgs& args, long long span_, int row0, long long before0) : a(args), span(span_) {
+    __device__ __forceinline__ Runs(const MmaArgs& args, int span_, int row0, int before0) : a(args), span(span_) {
         if (a.shares) {
-            w0 = static_cast<long long>(blockIdx.x) * span;
+            w0 = static_cast<int>(blockIdx.x) * span;
             w1 = w0 + span;
             row = row0;
             before = before0;
@@ -99,42 +105,39 @@ struct Runs {
         }
         len = row < a.p.B ? length_of(a.p, row) : 0;
     }
-    __device__ __forceinline__ bool next(Run& r) {
+    // cut: the unit's parts where it begins here (0: it is whole), else -1.
+    __device__ __forceinline__ bool next(Run& r, int& cut) {
         while (row < a.p.B) {
             r.row = row;
-            r.block = block;
+            r.h0 = block * 16;
             r.len = len;
-            r.unit = row * a.blocks + block;
-            r.n = row_tiles(a.p, len, r.sinks, r.skip);
+            const int n = row_tiles(a.p, len, r.sinks, r.skip);
             if (!a.shares) {
                 r.from = 0;
-                r.to = r.n;
-                r.part = -1;
-                const int u = r.unit + static_cast<int>(gridDim.x);
+                r.to = n;
+                r.part = cut = -1;
+                const int u = row * a.blocks + block + static_cast<int>(gridDim.x);
                 row = u / a.blocks;
                 block = u - row * a.blocks;
                 if (row < a.p.B) len = length_of(a.p, row);
                 return true;
             }
-            const long long weight = r.n + kRowCost, at = before + block * weight;
+            const int at = before + block * (n + kRowCost);
             if (at >= w1) return false;
-            r.from = static_cast<int>(min(max(w0 - at, 0LL), static_cast<long long>(r.n)));
-            r.to = static_cast<int>(min(w1 - at, static_cast<long long>(r.n)));
             const bool begins = at >= w0;
-            r.part = begins && r.to == r.n ? -1 : 2 * static_cast<int>(blockIdx.x) + (begins ? 1 : 0);
+            r.from = begins ? 0 : min(w0 - at, n);
+            r.to = min(w1 - at, n);
+            const bool whole = begins && r.to == n;
+            r.part = whole ? -1 : 2 * static_cast<int>(blockIdx.x) + (begins ? 1 : 0);
+            cut = !begins ? -1 : whole ? 0 : (at + n - 1) / span - static_cast<int>(blockIdx.x) + 1;
             if (++block == a.blocks) {
                 block = 0;
-                before += a.blocks * weight;
+                before += a.blocks * (n + kRowCost);
                 if (++row < a.p.B) len = length_of(a.p, row);
             }
             if (begins || r.from < r.to) return true;
         }
         return false;
-    }
-    // Parts of a unit that begins here and does not end here.
-    __device__ __forceinline__ int parts(const Run& r) const {
-        // its first tile's weight is w1 - to, so its last tile lies this many shares further
-        return static_cast<int>((w1 - r.to + r.n - 1) / span) - static_cast<int>(blockIdx.x) + 1;
     }
 };
 
@@ -178,7 +181,17 @@ __device__ __forceinline__ uint32_t codes2(uint32_t two) {  // two e4m3 codes as
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffff), __NV_E4M3);
     return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
 }
+// The four warps of the products, all of their threads.
 __device__ __forceinline__ void products_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool products_any(bool p) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r)
+        : "r"(static_cast<uint32_t>(p))
+        : "memory");
+    return r != 0;
+}
 __device__ __forceinline__ float quad_max(float v) {
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
     return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
@@ -199,14 +212,18 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                      const __grid_constant__ CUtensorMap map_rope, const __grid_constant__ CUtensorMap map_scale) {
     using C = MmaCfg<KV, R, Q8>;
     using TP = std::conditional_t<Q8, __half, T>;  // the second product's type (codes are exact in fp16)
-    constexpr float kLift = std::is_same<TP, __half>::value ? 10.f : 0.f;  // log2 of the largest weight: small ones stay normal
+    // log2 of the largest weight when its reference is taken: small fp16 ones stay normal, large ones below 2^16
+    constexpr float kGrowth = 8.f, kLift = !std::is_same<TP, __half>::value ? 0.f : C::CW > 1 ? 6.f : 10.f;
     extern __shared__ uint8_t mma_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(mma_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::oBar);
     uint64_t* empty = full + C::SLOTS;
-    volatile uint32_t* meta = reinterpret_cast<volatile uint32_t*>(smem + C::oMeta);
-    long long* plan = reinterpret_cast<long long*>(smem + C::oPlan);  // span, before, row; then a flag
-    volatile int* bad = reinterpret_cast<volatile int*>(smem + C::oPlan + 24);
+    uint64_t* run_full = empty + C::SLOTS;
+    uint64_t* run_empty = run_full + kQueue;
+    Run* queue = reinterpret_cast<Run*>(smem + C::oRuns);
+    volatile uint16_t* meta = reinterpret_cast<volatile uint16_t*>(smem + C::oMeta);  // per slot and 16 positions
+    int* plan = reinterpret_cast<int*>(smem + C::oPlan);  // the warps' sums; span, weight ahead, row
+    volatile int* bad = reinterpret_cast<volatile int*>(smem + C::oPlan + 44);
     const Attention& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -214,6 +231,10 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
         for (int i = 0; i < C::SLOTS; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], C::CW);
+        }
+        for (int i = 0; i < kQueue; ++i) {
+            mbar_init(&run_full[i], 1);
+            mbar_init(&run_empty[i], 4);
         }
         fence_mbar_init();
         *bad = 0;
@@ -225,41 +246,44 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
     }
     MM_PDL_ENTRY();
     if (a.shares) {
-        // the weight of all rows, and the row that this CTA's share begins in
-        long long* sums = reinterpret_cast<long long*>(smem);  // free until the first tile
+        // the weight of all rows, and the row that this CTA's share begins in: a thread sums some rows in line
         const int per = (p.B + kMmaThreads - 1) / kMmaThreads, b0 = tid * per, b1 = min(b0 + per, p.B);
         auto weight = [&](int b) {
             int st, skip;
-            return static_cast<long long>(row_tiles(p, length_of(p, b), st, skip) + kRowCost) * a.blocks;
+            return (row_tiles(p, length_of(p, b), st, skip) + kRowCost) * a.blocks;
         };
-        long long mine = 0;
+        int mine = 0;
+#pragma unroll 4
         for (int b = b0; b < b1; ++b) mine += weight(b);
-        sums[tid] = mine;
-        __syncthreads();
-        long long ahead = 0, total = 0;
-        for (int i = 0; i < kMmaThreads; ++i) {
-            const long long s = sums[i];
-            ahead += i < tid ? s : 0;
-            total += s;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
         }
-        const long long span = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kMinShare));
-        const long long w0 = static_cast<long long>(blockIdx.x) * span;
+        if (lane == 31) plan[warp] = upto;
+        __syncthreads();
+        int ahead = upto - mine, total = 0;
+#pragma unroll
+        for (int i = 0; i < kMmaThreads / 32; ++i) {
+            ahead += i < warp ? plan[i] : 0;
+            total += plan[i];
+        }
+        const int span = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), kMinShare);
+        const int w0 = static_cast<int>(blockIdx.x) * span;  // below the grid's shares, which fit 32 bits
         if (tid == 0) {
-            plan[0] = span;
-            if (w0 >= total) plan[2] = p.B;
+            plan[5] = span;
+            if (w0 >= total) plan[7] = p.B;
+            if (!a.by_unit) a.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
         }
         if (w0 >= ahead && w0 < ahead + mine) {
             int b = b0;
-            for (long long w; ahead + (w = weight(b)) <= w0; ++b) ahead += w;
-            plan[1] = ahead;
-            plan[2] = b;
+            for (int w; ahead + (w = weight(b)) <= w0; ++b) ahead += w;
+            plan[6] = ahead;
+            plan[7] = b;
         }
-        if (!a.by_unit && tid == 0) a.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
-        fence_proxy_async_smem();  // `sums`, before a tile lands there
     }
     __syncthreads();
-    Runs runs(a, a.shares ? plan[0] : 0, static_cast<int>(a.shares ? plan[2] : 0), a.shares ? plan[1] : 0);
-    Run run;
     bool ok = true;
     // a wait that ran out is recorded once; later waits of this thread are skipped
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -271,69 +295,79 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
 
     if (warp == 4) {
         // ------------------------------------------------------------ loads
-        int slot[C::KG];  // position in each group's ring
-        uint32_t phase = 0;  // bit g: parity of group g's round
-#pragma unroll
-        for (int g = 0; g < C::KG; ++g) slot[g] = 0;
-        const int per = kTile / a.box, page = p.pool.positions;
-        const int each = C::kBoxes + 1 + (Q8 ? 1 : 0);  // boxes of one stretch of `box` positions
-        // this lane's boxes of a tile: which stretch, which box of it (at most 18 of them)
-        const int stretch = lane / each, which = lane - stretch * each;
-        while (runs.next(run)) {
-            if (lane == 0 && a.shares && run.from == 0) {
-                const int parts = run.part < 0 ? 0 : runs.parts(run);
-                if (a.by_unit || parts) a.cut[a.by_unit ? run.unit : blockIdx.x] = make_int4(run.unit, parts, blockIdx.x, 0);
-            }
-            // lane l holds the page of stretch l of the 32 from `base` on, and of the next 32
-            auto pages_from = [&](int s) {
-                const int i = run.from + (s + lane) / per;
-                if (i >= run.to) return -1;
-                const int at = run.position(i) + (s + lane) % per * a.box;
-                if (at >= run.len) return -1;
-                const int id = __ldg(p.table.entry + run.row * p.table.stride + at / page);
-                return id >= 0 && id < p.pool.rows ? id : -1;
-            };
-            int base = 0, ids = pages_from(0), ids_next = pages_from(32);
-            for (int i = run.from; i < run.to; ++i) {
-                const int g = C::KG == 1 ? 0 : (i - run.from) % C::KG;
-                int s_of = 0;
-#pragma unroll
-                for (int x = 0; x < C::KG; ++x) s_of = x == g ? slot[x] : s_of;
-                const int s = g * C::SG + s_of;
-                const int first = (i - run.from) * per;
-                if (first - base == 32) {
-                    base = first;
-                    ids = ids_next;
-                    ids_next = pages_from(base + 32);
+        Runs runs(a, a.shares ? plan[5] : 0, a.shares ? plan[7] : 0, a.shares ? plan[6] : 0);
+        Run run;
+        // A step is a tile for each group. This lane's box of its group's tile: which stretch of `box` positions,
+        // which box of it (128 wide: 3 or 6 boxes for 8 lanes; 512 wide: at most 18 for 32).
+        constexpr int kLanes = 32 / C::KG, kEach = C::kBoxes + 1 + (Q8 ? 1 : 0);
+        const int group = lane / kLanes, sub = lane % kLanes, stretch = sub / kEach, which = sub % kEach;
+        const bool loads = stretch * a.box < kTile;
+        const int page = p.pool.positions;
+        const uint32_t offset = which < C::kBoxes    ? which * kTile * 128 + stretch * a.box * 128
+                                : which == C::kBoxes ? C::kLatent + stretch * a.box * R * 2
+                                                     : C::kLatent + C::kRope + stretch * 128;
+        const CUtensorMap* map = which < C::kBoxes ? &map_latent : which == C::kBoxes ? &map_rope : &map_scale;
+        const int column = which < C::kBoxes ? which * (Q8 ? 128 : 64) : Q8 ? 0 : KV;
+        int slot = 0, q = 0;
+        uint32_t phase = 0, q_phase = 0;  // parity of the round in this group's ring, in the queue
+        int cut;
+        while (ok) {
+            const bool more = runs.next(run, cut);
+            wait(&run_empty[q], q_phase ^ 1);
+            if (lane == 0) {
+                if (!more) run.row = -1;
+                queue[q] = run;
+                mbar_arrive(&run_full[q]);
+                if (more && (a.by_unit ? cut >= 0 : cut > 0)) {
+                    const int unit = run.row * a.blocks + run.h0 / 16;
+                    a.cut[a.by_unit ? unit : blockIdx.x] = make_int4(unit, cut, blockIdx.x, 0);
                 }
-                const int id0 = __shfl_sync(0xffffffffu, ids, first - base), id1 = __shfl_sync(0xffffffffu, ids, first - base + per - 1);
-                const int id = stretch == 0 ? id0 : id1;
-                wait(&empty[s], ((phase >> g) & 1) ^ 1);
-                if (__any_sync(0xffffffffu, !ok)) break;
-                if (lane == 0) {
-                    meta[s] = (id0 >= 0 ? 0xffffu : 0u) | (id1 >= 0 ? 0xffff0000u : 0u);
-                    mbar_arrive_expect_tx(&full[s], C::kBytes);
+            }
+            if (++q == kQueue) {
+                q = 0;
+                q_phase ^= 1;
+            }
+            if (!more) break;
+            // page and entry of this lane's stretch of tile i
+            int id, at;
+            auto ask = [&](int i) {
+                const int t = run.position(i) + stretch * a.box;
+                const int c = p.table.shift >= 0 ? t >> p.table.shift : t / page;
+                at = t - c * page;
+                id = -1;
+                if (loads && i < run.to && t < run.len) id = __ldg(p.table.entry + run.row * p.table.stride + c);
+            };
+            ask(run.from + group);
+            for (int i = run.from + group; i - group < run.to; i += C::KG) {
+                // a page outside the pool (or behind the row) is asked for behind the last one: zeros
+                const bool there = id >= 0 && id < p.pool.rows, mine = i < run.to;
+                const int z = there ? id : p.pool.rows, y = at;
+                ask(i + C::KG);
+                const int s = group * C::SG + slot;
+                if (mine) wait(&empty[s], phase ^ 1);
+                if (__any_sync(0xffffffffu, !ok)) {
+                    ok = false;
+                    break;
+                }
+                if (mine && loads && which == 0) {
+                    meta[2 * s + stretch] = there ? 0xffff : 0;
+                    if (a.box == kTile) meta[2 * s + 1] = there ? 0xffff : 0;
                 }
                 __syncwarp();
-                if (stretch < per) {
-                    // a page outside the pool (or behind the row) is asked for behind the last one: zeros
-                    const int at = (run.position(i) + stretch * a.box) % page, z = id >= 0 ? id : p.pool.rows;
-                    uint8_t* dst = smem + s * C::kSlot;
-                    if (which < C::kBoxes)
-                        tma_load_box(dst + which * kTile * 128 + stretch * a.box * 128, &map_latent, &full[s], which * (Q8 ? 128 : 64), at, z);
-                    else if (which == C::kBoxes)
-                        tma_load_box(dst + C::kLatent + stretch * a.box * R * 2, &map_rope, &full[s], Q8 ? 0 : KV, at, z);
-                    else
-                        tma_load_2d(dst + C::kLatent + C::kRope + stretch * 128, &map_scale, &full[s], at, z);
-                }
-#pragma unroll
-                for (int x = 0; x < C::KG; ++x)
-                    if (x == g && ++slot[x] == C::SG) {
-                        slot[x] = 0;
-                        phase ^= 1u << x;
+                if (mine && sub == 0) mbar_arrive_expect_tx(&full[s], C::kBytes);
+                __syncwarp();
+                if (mine) {
+                    if (loads) {
+                        uint8_t* dst = smem + s * C::kSlot + offset;
+                        if (Q8 && which > C::kBoxes) tma_load_2d(dst, map, &full[s], y, z);
+                        else tma_load_box(dst, map, &full[s], column, y, z);
                     }
+                    if (++slot == C::SG) {
+                        slot = 0;
+                        phase ^= 1;
+                    }
+                }
             }
-            if (!ok) break;
         }
     } else {
         // ------------------------------------------------------------ products
@@ -344,11 +378,29 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
         const int mrow = lane & 7, msel = lane >> 3;
         float* share = reinterpret_cast<float*>(smem + C::oShare);
         const float cs = p.scale * 1.4426950408889634f;
-        int slot = 0;
-        uint32_t phase = 0;
-        while (runs.next(run)) {
-            const int h0 = run.block * 16;
-            const int heads = min(16, p.H - h0);
+        // scales of the lane's positions 8 n + 2 t4 and the next (a second box of 16 starts 128 bytes on)
+        auto scales_of = [&](int sl, int n) {
+            const uint8_t* at = smem + (group * C::SG + sl) * C::kSlot + C::kLatent + C::kRope;
+            return *reinterpret_cast<const float2*>(at + (n * 8 + t4 * 2) * 4 + (n >= 2 && a.box == 16 ? 64 : 0));
+        };
+        int slot = 0, turn = 0;
+        uint32_t phase = 0, turn_phase = 0;
+        auto warp_arrive = [&](uint64_t* bar) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        while (true) {
+            wait(&run_full[turn], turn_phase);
+            if (products_any(!ok)) break;  // the four warps meet at barriers of their own: they leave together
+            const Run run = queue[turn];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&run_empty[turn]);
+            if (++turn == kQueue) {
+                turn = 0;
+                turn_phase ^= 1;
+            }
+            if (run.row < 0) break;
+            const int h0 = run.h0, heads = min(16, p.H - h0);
             uint32_t q[8][4], qr[4];
             float qf[2] = {1.f, 1.f};  // what the scores of codes are multiplied by (bf16 queries as fp16)
             {
@@ -417,50 +469,43 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
             for (int n = 0; n < 16; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
             float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
             const int start = window_start(p, run.len), sinks = min(p.sinks, start);
-            for (int i = run.from + group; i < run.to; i += C::KG) {
-                const uint32_t sp = ring + slot * C::kSlot;
-                wait(&full[group * C::SG + slot], phase);
-                // positions of the tile that the row sees
-                uint32_t seen = meta[group * C::SG + slot];
-                {
-                    const int p0 = run.position(i);
-                    auto below = [&](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
-                    seen &= below(run.len - p0) & (below(sinks - p0) | ~below(start - p0));
-                }
-                // ---- S
-                float s[4][4];
+            // S of the tile in slot sl: this warp's columns of it
+            auto scores = [&](int sl, float (&s)[4][4]) {
+                const uint32_t sp = ring + sl * C::kSlot;
 #pragma unroll
                 for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
                 if constexpr (!Q8) {
+                    // (loads one step ahead of the products: issue is in order)
                     const uint32_t box = sp + cw * 2 * (kTile * 128);
+                    uint32_t b[2][2][4];
+                    auto load = [&](int k, uint32_t (&d)[2][4]) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            uint32_t b[4];
-                            ldsm4(b, box + (k >> 2) * (kTile * 128) + swizzled(h * 16 + (msel >> 1) * 8 + mrow, (k & 3) * 2 + (msel & 1)));
-                            mma16<T>(s[2 * h], q[k], b[0], b[1]);
-                            mma16<T>(s[2 * h + 1], q[k], b[2], b[3]);
-                        }
-                } else {
-                    const uint32_t box = sp + cw * (kTile * 128);
+                        for (int h = 0; h < 2; ++h)
+                            ldsm4(d[h], box + (k >> 2) * (kTile * 128) + swizzled(h * 16 + (msel >> 1) * 8 + mrow, (k & 3) * 2 + (msel & 1)));
+                    };
+                    load(0, b[0]);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        uint32_t b[4];
-                        ldsm4(b, box + swizzled(msel * 8 + mrow, k));
+                        if (k < 7) load(k + 1, b[(k + 1) & 1]);
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) mma16<__half>(s[n], q[k], codes2(b[n]), codes2(b[n] >> 16));
+                        for (int h = 0; h < 2; ++h) {
+                            mma16<T>(s[2 * h], q[k], b[k & 1][h][0], b[k & 1][h][1]);
+                            mma16<T>(s[2 * h + 1], q[k], b[k & 1][h][2], b[k & 1][h][3]);
+                        }
                     }
-                }
-                float ks[8];  // scales of the lane's positions: 8 n + 2 t4 + e
-                if constexpr (Q8) {
-                    const float* sc = reinterpret_cast<const float*>(smem + (group * C::SG + slot) * C::kSlot + C::kLatent + C::kRope);
-                    const int gap = a.box == 16 ? 16 : 0;  // a second box of 16 starts 128 bytes on
+                } else {
+                    const uint32_t box = sp + cw * (kTile * 128);
+                    uint32_t b[2][4];
+                    ldsm4(b[0], box + swizzled(msel * 8 + mrow, 0));
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        if (k < 7) ldsm4(b[(k + 1) & 1], box + swizzled(msel * 8 + mrow, k + 1));
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) mma16<__half>(s[n], q[k], codes2(b[k & 1][n]), codes2(b[k & 1][n] >> 16));
+                    }
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
-                        const float2 v = *reinterpret_cast<const float2*>(sc + n * 8 + t4 * 2 + (n >= 2 ? gap : 0));
-                        ks[2 * n] = v.x;
-                        ks[2 * n + 1] = v.y;
+                        const float2 v = scales_of(sl, n);
                         s[n][0] *= qf[0] * v.x;
                         s[n][1] *= qf[0] * v.y;
                         s[n][2] *= qf[1] * v.x;
@@ -476,34 +521,32 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                         mma16<T>(s[2 * h + 1], qr, b[2], b[3]);
                     }
                 }
-                if constexpr (C::CW > 1) {
-                    // the four warps' shares, added in the same order by each
-                    float4* mine = reinterpret_cast<float4*>(share) + cw * 128 + lane;
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) mine[n * 32] = make_float4(s[n][0], s[n][1], s[n][2], s[n][3]);
-                    products_sync();
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const float4* v = reinterpret_cast<const float4*>(share) + n * 32 + lane;
-                        const float4 x = v[0], y = v[128], z = v[256], w = v[384];
-                        s[n][0] = (x.x + y.x) + (z.x + w.x);
-                        s[n][1] = (x.y + y.y) + (z.y + w.y);
-                        s[n][2] = (x.z + y.z) + (z.z + w.z);
-                        s[n][3] = (x.w + y.w) + (z.w + w.w);
-                    }
-                    products_sync();
-                }
-                // ---- softmax
+            };
+            // positions of tile i that the row sees
+            auto seen_of = [&](int sl, int i) {
+                const uint32_t there = meta[2 * (group * C::SG + sl)] | static_cast<uint32_t>(meta[2 * (group * C::SG + sl) + 1]) << 16;
+                const int p0 = run.position(i);
+                auto below = [&](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+                return there & below(run.len - p0) & (below(sinks - p0) | ~below(start - p0));
+            };
+            // Weights of tile i (the second product's operand, 16 positions each) from its scores.
+            auto weigh = [&](int sl, int i, float (&s)[4][4], uint32_t (&w)[2][4]) {
+                const uint32_t seen = seen_of(sl, i);
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
+                for (int n = 0; n < 4; ++n) {
+                    float2 e2 = make_float2(0.f, 0.f);
+                    if constexpr (Q8) {
+                        const float2 v = scales_of(sl, n);
+                        e2 = make_float2(exponent_of(v.x), exponent_of(v.y));
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         s[n][e] *= cs;
-                        const int key = n * 8 + t4 * 2 + (e & 1);
-                        if (seen != ~0u && !((seen >> key) & 1)) s[n][e] = -INFINITY;
-                        top[e >> 1] = fmaxf(top[e >> 1], Q8 ? s[n][e] + exponent_of(ks[2 * n + (e & 1)]) : s[n][e]);
+                        if (seen != ~0u && !((seen >> (n * 8 + t4 * 2 + (e & 1))) & 1)) s[n][e] = -INFINITY;
+                        top[e >> 1] = fmaxf(top[e >> 1], Q8 ? s[n][e] + (e & 1 ? e2.y : e2.x) : s[n][e]);
                     }
+                }
                 float corr[2], ref[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -524,23 +567,34 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     l[0] *= corr[0];
                     l[1] *= corr[1];
                 }
-                uint32_t w[2][4];  // the weights as the second product's operand: 16 positions each
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
+                    float2 v = make_float2(1.f, 1.f);
+                    if constexpr (Q8) {
+                        v = scales_of(sl, n);
+                        if (seen != ~0u) {  // (0 times what an unseen position has for a scale may be a NaN)
+                            if (!((seen >> (n * 8 + t4 * 2)) & 1)) v.x = 0.f;
+                            if (!((seen >> (n * 8 + t4 * 2 + 1)) & 1)) v.y = 0.f;
+                        }
+                    }
                     float e[4];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         e[x] = fast_exp2(s[n][x] - ref[x >> 1]);
                         l[x >> 1] += e[x];
-                        if (Q8) e[x] = seen == ~0u || ((seen >> (n * 8 + t4 * 2 + (x & 1))) & 1) ? e[x] * ks[2 * n + (x & 1)] : 0.f;
+                        if (Q8) e[x] *= x & 1 ? v.y : v.x;
                     }
                     w[n >> 1][(n & 1) * 2] = lat::pack2<TP>(e[0], e[1]);
                     w[n >> 1][(n & 1) * 2 + 1] = lat::pack2<TP>(e[2], e[3]);
                 }
-                // ---- positions that are not seen hold anything
-                if (seen != ~0u) {
+                return seen;
+            };
+            // O += P V over this warp's columns, and the slot goes back
+            auto values = [&](int sl, uint32_t seen, const uint32_t (&w)[2][4]) {
+                const uint32_t sp = ring + sl * C::kSlot;
+                if (seen != ~0u) {  // positions that are not seen hold anything
                     __syncwarp();
-                    uint8_t* boxes = smem + (group * C::SG + slot) * C::kSlot + cw * (Q8 ? 1 : 2) * (kTile * 128);
+                    uint8_t* boxes = smem + (group * C::SG + sl) * C::kSlot + cw * (Q8 ? 1 : 2) * (kTile * 128);
                     for (uint32_t hide = ~seen; hide; hide &= hide - 1) {
                         const int r = __ffs(hide) - 1;
                         if (lane < (Q8 ? 8 : 16))
@@ -548,48 +602,181 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     }
                     __syncwarp();
                 }
-                // ---- O
                 if constexpr (!Q8) {
                     const uint32_t box = sp + cw * 2 * (kTile * 128);
+                    uint32_t b[2][2][4];
+                    auto load = [&](int c, uint32_t (&d)[2][4]) {
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
+                        for (int k = 0; k < 2; ++k)
+                            ldsm4_t(d[k], box + (c >> 2) * (kTile * 128) + swizzled(k * 16 + (msel & 1) * 8 + mrow, (c & 3) * 2 + (msel >> 1)));
+                    };
+                    load(0, b[0]);
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            uint32_t b[4];
-                            ldsm4_t(b, box + (c >> 2) * (kTile * 128) + swizzled(k * 16 + (msel & 1) * 8 + mrow, (c & 3) * 2 + (msel >> 1)));
-                            mma16<T>(o[2 * c], w[k], b[0], b[1]);
-                            mma16<T>(o[2 * c + 1], w[k], b[2], b[3]);
+                    for (int c = 0; c < 8; ++c) {
+                        if (c < 7) load(c + 1, b[(c + 1) & 1]);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            mma16<T>(o[2 * c], w[k], b[c & 1][k][0], b[c & 1][k][1]);
+                            mma16<T>(o[2 * c + 1], w[k], b[c & 1][k][2], b[c & 1][k][3]);
                         }
+                    }
                 } else {
                     // a transposed pair of codes is two neighbouring columns of one position: the even columns of 16
                     // make one tile of the product, the odd ones another
                     const uint32_t box = sp + cw * (kTile * 128);
+                    uint32_t b[2][4];
+                    auto load = [&](int j, uint32_t (&d)[4]) {
+                        ldsm4_t(d, box + swizzled((j >> 2) * 16 + (msel & 1) * 8 + mrow, (j & 3) * 2 + (msel >> 1)));
+                    };
+                    load(0, b[0]);
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
+                    for (int j = 0; j < 8; ++j) {
+                        const int k = j >> 2, c = j & 3;
+                        if (j < 7) load(j + 1, b[(j + 1) & 1]);
+                        uint32_t v[4];
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t b[4];
-                            ldsm4_t(b, box + swizzled(k * 16 + (msel & 1) * 8 + mrow, c * 2 + (msel >> 1)));
+                        for (int x = 0; x < 4; ++x) v[x] = __byte_perm(b[j & 1][x], 0, 0x3120);
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) b[x] = __byte_perm(b[x], 0, 0x3120);
-#pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                mma16<__half>(o[4 * c + 2 * x], w[k], codes2(b[2 * x]), codes2(b[2 * x + 1]));
-                                mma16<__half>(o[4 * c + 2 * x + 1], w[k], codes2(b[2 * x] >> 16), codes2(b[2 * x + 1] >> 16));
-                            }
+                        for (int x = 0; x < 2; ++x) {
+                            mma16<__half>(o[4 * c + 2 * x], w[k], codes2(v[2 * x]), codes2(v[2 * x + 1]));
+                            mma16<__half>(o[4 * c + 2 * x + 1], w[k], codes2(v[2 * x] >> 16), codes2(v[2 * x + 1] >> 16));
                         }
+                    }
                 }
                 if (seen != ~0u) fence_proxy_async_smem();  // the cleared rows, before the next tile lands on them
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[group * C::SG + slot]);
-                if (++slot == C::SG) {
-                    slot = 0;
-                    phase ^= 1;
+                warp_arrive(&empty[group * C::SG + sl]);
+            };
+            uint32_t w[2][4];
+            float s[4][4];
+            if constexpr (C::CW == 1) {
+                for (int i = run.from + group; i < run.to; i += C::KG) {
+                    wait(&full[group * C::SG + slot], phase);
+                    scores(slot, s);
+                    const uint32_t seen = weigh(slot, i, s, w);
+                    values(slot, seen, w);
+                    if (++slot == C::SG) {
+                        slot = 0;
+                        phase ^= 1;
+                    }
+                }
+            } else {
+                // Each warp adds the four shares of S for 8 of the tile's positions and hands their weights to the
+                // others. The reference of the weights is the running maximum when it last moved, which it does
+                // only where a score passes it by 2^8 (or there was none): the warps vote on it with the barrier that
+                // hands the weights over. The next tile's shares are made before this tile's O product, which hides
+                // their exchange.
+                float4* mine = reinterpret_cast<float4*>(share) + cw * 128 + lane;
+                uint2* hand = reinterpret_cast<uint2*>(smem + C::oHand) + lane;
+                float* tops = reinterpret_cast<float*>(smem + C::oTops);
+                auto put = [&](int sl) {  // (the last tile's shares were read before its weights were handed over)
+                    scores(sl, s);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) mine[n * 32] = make_float4(s[n][0], s[n][1], s[n][2], s[n][3]);
+                };
+                if (run.from < run.to) {
+                    wait(&full[slot], phase);
+                    put(slot);
+                }
+                for (int i = run.from; i < run.to; ++i) {
+                    products_sync();
+                    float z[4];
+                    {
+                        const float4* v = reinterpret_cast<const float4*>(share) + cw * 32 + lane;
+                        const float4 x = v[0], y = v[128], f = v[256], u = v[384];
+                        z[0] = ((x.x + y.x) + (f.x + u.x)) * cs;
+                        z[1] = ((x.y + y.y) + (f.y + u.y)) * cs;
+                        z[2] = ((x.z + y.z) + (f.z + u.z)) * cs;
+                        z[3] = ((x.w + y.w) + (f.w + u.w)) * cs;
+                    }
+                    const uint32_t seen = seen_of(slot, i);
+                    const bool see0 = (seen >> (cw * 8 + t4 * 2)) & 1, see1 = (seen >> (cw * 8 + t4 * 2 + 1)) & 1;
+                    if (!see0) z[0] = z[2] = -INFINITY;
+                    if (!see1) z[1] = z[3] = -INFINITY;
+                    float2 ks = make_float2(1.f, 1.f), e2 = make_float2(0.f, 0.f);
+                    if constexpr (Q8) {
+                        ks = scales_of(slot, cw);
+                        e2 = make_float2(exponent_of(ks.x), exponent_of(ks.y));
+                        if (!see0) ks.x = 0.f;  // (0 times what an unseen position has for a scale may be a NaN)
+                        if (!see1) ks.y = 0.f;
+                    }
+                    const float top0 = fmaxf(z[0] + e2.x, z[1] + e2.y), top1 = fmaxf(z[2] + e2.x, z[3] + e2.y);
+                    float add[2];
+                    auto give = [&] {
+                        float e[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) e[x] = fast_exp2(z[x] - ((m[x >> 1] == -INFINITY ? 0.f : m[x >> 1]) - kLift));
+                        add[0] = e[0] + e[1];
+                        add[1] = e[2] + e[3];
+                        if constexpr (Q8) {
+                            e[0] *= ks.x;
+                            e[1] *= ks.y;
+                            e[2] *= ks.x;
+                            e[3] *= ks.y;
+                        }
+                        hand[cw * 32] = make_uint2(lat::pack2<TP>(e[0], e[1]), lat::pack2<TP>(e[2], e[3]));
+                    };
+                    give();
+                    if (products_any(top0 > m[0] + kGrowth || top1 > m[1] + kGrowth)) {
+                        // the maximum over the tile, and the sums and products so far below it
+                        const float a0 = quad_max(top0), a1 = quad_max(top1);
+                        if (t4 == 0) {
+                            tops[cw * 16 + g] = a0;
+                            tops[cw * 16 + g + 8] = a1;
+                        }
+                        products_sync();
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float* t = tops + g + 8 * h;
+                            const float mn = fmaxf(fmaxf(m[h], fmaxf(t[0], t[16])), fmaxf(t[32], t[48]));
+                            const float corr = m[h] == mn ? 1.f : fast_exp2(m[h] - mn);
+                            m[h] = mn;
+                            l[h] *= corr;
+#pragma unroll
+                            for (int n = 0; n < 16; ++n) {
+                                o[n][2 * h] *= corr;
+                                o[n][2 * h + 1] *= corr;
+                            }
+                        }
+                        give();
+                        products_sync();
+                    }
+                    l[0] += add[0];
+                    l[1] += add[1];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const uint2 v = hand[n * 32];
+                        w[n >> 1][(n & 1) * 2] = v.x;
+                        w[n >> 1][(n & 1) * 2 + 1] = v.y;
+                    }
+                    const int sl = slot;
+                    if (++slot == C::SG) {
+                        slot = 0;
+                        phase ^= 1;
+                    }
+                    if (i + 1 < run.to) {
+                        wait(&full[slot], phase);
+                        put(slot);
+                    }
+                    values(sl, seen, w);
                 }
             }
             // ------------------------------------------------------------ results
             l[0] = quad_sum(l[0]);
             l[1] = quad_sum(l[1]);
+            if constexpr (C::CW > 1) {  // of the positions that each warp weighed
+                float* sums = reinterpret_cast<float*>(smem + C::oTops);
+                products_sync();
+                if (t4 == 0) {
+                    sums[cw * 16 + g] = l[0];
+                    sums[cw * 16 + g + 8] = l[1];
+                }
+                products_sync();
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float* t = sums + g + 8 * h;
+                    l[h] = (t[0] + t[16]) + (t[32] + t[48]);
+                }
+            }
             if (!ok || *bad) l[0] = l[1] = __int_as_float(0x7fc00000);
             const bool whole = run.part < 0;
             const long long first = static_cast<long long>(run.row) * p.H + h0;  // query row
@@ -701,57 +888,66 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
 }
 
 // Joins the parts of the units that were cut. Block (entry of the cut list, y) of 8 warps; a task is 128
-// columns of a head. Few parts: a warp a task; many: the warps divide the parts.
+// columns of a head. Up to kFew parts: a warp a task, all of its parts asked for at once; more: the warps of a
+// block divide a task's parts.
+constexpr int kFew = 8;
+struct Partial {  // a weighted mean in the making: 4 columns, maximum and sum
+    float4 o;
+    float m, l;
+    __device__ __forceinline__ void add(float4 v, float2 ml) {
+        const float top = fmaxf(m, ml.x), f = fast_exp2(m - top), g = fast_exp2(ml.x - top);
+        o = make_float4(fmaf(v.x, g, o.x * f), fmaf(v.y, g, o.y * f), fmaf(v.z, g, o.z * f), fmaf(v.w, g, o.w * f));
+        l = fmaf(ml.y, g, l * f);
+        m = top;
+    }
+};
 template <int KV, typename T>
-__global__ void __launch_bounds__(256) paged_join_kernel(const MmaArgs a) {
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ MmaArgs a) {
     MM_PDL_ENTRY();
     constexpr int NS = KV / 128;
     __shared__ float4 sum_s[8][32];
+    __shared__ float2 ml_s[8];
     const int4 cut = __ldcg(&a.cut[blockIdx.x]);
-    if (cut.y == 0) return;
+    const int parts = cut.y;
+    if (parts == 0) return;
     const Attention& p = a.p;
     const int row = cut.x / a.blocks, h0 = (cut.x - row * a.blocks) * 16, heads = min(16, p.H - h0);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = cut.y;
-    auto slot = [&](int i) { return i == 0 ? 2 * cut.z + 1 : 2 * (cut.z + i); };
-    const bool many = parts > 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool many = parts > kFew;
     for (int task = many ? blockIdx.y : blockIdx.y * 8 + warp; task < heads * NS; task += gridDim.y * (many ? 1 : 8)) {
         const int h = task / NS, c = (task - h * NS) * 128 + lane * 4;
-        float M = kNone, L = 0.f;
-        for (int i = lane; i < parts; i += 32) M = fmaxf(M, __ldcg(&a.part_ml[slot(i) * 16 + h]).x);
-        M = warp_max(M);
-        for (int i = lane; i < parts; i += 32) {
-            const float2 v = __ldcg(&a.part_ml[slot(i) * 16 + h]);
-            L += v.y * fast_exp2(v.x - M);
-        }
-        L = warp_sum(L);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int i = many ? warp : 0; i < parts; i += many ? 8 : 1) {
-            const float f = fast_exp2(__ldcg(&a.part_ml[slot(i) * 16 + h]).x - M);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + (static_cast<long long>(slot(i)) * 16 + h) * KV + c));
-            acc.x = fmaf(v.x, f, acc.x);
-            acc.y = fmaf(v.y, f, acc.y);
-            acc.z = fmaf(v.z, f, acc.z);
-            acc.w = fmaf(v.w, f, acc.w);
-        }
-        if (many) {
-            __syncthreads();
-            sum_s[warp][lane] = acc;
+        Partial sum{make_float4(0.f, 0.f, 0.f, 0.f), kNone, 0.f};
+        // parts i0, i0 + step, ...
+        auto take = [&](int i0, int step) {
+            float4 v[kFew];
+            float2 ml[kFew];
+#pragma unroll
+            for (int k = 0; k < kFew; ++k) {
+                const int i = i0 + k * step, at = (i == 0 ? 2 * cut.z + 1 : 2 * (cut.z + i)) * 16 + h;
+                if (i >= parts) continue;
+                v[k] = __ldcg(reinterpret_cast<const float4*>(a.part_o + static_cast<long long>(at) * KV + c));
+                ml[k] = __ldcg(&a.part_ml[at]);
+            }
+#pragma unroll
+            for (int k = 0; k < kFew; ++k)
+                if (i0 + k * step < parts) sum.add(v[k], ml[k]);
+        };
+        if (!many) {
+            take(0, 1);
+        } else {
+            for (int i = warp; i < parts; i += 8 * kFew) take(i, 8);
+            __syncthreads();  // the last task's sums have been read
+            sum_s[warp][lane] = sum.o;
+            if (lane == 0) ml_s[warp] = make_float2(sum.m, sum.l);
             __syncthreads();
             if (warp) continue;
-            for (int w = 1; w < 8; ++w) {
-                const float4 v = sum_s[w][lane];
-                acc.x += v.x;
-                acc.y += v.y;
-                acc.z += v.z;
-                acc.w += v.w;
-            }
+            for (int w = 1; w < 8; ++w) sum.add(sum_s[w][lane], ml_s[w]);
         }
-        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const float inv = sum.l == 0.f ? 0.f : 1.f / sum.l;
         const long long r = static_cast<long long>(row) * p.H + h0 + h;
         *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + r * KV + c) =
-            make_uint2(lat::pack2<T>(acc.x * inv, acc.y * inv), lat::pack2<T>(acc.z * inv, acc.w * inv));
-        if (p.lse && lane == 0 && c == 0) p.lse[r] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+            make_uint2(lat::pack2<T>(sum.o.x * inv, sum.o.y * inv), lat::pack2<T>(sum.o.z * inv, sum.o.w * inv));
+        if (p.lse && lane == 0 && c == 0) p.lse[r] = sum.l == 0.f ? -INFINITY : (sum.m + log2f(sum.l)) * 0.6931471805599453f;
     }
 }
 
