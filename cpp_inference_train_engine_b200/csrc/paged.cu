@@ -154,10 +154,10 @@ MmaPlan mma_plan(const mm::paged::Attention& p) {
     r.units = static_cast<int64_t>(p.B) * r.blocks;
     const int64_t all = (static_cast<int64_t>(p.max_length) + kTile - 1) / kTile;
     const int64_t tiles = p.window > 0 ? std::min(all, (static_cast<int64_t>(p.window) + p.sinks) / kTile + 3) : all;
-    const int64_t ctas = 2 * sm_count();
+    const int64_t ctas = 2 * sm_count(), least = min_share(p.kv);
     // rows of few tiles are not worth cutting (and weights are 32-bit)
-    r.shares = tiles > kMinShare && r.units * (tiles + kRowCost) < INT32_MAX / 2;
-    r.grid = static_cast<int>(std::min(ctas, r.shares ? (r.units * (tiles + kRowCost) + kMinShare - 1) / kMinShare : r.units));
+    r.shares = tiles > least && r.units * (tiles + kRowCost) < INT32_MAX / 2;
+    r.grid = static_cast<int>(std::min(ctas, r.shares ? (r.units * (tiles + kRowCost) + least - 1) / least : r.units));
     r.entries = static_cast<int>(std::min<int64_t>(r.units, r.grid));
     return r;
 }
@@ -178,8 +178,8 @@ void run_mma(const mm::paged::Attention& p, const MmaPlan& r, const PoolMaps& ma
     set_dynamic_smem<paged_mma_kernel<KV, R, T, Q8>>(C::kSmem);
     launch(s, paged_mma_kernel<KV, R, T, Q8>, dim3(r.grid), dim3(kMmaThreads), C::kSmem, a, maps.latent, maps.rope, maps.scale);
     if (r.shares) {
-        // a warp a task, or a block a task where the parts are many because the units are few
-        const int y = std::max(2 * KV / 128, std::min(2 * sm_count() / r.entries, 16 * KV / 128));
+        // a warp a head, or a block for 128 columns of one where the parts are many because the units are few
+        const int y = std::max(2, std::min(2 * sm_count() / r.entries, 16 * KV / 128));
         launch(s, paged_join_kernel<KV, T>, dim3(r.entries, y), dim3(256), 0, a);
     }
 }

@@ -39,7 +39,8 @@ struct MmaArgs {
 
 constexpr int kTile = 32;       // positions
 constexpr int kRowCost = 2;     // tiles that a row's queries and results cost
-constexpr int kMinShare = 6;    // tiles of a CTA at least
+// tiles of a CTA at least (128 wide they are a quarter of the bytes, and each of the four warps has its own)
+constexpr int min_share(int kv) { return kv == 128 ? 16 : 6; }
 constexpr int kMmaThreads = 160;
 constexpr int kQueue = 4;       // runs queued for the warps of the products
 constexpr float kNone = -3.402823466e38f;  // maximum of nothing (finite: its exp2 is 0, never NaN)
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
             ahead += i < warp ? plan[i] : 0;
             total += plan[i];
         }
-        const int span = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), kMinShare);
+        const int span = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), min_share(KV));
         const int w0 = static_cast<int>(blockIdx.x) * span;  // below the grid's shares, which fit 32 bits
         if (tid == 0) {
             plan[5] = span;
@@ -887,24 +888,27 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
     }
 }
 
-// Joins the parts of the units that were cut. Block (entry of the cut list, y) of 8 warps; a task is 128
-// columns of a head. Up to kFew parts: a warp a task, all of its parts asked for at once; more: the warps of a
-// block divide a task's parts.
+// Joins the parts of the units that were cut. Block (entry of the cut list, y) of 8 warps. Up to kFew parts: a warp
+// takes a head, eight 16-byte loads a lane at a time; more: the warps of a block divide the parts of 128 columns of
+// a head.
 constexpr int kFew = 8;
-struct Partial {  // a weighted mean in the making: 4 columns, maximum and sum
-    float4 o;
-    float m, l;
-    __device__ __forceinline__ void add(float4 v, float2 ml) {
+struct Mean {  // a weighted mean in the making: maximum and sum of the weights
+    float m = kNone, l = 0.f;
+    // Factors of what there is and of a part that comes.
+    __device__ __forceinline__ float2 add(float2 ml) {
         const float top = fmaxf(m, ml.x), f = fast_exp2(m - top), g = fast_exp2(ml.x - top);
-        o = make_float4(fmaf(v.x, g, o.x * f), fmaf(v.y, g, o.y * f), fmaf(v.z, g, o.z * f), fmaf(v.w, g, o.w * f));
         l = fmaf(ml.y, g, l * f);
         m = top;
+        return make_float2(f, g);
     }
 };
+__device__ __forceinline__ void blend(float4& o, float4 v, float2 f) {
+    o = make_float4(fmaf(v.x, f.y, o.x * f.x), fmaf(v.y, f.y, o.y * f.x), fmaf(v.z, f.y, o.z * f.x), fmaf(v.w, f.y, o.w * f.x));
+}
 template <int KV, typename T>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ MmaArgs a) {
     MM_PDL_ENTRY();
-    constexpr int NS = KV / 128;
+    constexpr int NS = KV / 128, PER = 8 / NS;
     __shared__ float4 sum_s[8][32];
     __shared__ float2 ml_s[8];
     const int4 cut = __ldcg(&a.cut[blockIdx.x]);
@@ -913,41 +917,70 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     const Attention& p = a.p;
     const int row = cut.x / a.blocks, h0 = (cut.x - row * a.blocks) * 16, heads = min(16, p.H - h0);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool many = parts > kFew;
-    for (int task = many ? blockIdx.y : blockIdx.y * 8 + warp; task < heads * NS; task += gridDim.y * (many ? 1 : 8)) {
-        const int h = task / NS, c = (task - h * NS) * 128 + lane * 4;
-        Partial sum{make_float4(0.f, 0.f, 0.f, 0.f), kNone, 0.f};
-        // parts i0, i0 + step, ...
-        auto take = [&](int i0, int step) {
-            float4 v[kFew];
-            float2 ml[kFew];
+    auto slot = [&](int i) { return i == 0 ? 2 * cut.z + 1 : 2 * (cut.z + i); };
+    const long long first = static_cast<long long>(row) * p.H + h0;
+    auto finish = [&](int h, int c, float4 o, const Mean& sum) {
+        const float inv = sum.l == 0.f ? 0.f : 1.f / sum.l;
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (first + h) * KV + c) =
+            make_uint2(lat::pack2<T>(o.x * inv, o.y * inv), lat::pack2<T>(o.z * inv, o.w * inv));
+        if (p.lse && c == 0) p.lse[first + h] = sum.l == 0.f ? -INFINITY : (sum.m + log2f(sum.l)) * 0.6931471805599453f;
+    };
+    if (parts <= kFew) {
+        for (int h = blockIdx.y * 8 + warp; h < heads; h += gridDim.y * 8) {
+            Mean sum;
+            float4 o[NS];
 #pragma unroll
-            for (int k = 0; k < kFew; ++k) {
-                const int i = i0 + k * step, at = (i == 0 ? 2 * cut.z + 1 : 2 * (cut.z + i)) * 16 + h;
-                if (i >= parts) continue;
-                v[k] = __ldcg(reinterpret_cast<const float4*>(a.part_o + static_cast<long long>(at) * KV + c));
-                ml[k] = __ldcg(&a.part_ml[at]);
+            for (int x = 0; x < NS; ++x) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i0 = 0; i0 < parts; i0 += PER) {
+                float4 v[PER][NS];
+                float2 ml[PER];
+#pragma unroll
+                for (int k = 0; k < PER; ++k) {
+                    if (i0 + k >= parts) continue;
+                    const int at = slot(i0 + k) * 16 + h;
+                    ml[k] = __ldcg(&a.part_ml[at]);
+#pragma unroll
+                    for (int x = 0; x < NS; ++x)
+                        v[k][x] = __ldcg(reinterpret_cast<const float4*>(a.part_o + static_cast<long long>(at) * KV + x * 128) + lane);
+                }
+#pragma unroll
+                for (int k = 0; k < PER; ++k) {
+                    if (i0 + k >= parts) continue;
+                    const float2 f = sum.add(ml[k]);
+#pragma unroll
+                    for (int x = 0; x < NS; ++x) blend(o[x], v[k][x], f);
+                }
             }
 #pragma unroll
-            for (int k = 0; k < kFew; ++k)
-                if (i0 + k * step < parts) sum.add(v[k], ml[k]);
-        };
-        if (!many) {
-            take(0, 1);
-        } else {
-            for (int i = warp; i < parts; i += 8 * kFew) take(i, 8);
-            __syncthreads();  // the last task's sums have been read
-            sum_s[warp][lane] = sum.o;
-            if (lane == 0) ml_s[warp] = make_float2(sum.m, sum.l);
-            __syncthreads();
-            if (warp) continue;
-            for (int w = 1; w < 8; ++w) sum.add(sum_s[w][lane], ml_s[w]);
+            for (int x = 0; x < NS; ++x) finish(h, x * 128 + lane * 4, o[x], sum);
         }
-        const float inv = sum.l == 0.f ? 0.f : 1.f / sum.l;
-        const long long r = static_cast<long long>(row) * p.H + h0 + h;
-        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + r * KV + c) =
-            make_uint2(lat::pack2<T>(sum.o.x * inv, sum.o.y * inv), lat::pack2<T>(sum.o.z * inv, sum.o.w * inv));
-        if (p.lse && lane == 0 && c == 0) p.lse[r] = sum.l == 0.f ? -INFINITY : (sum.m + log2f(sum.l)) * 0.6931471805599453f;
+        return;
+    }
+    for (int task = blockIdx.y; task < heads * NS; task += gridDim.y) {
+        const int h = task / NS, c = (task - h * NS) * 128 + lane * 4;
+        Mean sum;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = warp; i0 < parts; i0 += 8 * 8) {
+            float4 v[8];
+            float2 ml[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (i0 + 8 * k >= parts) continue;
+                const int at = slot(i0 + 8 * k) * 16 + h;
+                ml[k] = __ldcg(&a.part_ml[at]);
+                v[k] = __ldcg(reinterpret_cast<const float4*>(a.part_o + static_cast<long long>(at) * KV + c));
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i0 + 8 * k < parts) blend(o, v[k], sum.add(ml[k]));
+        }
+        __syncthreads();  // the last task's sums have been read
+        sum_s[warp][lane] = o;
+        if (lane == 0) ml_s[warp] = make_float2(sum.m, sum.l);
+        __syncthreads();
+        if (warp) continue;
+        for (int w = 1; w < 8; ++w) blend(o, sum_s[w][lane], sum.add(ml_s[w]));
+        finish(h, c, o, sum);
     }
 }
 
