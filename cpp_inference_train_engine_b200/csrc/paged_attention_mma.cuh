@@ -163,12 +163,12 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 }
 template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (std::is_same<T, __nv_bfloat16>::value)
-        asm volatile(
+        asm(
             "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile(
+        asm(
             "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -178,9 +178,12 @@ __device__ __forceinline__ uint32_t swizzled(int r, int c) { return r * 128 + ((
 template <int R> __device__ __forceinline__ uint32_t swizzled_rope(int r, int c) {
     return R == 32 ? r * 64 + ((c ^ ((r >> 1) & 3)) << 4) : r * 32 + ((c ^ ((r >> 2) & 1)) << 4);
 }
-__device__ __forceinline__ uint32_t codes2(uint32_t two) {  // two e4m3 codes as two fp16 values (exact)
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffff), __NV_E4M3);
-    return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+// Four e4m3 codes as fp16 values (exact): the first two, the last two.
+__device__ __forceinline__ void codes4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(four));
 }
 // The four warps of the products, all of their threads.
 __device__ __forceinline__ void products_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -502,7 +505,11 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     for (int k = 0; k < 8; ++k) {
                         if (k < 7) ldsm4(b[(k + 1) & 1], box + swizzled(msel * 8 + mrow, k + 1));
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) mma16<__half>(s[n], q[k], codes2(b[k & 1][n]), codes2(b[k & 1][n] >> 16));
+                        for (int n = 0; n < 4; ++n) {
+                            uint32_t lo, hi;
+                            codes4(b[k & 1][n], lo, hi);
+                            mma16<__half>(s[n], q[k], lo, hi);
+                        }
                     }
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
@@ -634,13 +641,13 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     for (int j = 0; j < 8; ++j) {
                         const int k = j >> 2, c = j & 3;
                         if (j < 7) load(j + 1, b[(j + 1) & 1]);
-                        uint32_t v[4];
+                        uint32_t even[4], odd[4];
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) v[x] = __byte_perm(b[j & 1][x], 0, 0x3120);
+                        for (int x = 0; x < 4; ++x) codes4(__byte_perm(b[j & 1][x], 0, 0x3120), even[x], odd[x]);
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            mma16<__half>(o[4 * c + 2 * x], w[k], codes2(v[2 * x]), codes2(v[2 * x + 1]));
-                            mma16<__half>(o[4 * c + 2 * x + 1], w[k], codes2(v[2 * x] >> 16), codes2(v[2 * x + 1] >> 16));
+                            mma16<__half>(o[4 * c + 2 * x], w[k], even[2 * x], even[2 * x + 1]);
+                            mma16<__half>(o[4 * c + 2 * x + 1], w[k], odd[2 * x], odd[2 * x + 1]);
                         }
                     }
                 }
