@@ -219,7 +219,8 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
     // log2 of the largest weight when its reference is taken: small fp16 ones stay normal, large ones below 2^16
     constexpr float kGrowth = 8.f, kLift = !std::is_same<TP, __half>::value ? 0.f : C::CW > 1 ? 6.f : 10.f;
     extern __shared__ uint8_t mma_smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(mma_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    // (an offset, not a rounded address: the compiler has to see that the pointers below are of shared memory)
+    uint8_t* smem = mma_smem_raw + ((1024 - (smem_u32(mma_smem_raw) & 1023)) & 1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::oBar);
     uint64_t* empty = full + C::SLOTS;
     uint64_t* run_full = empty + C::SLOTS;
@@ -380,6 +381,11 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
         const uint32_t ring = smem_u32(smem) + group * C::SG * C::kSlot;
         // this lane's rows of the matrices that ldmatrix reads
         const int mrow = lane & 7, msel = lane >> 3;
+        // offsets in a slot of its first matrices: the next columns are an exclusive or away (the swizzle's chunk is
+        // chunk ^ row, and slots and rows of a box keep those bits free), the next 16 rows 2,048 bytes
+        const uint32_t s_at = cw * (Q8 ? 1 : 2) * (kTile * 128) + (Q8 ? swizzled(msel * 8 + mrow, 0) : swizzled((msel >> 1) * 8 + mrow, msel & 1));
+        const uint32_t o_at = cw * (Q8 ? 1 : 2) * (kTile * 128) + swizzled((msel & 1) * 8 + mrow, msel >> 1);
+        const uint32_t rope_at = C::kLatent + swizzled_rope<R>((msel >> 1) * 8 + mrow, cw * 2 + (msel & 1));
         float* share = reinterpret_cast<float*>(smem + C::oShare);
         const float cs = p.scale * 1.4426950408889634f;
         // scales of the lane's positions 8 n + 2 t4 and the next (a second box of 16 starts 128 bytes on)
@@ -480,12 +486,11 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
                 if constexpr (!Q8) {
                     // (loads one step ahead of the products: issue is in order)
-                    const uint32_t box = sp + cw * 2 * (kTile * 128);
+                    const uint32_t box = sp + s_at;
                     uint32_t b[2][2][4];
                     auto load = [&](int k, uint32_t (&d)[2][4]) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            ldsm4(d[h], box + (k >> 2) * (kTile * 128) + swizzled(h * 16 + (msel >> 1) * 8 + mrow, (k & 3) * 2 + (msel & 1)));
+                        for (int h = 0; h < 2; ++h) ldsm4(d[h], (box ^ ((k & 3) * 32)) + (k >> 2) * (kTile * 128) + h * 2048);
                     };
                     load(0, b[0]);
 #pragma unroll
@@ -498,12 +503,12 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                         }
                     }
                 } else {
-                    const uint32_t box = sp + cw * (kTile * 128);
+                    const uint32_t box = sp + s_at;
                     uint32_t b[2][4];
-                    ldsm4(b[0], box + swizzled(msel * 8 + mrow, 0));
+                    ldsm4(b[0], box);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        if (k < 7) ldsm4(b[(k + 1) & 1], box + swizzled(msel * 8 + mrow, k + 1));
+                        if (k < 7) ldsm4(b[(k + 1) & 1], box ^ ((k + 1) * 16));
 #pragma unroll
                         for (int n = 0; n < 4; ++n) {
                             uint32_t lo, hi;
@@ -524,7 +529,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t b[4];
-                        ldsm4(b, sp + C::kLatent + swizzled_rope<R>(h * 16 + (msel >> 1) * 8 + mrow, cw * 2 + (msel & 1)));
+                        ldsm4(b, sp + rope_at + h * 16 * R * 2);
                         mma16<T>(s[2 * h], qr, b[0], b[1]);
                         mma16<T>(s[2 * h + 1], qr, b[2], b[3]);
                     }
@@ -611,12 +616,11 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     __syncwarp();
                 }
                 if constexpr (!Q8) {
-                    const uint32_t box = sp + cw * 2 * (kTile * 128);
+                    const uint32_t box = sp + o_at;
                     uint32_t b[2][2][4];
                     auto load = [&](int c, uint32_t (&d)[2][4]) {
 #pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            ldsm4_t(d[k], box + (c >> 2) * (kTile * 128) + swizzled(k * 16 + (msel & 1) * 8 + mrow, (c & 3) * 2 + (msel >> 1)));
+                        for (int k = 0; k < 2; ++k) ldsm4_t(d[k], (box ^ ((c & 3) * 32)) + (c >> 2) * (kTile * 128) + k * 2048);
                     };
                     load(0, b[0]);
 #pragma unroll
@@ -631,11 +635,9 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 } else {
                     // a transposed pair of codes is two neighbouring columns of one position: the even columns of 16
                     // make one tile of the product, the odd ones another
-                    const uint32_t box = sp + cw * (kTile * 128);
+                    const uint32_t box = sp + o_at;
                     uint32_t b[2][4];
-                    auto load = [&](int j, uint32_t (&d)[4]) {
-                        ldsm4_t(d, box + swizzled((j >> 2) * 16 + (msel & 1) * 8 + mrow, (j & 3) * 2 + (msel >> 1)));
-                    };
+                    auto load = [&](int j, uint32_t (&d)[4]) { ldsm4_t(d, (box ^ ((j & 3) * 32)) + (j >> 2) * 2048); };
                     load(0, b[0]);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
