@@ -214,21 +214,28 @@ struct Reorder {
 };
 
 struct Move {
-    int parent, full, part;  // the parent's full pages and the positions of its last one
-    int from, to;            // pages of the copy; part == 0: none
+    int parent, length, full;  // the parent, its positions and its full pages
+    bool swap;                 // the row's spare page becomes its entry `full`, its own page its spare one
+    int part;                  // positions to copy into it
+    int from, to;              // from this page of the pool, to that
 };
 __device__ __forceinline__ int length_of(const Reorder& a, int row) {
     return static_cast<int>(min(max(static_cast<long long>(a.lengths[row]), 0LL), static_cast<long long>(a.table.columns) * a.page));
 }
+// A row that takes over another one needs a page of its own behind the full ones. Its entry there is one where both
+// have the same whole number of pages (it is still to be filled); a row of another length may hold a page there
+// that others share, so that it takes its spare page even where there is nothing to copy.
 __device__ __forceinline__ Move move_of(const Reorder& a, int row) {
     Move m;
     m.parent = a.parents[row];
     if (m.parent < 0 || m.parent >= a.table.rows) m.parent = row;
-    const int n = length_of(a, m.parent);
-    m.full = n / a.page;
-    m.part = m.parent == row ? 0 : n - m.full * a.page;
+    m.length = length_of(a, m.parent);
+    m.full = m.length / a.page;
+    const int part = m.length - m.full * a.page;
+    m.swap = m.parent != row && m.full < a.table.columns && (part > 0 || m.length != length_of(a, row));
+    m.part = m.swap ? part : 0;
     m.from = m.to = -1;
-    if (m.part > 0) {
+    if (m.swap) {
         m.from = a.table.entry[m.parent * a.table.stride + m.full];
         m.to = a.spare[row];
     }
@@ -268,13 +275,13 @@ static __global__ void __launch_bounds__(256) reorder_kernel(const __grid_consta
     const int row = blockIdx.x, tid = threadIdx.x;
     const Move m = move_of(a, row);
     if (blockIdx.y == 0) {
-        const int own = m.part > 0 ? min(length_of(a, row) / a.page, a.table.columns - 1) : 0;
         for (int j = tid; j < a.table.columns; j += blockDim.x)
             a.out_table[static_cast<long long>(row) * a.table.columns + j] =
-                m.part > 0 && j == m.full ? m.to : a.table.entry[(j < m.full ? m.parent : row) * a.table.stride + j];
+                m.swap && j == m.full ? m.to : a.table.entry[(j < m.full ? m.parent : row) * a.table.stride + j];
         if (tid == 0) {
-            a.out_spare[row] = m.part > 0 ? a.table.entry[row * a.table.stride + own] : a.spare[row];
-            a.out_lengths[row] = length_of(a, m.parent);
+            const int own = length_of(a, row) / a.page;  // (a row that fills its table has no page of its own left)
+            a.out_spare[row] = !m.swap ? a.spare[row] : own < a.table.columns ? a.table.entry[row * a.table.stride + own] : -1;
+            a.out_lengths[row] = m.length;
         }
     }
     if (m.part == 0 || m.from < 0 || m.from >= a.pages || m.to < 0 || m.to >= a.pages || m.from == m.to) return;

@@ -107,8 +107,9 @@ def beam_reorder(cache, table: torch.Tensor, spare: torch.Tensor, lengths: torch
     """Lets every row take over its parent's cache: new (table, spare, lengths), the pools changed in place.
 
     cache has its layers ahead (``alloc_pages``); table [rows, columns], spare, lengths and parents [rows]
-    int32, parents as row numbers. Full pages are shared through the table. A row whose parent is another one and
-    whose last page is partly filled gets that page's positions in its own spare page, in every layer, and its
-    own page at its length becomes its spare. Every row needs an own page for each column that it may grow
-    into and one spare page, none of them another row's."""
+    int32, parents as row numbers. Full pages are shared through the table. A row whose parent is another one
+    gets the positions of its last, partly filled page in its own spare page, in every layer, and its own page at
+    its length becomes its spare (see include/mm_paged.h for rows of different lengths). Every row needs a page of
+    its own for each column that it may grow into and a spare one, none of them another row's; a row that fills its
+    table and then takes over a shorter one is left without a spare page (-1)."""
     return _ext.beam_reorder(cache, table, spare, lengths, parents)

@@ -89,11 +89,12 @@ int mm_beam_select(const void* logits, int64_t batch_stride, int64_t beam_stride
                    const uint8_t* finished, int eos, int batch, int beams, int vocab, int count, float* out_scores,
                    int32_t* out_parents, int32_t* out_tokens, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Rows take over their parents' caches. Every row owns the page its last, partly filled page is and a
- * spare one; row i with parent p = parents[i] and n = lengths[p] gets table entries [0, n / page) of p (full
- * pages are shared) and, when p != i and n % page > 0, its own spare page as entry n / page with p's
- * n % page positions copied into it in every layer; its page at entry lengths[i] / page is its new
- * spare. Other entries stay. out_lengths[i] = n. A parent outside [0, rows) is the row itself;
+/* Rows take over their parents' caches. Every row owns its last, partly filled page, the pages of the table
+ * entries behind it that it may grow into, and a spare page. Row i with parent p = parents[i] and n =
+ * lengths[p] gets table entries [0, n / page) of p (full pages are shared). When p != i, and n % page > 0 or n !=
+ * lengths[i], its spare page becomes its entry n / page, with p's n % page positions copied into it in every
+ * layer, and its own page at entry lengths[i] / page is its new spare (-1 where its lengths fill the table, which
+ * leaves it without). Other entries stay. out_lengths[i] = n. A parent outside [0, rows) is the row itself;
  * lengths are clamped to the table.
  * `cache` describes layer 0 (pages, page entries) and its table; layer l is layer_strides[0..2] * l
  * elements further in latent, rope and scale. out_table [rows][columns] contiguous, out_spare and

@@ -2,6 +2,7 @@
 in 64 bits: appending through a page table, attention of one token over pages, beam selection and
 reordering."""
 import math
+import random
 
 import pytest
 
@@ -503,11 +504,11 @@ def reorder_reference(torch, cache, table, spare, lengths, parents, page):
         full, part = n // page, n % page
         t2[i, :full] = table[p, :full]
         n2[i] = n
-        if p != i and part:
+        own = min(max(int(lengths[i]), 0), columns * page)
+        if p != i and full < columns and (part or n != own):
             source, target = int(table[p, full]), int(spare[i])
             t2[i, full] = target
-            own = min(max(int(lengths[i]), 0), columns * page)
-            s2[i] = table[i, min(own // page, columns - 1)]
+            s2[i] = table[i, own // page] if own < columns * page else -1
             pages = tensors[0].shape[1]
             if 0 <= source < pages and 0 <= target < pages:
                 for o, t in zip(old, new):
@@ -570,6 +571,48 @@ def test_reorder_of_rows_of_all_lengths_and_bad_entries():
         wide = torch.full((8, 9), -7, dtype=torch.int32, device="cuda")[:, 1:6]
         wide.copy_(table)
         check_reorder(torch, paged, cache, wide, spare, lengths, i32(torch, [1, 0, 3, 3, 5, 4, 7, 6]), 16)
+
+
+@pytest.mark.parametrize("page", [1, 4, 16])
+@pytest.mark.parametrize("seed", [0, 1, 2])
+def test_a_long_search_never_mixes_rows(page, seed):
+    """Rows that finish (and stop growing), are dropped, copied and taken over again for many steps: every row's
+    positions hold what its hypothesis stored, whatever pages they share."""
+    torch, paged = mods()
+    rng = random.Random(seed)
+    rows, columns = 6, 64 // page
+    cache = paged.alloc_pages(1, rows * (columns + 1), page, 8, 0, torch.bfloat16)
+    own = list(range(rows * (columns + 1)))
+    rng.shuffle(own)
+    table = i32(torch, own[:rows * columns]).view(rows, columns)
+    spare, lengths = i32(torch, own[rows * columns:]), i32(torch, [0] * rows)
+    held, done, mark = [[] for _ in range(rows)], [False] * rows, 0
+    for _ in range(55):
+        values = torch.zeros(rows, 8, device="cuda")
+        positions = []
+        for r in range(rows):  # rows that are not done store a number of their own
+            positions.append(-1 if done[r] else len(held[r]))
+            if not done[r]:
+                mark += 1
+                held[r] = held[r] + [mark]
+                values[r, 0], values[r, 1] = mark // 128, mark % 128  # (bf16 holds both)
+        paged.append(cache[0], values, table, i32(torch, positions), kv_rank=8)
+        lengths = i32(torch, [len(h) for h in held])
+        parents = [rng.choice([r, r, rng.randrange(rows)]) for r in range(rows)]
+        if all(done[p] for p in parents):  # some hypothesis goes on
+            parents[0] = next((r for r in range(rows) if not done[r]), parents[0])
+        table, spare, lengths = paged.beam_reorder(cache, table, spare, lengths, i32(torch, parents))
+        held = [held[p] for p in parents]
+        done = [done[p] or rng.random() < 0.08 for p in parents]
+        if all(done):
+            done[rng.randrange(rows)] = False if len(set(map(len, held))) == 1 else True
+        assert lengths.tolist() == [len(h) for h in held]
+        stored, pages = cache[0].float().cpu(), table.cpu()
+        for r, h in enumerate(held):
+            got = [int(stored[pages[r, t // page], t % page, 0] * 128 + stored[pages[r, t // page], t % page, 1]) for t in range(len(h))]
+            assert got == h, (r, parents)
+        if all(done):
+            break
 
 
 # ------------------------------------------------------------------ together
