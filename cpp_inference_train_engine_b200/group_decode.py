@@ -37,6 +37,43 @@ def _rmsnorm(x, w, eps):
     return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * w
 
 
+def check_parameters(cfg: ModelConfig, params):
+    """The model's parameters as one flat fp32 array; another model's are refused."""
+    params = np.ascontiguousarray(params, np.float32).reshape(-1)
+    if params.size != cfg.parameter_count():
+        raise EngineError(1, f"the model has {cfg.parameter_count()} parameters, got {params.size}")
+    return params
+
+
+def decode_weights(cfg: ModelConfig, params, device):
+    """(embedding, final norm, layers) of a flat parameter array as decode uses them: matrices in fp16, norms
+    in fp32, and per head `uk` [heads, nope, kv], which queries absorb, and `uv` [heads, kv, value], which
+    expands the latent context."""
+    flat = torch.from_numpy(params).to(device)
+    tensors, at = [], 0
+    for _, (r, c), _ in cfg.parameter_shapes():
+        tensors.append(flat[at:at + r * c].view(r, c))
+        at += r * c
+    layers = []
+    for l in range(cfg.n_layers):
+        w = dict(zip(_NAMES, tensors[2 + 13 * l:15 + 13 * l]))
+        w = {k: v.view(-1) if k.endswith("norm") else v.half() for k, v in w.items()}
+        w["uk"] = w["w_uk"].view(cfg.kv_lora_rank, cfg.n_heads, cfg.head_dim_nope).permute(1, 2, 0).contiguous()
+        w["uv"] = w["w_uv"].view(cfg.kv_lora_rank, cfg.n_heads, cfg.head_dim_value).permute(1, 0, 2).contiguous()
+        layers.append(w)
+    return tensors[0].half(), tensors[1].view(-1), layers
+
+
+def rotate(x, positions, theta: float):
+    """Adjacent pairs rotated by position * theta^(-j / width) (src/model/ops.cpp:88-108)."""
+    w = x.shape[-1]
+    j = torch.arange(0, w, 2, device=x.device, dtype=torch.float32)
+    angle = positions.float()[..., None] * torch.pow(theta, -j / w)
+    cos, sin = angle.cos(), angle.sin()
+    a, b = x[..., 0::2].float(), x[..., 1::2].float()
+    return torch.stack([a * cos - b * sin, a * sin + b * cos], -1).flatten(-2)
+
+
 class GroupDecoder:
     """`prompts`: one token list per group; `rows`: completions per group (a number, or one per
     group); `new_tokens` bounds every completion. `cache_bits` 8 or 16 is the storage of the
@@ -56,25 +93,10 @@ class GroupDecoder:
         prompts = [list(map(int, p)) for p in prompts]
         if any(not 0 <= t < cfg.vocab_size for p in prompts for t in p):
             raise EngineError(1, "a prompt's token is outside the vocabulary")
-        params = np.ascontiguousarray(params, np.float32).reshape(-1)
-        if params.size != cfg.parameter_count():
-            raise EngineError(1, f"the model has {cfg.parameter_count()} parameters, got {params.size}")
+        params = check_parameters(cfg, params)
         self.cfg, self.drafts, self.new_tokens, self.bits = cfg, drafts, new_tokens, cache_bits
         self.device = device
-        flat = torch.from_numpy(params).to(device)
-        tensors, at = [], 0
-        for _, (r, c), _ in cfg.parameter_shapes():
-            tensors.append(flat[at:at + r * c].view(r, c))
-            at += r * c
-        self.embedding, self.final_norm = tensors[0].half(), tensors[1].view(-1)
-        self.layers = []
-        for l in range(cfg.n_layers):
-            w = dict(zip(_NAMES, tensors[2 + 13 * l:15 + 13 * l]))
-            w = {k: v.view(-1) if k.endswith("norm") else v.half() for k, v in w.items()}
-            # per head: queries absorb w_uk, the latent context is expanded by w_uv
-            w["uk"] = w["w_uk"].view(cfg.kv_lora_rank, cfg.n_heads, cfg.head_dim_nope).permute(1, 2, 0).contiguous()
-            w["uv"] = w["w_uv"].view(cfg.kv_lora_rank, cfg.n_heads, cfg.head_dim_value).permute(1, 0, 2).contiguous()
-            self.layers.append(w)
+        self.embedding, self.final_norm, self.layers = decode_weights(cfg, params, device)
         G, B = len(prompts), sum(rows)
         i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=device)  # noqa: E731
         self.max_prompt, self.max_group = max(len(p) for p in prompts), max(rows)
@@ -121,13 +143,7 @@ class GroupDecoder:
         return sum(t.numel() * t.element_size() for t in tensors)
 
     def _rope(self, x, positions):
-        """Adjacent pairs rotated by position * theta^(-j / width) (src/model/ops.cpp:88-108)."""
-        w = x.shape[-1]
-        j = torch.arange(0, w, 2, device=self.device, dtype=torch.float32)
-        angle = positions.float()[..., None] * torch.pow(self.cfg.rope_theta, -j / w)
-        cos, sin = angle.cos(), angle.sin()
-        a, b = x[..., 0::2].float(), x[..., 1::2].float()
-        return torch.stack([a * cos - b * sin, a * sin + b * cos], -1).flatten(-2)
+        return rotate(x, positions, self.cfg.rope_theta)
 
     def _blocks(self, tokens, positions, slots, stores, attend):
         """The decoder over tokens [n, T] at `positions`; writes each position's latent row into

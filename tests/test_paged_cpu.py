@@ -146,3 +146,20 @@ def test_alloc_pages():
     for kw in (dict(dtype=torch.float32), dict(bits=4)):
         with pytest.raises(EngineError):
             paged.alloc_pages(1, 1, 16, 128, 16, device="cpu", **kw)
+
+
+@pytest.mark.parametrize("over, what", [
+    (dict(cache_bits=4), "cache_bits"), (dict(new=0), "new_tokens"), (dict(prompts=[]), "new_tokens"), (dict(prompts=[[1], []]), "new_tokens"),
+    (dict(beams=0), "beams"), (dict(beams=33), "beams"), (dict(page_size=0), "positive"), (dict(window=0), "positive"),
+    (dict(sinks=-1), "negative"), (dict(new=64), "exceeds context"), (dict(prompts=[[1, 264]]), "vocabulary"), (dict(prompts=[[-1]]), "vocabulary"),
+    (dict(extra=1), "parameters")])
+def test_beam_decoder_refuses(over, what):
+    import numpy as np
+
+    from cpp_inference_train_engine_b200 import TINY
+    from cpp_inference_train_engine_b200.beam_decode import BeamDecoder
+    d = dict(prompts=[[1, 2]], beams=2, new=4, page_size=4, cache_bits=16, window=None, sinks=0, extra=0)
+    d.update(over)
+    with pytest.raises(EngineError, match=what):
+        BeamDecoder(TINY, np.zeros(TINY.parameter_count() + d["extra"], np.float32), d["prompts"], d["beams"], d["new"], d["page_size"],
+                    d["cache_bits"], d["window"], d["sinks"], device="cpu")
