@@ -73,14 +73,34 @@ struct Best {
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
 
+// Two fp32 values in one register pair: sums and products of both in one instruction.
+struct Two {
+    unsigned long long v;
+    __device__ __forceinline__ Two(unsigned long long x) : v(x) {}
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ float lo() const { return __uint_as_float(static_cast<uint32_t>(v)); }
+    __device__ __forceinline__ float hi() const { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
 // Block (part, beam row). E values of 16 bytes a load; a row's first and last tokens that are not in a whole
 // aligned load are taken one a lane.
 template <typename T>
-__global__ void __launch_bounds__(128) select_parts_kernel(const Select a) {
+__global__ void __launch_bounds__(128, 8) select_parts_kernel(const Select a) {
     MM_PDL_ENTRY();
-    constexpr int E = 16 / sizeof(T), U = 4, kSteps = 4;  // values per load, loads per step, steps per stretch
+    constexpr int E = 16 / sizeof(T), U = 4, kSteps = 8;  // values per load, loads per step, steps per stretch
     __shared__ Pair wait_s[4][64];
     __shared__ float2 sum_s[4];
+    __shared__ uint8_t pairs_s[4][32 * kSteps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
     if (!finite(__ldg(a.scores + row)) || (a.finished && a.finished[row])) return;  // the join does not read it either
@@ -115,7 +135,7 @@ __global__ void __launch_bounds__(128) select_parts_kernel(const Select a) {
     };
     constexpr float kLog2e = 1.4426950408889634f;
     float m = kLowest, s = 0.f;  // (a finite maximum of nothing: differences from it are no NaN)
-    uint4 raw[U];
+    uint4 raw[U];  // a step ahead
     auto fetch = [&](int i0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -135,22 +155,34 @@ __global__ void __launch_bounds__(128) select_parts_kernel(const Select a) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    v[u][e] = i0 + u * 32 + lane < l1 ? lat::to_f32(reinterpret_cast<const T*>(&raw[u])[e]) : -INFINITY;
-                    tops[st] = fmaxf(tops[st], v[u][e]);
-                }
+                for (int e = 0; e < E; ++e) v[u][e] = lat::to_f32(reinterpret_cast<const T*>(&raw[u])[e]);
+            if (i0 + 32 * U > l1) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (i0 + u * 32 + lane >= l1) {
+#pragma unroll
+                        for (int e = 0; e < E; ++e) v[u][e] = -INFINITY;
+                    }
+            }
             fetch(i0 + 32 * U);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < E; ++e) tops[st] = fmaxf(tops[st], v[u][e]);
             const float mn = fmaxf(m, tops[st]);
             s *= fast_exp2((m - mn) * kLog2e);
             m = mn;
-            float sums[U];
+            const Two ref(-m, -m), by(kLog2e, kLog2e);
+            Two sums[2] = {Two(0.f, 0.f), Two(0.f, 0.f)};
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                sums[u] = 0.f;
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int e = 0; e < E; ++e) sums[u] += fast_exp2((v[u][e] - m) * kLog2e);
-            }
-            s += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                for (int e = 0; e < E; e += 2) {
+                    const Two z = (Two(v[u][e], v[u][e + 1]) + ref) * by;
+                    sums[u & 1] = sums[u & 1] + Two(fast_exp2(z.lo()), fast_exp2(z.hi()));
+                }
+            sums[0] = sums[0] + sums[1];
+            s += sums[0].lo() + sums[0].hi();
             most = fmaxf(most, tops[st]);
         }
         // `count` of the lanes' largest are `count` candidates: nothing below the least of them enters
@@ -160,12 +192,32 @@ __global__ void __launch_bounds__(128) select_parts_kernel(const Select a) {
             const float floor = all.rank(a.count - 1).value;
             if (floor > last.value) last = {floor, kNobody};
         }
+        // the steps and lanes that reach it, in line; their values from the cache, kAtOnce pairs' at a time
+        int pairs = 0;
 #pragma unroll
-        for (int st = 0; st < kSteps; ++st)
-            for (unsigned who = __ballot_sync(0xffffffffu, tops[st] >= last.value && tops[st] > -INFINITY); who; who &= who - 1) {
-                const int i = base + st * 32 * U + lane / E * 32 + __ffs(who) - 1, t = head + i * E + lane % E;
-                offer(lane < U * E && i < l1 ? lat::to_f32(x[t]) : -INFINITY, t);
+        for (int st = 0; st < kSteps; ++st) {
+            const bool in = tops[st] >= last.value && tops[st] > -INFINITY;
+            const unsigned who = __ballot_sync(0xffffffffu, in);
+            if (in) pairs_s[warp][pairs + __popc(who & ((1u << lane) - 1))] = static_cast<uint8_t>(st * 32 + lane);
+            pairs += __popc(who);
+        }
+        __syncwarp();
+        constexpr int kSide = 32 / (U * E), kAtOnce = 4 * kSide;  // pairs side by side in a warp: 2 for 16 values
+        const int place = lane % (U * E);
+        for (int j0 = 0; j0 < pairs; j0 += kAtOnce) {
+            float v[4];
+            int t[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int pair = j0 + j * kSide + lane / (U * E), code = pair < pairs ? pairs_s[warp][pair] : 0;
+                const int i = base + (code >> 5) * 32 * U + place / E * 32 + (code & 31);
+                t[j] = head + i * E + place % E;
+                v[j] = pair < pairs && i < l1 ? lat::to_f32(x[t[j]]) : -INFINITY;
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) offer(v[j], t[j]);
+        }
+        __syncwarp();
     }
     if (part == 0 && warp == 0) {  // the ends, at most 2 (E - 1) <= 14 tokens
         const int tail = head + loads * E;
@@ -205,20 +257,22 @@ static __global__ void __launch_bounds__(1024) select_join_kernel(const Select a
     __shared__ int at_s[kMaxBeams * kMaxBeams];
     const int b = blockIdx.x, k = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = b * a.beams + k, n = a.parts * a.count;
+    // everything asked for at once: what the parts of a finished or dead beam hold is not used
+    const long long p0 = static_cast<long long>(row) * a.parts;
+    auto entry = [&](int i) { return i < n ? Pair{__ldcg(a.best + p0 * a.count + i), __ldcg(a.token + p0 * a.count + i)} : Pair{-INFINITY, kNobody}; };
+    Pair next = entry(lane);
+    const float2 sum = lane < a.parts ? __ldcg(a.sum + p0 + lane) : make_float2(kLowest, 0.f);
     const float score = __ldg(a.scores + row);
+    const bool ended = a.finished && __ldg(a.finished + row);
     double cand = -INFINITY;
     int at = kNobody;
     if (finite(score)) {
-        if (a.finished && a.finished[row]) {
+        if (ended) {
             if (lane == 0) {
                 cand = score;
                 at = k * a.vocab + a.eos;
             }
         } else {
-            const long long p0 = static_cast<long long>(row) * a.parts;
-            auto entry = [&](int i) { return i < n ? Pair{a.best[p0 * a.count + i], a.token[p0 * a.count + i]} : Pair{-INFINITY, kNobody}; };
-            Pair next = entry(lane);
-            const float2 sum = lane < a.parts ? a.sum[p0 + lane] : make_float2(kLowest, 0.f);
             const float top = warp_max(sum.x);
             const double s = static_cast<double>(sum.y) * exp(static_cast<double>(sum.x) - top);
             const double lse = top + log(warp_sum(s));
@@ -241,17 +295,22 @@ static __global__ void __launch_bounds__(1024) select_join_kernel(const Select a
     const int all = a.beams * a.count, i = threadIdx.x;
     const long long o = static_cast<long long>(b) * a.count;
     const int candidates = __syncthreads_count(lane < a.count && at != kNobody);
-    if (i < all && at_s[i] != kNobody) {
-        const double c = score_s[i];
-        const int t = at_s[i];
-        int rank = 0;
-#pragma unroll 8
-        for (int j = 0; j < all; ++j) rank += at_s[j] != kNobody && (score_s[j] > c || (score_s[j] == c && at_s[j] < t));
-        if (rank < a.count) {
-            a.out_scores[o + rank] = static_cast<float>(c);
-            a.out_parents[o + rank] = t / a.vocab;
-            a.out_tokens[o + rank] = t % a.vocab;
-        }
+    // 2^side threads a candidate, which fit: the block has 32 threads a beam
+    const int side = 31 - __clz(32 / a.count), mine = i >> side;
+    double c = 0;
+    int t = kNobody, rank = 0;
+    if (mine < all && at_s[mine] != kNobody) {
+        c = score_s[mine];
+        t = at_s[mine];
+#pragma unroll 4
+        for (int j = i & ((1 << side) - 1); j < all; j += 1 << side)
+            rank += at_s[j] != kNobody && (score_s[j] > c || (score_s[j] == c && at_s[j] < t));
+    }
+    for (int d = 1; d < 1 << side; d <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, d);
+    if (t != kNobody && rank < a.count && (i & ((1 << side) - 1)) == 0) {
+        a.out_scores[o + rank] = static_cast<float>(c);
+        a.out_parents[o + rank] = t / a.vocab;
+        a.out_tokens[o + rank] = t % a.vocab;
     }
     if (i >= candidates && i < a.count) {  // left over
         a.out_scores[o + i] = -INFINITY;
