@@ -1,10 +1,11 @@
 // Beam search's selection over beams and vocabulary (mm_beam_select).
 //
-// One pass over the logits: a block takes a part of a beam's tokens, each of its warps a quarter, and keeps
-// their maximum, the sum of exponentials below it and the best `count` of them (rank r in lane r); a second kernel
-// joins the parts of a beam and then the beams. The pass itself keeps one maximum per lane and step: of the 32
-// lanes' maxima over a stretch of steps the count-th largest bounds the list from below, so that only the few (lane,
-// step) pairs that reach it are looked at again, from the cache.
+// One pass over the logits: a block takes a part of a beam's tokens, each of its warps an eighth, and keeps their
+// maximum, the sum of exponentials below it and the best 32 of them (rank r in lane r); then the parts of a beam are
+// joined, and the beams. The pass itself keeps one maximum per lane and step: of the 32 lanes' maxima over a
+// stretch of steps the count-th largest bounds the list from below, so that only the few (lane, step) pairs that
+// reach it are looked at again, from the cache. Where a batch entry's blocks fit a cluster (16) its first block joins
+// them from their shared memory, else a second kernel from the workspace.
 #pragma once
 #include "latent_cache.cuh"
 
@@ -14,8 +15,16 @@ namespace beam {
 constexpr int kMaxBeams = 32;
 constexpr int kMaxVocab = 1 << 20;  // flat candidates k * vocab + v stay below 2^25
 constexpr float kLowest = -3.402823466e38f;
-constexpr int kMaxParts = 32;       // of a beam's tokens
+constexpr int kMaxParts = 32;       // of a beam's tokens, a block each
+constexpr int kWarps = 8;           // of such a block
+constexpr int kMaxCluster = 16;
 
+// Candidates in order: by value, then by the lower index. Nobody: (-infinity, kNobody).
+constexpr int kNobody = 0x7fffffff;
+struct alignas(8) Pair {
+    float value;
+    int at;
+};
 struct Select {
     const void* logits;
     long long batch_stride, beam_stride;
@@ -25,18 +34,11 @@ struct Select {
     float* out_scores;
     int* out_parents;
     int* out_tokens;
-    // a part's best values and tokens, maximum and sum: [batch * beams * parts][count], [batch * beams * parts]
-    float* best;
-    int* token;
+    // without a cluster, of each part [batch * beams * parts]: its best tokens [32], maximum and sum
+    Pair* best;
     float2* sum;
 };
 
-// Candidates in order: by value, then by the lower index. Nobody: (-infinity, kNobody).
-constexpr int kNobody = 0x7fffffff;
-struct Pair {
-    float value;
-    int at;
-};
 __device__ __forceinline__ bool ahead(Pair a, Pair b) { return a.value > b.value || (a.value == b.value && a.at < b.at); }
 __device__ __forceinline__ Pair from_lane(Pair p, int lane_xor) {
     return {__shfl_xor_sync(0xffffffffu, p.value, lane_xor), __shfl_xor_sync(0xffffffffu, p.at, lane_xor)};
@@ -92,24 +94,110 @@ __device__ __forceinline__ Two operator*(Two a, Two b) {
     return r;
 }
 
+// Candidates of several beams: scores in fp64, k * vocab + v.
+struct Scored {
+    double value;
+    int at;
+};
+__device__ __forceinline__ Scored from_lane(Scored p, int lane_xor) {
+    return {__shfl_xor_sync(0xffffffffu, p.value, lane_xor), __shfl_xor_sync(0xffffffffu, p.at, lane_xor)};
+}
+__device__ __forceinline__ bool ahead(Scored a, Scored b) { return a.value > b.value || (a.value == b.value && a.at < b.at); }
+// Best::join_sorted of these: p's lanes become the best 32 of both lists, in order.
+__device__ __forceinline__ void join_sorted(Scored& p, Scored q) {
+    q = from_lane(q, 31);
+    if (ahead(q, p)) p = q;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const Scored u = from_lane(p, o);
+        if (ahead(u, p) == ((threadIdx.x & o) == 0)) p = u;
+    }
+}
+
+// Joins a batch entry's parts and beams with `warps` warps, which all come here. list(k, part) is the lane's entry
+// of a part's list, sum(k, part) its maximum and sum. scratch: 512 bytes for each warp.
+template <class List, class Sum>
+__device__ __forceinline__ void finish(const Select& a, int b, int warps, uint8_t* scratch, List list, Sum sum) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Scored all{-INFINITY, kNobody};
+    for (int k = warp; k < a.beams; k += warps) {
+        const int row = b * a.beams + k;
+        // asked for together: what the parts of a finished or dead beam hold is not used
+        Pair next = list(k, 0);
+        const float2 part = lane < a.parts ? sum(k, lane) : make_float2(kLowest, 0.f);
+        const float score = __ldg(a.scores + row);
+        const bool ended = a.finished && __ldg(a.finished + row);
+        Scored mine{-INFINITY, kNobody};
+        if (finite(score) && ended) {
+            if (lane == 0) mine = {score, k * a.vocab + a.eos};
+        } else if (finite(score)) {
+            const float top = warp_max(part.x);
+            const double s = static_cast<double>(part.y) * exp(static_cast<double>(part.x) - top);
+            const double lse = top + log(warp_sum(s));
+            Best best;
+#pragma unroll 1
+            for (int i = 1; i <= a.parts; ++i) {
+                const Pair q = next;
+                if (i < a.parts) next = list(k, i);
+                best.join_sorted(q);
+            }
+            // a log-sum-exp that is not finite makes no candidate; what fp32 cannot hold is no score
+            const double c = score + (static_cast<double>(best.p.value) - lse);
+            if (best.p.at != kNobody && fabs(lse) < INFINITY && static_cast<float>(c) > -INFINITY) mine = {c, k * a.vocab + best.p.at};
+        }
+        join_sorted(all, mine);
+    }
+    // the warps' lists two by two
+    double* value_s = reinterpret_cast<double*>(scratch);
+    int* at_s = reinterpret_cast<int*>(value_s + warps * 32);
+    for (int d = 1; d < warps; d <<= 1) {
+        if (warp % (2 * d) == d) {
+            value_s[warp * 32 + lane] = all.value;
+            at_s[warp * 32 + lane] = all.at;
+        }
+        __syncthreads();
+        if (warp % (2 * d) == 0 && warp + d < warps) join_sorted(all, {value_s[(warp + d) * 32 + lane], at_s[(warp + d) * 32 + lane]});
+    }
+    if (warp == 0 && lane < a.count) {
+        const bool none = all.at == kNobody;
+        const long long o = static_cast<long long>(b) * a.count + lane;
+        a.out_scores[o] = static_cast<float>(all.value);
+        a.out_parents[o] = none ? min(lane, a.beams - 1) : all.at / a.vocab;
+        a.out_tokens[o] = none ? -1 : all.at % a.vocab;
+    }
+}
+
+__device__ __forceinline__ unsigned long long load_cluster64(uint32_t cluster_addr) {
+    unsigned long long v;
+    asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
 // Block (part, beam row). E values of 16 bytes a load; a row's first and last tokens that are not in a whole
-// aligned load are taken one a lane.
-template <typename T>
-__global__ void __launch_bounds__(128, 8) select_parts_kernel(const Select a) {
+// aligned load are taken one a lane. Loads stand in shared memory two steps ahead, where the lane that asked for
+// them takes them itself.
+constexpr int kLoads = 4, kStages = 3;
+constexpr int kRing = kWarps * kStages * kLoads * 32 * 16;  // 48 KB: four blocks an SM
+template <typename T, bool CLUSTER>
+__global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(const Select a) {
     MM_PDL_ENTRY();
-    constexpr int E = 16 / sizeof(T), U = 4, kSteps = 8;  // values per load, loads per step, steps per stretch
-    __shared__ Pair wait_s[4][64];
-    __shared__ float2 sum_s[4];
-    __shared__ uint8_t pairs_s[4][32 * kSteps];
+    constexpr int E = 16 / sizeof(T), U = kLoads, kSteps = 8;  // values per load, loads per step, steps per stretch
+    extern __shared__ uint4 ring_s[];
+    __shared__ Pair list_s[32];
+    __shared__ float2 total_s;
+    __shared__ Pair wait_s[kWarps][64];
+    __shared__ float2 sum_s[kWarps];
+    __shared__ uint8_t pairs_s[kWarps][32 * kSteps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
-    if (!finite(__ldg(a.scores + row)) || (a.finished && a.finished[row])) return;  // the join does not read it either
     const int b = row / a.beams;
+    const bool dead = !finite(__ldg(a.scores + row)) || (a.finished && a.finished[row]);
+    if (!CLUSTER && dead) return;  // the join does not use it either
     const T* x = static_cast<const T*>(a.logits) + b * a.batch_stride + (row - b * a.beams) * a.beam_stride;
     // whole loads begin at token `head`, which is where the address is a multiple of 16
     const int head = min(a.vocab, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
-    const int loads = (a.vocab - head) / E;
-    const int per = (loads + 4 * a.parts - 1) / (4 * a.parts), l0 = min((part * 4 + warp) * per, loads), l1 = min(l0 + per, loads);
+    const int loads = dead ? 0 : (a.vocab - head) / E;
+    const int per = (loads + kWarps * a.parts - 1) / (kWarps * a.parts), l0 = min((part * kWarps + warp) * per, loads), l1 = min(l0 + per, loads);
     // Candidates wait in shared memory until there are 32 (or no more): joining the list costs a sort. What is
     // behind the list's last entry does not wait.
     Pair* wait = wait_s[warp];
@@ -135,15 +223,19 @@ __global__ void __launch_bounds__(128, 8) select_parts_kernel(const Select a) {
     };
     constexpr float kLog2e = 1.4426950408889634f;
     float m = kLowest, s = 0.f;  // (a finite maximum of nothing: differences from it are no NaN)
-    uint4 raw[U];  // a step ahead
+    uint4* ring = ring_s + warp * (kStages * U * 32) + lane;
+    int stage = 0, filled = 0;
     auto fetch = [&](int i0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * 32 + lane;
-            if (i < l1) raw[u] = __ldg(reinterpret_cast<const uint4*>(x + head) + i);
+            cp_async16(ring + (filled * U + u) * 32, reinterpret_cast<const uint4*>(x + head) + (i < l1 ? i : 0), i < l1);
         }
+        cp_async_commit();
+        filled = filled == kStages - 1 ? 0 : filled + 1;
     };
     fetch(l0);
+    fetch(l0 + 32 * U);
     for (int base = l0; base < l1; base += 32 * U * kSteps) {
         float tops[kSteps], most = -INFINITY;
 #pragma unroll
@@ -152,10 +244,14 @@ __global__ void __launch_bounds__(128, 8) select_parts_kernel(const Select a) {
             tops[st] = -INFINITY;
             if (i0 >= l1) continue;
             float v[U][E];
+            cp_async_wait<kStages - 2>();
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                const uint4 raw = ring[(stage * U + u) * 32];
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[u][e] = lat::to_f32(reinterpret_cast<const T*>(&raw[u])[e]);
+                for (int e = 0; e < E; ++e) v[u][e] = lat::to_f32(reinterpret_cast<const T*>(&raw)[e]);
+            }
+            stage = stage == kStages - 1 ? 0 : stage + 1;
             if (i0 + 32 * U > l1) {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
@@ -164,7 +260,7 @@ __global__ void __launch_bounds__(128, 8) select_parts_kernel(const Select a) {
                         for (int e = 0; e < E; ++e) v[u][e] = -INFINITY;
                     }
             }
-            fetch(i0 + 32 * U);
+            fetch(i0 + 2 * 32 * U);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -219,7 +315,8 @@ __global__ void __launch_bounds__(128, 8) select_parts_kernel(const Select a) {
         }
         __syncwarp();
     }
-    if (part == 0 && warp == 0) {  // the ends, at most 2 (E - 1) <= 14 tokens
+    cp_async_wait<0>();
+    if (part == 0 && warp == 0 && !dead) {  // the ends, at most 2 (E - 1) <= 14 tokens
         const int tail = head + loads * E;
         const int t = lane < head ? lane : tail + lane - head;
         const float v = t < a.vocab ? lat::to_f32(x[t]) : -INFINITY;
@@ -234,89 +331,56 @@ __global__ void __launch_bounds__(128, 8) select_parts_kernel(const Select a) {
     float top = warp_max(m);
     s = warp_sum(scaled({m, s}, top));
     if (lane == 0) sum_s[warp] = make_float2(top, s);
+    // the warps' lists two by two
     wait[lane] = best.p;
-    __syncthreads();
-    if (warp) return;
-    for (int w = 1; w < 4; ++w) best.join_sorted(wait_s[w][lane]);
-    const long long o = static_cast<long long>(blockIdx.x) * a.count + lane;
-    if (lane < a.count) {
-        a.best[o] = best.p.value;
-        a.token[o] = best.p.at;
+    for (int d = 1; d < kWarps; d <<= 1) {
+        __syncthreads();
+        if (warp % (2 * d) == 0) {
+            best.join_sorted(wait_s[warp + d][lane]);
+            wait[lane] = best.p;
+        }
     }
-    if (lane == 0) {
-        top = fmaxf(fmaxf(sum_s[0].x, sum_s[1].x), fmaxf(sum_s[2].x, sum_s[3].x));
-        a.sum[blockIdx.x] = make_float2(top, (scaled(sum_s[0], top) + scaled(sum_s[1], top)) + (scaled(sum_s[2], top) + scaled(sum_s[3], top)));
+    if (warp == 0) {
+        const float2 mine = lane < kWarps ? sum_s[lane] : make_float2(kLowest, 0.f);
+        top = warp_max(mine.x);
+        s = warp_sum(scaled(mine, top));
+        if constexpr (CLUSTER) {
+            list_s[lane] = best.p;
+            if (lane == 0) total_s = make_float2(top, s);
+        } else {
+            a.best[static_cast<long long>(blockIdx.x) * 32 + lane] = best.p;
+            if (lane == 0) a.sum[blockIdx.x] = make_float2(top, s);
+        }
+    }
+    if constexpr (CLUSTER) {
+        cluster_sync_all();
+        if (cluster_ctarank() == 0) {
+            const uint32_t lists = smem_u32(list_s), totals = smem_u32(&total_s);
+            finish(a, b, kWarps, reinterpret_cast<uint8_t*>(ring_s),
+                   [&](int k, int p) {
+                       const unsigned long long v = load_cluster64(mapa_shared(lists + lane * 8, k * a.parts + p));
+                       return Pair{__uint_as_float(static_cast<uint32_t>(v)), static_cast<int>(v >> 32)};
+                   },
+                   [&](int k, int p) {
+                       const unsigned long long v = load_cluster64(mapa_shared(totals, k * a.parts + p));
+                       return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
+                   });
+        }
+        cluster_sync_all();  // no block's shared memory goes before it has been read
     }
 }
 
-// Block per batch entry, a warp per beam: its log-sum-exp and the best of its parts' lists; then the rank of
-// every beam's candidates among all of them, counted by a thread each.
+// Block per batch entry, a warp per beam.
 static __global__ void __launch_bounds__(1024) select_join_kernel(const Select a) {
     MM_PDL_ENTRY();
-    __shared__ double score_s[kMaxBeams * kMaxBeams];
-    __shared__ int at_s[kMaxBeams * kMaxBeams];
-    const int b = blockIdx.x, k = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = b * a.beams + k, n = a.parts * a.count;
-    // everything asked for at once: what the parts of a finished or dead beam hold is not used
-    const long long p0 = static_cast<long long>(row) * a.parts;
-    auto entry = [&](int i) { return i < n ? Pair{__ldcg(a.best + p0 * a.count + i), __ldcg(a.token + p0 * a.count + i)} : Pair{-INFINITY, kNobody}; };
-    Pair next = entry(lane);
-    const float2 sum = lane < a.parts ? __ldcg(a.sum + p0 + lane) : make_float2(kLowest, 0.f);
-    const float score = __ldg(a.scores + row);
-    const bool ended = a.finished && __ldg(a.finished + row);
-    double cand = -INFINITY;
-    int at = kNobody;
-    if (finite(score)) {
-        if (ended) {
-            if (lane == 0) {
-                cand = score;
-                at = k * a.vocab + a.eos;
-            }
-        } else {
-            const float top = warp_max(sum.x);
-            const double s = static_cast<double>(sum.y) * exp(static_cast<double>(sum.x) - top);
-            const double lse = top + log(warp_sum(s));
-            Best best;
-#pragma unroll 1
-            for (int i = 32; i < n + 32; i += 32) {
-                const Pair q = next;
-                next = entry(i + lane);
-                best.join(q);
-            }
-            // a log-sum-exp that is not finite makes no candidate; what fp32 cannot hold is no score
-            cand = score + (static_cast<double>(best.p.value) - lse);
-            if (best.p.at != kNobody && fabs(lse) < INFINITY && static_cast<float>(cand) > -INFINITY) at = k * a.vocab + best.p.at;
-        }
-    }
-    if (lane < a.count) {
-        score_s[k * a.count + lane] = cand;
-        at_s[k * a.count + lane] = at;
-    }
-    const int all = a.beams * a.count, i = threadIdx.x;
-    const long long o = static_cast<long long>(b) * a.count;
-    const int candidates = __syncthreads_count(lane < a.count && at != kNobody);
-    // 2^side threads a candidate, which fit: the block has 32 threads a beam
-    const int side = 31 - __clz(32 / a.count), mine = i >> side;
-    double c = 0;
-    int t = kNobody, rank = 0;
-    if (mine < all && at_s[mine] != kNobody) {
-        c = score_s[mine];
-        t = at_s[mine];
-#pragma unroll 4
-        for (int j = i & ((1 << side) - 1); j < all; j += 1 << side)
-            rank += at_s[j] != kNobody && (score_s[j] > c || (score_s[j] == c && at_s[j] < t));
-    }
-    for (int d = 1; d < 1 << side; d <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, d);
-    if (t != kNobody && rank < a.count && (i & ((1 << side) - 1)) == 0) {
-        a.out_scores[o + rank] = static_cast<float>(c);
-        a.out_parents[o + rank] = t / a.vocab;
-        a.out_tokens[o + rank] = t % a.vocab;
-    }
-    if (i >= candidates && i < a.count) {  // left over
-        a.out_scores[o + i] = -INFINITY;
-        a.out_parents[o + i] = min(i, a.beams - 1);
-        a.out_tokens[o + i] = -1;
-    }
+    extern __shared__ uint4 join_s[];
+    const int b = blockIdx.x, lane = threadIdx.x & 31;
+    finish(a, b, a.beams, reinterpret_cast<uint8_t*>(join_s),
+           [&](int k, int p) {
+               const float2 v = __ldcg(reinterpret_cast<const float2*>(a.best + (static_cast<long long>(b * a.beams + k) * a.parts + p) * 32 + lane));
+               return Pair{v.x, __float_as_int(v.y)};
+           },
+           [&](int k, int p) { return __ldcg(a.sum + static_cast<long long>(b * a.beams + k) * a.parts + p); });
 }
 
 }  // namespace beam

@@ -190,14 +190,55 @@ void check_select(int batch, int beams, int vocab, int count) {
     if (vocab > mm::beam::kMaxVocab) refuse(MM_UNSUPPORTED, "beam selection: vocabulary over 1,048,576");
 }
 
-// Parts of a beam's tokens, a block of four warps each: as many as fill the multiprocessors with 32 warps, of
-// 2,048 tokens or more.
-int select_parts(int batch, int beams, int vocab) {
-    const int64_t rows = static_cast<int64_t>(batch) * beams, most = std::min((vocab + 2047) / 2048, mm::beam::kMaxParts);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 8 * sm_count() / std::max<int64_t>(rows, 1))));
+// How a selection is launched: parts of a beam's tokens, a block of eight warps each, as many as fill the
+// multiprocessors with 32 warps, of 4,096 tokens or more. In clusters where a batch entry's blocks can be one, none
+// has more than 32,768 tokens then and there are few: us in clusters / with a second kernel, 1 x 4 beams of 16,384
+// 8.7 / 11.6, 4 x 16 of 32,768 13.6 / 17.7, 16 x 8 (128 blocks) 17.5 / 17.0, 64 x 8 (512) 25.0 / 23.5.
+struct SelectPlan {
+    int parts;
+    bool cluster;
+    int64_t bytes;
+};
+SelectPlan select_plan(int batch, int beams, int vocab) {
+    const int64_t rows = std::max<int64_t>(1, static_cast<int64_t>(batch) * beams), most = std::min((vocab + 4095) / 4096, mm::beam::kMaxParts);
+    SelectPlan r{static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 4 * sm_count() / rows))), false, 0};
+    const int fits = mm::beam::kMaxCluster / beams;
+    const int parts = std::min(fits, r.parts);
+    if (parts > 0 && (vocab + parts - 1) / parts <= 32768 && rows * parts <= sm_count() / 2) {
+        r.parts = parts;
+        r.cluster = true;
+    } else {
+        r.bytes = static_cast<int64_t>(batch) * beams * r.parts * (32 * sizeof(mm::beam::Pair) + sizeof(float2));
+    }
+    return r;
 }
-int64_t select_bytes(int batch, int beams, int vocab, int count) {
-    return batch == 0 ? 0 : static_cast<int64_t>(batch) * beams * select_parts(batch, beams, vocab) * (8 + 8LL * count);
+
+template <typename T> void launch_select(const mm::beam::Select& a, const SelectPlan& r, cudaStream_t s) {
+    using namespace mm::beam;
+    const unsigned grid = blocks(static_cast<long long>(a.batch) * a.beams * r.parts, 1);
+    if (!r.cluster) {
+        set_dynamic_smem<select_parts_kernel<T, false>>(kRing);
+        launch(s, select_parts_kernel<T, false>, dim3(grid), dim3(32 * kWarps), kRing, a);
+        launch(s, select_join_kernel, dim3(a.batch), dim3(32 * a.beams), 512 * a.beams, a);
+        return;
+    }
+    static_assert(512 * kWarps <= kRing, "the join's scratch");
+    set_dynamic_smem<select_parts_kernel<T, true>>(kRing);
+    check(cudaFuncSetAttribute(select_parts_kernel<T, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cluster size");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(32 * kWarps);
+    cfg.dynamicSmemBytes = kRing;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = static_cast<unsigned>(a.beams * r.parts);
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    check(cudaLaunchKernelEx(&cfg, select_parts_kernel<T, true>, a), "kernel launch");
 }
 
 }  // namespace
@@ -305,7 +346,7 @@ int64_t mm_beam_select_workspace(int batch, int beams, int vocab, int count) {
     int64_t bytes = 0;
     const int rc = guarded([&] {
         check_select(batch, beams, vocab, count);
-        bytes = select_bytes(batch, beams, vocab, count);
+        if (batch > 0) bytes = select_plan(batch, beams, vocab).bytes;
     });
     return rc ? -static_cast<int64_t>(rc) : bytes;
 }
@@ -323,20 +364,14 @@ int mm_beam_select(const void* logits, int64_t batch_stride, int64_t beam_stride
         with_type(dtype, [&](auto t) {
             require(multiple(logits, sizeof(typename decltype(t)::type)), "beam selection: logits not aligned to their elements");
         });
-        require(workspace && multiple(workspace, 16) && workspace_bytes >= static_cast<size_t>(select_bytes(batch, beams, vocab, count)),
+        const SelectPlan r = select_plan(batch, beams, vocab);
+        require(r.bytes == 0 || (workspace && multiple(workspace, 16) && workspace_bytes >= static_cast<size_t>(r.bytes)),
                 "beam selection: workspace too small or not 16-byte aligned");
-        const int parts = select_parts(batch, beams, vocab);
-        const int64_t lists = static_cast<int64_t>(batch) * beams * parts;
-        float2* sums = static_cast<float2*>(workspace);
-        float* best = reinterpret_cast<float*>(sums + lists);
-        mm::beam::Select a{logits, batch_stride, beam_stride, scores, finished, eos, batch, beams, vocab, count, parts,
-                           out_scores, out_parents, out_tokens, best, reinterpret_cast<int*>(best + lists * count), sums};
-        cudaStream_t s = static_cast<cudaStream_t>(stream);
-        with_type(dtype, [&](auto t) {
-            using T = typename decltype(t)::type;
-            launch(s, mm::beam::select_parts_kernel<T>, dim3(blocks(lists, 1)), dim3(128), 0, a);
-            launch(s, mm::beam::select_join_kernel, dim3(batch), dim3(32 * beams), 0, a);
-        });
+        mm::beam::Pair* best = static_cast<mm::beam::Pair*>(workspace);
+        const mm::beam::Select a{logits, batch_stride, beam_stride, scores, finished, eos, batch, beams, vocab, count, r.parts,
+                                 out_scores, out_parents, out_tokens, best,
+                                 reinterpret_cast<float2*>(best + static_cast<int64_t>(batch) * beams * r.parts * 32)};
+        with_type(dtype, [&](auto t) { launch_select<typename decltype(t)::type>(a, r, static_cast<cudaStream_t>(stream)); });
     });
 }
 
