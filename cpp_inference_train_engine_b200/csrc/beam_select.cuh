@@ -7,10 +7,12 @@
 // reach it are looked at again, from the cache. Where a batch entry's blocks fit a cluster (16) its first block joins
 // them from their shared memory, else a second kernel from the workspace.
 #pragma once
-#include "latent_cache.cuh"
+#include "paged_cache.cuh"
 
 namespace mm {
 namespace beam {
+
+using paged::Two;
 
 constexpr int kMaxBeams = 32;
 constexpr int kMaxVocab = 1 << 20;  // flat candidates k * vocab + v stay below 2^25
@@ -74,25 +76,6 @@ struct Best {
 };
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
-
-// Two fp32 values in one register pair: sums and products of both in one instruction.
-struct Two {
-    unsigned long long v;
-    __device__ __forceinline__ Two(unsigned long long x) : v(x) {}
-    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-    __device__ __forceinline__ float lo() const { return __uint_as_float(static_cast<uint32_t>(v)); }
-    __device__ __forceinline__ float hi() const { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
-};
-__device__ __forceinline__ Two operator+(Two a, Two b) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ Two operator*(Two a, Two b) {
-    unsigned long long r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
-    return r;
-}
 
 // Candidates of several beams: scores in fp64, k * vocab + v.
 struct Scored {

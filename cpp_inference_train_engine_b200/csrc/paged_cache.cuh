@@ -6,6 +6,30 @@
 namespace mm {
 namespace paged {
 
+// Two fp32 values in one register pair: sums and products of both in one instruction.
+struct Two {
+    unsigned long long v;
+    __device__ __forceinline__ Two(unsigned long long x) : v(x) {}
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ float lo() const { return __uint_as_float(static_cast<uint32_t>(v)); }
+    __device__ __forceinline__ float hi() const { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
 struct Table {
     const int* entry;
     long long stride;
@@ -90,7 +114,7 @@ __global__ void __launch_bounds__(256) append_kernel(lat::CacheOut c, Table tabl
 
 // KV = 128 or 512, 16-byte accesses: KV / 16 lanes take a token, 16 latent values and (the first R / 2 of them)
 // one pair of the key each; sums and maxima are shuffle reductions over the lane group. The CTAs that fit walk
-// the tokens, the next one already loaded. Bound by the bytes in and out.
+// the tokens, the next ones already on their way. Bound by the bytes that so few tokens keep in flight.
 template <typename T> struct AppendRow {
     uint4 x[sizeof(T)];
     T key[2];
@@ -102,14 +126,13 @@ __global__ void __launch_bounds__(256, kAppendCtas<T>) append_vec_kernel(
     lat::CacheOut c, Table table, const T* __restrict__ values, long long stride, const int* __restrict__ rows,
     const int* __restrict__ positions, long long n, const float* __restrict__ norm, float eps, const __grid_constant__ Rotation rot) {
     constexpr int L = KV / 16, P = 32 / L;  // lanes per token, tokens side by side in a warp
+    __shared__ float4 norm_s[KV / 4];       // (in registers they would cost the second token ahead)
     const int lane = threadIdx.x & 31, sub = lane % L;
     const double f = sub < R / 2 ? rot.f[sub] : 0.0;
     MM_PDL_ENTRY();
-    float w[16];
-    if (norm) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) *reinterpret_cast<float4*>(w + 4 * e) = __ldg(reinterpret_cast<const float4*>(norm + sub * 16) + e);
-    }
+    // (quarter q of every lane's 16 in line: no bank is asked twice)
+    if (norm && threadIdx.x < KV / 4) norm_s[threadIdx.x % 4 * L + threadIdx.x / 4] = __ldg(reinterpret_cast<const float4*>(norm) + threadIdx.x);
+    __syncthreads();
     auto fetch = [&](long long i) {
         AppendRow<T> v;
         v.position = -1;
@@ -133,23 +156,36 @@ __global__ void __launch_bounds__(256, kAppendCtas<T>) append_vec_kernel(
     const long long step = static_cast<long long>(gridDim.x) * 8 * P;
     long long i0 = (static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * P;
     const int mine = lane / L;
-    AppendRow<T> next = fetch(i0 + mine);
+    constexpr int kAhead = sizeof(T) == 4 ? 1 : 2;  // tokens of a lane group on their way
+    AppendRow<T> next[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) next[k] = fetch(i0 + mine + k * step);
     for (; i0 < n; i0 += step) {  // whole warps walk together (the reductions' shuffles)
-        const AppendRow<T> r = next;
+        const AppendRow<T> r = next[0];
         int at = 0;
         const long long p = page_of(table, c.rows, c.positions, r.row, r.position, at);
-        next = fetch(i0 + mine + step);
+#pragma unroll
+        for (int k = 0; k + 1 < kAhead; ++k) next[k] = next[k + 1];
+        next[kAhead - 1] = fetch(i0 + mine + kAhead * step);
         float v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = lat::to_f32(reinterpret_cast<const T*>(r.x)[e]);
         float inv = 1.f;  // what the values below are still to be multiplied by
         if (norm) {
-            float sum = 0.f;
+            Two sums[2] = {Two(0.f, 0.f), Two(0.f, 0.f)};
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                sum = fmaf(v[e], v[e], sum);
-                v[e] *= w[e];
+            for (int e = 0; e < 16; e += 4) {
+                const float4 w = norm_s[e / 4 * L + sub];
+                const Two x(v[e], v[e + 1]), y(v[e + 2], v[e + 3]), a = x * Two(w.x, w.y), b = y * Two(w.z, w.w);
+                sums[0] = fma2(x, x, sums[0]);
+                sums[1] = fma2(y, y, sums[1]);
+                v[e] = a.lo();
+                v[e + 1] = a.hi();
+                v[e + 2] = b.lo();
+                v[e + 3] = b.hi();
             }
+            sums[0] = sums[0] + sums[1];
+            float sum = sums[0].lo() + sums[0].hi();
 #pragma unroll
             for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             inv = rsqrtf(sum * (1.f / KV) + eps);
@@ -169,9 +205,11 @@ __global__ void __launch_bounds__(256, kAppendCtas<T>) append_vec_kernel(
             const float f8 = inv * __frcp_rn(s);
             uint32_t q[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                q[e] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(v[4 * e] * f8, v[4 * e + 1] * f8), __NV_SATFINITE, __NV_E4M3)) |
-                       (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(v[4 * e + 2] * f8, v[4 * e + 3] * f8), __NV_SATFINITE, __NV_E4M3)) << 16);
+            for (int e = 0; e < 4; ++e) {
+                const Two by(f8, f8), x = Two(v[4 * e], v[4 * e + 1]) * by, y = Two(v[4 * e + 2], v[4 * e + 3]) * by;
+                q[e] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x.lo(), x.hi()), __NV_SATFINITE, __NV_E4M3)) |
+                       (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(y.lo(), y.hi()), __NV_SATFINITE, __NV_E4M3)) << 16);
+            }
             *reinterpret_cast<uint4*>(c.latent + p * c.row_stride + at * c.pos_stride + sub * 16) = make_uint4(q[0], q[1], q[2], q[3]);
             if (sub == 0) c.scale[p * c.scale_row_stride + at] = s;
             key = reinterpret_cast<T16*>(c.rope) + p * c.rope_row_stride + at * c.rope_pos_stride;
