@@ -156,8 +156,8 @@ MmaPlan mma_plan(const mm::paged::Attention& p) {
     const int64_t tiles = p.window > 0 ? std::min(all, (static_cast<int64_t>(p.window) + p.sinks) / kTile + 3) : all;
     const int64_t ctas = 2 * sm_count(), least = min_share(p.kv);
     // rows of few tiles are not worth cutting (and weights are 32-bit)
-    r.shares = tiles > least && r.units * (tiles + kRowCost) < INT32_MAX / 2;
-    r.grid = static_cast<int>(std::min(ctas, r.shares ? (r.units * (tiles + kRowCost) + least - 1) / least : r.units));
+    r.shares = tiles > least && r.units * (tiles + row_cost(p.kv)) < INT32_MAX / 2;
+    r.grid = static_cast<int>(std::min(ctas, r.shares ? (r.units * (tiles + row_cost(p.kv)) + least - 1) / least : r.units));
     r.entries = static_cast<int>(std::min<int64_t>(r.units, r.grid));
     return r;
 }

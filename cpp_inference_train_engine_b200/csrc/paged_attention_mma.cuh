@@ -16,7 +16,7 @@
 // would be one). Two CTAs an SM, each with a ring of its own; the row's sums and maxima are fp32, the weights of
 // the second product are rounded to 16 bits once, as its operand has to be.
 //
-// The tiles of all rows, in line, are divided evenly over the CTAs (a row costs kRowCost tiles more); a row
+// The tiles of all rows, in line, are divided evenly over the CTAs (a row costs row_cost() tiles more); a row
 // that is cut leaves partial results to the join kernel.
 #pragma once
 #include <type_traits>
@@ -38,7 +38,10 @@ struct MmaArgs {
 };
 
 constexpr int kTile = 32;       // positions
-constexpr int kRowCost = 2;     // tiles that a row's queries and results cost
+// Tiles that a row's queries and results cost: of 4 to 40, by 512 rows of up to 2,048, 128 wide (2: 42.7 us, 6: 41.0,
+// 10: 39.8, 20: 40.2, 40: 44.2), and 96 of up to 8,192 and 400 of up to 700, 512 wide (2: 86.7 and 47, 4: 84.2 and
+// 46, 6: 83.4 and 46.8, 10: 83.7 and 47.9).
+constexpr int row_cost(int kv) { return kv == 128 ? 10 : 4; }
 // tiles of a CTA at least (128 wide they are a quarter of the bytes, and each of the four warps has its own)
 constexpr int min_share(int kv) { return kv == 128 ? 16 : 6; }
 constexpr int kMmaThreads = 160;
@@ -57,7 +60,8 @@ template <int KV, int R, bool Q8> struct MmaCfg {
     static constexpr int SG = KV == 512 ? (Q8 ? 5 : 3) : (Q8 ? 3 : 2);     // slots of a group
     static constexpr int SLOTS = KG * SG;
     // 512: the four shares of S; 128: the four results of a row
-    static constexpr int kShare = KV == 512 ? 4 * 16 * kTile * 4 : 4 * 16 * 128 * 4;
+    static constexpr int kShareRow = 136;  // (128 columns and 8 more, which spread eight rows over all banks)
+    static constexpr int kShare = KV == 512 ? 4 * 16 * kTile * 4 : 4 * 16 * kShareRow * 4;
     static constexpr int oShare = SLOTS * kSlot;
     static constexpr int oStat = oShare + kShare;           // [4][16] maxima and sums (128 wide)
     static constexpr int oTops = oStat;                     // [4][16] maxima, sums (512 wide)
@@ -88,12 +92,14 @@ __device__ __forceinline__ int row_tiles(const Attention& p, int len, int& sink_
 }
 
 // The runs of a CTA. With even shares, the CTA's are the tiles of weight [w0, w1) of all rows in line, where a
-// row's tiles are followed by kRowCost more.
+// row's tiles are followed by its cost.
 struct Runs {
     const MmaArgs& a;
     int w0, w1, span, before;  // the share, and the weight ahead of row `row`
+    int cost;
     int row, block, len;
-    __device__ __forceinline__ Runs(const MmaArgs& args, int span_, int row0, int before0) : a(args), span(span_) {
+    __device__ __forceinline__ Runs(const MmaArgs& args, int cost_, int span_, int row0, int before0)
+        : a(args), span(span_), cost(cost_) {
         if (a.shares) {
             w0 = static_cast<int>(blockIdx.x) * span;
             w1 = w0 + span;
@@ -123,7 +129,7 @@ struct Runs {
                 if (row < a.p.B) len = length_of(a.p, row);
                 return true;
             }
-            const int at = before + block * (n + kRowCost);
+            const int at = before + block * (n + cost);
             if (at >= w1) return false;
             const bool begins = at >= w0;
             r.from = begins ? 0 : min(w0 - at, n);
@@ -133,7 +139,7 @@ struct Runs {
             cut = !begins ? -1 : whole ? 0 : (at + n - 1) / span - static_cast<int>(blockIdx.x) + 1;
             if (++block == a.blocks) {
                 block = 0;
-                before += a.blocks * (n + kRowCost);
+                before += a.blocks * (n + cost);
                 if (++row < a.p.B) len = length_of(a.p, row);
             }
             if (begins || r.from < r.to) return true;
@@ -255,7 +261,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
         const int per = (p.B + kMmaThreads - 1) / kMmaThreads, b0 = tid * per, b1 = min(b0 + per, p.B);
         auto weight = [&](int b) {
             int st, skip;
-            return (row_tiles(p, length_of(p, b), st, skip) + kRowCost) * a.blocks;
+            return (row_tiles(p, length_of(p, b), st, skip) + row_cost(KV)) * a.blocks;
         };
         int mine = 0;
 #pragma unroll 4
@@ -300,7 +306,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
 
     if (warp == 4) {
         // ------------------------------------------------------------ loads
-        Runs runs(a, a.shares ? plan[5] : 0, a.shares ? plan[7] : 0, a.shares ? plan[6] : 0);
+        Runs runs(a, row_cost(KV), a.shares ? plan[5] : 0, a.shares ? plan[7] : 0, a.shares ? plan[6] : 0);
         Run run;
         // A step is a tile for each group. This lane's box of its group's tile: which stretch of `box` positions,
         // which box of it (128 wide: 3 or 6 boxes for 8 lanes; 512 wide: at most 18 for 32).
@@ -333,6 +339,12 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 q_phase ^= 1;
             }
             if (!more) break;
+            {  // its queries, for the warps of the products
+                constexpr int kLines = ((KV + R) * 2 + 127) / 128;
+                const T* heads = static_cast<const T*>(p.q) + run.row * p.q_row + run.h0 * p.q_head;
+                const int n = min(16, p.H - run.h0) * kLines;
+                for (int e = lane; e < n; e += 32) prefetch_l1(heads + e / kLines * p.q_head + min(e % kLines * 64, KV + R - 1));
+            }
             // page and entry of this lane's stretch of tile i
             int id, at;
             auto ask = [&](int i) {
@@ -837,7 +849,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int row = g + 8 * h;
-                    float* dst = share + (warp * 16 + row) * 128;
+                    float* dst = share + (warp * 16 + row) * C::kShareRow;
 #pragma unroll
                     for (int n = 0; n < 16; n += 2) {
                         if constexpr (!Q8) {
@@ -870,7 +882,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     for (int x = 0; x < 4; ++x) {
                         const float fx = fast_exp2(st[x].x - M);
                         L = fmaf(st[x].y, fx, L);
-                        const float4 y = *reinterpret_cast<const float4*>(share + (x * 16 + row) * 128 + lane * 4);
+                        const float4 y = *reinterpret_cast<const float4*>(share + (x * 16 + row) * C::kShareRow + lane * 4);
                         v.x = fmaf(y.x, fx, v.x);
                         v.y = fmaf(y.y, fx, v.y);
                         v.z = fmaf(y.z, fx, v.z);

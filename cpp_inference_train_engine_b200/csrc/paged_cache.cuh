@@ -120,7 +120,9 @@ template <typename T> struct AppendRow {
     T key[2];
     int position, row;
 };
-template <typename T> constexpr int kAppendCtas = sizeof(T) == 4 ? 3 : 4;  // CTAs per SM
+// CTAs per SM (131,072 fp16 tokens of 512 + 32 into 8-bit pages, two ahead: 51 us; with three CTAs 53, with three
+// tokens ahead 57, and where either spills 80 to 120)
+template <typename T> constexpr int kAppendCtas = sizeof(T) == 4 ? 3 : 4;
 template <typename T, typename T16, int KV, int R, bool Q8>
 __global__ void __launch_bounds__(256, kAppendCtas<T>) append_vec_kernel(
     lat::CacheOut c, Table table, const T* __restrict__ values, long long stride, const int* __restrict__ rows,
