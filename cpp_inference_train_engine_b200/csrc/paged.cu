@@ -162,10 +162,11 @@ MmaPlan mma_plan(const mm::paged::Attention& p) {
     return r;
 }
 
-template <int KV, int R, typename T, bool Q8>
+template <int KV, int R, typename T, bool Q8, bool HALF = false>
 void run_mma(const mm::paged::Attention& p, const MmaPlan& r, const PoolMaps& maps, void* workspace, cudaStream_t s) {
     using namespace mm::paged;
     using C = MmaCfg<KV, R, Q8>;
+    if (KV == 128 && !HALF && p.H <= 8) return run_mma<KV, R, T, Q8, KV == 128>(p, r, maps, workspace, s);
     MmaArgs a{};
     a.p = p;
     a.box = p.pool.positions % 32 == 0 ? 32 : 16;
@@ -175,8 +176,8 @@ void run_mma(const mm::paged::Attention& p, const MmaPlan& r, const PoolMaps& ma
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(2) * r.grid * 16 * KV);
     a.cut = reinterpret_cast<int4*>(a.part_ml + int64_t(2) * r.grid * 16);
-    set_dynamic_smem<paged_mma_kernel<KV, R, T, Q8>>(C::kSmem);
-    launch(s, paged_mma_kernel<KV, R, T, Q8>, dim3(r.grid), dim3(kMmaThreads), C::kSmem, a, maps.latent, maps.rope, maps.scale);
+    set_dynamic_smem<paged_mma_kernel<KV, R, T, Q8, HALF>>(C::kSmem);
+    launch(s, paged_mma_kernel<KV, R, T, Q8, HALF>, dim3(r.grid), dim3(kMmaThreads), C::kSmem, a, maps.latent, maps.rope, maps.scale);
     if (r.shares) {
         // a warp a head, or a block for 128 columns of one where the parts are many because the units are few
         const int y = std::max(2, std::min(2 * sm_count() / r.entries, 16 * KV / 128));

@@ -216,11 +216,13 @@ __device__ __forceinline__ float exponent_of(float s) {
     return static_cast<float>(min(max(static_cast<int>((__float_as_uint(s) >> 23) & 255) - 127, -40), 100));
 }
 
-template <int KV, int R, typename T, bool Q8>
+// HALF: at most 8 heads, whose rows are the first 8 of the products': nothing is done for the others.
+template <int KV, int R, typename T, bool Q8, bool HALF>
 __global__ void __launch_bounds__(kMmaThreads, 2)
     paged_mma_kernel(const __grid_constant__ MmaArgs a, const __grid_constant__ CUtensorMap map_latent,
                      const __grid_constant__ CUtensorMap map_rope, const __grid_constant__ CUtensorMap map_scale) {
     using C = MmaCfg<KV, R, Q8>;
+    constexpr int RH = HALF ? 1 : 2;               // halves of the 16 rows
     using TP = std::conditional_t<Q8, __half, T>;  // the second product's type (codes are exact in fp16)
     // log2 of the largest weight when its reference is taken: small fp16 ones stay normal, large ones below 2^16
     constexpr float kGrowth = 8.f, kLift = !std::is_same<TP, __half>::value ? 0.f : C::CW > 1 ? 6.f : 10.f;
@@ -559,6 +561,17 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 const uint32_t seen = seen_of(sl, i);
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2 * RH; ++e) s[n][e] *= cs;
+                if (seen != ~0u) {
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2 * RH; ++e)
+                            if (!((seen >> (n * 8 + t4 * 2 + (e & 1))) & 1)) s[n][e] = -INFINITY;
+                }
+#pragma unroll
                 for (int n = 0; n < 4; ++n) {
                     float2 e2 = make_float2(0.f, 0.f);
                     if constexpr (Q8) {
@@ -566,15 +579,12 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                         e2 = make_float2(exponent_of(v.x), exponent_of(v.y));
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[n][e] *= cs;
-                        if (seen != ~0u && !((seen >> (n * 8 + t4 * 2 + (e & 1))) & 1)) s[n][e] = -INFINITY;
+                    for (int e = 0; e < 2 * RH; ++e)
                         top[e >> 1] = fmaxf(top[e >> 1], Q8 ? s[n][e] + (e & 1 ? e2.y : e2.x) : s[n][e]);
-                    }
                 }
-                float corr[2], ref[2];
+                float corr[2] = {1.f, 1.f}, ref[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < RH; ++h) {
                     const float mn = fmaxf(m[h], quad_max(top[h]));
                     const float at = mn == -INFINITY ? 0.f : mn;
                     corr[h] = m[h] == mn ? 1.f : fast_exp2(m[h] - at);
@@ -586,8 +596,10 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     for (int n = 0; n < 16; ++n) {
                         o[n][0] *= corr[0];
                         o[n][1] *= corr[0];
-                        o[n][2] *= corr[1];
-                        o[n][3] *= corr[1];
+                        if (RH == 2) {
+                            o[n][2] *= corr[1];
+                            o[n][3] *= corr[1];
+                        }
                     }
                     l[0] *= corr[0];
                     l[1] *= corr[1];
@@ -602,9 +614,9 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                             if (!((seen >> (n * 8 + t4 * 2 + 1)) & 1)) v.y = 0.f;
                         }
                     }
-                    float e[4];
+                    float e[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
+                    for (int x = 0; x < 2 * RH; ++x) {
                         e[x] = fast_exp2(s[n][x] - ref[x >> 1]);
                         l[x >> 1] += e[x];
                         if (Q8) e[x] *= x & 1 ? v.y : v.x;
@@ -847,7 +859,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 float2* stat = reinterpret_cast<float2*>(smem + C::oStat);
                 products_sync();  // the last row's have been read
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < RH; ++h) {
                     const int row = g + 8 * h;
                     float* dst = share + (warp * 16 + row) * C::kShareRow;
 #pragma unroll
@@ -864,10 +876,10 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     if (t4 == 0) stat[warp * 16 + row] = make_float2(l[h] == 0.f ? kNone : m[h] - kLift, l[h]);
                 }
                 products_sync();
-                // a warp takes four query rows, a lane four columns
+                // a warp takes every fourth query row, a lane four columns
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = warp * 4 + r;
+                for (int r = 0; r < 2 * RH; ++r) {
+                    const int row = r * 4 + warp;
                     if (row >= heads) break;
                     float2 st[4];
                     float M = kNone;
