@@ -179,6 +179,17 @@ template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The same from zero.
+template <typename T> __device__ __forceinline__ void mma16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 // Byte offset of 16-byte chunk c of row r in a box of 128-, 64- or 32-byte rows, as TMA swizzles it.
 __device__ __forceinline__ uint32_t swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 template <int R> __device__ __forceinline__ uint32_t swizzled_rope(int r, int c) {
@@ -234,7 +245,8 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
     uint64_t* run_full = empty + C::SLOTS;
     uint64_t* run_empty = run_full + kQueue;
     Run* queue = reinterpret_cast<Run*>(smem + C::oRuns);
-    volatile uint16_t* meta = reinterpret_cast<volatile uint16_t*>(smem + C::oMeta);  // per slot and 16 positions
+    // positions of the tile in a slot that the row sees, by halves of 16
+    volatile uint16_t* meta = reinterpret_cast<volatile uint16_t*>(smem + C::oMeta);
     int* plan = reinterpret_cast<int*>(smem + C::oPlan);  // the warps' sums; span, weight ahead, row
     volatile int* bad = reinterpret_cast<volatile int*>(smem + C::oPlan + 44);
     const Attention& p = a.p;
@@ -357,6 +369,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 if (loads && i < run.to && t < run.len) id = __ldg(p.table.entry + run.row * p.table.stride + c);
             };
             ask(run.from + group);
+            const int start = window_start(p, run.len), sinks = min(p.sinks, start);
             for (int i = run.from + group; i - group < run.to; i += C::KG) {
                 // a page outside the pool (or behind the row) is asked for behind the last one: zeros
                 const bool there = id >= 0 && id < p.pool.rows, mine = i < run.to;
@@ -369,8 +382,14 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     break;
                 }
                 if (mine && loads && which == 0) {
-                    meta[2 * s + stretch] = there ? 0xffff : 0;
-                    if (a.box == kTile) meta[2 * s + 1] = there ? 0xffff : 0;
+                    uint32_t seen = 0;
+                    if (there) {
+                        const int t = run.position(i);
+                        auto below = [&](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+                        seen = below(run.len - t) & (below(sinks - t) | ~below(start - t));
+                    }
+                    if (a.box == kTile) *reinterpret_cast<volatile uint32_t*>(meta + 2 * s) = seen;
+                    else meta[2 * s + stretch] = static_cast<uint16_t>(seen >> (16 * stretch));
                 }
                 __syncwarp();
                 if (mine && sub == 0) mbar_arrive_expect_tx(&full[s], C::kBytes);
@@ -492,12 +511,9 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
 #pragma unroll
             for (int n = 0; n < 16; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
             float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-            const int start = window_start(p, run.len), sinks = min(p.sinks, start);
             // S of the tile in slot sl: this warp's columns of it
             auto scores = [&](int sl, float (&s)[4][4]) {
                 const uint32_t sp = ring + sl * C::kSlot;
-#pragma unroll
-                for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
                 if constexpr (!Q8) {
                     // (loads one step ahead of the products: issue is in order)
                     const uint32_t box = sp + s_at;
@@ -512,8 +528,13 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                         if (k < 7) load(k + 1, b[(k + 1) & 1]);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            mma16<T>(s[2 * h], q[k], b[k & 1][h][0], b[k & 1][h][1]);
-                            mma16<T>(s[2 * h + 1], q[k], b[k & 1][h][2], b[k & 1][h][3]);
+                            if (k == 0) {
+                                mma16_first<T>(s[2 * h], q[k], b[0][h][0], b[0][h][1]);
+                                mma16_first<T>(s[2 * h + 1], q[k], b[0][h][2], b[0][h][3]);
+                            } else {
+                                mma16<T>(s[2 * h], q[k], b[k & 1][h][0], b[k & 1][h][1]);
+                                mma16<T>(s[2 * h + 1], q[k], b[k & 1][h][2], b[k & 1][h][3]);
+                            }
                         }
                     }
                 } else {
@@ -527,7 +548,8 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                         for (int n = 0; n < 4; ++n) {
                             uint32_t lo, hi;
                             codes4(b[k & 1][n], lo, hi);
-                            mma16<__half>(s[n], q[k], lo, hi);
+                            if (k == 0) mma16_first<__half>(s[n], q[k], lo, hi);
+                            else mma16<__half>(s[n], q[k], lo, hi);
                         }
                     }
 #pragma unroll
@@ -549,16 +571,11 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     }
                 }
             };
-            // positions of tile i that the row sees
-            auto seen_of = [&](int sl, int i) {
-                const uint32_t there = meta[2 * (group * C::SG + sl)] | static_cast<uint32_t>(meta[2 * (group * C::SG + sl) + 1]) << 16;
-                const int p0 = run.position(i);
-                auto below = [&](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
-                return there & below(run.len - p0) & (below(sinks - p0) | ~below(start - p0));
-            };
-            // Weights of tile i (the second product's operand, 16 positions each) from its scores.
-            auto weigh = [&](int sl, int i, float (&s)[4][4], uint32_t (&w)[2][4]) {
-                const uint32_t seen = seen_of(sl, i);
+            // positions of the tile in slot sl that the row sees
+            auto seen_of = [&](int sl) { return reinterpret_cast<volatile const uint32_t*>(meta)[group * C::SG + sl]; };
+            // Weights of the tile in slot sl (the second product's operand, 16 positions each) from its scores.
+            auto weigh = [&](int sl, float (&s)[4][4], uint32_t (&w)[2][4]) {
+                const uint32_t seen = seen_of(sl);
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
@@ -686,7 +703,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 for (int i = run.from + group; i < run.to; i += C::KG) {
                     wait(&full[group * C::SG + slot], phase);
                     scores(slot, s);
-                    const uint32_t seen = weigh(slot, i, s, w);
+                    const uint32_t seen = weigh(slot, s, w);
                     values(slot, seen, w);
                     if (++slot == C::SG) {
                         slot = 0;
@@ -702,6 +719,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 float4* mine = reinterpret_cast<float4*>(share) + cw * 128 + lane;
                 uint2* hand = reinterpret_cast<uint2*>(smem + C::oHand) + lane;
                 float* tops = reinterpret_cast<float*>(smem + C::oTops);
+                float ref[2] = {-kLift, -kLift};  // what scores are taken from: m, or 0 where there is none, below the lift
                 auto put = [&](int sl) {  // (the last tile's shares were read before its weights were handed over)
                     scores(sl, s);
 #pragma unroll
@@ -715,30 +733,37 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     products_sync();
                     float z[4];
                     {
-                        const float4* v = reinterpret_cast<const float4*>(share) + cw * 32 + lane;
-                        const float4 x = v[0], y = v[128], f = v[256], u = v[384];
-                        z[0] = ((x.x + y.x) + (f.x + u.x)) * cs;
-                        z[1] = ((x.y + y.y) + (f.y + u.y)) * cs;
-                        z[2] = ((x.z + y.z) + (f.z + u.z)) * cs;
-                        z[3] = ((x.w + y.w) + (f.w + u.w)) * cs;
+                        const ulonglong2* v = reinterpret_cast<const ulonglong2*>(share) + cw * 32 + lane;
+                        const ulonglong2 x = v[0], y = v[128], f = v[256], u = v[384];
+                        const Two by(cs, cs), lo = ((Two(x.x) + Two(y.x)) + (Two(f.x) + Two(u.x))) * by,
+                                  hi = ((Two(x.y) + Two(y.y)) + (Two(f.y) + Two(u.y))) * by;
+                        z[0] = lo.lo();
+                        z[1] = lo.hi();
+                        z[2] = hi.lo();
+                        z[3] = hi.hi();
                     }
-                    const uint32_t seen = seen_of(slot, i);
-                    const bool see0 = (seen >> (cw * 8 + t4 * 2)) & 1, see1 = (seen >> (cw * 8 + t4 * 2 + 1)) & 1;
-                    if (!see0) z[0] = z[2] = -INFINITY;
-                    if (!see1) z[1] = z[3] = -INFINITY;
+                    const uint32_t seen = seen_of(slot);
                     float2 ks = make_float2(1.f, 1.f), e2 = make_float2(0.f, 0.f);
                     if constexpr (Q8) {
                         ks = scales_of(slot, cw);
                         e2 = make_float2(exponent_of(ks.x), exponent_of(ks.y));
-                        if (!see0) ks.x = 0.f;  // (0 times what an unseen position has for a scale may be a NaN)
-                        if (!see1) ks.y = 0.f;
+                    }
+                    if (seen != ~0u) {
+                        if (!((seen >> (cw * 8 + t4 * 2)) & 1)) {
+                            z[0] = z[2] = -INFINITY;
+                            ks.x = 0.f;  // (0 times what an unseen position has for a scale may be a NaN)
+                        }
+                        if (!((seen >> (cw * 8 + t4 * 2 + 1)) & 1)) {
+                            z[1] = z[3] = -INFINITY;
+                            ks.y = 0.f;
+                        }
                     }
                     const float top0 = fmaxf(z[0] + e2.x, z[1] + e2.y), top1 = fmaxf(z[2] + e2.x, z[3] + e2.y);
                     float add[2];
                     auto give = [&] {
                         float e[4];
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) e[x] = fast_exp2(z[x] - ((m[x >> 1] == -INFINITY ? 0.f : m[x >> 1]) - kLift));
+                        for (int x = 0; x < 4; ++x) e[x] = fast_exp2(z[x] - ref[x >> 1]);
                         add[0] = e[0] + e[1];
                         add[1] = e[2] + e[3];
                         if constexpr (Q8) {
@@ -764,6 +789,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                             const float mn = fmaxf(fmaxf(m[h], fmaxf(t[0], t[16])), fmaxf(t[32], t[48]));
                             const float corr = m[h] == mn ? 1.f : fast_exp2(m[h] - mn);
                             m[h] = mn;
+                            ref[h] = (mn == -INFINITY ? 0.f : mn) - kLift;
                             l[h] *= corr;
 #pragma unroll
                             for (int n = 0; n < 16; ++n) {
