@@ -42,8 +42,11 @@ constexpr int kTile = 32;       // positions
 // 10: 39.8, 20: 40.2, 40: 44.2), and 96 of up to 8,192 and 400 of up to 700, 512 wide (2: 86.7 and 47, 4: 84.2 and
 // 46, 6: 83.4 and 46.8, 10: 83.7 and 47.9).
 constexpr int row_cost(int kv) { return kv == 128 ? 10 : 4; }
-// tiles of a CTA at least (128 wide they are a quarter of the bytes, and each of the four warps has its own)
-constexpr int min_share(int kv) { return kv == 128 ? 16 : 6; }
+// Tiles of a CTA at least, so that few rows make no more partial results than they gain: 512 wide, 8 rows of up to
+// 4,096 take 24.5 us with 12, 19.3 with 6, 17.3 with 4, 16.2 with 2, one of 300 13.5, 12.5 and 13.4 with 6, 4 and 2. 128
+// wide a tile is a quarter of the bytes and each of the four warps has its own: 5 rows of up to 900 take 13.6 us
+// with 8 or 16 and 9.2 with 24.
+constexpr int min_share(int kv) { return kv == 128 ? 24 : 4; }
 constexpr int kMmaThreads = 160;
 constexpr int kQueue = 4;       // runs queued for the warps of the products
 constexpr float kNone = -3.402823466e38f;  // maximum of nothing (finite: its exp2 is 0, never NaN)
