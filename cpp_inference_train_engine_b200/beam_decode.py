@@ -56,26 +56,23 @@ class BeamDecoder:
         self.prompt_len = i32([len(p) for p in prompts])
         self.max_prompt = max(len(p) for p in prompts)
         # Pages: every request's prompt in line (so that its rows are a contiguous cache too), then each beam's own
-        # for the columns it may write, and its spare one.
+        # for the columns it may write, and its spare one. The prompts are rows of their own behind the beams', from
+        # which a search's first beams descend.
         held = -(-self.max_prompt // P)                       # pages of a prompt's stretch
         columns = -(-(self.max_prompt + new_tokens) // P)
-        table = torch.full((R, columns), -1, dtype=torch.int32)
-        spare, free, first = torch.zeros(R, dtype=torch.int32), G * held, []
+        table = torch.full((R + G, columns), -1, dtype=torch.int32)
+        spare, lengths, free = torch.full((R + G,), -1, dtype=torch.int32), torch.zeros(R + G, dtype=torch.int32), G * held
         for g, p in enumerate(prompts):
-            full = len(p) // P
-            for k in range(beams):
-                r = g * beams + k
-                begin = full
-                if k == 0:  # the prompt's pages are the first beam's, the others take them over from it
-                    begin = -(-len(p) // P)
-                    table[r, :begin] = g * held + torch.arange(begin)
-                end = -(-(len(p) + new_tokens) // P)
+            table[R + g, :-(-len(p) // P)] = g * held + torch.arange(-(-len(p) // P))
+            lengths[R + g] = len(p)
+            begin, end = len(p) // P, -(-(len(p) + new_tokens) // P)
+            for r in range(g * beams, (g + 1) * beams):
                 table[r, begin:end] = free + torch.arange(end - begin)
-                spare[r] = free + end - begin
+                spare[r], lengths[r] = free + end - begin, begin * P
                 free += end - begin + 1
-                first.append(len(p) if k == 0 else full * P)
         self.cache = paged.alloc_pages(cfg.n_layers, free, P, cfg.kv_lora_rank, cfg.head_dim_rope, torch.float16, cache_bits, device)
-        self.start = (table.to(device), spare.to(device), i32(first))
+        self.start = (table.to(device), spare.to(device), lengths.to(device))
+        self.prompt_rows = torch.arange(R, R + G, dtype=torch.int32, device=device)
         self.base = (torch.arange(G, dtype=torch.int32, device=device) * beams)[:, None]  # a request's first row
         padded = torch.zeros(G, self.max_prompt, dtype=torch.int32, device=device)
         for g, p in enumerate(prompts):
@@ -115,7 +112,7 @@ class BeamDecoder:
         G, T = padded.shape
         P, c = self.page, self.cfg
         positions = torch.arange(T, dtype=torch.int32, device=self.device)[None] - (T - self.prompt_len[:, None])
-        rows = torch.repeat_interleave(self.base[:, 0], T)
+        rows = torch.repeat_interleave(self.prompt_rows, T)
 
         def attend(l, q):
             pool = paged.layer(self.cache, l)
@@ -126,7 +123,7 @@ class BeamDecoder:
                 return latent.shared_prefix_attention(q, None, stored, None, None, self.prompt_len, self.scale, kv_rank=c.kv_lora_rank)
             # with a window a prompt's tokens go one at a time: token t of every prompt is a row
             context = torch.zeros(*q.shape[:3], c.kv_lora_rank, dtype=q.dtype, device=q.device)
-            table = self.start[0][::self.beams].contiguous()
+            table = self.start[0][G * self.beams:]
             for t in range(T):
                 context[:, t] = paged.attention(q[:, t], pool, table, positions[:, t].clamp_min(-1) + 1, self.scale,
                                                 kv_rank=c.kv_lora_rank, window=self.window, sinks=self.sinks)
@@ -154,14 +151,15 @@ class BeamDecoder:
         request has no continuation left (its logits hold a NaN)."""
         c, K, N = self.cfg, self.beams, self.new_tokens
         G = self.base.shape[0]
-        table, spare, lengths = self.start
+        R = G * K
         zero = torch.zeros(G, 1, device=self.device)
-        scores, parents, tokens = paged.beam_select(self.prompt_logits[:, None].contiguous(), zero, beams=K)
+        scores, _, tokens = paged.beam_select(self.prompt_logits[:, None].contiguous(), zero, beams=K)
+        table, spare, lengths = (t[:R] for t in paged.beam_reorder(
+            self.cache, *self.start, torch.cat([torch.repeat_interleave(self.prompt_rows, K), self.prompt_rows])))
         history = torch.full((G, K, N), -1, dtype=torch.int32, device=self.device)
         history[:, :, 0] = tokens
         finished = tokens == c.eos_id
         count = torch.ones_like(tokens)
-        parents = parents + self.base  # all of them the first row's
         for step in range(1, N + 1):
             failed = torch.isneginf(scores[:, 0]).any()
             stop, none = torch.stack([finished.all(), failed]).tolist()
@@ -169,11 +167,10 @@ class BeamDecoder:
                 raise EngineError(6, "a request has no continuation with a probability (its logits hold a NaN)")
             if stop or step == N:
                 break
-            table, spare, lengths = paged.beam_reorder(self.cache, table, spare, lengths, parents.view(-1))
             live = ~finished.view(-1)
             positions = torch.where(live, lengths, -1)
             logits = self.step_logits(tokens.view(-1), positions, table)
-            lengths = lengths + live
+            lengths = lengths + live.int()
             scores, chosen, tokens = paged.beam_select(logits, scores, finished=finished, eos=c.eos_id)
             at = chosen.long()
             follow = lambda t: t.gather(1, at)  # noqa: E731
@@ -182,7 +179,7 @@ class BeamDecoder:
             history[:, :, step] = torch.where(was, -1, tokens)
             count = follow(count) + ~was
             finished = was | (tokens == c.eos_id) | (tokens < 0)
-            parents = chosen + self.base
+            table, spare, lengths = paged.beam_reorder(self.cache, table, spare, lengths, (chosen + self.base).view(-1))
         paged.check_status(self.device)
         ranked = (scores / count.float().pow(length_penalty)).nan_to_num(nan=-math.inf, neginf=-math.inf)
         order = ranked.sort(dim=1, descending=True, stable=True).indices.cpu()

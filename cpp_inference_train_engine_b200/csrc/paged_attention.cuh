@@ -49,10 +49,10 @@ __global__ void __launch_bounds__(32 * kAnyWarps) any_width_kernel(const Attenti
     const int len = length_of(p, b), start = window_start(p, len);
     float m = -INFINITY, l = 0.f;
     const int sinks = min(p.sinks, start);  // positions [0, sinks) and [start, len) are seen
-    for (int i0 = 0; i0 < sinks + len - start; i0 += 32) {
-        const int i = i0 + lane, j = i < sinks ? i : start + i - sinks;
+    for (long long i0 = 0; i0 < sinks + len - start; i0 += 32) {
+        const long long i = i0 + lane, j = i < sinks ? i : start + i - sinks;
         int at = 0;
-        const long long page = j < len ? page_of(p.table, p.pool.rows, p.pool.positions, b, j, at) : -1;
+        const long long page = j < len ? page_of(p.table, p.pool.rows, p.pool.positions, b, static_cast<int>(j), at) : -1;
         float s = -INFINITY, ks = 1.f;
         const uint8_t* k = p.pool.latent + (page * p.pool.row_stride + at * p.pool.pos_stride) * (Q8 ? 1 : 2);
         if (page >= 0) {

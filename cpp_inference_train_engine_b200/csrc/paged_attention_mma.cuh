@@ -83,15 +83,17 @@ template <int KV, int R, bool Q8> struct MmaCfg {
 struct alignas(16) Run {
     int row, h0, len, sinks, skip, from, to;
     int part;  // slot of partial results, -1: the whole row
-    __device__ __forceinline__ int position(int i) const { return kTile * (i < sinks ? i : i + skip); }
+    // (unsigned: a step past a row of 2^31 positions wraps around, and is not used)
+    __device__ __forceinline__ int position(int i) const { return static_cast<int>(32u * static_cast<unsigned>(i < sinks ? i : i + skip)); }
 };
 
 // Tiles of row b: those with one of the first `sinks` positions, then those from the window's on.
 __device__ __forceinline__ int row_tiles(const Attention& p, int len, int& sink_tiles, int& skip) {
-    const int start = window_start(p, len), all = (len + kTile - 1) / kTile;
-    sink_tiles = (min(p.sinks, start) + kTile - 1) / kTile;
+    auto tiles = [](int n) { return n / kTile + (n % kTile > 0); };  // (n + kTile - 1 may pass 32 bits)
+    const int start = window_start(p, len);
+    sink_tiles = tiles(min(p.sinks, start));
     skip = max(start / kTile, sink_tiles) - sink_tiles;
-    return all - skip;
+    return tiles(len) - skip;
 }
 
 // The runs of a CTA. With even shares, the CTA's are the tiles of weight [w0, w1) of all rows in line, where a
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
             // page and entry of this lane's stretch of tile i
             int id, at;
             auto ask = [&](int i) {
-                const int t = run.position(i) + stretch * a.box;
+                const int t = static_cast<int>(static_cast<unsigned>(run.position(i)) + static_cast<unsigned>(stretch * a.box));
                 const int c = p.table.shift >= 0 ? t >> p.table.shift : t / page;
                 at = t - c * page;
                 id = -1;

@@ -63,8 +63,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             norm = static_cast<const float*>(w.data_ptr());
         }
         const c10::cuda::CUDAGuard guard(d);
-        call(mm_paged_append(&c, values.data_ptr(), values.stride(0), kind, rows, positions, n, number(a[6]), norm,
-                             static_cast<float>(number(a[8])), stream_of(d)));
+        call(mm_paged_append(&c, values.data_ptr(), values.stride(0), kind, rows, positions, n, number(a[6], "theta"), norm,
+                             static_cast<float>(number(a[8], "eps")), stream_of(d)));
         written(a[0]);
         Py_RETURN_NONE;
     });

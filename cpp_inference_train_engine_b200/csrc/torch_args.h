@@ -84,11 +84,11 @@ int kind_of(at::ScalarType t) {
 bool half(int kind) { return kind == MM_F16 || kind == MM_BF16; }
 bool last_adjacent(const at::Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
 
-double number(PyObject* o) {
+double number(PyObject* o, const char* what = "scale") {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) {
         PyErr_Clear();
-        bad("scale must be a number");
+        bad(std::string(what) + " must be a number");
     }
     return v;
 }

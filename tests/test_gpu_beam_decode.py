@@ -94,7 +94,9 @@ def test_8_bit_pages_and_repeated_searches(name):
         replay = make(name, bits=8, beams=1, lens=(17, 1, 16))[3]
         # one beam, its tokens given: the logits along the hypothesis
         import torch
-        table, spare, lengths = replay.start
+        from cpp_inference_train_engine_b200 import paged
+        prompts_of = torch.cat([replay.prompt_rows, replay.prompt_rows])  # every beam descends from its prompt's row
+        table, spare, lengths = (t[:3] for t in paged.beam_reorder(replay.cache, *replay.start, prompts_of))
         total = float(torch.log_softmax(replay.prompt_logits[g].double(), -1)[tokens[0]])
         for i, t in enumerate(tokens[:-1]):
             step = torch.zeros(3, dtype=torch.int32, device="cuda")
@@ -104,6 +106,15 @@ def test_8_bit_pages_and_repeated_searches(name):
             total += float(torch.log_softmax(logits[g, 0].double(), -1)[tokens[i + 1]])
         # the rows of a product differ in the order of its sums by the number of rows alone
         assert abs(total - s) <= TOL[name] * len(tokens)
+
+
+@pytest.mark.parametrize("page", [4, 16, 64])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_searches_leave_the_prompts_as_they_were(page, bits):
+    """A search's beams copy over each other's last pages: the next one finds the prompts' own untouched."""
+    d = make("tiny", bits=bits, beams=5, page=page, new=20)[3]
+    first = d.search()
+    assert all(d.search() == first for _ in range(3))
 
 
 def test_windowed_search():

@@ -295,6 +295,23 @@ def test_offsets_past_32_bits():
     assert torch.equal(pool[-1, 9, :kv], values[0, :kv].bfloat16())
 
 
+@pytest.mark.parametrize("width", [(128, 16, 8), (512, 32, 16), (40, 6, 3)], ids=str)
+@pytest.mark.parametrize("window,sinks", [(50, 3), (1, 0), (33, 70)])
+def test_rows_of_2_31_positions_through_a_window(width, window, sinks):
+    """The last positions that 32 bits hold: every column of the table is one of two pages."""
+    torch, paged = mods()
+    kv, rope, H = width
+    g = torch.Generator(device="cuda").manual_seed(0)
+    pool = torch.randn(2, 16, kv + rope, generator=g, device="cuda").half()
+    table = torch.zeros(1, 2 ** 27 - 1, dtype=torch.int32, device="cuda")
+    table[0, -3:] = 1
+    q = torch.randn(1, H, kv + rope, generator=g, device="cuda").half()
+    for n in (2 ** 31 - 16, 2 ** 31 - 17, 2 ** 31 - 40):
+        at = list(range(sinks)) + list(range(n - window, n))
+        keys = torch.stack([pool[int(table[0, t // 16]), t % 16] for t in at]).double()
+        check_attention(torch, paged, q, pool, table, [n], [keys], kv, 0.1, window=window, sinks=sinks)
+
+
 # ------------------------------------------------------------------ append
 def entry_bits(torch, cache):
     return [t.view(torch.uint8).clone() for t in (cache if isinstance(cache, tuple) else (cache,))]
@@ -682,6 +699,72 @@ def test_a_step_on_another_stream_and_in_a_graph(bits):
         graph.replay()
         torch.cuda.synchronize()
         assert all(same(a, b) for a, b in zip(got, w))
+
+
+@pytest.mark.parametrize("width", [(128, 16, 8), (512, 32, 16)], ids=str)
+@pytest.mark.parametrize("fp8", [False, True])
+def test_cut_rows_in_graphs_and_on_two_streams_at_once(width, fp8):
+    """Calls whose rows are cut between blocks (partial results in a workspace of the call's own) give the same bits
+    eagerly, side by side on two streams, and from two graphs replayed in turn."""
+    torch, paged = mods()
+    kv, rope, H = width
+    g = torch.Generator(device="cuda").manual_seed(0)
+    sets = []
+    for lens in ([9000, 5, 4000], [300 * i for i in range(40)]):
+        cache, table, _ = make_pages(torch, g, lens, 32, kv, rope, torch.float16, fp8)
+        q = torch.randn(len(lens), H, kv + rope, generator=g, device="cuda").half()
+        sets.append((q, cache, table, i32(torch, lens)))
+    call = lambda s: paged.attention(*s, 0.1, kv_rank=kv, return_lse=True)  # noqa: E731
+    want = [call(s) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(call(sets[i]))
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(call(s))
+    for _ in range(3):
+        for gr in graphs:
+            gr.replay()
+    torch.cuda.synchronize()
+    for w, many, out in zip(want, got, outs):
+        for r in many + [out]:
+            assert torch.equal(w[0], r[0]) and torch.equal(w[1], r[1])
+
+
+@pytest.mark.parametrize("shape", [(1, 4, 16384), (60, 6, 3001), (2, 20, 40000)], ids=str)
+def test_beam_select_in_graphs_and_on_two_streams_at_once(shape):
+    torch, paged = mods()
+    g = torch.Generator(device="cuda").manual_seed(0)
+    sets = [(torch.randn(*shape, generator=g, device="cuda"), -torch.rand(shape[:2], generator=g, device="cuda")) for _ in range(2)]
+    want = [paged.beam_select(*s) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(paged.beam_select(*sets[i]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    x, s = sets[0][0].clone(), sets[0][1].clone()
+    with torch.cuda.graph(graph):
+        out = paged.beam_select(x, s)
+    for i in (0, 1):
+        x.copy_(sets[i][0])
+        s.copy_(sets[i][1])
+        graph.replay()
+        torch.cuda.synchronize()
+        for r in got[i] + [out]:
+            assert all(torch.equal(a, b) for a, b in zip(want[i], r))
 
 
 def test_writes_count_as_in_place():
