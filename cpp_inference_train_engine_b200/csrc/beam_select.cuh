@@ -51,18 +51,19 @@ __device__ __forceinline__ void exchange(Pair& p, int o, bool down) {
     const bool lower = (threadIdx.x & o) == 0;
     if (ahead(q, p) == (lower == down)) p = q;
 }
+// The lanes' candidates in order, the best in lane 0. A function of its own: it is called from several places, once or
+// twice a warp, and its instructions come from memory the first time.
+static __device__ __noinline__ Pair sorted(Pair q) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) exchange(q, o, (threadIdx.x & size) == 0 || size == 32);
+    return q;
+}
 // The best 32 candidates so far, rank r in lane r.
 struct Best {
     Pair p{-INFINITY, kNobody};
-    // Joins 32 more, one a lane, in any order.
-    __device__ __forceinline__ void join(Pair q) {
-#pragma unroll
-        for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-            for (int o = size >> 1; o > 0; o >>= 1) exchange(q, o, (threadIdx.x & size) == 0 || size == 32);
-        join_sorted(q);
-    }
-    // The same, from the best to the last.
+    // Joins 32 more, in order.
     __device__ __forceinline__ void join_sorted(Pair q) {
         // the better of rank r and rank 31 - r are the best 32, rising and falling once
         q = from_lane(q, 31);
@@ -74,6 +75,17 @@ struct Best {
         return {__shfl_sync(0xffffffffu, p.value, r), __shfl_sync(0xffffffffu, p.at, r)};
     }
 };
+// The k-th largest (from 1) of the lanes' values.
+__device__ __forceinline__ float kth_largest(float v, int k) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const float u = __shfl_xor_sync(0xffffffffu, v, o);
+            v = ((threadIdx.x & o) == 0) == ((threadIdx.x & size) == 0 || size == 32) ? fmaxf(u, v) : fminf(u, v);
+        }
+    return __shfl_sync(0xffffffffu, v, k - 1);
+}
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
 
@@ -189,7 +201,7 @@ __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(
     Pair last{-INFINITY, kNobody};
     auto join = [&] {
         __syncwarp();
-        best.join(lane < waiting ? wait[lane] : Pair{-INFINITY, kNobody});
+        best.join_sorted(sorted(lane < waiting ? wait[lane] : Pair{-INFINITY, kNobody}));
         const Pair l = best.rank(a.count - 1);
         if (l.at != kNobody) last = l;  // (a list that is not full keeps its floor)
         const Pair rest = wait[32 + lane];
@@ -212,6 +224,7 @@ __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * 32 + lane;
+            if (i0 >= l1) break;  // (nothing is written behind the last step)
             cp_async16(ring + (filled * U + u) * 32, reinterpret_cast<const uint4*>(x + head) + (i < l1 ? i : 0), i < l1);
         }
         cp_async_commit();
@@ -266,12 +279,10 @@ __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(
         }
         // `count` of the lanes' largest are `count` candidates: nothing below the least of them enters
         {
-            Best all;
-            all.join({most, lane});
-            const float floor = all.rank(a.count - 1).value;
+            const float floor = kth_largest(most, a.count);
             if (floor > last.value) last = {floor, kNobody};
         }
-        // the steps and lanes that reach it, in line; their values from the cache, kAtOnce pairs' at a time
+        // the steps and lanes that reach it, in line; their values from the ring or the cache, kAtOnce pairs' at a time
         int pairs = 0;
 #pragma unroll
         for (int st = 0; st < kSteps; ++st) {
@@ -281,6 +292,7 @@ __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(
             pairs += __popc(who);
         }
         __syncwarp();
+        const bool held = l1 - l0 <= 32 * U * kStages;  // in the ring: no step has been overwritten
         constexpr int kSide = 32 / (U * E), kAtOnce = 4 * kSide;  // pairs side by side in a warp: 2 for 16 values
         const int place = lane % (U * E);
         for (int j0 = 0; j0 < pairs; j0 += kAtOnce) {
@@ -291,7 +303,9 @@ __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(
                 const int pair = j0 + j * kSide + lane / (U * E), code = pair < pairs ? pairs_s[warp][pair] : 0;
                 const int i = base + (code >> 5) * 32 * U + place / E * 32 + (code & 31);
                 t[j] = head + i * E + place % E;
-                v[j] = pair < pairs && i < l1 ? lat::to_f32(x[t[j]]) : -INFINITY;
+                const T* from = held ? reinterpret_cast<const T*>(ring_s + ((warp * kStages + (code >> 5)) * U + place / E) * 32 + (code & 31)) + place % E
+                                     : x + t[j];
+                v[j] = pair < pairs && i < l1 ? lat::to_f32(*from) : -INFINITY;
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) offer(v[j], t[j]);
