@@ -1,6 +1,6 @@
 // Beam search's selection over beams and vocabulary (mm_beam_select).
 //
-// One pass over the logits: a block takes a part of a beam's tokens, each of its warps an eighth, and keeps their
+// One pass over the logits: a block takes a part of a beam's tokens, its warps divide them, and keeps their
 // maximum, the sum of exponentials below it and the best 32 of them (rank r in lane r); then the parts of a beam are
 // joined, and the beams. The pass itself keeps one maximum per lane and step: of the 32 lanes' maxima over a
 // stretch of steps the count-th largest bounds the list from below, so that only the few (lane, step) pairs that
@@ -18,7 +18,6 @@ constexpr int kMaxBeams = 32;
 constexpr int kMaxVocab = 1 << 20;  // flat candidates k * vocab + v stay below 2^25
 constexpr float kLowest = -3.402823466e38f;
 constexpr int kMaxParts = 32;       // of a beam's tokens, a block each
-constexpr int kWarps = 8;           // of such a block
 constexpr int kMaxCluster = 16;
 
 // Candidates in order: by value, then by the lower index. Nobody: (-infinity, kNobody).
@@ -172,8 +171,8 @@ __device__ __forceinline__ unsigned long long load_cluster64(uint32_t cluster_ad
 // aligned load are taken one a lane. Loads stand in shared memory two steps ahead, where the lane that asked for
 // them takes them itself.
 constexpr int kLoads = 4, kStages = 3;
-constexpr int kRing = kWarps * kStages * kLoads * 32 * 16;  // 48 KB: four blocks an SM
-template <typename T, bool CLUSTER>
+constexpr int ring_bytes(int warps) { return warps * kStages * kLoads * 32 * 16; }  // 192 KB an SM
+template <typename T, int kWarps, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(const Select a) {
     MM_PDL_ENTRY();
     constexpr int E = 16 / sizeof(T), U = kLoads, kSteps = 8;  // values per load, loads per step, steps per stretch

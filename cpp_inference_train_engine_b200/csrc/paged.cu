@@ -191,24 +191,28 @@ void check_select(int batch, int beams, int vocab, int count) {
     if (vocab > mm::beam::kMaxVocab) refuse(MM_UNSUPPORTED, "beam selection: vocabulary over 1,048,576");
 }
 
-// How a selection is launched: parts of a beam's tokens, a block of eight warps each, as many as fill the
-// multiprocessors with 32 warps, of 4,096 tokens or more. In clusters where a batch entry's blocks can be one, none
-// has more than 32,768 tokens then and there are few: us in clusters / with a second kernel, 1 x 4 beams of 16,384
-// 8.7 / 11.6, 4 x 16 of 32,768 13.6 / 17.7, 16 x 8 (128 blocks) 17.5 / 17.0, 64 x 8 (512) 25.0 / 23.5.
+// How a selection is launched: parts of a beam's tokens, a block each, as many as fill the multiprocessors with 32
+// warps, of 4,096 tokens or more. Blocks have eight warps, where there are many beams fewer, whose lists have to be joined:
+// us with 8 / 4 / 2, 400 beams of 50,000 26.7 / 28.2 / 36.3, 512 of 32,768 23.2 / 21.0 / 26.4, 1,800 of 20,000 (fp16) 46.3 /
+// 34.7 / 40.3, 1,000 of 4,000 20.5 / 15.6 / 12.8.
+// In clusters where a batch entry's blocks can be one, none has more than 32,768 tokens then and there are few: us in
+// clusters / with a second kernel, 1 x 4 beams of 16,384 8.7 / 11.6, 4 x 16 of 32,768 13.6 / 17.7, 16 x 8 (128 blocks)
+// 17.5 / 17.0, 64 x 8 (512) 25.0 / 23.5.
 struct SelectPlan {
-    int parts;
+    int parts, warps;
     bool cluster;
     int64_t bytes;
 };
 SelectPlan select_plan(int batch, int beams, int vocab) {
     const int64_t rows = std::max<int64_t>(1, static_cast<int64_t>(batch) * beams), most = std::min((vocab + 4095) / 4096, mm::beam::kMaxParts);
-    SelectPlan r{static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 4 * sm_count() / rows))), false, 0};
+    SelectPlan r{static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 4 * sm_count() / rows))), 8, false, 0};
     const int fits = mm::beam::kMaxCluster / beams;
     const int parts = std::min(fits, r.parts);
     if (parts > 0 && (vocab + parts - 1) / parts <= 32768 && rows * parts <= sm_count() / 2) {
         r.parts = parts;
         r.cluster = true;
     } else {
+        if (rows >= 3 * sm_count()) r.warps = vocab <= 8192 ? 2 : 4;
         r.bytes = static_cast<int64_t>(batch) * beams * r.parts * (32 * sizeof(mm::beam::Pair) + sizeof(float2));
     }
     return r;
@@ -218,14 +222,21 @@ template <typename T> void launch_select(const mm::beam::Select& a, const Select
     using namespace mm::beam;
     const unsigned grid = blocks(static_cast<long long>(a.batch) * a.beams * r.parts, 1);
     if (!r.cluster) {
-        set_dynamic_smem<select_parts_kernel<T, false>>(kRing);
-        launch(s, select_parts_kernel<T, false>, dim3(grid), dim3(32 * kWarps), kRing, a);
+        auto parts = [&](auto n) {
+            constexpr int W = decltype(n)::value;
+            set_dynamic_smem<select_parts_kernel<T, W, false>>(ring_bytes(W));
+            launch(s, select_parts_kernel<T, W, false>, dim3(grid), dim3(32 * W), ring_bytes(W), a);
+        };
+        if (r.warps == 8) parts(std::integral_constant<int, 8>{});
+        else if (r.warps == 4) parts(std::integral_constant<int, 4>{});
+        else parts(std::integral_constant<int, 2>{});
         launch(s, select_join_kernel, dim3(a.batch), dim3(32 * a.beams), 512 * a.beams, a);
         return;
     }
+    constexpr int kWarps = 8, kRing = ring_bytes(kWarps);
     static_assert(512 * kWarps <= kRing, "the join's scratch");
-    set_dynamic_smem<select_parts_kernel<T, true>>(kRing);
-    check(cudaFuncSetAttribute(select_parts_kernel<T, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cluster size");
+    set_dynamic_smem<select_parts_kernel<T, kWarps, true>>(kRing);
+    check(cudaFuncSetAttribute(select_parts_kernel<T, kWarps, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cluster size");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(32 * kWarps);
@@ -239,7 +250,7 @@ template <typename T> void launch_select(const mm::beam::Select& a, const Select
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    check(cudaLaunchKernelEx(&cfg, select_parts_kernel<T, true>, a), "kernel launch");
+    check(cudaLaunchKernelEx(&cfg, select_parts_kernel<T, kWarps, true>, a), "kernel launch");
 }
 
 }  // namespace
