@@ -953,8 +953,8 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
 }
 
 // Joins the parts of the units that were cut. Block (entry of the cut list, y) of 8 warps. Up to kFew parts: a warp
-// takes a head, eight 16-byte loads a lane at a time; more: the warps of a block divide the parts of 128 columns of
-// a head.
+// takes NG times 128 columns of a head, eight 16-byte loads a lane at a time; more: the warps of a block divide the
+// parts of 128 columns of a head.
 constexpr int kFew = 8;
 struct Mean {  // a weighted mean in the making: maximum and sum of the weights
     float m = kNone, l = 0.f;
@@ -969,10 +969,10 @@ struct Mean {  // a weighted mean in the making: maximum and sum of the weights
 __device__ __forceinline__ void blend(float4& o, float4 v, float2 f) {
     o = make_float4(fmaf(v.x, f.y, o.x * f.x), fmaf(v.y, f.y, o.y * f.x), fmaf(v.z, f.y, o.z * f.x), fmaf(v.w, f.y, o.w * f.x));
 }
-template <int KV, typename T>
+template <int KV, int NG, typename T>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ MmaArgs a) {
     MM_PDL_ENTRY();
-    constexpr int NS = KV / 128, PER = 8 / NS;
+    constexpr int NS = KV / 128, PER = 8 / NG;
     __shared__ float4 sum_s[8][32];
     __shared__ float2 ml_s[8];
     const int4 cut = __ldcg(&a.cut[blockIdx.x]);
@@ -990,13 +990,14 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
         if (p.lse && c == 0) p.lse[first + h] = sum.l == 0.f ? -INFINITY : (sum.m + log2f(sum.l)) * 0.6931471805599453f;
     };
     if (parts <= kFew) {
-        for (int h = blockIdx.y * 8 + warp; h < heads; h += gridDim.y * 8) {
+        for (int task = blockIdx.y * 8 + warp; task < heads * (NS / NG); task += gridDim.y * 8) {
+            const int h = task / (NS / NG), c = (task - h * (NS / NG)) * NG * 128 + lane * 4;
             Mean sum;
-            float4 o[NS];
+            float4 o[NG];
 #pragma unroll
-            for (int x = 0; x < NS; ++x) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int x = 0; x < NG; ++x) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int i0 = 0; i0 < parts; i0 += PER) {
-                float4 v[PER][NS];
+                float4 v[PER][NG];
                 float2 ml[PER];
 #pragma unroll
                 for (int k = 0; k < PER; ++k) {
@@ -1004,19 +1005,19 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
                     const int at = slot(i0 + k) * 16 + h;
                     ml[k] = __ldcg(&a.part_ml[at]);
 #pragma unroll
-                    for (int x = 0; x < NS; ++x)
-                        v[k][x] = __ldcg(reinterpret_cast<const float4*>(a.part_o + static_cast<long long>(at) * KV + x * 128) + lane);
+                    for (int x = 0; x < NG; ++x)
+                        v[k][x] = __ldcg(reinterpret_cast<const float4*>(a.part_o + static_cast<long long>(at) * KV + c + x * 128));
                 }
 #pragma unroll
                 for (int k = 0; k < PER; ++k) {
                     if (i0 + k >= parts) continue;
                     const float2 f = sum.add(ml[k]);
 #pragma unroll
-                    for (int x = 0; x < NS; ++x) blend(o[x], v[k][x], f);
+                    for (int x = 0; x < NG; ++x) blend(o[x], v[k][x], f);
                 }
             }
 #pragma unroll
-            for (int x = 0; x < NS; ++x) finish(h, x * 128 + lane * 4, o[x], sum);
+            for (int x = 0; x < NG; ++x) finish(h, c + x * 128, o[x], sum);
         }
         return;
     }
