@@ -171,12 +171,19 @@ __device__ __forceinline__ unsigned long long load_cluster64(uint32_t cluster_ad
     return v;
 }
 
-// Block (part, beam row). E values of 16 bytes a load; a row's first and last tokens that are not in a whole
-// aligned load are taken one a lane. Loads stand in shared memory two steps ahead, where the lane that asked for
-// them takes them itself.
+// `n` bytes (0 to 16) of a 16-byte piece, the others as zeros.
+__device__ __forceinline__ void copy_piece(void* dst, const void* src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(n) : "memory");
+}
+
+// Block (part, beam row). A load is E values, counted from the row's first token, so that equal rows have equal sums
+// wherever they stand (a beam's continuations tie with those of an equal one). The memory comes in aligned pieces of
+// 16 bytes, two steps ahead, through shared memory; of a row that begins inside a piece (by `shift` values) a load is the
+// end of one piece and the beginning of the next.
 constexpr int kLoads = 4, kStages = 3;
-constexpr int ring_bytes(int warps) { return warps * kStages * kLoads * 32 * 16; }  // 192 KB an SM
-template <typename T, int kWarps, bool CLUSTER>
+constexpr int kPieces = kStages * kLoads * 33;  // a warp's: each 32 loads and one piece more
+constexpr int ring_bytes(int warps) { return warps * kPieces * 16; }  // 198 KB an SM
+template <typename T, int kWarps, bool CLUSTER, bool SHIFTED>
 __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(const Select a) {
     MM_PDL_ENTRY();
     constexpr int E = 16 / sizeof(T), U = kLoads, kSteps = 8;  // values per load, loads per step, steps per stretch
@@ -192,9 +199,9 @@ __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(
     const bool dead = !finite(__ldg(a.scores + row)) || (a.finished && a.finished[row]);
     if (!CLUSTER && dead) return;  // the join does not use it either
     const T* x = static_cast<const T*>(a.logits) + b * a.batch_stride + (row - b * a.beams) * a.beam_stride;
-    // whole loads begin at token `head`, which is where the address is a multiple of 16
-    const int head = min(a.vocab, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
-    const int loads = dead ? 0 : (a.vocab - head) / E;
+    const int shift = SHIFTED ? static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)) : 0;
+    const uint8_t* pieces = reinterpret_cast<const uint8_t*>(x - shift);
+    const int loads = dead ? 0 : (a.vocab + E - 1) / E;
     const int per = (loads + kWarps * a.parts - 1) / (kWarps * a.parts), l0 = min((part * kWarps + warp) * per, loads), l1 = min(l0 + per, loads);
     // Candidates wait in shared memory until there are 32 (or no more): joining the list costs a sort. What is
     // behind the list's last entry does not wait.
@@ -221,17 +228,54 @@ __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(
     };
     constexpr float kLog2e = 1.4426950408889634f;
     float m = kLowest, s = 0.f;  // (a finite maximum of nothing: differences from it are no NaN)
-    uint4* ring = ring_s + warp * (kStages * U * 32) + lane;
+    uint4* ring = ring_s + warp * kPieces + lane;
     int stage = 0, filled = 0;
+    auto bring = [&](uint4* dst, int piece) {
+        const int n = (a.vocab + shift - piece * E) * static_cast<int>(sizeof(T));  // up to the row's end
+        if (SHIFTED && piece == 0) {  // what is before the row is not read
+            for (int e = shift; e < min(E, a.vocab + shift); ++e) reinterpret_cast<T*>(dst)[e] = x[e - shift];
+        } else if (n > 0) {
+            copy_piece(dst, pieces + static_cast<long long>(piece) * 16, min(n, 16));
+        }
+    };
     auto fetch = [&](int i0) {
+        uint4* to = ring + filled * U * 33;
+        const int i = i0 + lane;
+        if (i0 + U * 32 <= l1 && (i0 + U * 32 + 1) * E <= a.vocab && (!SHIFTED || i0 > 0)) {  // whole pieces all
+            const uint8_t* from = pieces + static_cast<long long>(i) * 16;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * 32 + lane;
-            if (i0 >= l1) break;  // (nothing is written behind the last step)
-            cp_async16(ring + (filled * U + u) * 32, reinterpret_cast<const uint4*>(x + head) + (i < l1 ? i : 0), i < l1);
+            for (int u = 0; u < U; ++u) {
+                cp_async16(to + u * 33, from + u * 512, true);
+                if (SHIFTED && lane == 0) cp_async16(to + u * 33 + 32, from + u * 512 + 512, true);
+            }
+        } else if (i0 < l1) {  // (nothing is written behind the last step)
+#pragma unroll 1
+            for (int u = 0; u < U; ++u) {
+                if (i + u * 32 < l1 + (SHIFTED ? 1 : 0)) bring(to + u * 33, i + u * 32);
+                if (SHIFTED && lane == 0 && i + u * 32 + 32 <= l1) bring(to + u * 33 + 32, i + u * 32 + 32);
+            }
         }
         cp_async_commit();
         filled = filled == kStages - 1 ? 0 : filled + 1;
+    };
+    // The load in pieces p[0] and p[1], as 32-bit words.
+    auto words = [&](const uint4* p, uint32_t (&w)[4]) {
+        const uint4 first = p[0];
+        w[0] = first.x;
+        w[1] = first.y;
+        w[2] = first.z;
+        w[3] = first.w;
+        if constexpr (SHIFTED) {
+            const uint4 second = p[1];
+            uint32_t v[8] = {w[0], w[1], w[2], w[3], second.x, second.y, second.z, second.w};
+            const int whole = shift * static_cast<int>(sizeof(T)) / 4;
+#pragma unroll
+            for (int j = 0; j < 7; ++j) v[j] = whole & 1 ? v[j + 1] : v[j];
+#pragma unroll
+            for (int j = 0; j < 5; ++j) v[j] = whole & 2 ? v[j + 2] : v[j];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = sizeof(T) == 2 && (shift & 1) ? __funnelshift_r(v[j], v[j + 1], 16) : v[j];
+        }
     };
     fetch(l0);
     fetch(l0 + 32 * U);
@@ -244,20 +288,22 @@ __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(
             if (i0 >= l1) continue;
             float v[U][E];
             cp_async_wait<kStages - 2>();
+            if constexpr (SHIFTED) __syncwarp();  // (a lane's second piece is its neighbour's first)
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const uint4 raw = ring[(stage * U + u) * 32];
+                uint32_t raw[4];
+                words(ring + (stage * U + u) * 33, raw);
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[u][e] = lat::to_f32(reinterpret_cast<const T*>(&raw)[e]);
+                for (int e = 0; e < E; ++e) v[u][e] = lat::to_f32(reinterpret_cast<const T*>(raw)[e]);
             }
             stage = stage == kStages - 1 ? 0 : stage + 1;
-            if (i0 + 32 * U > l1) {
+            if (i0 + 32 * U > l1 || (i0 + 32 * U) * E > a.vocab) {
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (i0 + u * 32 + lane >= l1) {
+                for (int u = 0; u < U; ++u) {
+                    const int i = i0 + u * 32 + lane, n = i < l1 ? a.vocab - i * E : 0;  // values of the load
 #pragma unroll
-                        for (int e = 0; e < E; ++e) v[u][e] = -INFINITY;
-                    }
+                    for (int e = 0; e < E; ++e) v[u][e] = e < n ? v[u][e] : -INFINITY;
+                }
             }
             fetch(i0 + 2 * 32 * U);
 #pragma unroll
@@ -305,10 +351,10 @@ __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(
             for (int j = 0; j < 4; ++j) {
                 const int pair = j0 + j * kSide + lane / (U * E), code = pair < pairs ? pairs_s[warp][pair] : 0;
                 const int i = base + (code >> 5) * 32 * U + place / E * 32 + (code & 31);
-                t[j] = head + i * E + place % E;
-                const T* from = held ? reinterpret_cast<const T*>(ring_s + ((warp * kStages + (code >> 5)) * U + place / E) * 32 + (code & 31)) + place % E
+                t[j] = i * E + place % E;
+                const T* from = held ? reinterpret_cast<const T*>(ring_s + warp * kPieces + ((code >> 5) * U + place / E) * 33 + (code & 31)) + shift + place % E
                                      : x + t[j];
-                v[j] = pair < pairs && i < l1 ? lat::to_f32(*from) : -INFINITY;
+                v[j] = pair < pairs && i < l1 && t[j] < a.vocab ? lat::to_f32(*from) : -INFINITY;
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) offer(v[j], t[j]);
@@ -316,15 +362,6 @@ __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) select_parts_kernel(
         __syncwarp();
     }
     cp_async_wait<0>();
-    if (part == 0 && warp == 0 && !dead) {  // the ends, at most 2 (E - 1) <= 14 tokens
-        const int tail = head + loads * E;
-        const int t = lane < head ? lane : tail + lane - head;
-        const float v = t < a.vocab ? lat::to_f32(x[t]) : -INFINITY;
-        const float mn = fmaxf(m, v);
-        s = s * fast_exp2((m - mn) * kLog2e) + fast_exp2((v - mn) * kLog2e);
-        m = mn;
-        offer(v, t);
-    }
     join();
     // the lanes' sums below one maximum (a NaN or +infinity anywhere makes the sum a NaN), then the warps'
     auto scaled = [&](float2 v, float top) { return v.y * fast_exp2((v.x - top) * kLog2e); };

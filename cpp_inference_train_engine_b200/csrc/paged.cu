@@ -227,14 +227,14 @@ SelectPlan select_plan(int batch, int beams, int vocab) {
     return r;
 }
 
-template <typename T> void launch_select(const mm::beam::Select& a, const SelectPlan& r, cudaStream_t s) {
+template <typename T, bool SHIFTED> void launch_select(const mm::beam::Select& a, const SelectPlan& r, cudaStream_t s) {
     using namespace mm::beam;
     const unsigned grid = blocks(static_cast<long long>(a.batch) * a.beams * r.parts, 1);
     if (!r.cluster) {
         auto parts = [&](auto n) {
             constexpr int W = decltype(n)::value;
-            set_dynamic_smem<select_parts_kernel<T, W, false>>(ring_bytes(W));
-            launch(s, select_parts_kernel<T, W, false>, dim3(grid), dim3(32 * W), ring_bytes(W), a);
+            set_dynamic_smem<select_parts_kernel<T, W, false, SHIFTED>>(ring_bytes(W));
+            launch(s, select_parts_kernel<T, W, false, SHIFTED>, dim3(grid), dim3(32 * W), ring_bytes(W), a);
         };
         if (r.warps == 8) parts(std::integral_constant<int, 8>{});
         else if (r.warps == 4) parts(std::integral_constant<int, 4>{});
@@ -244,8 +244,9 @@ template <typename T> void launch_select(const mm::beam::Select& a, const Select
     }
     constexpr int kWarps = 8, kRing = ring_bytes(kWarps);
     static_assert(512 * kWarps <= kRing, "the join's scratch");
-    set_dynamic_smem<select_parts_kernel<T, kWarps, true>>(kRing);
-    check(cudaFuncSetAttribute(select_parts_kernel<T, kWarps, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cluster size");
+    constexpr auto kernel = select_parts_kernel<T, kWarps, true, SHIFTED>;
+    set_dynamic_smem<kernel>(kRing);
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cluster size");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(32 * kWarps);
@@ -259,7 +260,7 @@ template <typename T> void launch_select(const mm::beam::Select& a, const Select
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    check(cudaLaunchKernelEx(&cfg, select_parts_kernel<T, kWarps, true>, a), "kernel launch");
+    check(cudaLaunchKernelEx(&cfg, kernel, a), "kernel launch");
 }
 
 }  // namespace
@@ -392,7 +393,13 @@ int mm_beam_select(const void* logits, int64_t batch_stride, int64_t beam_stride
         const mm::beam::Select a{logits, batch_stride, beam_stride, scores, finished, eos, batch, beams, vocab, count, r.parts,
                                  out_scores, out_parents, out_tokens, best,
                                  reinterpret_cast<float2*>(best + static_cast<int64_t>(batch) * beams * r.parts * 32)};
-        with_type(dtype, [&](auto t) { launch_select<typename decltype(t)::type>(a, r, static_cast<cudaStream_t>(stream)); });
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        with_type(dtype, [&](auto t) {
+            using T = typename decltype(t)::type;
+            const int64_t e = 16 / sizeof(T);  // whether every row begins at a multiple of 16 bytes
+            if (multiple(logits, 16) && batch_stride % e == 0 && beam_stride % e == 0) launch_select<T, false>(a, r, s);
+            else launch_select<T, true>(a, r, s);
+        });
     });
 }
 

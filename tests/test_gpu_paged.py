@@ -421,9 +421,10 @@ def test_far_positions_keep_their_angle():
 
 
 # ------------------------------------------------------------------ beam selection
-def select_reference(torch, x, scores, count, finished, eos):
+def select_reference(torch, x, scores, count, finished, eos, equal=False):
     B, K, V = x.shape
-    lse = torch.logsumexp(x.double(), -1, keepdim=True)
+    # (of equal beams once: a sum's rounding may depend on where a row begins)
+    lse = torch.logsumexp(x[:, :1 if equal else K].double(), -1, keepdim=True)
     cand = scores.double()[..., None] + (x.double() - lse)
     live = torch.isfinite(scores)[..., None]
     if finished is not None:
@@ -440,9 +441,9 @@ def select_reference(torch, x, scores, count, finished, eos):
     return best, torch.where(none, slot, at // V).int(), torch.where(none, -1, at % V).int()
 
 
-def check_select(torch, paged, x, scores, count=None, finished=None, eos=None):
+def check_select(torch, paged, x, scores, count=None, finished=None, eos=None, equal=False):
     got = paged.beam_select(x, scores, beams=count, finished=finished, eos=eos)
-    want = select_reference(torch, x, scores, count or x.shape[1], finished, eos)
+    want = select_reference(torch, x, scores, count or x.shape[1], finished, eos, equal)
     assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
     fine = torch.isfinite(want[0])
     assert torch.equal(torch.isfinite(got[0]), fine) and torch.all(got[0][~fine] == float("-inf"))
@@ -483,6 +484,19 @@ def test_beam_select_takes_the_lowest_of_equal_candidates():
         x[:, :, V - 1] = 1.0
         check_select(torch, paged, x, s, count=7)
         check_select(torch, paged, x.half(), s, count=32)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("shape", [(3, 4, 257), (2, 8, 1003), (1, 7, 50001), (70, 8, 3001), (1, 3, 16387)], ids=str)
+def test_equal_beams_tie(shape, dtype):
+    """Beams with the same logits and scores have the same candidates, wherever their rows begin: the lowest beam's
+    come first, each token as often as there are beams."""
+    torch, paged = mods()
+    B, K, V = shape
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = (2 * torch.randn(B, 1, V, generator=g, device="cuda")).to(getattr(torch, dtype)).expand(B, K, V).contiguous()
+    s = torch.full((B, K), -3.25, device="cuda")
+    check_select(torch, paged, x, s, count=min(32, 2 * K + 1), equal=True)
 
 
 def test_beam_select_of_dead_beams_and_banned_tokens():
