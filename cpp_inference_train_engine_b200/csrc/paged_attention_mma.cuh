@@ -349,8 +349,25 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
         int slot = 0, q = 0;
         uint32_t phase = 0, q_phase = 0;  // parity of the round in this group's ring, in the queue
         int cut;
+        // page and entry of this lane's stretch of tile i
+        int id = -1, at = 0;
+        auto ask = [&](int i) {
+            const int t = static_cast<int>(static_cast<unsigned>(run.position(i)) + static_cast<unsigned>(stretch * a.box));
+            const int c = p.table.shift >= 0 ? t >> p.table.shift : t / page;
+            at = t - c * page;
+            id = -1;
+            if (loads && i < run.to && t < run.len) id = __ldg(p.table.entry + run.row * p.table.stride + c);
+        };
         while (ok) {
             const bool more = runs.next(run, cut);
+            if (more) {
+                ask(run.from + group);
+                // its queries, for the warps of the products
+                constexpr int kLines = ((KV + R) * 2 + 127) / 128;
+                const T* heads = static_cast<const T*>(p.q) + run.row * p.q_row + run.h0 * p.q_head;
+                const int n = min(16, p.H - run.h0) * kLines;
+                for (int e = lane; e < n; e += 32) prefetch_l1(heads + e / kLines * p.q_head + min(e % kLines * 64, KV + R - 1));
+            }
             wait(&run_empty[q], q_phase ^ 1);
             if (lane == 0) {
                 if (!more) run.row = -1;
@@ -366,22 +383,6 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 q_phase ^= 1;
             }
             if (!more) break;
-            {  // its queries, for the warps of the products
-                constexpr int kLines = ((KV + R) * 2 + 127) / 128;
-                const T* heads = static_cast<const T*>(p.q) + run.row * p.q_row + run.h0 * p.q_head;
-                const int n = min(16, p.H - run.h0) * kLines;
-                for (int e = lane; e < n; e += 32) prefetch_l1(heads + e / kLines * p.q_head + min(e % kLines * 64, KV + R - 1));
-            }
-            // page and entry of this lane's stretch of tile i
-            int id, at;
-            auto ask = [&](int i) {
-                const int t = static_cast<int>(static_cast<unsigned>(run.position(i)) + static_cast<unsigned>(stretch * a.box));
-                const int c = p.table.shift >= 0 ? t >> p.table.shift : t / page;
-                at = t - c * page;
-                id = -1;
-                if (loads && i < run.to && t < run.len) id = __ldg(p.table.entry + run.row * p.table.stride + c);
-            };
-            ask(run.from + group);
             const int start = window_start(p, run.len), sinks = min(p.sinks, start);
             for (int i = run.from + group; i - group < run.to; i += C::KG) {
                 // a page outside the pool (or behind the row) is asked for behind the last one: zeros
