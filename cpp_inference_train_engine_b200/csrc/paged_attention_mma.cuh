@@ -671,20 +671,23 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     __syncwarp();
                 }
                 if constexpr (!Q8) {
+                    // (16 positions after the other 16: a product follows the one that it adds to by 15 others)
                     const uint32_t box = sp + o_at;
                     uint32_t b[2][2][4];
-                    auto load = [&](int c, uint32_t (&d)[2][4]) {
+                    auto load = [&](int j, uint32_t (&d)[2][4]) {
+                        const int k = j >> 2, c = (j & 3) * 2;
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) ldsm4_t(d[k], (box ^ ((c & 3) * 32)) + (c >> 2) * (kTile * 128) + k * 2048);
+                        for (int x = 0; x < 2; ++x) ldsm4_t(d[x], (box ^ (((c + x) & 3) * 32)) + (c >> 2) * (kTile * 128) + k * 2048);
                     };
                     load(0, b[0]);
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        if (c < 7) load(c + 1, b[(c + 1) & 1]);
+                    for (int j = 0; j < 8; ++j) {
+                        const int k = j >> 2, c = (j & 3) * 2;
+                        if (j < 7) load(j + 1, b[(j + 1) & 1]);
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            mma16<T>(o[2 * c], w[k], b[c & 1][k][0], b[c & 1][k][1]);
-                            mma16<T>(o[2 * c + 1], w[k], b[c & 1][k][2], b[c & 1][k][3]);
+                        for (int x = 0; x < 2; ++x) {
+                            mma16<T>(o[2 * (c + x)], w[k], b[j & 1][x][0], b[j & 1][x][1]);
+                            mma16<T>(o[2 * (c + x) + 1], w[k], b[j & 1][x][2], b[j & 1][x][3]);
                         }
                     }
                 } else {
