@@ -344,11 +344,12 @@ int mm_paged_attention(const mm_paged_attention_desc* desc, const mm_paged_cache
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         const bool q8 = cache->pool.kind == MM_E4M3;
         PoolMaps maps;
-        if (mma_form(p, cache->pool) && pool_maps(maps, cache->pool, cache->pool.positions % 32 == 0 ? 32 : 16)) {
-            const MmaPlan r = mma_plan(p);
-            const int64_t need = r.bytes(p.kv);
-            require(need == 0 || (workspace && multiple(workspace, 16) && workspace_bytes >= static_cast<size_t>(need)),
-                    "paged attention: workspace too small or not 16-byte aligned");
+        const bool mma = mma_form(p, cache->pool);
+        const MmaPlan r = mma ? mma_plan(p) : MmaPlan{};
+        const int64_t need = r.bytes(p.kv);  // also of a pool whose strides the encoder turns out not to take
+        require(need == 0 || (workspace && multiple(workspace, 16) && workspace_bytes >= static_cast<size_t>(need)),
+                "paged attention: workspace too small or not 16-byte aligned");
+        if (mma && pool_maps(maps, cache->pool, cache->pool.positions % 32 == 0 ? 32 : 16)) {
             with_half(desc->dtype, [&](auto half) {
                 using T = typename decltype(half)::type;
                 if (p.kv == 128) q8 ? run_mma<128, 16, T, true>(p, r, maps, workspace, s) : run_mma<128, 16, T, false>(p, r, maps, workspace, s);

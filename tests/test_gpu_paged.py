@@ -790,3 +790,96 @@ def test_writes_count_as_in_place():
     version = cache._version
     paged.beam_reorder(cache, i32(torch, [[0]]), i32(torch, [1]), i32(torch, [3]), i32(torch, [0]))
     assert cache._version > version
+
+
+# ------------------------------------------------------------------ refusals
+# Every pointer is a tensor's and every entry of a table, length or parent is 0, so that a call that were not refused
+# would stay in bounds.
+@pytest.mark.parametrize("kv, rope", [(128, 16), (512, 32)])
+@pytest.mark.parametrize("page_stride", [None, 1 << 45])  # one page: of no meaning, but one that no tensor map takes
+def test_attention_wants_the_workspace_that_it_reports(kv, rope, page_stride):
+    torch, paged = mods()
+    from tests.test_paged_cpu import CACHE, F16, TABLE, desc, entries, message
+    L, w, page, columns = entries(), kv + rope, 64, 1000
+    pool, q = (torch.zeros(*s, dtype=torch.float16, device="cuda") for s in ((1, page, w), (2, 8, w)))
+    out, table, lengths = torch.zeros(2, 8, kv, dtype=torch.float16, device="cuda"), i32(torch, [[0] * columns] * 2), i32(torch, [0, 0])
+    p = pool.data_ptr()
+    c = CACHE.pack(p, p, p, page_stride or page * w, w, page * rope, rope, page, 1, page, kv, rope, F16, F16) + \
+        TABLE.pack(table.data_ptr(), columns, 2, columns)
+    d = desc(q=q.data_ptr(), q_row=8 * w, q_head=w, lengths=lengths.data_ptr(), max_length=columns * page, out=out.data_ptr())
+    need = L.mm_paged_attention_workspace(d, c)
+    assert need > 0
+    room = torch.zeros(need + 16, dtype=torch.uint8, device="cuda")
+    for work, n in ((room.data_ptr(), need - 1), (room.data_ptr(), 0), (room.data_ptr() + 8, need)):
+        assert L.mm_paged_attention(d, c, work, n, None) == 1 and "workspace" in message()
+    torch.cuda.synchronize()
+    assert L.mm_paged_attention(d, c, room.data_ptr(), need, None) == 0
+    torch.cuda.synchronize()
+    assert not out.any()
+
+
+def test_beam_select_wants_the_workspace_that_it_reports():
+    torch, paged = mods()
+    from tests.test_paged_cpu import F32, entries, message
+    L, B, K, V = entries(), 200, 4, 30000
+    x, s = torch.zeros(B, K, V, device="cuda"), torch.zeros(B, K, device="cuda")
+    out = [torch.zeros(B, K, dtype=torch.int32, device="cuda") for _ in range(3)]
+    need = L.mm_beam_select_workspace(B, K, V, K)
+    assert need > 0
+    room = torch.zeros(need + 16, dtype=torch.uint8, device="cuda")
+    for work, n in ((room.data_ptr(), need - 1), (room.data_ptr(), 0), (room.data_ptr() + 8, need)):
+        rc = L.mm_beam_select(x.data_ptr(), K * V, V, F32, s.data_ptr(), None, 0, B, K, V, K, *(t.data_ptr() for t in out), work, n, None)
+        assert rc == 1 and "workspace" in message()
+    torch.cuda.synchronize()
+
+
+def attention_refusals(torch, paged, d):
+    pool = paged.alloc_pages(2, 4, 16, 128, 16, device=d)
+    q = torch.zeros(2, 8, 144, dtype=torch.float16, device=d)
+    table, ints = torch.zeros(2, 3, dtype=torch.int32, device=d), torch.zeros(2, dtype=torch.int32, device=d)
+    att = lambda *a, **k: paged.attention(*a, **{"kv_rank": 128, **k})  # noqa: E731
+    return [
+        (lambda: att(q[0], pool[0], table, ints, 0.1), "q is"), (lambda: att(q.float(), pool[0], table, ints, 0.1), "q is"),
+        (lambda: att(q.bfloat16(), pool[0], table, ints, 0.1), "type"), (lambda: att(q, pool, table, ints, 0.1), "16-bit cache"),
+        (lambda: att(q, pool[0], table.long(), ints, 0.1), "table"), (lambda: att(q, pool[0], table[:1], ints, 0.1), "table row"),
+        (lambda: att(q, pool[0], table, ints[:1], 0.1), "lengths"), (lambda: att(q, pool[0], table, ints.long(), 0.1), "lengths"),
+        (lambda: att(q, pool[0], table, ints, None), "scale"), (lambda: att(q, pool[0], table, ints, 0.1, kv_rank=0), "kv_rank"),
+        (lambda: att(q, pool[0], table, ints, 0.1, kv_rank=145), "kv_rank"), (lambda: att(q, pool[0], table, ints, 0.1, window=0), "window"),
+        (lambda: att(q, pool[0], table, ints, 0.1, window=-3), "window"), (lambda: att(q, pool[0], table, ints, 0.1, sinks=-1), "sinks"),
+        (lambda: att(q, pool[0], table, ints, 0.1, max_length=49), "max_length"), (lambda: att(q[..., :140], pool[0], table, ints, 0.1), "width"),
+        (lambda: paged.append(pool[0], q[:, 0, :100], table, ints, kv_rank=128), "values"),
+        (lambda: paged.append(pool[0], q[:, 0], table, ints[:1], kv_rank=128), "positions"),
+        (lambda: paged.append(pool[0], q[:1, 0], table, ints[:1], kv_rank=128), "per table row"),
+        (lambda: paged.append(pool[0], q[:, 0], table, ints, kv_rank=128, rows=ints[:1]), "rows"),
+        (lambda: paged.append(pool[0], q[:, 0], table, ints, kv_rank=128, norm=torch.ones(127, device=d)), "norm"),
+        (lambda: paged.append(pool[0], q[:, 0], table, ints, kv_rank=128, theta=0.0), "theta"),
+        (lambda: paged.append(pool[0], q[:, 0], table, ints, kv_rank=128, theta="x"), "theta"),
+        (lambda: paged.append(pool[0], q[:, 0], table, ints, kv_rank=128, norm=torch.ones(128, device=d), eps=-1.0), "eps"),
+        (lambda: paged.append(pool[0], q[:, 0], table, ints, kv_rank=129), "even")]
+
+
+def beam_refusals(torch, paged, d):
+    pool = paged.alloc_pages(2, 4, 16, 128, 16, device=d)
+    table, ints = torch.zeros(2, 3, dtype=torch.int32, device=d), torch.zeros(2, dtype=torch.int32, device=d)
+    x, s = torch.zeros(2, 4, 10, device=d), torch.zeros(2, 4, device=d)
+    return [
+        (lambda: paged.beam_select(x[0], s), "logits"), (lambda: paged.beam_select(x, s[:, :3]), "scores"),
+        (lambda: paged.beam_select(x, s.double()), "scores"), (lambda: paged.beam_select(x, s, beams=0), "beams"),
+        (lambda: paged.beam_select(x, s, beams=33), "32 beams"), (lambda: paged.beam_select(x, s, finished=s > 0), "eos"),
+        (lambda: paged.beam_select(x, s, finished=s, eos=1), "finished"), (lambda: paged.beam_select(x, s, finished=s > 0, eos=10), "eos"),
+        (lambda: paged.beam_reorder(pool[0], table, ints, ints, ints), "layers"),
+        (lambda: paged.beam_reorder(pool, table, ints[:1], ints, ints), "spare"),
+        (lambda: paged.beam_reorder(pool, table, ints, ints, ints.long()), "parents"),
+        (lambda: paged.beam_reorder(pool.float(), table, ints, ints, ints), "16-bit"),
+        (lambda: paged.beam_reorder((pool, pool), table, ints, ints, ints), "cache is"),
+        (lambda: paged.beam_reorder(pool, table[:, :0], ints, ints, ints), "no pages")]
+
+
+@pytest.mark.parametrize("calls", [attention_refusals, beam_refusals])
+def test_calls_refuse_what_they_can_see(calls):
+    torch, paged = mods()
+    from cpp_inference_train_engine_b200 import EngineError
+    for call, what in calls(torch, paged, "cuda"):
+        with pytest.raises(EngineError, match=what):
+            call()
+    torch.cuda.synchronize()
