@@ -66,23 +66,27 @@ template <int KV, int R, bool Q8> struct MmaCfg {
     static constexpr int kLatent = kBoxes * kTile * 128;
     static constexpr int kRope = kTile * R * 2;
     static constexpr int kScale = Q8 ? 256 : 0;             // two boxes of 16 at 128-byte addresses
-    static constexpr int kSlot = (kLatent + kRope + kScale + 1023) / 1024 * 1024;
+    static constexpr int kSlot = (kLatent + kRope + 1023) / 1024 * 1024;
     static constexpr int kBytes = kLatent + kRope + (Q8 ? kTile * 4 : 0);  // that TMA brings
     static constexpr int SG = KV == 512 ? (Q8 ? 5 : 3) : (Q8 ? 3 : 2);     // slots of a group
     static constexpr int SLOTS = KG * SG;
+    // Tiles that warps who share them weigh at a time. 8-bit ones, of which an SM has to do more in the same time, two:
+    // the exchange costs as much (120 rows of up to 6,001 positions 79.0 -> 75.7 us); the others' ring has no room for it.
+    static constexpr int TW = CW > 1 && Q8 ? 2 : 1;
     // 512: the four shares of S; 128: the four results of a row
     static constexpr int kShareRow = 136;  // (128 columns and 8 more, which spread eight rows over all banks)
-    static constexpr int kShare = KV == 512 ? 4 * 16 * kTile * 4 : 4 * 16 * kShareRow * 4;
+    static constexpr int kShare = KV == 512 ? TW * 4 * 16 * kTile * 4 : 4 * 16 * kShareRow * 4;
     static constexpr int oShare = SLOTS * kSlot;
-    static constexpr int oStat = oShare + kShare;           // [4][16] maxima and sums (128 wide)
+    static constexpr int oScale = oShare + kShare;          // of the slots' positions
+    static constexpr int oStat = oScale + SLOTS * kScale;   // [4][16] maxima and sums (128 wide)
     static constexpr int oTops = oStat;                     // [4][16] maxima, sums (512 wide)
-    static constexpr int oHand = oStat + 4 * 16 * 8;        // [4][32] weights, 8 positions from each warp (512 wide)
-    static constexpr int oRuns = oHand + (KV == 512 ? 1024 : 0);
+    static constexpr int oHand = oStat + 4 * 16 * 8;        // [TW][4][32] weights, 8 positions from each warp (512 wide)
+    static constexpr int oRuns = oHand + (KV == 512 ? TW * 1024 : 0);
     static constexpr int oPlan = oRuns + kQueue * 32;
     static constexpr int oBar = oPlan + 48;
     static constexpr int oMeta = oBar + (2 * SLOTS + 2 * kQueue) * 8;
     static constexpr int kSmem = oMeta + SLOTS * 4 + 1024;  // + alignment of the base
-    static_assert(oBar % 8 == 0 && oRuns % 16 == 0 && oStat % 8 == 0 && oShare % 1024 == 0 && kSlot % 1024 == 0, "alignment");
+    static_assert(oBar % 8 == 0 && oRuns % 16 == 0 && oStat % 8 == 0 && oShare % 1024 == 0 && oScale % 128 == 0 && kSlot % 1024 == 0, "alignment");
     static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
@@ -343,7 +347,8 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
         const int page = p.pool.positions;
         const uint32_t offset = which < C::kBoxes    ? which * kTile * 128 + stretch * a.box * 128
                                 : which == C::kBoxes ? C::kLatent + stretch * a.box * R * 2
-                                                     : C::kLatent + C::kRope + stretch * 128;
+                                                     : C::oScale + stretch * 128;
+        const int each = which <= C::kBoxes ? C::kSlot : C::kScale;  // from one slot's to the next one's
         const CUtensorMap* map = which < C::kBoxes ? &map_latent : which == C::kBoxes ? &map_rope : &map_scale;
         const int column = which < C::kBoxes ? which * (Q8 ? 128 : 64) : Q8 ? 0 : KV;
         int slot = 0, q = 0;
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 __syncwarp();
                 if (mine) {
                     if (loads) {
-                        uint8_t* dst = smem + s * C::kSlot + offset;
+                        uint8_t* dst = smem + s * each + offset;
                         if (Q8 && which > C::kBoxes) tma_load_2d(dst, map, &full[s], y, z);
                         else tma_load_box(dst, map, &full[s], column, y, z);
                     }
@@ -437,7 +442,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
         const float cs = p.scale * 1.4426950408889634f;
         // scales of the lane's positions 8 n + 2 t4 and the next (a second box of 16 starts 128 bytes on)
         auto scales_of = [&](int sl, int n) {
-            const uint8_t* at = smem + (group * C::SG + sl) * C::kSlot + C::kLatent + C::kRope;
+            const uint8_t* at = smem + C::oScale + (group * C::SG + sl) * C::kScale;
             return *reinterpret_cast<const float2*>(at + (n * 8 + t4 * 2) * 4 + (n >= 2 && a.box == 16 ? 64 : 0));
         };
         int slot = 0, turn = 0;
@@ -733,68 +738,88 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 // only where a score passes it by 2^8 (or there was none): the warps vote on it with the barrier that
                 // hands the weights over. The next tile's shares are made before this tile's O product, which hides
                 // their exchange.
+                constexpr int TW = C::TW;
                 float4* mine = reinterpret_cast<float4*>(share) + cw * 128 + lane;
                 uint2* hand = reinterpret_cast<uint2*>(smem + C::oHand) + lane;
                 float* tops = reinterpret_cast<float*>(smem + C::oTops);
                 float ref[2] = {-kLift, -kLift};  // what scores are taken from: m, or 0 where there is none, below the lift
-                auto put = [&](int sl) {  // (the last tile's shares were read before its weights were handed over)
+                // waits for the next tile and makes its shares as tile x of a round (the last round's were read before
+                // its weights were handed over)
+                auto take = [&](int x) {
+                    const int sl = slot;
+                    wait(&full[sl], phase);
+                    if (++slot == C::SG) {
+                        slot = 0;
+                        phase ^= 1;
+                    }
                     scores(sl, s);
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) mine[n * 32] = make_float4(s[n][0], s[n][1], s[n][2], s[n][3]);
+                    for (int n = 0; n < 4; ++n) mine[x * 512 + n * 32] = make_float4(s[n][0], s[n][1], s[n][2], s[n][3]);
+                    return sl;
                 };
-                if (run.from < run.to) {
-                    wait(&full[slot], phase);
-                    put(slot);
-                }
-                for (int i = run.from; i < run.to; ++i) {
+                int at[TW] = {};  // the round's slots
+#pragma unroll
+                for (int x = 0; x < TW; ++x)
+                    if (run.from + x < run.to) at[x] = take(x);
+                for (int i = run.from; i < run.to; i += TW) {
                     products_sync();
-                    float z[4];
-                    {
-                        const ulonglong2* v = reinterpret_cast<const ulonglong2*>(share) + cw * 32 + lane;
-                        const ulonglong2 x = v[0], y = v[128], f = v[256], u = v[384];
-                        const Two by(cs, cs), lo = ((Two(x.x) + Two(y.x)) + (Two(f.x) + Two(u.x))) * by,
-                                  hi = ((Two(x.y) + Two(y.y)) + (Two(f.y) + Two(u.y))) * by;
-                        z[0] = lo.lo();
-                        z[1] = lo.hi();
-                        z[2] = hi.lo();
-                        z[3] = hi.hi();
-                    }
-                    const uint32_t seen = seen_of(slot);
-                    float2 ks = make_float2(1.f, 1.f), e2 = make_float2(0.f, 0.f);
-                    if constexpr (Q8) {
-                        ks = scales_of(slot, cw);
-                        e2 = make_float2(exponent_of(ks.x), exponent_of(ks.y));
-                    }
-                    if (seen != ~0u) {
-                        if (!((seen >> (cw * 8 + t4 * 2)) & 1)) {
-                            z[0] = z[2] = -INFINITY;
-                            ks.x = 0.f;  // (0 times what an unseen position has for a scale may be a NaN)
+                    float z[TW][4], top[2] = {-INFINITY, -INFINITY};
+                    float2 ks[TW];
+#pragma unroll
+                    for (int x = 0; x < TW; ++x) {
+                        ks[x] = make_float2(0.f, 0.f);
+                        z[x][0] = z[x][1] = z[x][2] = z[x][3] = -INFINITY;
+                        if (x > 0 && i + x >= run.to) continue;
+                        const ulonglong2* v = reinterpret_cast<const ulonglong2*>(share) + x * 512 + cw * 32 + lane;
+                        const ulonglong2 u0 = v[0], u1 = v[128], u2 = v[256], u3 = v[384];
+                        const Two by(cs, cs), lo = ((Two(u0.x) + Two(u1.x)) + (Two(u2.x) + Two(u3.x))) * by,
+                                  hi = ((Two(u0.y) + Two(u1.y)) + (Two(u2.y) + Two(u3.y))) * by;
+                        z[x][0] = lo.lo();
+                        z[x][1] = lo.hi();
+                        z[x][2] = hi.lo();
+                        z[x][3] = hi.hi();
+                        const uint32_t seen = seen_of(at[x]);
+                        float2 e2 = make_float2(0.f, 0.f);
+                        if constexpr (Q8) {
+                            ks[x] = scales_of(at[x], cw);
+                            e2 = make_float2(exponent_of(ks[x].x), exponent_of(ks[x].y));
                         }
-                        if (!((seen >> (cw * 8 + t4 * 2 + 1)) & 1)) {
-                            z[1] = z[3] = -INFINITY;
-                            ks.y = 0.f;
+                        if (seen != ~0u) {
+                            if (!((seen >> (cw * 8 + t4 * 2)) & 1)) {
+                                z[x][0] = z[x][2] = -INFINITY;
+                                ks[x].x = 0.f;  // (0 times what an unseen position has for a scale may be a NaN)
+                            }
+                            if (!((seen >> (cw * 8 + t4 * 2 + 1)) & 1)) {
+                                z[x][1] = z[x][3] = -INFINITY;
+                                ks[x].y = 0.f;
+                            }
                         }
+                        top[0] = fmaxf(top[0], fmaxf(z[x][0] + e2.x, z[x][1] + e2.y));
+                        top[1] = fmaxf(top[1], fmaxf(z[x][2] + e2.x, z[x][3] + e2.y));
                     }
-                    const float top0 = fmaxf(z[0] + e2.x, z[1] + e2.y), top1 = fmaxf(z[2] + e2.x, z[3] + e2.y);
                     float add[2];
                     auto give = [&] {
-                        float e[4];
+                        add[0] = add[1] = 0.f;
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) e[x] = fast_exp2(z[x] - ref[x >> 1]);
-                        add[0] = e[0] + e[1];
-                        add[1] = e[2] + e[3];
-                        if constexpr (Q8) {
-                            e[0] *= ks.x;
-                            e[1] *= ks.y;
-                            e[2] *= ks.x;
-                            e[3] *= ks.y;
+                        for (int x = 0; x < TW; ++x) {
+                            float e[4];
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) e[y] = fast_exp2(z[x][y] - ref[y >> 1]);
+                            add[0] += e[0] + e[1];
+                            add[1] += e[2] + e[3];
+                            if constexpr (Q8) {
+                                e[0] *= ks[x].x;
+                                e[1] *= ks[x].y;
+                                e[2] *= ks[x].x;
+                                e[3] *= ks[x].y;
+                            }
+                            hand[(x * 4 + cw) * 32] = make_uint2(lat::pack2<TP>(e[0], e[1]), lat::pack2<TP>(e[2], e[3]));
                         }
-                        hand[cw * 32] = make_uint2(lat::pack2<TP>(e[0], e[1]), lat::pack2<TP>(e[2], e[3]));
                     };
                     give();
-                    if (products_any(top0 > m[0] + kGrowth || top1 > m[1] + kGrowth)) {
-                        // the maximum over the tile, and the sums and products so far below it
-                        const float a0 = quad_max(top0), a1 = quad_max(top1);
+                    if (products_any(top[0] > m[0] + kGrowth || top[1] > m[1] + kGrowth)) {
+                        // the maximum over the tiles, and the sums and products so far below it
+                        const float a0 = quad_max(top[0]), a1 = quad_max(top[1]);
                         if (t4 == 0) {
                             tops[cw * 16 + g] = a0;
                             tops[cw * 16 + g + 8] = a1;
@@ -819,22 +844,23 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                     }
                     l[0] += add[0];
                     l[1] += add[1];
+                    // (a slot is given back before the next round's second tile is waited for)
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const uint2 v = hand[n * 32];
-                        w[n >> 1][(n & 1) * 2] = v.x;
-                        w[n >> 1][(n & 1) * 2 + 1] = v.y;
+                    for (int x = 0; x < TW; ++x) {
+                        const int sl = at[x];
+                        auto handed = [&] {
+#pragma unroll
+                            for (int n = 0; n < 4; ++n) {
+                                const uint2 v = hand[(x * 4 + n) * 32];
+                                w[n >> 1][(n & 1) * 2] = v.x;
+                                w[n >> 1][(n & 1) * 2 + 1] = v.y;
+                            }
+                        };
+                        if constexpr (TW == 1) handed();
+                        if (i + TW + x < run.to) at[x] = take(x);
+                        if constexpr (TW > 1) handed();
+                        if (x == 0 || i + x < run.to) values(sl, seen_of(sl), w);
                     }
-                    const int sl = slot;
-                    if (++slot == C::SG) {
-                        slot = 0;
-                        phase ^= 1;
-                    }
-                    if (i + 1 < run.to) {
-                        wait(&full[slot], phase);
-                        put(slot);
-                    }
-                    values(sl, seen, w);
                 }
             }
             // ------------------------------------------------------------ results
