@@ -304,9 +304,10 @@ int mm_paged_append(const mm_paged_cache* cache, const void* values, int64_t val
                 if (append_vector_form<T>(cache->pool, values, values_stride, norm)) {
                     auto run = [&](auto kv, auto rd, auto codes) {
                         constexpr int kKv = decltype(kv)::value, kRd = decltype(rd)::value;
+                        constexpr bool kQ8 = decltype(codes)::value;
                         const unsigned ctas = std::min(blocks(n, 8 * (512 / kKv)),
-                                                       static_cast<unsigned>(sm_count() * mm::paged::kAppendCtas<T>));
-                        launch(s, mm::paged::append_vec_kernel<T, T16, kKv, kRd, decltype(codes)::value>, dim3(ctas), dim3(256), 0,
+                                                       static_cast<unsigned>(sm_count() * mm::paged::AppendRing<T, kQ8>::kCtas));
+                        launch(s, mm::paged::append_vec_kernel<T, T16, kKv, kRd, kQ8>, dim3(ctas), dim3(256), 0,
                                out_view(&cache->pool), table_of(cache), static_cast<const T*>(values),
                                static_cast<long long>(values_stride), rows, positions, static_cast<long long>(n), norm, eps, rot);
                     };

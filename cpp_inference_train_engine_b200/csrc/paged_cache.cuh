@@ -114,65 +114,99 @@ __global__ void __launch_bounds__(256) append_kernel(lat::CacheOut c, Table tabl
 
 // KV = 128 or 512, 16-byte accesses: KV / 16 lanes take a token, 16 latent values and (the first R / 2 of them)
 // one pair of the key each; sums and maxima are shuffle reductions over the lane group. The CTAs that fit walk
-// the tokens, the next ones already on their way. Bound by its 300 instructions a token and by the bytes that so few
-// tokens keep in flight: 131,072 fp16 tokens of 512 + 32 into 8-bit pages 51 us (4.3 TB/s), into 16-bit ones 54 (5.3).
-template <typename T> struct AppendRow {
-    uint4 x[sizeof(T)];
-    T key[2];
-    int position, row;
+// the tokens, the next ones already on their way to shared memory, where a lane finds what it asked for itself (no
+// barrier); where they go each lane looks up for one of the group's next tokens (a lookup a token, by all of its lanes,
+// took 51.8 us for the first of the following, and what was on its way in registers 50.5). 131,072 fp16 tokens of 512 + 32
+// take 41 us into 8-bit pages (5.3 TB/s; bound by instructions, without the rotation it is 1 less), 51 into 16-bit ones
+// (5.6 TB/s of reads and writes mixed).
+//
+// Slots of a warp (the token at hand and those on their way) and CTAs per SM: more are not better where the bytes are the
+// bound. us of that, into 8-bit and 16-bit pages, of 65,536 fp32 tokens and of 300,000 bf16 ones of 128 + 16 into 16 bits: 2 slots
+// and 3 CTAs 44.2, 51.1, 31.2, 32.0; 3 and 4 41.1, 56.2, 32.9 (2 slots), 31.7; 4 and 4 42.3, 56.5, -, 35.1.
+template <typename T, bool Q8> struct AppendRing {
+    static constexpr bool kMore = Q8 && sizeof(T) == 2;
+    static constexpr int kSlots = kMore ? 3 : 2, kCtas = kMore ? 4 : 3;
+    static constexpr int kKey = 512 * static_cast<int>(sizeof(T));  // [chunk][lane] 16 bytes, then [lane] a pair
+    static constexpr int kSlot = kKey + 32 * 2 * static_cast<int>(sizeof(T));
 };
-// CTAs per SM (131,072 fp16 tokens of 512 + 32 into 8-bit pages, two ahead: 51 us; with three CTAs 53, with three
-// tokens ahead 57, and where either spills 80 to 120)
-template <typename T> constexpr int kAppendCtas = sizeof(T) == 4 ? 3 : 4;
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
 template <typename T, typename T16, int KV, int R, bool Q8>
-__global__ void __launch_bounds__(256, kAppendCtas<T>) append_vec_kernel(
+__global__ void __launch_bounds__(256, AppendRing<T, Q8>::kCtas) append_vec_kernel(
     lat::CacheOut c, Table table, const T* __restrict__ values, long long stride, const int* __restrict__ rows,
     const int* __restrict__ positions, long long n, const float* __restrict__ norm, float eps, const __grid_constant__ Rotation rot) {
-    constexpr int L = KV / 16, P = 32 / L;  // lanes per token, tokens side by side in a warp
-    __shared__ float4 norm_s[KV / 4];       // (in registers they would cost the second token ahead)
-    const int lane = threadIdx.x & 31, sub = lane % L;
+    using Ring = AppendRing<T, Q8>;
+    constexpr int L = KV / 16, P = 32 / L;                              // lanes per token, tokens side by side in a warp
+    constexpr int E = 16 / static_cast<int>(sizeof(T)), NC = 16 / E;    // values of a chunk, chunks of a lane: every L-th
+    __shared__ float4 norm_s[KV / 4];
+    __shared__ alignas(16) uint8_t ring_s[8][Ring::kSlots][Ring::kSlot];
+    const int lane = threadIdx.x & 31, sub = lane % L, mine = lane / L;
     const double f = sub < R / 2 ? rot.f[sub] : 0.0;
+    uint8_t* ring = ring_s[threadIdx.x >> 5][0];
+    const uint32_t chunks = smem_u32(ring) + lane * 16, keys = smem_u32(ring) + Ring::kKey + lane * 2 * static_cast<int>(sizeof(T));
     MM_PDL_ENTRY();
     // (quarter q of every lane's 16 in line: no bank is asked twice)
-    if (norm && threadIdx.x < KV / 4) norm_s[threadIdx.x % 4 * L + threadIdx.x / 4] = __ldg(reinterpret_cast<const float4*>(norm) + threadIdx.x);
+    if (norm && threadIdx.x < KV / 4) {
+        const int q = threadIdx.x / L, l = threadIdx.x % L;  // 4 values of chunk q * 4 / E
+        norm_s[threadIdx.x] = __ldg(reinterpret_cast<const float4*>(norm + q * 4 / E * (KV / NC) + l * E + q * 4 % E));
+    }
     __syncthreads();
-    auto fetch = [&](long long i) {
-        AppendRow<T> v;
-        v.position = -1;
-        v.row = 0;
-        if (i < n) {
-            v.position = __ldg(positions + i);
-            v.row = rows ? __ldg(rows + i) : static_cast<int>(i);
-            const T* x = values + i * stride;
-#pragma unroll
-            for (int e = 0; e < static_cast<int>(sizeof(T)); ++e) v.x[e] = __ldcs(reinterpret_cast<const uint4*>(x + sub * 16) + e);
-            if (sub < R / 2) {
-                v.key[0] = __ldcs(x + KV + 2 * sub);
-                v.key[1] = __ldcs(x + KV + 2 * sub + 1);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < static_cast<int>(sizeof(T)); ++e) v.x[e] = make_uint4(0, 0, 0, 0);
-        }
-        return v;
-    };
     const long long step = static_cast<long long>(gridDim.x) * 8 * P;
-    long long i0 = (static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * P;
-    const int mine = lane / L;
-    constexpr int kAhead = sizeof(T) == 4 ? 1 : 2;  // tokens of a lane group on their way
-    AppendRow<T> next[kAhead];
+    const long long first = (static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * P;
+    long long i = first + mine;  // this lane group's token
+    const T* x = values + i * stride + sub * E;
+    auto ask = [&](long long j, const T* from, int slot) {
+        if (j < n) {
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) next[k] = fetch(i0 + mine + k * step);
-    for (; i0 < n; i0 += step) {  // whole warps walk together (the reductions' shuffles)
-        const AppendRow<T> r = next[0];
+            for (int q = 0; q < NC; ++q) copy_async<16>(chunks + slot + q * 512, from + q * (KV / NC));
+            if (sub < R / 2) copy_async<2 * sizeof(T)>(keys + slot, from + (KV - (E - 2) * sub));
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const long long stride_step = step * stride;
+    // Where the group's next L tokens go, a token a lane.
+    long long latent_at = 0, rope_at = 0, scale_at = 0;
+    int position = -1;
+    auto look_up = [&](long long j) {
         int at = 0;
-        const long long p = page_of(table, c.rows, c.positions, r.row, r.position, at);
+        position = j < n ? __ldg(positions + j) : -1;
+        const int p = page_of(table, c.rows, c.positions, rows && j < n ? __ldg(rows + j) : static_cast<int>(j), position, at);
+        if (p < 0) position = -1;
+        latent_at = p * c.row_stride + at * c.pos_stride;
+        if (Q8) {
+            rope_at = p * c.rope_row_stride + at * c.rope_pos_stride;
+            scale_at = p * c.scale_row_stride + at;
+        }
+    };
+    look_up(i + sub * step);
 #pragma unroll
-        for (int k = 0; k + 1 < kAhead; ++k) next[k] = next[k + 1];
-        next[kAhead - 1] = fetch(i0 + mine + kAhead * step);
+    for (int k = 0; k + 1 < Ring::kSlots; ++k, x += stride_step) ask(i + k * step, x, k * Ring::kSlot);
+    int slot = 0, turn = 0;
+    for (long long i0 = first; i0 < n; i0 += step, i += step, x += stride_step) {  // whole warps walk together (their shuffles)
+        ask(i + (Ring::kSlots - 1) * step, x, slot == 0 ? (Ring::kSlots - 1) * Ring::kSlot : slot - Ring::kSlot);
+        if (turn == 0 && i0 != first) look_up(i + sub * step);
+        const int now = __shfl_sync(0xffffffffu, position, turn, L);
+        const long long to = __shfl_sync(0xffffffffu, latent_at, turn, L);
+        long long rope_to = 0, scale_to = 0;
+        if (Q8) {
+            rope_to = __shfl_sync(0xffffffffu, rope_at, turn, L);
+            scale_to = __shfl_sync(0xffffffffu, scale_at, turn, L);
+        }
+        turn = (turn + 1) % L;
+        asm volatile("cp.async.wait_group %0;" ::"n"(Ring::kSlots - 1) : "memory");
         float v[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = lat::to_f32(reinterpret_cast<const T*>(r.x)[e]);
+        for (int q = 0; q < NC; ++q) {
+            const uint4 x = *reinterpret_cast<const uint4*>(ring + slot + q * 512 + lane * 16);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[q * E + e] = lat::to_f32(reinterpret_cast<const T*>(&x)[e]);
+        }
+        T pair[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) pair[e] = reinterpret_cast<const T*>(ring + slot + Ring::kKey)[2 * lane + e];
+        slot = slot == (Ring::kSlots - 1) * Ring::kSlot ? 0 : slot + Ring::kSlot;
         float inv = 1.f;  // what the values below are still to be multiplied by
         if (norm) {
             Two sums[2] = {Two(0.f, 0.f), Two(0.f, 0.f)};
@@ -197,11 +231,15 @@ __global__ void __launch_bounds__(256, kAppendCtas<T>) append_vec_kernel(
         if constexpr (Q8) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) s = fmaxf(s, fabsf(v[e]));
+            if constexpr (L == 32) {  // (of values that are not negative their bits have the same order)
+                s = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s)));
+            } else {
 #pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
+                for (int o = L / 2; o > 0; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
+            }
             s = fmaxf(__fdiv_rn(s * inv, lat::kE4m3Max), lat::kScaleFloor);
         }
-        if (p < 0) continue;
+        if (now < 0) continue;
         T16* key;
         if constexpr (Q8) {
             // by the reciprocal: within 2 ulp of the quotient, as the normalised values are of theirs
@@ -213,25 +251,39 @@ __global__ void __launch_bounds__(256, kAppendCtas<T>) append_vec_kernel(
                 q[e] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x.lo(), x.hi()), __NV_SATFINITE, __NV_E4M3)) |
                        (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(y.lo(), y.hi()), __NV_SATFINITE, __NV_E4M3)) << 16);
             }
-            *reinterpret_cast<uint4*>(c.latent + p * c.row_stride + at * c.pos_stride + sub * 16) = make_uint4(q[0], q[1], q[2], q[3]);
-            if (sub == 0) c.scale[p * c.scale_row_stride + at] = s;
-            key = reinterpret_cast<T16*>(c.rope) + p * c.rope_row_stride + at * c.rope_pos_stride;
+            uint8_t* dst = c.latent + to + sub * E;
+#pragma unroll
+            for (int x = 0; x < NC; ++x) {
+                if constexpr (E == 8) *reinterpret_cast<uint2*>(dst + x * (KV / NC)) = make_uint2(q[2 * x], q[2 * x + 1]);
+                else *reinterpret_cast<uint32_t*>(dst + x * (KV / NC)) = q[x];
+            }
+            if (sub == 0) c.scale[scale_to] = s;
+            key = reinterpret_cast<T16*>(c.rope) + rope_to;
         } else {
-            T16* dst = reinterpret_cast<T16*>(c.latent) + p * c.row_stride + at * c.pos_stride;
+            T16* dst = reinterpret_cast<T16*>(c.latent) + to;
             if (norm) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) v[e] *= inv;
             }
-            lat::store16(dst + sub * 16, v);
+#pragma unroll
+            for (int x = 0; x < NC; ++x) {
+                uint32_t w[E / 2];
+#pragma unroll
+                for (int e = 0; e < E; e += 2) w[e / 2] = lat::pack2<T16>(v[x * E + e], v[x * E + e + 1]);
+                T16* to = dst + x * (KV / NC) + sub * E;
+                if constexpr (E == 8) *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                else *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+            }
             key = dst + KV;
         }
         if (sub < R / 2) {
             float sn, cs;
-            rotation(f, r.position, sn, cs);
-            const float a = lat::to_f32(r.key[0]), b = lat::to_f32(r.key[1]);
+            rotation(f, now, sn, cs);
+            const float a = lat::to_f32(pair[0]), b = lat::to_f32(pair[1]);
             *reinterpret_cast<uint32_t*>(key + 2 * sub) = lat::pack2<T16>(a * cs - b * sn, a * sn + b * cs);
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // ------------------------------------------------------------------ reorder

@@ -408,6 +408,32 @@ def test_append_of_a_step(width, bits):
     assert torch.isnan(stored).all()
 
 
+@pytest.mark.parametrize("width", [(128, 16), (512, 32)], ids=str)
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_append_of_many_tokens(width, dtype, bits):
+    """More tokens than the blocks of one launch look up at a time: the same bits as in small calls."""
+    torch, paged = mods()
+    kv, rope = width
+    n, page, columns, group = 160001, 64, 4, 9973
+    g = torch.Generator(device="cuda").manual_seed(kv + bits)
+    count = -(-n // (page * columns))
+    values = torch.randn(n, kv + rope, generator=g, device="cuda").to(getattr(torch, dtype))
+    place = torch.randperm(count * page * columns, generator=g, device="cuda")[:n].int()
+    rows, positions = place // (page * columns), place % (page * columns)
+    positions[::1013] = -1
+    table = torch.randperm(count * columns, generator=g, device="cuda").int().view(count, columns)
+    table[3, 2], table[5, 0] = -1, count * columns
+    norm = torch.rand(kv, generator=g, device="cuda") + 0.5
+    a, b = (paged.layer(paged.alloc_pages(1, count * columns, page, kv, rope, torch.float16, bits=bits), 0) for _ in range(2))
+    paged.append(a, values, table, positions, kv_rank=kv, rows=rows, norm=norm)
+    for i in range(0, n, group):
+        at = slice(i, i + group)
+        paged.append(b, values[at], table, positions[at], kv_rank=kv, rows=rows[at], norm=norm)
+    for x, y in zip(*((t if bits == 8 else [t]) for t in (a, b))):
+        assert x.float().any() and torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
 def test_far_positions_keep_their_angle():
     """Angles of positions up to the last 32-bit one: fp32 products would lose them."""
     torch, paged = mods()
