@@ -8,7 +8,7 @@
 // scores crosses threads. Warps:
 //   products   4. Each owns 128 latent columns of the tiles it reads, in both products: its share of Q and
 //              its O [16 x 128] stay in registers, and it alone reads (and clears) those columns. 512 wide: the
-//              four take a tile together and add their shares of S through shared memory; 128 wide: each has
+//              four take a tile (8-bit ones: two) together and add their shares of S through shared memory; 128 wide: each has
 //              tiles of its own (every fourth) and the four results are joined at the row's end.
 //   loads      1, which walks the CTA's runs ahead of them and queues what they need to know of each: a box a
 //              lane, its page number asked for a step ahead.
@@ -19,12 +19,12 @@
 // The tiles of all rows, in line, are divided evenly over the CTAs (a row costs row_cost() tiles more); a row
 // that is cut leaves partial results to the join kernel.
 //
-// Measured on one B200, back to back. Loads alone (no products) of 296 rows of 1,312 positions, 512 + 32 wide, bf16, page
-// by page take 73.8 us (5.7 TB/s); with the products 74.9. Why mma.sync and not tcgen05: with so few rows it needs no
-// tensor memory, no descriptors and no proxy fence between the loads and the products, and its tensor pipe is 33 %
+// Measured on one B200, back to back. 296 rows of 1,312 positions, 512 + 32 wide, bf16, take 72.9 us (5.8 TB/s), as an
+// earlier form of the loads alone did (73.8). Why mma.sync and not tcgen05: with so few rows it needs no
+// tensor memory, no descriptors and no proxy fence between the loads and the products, and its tensor pipe is 36 %
 // busy. The tcgen05 kernel of contiguous caches (shared_prefix_tc.cuh) takes 84.0 us for the same rows, 98.3 against
-// 68.6 with e4m3 caches; 512 rows of 1,024, 128 + 16 wide, 36.1 against 33.6; one row of 131,072 187 against 43. 8-bit
-// rows are bound by the chain of a tile's steps (33 % of the issue slots) and by the unpacking of the codes, once for
+// 63.9 with e4m3 caches; 512 rows of 1,024, 128 + 16 wide, 36.1 against 33.6; one row of 131,072 187 against 42. 8-bit
+// rows are bound by the chain of a tile's steps (40 % of the issue slots) and by the unpacking of the codes, once for
 // each product; products of e4m3 operands (queries in 2 or 3 parts) were slower, 110 us.
 #pragma once
 #include <type_traits>
@@ -990,7 +990,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
     }
 }
 
-// Bound by the latency of two rounds of loads from L2 and by the launch: 5 us of the 81 that 96 wide rows of up to 8,192
+// Bound by the latency of two rounds of loads from L2 and by the launch: 5 us of the 80 that 96 wide rows of up to 8,192
 // positions take.
 //
 // Joins the parts of the units that were cut. Block (entry of the cut list, y) of 8 warps. Up to kFew parts: a warp
