@@ -120,9 +120,10 @@ __global__ void __launch_bounds__(256) append_kernel(lat::CacheOut c, Table tabl
 // take 41 us into 8-bit pages (5.3 TB/s; bound by instructions, without the rotation it is 1 less), 51 into 16-bit ones
 // (5.6 TB/s of reads and writes mixed).
 //
-// Slots of a warp (the token at hand and those on their way) and CTAs per SM: more are not better where the bytes are the
-// bound. us of that, into 8-bit and 16-bit pages, of 65,536 fp32 tokens and of 300,000 bf16 ones of 128 + 16 into 16 bits: 2 slots
-// and 3 CTAs 44.2, 51.1, 31.2, 32.0; 3 and 4 41.1, 56.2, 32.9 (2 slots), 31.7; 4 and 4 42.3, 56.5, -, 35.1.
+// Slots of a warp (the token at hand and those on their way) and CTAs per SM: more are not better where the bytes are
+// the bound. us of the above into 8-bit pages, into 16-bit ones, of 65,536 fp32 tokens into 8-bit ones, and of 300,000
+// bf16 ones of 128 + 16 into 16-bit ones: 2 slots and 3 CTAs 44.2, 51.1, 31.2, 32.0; 3 and 4 41.1, 56.2, 32.9 (with 2
+// slots), 31.7; 4 and 4 42.3, 56.5, -, 35.1.
 template <typename T, bool Q8> struct AppendRing {
     static constexpr bool kMore = Q8 && sizeof(T) == 2;
     static constexpr int kSlots = kMore ? 3 : 2, kCtas = kMore ? 4 : 3;
