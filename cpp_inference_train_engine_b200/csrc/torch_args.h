@@ -7,6 +7,7 @@
 #include <torch/csrc/Dtype.h>
 
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -55,11 +56,20 @@ void call(int rc) {
     throw Refusal{rc, text};
 }
 
-// The calls go past autograd: a result would silently be a constant of its inputs.
+// The calls read the storage: a view that stands for other values than it holds (a negated one, as of a conjugate's
+// imaginary part, or one of zeros without storage) would be taken for what is stored.
+const at::Tensor& as_stored(const at::Tensor& t) {
+    if (t.is_neg() || t.is_conj() || t._is_zerotensor())
+        bad("a tensor whose storage does not hold its values: call resolve_neg() or clone() on it");
+    return t;
+}
+// The calls go past autograd: a result would silently be a constant of its inputs, in backward and in forward mode.
 const at::Tensor& no_gradient(const at::Tensor& t) {
     if (t.requires_grad() && at::GradMode::is_enabled())
         bad("no gradient flows through these operators: detach the tensors that require one, or call under torch.no_grad()");
-    return t;
+    if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        bad("no tangent flows through these operators: unpack the dual tensors");
+    return as_stored(t);
 }
 const at::Tensor& tensor(PyObject* o, const char* what) {
     if (!THPVariable_Check(o)) bad(std::string(what) + " must be a tensor");
@@ -171,7 +181,7 @@ const int64_t* slots(PyObject* o, c10::Device d, int64_t* n) {
 }
 const int32_t* ints(PyObject* o, c10::Device d, int64_t n, const char* what) {
     if (!THPVariable_Check(o)) bad(std::string(what) + " is a contiguous int32 vector of " + std::to_string(n));
-    const at::Tensor& t = THPVariable_Unpack(o);
+    const at::Tensor& t = as_stored(THPVariable_Unpack(o));
     if (t.scalar_type() != at::kInt || t.dim() != 1 || t.size(0) != n || !t.is_contiguous())
         bad(std::string(what) + " is a contiguous int32 vector of " + std::to_string(n));
     on(t, d);
