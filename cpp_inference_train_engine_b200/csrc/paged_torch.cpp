@@ -2,6 +2,8 @@
 // the shared-prompt ones in _latent_torch: argument checks, outputs and workspace from torch's allocator
 // on the tensors' current stream, and the C call. paged.py documents the functions and gives names
 // and defaults; every refusal is an EngineError with the C code.
+#include <algorithm>
+
 #include "torch_args.h"
 
 #include "../../include/mm_paged.h"
@@ -177,7 +179,9 @@ PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             c.pool.pos_stride = x.stride(2);
             c.pool.rows = size32(x.size(1));
             c.pool.positions = size32(x.size(2));
-            c.pool.kv = size32(x.size(3));
+            // (kv_rank is not an argument: the copies take positions whole, so that any cut which the C entry takes will do)
+            c.pool.kv = std::min(size32(x.size(3)), 1024);
+            c.pool.rope_dim = size32(x.size(3)) - c.pool.kv;
             c.pool.kind = c.pool.rope_kind = kind;
             layers = x.size(0);
             strides[0] = x.stride(0);
