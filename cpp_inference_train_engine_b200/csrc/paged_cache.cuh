@@ -336,6 +336,15 @@ __device__ __forceinline__ Move move_of(const Reorder& a, int row) {
     return m;
 }
 
+// Whether another row has the page that `row` has in column j (rows share pages in one column); looks at every `step`-th.
+__device__ __forceinline__ bool shared_at(const Reorder& a, int row, int j, int first, int step) {
+    const int* column = a.table.entry + j;
+    const int page = column[row * a.table.stride];
+    for (int r = first; r < a.table.rows; r += step)
+        if (r != row && column[r * a.table.stride] == page) return true;
+    return false;
+}
+
 // `n` elements of type V per position, `positions` of them; all loads of a step ahead of its stores.
 template <typename V>
 __device__ __forceinline__ void copy_tail(const Plane& p, const uint8_t* src, uint8_t* dst, int positions) {
@@ -369,12 +378,24 @@ static __global__ void __launch_bounds__(256) reorder_kernel(const __grid_consta
     const int row = blockIdx.x, tid = threadIdx.x;
     const Move m = move_of(a, row);
     if (blockIdx.y == 0) {
-        for (int j = tid; j < a.table.columns; j += blockDim.x)
-            a.out_table[static_cast<long long>(row) * a.table.columns + j] =
-                m.swap && j == m.full ? m.to : a.table.entry[(j < m.full ? m.parent : row) * a.table.stride + j];
+        const int length = length_of(a, row), own = length / a.page;  // (a row that fills its table has no page of its own left)
+        // The page that the row begins, or lays aside unwritten: its own, but for a row that took over one shorter by a page
+        // or more, whose entries up to its old length are pages that others may have, the last of them its spare one.
+        const int begun = m.swap ? (length % a.page ? a.table.columns : own) : m.length % a.page ? a.table.columns : m.full;
+        int kept = -1;
+        if (begun < a.table.columns) {
+            const int page = a.table.entry[row * a.table.stride + begun];
+            if (!__syncthreads_or(page == a.spare[row] || shared_at(a, row, begun, tid, blockDim.x))) kept = page;
+        }
+        for (int j = tid; j < a.table.columns; j += blockDim.x) {
+            int page = a.table.entry[(j < m.full ? m.parent : row) * a.table.stride + j];
+            if (j == m.full && m.swap) page = m.to;
+            else if (j == m.full && j == begun) page = kept;
+            else if (j > m.full && m.swap && (page == m.to || (j < own && shared_at(a, row, j, 0, 1)))) page = -1;
+            a.out_table[static_cast<long long>(row) * a.table.columns + j] = page;
+        }
         if (tid == 0) {
-            const int own = length_of(a, row) / a.page;  // (a row that fills its table has no page of its own left)
-            a.out_spare[row] = !m.swap ? a.spare[row] : own < a.table.columns ? a.table.entry[row * a.table.stride + own] : -1;
+            a.out_spare[row] = !m.swap ? a.spare[row] : own >= a.table.columns ? -1 : own == begun ? kept : a.table.entry[row * a.table.stride + own];
             a.out_lengths[row] = m.length;
         }
     }

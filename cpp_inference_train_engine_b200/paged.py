@@ -109,7 +109,10 @@ def beam_reorder(cache, table: torch.Tensor, spare: torch.Tensor, lengths: torch
     cache has its layers ahead (``alloc_pages``); table [rows, columns], spare, lengths and parents [rows]
     int32, parents as row numbers. Full pages are shared through the table. A row whose parent is another one
     gets the positions of its last, partly filled page in its own spare page, in every layer, and its own page at
-    its length becomes its spare (see include/mm_paged.h for rows of different lengths). Every row needs a page of
-    its own for each column that it may grow into and a spare one, none of them another row's; a row that fills its
-    table and then takes over a shorter one is left without a spare page (-1)."""
+    its length becomes its spare. Every row needs a page of its own for each column that it may grow into and a spare
+    one, none of them another row's; a row that fills its table and then takes over a shorter one is left without a
+    spare page (-1). A row that takes over one shorter by a page or more, and grows again, lacks pages: its entries up
+    to its old length are others' too. They become -1, at the latest in the call after which the row begins them: put a
+    page of its own there before it stores (a position without a page is not stored), and store no further than to
+    the end of its last page between two calls (see include/mm_paged.h)."""
     return _ext.beam_reorder(cache, table, spare, lengths, parents)

@@ -94,7 +94,12 @@ int mm_beam_select(const void* logits, int64_t batch_stride, int64_t beam_stride
  * lengths[p] gets table entries [0, n / page) of p (full pages are shared). When p != i, and n % page > 0 or n !=
  * lengths[i], its spare page becomes its entry n / page, with p's n % page positions copied into it in every
  * layer, and its own page at entry lengths[i] / page is its new spare (-1 where its lengths fill the table, which
- * leaves it without). Other entries stay. out_lengths[i] = n. A parent outside [0, rows) is the row itself;
+ * leaves it without). Other entries stay, but for those of a row that takes over one shorter by a page or more
+ * (of pages that it would write, and others read): what stands between n / page and lengths[i] / page becomes -1 where
+ * another row has that page; so does, in the call after which the row begins a page (n % page = 0) or lays one aside
+ * unwritten, an entry that another row has or that is the row's spare page. Such a row needs a page of its own where its
+ * entry is -1 before it stores there, and between two calls it stores no further than to the end of its last page.
+ * (Other tables that hold a page are not looked at.) out_lengths[i] = n. A parent outside [0, rows) is the row itself;
  * lengths are clamped to the table.
  * `cache` describes layer 0 (pages, page entries) and its table; layer l is layer_strides[0..2] * l
  * elements further in latent, rope and scale. out_table [rows][columns] contiguous, out_spare and

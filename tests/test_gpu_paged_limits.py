@@ -36,3 +36,92 @@ def test_reorder_of_every_width_that_is_appended(kv, rope, bits):
     for x, want in zip(cache if bits == 8 else (cache,), held):
         assert want.float().any() or want.numel() == 0
         assert torch.equal(x[:, 4, :2].float(), want.float())
+
+
+def marks(torch, cache, table, held, page):
+    """Of every row the numbers that stand at its positions (0 where it has no page)."""
+    stored, pages = cache[0].float().cpu(), table.cpu()
+    at = lambda r, t: int(pages[r, t // page])  # noqa: E731
+    return [[int(stored[at(r, t), t % page, 0] * 128 + stored[at(r, t), t % page, 1]) if at(r, t) >= 0 else 0 for t in range(len(h))]
+            for r, h in enumerate(held)]
+
+
+def store(torch, paged, cache, table, positions, numbers):
+    values = torch.zeros(len(positions), 8, device="cuda")
+    for r, m in enumerate(numbers):
+        values[r, 0], values[r, 1] = m // 128, m % 128  # (bf16 holds both)
+    paged.append(cache[0], values, table, i32(torch, positions), kv_rank=8)
+
+
+def test_a_row_that_takes_over_a_shorter_one_leaves_the_others_alone():
+    """Rows 0 and 1 share five pages of four positions; row 0 takes over row 2, which is half as long, and grows on: what it
+    has no page for is not stored, and nothing changes under row 1. With pages of its own there it stores again."""
+    torch, paged = mods()
+    page = 4
+    for refill in (False, True):
+        cache = paged.alloc_pages(1, 80, page, 8, 0, torch.bfloat16)
+        table = i32(torch, [[0, 1, 2, 3, 4, 10, 11, 12], [0, 1, 2, 3, 4, 20, 21, 22], [30, 31, 32, 33, 34, 35, 36, 37]])
+        spare, lengths = i32(torch, [50, 51, 52]), i32(torch, [22, 22, 11])
+        held = [list(range(1, 23)), list(range(1, 21)) + [201, 202], list(range(301, 312))]
+        for t in range(22):
+            store(torch, paged, cache, table, [t, t if t > 19 else -1, t if t < 11 else -1], [h[t] if t < len(h) else 0 for h in held])
+        table, spare, lengths = paged.beam_reorder(cache, table, spare, lengths, i32(torch, [2, 1, 2]))
+        held[0] = held[2][:]
+        assert table[0, :5].tolist() == [30, 31, 50, -1, -1] and table[1:].tolist() == [[0, 1, 2, 3, 4, 20, 21, 22], list(range(30, 38))]
+        free = iter((70, 71, 72, 73, 74))
+        for step in range(20):
+            n = len(held[0])
+            if table[0, n // page] < 0 and refill:
+                table[0, n // page] = next(free)
+            there = int(table[0, n // page]) >= 0
+            store(torch, paged, cache, table, [n, -1, -1], [1000 + step, 0, 0])
+            held[0] = held[0] + [1000 + step if there else 0]
+            assert there or not refill
+            lengths = i32(torch, [len(h) for h in held])
+            table, spare, lengths = paged.beam_reorder(cache, table, spare, lengths, i32(torch, [0, 1, 2]))
+            assert marks(torch, cache, table, held, page) == held, step
+
+
+@pytest.mark.parametrize("page", [1, 2, 4, 16])
+@pytest.mark.parametrize("seed", range(4))
+def test_rows_that_grow_at_different_paces_never_write_into_each_others_pages(page, seed):
+    """Rows grow or not, and take over any other row, longer or shorter, for many steps. What a row stored under a page
+    stays for all that descend from it, and the page that a row writes next and its spare one are no other row's. A position
+    is lost only where the table has no page for it, or the row lacks the pages to take over its parent's tail."""
+    import random
+    torch, paged = mods()
+    rng = random.Random(seed)
+    rows, most = 6, 64
+    columns = most // page
+    own = list(range(rows * (columns + 1)))
+    rng.shuffle(own)
+    cache = paged.alloc_pages(1, len(own), page, 8, 0, torch.bfloat16)
+    table, spare = i32(torch, own[:rows * columns]).view(rows, columns), i32(torch, own[rows * columns:])
+    held, mark, kept = [[] for _ in range(rows)], 0, 0
+    for _ in range(100):
+        positions, numbers, pages = [], [], table.cpu()
+        for r in range(rows):
+            grows = len(held[r]) < most and rng.random() < 0.75
+            positions.append(len(held[r]) if grows else -1)
+            mark += 1
+            numbers.append(mark)
+            if grows:
+                held[r] = held[r] + [mark if pages[r, len(held[r]) // page] >= 0 else 0]
+        store(torch, paged, cache, table, positions, numbers)
+        parents = [rng.choice([r, r, r, rng.randrange(rows)]) for r in range(rows)]
+        before, aside = table.cpu(), spare.cpu()
+        table, spare, lengths = paged.beam_reorder(cache, table, spare, i32(torch, [len(h) for h in held]), i32(torch, parents))
+        held = [list(held[p]) for p in parents]
+        for r, p in enumerate(parents):
+            n, full = len(held[r]), len(held[r]) // page
+            if p != r and n % page and (before[p, full] < 0 or aside[r] < 0):
+                held[r][full * page:] = [0] * (n % page)  # (a parent's tail without a page, or no page to copy it into)
+        got = marks(torch, cache, table, held, page)
+        assert all(h in (0, m) for row, want in zip(got, held) for m, h in zip(row, want)) and lengths.tolist() == [len(h) for h in held]
+        kept += sum(m > 0 for h in held for m in h)
+        pages = table.cpu()
+        mine = [int(pages[r, len(h) // page]) for r, h in enumerate(held) if len(h) < most] + spare.tolist()
+        mine = [p for p in mine if p >= 0]
+        used = {int(pages[r, j]) for r, h in enumerate(held) for j in range(len(h) // page)}
+        assert len(set(mine)) == len(mine) and not used & set(mine)
+    assert kept > 1000
