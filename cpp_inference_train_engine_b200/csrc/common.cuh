@@ -146,10 +146,10 @@ __device__ __forceinline__ bool mbar_wait_bounded_cluster(uint64_t* bar, uint32_
     raise_error(err, kErrWaitTimeout);
     return false;
 }
-// Waits for the phase of `parity` to complete, for at most ~2^22 polls with back-off
-// (well over a second). On timeout records kErrWaitTimeout and returns false.
-__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, int* err) {
-    for (uint32_t i = 0; i < (1u << 22); ++i) {
+// Waits for the phase of `parity` to complete, for at most `polls` polls with back-off (a poll that
+// fails takes some 4 us: 2^22 are 17 s). On timeout records kErrWaitTimeout and returns false.
+__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, int* err, uint32_t polls = 1u << 22) {
+    for (uint32_t i = 0; i < polls; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if (i > 64) __nanosleep(i > 4096 ? 256 : 32);
     }

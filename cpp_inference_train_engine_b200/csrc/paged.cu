@@ -163,16 +163,17 @@ MmaPlan mma_plan(const mm::paged::Attention& p) {
 }
 
 template <int KV, int R, typename T, bool Q8, bool HALF = false>
-void run_mma(const mm::paged::Attention& p, const MmaPlan& r, const PoolMaps& maps, void* workspace, cudaStream_t s) {
+void run_mma(const mm::paged::Attention& p, const MmaPlan& r, const PoolMaps& maps, void* workspace, int give_up, cudaStream_t s) {
     using namespace mm::paged;
     using C = MmaCfg<KV, R, Q8>;
-    if (KV == 128 && !HALF && p.H <= 8) return run_mma<KV, R, T, Q8, KV == 128>(p, r, maps, workspace, s);
+    if (KV == 128 && !HALF && p.H <= 8) return run_mma<KV, R, T, Q8, KV == 128>(p, r, maps, workspace, give_up, s);
     MmaArgs a{};
     a.p = p;
     a.box = p.pool.positions % 32 == 0 ? 32 : 16;
     a.blocks = r.blocks;
     a.shares = r.shares;
     a.by_unit = r.units <= r.grid;
+    a.give_up = give_up;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(2) * r.grid * 16 * KV);
     a.cut = reinterpret_cast<int4*>(a.part_ml + int64_t(2) * r.grid * 16);
@@ -192,6 +193,34 @@ void run_mma(const mm::paged::Attention& p, const MmaPlan& r, const PoolMaps& ma
         else if (r.entries > sm_count() * 2 / 5) join(std::integral_constant<int, kMost == 4 ? 2 : 1>{});
         else join(std::integral_constant<int, 1>{});
     }
+}
+
+// give_up: MmaArgs::give_up.
+void attend(const mm_paged_attention_desc* desc, const mm_paged_cache* cache, void* workspace, size_t workspace_bytes, int give_up,
+            cudaStream_t s) {
+    const mm::paged::Attention p = problem(desc, cache);
+    if (p.B == 0) return;
+    const bool q8 = cache->pool.kind == MM_E4M3;
+    PoolMaps maps;
+    const bool mma = mma_form(p, cache->pool);
+    const MmaPlan r = mma ? mma_plan(p) : MmaPlan{};
+    const int64_t need = r.bytes(p.kv);  // also of a pool whose strides the encoder turns out not to take
+    require(need == 0 || (workspace && multiple(workspace, 16) && workspace_bytes >= static_cast<size_t>(need)),
+            "paged attention: workspace too small or not 16-byte aligned");
+    if (mma && pool_maps(maps, cache->pool, cache->pool.positions % 32 == 0 ? 32 : 16)) {
+        with_half(desc->dtype, [&](auto half) {
+            using T = typename decltype(half)::type;
+            if (p.kv == 128) q8 ? run_mma<128, 16, T, true>(p, r, maps, workspace, give_up, s) : run_mma<128, 16, T, false>(p, r, maps, workspace, give_up, s);
+            else q8 ? run_mma<512, 32, T, true>(p, r, maps, workspace, give_up, s) : run_mma<512, 32, T, false>(p, r, maps, workspace, give_up, s);
+        });
+        return;
+    }
+    if (give_up >= 0) refuse(MM_UNSUPPORTED, "paged attention: this form waits for nothing");
+    with_half(desc->dtype, [&](auto half) {
+        using T = typename decltype(half)::type;
+        if (q8) launch_any_width<T, true>(p, s);
+        else launch_any_width<T, false>(p, s);
+    });
 }
 
 void check_select(int batch, int beams, int vocab, int count) {
@@ -339,30 +368,14 @@ int64_t mm_paged_attention_workspace(const mm_paged_attention_desc* desc, const 
 
 int mm_paged_attention(const mm_paged_attention_desc* desc, const mm_paged_cache* cache, void* workspace, size_t workspace_bytes,
                        void* stream) {
+    return guarded([&] { attend(desc, cache, workspace, workspace_bytes, -1, static_cast<cudaStream_t>(stream)); });
+}
+
+int mm_paged_selftest_wait_timeout(const mm_paged_attention_desc* desc, const mm_paged_cache* cache, void* workspace,
+                                   size_t workspace_bytes, int steps, void* stream) {
     return guarded([&] {
-        const mm::paged::Attention p = problem(desc, cache);
-        if (p.B == 0) return;
-        cudaStream_t s = static_cast<cudaStream_t>(stream);
-        const bool q8 = cache->pool.kind == MM_E4M3;
-        PoolMaps maps;
-        const bool mma = mma_form(p, cache->pool);
-        const MmaPlan r = mma ? mma_plan(p) : MmaPlan{};
-        const int64_t need = r.bytes(p.kv);  // also of a pool whose strides the encoder turns out not to take
-        require(need == 0 || (workspace && multiple(workspace, 16) && workspace_bytes >= static_cast<size_t>(need)),
-                "paged attention: workspace too small or not 16-byte aligned");
-        if (mma && pool_maps(maps, cache->pool, cache->pool.positions % 32 == 0 ? 32 : 16)) {
-            with_half(desc->dtype, [&](auto half) {
-                using T = typename decltype(half)::type;
-                if (p.kv == 128) q8 ? run_mma<128, 16, T, true>(p, r, maps, workspace, s) : run_mma<128, 16, T, false>(p, r, maps, workspace, s);
-                else q8 ? run_mma<512, 32, T, true>(p, r, maps, workspace, s) : run_mma<512, 32, T, false>(p, r, maps, workspace, s);
-            });
-            return;
-        }
-        with_half(desc->dtype, [&](auto half) {
-            using T = typename decltype(half)::type;
-            if (q8) launch_any_width<T, true>(p, s);
-            else launch_any_width<T, false>(p, s);
-        });
+        require(steps >= 0, "paged attention: a negative number of steps");
+        attend(desc, cache, workspace, workspace_bytes, steps, static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -40,6 +40,7 @@ struct MmaArgs {
     int blocks;        // blocks of 16 heads per row
     int shares;        // even shares of all tiles (else a CTA takes whole rows in turn)
     int by_unit;       // the cut list is indexed by unit (no more units than CTAs), else by CTA
+    int give_up;       // -1; the self-test: steps of a run after which the loads of every other CTA end as after a wait that ran out
     float* part_o;     // [2 CTAs][16][kv], unnormalised
     float2* part_ml;   // [2 CTAs][16] maximum and sum, base 2
     int4* cut;         // (unit, parts, first CTA): a unit cut at the end of the share it begins in; no parts: none
@@ -57,6 +58,7 @@ constexpr int row_cost(int kv) { return kv == 128 ? 10 : 4; }
 constexpr int min_share(int kv) { return kv == 128 ? 24 : 4; }
 constexpr int kMmaThreads = 160;
 constexpr int kQueue = 4;       // runs queued for the warps of the products
+constexpr uint32_t kPolls = 1u << 18;  // of a wait until it has run out: about a second
 constexpr float kNone = -3.402823466e38f;  // maximum of nothing (finite: its exp2 is 0, never NaN)
 
 template <int KV, int R, bool Q8> struct MmaCfg {
@@ -244,6 +246,38 @@ __device__ __forceinline__ float exponent_of(float s) {
     return static_cast<float>(min(max(static_cast<int>((__float_as_uint(s) >> 23) & 255) - 127, -40), 100));
 }
 
+// The end of a CTA in which a wait ran out. What it asked for lands (the phases of the slots' barriers that are open; one
+// that nothing is in lasts its limit, a quarter of a second) before the shared memory is another CTA's. Its runs, walked once more
+// from the start, get NaN for results, the parts of cut rows too, and the join gets every entry that it reads: nothing is left
+// as the memory was. (As a function that is called it costs the product warps 32 bytes of spills.)
+template <int KV, typename T>
+__device__ __forceinline__ void end_after_timeout(const MmaArgs& a, const int* plan, uint64_t* full, int slots) {
+    const Attention& p = a.p;
+    const int tid = threadIdx.x;
+    const float nan = __int_as_float(0x7fc00000);
+    if (tid < slots) {
+        const uint32_t open = mbar_try_wait(&full[tid], 0) ? 1 : 0;
+        for (int k = 0; k < 1 << 16 && !mbar_try_wait(&full[tid], open); ++k) __nanosleep(256);
+    }
+    Runs runs(a, row_cost(KV), a.shares ? plan[5] : 0, a.shares ? plan[7] : 0, a.shares ? plan[6] : 0);
+    Run run;
+    int cut;
+    while (runs.next(run, cut)) {
+        const int heads = min(16, p.H - run.h0);
+        const long long first = static_cast<long long>(run.row) * p.H + run.h0;
+        if (run.part < 0) {
+            for (int i = tid; i < heads * KV; i += kMmaThreads) static_cast<T*>(p.out)[first * KV + i] = lat::from_f32<T>(nan);
+            if (p.lse && tid < heads) p.lse[first + tid] = nan;
+        } else if (tid < 16) {
+            a.part_ml[run.part * 16 + tid] = make_float2(0.f, nan);  // (whatever its values are: a sum of NaN divides them)
+        }
+        if (tid == 0 && (a.by_unit ? cut >= 0 : cut > 0)) {
+            const int unit = run.row * a.blocks + run.h0 / 16;
+            a.cut[a.by_unit ? unit : blockIdx.x] = make_int4(unit, cut, blockIdx.x, 0);
+        }
+    }
+}
+
 // HALF: at most 8 heads, whose rows are the first 8 of the products': nothing is done for the others.
 template <int KV, int R, typename T, bool Q8, bool HALF>
 __global__ void __launch_bounds__(kMmaThreads, 2)
@@ -329,10 +363,15 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
     bool ok = true;
     // a wait that ran out is recorded once; later waits of this thread are skipped
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok && !mbar_wait_bounded(bar, parity, &paged_status)) {
+        if (ok && !mbar_wait_bounded(bar, parity, &paged_status, kPolls)) {
             ok = false;
             *bad = 1;
         }
+    };
+    auto give_up = [&] {
+        raise_error(&paged_status, kErrWaitTimeout);
+        ok = false;
+        *bad = 1;
     };
 
     if (warp == 4) {
@@ -374,6 +413,8 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 for (int e = lane; e < n; e += 32) prefetch_l1(heads + e / kLines * p.q_head + min(e % kLines * 64, KV + R - 1));
             }
             wait(&run_empty[q], q_phase ^ 1);
+            // (all lanes or none: the votes below are of whole warps, and a queue entry that is still read is not written)
+            if (__any_sync(0xffffffffu, !ok)) break;
             if (lane == 0) {
                 if (!more) run.row = -1;
                 queue[q] = run;
@@ -396,6 +437,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
                 ask(i + C::KG);
                 const int s = group * C::SG + slot;
                 if (mine) wait(&empty[s], phase ^ 1);
+                if (i - group - run.from == a.give_up * C::KG && blockIdx.x & 1) give_up();
                 if (__any_sync(0xffffffffu, !ok)) {
                     ok = false;
                     break;
@@ -983,11 +1025,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
         }
     }
     __syncthreads();
-    if (*bad && tid < C::SLOTS) {
-        // what was asked for lands (or a limit runs out) before the shared memory is another CTA's
-        const uint32_t open = mbar_try_wait(&full[tid], 0) ? 1 : 0;
-        for (int k = 0; k < 1 << 16 && !mbar_try_wait(&full[tid], open); ++k) __nanosleep(256);
-    }
+    if (*bad) end_after_timeout<KV, T>(a, plan, full, C::SLOTS);
 }
 
 // Bound by the latency of two rounds of loads from L2 and by the launch: 5 us of the 80 that 96 wide rows of up to 8,192

@@ -75,6 +75,13 @@ int64_t mm_paged_attention_workspace(const mm_paged_attention_desc* desc, const 
 int mm_paged_attention(const mm_paged_attention_desc* desc, const mm_paged_cache* cache, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* Self-test of what follows a wait that ran out: mm_paged_attention in which the loads of every other CTA end after `steps`
+ * steps of a run of tiles, so that its other warps wait for what does not come (a second or two). The rows that it has
+ * tiles of are NaN, the others as ever, and mm_paged_status reports MM_GPU_ERROR once. Refused for calls of the slower form, which has no
+ * waits. */
+int mm_paged_selftest_wait_timeout(const mm_paged_attention_desc* desc, const mm_paged_cache* cache, void* workspace,
+                                   size_t workspace_bytes, int steps, void* stream);
+
 /* Beam search's selection. For batch entry b, candidate (k, v) has the score
  *   scores[b][k] + logits[b][k][v] - ln sum_u exp(logits[b][k][u]),
  * a finished beam (finished[b][k] != 0) the one candidate (k, eos) with scores[b][k]. The `count`

@@ -125,3 +125,59 @@ def test_rows_that_grow_at_different_paces_never_write_into_each_others_pages(pa
         used = {int(pages[r, j]) for r, h in enumerate(held) for j in range(len(h) // page)}
         assert len(set(mine)) == len(mine) and not used & set(mine)
     assert kept > 1000
+
+
+# rows, heads, latent width, rope width, longest row, 8-bit pages, steps until the loads end: whole rows a CTA, several in turn;
+# few rows that many CTAs share; more rows than CTAs; heads of two blocks; a row that no CTA has for itself
+GIVE_UP = [(700, 8, 128, 16, 197, False, 1), (700, 8, 128, 16, 197, False, 0), (5, 16, 512, 32, 4000, False, 2), (400, 16, 512, 32, 700, False, 4),
+           (90, 19, 128, 16, 2500, True, 2), (300, 16, 512, 32, 900, True, 9), (1, 16, 512, 32, 30000, True, 0)]
+
+
+@pytest.mark.parametrize("case", GIVE_UP, ids=str)
+def test_a_wait_that_runs_out_makes_its_rows_nan_and_is_reported(case):
+    """The loads of every other CTA end early, so that the waits for them run out. A row that one of these CTAs has a part of
+    is NaN, every other one is as ever, and none is what the memory held before; the host is told once, and the next
+    call is as ever. (The workspace holds zeros: a cut that the join were not told of would leave the outputs' mark.)"""
+    import ctypes
+    torch, paged = mods()
+    import cpp_inference_train_engine_b200 as E
+    from cpp_inference_train_engine_b200 import EngineError
+    from tests.test_latent_cpu import E4M3, F16
+    from tests.test_paged_cpu import cache as describe, desc, entries
+    rows, heads, kv, rope, longest, fp8, steps = case
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    page, columns = 32, -(-longest // 32)
+    pools = paged.layer(paged.alloc_pages(1, 600, page, kv, rope, torch.float16, 8 if fp8 else 16), 0)
+    for t in pools if fp8 else (pools,):
+        t.copy_(torch.randn(t.shape, generator=g, device="cuda").abs() + 0.5 if t.dim() == 2 else torch.randn(t.shape, generator=g, device="cuda"))
+    table = torch.randint(0, 600, (rows, columns), generator=g, device="cuda", dtype=torch.int32)
+    lengths = torch.randint(1, longest + 1, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    lengths[-1] = longest
+    if rows > 2:
+        lengths[1] = 0
+    q = torch.randn(rows, heads, kv + rope, generator=g, device="cuda").half()
+    want, want_lse = paged.attention(q, pools, table, lengths, 0.05, kv_rank=kv, return_lse=True)
+    out, lse = torch.full_like(want, 777.0), torch.full_like(want_lse, 777.0)
+    latent, rk, scale = (t.data_ptr() for t in pools) if fp8 else (pools.data_ptr(), 0, 0)
+    c = describe(kind=E4M3 if fp8 else F16, pages=600, page=page, kv=kv, rope=rope, table=table.data_ptr(), rows=rows, columns=columns,
+                 latent=latent, rk=rk, scale=scale)
+    d = desc(q=q.data_ptr(), q_row=heads * (kv + rope), q_head=kv + rope, lengths=lengths.data_ptr(), rows=rows, heads=heads,
+             max_length=columns * page, scale=0.05, out=out.data_ptr(), lse=lse.data_ptr())
+    L = entries()
+    f = L.mm_paged_selftest_wait_timeout
+    f.restype, f.argtypes = ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_void_p]
+    n = L.mm_paged_attention_workspace(d, c)
+    work = torch.zeros(max(n, 16), dtype=torch.uint8, device="cuda")
+    paged.check_status()
+    assert f(d, c, work.data_ptr(), n, steps, torch.cuda.current_stream().cuda_stream) == 0
+    with pytest.raises(EngineError, match="gave up"):
+        paged.check_status()
+    paged.check_status()
+    lost = torch.isnan(lse)
+    assert torch.equal(torch.isnan(out), lost[..., None].expand_as(out))
+    assert torch.equal(torch.where(lost[..., None], 0, out), torch.where(lost[..., None], 0, want))
+    assert torch.equal(torch.where(lost, 0, lse), torch.where(lost, 0, want_lse))
+    assert lost.any() and (rows < 100 or not lost.all())
+    again = paged.attention(q, pools, table, lengths, 0.05, kv_rank=kv, return_lse=True)
+    assert torch.equal(again[0], want) and torch.equal(again[1], want_lse)
+    assert f(d, c, work.data_ptr(), n, -1, None) == 1 and E.lib() is not None

@@ -52,3 +52,16 @@ def test_views_that_stand_for_other_values_are_refused(name):
         calls(*views, pool)[name]()
     with pytest.raises(EngineError, match="CUDA tensor"):
         calls(*(t.resolve_neg() for t in views), pool)[name]()
+
+
+def test_the_self_test_of_waits_refuses_what_has_none():
+    """The slower form of attention waits for nothing; a negative number of steps is no number of steps."""
+    import ctypes
+
+    from tests.test_paged_cpu import P, cache, desc, entries, message
+    f = entries().mm_paged_selftest_wait_timeout
+    f.restype, f.argtypes = ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_void_p]
+    narrow = (desc(heads=2, q_row=24, q_head=12), cache(kv=8, rope=4))
+    assert f(*narrow, P, 1 << 40, 0, None) == 3 and "waits for nothing" in message()
+    assert f(*narrow, P, 1 << 40, -1, None) == 1 and "steps" in message()
+    assert f(desc(rows=-1), cache(), P, 1 << 40, 0, None) == 1 and "sizes" in message()
