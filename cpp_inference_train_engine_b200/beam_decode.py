@@ -78,6 +78,13 @@ class BeamDecoder:
         for g, p in enumerate(prompts):
             padded[g, self.max_prompt - len(p):] = i32(p)  # aligned at the end: the positions before the first are negative
         self.prompt_logits = self._prefill(padded, held)
+        self._check_status()
+
+    def _check_status(self):
+        """Waits, and raises EngineError where a kernel gave up on a wait: of the prompts' attention (latent) or of the
+        beams' (paged)."""
+        latent.check_status(self.device)
+        paged.check_status(self.device)
 
     def _layer(self, l, x, w, positions, table, rows, attend):
         """One block over hidden rows x [n, T, d] whose tokens stand at `positions` [n, T] (negative: none)."""
@@ -164,6 +171,7 @@ class BeamDecoder:
             failed = torch.isneginf(scores[:, 0]).any()
             stop, none = torch.stack([finished.all(), failed]).tolist()
             if none:
+                self._check_status()  # results of a kernel that gave up are NaN too
                 raise EngineError(6, "a request has no continuation with a probability (its logits hold a NaN)")
             if stop or step == N:
                 break
@@ -180,7 +188,7 @@ class BeamDecoder:
             count = follow(count) + ~was
             finished = was | (tokens == c.eos_id) | (tokens < 0)
             table, spare, lengths = paged.beam_reorder(self.cache, table, spare, lengths, (chosen + self.base).view(-1))
-        paged.check_status(self.device)
+        self._check_status()
         ranked = (scores / count.float().pow(length_penalty)).nan_to_num(nan=-math.inf, neginf=-math.inf)
         order = ranked.sort(dim=1, descending=True, stable=True).indices.cpu()
         history, count, scores = history.cpu(), count.cpu(), scores.cpu()
