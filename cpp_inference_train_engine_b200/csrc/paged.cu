@@ -336,8 +336,11 @@ int mm_paged_append(const mm_paged_cache* cache, const void* values, int64_t val
                         constexpr bool kQ8 = decltype(codes)::value;
                         const unsigned ctas = std::min(blocks(n, 8 * (512 / kKv)),
                                                        static_cast<unsigned>(sm_count() * mm::paged::AppendRing<T, kQ8>::kCtas));
-                        launch(s, mm::paged::append_vec_kernel<T, T16, kKv, kRd, kQ8>, dim3(ctas), dim3(256), 0,
-                               out_view(&cache->pool), table_of(cache), static_cast<const T*>(values),
+                        // (8-bit codes with and without a norm in one instance: 43.7 us instead of 41 for 131,072 fp16 tokens;
+                        // 16-bit values in two instances 52.6 instead of 51.5)
+                        launch(s, kQ8 && !norm ? mm::paged::append_vec_kernel<T, T16, kKv, kRd, kQ8, !kQ8>
+                                               : mm::paged::append_vec_kernel<T, T16, kKv, kRd, kQ8, true>,
+                               dim3(ctas), dim3(256), 0, out_view(&cache->pool), table_of(cache), static_cast<const T*>(values),
                                static_cast<long long>(values_stride), rows, positions, static_cast<long long>(n), norm, eps, rot);
                     };
                     using Narrow = std::integral_constant<int, 128>;

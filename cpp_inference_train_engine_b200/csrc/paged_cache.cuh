@@ -117,8 +117,9 @@ __global__ void __launch_bounds__(256) append_kernel(lat::CacheOut c, Table tabl
 // the tokens, the next ones already on their way to shared memory, where a lane finds what it asked for itself (no
 // barrier); where they go each lane looks up for one of the group's next tokens (a lookup a token, by all of its lanes,
 // took 51.8 us for the first of the following, and what was on its way in registers 50.5). 131,072 fp16 tokens of 512 + 32
-// take 41 us into 8-bit pages (5.3 TB/s; bound by instructions, without the rotation it is 1 less), 51 into 16-bit ones
-// (5.6 TB/s of reads and writes mixed).
+// take 41 us into 8-bit pages (5.3 TB/s; 44 to 46 us where other inputs come in between; bound by instructions, without the
+// rotation it is 1 less), without a norm, whose codes are the quotients', 45; 51 into 16-bit ones (5.6 TB/s of reads and
+// writes mixed).
 //
 // Slots of a warp (the token at hand and those on their way) and CTAs per SM: more are not better where the bytes are
 // the bound. us of the above into 8-bit pages, into 16-bit ones, of 65,536 fp32 tokens into 8-bit ones, and of 300,000
@@ -134,11 +135,12 @@ template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, co
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
-template <typename T, typename T16, int KV, int R, bool Q8>
+template <typename T, typename T16, int KV, int R, bool Q8, bool NORM>
 __global__ void __launch_bounds__(256, AppendRing<T, Q8>::kCtas) append_vec_kernel(
     lat::CacheOut c, Table table, const T* __restrict__ values, long long stride, const int* __restrict__ rows,
     const int* __restrict__ positions, long long n, const float* __restrict__ norm, float eps, const __grid_constant__ Rotation rot) {
     using Ring = AppendRing<T, Q8>;
+    const bool normed = Q8 ? NORM : norm != nullptr;
     constexpr int L = KV / 16, P = 32 / L;                              // lanes per token, tokens side by side in a warp
     constexpr int E = 16 / static_cast<int>(sizeof(T)), NC = 16 / E;    // values of a chunk, chunks of a lane: every L-th
     __shared__ float4 norm_s[KV / 4];
@@ -149,7 +151,7 @@ __global__ void __launch_bounds__(256, AppendRing<T, Q8>::kCtas) append_vec_kern
     const uint32_t chunks = smem_u32(ring) + lane * 16, keys = smem_u32(ring) + Ring::kKey + lane * 2 * static_cast<int>(sizeof(T));
     MM_PDL_ENTRY();
     // (quarter q of every lane's 16 in line: no bank is asked twice)
-    if (norm && threadIdx.x < KV / 4) {
+    if (normed && threadIdx.x < KV / 4) {
         const int q = threadIdx.x / L, l = threadIdx.x % L;  // 4 values of chunk q * 4 / E
         norm_s[threadIdx.x] = __ldg(reinterpret_cast<const float4*>(norm + q * 4 / E * (KV / NC) + l * E + q * 4 % E));
     }
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(256, AppendRing<T, Q8>::kCtas) append_vec_kern
         for (int e = 0; e < 2; ++e) pair[e] = reinterpret_cast<const T*>(ring + slot + Ring::kKey)[2 * lane + e];
         slot = slot == (Ring::kSlots - 1) * Ring::kSlot ? 0 : slot + Ring::kSlot;
         float inv = 1.f;  // what the values below are still to be multiplied by
-        if (norm) {
+        if (normed) {
             Two sums[2] = {Two(0.f, 0.f), Two(0.f, 0.f)};
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
@@ -243,14 +245,38 @@ __global__ void __launch_bounds__(256, AppendRing<T, Q8>::kCtas) append_vec_kern
         if (now < 0) continue;
         T16* key;
         if constexpr (Q8) {
-            // by the reciprocal: within 2 ulp of the quotient, as the normalised values are of theirs
-            const float f8 = inv * __frcp_rn(s);
+            auto codes4 = [](float a, float b, float c, float d) {
+                return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3)) |
+                       (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16);
+            };
+            auto codes = [&](int e, float by) {
+                const Two f(by, by), x = Two(v[4 * e], v[4 * e + 1]) * f, y = Two(v[4 * e + 2], v[4 * e + 3]) * f;
+                return codes4(x.lo(), x.hi(), y.lo(), y.hi());
+            };
+            const float r = __frcp_rn(s);
             uint32_t q[4];
+            if (normed) {
+                // by the reciprocal: within 3 ulp of the quotient, as the normalised values are of theirs (the quotients' own
+                // codes, as below, take 7 us more for the first of the tokens above)
+                const float by = inv * r;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const Two by(f8, f8), x = Two(v[4 * e], v[4 * e + 1]) * by, y = Two(v[4 * e + 2], v[4 * e + 3]) * by;
-                q[e] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x.lo(), x.hi()), __NV_SATFINITE, __NV_E4M3)) |
-                       (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(y.lo(), y.hi()), __NV_SATFINITE, __NV_E4M3)) << 16);
+                for (int e = 0; e < 4; ++e) q[e] = codes(e, by);
+            } else {
+                // The codes of the quotients. The product with the reciprocal is within 2 ulp of the quotient, and rounding is
+                // monotonic: where the products with one 2^-21 lower and higher have the same code, so has the quotient. A
+                // lane in which they differ anywhere (a quotient that close to the middle of two codes) divides.
+                const float below = r * (1.f - 4.76837158e-7f), above = r * (1.f + 4.76837158e-7f);
+                uint32_t differ = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    q[e] = codes(e, below);
+                    differ |= q[e] ^ codes(e, above);
+                }
+                if (differ) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        q[e] = codes4(__fdiv_rn(v[4 * e], s), __fdiv_rn(v[4 * e + 1], s), __fdiv_rn(v[4 * e + 2], s), __fdiv_rn(v[4 * e + 3], s));
+                }
             }
             uint8_t* dst = c.latent + to + sub * E;
 #pragma unroll
@@ -262,7 +288,7 @@ __global__ void __launch_bounds__(256, AppendRing<T, Q8>::kCtas) append_vec_kern
             key = reinterpret_cast<T16*>(c.rope) + rope_to;
         } else {
             T16* dst = reinterpret_cast<T16*>(c.latent) + to;
-            if (norm) {
+            if (normed) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) v[e] *= inv;
             }

@@ -41,7 +41,9 @@ int mm_paged_status(void* stream);
  *   (a, b) -> (a cos t - b sin t, a sin t + b cos t),  t = position * theta^(-2 j / rope_dim)
  * on the adjacent pairs j of the key (angles in fp64, src/model/ops.cpp:88-108), a 16-bit pool gets
  * c and the key rounded once; an MM_E4M3 one scale = max(max |c| / 448, 2^-100), codes e4m3(c / scale)
- * and the key in its rope_kind. Two tokens of one call for one position leave a mix of both. */
+ * and the key in its rope_kind. (Without norm the codes are exactly those; with it c and the quotient are off by some units
+ * in the last place of fp32, by how many depends on the strides, which may show in the code of a quotient that is as near to
+ * the middle of two.) Two tokens of one call for one position leave a mix of both. */
 int mm_paged_append(const mm_paged_cache* cache, const void* values, int64_t values_stride, int dtype,
                     const int32_t* rows, const int32_t* positions, int64_t n, double theta,
                     const float* norm, float eps, void* stream);

@@ -181,3 +181,36 @@ def test_a_wait_that_runs_out_makes_its_rows_nan_and_is_reported(case):
     again = paged.attention(q, pools, table, lengths, 0.05, kv_rank=kv, return_lse=True)
     assert torch.equal(again[0], want) and torch.equal(again[1], want_lse)
     assert f(d, c, work.data_ptr(), n, -1, None) == 1 and E.lib() is not None
+
+
+@pytest.mark.parametrize("kv, rope", [(128, 16), (512, 32), (40, 8)])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_codes_are_those_of_the_quotients(kv, rope, dtype):
+    """Latents that are a scale times the middle of two e4m3 codes: the quotient is that middle and goes to the even code,
+    where a product with the scale's reciprocal may come out on either side of it. The codes are the same in pools that
+    take 16 bytes at a time and in those that do not."""
+    torch, paged = mods()
+    g = torch.Generator(device="cuda").manual_seed(kv)
+    n, bits = 600, {"float32": 18, "float16": 6, "bfloat16": 3}[dtype]  # (of a scale: its products with a middle's 5 bits are exact)
+    scales = (torch.randint(0, 2 ** (bits - 2), (n,), generator=g, device="cuda") * 2 + 2 ** (bits - 1) + 1).float() * 2.0 ** -(bits - 1)
+    middles = (2 * torch.randint(8, 16, (n, kv), generator=g, device="cuda") + 1).float() / 16
+    size = torch.randint(-6, 8, (n, kv), generator=g, device="cuda").float()
+    sign = torch.randint(0, 2, (n, kv), generator=g, device="cuda").float() * 2 - 1
+    lat = middles * 2.0 ** size * sign * scales[:, None]
+    lat[:, 5] = 448 * scales
+    values = torch.cat([lat, torch.randn(n, rope, generator=g, device="cuda")], 1).to(getattr(torch, dtype))
+    assert torch.equal(values[:, :kv].float(), lat)
+    by_quotient = (lat / scales[:, None]).to(torch.float8_e4m3fn).view(torch.uint8)
+    by_product = (lat * (1 / scales)[:, None]).to(torch.float8_e4m3fn).view(torch.uint8)
+    assert dtype != "float32" or (by_quotient != by_product).sum() > 100  # (the inputs tell the two apart)
+    table = torch.arange(n, dtype=torch.int32, device="cuda")[:, None]
+    positions = torch.arange(n, dtype=torch.int32, device="cuda") % 16
+    for aligned in (True, False):
+        pools = paged.layer(paged.alloc_pages(1, n, 16, kv, rope, bits=8), 0)
+        if not aligned:  # rows of an odd stride
+            wide = torch.zeros(n, 16, kv + 1, dtype=torch.uint8, device="cuda")[..., 1:].view(torch.float8_e4m3fn)
+            pools = pools._replace(latent=wide)
+        paged.append(pools, values, table, positions, kv_rank=kv)
+        at = torch.arange(n, device="cuda"), positions.long()
+        assert torch.equal(pools.scale[at], scales)
+        assert torch.equal(pools.latent.view(torch.uint8)[at], by_quotient), aligned
