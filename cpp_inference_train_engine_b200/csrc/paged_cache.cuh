@@ -258,7 +258,12 @@ __global__ void __launch_bounds__(256, AppendRing<T, Q8>::kCtas) append_vec_kern
             if (normed) {
                 // by the reciprocal: within 3 ulp of the quotient, as the normalised values are of theirs (the quotients' own
                 // codes, as below, take 7 us more for the first of the tokens above)
-                const float by = inv * r;
+                float by = inv * r;
+                if (by > 3.402823466e38f) {  // (zero weights over tiny values: not 0 times an infinity)
+                    by = r;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] *= inv;
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) q[e] = codes(e, by);
             } else {

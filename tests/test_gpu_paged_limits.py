@@ -214,3 +214,14 @@ def test_codes_are_those_of_the_quotients(kv, rope, dtype):
         at = torch.arange(n, device="cuda"), positions.long()
         assert torch.equal(pools.scale[at], scales)
         assert torch.equal(pools.latent.view(torch.uint8)[at], by_quotient), aligned
+
+
+def test_normalised_codes_where_the_weights_are_zero():
+    """Tiny latents without eps have a large reciprocal norm: what the weights make zero stays zero."""
+    torch, paged = mods()
+    for kv, rope in ((128, 16), (512, 32), (40, 8)):
+        pools = paged.layer(paged.alloc_pages(1, 2, 16, kv, rope, bits=8), 0)
+        pools.latent.view(torch.uint8).fill_(0x7F)
+        norm = torch.zeros(kv, device="cuda")
+        paged.append(pools, torch.full((1, kv + rope), 1e-12, device="cuda"), i32(torch, [[1]]), i32(torch, [3]), kv_rank=kv, norm=norm, eps=0.0)
+        assert not pools.latent[1, 3].float().any() and float(pools.scale[1, 3]) == 2.0 ** -100
