@@ -107,7 +107,7 @@ PyObject* shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n_ar
             p.suffix_len = ints(a[5], d, B, "suffix_len");
             p.max_suffix = static_cast<int32_t>(integer(a[10], suffix.positions, "max_suffix"));
         }
-        const int want_lse = PyObject_IsTrue(a[11]);
+        const bool want_lse = truth(a[11], "return_lse");
         const c10::cuda::CUDAGuard guard(d);
         at::Tensor out = empty({B, T, H, kv}, q.scalar_type(), d), lse;
         p.out = out.data_ptr();

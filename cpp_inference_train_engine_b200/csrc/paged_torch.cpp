@@ -103,7 +103,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         }
         p.sinks = static_cast<int32_t>(integer(a[7], 0, "sinks"));
         p.scale = static_cast<float>(number(a[4]));
-        const int want_lse = PyObject_IsTrue(a[9]);
+        const bool want_lse = truth(a[9], "return_lse");
         const c10::cuda::CUDAGuard guard(d);
         at::Tensor out = empty({B, H, kv}, q.scalar_type(), d), lse;
         p.out = out.data_ptr();

@@ -112,6 +112,15 @@ int64_t integer(PyObject* o, int64_t absent, const char* what) {
     }
     return v;
 }
+// An object's truth value, where it has one.
+bool truth(PyObject* o, const char* what) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) {
+        PyErr_Clear();
+        bad(std::string(what) + " must be true or false");
+    }
+    return v != 0;
+}
 int32_t size32(int64_t v) {
     if (v > INT32_MAX) bad("a dimension exceeds 32 bits");
     return static_cast<int32_t>(v);

@@ -225,3 +225,15 @@ def test_normalised_codes_where_the_weights_are_zero():
         norm = torch.zeros(kv, device="cuda")
         paged.append(pools, torch.full((1, kv + rope), 1e-12, device="cuda"), i32(torch, [[1]]), i32(torch, [3]), kv_rank=kv, norm=norm, eps=0.0)
         assert not pools.latent[1, 3].float().any() and float(pools.scale[1, 3]) == 2.0 ** -100
+
+
+def test_a_flag_without_a_truth_value_is_refused():
+    torch, paged = mods()
+    from cpp_inference_train_engine_b200 import EngineError, latent
+    pool = torch.zeros(2, 16, 144, dtype=torch.float16, device="cuda")
+    q, table, ints = torch.zeros(2, 8, 144, dtype=torch.float16, device="cuda"), i32(torch, [[0], [1]]), i32(torch, [3, 4])
+    for call in (lambda flag: paged.attention(q, pool, table, ints, 0.1, kv_rank=128, return_lse=flag),
+                 lambda flag: latent.shared_prefix_attention(q[:, None], None, pool, None, None, ints, 0.1, kv_rank=128, return_lse=flag)):
+        with pytest.raises(EngineError, match="return_lse"):
+            call(torch.zeros(2))
+        assert len(call(1)) == 2 and torch.is_tensor(call(0))
