@@ -182,7 +182,7 @@ void run_mma(const mm::paged::Attention& p, const MmaPlan& r, const PoolMaps& ma
     if (r.shares) {
         // the fewer units, the more parts each has and the more warps join one (a block for 128 columns of a head where
         // the parts are many): 512 wide with 4, 2 or 1 times 128 columns a warp, us of the whole call, 250 rows of up to
-        // 3,000 positions 68.7 / 68.9 / 70.9, 96 of 8,192 83.1 / 80.8 / 81.2, 48 of 8,000 57.0 / 57.2 / 53.8
+        // 3,000 positions 67.3 / 68.2 / 70.0, 96 of 8,192 80.4 / 79.1 / 79.7, 48 of 8,000 56.6 / 56.6 / 53.4
         constexpr int kMost = KV / 128;
         auto join = [&](auto ng) {
             constexpr int NG = decltype(ng)::value;
@@ -231,11 +231,11 @@ void check_select(int batch, int beams, int vocab, int count) {
 
 // How a selection is launched: parts of a beam's tokens, a block each, as many as fill the multiprocessors with 32
 // warps, of 4,096 tokens or more. Blocks have eight warps, where there are many beams fewer, whose lists have to be joined:
-// us with 8 / 4 / 2, 400 beams of 50,000 26.7 / 28.2 / 36.3, 512 of 32,768 23.2 / 21.0 / 26.4, 1,800 of 20,000 (fp16) 46.3 /
-// 34.7 / 40.3, 1,000 of 4,000 20.5 / 15.6 / 12.8.
+// us with 8 / 4 / 2, 400 beams of 50,000 26.8 / 26.7 / 35.5, 512 of 32,768 24.0 / 22.2 / 26.7, 1,800 of 20,000 (fp16) 42.7 /
+// 32.8 / 32.7, 1,000 of 4,000 19.2 / 16.3 / 13.9.
 // In clusters where a batch entry's blocks can be one, none has more than 32,768 tokens then and there are few: us in
-// clusters / with a second kernel, 1 x 4 beams of 16,384 8.7 / 11.6, 4 x 16 of 32,768 13.6 / 17.7, 16 x 8 (128 blocks)
-// 17.5 / 17.0, 64 x 8 (512) 25.0 / 23.5.
+// clusters / with a second kernel, 1 x 4 beams of 16,384 8.8 / 13.0, 4 x 16 of 32,768 13.8 / 16.6, 16 x 8 (256 blocks)
+// 15.7 / 15.8, 64 x 8 (512) 22.0 / 22.2.
 struct SelectPlan {
     int parts, warps;
     bool cluster;

@@ -29,8 +29,8 @@ __device__ __forceinline__ int window_start(const Attention& p, int len) { retur
 // One warp per (row, head), positions in tiles of 32: lane j scores position j of the tile, the tile's softmax
 // is one warp reduction with the running maximum and sum, then every lane adds p_j * value for its
 // columns. The query (fp32, scaled) and the output row live in shared memory. For the widths, page
-// sizes and alignments that have no tensor-core form; bound by its scalar loads (4 rows of 8 heads over 197 positions,
-// 128 + 16 wide: 76 us where that takes 7).
+// sizes and alignments that have no tensor-core form; bound by its scalar loads, a position's by one lane, and one
+// warp's chain a row and head (120 + 16 wide, 8 heads: 4 rows of 197 positions 95 us where 128 + 16 take 7, 64 of 1,024 581).
 constexpr int kAnyWarps = 4;
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(32 * kAnyWarps) any_width_kernel(const Attention p) {

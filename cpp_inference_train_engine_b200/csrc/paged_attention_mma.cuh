@@ -47,14 +47,14 @@ struct MmaArgs {
 };
 
 constexpr int kTile = 32;       // positions
-// Tiles that a row's queries and results cost: of 4 to 40, by 512 rows of up to 2,048, 128 wide (2: 42.7 us, 6: 41.0,
-// 10: 39.8, 20: 40.2, 40: 44.2), and 96 of up to 8,192 and 400 of up to 700, 512 wide (2: 86.7 and 47, 4: 84.2 and
-// 46, 6: 83.4 and 46.8, 10: 83.7 and 47.9).
+// Tiles that a row's queries and results cost: by 512 rows of up to 2,048, 128 wide (2: 36.4 us, 6: 35.0, 10: 35.5, 20:
+// 36.7, 40: 40.4), and 96 of up to 8,192 and 400 of up to 700, 512 wide (2: 79.4 and 46.5, 4: 79.2 and 43.8, 6: 79.5 and
+// 44.3, 10: 80.2 and 45.0).
 constexpr int row_cost(int kv) { return kv == 128 ? 10 : 4; }
 // Tiles of a CTA at least, so that few rows make no more partial results than they gain: 512 wide, 8 rows of up to
-// 4,096 take 24.5 us with 12, 19.3 with 6, 17.3 with 4, 16.2 with 2, one of 300 13.5, 12.5 and 13.4 with 6, 4 and 2. 128
-// wide a tile is a quarter of the bytes and each of the four warps has its own: 5 rows of up to 900 take 13.6 us
-// with 8 or 16 and 9.2 with 24.
+// 4,096 take 25.8 us with 12, 19.9 with 6, 18.4 with 4, 18.0 with 2, one of 300 16.3, 13.7, 12.1 to 13.5 and 13.7. 128
+// wide a tile is a quarter of the bytes and each of the four warps has its own: 5 rows of up to 900 take 9.3 us with 8, 11
+// to 13.5 with 16 and 9.3, without a join, with 24.
 constexpr int min_share(int kv) { return kv == 128 ? 24 : 4; }
 constexpr int kMmaThreads = 160;
 constexpr int kQueue = 4;       // runs queued for the warps of the products

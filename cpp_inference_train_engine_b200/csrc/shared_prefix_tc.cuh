@@ -60,7 +60,7 @@ namespace spa {
 __device__ int latent_status;  // DeviceError bits since they were last read (mm_latent_status)
 
 // A CTA that gave up on a wait notes it and stays until the tiles that it asked for have landed (the phases
-// of their barriers that are open; a phase that nothing is in lasts its limit, some 20 ms): its shared memory
+// of their barriers that are open; a phase that nothing is in lasts its limit, a quarter of a second): its shared memory
 // is another CTA's after that. Out of line: the code is never run and costs the tile loops registers.
 __device__ __noinline__ void end_after_timeout(uint64_t* tile_in, int n) {
     raise_error(&latent_status, kErrWaitTimeout);

@@ -53,8 +53,9 @@ int mm_paged_append(const mm_paged_cache* cache, const void* values, int64_t val
  * except those of pages outside the pool (entries of pages that were given back may hold -1):
  *   s = scale * q . K_j,  out = sum_j softmax(s)_j K_j[0, kv),  lse = ln sum_j e^s
  * A query that sees no position gets out = 0, lse = -infinity. What unseen positions hold (NaN
- * included) never reaches a result; a NaN or an infinity in a seen one makes the row's results not
- * finite. Lengths are clamped to [0, max_length], max_length <= table_columns * page: a host-side
+ * included) never reaches a result; a NaN or an infinity in a seen one reaches its row's alone, as the
+ * formula has it (a score of -infinity is a weight of zero). e4m3 scales above 2^100 may make results infinite.
+ * Lengths are clamped to [0, max_length], max_length <= table_columns * page: a host-side
  * bound that sizes the launch.
  * q: MM_F16 / MM_BF16 [rows][heads][kv + rope_dim], last dimension adjacent; 16-bit pools have its
  * type, e4m3 ones its rope_kind. out [rows][heads][kv] of dtype and lse [rows][heads] fp32 (may be
