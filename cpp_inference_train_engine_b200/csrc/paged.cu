@@ -377,7 +377,7 @@ int mm_paged_attention(const mm_paged_attention_desc* desc, const mm_paged_cache
 int mm_paged_selftest_wait_timeout(const mm_paged_attention_desc* desc, const mm_paged_cache* cache, void* workspace,
                                    size_t workspace_bytes, int steps, void* stream) {
     return guarded([&] {
-        require(steps >= 0, "paged attention: a negative number of steps");
+        require(steps >= 0 && steps <= 1 << 24, "paged attention: invalid number of steps");
         attend(desc, cache, workspace, workspace_bytes, steps, static_cast<cudaStream_t>(stream));
     });
 }

@@ -63,5 +63,6 @@ def test_the_self_test_of_waits_refuses_what_has_none():
     f.restype, f.argtypes = ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_void_p]
     narrow = (desc(heads=2, q_row=24, q_head=12), cache(kv=8, rope=4))
     assert f(*narrow, P, 1 << 40, 0, None) == 3 and "waits for nothing" in message()
-    assert f(*narrow, P, 1 << 40, -1, None) == 1 and "steps" in message()
+    for steps in (-1, 2 ** 24 + 1, 2 ** 31 - 1):
+        assert f(*narrow, P, 1 << 40, steps, None) == 1 and "steps" in message()
     assert f(desc(rows=-1), cache(), P, 1 << 40, 0, None) == 1 and "sizes" in message()
